@@ -170,6 +170,11 @@ EXPORTS = [
      [ctypes.POINTER(GDNRunState), ctypes.POINTER(ctypes.c_float), ctypes.c_size_t, ctypes.POINTER(ctypes.c_float),
       ctypes.c_size_t, ctypes.POINTER(ctypes.c_int32), ctypes.POINTER(ctypes.c_int32),
       ctypes.POINTER(ctypes.c_int32)]),
+    # GdnB200DeltaArgs / GdnB200LogitsArgs as packed bytes (ops.py)
+    ("gdn_b200_delta_step", ctypes.c_int, [ctypes.c_char_p]),
+    ("gdn_b200_delta_chunk", ctypes.c_int, [ctypes.c_char_p]),
+    ("gdn_b200_delta_chunk_workspace", ctypes.c_size_t, [ctypes.c_char_p]),
+    ("gdn_b200_constrain_logits", ctypes.c_int, [ctypes.c_char_p]),
 ]
 
 GDN_B200_TP_TOKEN_BYTES = 128

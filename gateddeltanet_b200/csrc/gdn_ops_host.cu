@@ -1,0 +1,162 @@
+/* gdn_ops_host.cu -- C entries of the serving operators (include/gdn_b200.h):
+ * the checks of their arguments and the launches. Device pointers on the
+ * caller's stream; nothing is allocated or synchronised. */
+#include "gdn_b200.h"
+#include "gdn_ops.h"
+
+#include <stdarg.h>
+#include <stdio.h>
+
+namespace gdn {
+int host_fail(const char *msg); /* gdn_host.cu: records the message, returns -1 */
+}
+
+namespace {
+
+int failf(const char *fmt, ...) {
+    char buf[256];
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(buf, sizeof(buf), fmt, ap);
+    va_end(ap);
+    return gdn::host_fail(buf);
+}
+
+bool aligned(const void *p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+/* The call's device for the thread, and the previous one afterwards. */
+struct DeviceScope {
+    int prev = -1;
+    bool ok = false;
+    explicit DeviceScope(int device) {
+        if (cudaGetDevice(&prev) != cudaSuccess) return;
+        if (prev == device) {
+            prev = -1;
+            ok = true;
+        } else {
+            ok = cudaSetDevice(device) == cudaSuccess;
+        }
+    }
+    ~DeviceScope() {
+        if (prev >= 0) cudaSetDevice(prev);
+    }
+};
+
+int sm_count(int device) {
+    static int counts[64]; /* 0: not asked yet; every writer writes the same value */
+    if (device < 0 || device >= 64) return 0;
+    if (counts[device] == 0) {
+        int n = 0;
+        if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) return 0;
+        counts[device] = n;
+    }
+    return counts[device];
+}
+
+/* Checks what both forms of the rule ask of their arguments; > 0: nothing to do. */
+int delta_params(const char *who, const GdnB200DeltaArgs *a, gdn::ops::DeltaParams &p) {
+    if (a == nullptr) return failf("%s: no arguments", who);
+    if (a->dtype != 0 && a->dtype != 1) return failf("%s: dtype %d is neither FP32 (0) nor BF16 (1)", who, a->dtype);
+    if (a->key_dim != 64 && a->key_dim != 128 && a->key_dim != 256)
+        return failf("%s: key_dim %u is not 64, 128 or 256", who, a->key_dim);
+    if (a->value_dim == 0 || a->value_dim > 256 || a->value_dim % 32 != 0)
+        return failf("%s: value_dim %u is not a multiple of 32 up to 256", who, a->value_dim);
+    if (a->heads == 0 || a->v_heads == 0 || a->v_heads % a->heads != 0 || a->v_heads > 65535)
+        return failf("%s: %u value heads do not share %u query/key heads evenly", who, a->v_heads, a->heads);
+    if (a->tokens > 0x7fffffffu || a->sequences > 0x3fffffu)
+        return failf("%s: %u tokens in %u sequences are too many", who, a->tokens, a->sequences);
+    if (a->starts == nullptr && a->tokens != a->sequences)
+        return failf("%s: without starts every sequence has one token (%u tokens, %u sequences)", who, a->tokens,
+                     a->sequences);
+    if (a->sequences == 0) {
+        if (a->tokens != 0) return failf("%s: %u tokens but no sequence", who, a->tokens);
+        return 1;
+    }
+    if (a->slots == nullptr && a->state_slots < a->sequences)
+        return failf("%s: %u state slots for %u sequences", who, a->state_slots, a->sequences);
+    if (a->state == nullptr || !aligned(a->state, 16))
+        return failf("%s: state is missing or not on a 16-byte boundary", who);
+    const int64_t slot = (int64_t)a->v_heads * a->value_dim * a->key_dim;
+    if (a->state_slot % 4 != 0 || (a->state_slot < slot && a->state_slots > 1))
+        return failf("%s: state slots overlap or leave the 16-byte boundary (stride %lld)", who,
+                     (long long)a->state_slot);
+    if (a->tokens != 0 && (a->q == nullptr || a->k == nullptr || a->v == nullptr || a->g == nullptr ||
+                           a->beta == nullptr || a->out == nullptr))
+        return failf("%s: q, k, v, g, beta or out is missing", who);
+    p = gdn::ops::DeltaParams{a->q, a->k, a->v, a->g, a->beta, a->state, a->out, a->starts, a->slots, a->fresh,
+                              a->q_token, a->q_head, a->k_token, a->k_head, a->v_token, a->v_head,
+                              a->g_token, a->g_head, a->beta_token, a->beta_head, a->out_token, a->out_head,
+                              a->state_slot, a->sequences, a->tokens, a->heads, a->v_heads, a->key_dim,
+                              a->value_dim, a->state_slots, a->normalize != 0, a->scale};
+    return 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+int gdn_b200_delta_step(const GdnB200DeltaArgs *args) {
+    gdn::ops::DeltaParams p;
+    const int rc = delta_params("gdn_b200_delta_step", args, p);
+    if (rc != 0) return rc > 0 ? 0 : -1;
+    DeviceScope scope(args->device);
+    if (!scope.ok) return failf("gdn_b200_delta_step: cannot use device %d", args->device);
+    const cudaError_t e = gdn::ops::launch_delta_step(p, args->dtype == 1, static_cast<cudaStream_t>(args->stream));
+    return e == cudaSuccess ? 0 : failf("gdn_b200_delta_step: launch failed: %s", cudaGetErrorString(e));
+}
+
+size_t gdn_b200_delta_chunk_workspace(const GdnB200DeltaArgs *args) {
+    (void)args;
+    return 0;
+}
+
+int gdn_b200_delta_chunk(const GdnB200DeltaArgs *args) {
+    gdn::ops::DeltaParams p;
+    const int rc = delta_params("gdn_b200_delta_chunk", args, p);
+    if (rc != 0) return rc > 0 ? 0 : -1;
+    if (args->dtype != 1)
+        return failf("gdn_b200_delta_chunk: q, k and v must be BF16 (gdn_b200_delta_step takes FP32 of any length)");
+    if (!aligned(args->q, 16) || !aligned(args->k, 16) || !aligned(args->v, 16) || args->q_token % 8 != 0 ||
+        args->q_head % 8 != 0 || args->k_token % 8 != 0 || args->k_head % 8 != 0 || args->v_token % 8 != 0 ||
+        args->v_head % 8 != 0)
+        return failf("gdn_b200_delta_chunk: rows of q, k and v must start on 16-byte boundaries");
+    DeviceScope scope(args->device);
+    if (!scope.ok) return failf("gdn_b200_delta_chunk: cannot use device %d", args->device);
+    const cudaError_t e = gdn::ops::launch_delta_step(p, true, static_cast<cudaStream_t>(args->stream));
+    return e == cudaSuccess ? 0 : failf("gdn_b200_delta_chunk: launch failed: %s", cudaGetErrorString(e));
+}
+
+int gdn_b200_constrain_logits(const GdnB200LogitsArgs *args) {
+    const char *who = "gdn_b200_constrain_logits";
+    if (args == nullptr) return failf("%s: no arguments", who);
+    const GdnB200LogitsArgs &a = *args;
+    if (a.dtype != 0 && a.dtype != 1) return failf("%s: dtype %d is neither FP32 (0) nor BF16 (1)", who, a.dtype);
+    if (a.rows == 0) return 0;
+    if (a.rows > 0xffffffu) return failf("%s: %u rows are too many", who, a.rows);
+    if (a.vocab == 0 || a.vocab > gdn::ops::kMaxVocab)
+        return failf("%s: vocab %u is not in 1 .. %u", who, a.vocab, gdn::ops::kMaxVocab);
+    if (a.history > gdn::ops::kMaxHistory)
+        return failf("%s: a history of %u tokens is longer than %u", who, a.history, gdn::ops::kMaxHistory);
+    if (a.biases > gdn::ops::kMaxBiases)
+        return failf("%s: %u biases a row are more than %u", who, a.biases, gdn::ops::kMaxBiases);
+    if (a.logits == nullptr || a.out == nullptr || a.picks == nullptr)
+        return failf("%s: logits, out or picks is missing", who);
+    if (a.tokens == nullptr && a.history != 0) return failf("%s: tokens is missing", who);
+    if ((a.bias_ids == nullptr) != (a.bias == nullptr)) return failf("%s: bias_ids and bias go together", who);
+    const uintptr_t elem = a.dtype == 1 ? 2 : 4;
+    if (!aligned(a.logits, elem) || !aligned(a.out, elem)) return failf("%s: logits or out is misaligned", who);
+    if (a.rows > 1 && a.out_row < (int64_t)a.vocab) return failf("%s: rows of out overlap", who);
+    if (a.logits_row < 0) return failf("%s: negative row stride", who);
+    DeviceScope scope(a.device);
+    if (!scope.ok) return failf("%s: cannot use device %d", who, a.device);
+    const int sms = sm_count(a.device);
+    if (sms == 0) return failf("%s: device %d does not answer", who, a.device);
+    gdn::ops::LogitsParams p{a.logits, a.out, a.picks, a.history ? a.tokens : nullptr, a.lens, a.prompt_lens,
+                             a.repetition, a.presence, a.frequency, a.biases ? a.bias_ids : nullptr, a.bias, a.mask,
+                             a.logits_row, a.out_row, a.tokens_row, a.bias_ids_row, a.bias_row, a.mask_row,
+                             a.rows, a.vocab, a.history, a.biases, 0};
+    const cudaError_t e = gdn::ops::launch_logits(p, a.dtype == 1, sms, static_cast<cudaStream_t>(a.stream));
+    return e == cudaSuccess ? 0 : failf("%s: launch failed: %s", who, cudaGetErrorString(e));
+}
+
+}  // extern "C"

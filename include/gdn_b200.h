@@ -280,6 +280,89 @@ int gdn_b200_score_window(const GDNModel *model, GDNRunState *state, const int32
  * k a multiple of 64, n <= 80). */
 int gdn_b200_test_tile_gemm(uint32_t m, uint32_t k, uint32_t n, const float *w, const float *x, float *y);
 
+/* ------------------------------------------------ serving operators
+ * Operators of a server that keeps its own tensors: device pointers, the
+ * caller's stream, nothing allocated, nothing synchronised (a launch only, so
+ * that a call can be captured into a CUDA graph). No counterpart in the
+ * reference, whose decode ABI is one stream of the whole model.
+ *
+ * Gated delta rule over pooled states. The tokens of `sequences` sequences
+ * are packed: sequence n has the tokens starts[n] .. starts[n + 1] - 1
+ * (int32 [sequences + 1] from 0, not decreasing; NULL: token n alone, with
+ * tokens == sequences) and the state of pool slot slots[n] (int32, distinct;
+ * NULL: slot n), which is advanced in place; fresh[n] != 0 (bytes; NULL:
+ * none) starts from zero instead of the slot's content. Value head h uses
+ * query/key head h / (v_heads / heads). Per value head and token, S [V][K]:
+ *   S = e^g S;  d = beta (v - S k);  S = S + d k^T;  o = scale S q
+ * with q and k first divided by sqrt(sum x^2 + 1e-6) if normalize != 0.
+ * q, k, v and out are BF16 (dtype 1) or FP32 (dtype 0); g (the log decay),
+ * beta and the pool are FP32; all arithmetic is FP32 or closer. Strides count
+ * elements; the innermost dimension (K or V) is contiguous, and a slot of the
+ * pool is one block [v_heads][V][K] on a 16-byte boundary. A sequence
+ * whose slot lies outside the pool changes no state and gives zeros, as do
+ * tokens that no sequence covers. Entries of starts are clamped to [0, tokens].
+ * key_dim is 64, 128 or 256, value_dim a multiple of 32 up to 256. */
+typedef struct {
+    const void *q, *k, *v;
+    const float *g, *beta;
+    float *state;
+    void *out;
+    const int32_t *starts, *slots;
+    const uint8_t *fresh;
+    void *workspace;
+    size_t workspace_bytes;
+    void *stream; /* cudaStream_t */
+    int64_t q_token, q_head, k_token, k_head, v_token, v_head;
+    int64_t g_token, g_head, beta_token, beta_head, out_token, out_head, state_slot;
+    uint32_t sequences, tokens, heads, v_heads, key_dim, value_dim, state_slots;
+    int32_t dtype, normalize, device;
+    float scale;
+    uint32_t reserved; /* 0 */
+} GdnB200DeltaArgs;
+
+/* Token by token: the new token of every stream, or a few tokens of each
+ * (any number is right; its time grows with the longest sequence). Reads and
+ * writes each state once. The workspace is not used. */
+int gdn_b200_delta_step(const GdnB200DeltaArgs *args);
+/* Prompts: any lengths, BF16 only. 16-byte aligned q, k and v rows. */
+int gdn_b200_delta_chunk(const GdnB200DeltaArgs *args);
+/* Bytes of 256-byte aligned device memory that gdn_b200_delta_chunk needs as
+ * args->workspace for these sizes (its other fields are not read). */
+size_t gdn_b200_delta_chunk_workspace(const GdnB200DeltaArgs *args);
+
+/* Constraints on the logits of `rows` streams, and the greedy pick. With n
+ * the times token v stands in the row's history after its prompt:
+ *   in the history:    x = x > 0 ? x / repetition : x * repetition
+ *   n > 0:             x = (x - frequency n) - presence
+ *                      x = x + (the row's biases of v, summed in list order)
+ *   mask bit clear:    x = -inf
+ * each operation rounded to FP32, the result once to the logits' type. picks
+ * gets the lowest index of the row's largest result; NaN is never picked, and
+ * -1 says that nothing is above -inf. logits and out (may be logits itself):
+ * [rows][vocab], BF16 (dtype 1) or FP32 (dtype 0). tokens [rows][history]
+ * int32 with the first lens[row] in use (NULL: all) of which prompt_lens[row]
+ * are the prompt (NULL: none); repetition, presence, frequency FP32 [rows];
+ * bias_ids int32 and bias FP32 [rows][biases]; mask uint32
+ * [rows][ceil(vocab / 32)], bit v % 32 of word v / 32 set where v is allowed.
+ * Every one of them may be NULL (tokens only where history is 0, bias_ids and
+ * bias together); token ids outside [0, vocab) are skipped. vocab <= 262144, history <= 1048575,
+ * biases <= 2047. Row strides count elements, rows are contiguous. */
+typedef struct {
+    const void *logits;
+    void *out;
+    int32_t *picks;
+    const int32_t *tokens, *lens, *prompt_lens;
+    const float *repetition, *presence, *frequency;
+    const int32_t *bias_ids;
+    const float *bias;
+    const uint32_t *mask;
+    void *stream; /* cudaStream_t */
+    int64_t logits_row, out_row, tokens_row, bias_ids_row, bias_row, mask_row;
+    uint32_t rows, vocab, history, biases;
+    int32_t dtype, device;
+} GdnB200LogitsArgs;
+int gdn_b200_constrain_logits(const GdnB200LogitsArgs *args);
+
 #ifdef __cplusplus
 }
 #endif
