@@ -18,7 +18,8 @@ REPO = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libgdn_b200.so")
 SOURCES = ["gdn_decode.cu", "gdn_recurrence.cu", "gdn_batch.cu", "gdn_score.cu", "gdn_host.cu", "gdn_batch_host.cu",
-           "gdn_abi_host.cpp", "gdn_delta.cu", "gdn_logits.cu", "gdn_ops_host.cu"]
+           "gdn_abi_host.cpp", "gdn_delta.cu", "gdn_delta_chunk.cu",
+           "gdn_logits.cu", "gdn_ops_host.cu"]
 HEADERS = ["gdn_engine.h", "gdn_batch.h", "gdn_synth.h", "gdn_math.h", "gdn_ops.h", "exports.map"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 

@@ -1,0 +1,780 @@
+/* gdn_delta_chunk.cu -- the gated delta rule over prompts, 64 tokens at a
+ * time on the tensor cores (BF16 q, k, v; FP32 states in the pool).
+ *
+ * Within a chunk of C = 64 tokens, with G_i the sum of the log decays up to
+ * token i and khat, qhat the (normalised) keys and queries:
+ *   A_ij = beta_i e^(G_i - G_j) khat_i.khat_j (j < i),   T = (I + A)^-1
+ *   P_ij = scale e^(G_i - G_j) qhat_i.khat_j (j <= i)
+ *   R = beta (V - e^G khat S0^T),   D = T R
+ *   O = scale e^G qhat S0^T + (P T) R
+ *   S = e^(G_C) S0 + sum_j e^(G_C - G_j) D_j khat_j^T
+ * T and P T do not depend on the state, so a first kernel forms them for all
+ * chunks at once; a second one walks each sequence's chunks. The columns of
+ * S0^T (value rows) do not mix: a CTA takes kVB of them through the whole
+ * sequence, with the state in registers.
+ *
+ * The state has to come out as FP32 arithmetic would give it, from BF16
+ * tensor cores with FP32 accumulators: k and q enter as they are (exact), their
+ * norms and the decays scale rows of results, and each FP32 operand enters
+ * as BF16 terms that sum to it: three for S0, R and D (24 bits), two for T and
+ * P T (16 bits: T's unit diagonal is exact, so what is rounded is its smaller
+ * part below, and the outputs are BF16). The terms of an operand are columns
+ * of one MMA (N = 3 kVB), whose sums are added when they are read back.
+ */
+#include "gdn_ops.h"
+
+#include <cuda_bf16.h>
+
+namespace gdn {
+namespace ops {
+
+namespace {
+
+constexpr int kC = 64;      /* tokens of a chunk */
+constexpr int kVB = 16;     /* value rows of a CTA */
+constexpr uint64_t kWaitNs = 2000000000ull;
+
+/* per (chunk, value head): [T; P T] as two BF16 terms in the MMA's layout,
+ * then five rows of 64 floats */
+constexpr uint32_t kTermBytes = 2 * kC * 128;       /* 128 rows of 64 BF16 */
+constexpr uint32_t kPairBytes = 2 * kTermBytes;
+constexpr uint32_t kScalBytes = 5 * kC * 4;
+constexpr uint32_t kRecordBytes = kPairBytes + kScalBytes;
+enum { kScalC = 0, kScalBeta = 1, kScalQ = 2, kScalEnd = 3, kScalDecay = 4 };
+
+/* set when a wait of a kernel ran out; read and cleared by the host */
+__device__ int g_chunk_status;
+
+__device__ __forceinline__ uint32_t smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ uint64_t gtimer() {
+    uint64_t t;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+    return t;
+}
+__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+/* Bounded wait; false when the CTA gives up (here or elsewhere). */
+__device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, volatile uint32_t *abort) {
+    if (mbar_try(bar, parity)) return true;
+    const uint64_t t0 = gtimer();
+    while (!mbar_try(bar, parity)) {
+        if (*abort) return false;
+        if (gtimer() - t0 > kWaitNs) {
+            *abort = 1;
+            atomicExch(&g_chunk_status, 1);
+            return false;
+        }
+    }
+    return true;
+}
+/* the same for a whole warp, with one answer */
+__device__ __forceinline__ bool wait_bar_warp(uint32_t bar, uint32_t parity, volatile uint32_t *abort) {
+    return __all_sync(0xffffffffu, wait_bar(bar, parity, abort));
+}
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+/* Shared-memory matrix descriptors in the 128-byte swizzle (rows of 128 bytes,
+ * 16-byte piece p of row r at p ^ (r & 7), 1 KB per eight rows): start >> 4
+ * (bits 0-13), leading offset >> 4 (16-29), stride offset >> 4 (32-45),
+ * version 1 (46-47), layout 2 (61-63). The stride of 1 KB goes from one group
+ * of eight rows to the next. K-major (a row is an index of M or N): the leading
+ * offset is not used. MN-major (a row is an index of K, its 64 elements are
+ * indexes of M or N): it goes to the next 64 of them. */
+__device__ __forceinline__ uint64_t desc(uint32_t addr, uint32_t lead) {
+    return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(lead >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+           ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+/* kind::f16: D FP32, A and B BF16, A and B K-major or MN-major */
+__host__ __device__ constexpr uint32_t instr_desc(uint32_t m, uint32_t n, bool a_mn, bool b_mn) {
+    return (1u << 4) | (1u << 7) | (1u << 10) | ((a_mn ? 1u : 0u) << 15) | ((b_mn ? 1u : 0u) << 16) | ((n >> 3) << 17) |
+           ((m >> 4) << 24);
+}
+__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+/* eight FP32 columns of this thread's TMEM lane; tc_wait before the values are used */
+__device__ __forceinline__ void tc_ld8(uint32_t addr, uint32_t (&r)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];\n"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(addr));
+}
+__device__ __forceinline__ void tc_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+/* the sums of the three terms' columns: eight value rows starting at addr */
+__device__ __forceinline__ void tc_sum3(uint32_t addr, float (&x)[8]) {
+    uint32_t a[8], b[8], c[8];
+    __syncwarp();
+    tc_ld8(addr, a);
+    tc_ld8(addr + kVB, b);
+    tc_ld8(addr + 2 * kVB, c);
+    tc_wait();
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        x[i] = __uint_as_float(a[i]) + (__uint_as_float(b[i]) + __uint_as_float(c[i]));
+}
+
+/* 16-byte piece `piece` of row `row` in the 128-byte swizzle */
+__device__ __forceinline__ uint32_t piece_at(uint32_t row, uint32_t piece) { return row * 128u + ((piece ^ (row & 7u)) << 4); }
+
+__device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+/* Eight values as three BF16 terms (each residual is exact; an infinity's or a
+ * NaN's second term is NaN, as the value would make every sum it enters):
+ * row `row` of an MN-major operand, pieces term * kVB / 8 + half. */
+__device__ __forceinline__ void put_terms(uint8_t *base, uint32_t row, uint32_t half, const float (&x)[8]) {
+    float r[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = x[i];
+#pragma unroll
+    for (int term = 0; term < 3; ++term) {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            w[i] = bf16_pair(r[2 * i], r[2 * i + 1]);
+            r[2 * i] -= __uint_as_float(w[i] << 16);
+            r[2 * i + 1] -= __uint_as_float(w[i] & 0xFFFF0000u);
+        }
+        *reinterpret_cast<uint4 *>(base + piece_at(row, term * (kVB / 8) + half)) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+}
+
+/* `rows` tokens from t0 on of one head (zeros up to 64) as the rows `first`
+ * .. first + 63 of [128 rows][64 columns] blocks in the 128-byte swizzle */
+template <int K>
+__device__ __forceinline__ void load_rows(uint32_t tile, uint32_t first, const __nv_bfloat16 *x, int64_t t0, int64_t stride,
+                                          uint32_t rows, uint32_t thread, uint32_t threads) {
+    constexpr uint32_t kPieces = K / 8;
+#pragma unroll 8
+    for (uint32_t i = thread; i < kC * kPieces; i += threads) {
+        const uint32_t r = i / kPieces, c = i % kPieces;
+        const uint32_t dst = tile + (c >> 3) * kTermBytes + piece_at(first + r, c & 7);
+        const __nv_bfloat16 *src = r < rows ? x + (t0 + r) * stride + c * 8 : x;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(r < rows ? 16u : 0u)
+                     : "memory");
+    }
+}
+__device__ __forceinline__ void cp_async_wait_all() {
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+}
+
+/* Records are numbered so that no prefix sum over the sequences is needed:
+ * chunk c of sequence n has number starts[n] / 64 + n + c. */
+__host__ __device__ __forceinline__ uint32_t record_of(uint32_t t0, uint32_t n) { return t0 / kC + n; }
+
+/* ------------------------------------------------------------ first kernel */
+
+constexpr int kPrepThreads = 256;
+constexpr uint32_t kLd = kC + 4; /* row stride of the FP32 matrices, floats */
+
+template <int K>
+struct PrepSmem {
+    static constexpr uint32_t kTile = 0;                                  /* [K; Q] */
+    static constexpr uint32_t kA = kTile + (K / 64) * kTermBytes;         /* A, then T */
+    static constexpr uint32_t kP = kA + kC * kLd * 4;
+    static constexpr uint32_t kX = kP + kC * kLd * 4;                     /* products of the inversion */
+    static constexpr uint32_t kG = kX + 32 * kLd * 4;                     /* G hi, lo, beta, inverse norms of k, q */
+    static constexpr uint32_t kBar = kG + 5 * kC * 4;
+    static constexpr uint32_t kBytes = kBar + 32 + 1024;                  /* room to align */
+};
+
+/* out[r][c] (m x m, at out) = sign * a[m x m] b[m x m], all in rows of kLd;
+ * the threads of a group of `threads` take one element group each */
+__device__ __forceinline__ void small_product(float *out, const float *a, const float *b, int m, float sign, int thread,
+                                              int threads) {
+    for (int i = thread; i < m * (m / 4); i += threads) {
+        const int r = i / (m / 4), c = (i % (m / 4)) * 4;
+        float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+        for (int j = 0; j < m; ++j) {
+            const float x = a[r * kLd + j];
+            const float4 y = *reinterpret_cast<const float4 *>(b + j * kLd + c);
+            s.x = fmaf(x, y.x, s.x);
+            s.y = fmaf(x, y.y, s.y);
+            s.z = fmaf(x, y.z, s.z);
+            s.w = fmaf(x, y.w, s.w);
+        }
+        *reinterpret_cast<float4 *>(out + r * kLd + c) = make_float4(sign * s.x, sign * s.y, sign * s.z, sign * s.w);
+    }
+}
+
+/* four values of row `row` as two BF16 terms of the record's [T; P T] */
+__device__ __forceinline__ void put_pair4(uint8_t *rec, uint32_t row, uint32_t col, float4 x) {
+    const uint32_t w0 = bf16_pair(x.x, x.y), w1 = bf16_pair(x.z, x.w);
+    const uint32_t u0 = bf16_pair(x.x - __uint_as_float(w0 << 16), x.y - __uint_as_float(w0 & 0xFFFF0000u));
+    const uint32_t u1 = bf16_pair(x.z - __uint_as_float(w1 << 16), x.w - __uint_as_float(w1 & 0xFFFF0000u));
+    uint8_t *p = rec + piece_at(row, col >> 3) + (col & 7) * 2;
+    *reinterpret_cast<uint2 *>(p) = make_uint2(w0, w1);
+    *reinterpret_cast<uint2 *>(p + kTermBytes) = make_uint2(u0, u1);
+}
+
+template <int K>
+__global__ void __launch_bounds__(kPrepThreads) chunk_prep_kernel(const __grid_constant__ DeltaParams p, uint8_t *records) {
+    using L = PrepSmem<K>;
+    extern __shared__ uint8_t raw[];
+    uint8_t *sm = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
+    const uint32_t base = smem_u32(sm);
+    const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const uint32_t rec = blockIdx.x, h = blockIdx.y, hq = h / (p.HV / p.H);
+    __nv_bfloat16 *out = static_cast<__nv_bfloat16 *>(p.out);
+
+    /* the sequence whose records hold number rec: the last one that starts at or before it */
+    uint32_t t0, t1, n;
+    uint32_t lo = 0, hi = p.N; /* N: the tokens after the last sequence */
+    while (lo < hi) {
+        const uint32_t mid = (lo + hi + 1) / 2;
+        uint32_t a, b;
+        if (mid == p.N) {
+            sequence_tokens(p, p.N - 1, b, a);
+        } else {
+            sequence_tokens(p, mid, a, b);
+        }
+        if (record_of(a, mid) <= rec)
+            lo = mid;
+        else
+            hi = mid - 1;
+    }
+    n = lo;
+    if (n == 0 && p.starts != nullptr) {
+        /* tokens before the first sequence give zeros */
+        sequence_tokens(p, 0, t0, t1);
+        const uint32_t z1 = min(t0, (rec + 1) * kC);
+        for (uint32_t t = rec * kC; t < z1; ++t)
+            for (uint32_t i = tid; i < p.V; i += kPrepThreads)
+                out[(int64_t)t * p.out_token + (int64_t)h * p.out_head + i] = __float2bfloat16_rn(0.0f);
+        if (rec < record_of(t0, 0)) return;
+    }
+    if (n == p.N) {
+        uint32_t a;
+        sequence_tokens(p, p.N - 1, a, t0);
+        t0 += (rec - record_of(t0, p.N)) * kC;
+        for (uint32_t t = t0; t < min(p.tokens, t0 + kC); ++t)
+            for (uint32_t i = tid; i < p.V; i += kPrepThreads)
+                out[(int64_t)t * p.out_token + (int64_t)h * p.out_head + i] = __float2bfloat16_rn(0.0f);
+        return;
+    }
+    sequence_tokens(p, n, t0, t1);
+    t0 += (rec - record_of(t0, n)) * kC;
+    if (t0 >= t1) return;
+    const uint32_t rows = min((uint32_t)kC, t1 - t0);
+    uint8_t *record = records + ((size_t)rec * p.HV + h) * kRecordBytes;
+
+    const __nv_bfloat16 *q = static_cast<const __nv_bfloat16 *>(p.q) + (int64_t)hq * p.q_head;
+    const __nv_bfloat16 *k = static_cast<const __nv_bfloat16 *>(p.k) + (int64_t)hq * p.k_head;
+    load_rows<K>(base + L::kTile, 0, k, t0, p.k_token, rows, tid, kPrepThreads);
+    load_rows<K>(base + L::kTile, kC, q, t0, p.q_token, rows, tid, kPrepThreads);
+
+    float *A = reinterpret_cast<float *>(sm + L::kA), *P = reinterpret_cast<float *>(sm + L::kP);
+    float *X = reinterpret_cast<float *>(sm + L::kX), *G = reinterpret_cast<float *>(sm + L::kG);
+    float *Glo = G + kC, *bet = G + 2 * kC, *kin = G + 3 * kC, *qin = G + 4 * kC;
+    const uint32_t bar = base + L::kBar;
+    uint32_t *slot = reinterpret_cast<uint32_t *>(sm + L::kBar + 8);
+    volatile uint32_t *abort = reinterpret_cast<volatile uint32_t *>(sm + L::kBar + 16);
+    if (tid == 0) {
+        mbar_init(bar, 1);
+        *abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 0) {
+        __syncwarp();
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(64u)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    if (warp == 1) {
+        /* sums of the log decays in 64 bits, kept as two floats: differences of
+         * nearby sums stay exact however far the sums have gone. e^-10000 is
+         * 0 like any decay below it. */
+        double s[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint32_t r = 2 * lane + i;
+            const float gv = r < rows ? p.g[(int64_t)(t0 + r) * p.g_token + (int64_t)h * p.g_head] : 0.0f;
+            s[i] = (double)(gv < -10000.0f ? -10000.0f : gv);
+            bet[r] = r < rows ? p.beta[(int64_t)(t0 + r) * p.beta_token + (int64_t)h * p.beta_head] : 0.0f;
+        }
+        s[1] += s[0];
+        double run = s[1];
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const double below = __shfl_up_sync(0xffffffffu, run, o);
+            if (lane >= (uint32_t)o) run += below;
+        }
+        double before = __shfl_up_sync(0xffffffffu, run, 1);
+        if (lane == 0) before = 0.0;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const double x = before + s[i];
+            const float hi32 = (float)x;
+            G[2 * lane + i] = hi32;
+            Glo[2 * lane + i] = (float)(x - (double)hi32);
+        }
+    }
+    cp_async_wait_all();
+    fence_async();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *slot;
+    if (tid == 0) {
+        /* [K; Q] K^T */
+#pragma unroll
+        for (int kk = 0; kk < K / 16; ++kk) {
+            const uint32_t at = base + L::kTile + (kk / 4) * kTermBytes + (kk % 4) * 32;
+            mma(tmem, desc(at, 16), desc(at, 16), instr_desc(2 * kC, kC, false, false), kk != 0);
+        }
+        commit(bar);
+    }
+    /* norms meanwhile: two lanes per row */
+    {
+        const uint32_t r = tid >> 1; /* 0..127: K rows, then Q rows */
+        float ss = 0.0f;
+        for (uint32_t c = tid & 1; c < K / 8; c += 2) {
+            const uint4 w = *reinterpret_cast<const uint4 *>(sm + L::kTile + (c >> 3) * kTermBytes + piece_at(r, c & 7));
+            const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float a = __uint_as_float(u[i] << 16), b = __uint_as_float(u[i] & 0xFFFF0000u);
+                ss = fmaf(a, a, ss);
+                ss = fmaf(b, b, ss);
+            }
+        }
+        ss += __shfl_xor_sync(0xffffffffu, ss, 1);
+        const float inv = p.normalize ? 1.0f / sqrtf(ss + 1e-6f) : 1.0f;
+        if ((tid & 1) == 0) {
+            if (r < kC)
+                kin[r] = inv;
+            else
+                qin[r - kC] = inv * p.scale;
+        }
+    }
+    __syncthreads();
+    /* the record's rows of scalars */
+    if (tid < kC) {
+        float *sc = reinterpret_cast<float *>(record + kPairBytes);
+        const float g1 = G[tid] + Glo[tid], eg = expf(g1);
+        const bool there = tid < rows;
+        sc[kScalC * kC + tid] = there ? eg * kin[tid] : 0.0f;
+        sc[kScalBeta * kC + tid] = bet[tid];
+        sc[kScalQ * kC + tid] = eg * qin[tid];
+        sc[kScalEnd * kC + tid] = there ? expf((G[kC - 1] - G[tid]) + (Glo[kC - 1] - Glo[tid])) * kin[tid] : 0.0f;
+        if (tid == kC - 1) sc[kScalDecay * kC] = eg;
+    }
+    bool ok = wait_bar_warp(bar, 0, abort);
+    tc_fence_after();
+    if (ok) {
+        /* lanes 0..63: rows of A; 64..127: rows of P; warps 4..7 take columns 32..63 */
+        const uint32_t row = 32 * (warp & 3) + lane, i = row & (kC - 1), c0 = (warp >> 2) * 32;
+        const bool is_p = row >= kC;
+        const float gi = G[i], gl = Glo[i], f = is_p ? qin[i] : bet[i] * kin[i];
+        float *dst = (is_p ? P : A) + i * kLd;
+#pragma unroll
+        for (int c = 0; c < 32; c += 8) {
+            uint32_t r[8];
+            __syncwarp();
+            tc_ld8(tmem + ((32 * (warp & 3)) << 16) + c0 + c, r);
+            tc_wait();
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const uint32_t j = c0 + c + e;
+                float x = 0.0f;
+                if (j < i || (is_p && j == i))
+                    x = f * kin[j] * expf((gi - G[j]) + (gl - Glo[j])) * __uint_as_float(r[e]);
+                if (!is_p && j == i) x = 1.0f;
+                dst[j] = x;
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 0) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(64u) : "memory");
+    }
+    /* T = (I + A)^-1 in place: the 16 x 16 diagonal blocks by forward
+     * substitution (a lane per column), then twice
+     * [[a 0] [c b]]^-1 = [[a^-1 0] [-b^-1 c a^-1, b^-1]] */
+    if (warp < 4) {
+        float *D = A + (16 * warp) * kLd + 16 * warp;
+        if (lane < 16) {
+            float x[16];
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                float s = r == (int)lane ? 1.0f : 0.0f;
+#pragma unroll
+                for (int j = 0; j < 16; ++j)
+                    if (j < r) s = fmaf(-D[r * kLd + j], x[j], s);
+                x[r] = s;
+            }
+            __syncwarp(0xffffu);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) D[r * kLd + lane] = x[r];
+        }
+    }
+    __syncthreads();
+    {
+        /* two blocks of 32: half of the threads each */
+        const int b = tid >> 7, th = tid & 127;
+        float *D = A + (32 * b) * kLd + 32 * b, *Y = X + (16 * b) * kLd;
+        small_product(Y, D + 16 * kLd, D, 16, 1.0f, th, 128);
+        __syncthreads();
+        small_product(D + 16 * kLd, D + 16 * kLd + 16, Y, 16, -1.0f, th, 128);
+    }
+    __syncthreads();
+    small_product(X, A + 32 * kLd, A, 32, 1.0f, tid, kPrepThreads);
+    __syncthreads();
+    small_product(A + 32 * kLd, A + 32 * kLd + 32, X, 32, -1.0f, tid, kPrepThreads);
+    __syncthreads();
+    /* the record: rows 0..63 T, rows 64..127 P T (both lower triangular) */
+    for (uint32_t i = tid; i < kC * (kC / 4); i += kPrepThreads) {
+        const uint32_t r = i / (kC / 4), c = (i % (kC / 4)) * 4;
+        float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (uint32_t j = c; j <= r; ++j) {
+            const float x = P[r * kLd + j];
+            const float4 y = *reinterpret_cast<const float4 *>(A + j * kLd + c);
+            s.x = fmaf(x, y.x, s.x);
+            s.y = fmaf(x, y.y, s.y);
+            s.z = fmaf(x, y.z, s.z);
+            s.w = fmaf(x, y.w, s.w);
+        }
+        put_pair4(record, r, c, *reinterpret_cast<const float4 *>(A + r * kLd + c));
+        put_pair4(record, kC + r, c, s);
+    }
+}
+
+/* ----------------------------------------------------------- second kernel */
+
+/* warps 0-7 epilogues, 8 MMAs, 9 records, 10-13 loads of k and q */
+constexpr int kScanThreads = 14 * 32;
+constexpr uint32_t kLoadThreads = 128;
+
+template <int K>
+struct ScanSmem {
+    static constexpr uint32_t kStage = (K / 64) * kTermBytes;    /* [K; Q] */
+    static constexpr uint32_t kKQ = 0;
+    static constexpr uint32_t kPair = kKQ + 2 * kStage;          /* [T; P T] */
+    static constexpr uint32_t kS = kPair + kPairBytes;           /* terms of S0, rows k */
+    static constexpr uint32_t kR = kS + K * 128;                 /* terms of R, rows token */
+    static constexpr uint32_t kD = kR + kC * 128;                /* terms of the scaled D */
+    static constexpr uint32_t kBar = kD + kC * 128;
+    static constexpr uint32_t kBytes = kBar + 256 + 1024;
+};
+
+template <int K>
+__global__ void __launch_bounds__(kScanThreads, 1) chunk_scan_kernel(const __grid_constant__ DeltaParams p, const uint8_t *records,
+                                                                     uint32_t out_wide) {
+    using L = ScanSmem<K>;
+    constexpr int kTiles = K > 128 ? K / 128 : 1; /* M = 128 tiles of key rows */
+    extern __shared__ uint8_t raw[];
+    uint8_t *sm = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
+    const uint32_t base = smem_u32(sm);
+    const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const uint32_t vblocks = p.V / kVB;
+    const uint32_t n = blockIdx.x / (p.HV * vblocks), rem = blockIdx.x - n * (p.HV * vblocks);
+    const uint32_t h = rem / vblocks, v0 = (rem - h * vblocks) * kVB, hq = h / (p.HV / p.H);
+    __nv_bfloat16 *out = static_cast<__nv_bfloat16 *>(p.out) + (int64_t)h * p.out_head + v0;
+
+    uint32_t t0, t1;
+    sequence_tokens(p, n, t0, t1);
+    const int64_t pool = sequence_slot(p, n);
+    const bool fresh = p.fresh != nullptr && p.fresh[n] != 0;
+    if (pool < 0) {
+        for (uint32_t i = tid; i < (t1 - t0) * kVB; i += kScanThreads)
+            out[(int64_t)(t0 + i / kVB) * p.out_token + i % kVB] = __float2bfloat16_rn(0.0f);
+        return;
+    }
+    float *S = p.state + pool * p.state_slot + ((int64_t)h * p.V + v0) * K;
+    if (t0 == t1) {
+        if (fresh)
+            for (uint32_t i = tid; i < kVB * K; i += kScanThreads) S[i] = 0.0f;
+        return;
+    }
+    const uint32_t chunks = (t1 - t0 + kC - 1) / kC, rec0 = record_of(t0, n);
+
+    const uint32_t bar = base + L::kBar;
+    const uint32_t full_kq = bar, empty_k = bar + 16, empty_q = bar + 32, full_pair = bar + 48, empty_pair = bar + 56,
+                   s_ready = bar + 64, d1_full = bar + 72, r_ready = bar + 80, d3_full = bar + 88, d_ready = bar + 96,
+                   d4_full = bar + 104, drain = bar + 112;
+    uint32_t *slot = reinterpret_cast<uint32_t *>(sm + L::kBar + 128);
+    volatile uint32_t *abort = reinterpret_cast<volatile uint32_t *>(sm + L::kBar + 136);
+    if (tid == 0) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(full_kq + 8 * i, kLoadThreads);
+            mbar_init(empty_k + 8 * i, 1);
+            mbar_init(empty_q + 8 * i, 1);
+        }
+        mbar_init(full_pair, 1);
+        mbar_init(empty_pair, 1);
+        mbar_init(s_ready, 256);
+        mbar_init(d1_full, 1);
+        mbar_init(r_ready, 128);
+        mbar_init(d3_full, 1);
+        mbar_init(d_ready, 128);
+        mbar_init(d4_full, 1);
+        mbar_init(drain, 1);
+        *abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 0) {
+        __syncwarp();
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(256u)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *slot;
+    const uint32_t d1 = tmem, d3 = tmem + 64, d4 = tmem + 128;
+
+    if (warp >= 10) {
+        /* k and q of the chunks, two in flight; a stage's q rows are free once
+         * its first MMAs are done, its k rows after the last ones */
+        const __nv_bfloat16 *q = static_cast<const __nv_bfloat16 *>(p.q) + (int64_t)hq * p.q_head;
+        const __nv_bfloat16 *k = static_cast<const __nv_bfloat16 *>(p.k) + (int64_t)hq * p.k_head;
+        const uint32_t th = tid - 10 * 32;
+        for (uint32_t c = 0; c < chunks; ++c) {
+            const uint32_t st = c & 1, tile = base + L::kKQ + st * L::kStage;
+            const uint32_t tc = t0 + c * kC, rows = min((uint32_t)kC, t1 - tc);
+            if (c >= 2 && !wait_bar(empty_q + 8 * st, ((c >> 1) - 1) & 1u, abort)) break;
+            load_rows<K>(tile, kC, q, tc, p.q_token, rows, th, kLoadThreads);
+            if (c >= 2 && !wait_bar(empty_k + 8 * st, ((c >> 1) - 1) & 1u, abort)) break;
+            load_rows<K>(tile, 0, k, tc, p.k_token, rows, th, kLoadThreads);
+            cp_async_wait_all();
+            fence_async();
+            mbar_arrive(full_kq + 8 * st);
+        }
+        cp_async_wait_all();
+    } else if (warp == 9) {
+        if (lane == 0) {
+            uint32_t c = 0;
+            for (; c < chunks; ++c) {
+                if (c >= 1 && !wait_bar(empty_pair, (c - 1) & 1u, abort)) break;
+                const uint8_t *src = records + ((size_t)(rec0 + c) * p.HV + h) * kRecordBytes;
+                asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(full_pair), "r"(kPairBytes)
+                             : "memory");
+                asm volatile(
+                    "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                        base + L::kPair),
+                    "l"(src), "r"(kPairBytes), "r"(full_pair)
+                    : "memory");
+            }
+            /* the last copy lands before the CTA ends (an abort does not stop it) */
+            const uint64_t w0 = gtimer();
+            while (!mbar_try(full_pair, (c - 1) & 1u) && gtimer() - w0 < kWaitNs) {
+            }
+        }
+    } else if (warp == 8) {
+        if (lane == 0) {
+            for (uint32_t c = 0; c < chunks; ++c) {
+                const uint32_t st = c & 1, ph = c & 1, tile = base + L::kKQ + st * L::kStage;
+                if (!wait_bar(full_kq + 8 * st, (c >> 1) & 1u, abort) || !wait_bar(s_ready, ph, abort)) break;
+                tc_fence_after();
+                /* [K; Q] S0^T */
+#pragma unroll
+                for (int kk = 0; kk < K / 16; ++kk)
+                    mma(d1, desc(tile + (kk / 4) * kTermBytes + (kk % 4) * 32, 16), desc(base + L::kS + kk * 2048, 1024),
+                        instr_desc(128, 3 * kVB, false, true), kk != 0);
+                commit(d1_full);
+                commit(empty_q + 8 * st);
+                if (!wait_bar(full_pair, ph, abort) || !wait_bar(r_ready, ph, abort)) break;
+                tc_fence_after();
+                /* [T; P T] R: the first term with all of R, the second with R's first two */
+#pragma unroll
+                for (int kk = 0; kk < kC / 16; ++kk)
+                    mma(d3, desc(base + L::kPair + kk * 32, 16), desc(base + L::kR + kk * 2048, 1024),
+                        instr_desc(128, 3 * kVB, false, true), kk != 0);
+#pragma unroll
+                for (int kk = 0; kk < kC / 16; ++kk)
+                    mma(d3, desc(base + L::kPair + kTermBytes + kk * 32, 16), desc(base + L::kR + kk * 2048, 1024),
+                        instr_desc(128, 2 * kVB, false, true), true);
+                commit(d3_full);
+                commit(empty_pair);
+                if (!wait_bar(d_ready, ph, abort)) break;
+                tc_fence_after();
+                /* K^T D (64 key rows: the upper half of M runs into the q rows and is not read) */
+#pragma unroll
+                for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+                    for (int kk = 0; kk < kC / 16; ++kk)
+                        mma(d4 + 64 * t, desc(tile + t * 2 * kTermBytes + kk * 2048, K >= 128 ? kTermBytes : kTermBytes / 2),
+                            desc(base + L::kD + kk * 2048, 1024), instr_desc(128, 3 * kVB, true, true), kk != 0);
+                commit(d4_full);
+                commit(empty_k + 8 * st);
+            }
+            /* every MMA issued is done before TMEM is released */
+            commit(drain);
+            const uint64_t w0 = gtimer();
+            while (!mbar_try(drain, 0) && gtimer() - w0 < kWaitNs) {
+            }
+        }
+    } else {
+        /* epilogues: thread = TMEM lane (token of [K; Q], or key row) and eight
+         * of the value rows */
+        const uint32_t ln = 32 * (warp & 3) + lane, half = warp >> 2;
+        const uint32_t at = ((32 * (warp & 3)) << 16) + 8 * half;
+        const bool is_o = ln >= kC; /* uniform in a warp */
+        const uint32_t i = ln & (kC - 1);
+        const __nv_bfloat16 *v = static_cast<const __nv_bfloat16 *>(p.v) + (int64_t)h * p.v_head + v0 + 8 * half;
+        const bool has_s = K >= 128 || ln < (uint32_t)K;
+        float s[kTiles][8];
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                s[t][e] = (has_s && !fresh) ? S[(int64_t)(8 * half + e) * K + 128 * t + ln] : 0.0f;
+        bool ok = true;
+        for (uint32_t c = 0; c < chunks; ++c) {
+            const uint32_t ph = c & 1, tc = t0 + c * kC, rows = min((uint32_t)kC, t1 - tc);
+            if (has_s) {
+#pragma unroll
+                for (int t = 0; t < kTiles; ++t) put_terms(sm + L::kS, 128 * t + ln, half, s[t]);
+            }
+            fence_async();
+            tc_fence_before();
+            mbar_arrive(s_ready);
+            /* this token's scalars and values, while the MMAs run */
+            const float *sc = reinterpret_cast<const float *>(records + ((size_t)(rec0 + c) * p.HV + h) * kRecordBytes + kPairBytes);
+            const float decay = sc[kScalDecay * kC];
+            float f0, f1 = 0.0f, f2 = 0.0f;
+            uint4 vw = make_uint4(0, 0, 0, 0);
+            if (is_o) {
+                f0 = sc[kScalQ * kC + i];
+            } else {
+                f0 = sc[kScalC * kC + i];
+                f1 = sc[kScalBeta * kC + i];
+                f2 = sc[kScalEnd * kC + i];
+                if (i < rows) vw = *reinterpret_cast<const uint4 *>(v + (int64_t)(tc + i) * p.v_token);
+            }
+            float x[8], o[8];
+            if (!(ok = wait_bar_warp(d1_full, ph, abort))) break;
+            tc_fence_after();
+            tc_sum3(d1 + at, x);
+            if (is_o) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) o[e] = f0 * x[e];
+            } else {
+                const uint32_t u[4] = {vw.x, vw.y, vw.z, vw.w};
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float vv = __uint_as_float((e & 1) ? (u[e >> 1] & 0xFFFF0000u) : (u[e >> 1] << 16));
+                    x[e] = i < rows ? f1 * fmaf(-f0, x[e], vv) : 0.0f;
+                }
+                put_terms(sm + L::kR, i, half, x);
+                fence_async();
+                tc_fence_before();
+                mbar_arrive(r_ready);
+            }
+            if (!(ok = wait_bar_warp(d3_full, ph, abort))) break;
+            tc_fence_after();
+            tc_sum3(d3 + at, x);
+            if (is_o) {
+                if (i < rows) {
+                    __nv_bfloat16 *dst = out + (int64_t)(tc + i) * p.out_token + 8 * half;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) o[e] += x[e];
+                    if (out_wide) {
+                        *reinterpret_cast<uint4 *>(dst) = make_uint4(bf16_pair(o[0], o[1]), bf16_pair(o[2], o[3]),
+                                                                     bf16_pair(o[4], o[5]), bf16_pair(o[6], o[7]));
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) dst[e] = __float2bfloat16_rn(o[e]);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] *= f2;
+                put_terms(sm + L::kD, i, half, x);
+                fence_async();
+                tc_fence_before();
+                mbar_arrive(d_ready);
+            }
+            if (!(ok = wait_bar_warp(d4_full, ph, abort))) break;
+            tc_fence_after();
+#pragma unroll
+            for (int t = 0; t < kTiles; ++t) {
+                tc_sum3(d4 + 64 * t + at, x);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) s[t][e] = fmaf(decay, s[t][e], x[e]);
+            }
+        }
+        if (has_s) {
+            /* a sequence that was given up leaves no state that could pass for one */
+            const float bad = ok ? 0.0f : __int_as_float(0x7fc00000);
+#pragma unroll
+            for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) S[(int64_t)(8 * half + e) * K + 128 * t + ln] = ok ? s[t][e] : bad;
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 0) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(256u) : "memory");
+    }
+}
+
+uint32_t record_count(uint32_t tokens, uint32_t sequences) { return tokens / kC + sequences + 2; }
+
+template <int K>
+cudaError_t launch_chunk_k(const DeltaParams &p, uint8_t *records, cudaStream_t stream) {
+    cudaError_t e = cudaFuncSetAttribute(chunk_prep_kernel<K>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         (int)PrepSmem<K>::kBytes);
+    if (e != cudaSuccess) return e;
+    e = cudaFuncSetAttribute(chunk_scan_kernel<K>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ScanSmem<K>::kBytes);
+    if (e != cudaSuccess) return e;
+    chunk_prep_kernel<K><<<dim3(record_count(p.tokens, p.N), p.HV), kPrepThreads, PrepSmem<K>::kBytes, stream>>>(p, records);
+    if ((e = cudaGetLastError()) != cudaSuccess) return e;
+    const bool wide = (reinterpret_cast<uintptr_t>(p.out) & 15) == 0 && p.out_token % 8 == 0 && p.out_head % 8 == 0;
+    chunk_scan_kernel<K><<<p.N * p.HV * (p.V / kVB), kScanThreads, ScanSmem<K>::kBytes, stream>>>(p, records, wide);
+    return cudaGetLastError();
+}
+
+}  // namespace
+
+size_t delta_chunk_workspace(uint32_t tokens, uint32_t sequences, uint32_t v_heads) {
+    return (size_t)record_count(tokens, sequences) * v_heads * kRecordBytes;
+}
+
+cudaError_t launch_delta_chunk(const DeltaParams &p, void *workspace, cudaStream_t stream) {
+    uint8_t *records = static_cast<uint8_t *>(workspace);
+    switch (p.K) {
+        case 64: return launch_chunk_k<64>(p, records, stream);
+        case 128: return launch_chunk_k<128>(p, records, stream);
+        default: return launch_chunk_k<256>(p, records, stream);
+    }
+}
+
+cudaError_t delta_chunk_status(int *status) {
+    cudaError_t e = cudaMemcpyFromSymbol(status, g_chunk_status, sizeof(int));
+    const int zero = 0;
+    if (e == cudaSuccess && *status != 0) e = cudaMemcpyToSymbol(g_chunk_status, &zero, sizeof(int));
+    return e;
+}
+
+}  // namespace ops
+}  // namespace gdn

@@ -106,8 +106,15 @@ int gdn_b200_delta_step(const GdnB200DeltaArgs *args) {
 }
 
 size_t gdn_b200_delta_chunk_workspace(const GdnB200DeltaArgs *args) {
-    (void)args;
-    return 0;
+    return args == nullptr ? 0 : gdn::ops::delta_chunk_workspace(args->tokens, args->sequences, args->v_heads);
+}
+
+int gdn_b200_delta_chunk_status(int device) {
+    DeviceScope scope(device);
+    int status = 0;
+    if (!scope.ok || gdn::ops::delta_chunk_status(&status) != cudaSuccess)
+        return failf("gdn_b200_delta_chunk_status: cannot read the status of device %d", device);
+    return status == 0 ? 0 : failf("gdn_b200_delta_chunk: a wait on the device ran out; the call's states are not valid");
 }
 
 int gdn_b200_delta_chunk(const GdnB200DeltaArgs *args) {
@@ -120,9 +127,12 @@ int gdn_b200_delta_chunk(const GdnB200DeltaArgs *args) {
         args->q_head % 8 != 0 || args->k_token % 8 != 0 || args->k_head % 8 != 0 || args->v_token % 8 != 0 ||
         args->v_head % 8 != 0)
         return failf("gdn_b200_delta_chunk: rows of q, k and v must start on 16-byte boundaries");
+    const size_t need = gdn::ops::delta_chunk_workspace(args->tokens, args->sequences, args->v_heads);
+    if (args->workspace == nullptr || !aligned(args->workspace, 256) || args->workspace_bytes < need)
+        return failf("gdn_b200_delta_chunk: a workspace of %zu bytes on a 256-byte boundary is needed", need);
     DeviceScope scope(args->device);
     if (!scope.ok) return failf("gdn_b200_delta_chunk: cannot use device %d", args->device);
-    const cudaError_t e = gdn::ops::launch_delta_step(p, true, static_cast<cudaStream_t>(args->stream));
+    const cudaError_t e = gdn::ops::launch_delta_chunk(p, args->workspace, static_cast<cudaStream_t>(args->stream));
     return e == cudaSuccess ? 0 : failf("gdn_b200_delta_chunk: launch failed: %s", cudaGetErrorString(e));
 }
 

@@ -329,6 +329,10 @@ int gdn_b200_delta_chunk(const GdnB200DeltaArgs *args);
 /* Bytes of 256-byte aligned device memory that gdn_b200_delta_chunk needs as
  * args->workspace for these sizes (its other fields are not read). */
 size_t gdn_b200_delta_chunk_workspace(const GdnB200DeltaArgs *args);
+/* 0, or -1 if a wait inside gdn_b200_delta_chunk ran out (2 s) on `device`
+ * since the last call of this function: the states of that call are then NaN.
+ * Waits for the device; for a server's health checks and for tests. */
+int gdn_b200_delta_chunk_status(int device);
 
 /* Constraints on the logits of `rows` streams, and the greedy pick. With n
  * the times token v stands in the row's history after its prompt:
