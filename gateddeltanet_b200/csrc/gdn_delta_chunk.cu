@@ -57,12 +57,19 @@ __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
+/* One arrival for the warp, after all its lanes got here: a barrier's arrivals
+ * are served one after the other, and 256 of them took longer than the MMAs
+ * they were to start. */
+__device__ __forceinline__ void warp_arrive(uint32_t bar) {
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
+}
 __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
     uint32_t ok;
     asm volatile(
-        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n selp.u32 %0, 1, 0, p;\n}\n"
         : "=r"(ok)
-        : "r"(bar), "r"(parity)
+        : "r"(bar), "r"(parity), "r"(20000u)
         : "memory");
     return ok != 0;
 }
@@ -94,21 +101,28 @@ __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::
  * version 1 (46-47), layout 2 (61-63). The stride of 1 KB goes from one group
  * of eight rows to the next. K-major (a row is an index of M or N): the leading
  * offset is not used. MN-major (a row is an index of K, its 64 elements are
- * indexes of M or N): it goes to the next 64 of them. */
-__device__ __forceinline__ uint64_t desc(uint32_t addr, uint32_t lead) {
-    return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(lead >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
-           ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
-}
+ * indexes of M or N): it goes to the next 64 of them. The high word is the
+ * same for all; a later start only adds to the low word. */
+constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc(uint32_t addr, uint32_t lead) { return (addr >> 4) | ((lead >> 4) << 16); }
 /* kind::f16: D FP32, A and B BF16, A and B K-major or MN-major */
 __host__ __device__ constexpr uint32_t instr_desc(uint32_t m, uint32_t n, bool a_mn, bool b_mn) {
     return (1u << 4) | (1u << 7) | (1u << 10) | ((a_mn ? 1u : 0u) << 15) | ((b_mn ? 1u : 0u) << 16) | ((n >> 3) << 17) |
            ((m >> 4) << 24);
 }
-__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+/* D (+)= A B; a and b are low words of descriptors */
+__device__ __forceinline__ void mma(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool accumulate) {
     asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+        "{\n .reg .pred p;\n .reg .b64 da, db;\n setp.ne.b32 p, %4, 0;\n mov.b64 da, {%1, %5};\n mov.b64 db, {%2, %5};\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n}\n" ::"r"(d),
+        "r"(a), "r"(b), "r"(idesc), "r"((uint32_t)accumulate), "r"(kDescHigh)
         : "memory");
+}
+/* one lane of a converged warp */
+__device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(r));
+    return r != 0;
 }
 __device__ __forceinline__ void commit(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
@@ -141,23 +155,25 @@ __device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
 }
-/* Eight values as three BF16 terms (each residual is exact; an infinity's or a
- * NaN's second term is NaN, as the value would make every sum it enters):
- * row `row` of an MN-major operand, pieces term * kVB / 8 + half. */
+/* Eight values as three BF16 terms, eight significant bits each from the top:
+ * with the 24 bits of FP32 their sum is the value itself (an infinity or a
+ * NaN makes NaN terms, as it would make every sum it enters). Row `row` of an
+ * MN-major operand, pieces term * kVB / 8 + half. */
 __device__ __forceinline__ void put_terms(uint8_t *base, uint32_t row, uint32_t half, const float (&x)[8]) {
-    float r[8];
+    uint32_t r[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) r[i] = x[i];
+    for (int i = 0; i < 8; ++i) r[i] = __float_as_uint(x[i]);
 #pragma unroll
     for (int term = 0; term < 3; ++term) {
         uint32_t w[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            w[i] = bf16_pair(r[2 * i], r[2 * i + 1]);
-            r[2 * i] -= __uint_as_float(w[i] << 16);
-            r[2 * i + 1] -= __uint_as_float(w[i] & 0xFFFF0000u);
-        }
+        for (int i = 0; i < 4; ++i) w[i] = __byte_perm(r[2 * i], r[2 * i + 1], 0x7632);
         *reinterpret_cast<uint4 *>(base + piece_at(row, term * (kVB / 8) + half)) = make_uint4(w[0], w[1], w[2], w[3]);
+        if (term < 2) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                r[i] = __float_as_uint(__uint_as_float(r[i]) - __uint_as_float(r[i] & 0xFFFF0000u));
+        }
     }
 }
 
@@ -339,12 +355,13 @@ __global__ void __launch_bounds__(kPrepThreads) chunk_prep_kernel(const __grid_c
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *slot;
-    if (tid == 0) {
+    if (warp == 0 && elect_one()) {
         /* [K; Q] K^T */
+        const uint32_t at = desc(base + L::kTile, 16);
 #pragma unroll
         for (int kk = 0; kk < K / 16; ++kk) {
-            const uint32_t at = base + L::kTile + (kk / 4) * kTermBytes + (kk % 4) * 32;
-            mma(tmem, desc(at, 16), desc(at, 16), instr_desc(2 * kC, kC, false, false), kk != 0);
+            const uint32_t off = ((kk / 4) * kTermBytes + (kk % 4) * 32) >> 4;
+            mma(tmem, at + off, at + off, instr_desc(2 * kC, kC, false, false), kk != 0);
         }
         commit(bar);
     }
@@ -522,17 +539,17 @@ __global__ void __launch_bounds__(kScanThreads, 1) chunk_scan_kernel(const __gri
     volatile uint32_t *abort = reinterpret_cast<volatile uint32_t *>(sm + L::kBar + 136);
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
-            mbar_init(full_kq + 8 * i, kLoadThreads);
+            mbar_init(full_kq + 8 * i, kLoadThreads / 32);
             mbar_init(empty_k + 8 * i, 1);
             mbar_init(empty_q + 8 * i, 1);
         }
         mbar_init(full_pair, 1);
         mbar_init(empty_pair, 1);
-        mbar_init(s_ready, 256);
+        mbar_init(s_ready, 8);
         mbar_init(d1_full, 1);
-        mbar_init(r_ready, 128);
+        mbar_init(r_ready, 4);
         mbar_init(d3_full, 1);
-        mbar_init(d_ready, 128);
+        mbar_init(d_ready, 4);
         mbar_init(d4_full, 1);
         mbar_init(drain, 1);
         *abort = 0;
@@ -559,13 +576,13 @@ __global__ void __launch_bounds__(kScanThreads, 1) chunk_scan_kernel(const __gri
         for (uint32_t c = 0; c < chunks; ++c) {
             const uint32_t st = c & 1, tile = base + L::kKQ + st * L::kStage;
             const uint32_t tc = t0 + c * kC, rows = min((uint32_t)kC, t1 - tc);
-            if (c >= 2 && !wait_bar(empty_q + 8 * st, ((c >> 1) - 1) & 1u, abort)) break;
+            if (c >= 2 && !wait_bar_warp(empty_q + 8 * st, ((c >> 1) - 1) & 1u, abort)) break;
             load_rows<K>(tile, kC, q, tc, p.q_token, rows, th, kLoadThreads);
-            if (c >= 2 && !wait_bar(empty_k + 8 * st, ((c >> 1) - 1) & 1u, abort)) break;
+            if (c >= 2 && !wait_bar_warp(empty_k + 8 * st, ((c >> 1) - 1) & 1u, abort)) break;
             load_rows<K>(tile, 0, k, tc, p.k_token, rows, th, kLoadThreads);
             cp_async_wait_all();
             fence_async();
-            mbar_arrive(full_kq + 8 * st);
+            warp_arrive(full_kq + 8 * st);
         }
         cp_async_wait_all();
     } else if (warp == 9) {
@@ -588,44 +605,57 @@ __global__ void __launch_bounds__(kScanThreads, 1) chunk_scan_kernel(const __gri
             }
         }
     } else if (warp == 8) {
-        if (lane == 0) {
-            for (uint32_t c = 0; c < chunks; ++c) {
-                const uint32_t st = c & 1, ph = c & 1, tile = base + L::kKQ + st * L::kStage;
-                if (!wait_bar(full_kq + 8 * st, (c >> 1) & 1u, abort) || !wait_bar(s_ready, ph, abort)) break;
-                tc_fence_after();
+        /* the whole warp walks along, so that what the MMAs take stays in
+         * uniform registers; one lane issues */
+        const uint32_t leader = elect_one();
+        const uint32_t s_desc = desc(base + L::kS, 1024), r_desc = desc(base + L::kR, 1024), x_desc = desc(base + L::kD, 1024),
+                       pair_desc = desc(base + L::kPair, 16);
+        for (uint32_t c = 0; c < chunks; ++c) {
+            const uint32_t st = c & 1, ph = c & 1, tile = base + L::kKQ + st * L::kStage;
+            if (!wait_bar_warp(full_kq + 8 * st, (c >> 1) & 1u, abort) || !wait_bar_warp(s_ready, ph, abort)) break;
+            tc_fence_after();
+            if (leader) {
                 /* [K; Q] S0^T */
+                const uint32_t a = desc(tile, 16);
 #pragma unroll
                 for (int kk = 0; kk < K / 16; ++kk)
-                    mma(d1, desc(tile + (kk / 4) * kTermBytes + (kk % 4) * 32, 16), desc(base + L::kS + kk * 2048, 1024),
+                    mma(d1, a + (((kk / 4) * kTermBytes + (kk % 4) * 32) >> 4), s_desc + ((kk * 2048) >> 4),
                         instr_desc(128, 3 * kVB, false, true), kk != 0);
                 commit(d1_full);
                 commit(empty_q + 8 * st);
-                if (!wait_bar(full_pair, ph, abort) || !wait_bar(r_ready, ph, abort)) break;
-                tc_fence_after();
+            }
+            if (!wait_bar_warp(full_pair, ph, abort) || !wait_bar_warp(r_ready, ph, abort)) break;
+            tc_fence_after();
+            if (leader) {
                 /* [T; P T] R: the first term with all of R, the second with R's first two */
 #pragma unroll
                 for (int kk = 0; kk < kC / 16; ++kk)
-                    mma(d3, desc(base + L::kPair + kk * 32, 16), desc(base + L::kR + kk * 2048, 1024),
-                        instr_desc(128, 3 * kVB, false, true), kk != 0);
+                    mma(d3, pair_desc + ((kk * 32) >> 4), r_desc + ((kk * 2048) >> 4), instr_desc(128, 3 * kVB, false, true),
+                        kk != 0);
 #pragma unroll
                 for (int kk = 0; kk < kC / 16; ++kk)
-                    mma(d3, desc(base + L::kPair + kTermBytes + kk * 32, 16), desc(base + L::kR + kk * 2048, 1024),
+                    mma(d3, pair_desc + ((kTermBytes + kk * 32) >> 4), r_desc + ((kk * 2048) >> 4),
                         instr_desc(128, 2 * kVB, false, true), true);
                 commit(d3_full);
                 commit(empty_pair);
-                if (!wait_bar(d_ready, ph, abort)) break;
-                tc_fence_after();
+            }
+            if (!wait_bar_warp(d_ready, ph, abort)) break;
+            tc_fence_after();
+            if (leader) {
                 /* K^T D (64 key rows: the upper half of M runs into the q rows and is not read) */
+                const uint32_t a = desc(tile, K >= 128 ? kTermBytes : kTermBytes / 2);
 #pragma unroll
                 for (int t = 0; t < kTiles; ++t)
 #pragma unroll
                     for (int kk = 0; kk < kC / 16; ++kk)
-                        mma(d4 + 64 * t, desc(tile + t * 2 * kTermBytes + kk * 2048, K >= 128 ? kTermBytes : kTermBytes / 2),
-                            desc(base + L::kD + kk * 2048, 1024), instr_desc(128, 3 * kVB, true, true), kk != 0);
+                        mma(d4 + 64 * t, a + ((t * 2 * kTermBytes + kk * 2048) >> 4), x_desc + ((kk * 2048) >> 4),
+                            instr_desc(128, 3 * kVB, true, true), kk != 0);
                 commit(d4_full);
                 commit(empty_k + 8 * st);
             }
-            /* every MMA issued is done before TMEM is released */
+        }
+        /* every MMA issued is done before TMEM is released */
+        if (leader) {
             commit(drain);
             const uint64_t w0 = gtimer();
             while (!mbar_try(drain, 0) && gtimer() - w0 < kWaitNs) {
@@ -646,6 +676,21 @@ __global__ void __launch_bounds__(kScanThreads, 1) chunk_scan_kernel(const __gri
 #pragma unroll
             for (int e = 0; e < 8; ++e)
                 s[t][e] = (has_s && !fresh) ? S[(int64_t)(8 * half + e) * K + 128 * t + ln] : 0.0f;
+        struct {
+            float f0, f1, f2, decay;
+            uint4 v;
+        } next;
+        auto fetch = [&](uint32_t c) {
+            const float *sc = reinterpret_cast<const float *>(records + ((size_t)(rec0 + c) * p.HV + h) * kRecordBytes + kPairBytes);
+            const uint32_t t = t0 + c * kC + i;
+            next.decay = sc[kScalDecay * kC];
+            next.f0 = sc[(is_o ? kScalQ : kScalC) * kC + i];
+            next.f1 = sc[kScalBeta * kC + i];
+            next.f2 = sc[kScalEnd * kC + i];
+            next.v = make_uint4(0, 0, 0, 0);
+            if (!is_o && t < t1) next.v = *reinterpret_cast<const uint4 *>(v + (int64_t)t * p.v_token);
+        };
+        fetch(0);
         bool ok = true;
         for (uint32_t c = 0; c < chunks; ++c) {
             const uint32_t ph = c & 1, tc = t0 + c * kC, rows = min((uint32_t)kC, t1 - tc);
@@ -655,20 +700,11 @@ __global__ void __launch_bounds__(kScanThreads, 1) chunk_scan_kernel(const __gri
             }
             fence_async();
             tc_fence_before();
-            mbar_arrive(s_ready);
-            /* this token's scalars and values, while the MMAs run */
-            const float *sc = reinterpret_cast<const float *>(records + ((size_t)(rec0 + c) * p.HV + h) * kRecordBytes + kPairBytes);
-            const float decay = sc[kScalDecay * kC];
-            float f0, f1 = 0.0f, f2 = 0.0f;
-            uint4 vw = make_uint4(0, 0, 0, 0);
-            if (is_o) {
-                f0 = sc[kScalQ * kC + i];
-            } else {
-                f0 = sc[kScalC * kC + i];
-                f1 = sc[kScalBeta * kC + i];
-                f2 = sc[kScalEnd * kC + i];
-                if (i < rows) vw = *reinterpret_cast<const uint4 *>(v + (int64_t)(tc + i) * p.v_token);
-            }
+            warp_arrive(s_ready);
+            /* this chunk's scalars and values were requested a chunk ago; now the next one's */
+            const float f0 = next.f0, f1 = next.f1, f2 = next.f2, decay = next.decay;
+            const uint4 vw = next.v;
+            if (c + 1 < chunks) fetch(c + 1);
             float x[8], o[8];
             if (!(ok = wait_bar_warp(d1_full, ph, abort))) break;
             tc_fence_after();
@@ -686,7 +722,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) chunk_scan_kernel(const __gri
                 put_terms(sm + L::kR, i, half, x);
                 fence_async();
                 tc_fence_before();
-                mbar_arrive(r_ready);
+                warp_arrive(r_ready);
             }
             if (!(ok = wait_bar_warp(d3_full, ph, abort))) break;
             tc_fence_after();
@@ -710,7 +746,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) chunk_scan_kernel(const __gri
                 put_terms(sm + L::kD, i, half, x);
                 fence_async();
                 tc_fence_before();
-                mbar_arrive(d_ready);
+                warp_arrive(d_ready);
             }
             if (!(ok = wait_bar_warp(d4_full, ph, abort))) break;
             tc_fence_after();

@@ -105,8 +105,8 @@ int gdn_b200_delta_step(const GdnB200DeltaArgs *args) {
     return e == cudaSuccess ? 0 : failf("gdn_b200_delta_step: launch failed: %s", cudaGetErrorString(e));
 }
 
-size_t gdn_b200_delta_chunk_workspace(const GdnB200DeltaArgs *args) {
-    return args == nullptr ? 0 : gdn::ops::delta_chunk_workspace(args->tokens, args->sequences, args->v_heads);
+size_t gdn_b200_delta_chunk_workspace(uint32_t tokens, uint32_t sequences, uint32_t v_heads) {
+    return gdn::ops::delta_chunk_workspace(tokens, sequences, v_heads);
 }
 
 int gdn_b200_delta_chunk_status(int device) {

@@ -20,9 +20,15 @@ from . import check, lib
 __all__ = ["delta_step", "delta_chunk", "constrain_logits"]
 
 _DTYPE = {torch.float32: 0, torch.bfloat16: 1}
+_F32, _I32 = torch.float32, torch.int32
 _DELTA = struct.Struct("@13Q13q7I3ifI")     # GdnB200DeltaArgs
 _LOGITS = struct.Struct("@13Q6q4I2i")       # GdnB200LogitsArgs
 _entries = {}
+try:
+    _stream = torch._C._cuda_getCurrentRawStream  # the address alone: a tenth of the time of a stream object
+except AttributeError:
+    def _stream(device: int) -> int:
+        return torch.cuda.current_stream(device).cuda_stream
 
 
 def _entry(name: str):
@@ -32,74 +38,86 @@ def _entry(name: str):
     return fn
 
 
-def _need(ok: bool, what: str) -> None:
-    if not ok:
-        raise ValueError(what)
-
-
-def _pointer(t: Optional[torch.Tensor], what: str, dtype, shape: tuple, device) -> int:
-    """Address of an optional tensor of this type and shape whose last dimension is contiguous."""
-    if t is None:
-        return 0
-    _need(t.dtype in dtype if isinstance(dtype, tuple) else t.dtype == dtype, f"{what}: type {t.dtype}")
-    _need(t.shape == shape, f"{what}: shape {tuple(t.shape)}, expected {shape}")
-    _need(t.device == device, f"{what}: on {t.device}, expected {device}")
-    _need(t.stride(-1) == 1 or shape[-1] == 1, f"{what}: the last dimension is not contiguous")
-    return t.data_ptr()
-
-
-def _disjoint(t: torch.Tensor, what: str) -> None:
+def _disjoint(shape, strides) -> bool:
     """Outputs may have any order of dimensions, but no two elements in one place."""
     reach = 1
-    for stride, size in sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz > 1):
-        _need(stride >= reach, f"{what}: elements overlap (strides {t.stride()})")
+    for stride, size in sorted((st, sz) for st, sz in zip(strides, shape) if sz > 1):
+        if stride < reach:
+            return False
         reach = stride * size
+    return True
+
+
+def _no_gradient(name: str, *tensors) -> None:
+    for t in tensors:
+        if t.requires_grad:
+            raise RuntimeError(f"{name}: no gradient is computed (call it under torch.no_grad())")
+
+
+def _refuse(name: str, device: int, wanted) -> None:
+    """Says which argument is not as (argument, tensor, types, shape) of `wanted` ask; the calls test them all at once."""
+    for what, t, types, shape in wanted:
+        if t is None:
+            continue
+        if t.dtype not in types:
+            raise ValueError(f"{name}: {what} has type {t.dtype}")
+        if t.get_device() != device or device < 0:
+            raise ValueError(f"{name}: {what} is on {t.device}, all on one CUDA device expected")
+        if shape is not None and tuple(t.shape) != tuple(shape):
+            raise ValueError(f"{name}: {what} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+        if t.dim() == 1 and not t.is_contiguous() or t.dim() > 1 and t.stride(-1) != 1 and what not in ("g", "beta"):
+            raise ValueError(f"{name}: the last dimension of {what} is not contiguous")
+    raise ValueError(f"{name}: elements of out overlap, or a slot of state is not one block [v_heads, value_dim, key_dim]")
 
 
 def _delta(name, q, k, v, g, beta, state, starts, slots, fresh, scale, normalize, out):
-    _need(q.dim() == 3 and v.dim() == 3 and state.dim() == 4, f"{name}: q, k, v [tokens, heads, dim], state "
-          f"[slots, v_heads, value_dim, key_dim] expected")
-    device, dtype = q.device, q.dtype
-    _need(device.type == "cuda", f"{name}: CUDA tensors expected")
-    _need(dtype in _DTYPE, f"{name}: {dtype} is neither float32 nor bfloat16")
-    tokens, heads, key_dim = q.shape
-    v_heads, value_dim = v.shape[1:]
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or g.requires_grad
-                                    or beta.requires_grad or state.requires_grad):
-        raise RuntimeError(f"{name}: no gradient is computed (call it under torch.no_grad())")
-    pq = _pointer(q, "q", dtype, q.shape, device)
-    pk = _pointer(k, "k", dtype, q.shape, device)
-    pv = _pointer(v, "v", dtype, (tokens, v_heads, value_dim), device)
-    _need(g.shape == (tokens, v_heads) and beta.shape == (tokens, v_heads), f"{name}: g and beta [tokens, v_heads] expected")
-    _need(g.dtype == torch.float32 and beta.dtype == torch.float32, f"{name}: g and beta are float32")
-    _need(g.device == device and beta.device == device, f"{name}: g or beta is on another device")
+    """Checks the tensors; returns (out, pack), pack(workspace, bytes) being the C entry's arguments."""
+    if q.dim() != 3 or v.dim() != 3 or state.dim() != 4 or k.dim() != 3:
+        raise ValueError(f"{name}: q, k, v [tokens, heads, dim], state [slots, v_heads, value_dim, key_dim] expected")
+    if torch.is_grad_enabled():
+        _no_gradient(name, q, k, v, g, beta, state)
+    dtype, device = q.dtype, q.get_device()
+    code = _DTYPE.get(dtype, -1)
+    q_shape, v_shape = q.shape, v.shape
+    tokens, heads, key_dim = q_shape
+    _, v_heads, value_dim = v_shape
     n_slots = state.shape[0]
-    ps = _pointer(state, "state", torch.float32, (n_slots, v_heads, value_dim, key_dim), device)
-    state_strides = state.stride()
-    _need(state_strides[2] == key_dim and (state_strides[1] == value_dim * key_dim or v_heads == 1),
-          "state: a slot is not one block [v_heads, value_dim, key_dim]")
-    if starts is not None:
-        _need(starts.dim() == 1 and starts.numel() >= 1, "starts: [sequences + 1] expected")
-        sequences = starts.numel() - 1
-    else:
-        sequences = tokens
-    pst = _pointer(starts, "starts", torch.int32, (sequences + 1,), device)
-    psl = _pointer(slots, "slots", torch.int32, (sequences,), device)
-    pf = _pointer(fresh, "fresh", (torch.bool, torch.uint8), (sequences,), device)
+    sequences = tokens if starts is None else starts.shape[0] - 1 if starts.dim() == 1 else -1
     if out is None:
-        out = torch.empty((tokens, v_heads, value_dim), dtype=dtype, device=device)
+        out = torch.empty_like(v) if v.is_contiguous() else torch.empty(v_shape, dtype=dtype, device=v.device)
+        out_ok = True
     else:
-        _disjoint(out, "out")
-    po = _pointer(out, "out", dtype, (tokens, v_heads, value_dim), device)
-    (qt, qh, _), (kt, kh, _), (vt, vh, _) = q.stride(), k.stride(), v.stride()
-    (gt, gh), (bt, bh), (ot, oh, _) = g.stride(), beta.stride(), out.stride()
-    stream = torch.cuda.current_stream(device).cuda_stream
+        out_ok = (out.dtype is dtype and out.get_device() == device and out.shape == v_shape
+                  and _disjoint(v_shape, out.stride()))
+    gates = (tokens, v_heads)
+    if not (out_ok and code >= 0 and device >= 0 and k.dtype is dtype and v.dtype is dtype and k.shape == q_shape
+            and v_shape[0] == tokens and g.dtype is _F32 and beta.dtype is _F32 and g.shape == gates
+            and beta.shape == gates and state.dtype is _F32 and state.shape == (n_slots, v_heads, value_dim, key_dim)
+            and k.get_device() == device and v.get_device() == device and g.get_device() == device
+            and beta.get_device() == device and state.get_device() == device and sequences >= 0
+            and (starts is None or starts.dtype is _I32 and starts.get_device() == device and starts.is_contiguous())
+            and (slots is None or slots.dtype is _I32 and slots.shape == (sequences,) and slots.get_device() == device
+                 and slots.is_contiguous())
+            and (fresh is None or fresh.element_size() == 1 and fresh.dtype in (torch.bool, torch.uint8)
+                 and fresh.shape == (sequences,) and fresh.get_device() == device and fresh.is_contiguous())):
+        _refuse(name, device, (("q", q, _DTYPE, None), ("k", k, (dtype,), q_shape), ("v", v, (dtype,), (tokens, *v_shape[1:])),
+                               ("g", g, (_F32,), gates), ("beta", beta, (_F32,), gates),
+                               ("state", state, (_F32,), (n_slots, v_heads, value_dim, key_dim)),
+                               ("starts", starts, (_I32,), None if sequences >= 0 else ("sequences + 1",)),
+                               ("slots", slots, (_I32,), (sequences,)),
+                               ("fresh", fresh, (torch.bool, torch.uint8), (sequences,)), ("out", out, (dtype,), v_shape)))
+    (qt, qh, q1), (kt, kh, k1), (vt, vh, v1), (ot, oh, o1) = q.stride(), k.stride(), v.stride(), out.stride()
+    (gt, gh), (bt, bh), (ss, sh, sv, sk) = g.stride(), beta.stride(), state.stride()
+    if not (q1 == k1 == v1 == o1 == sk == 1 and sv == key_dim and (sh == value_dim * key_dim or v_heads == 1)):
+        _refuse(name, device, (("q", q, _DTYPE, None), ("k", k, _DTYPE, None), ("v", v, _DTYPE, None),
+                               ("out", out, _DTYPE, None), ("state", state, (_F32,), None)))
 
     def pack(workspace, workspace_bytes):
-        return _DELTA.pack(pq, pk, pv, g.data_ptr(), beta.data_ptr(), ps, po, pst, psl, pf, workspace, workspace_bytes,
-                           stream, qt, qh, kt, kh, vt, vh, gt, gh, bt, bh, ot, oh, state_strides[0], sequences, tokens,
-                           heads, v_heads, key_dim, value_dim, n_slots, _DTYPE[dtype], 1 if normalize else 0,
-                           device.index, key_dim ** -0.5 if scale is None else scale, 0)
+        return _DELTA.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(), state.data_ptr(),
+                           out.data_ptr(), 0 if starts is None else starts.data_ptr(), 0 if slots is None else slots.data_ptr(),
+                           0 if fresh is None else fresh.data_ptr(), workspace, workspace_bytes, _stream(device), qt, qh, kt,
+                           kh, vt, vh, gt, gh, bt, bh, ot, oh, ss, sequences, tokens, heads, v_heads, key_dim, value_dim,
+                           n_slots, code, 1 if normalize else 0, device, key_dim ** -0.5 if scale is None else scale, 0)
 
     return out, pack
 
@@ -118,7 +136,9 @@ def delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tenso
     scale defaults to key_dim ** -0.5; normalize divides q and k by their L2
     norms. Returns the outputs [tokens, v_heads, value_dim]."""
     out, pack = _delta("delta_step", q, k, v, g, beta, state, starts, slots, fresh, scale, normalize, out)
-    check(_entry("gdn_b200_delta_step")(pack(0, 0)), "gdn_b200_delta_step")
+    rc = _entry("gdn_b200_delta_step")(pack(0, 0))
+    if rc:
+        check(rc, "gdn_b200_delta_step")
     return out
 
 
@@ -130,9 +150,11 @@ def delta_chunk(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tens
     prompts, 64 tokens at a time on the tensor cores. q, k, v bfloat16 with
     16-byte aligned rows."""
     out, pack = _delta("delta_chunk", q, k, v, g, beta, state, starts, slots, fresh, scale, normalize, out)
-    size = _entry("gdn_b200_delta_chunk_workspace")(pack(0, 0))
+    size = _entry("gdn_b200_delta_chunk_workspace")(v.shape[0], v.shape[0] if starts is None else starts.shape[0] - 1, v.shape[1])
     workspace = torch.empty(size, dtype=torch.uint8, device=q.device)
-    check(_entry("gdn_b200_delta_chunk")(pack(workspace.data_ptr(), size)), "gdn_b200_delta_chunk")
+    rc = _entry("gdn_b200_delta_chunk")(pack(workspace.data_ptr(), size))
+    if rc:
+        check(rc, "gdn_b200_delta_chunk")
     return out
 
 
@@ -150,41 +172,55 @@ def constrain_logits(logits: torch.Tensor, *, tokens: Optional[torch.Tensor] = N
     (id -1: not used); mask int32 [rows, ceil(vocab / 32)], bit v % 32 of word
     v // 32 set where token v is allowed. Returns (out, picks int32 [rows]);
     out may be the logits themselves, and a pick is -1 where nothing is left."""
-    _need(logits.dim() == 2, "constrain_logits: logits [rows, vocab] expected")
-    device, dtype = logits.device, logits.dtype
-    _need(device.type == "cuda", "constrain_logits: CUDA tensors expected")
-    _need(dtype in _DTYPE, f"constrain_logits: {dtype} is neither float32 nor bfloat16")
-    if logits.requires_grad and torch.is_grad_enabled():
-        raise RuntimeError("constrain_logits: no gradient is computed (call it under torch.no_grad())")
-    rows, vocab = logits.shape
-    pl = _pointer(logits, "logits", dtype, logits.shape, device)
+    name = "constrain_logits"
+    if logits.dim() != 2:
+        raise ValueError(f"{name}: logits [rows, vocab] expected")
+    if torch.is_grad_enabled():
+        _no_gradient(name, logits)
+    dtype, device, shape = logits.dtype, logits.get_device(), logits.shape
+    code = _DTYPE.get(dtype, -1)
+    rows, vocab = shape
     if out is None:
-        out = torch.empty((rows, vocab), dtype=dtype, device=device)
-    elif out is not logits:
-        _disjoint(out, "out")
-    po = _pointer(out, "out", dtype, logits.shape, device)
+        out = torch.empty_like(logits) if logits.is_contiguous() else torch.empty(shape, dtype=dtype, device=logits.device)
     history = biases = 0
     if tokens is not None:
-        _need(tokens.dim() == 2, "tokens: [rows, history] expected")
-        history = tokens.shape[1]
-    else:
-        _need(lens is None and prompt_lens is None and repetition is None and presence is None and frequency is None,
-              "constrain_logits: lens, prompt_lens and penalties need tokens")
-    _need((bias is None) == (bias_ids is None), "constrain_logits: bias and bias_ids go together")
+        history = tokens.shape[1] if tokens.dim() == 2 else -1
+    elif not (lens is None and prompt_lens is None and repetition is None and presence is None and frequency is None):
+        raise ValueError(f"{name}: lens, prompt_lens and penalties need tokens")
+    if (bias is None) != (bias_ids is None):
+        raise ValueError(f"{name}: bias and bias_ids go together")
     if bias is not None:
-        _need(bias.dim() == 2, "bias: [rows, entries] expected")
-        biases = bias.shape[1]
-    i32, f32, each = torch.int32, torch.float32, (rows,)
-    pt = _pointer(tokens, "tokens", i32, (rows, history), device)
-    pln, pp = _pointer(lens, "lens", i32, each, device), _pointer(prompt_lens, "prompt_lens", i32, each, device)
-    pr = _pointer(repetition, "repetition", f32, each, device)
-    ppr, pfr = _pointer(presence, "presence", f32, each, device), _pointer(frequency, "frequency", f32, each, device)
-    pbi, pb = _pointer(bias_ids, "bias_ids", i32, (rows, biases), device), _pointer(bias, "bias", f32, (rows, biases), device)
-    pm = _pointer(mask, "mask", i32, (rows, (vocab + 31) // 32), device)
-    picks = torch.empty(rows, dtype=i32, device=device)
-    check(_entry("gdn_b200_constrain_logits")(_LOGITS.pack(
-        pl, po, picks.data_ptr(), pt, pln, pp, pr, ppr, pfr, pbi, pb, pm, torch.cuda.current_stream(device).cuda_stream,
-        logits.stride(0), out.stride(0), tokens.stride(0) if tokens is not None else 0,
-        bias_ids.stride(0) if biases else 0, bias.stride(0) if biases else 0, mask.stride(0) if mask is not None else 0,
-        rows, vocab, history, biases, _DTYPE[dtype], device.index)), "gdn_b200_constrain_logits")
+        biases = bias.shape[1] if bias.dim() == 2 else -1
+    each = (rows,)
+
+    def ok1(t, of):
+        return t is None or t.dtype is of and t.shape == each and t.get_device() == device and t.is_contiguous()
+
+    def ok2(t, of, width):
+        return t is None or (t.dtype is of and t.shape == (rows, width) and t.get_device() == device
+                             and (t.stride(1) == 1 or width <= 1))
+
+    if not (code >= 0 and device >= 0 and ok2(logits, dtype, vocab) and (out is logits or ok2(out, dtype, vocab)
+            and _disjoint(shape, out.stride())) and ok2(tokens, _I32, history) and ok1(lens, _I32) and ok1(prompt_lens, _I32)
+            and ok1(repetition, _F32) and ok1(presence, _F32) and ok1(frequency, _F32) and ok2(bias_ids, _I32, biases)
+            and ok2(bias, _F32, biases) and ok2(mask, _I32, (vocab + 31) // 32)):
+        wide = lambda n: ("rows", "width") if n < 0 else (rows, n)  # noqa: E731
+        _refuse(name, device, (("logits", logits, _DTYPE, None), ("out", out, (dtype,), shape),
+                               ("tokens", tokens, (_I32,), wide(history)), ("lens", lens, (_I32,), each),
+                               ("prompt_lens", prompt_lens, (_I32,), each), ("repetition", repetition, (_F32,), each),
+                               ("presence", presence, (_F32,), each), ("frequency", frequency, (_F32,), each),
+                               ("bias_ids", bias_ids, (_I32,), wide(biases)), ("bias", bias, (_F32,), wide(biases)),
+                               ("mask", mask, (_I32,), (rows, (vocab + 31) // 32))))
+
+    def at(t):
+        return 0 if t is None else t.data_ptr()
+
+    picks = torch.empty(rows, dtype=_I32, device=logits.device)
+    rc = _entry("gdn_b200_constrain_logits")(_LOGITS.pack(
+        logits.data_ptr(), out.data_ptr(), picks.data_ptr(), at(tokens), at(lens), at(prompt_lens), at(repetition),
+        at(presence), at(frequency), at(bias_ids), at(bias), at(mask), _stream(device), logits.stride(0), out.stride(0),
+        tokens.stride(0) if history else 0, bias_ids.stride(0) if biases else 0, bias.stride(0) if biases else 0,
+        0 if mask is None else mask.stride(0), rows, vocab, history, biases, code, device))
+    if rc:
+        check(rc, "gdn_b200_constrain_logits")
     return out, picks

@@ -327,8 +327,8 @@ int gdn_b200_delta_step(const GdnB200DeltaArgs *args);
 /* Prompts: any lengths, BF16 only. 16-byte aligned q, k and v rows. */
 int gdn_b200_delta_chunk(const GdnB200DeltaArgs *args);
 /* Bytes of 256-byte aligned device memory that gdn_b200_delta_chunk needs as
- * args->workspace for these sizes (its other fields are not read). */
-size_t gdn_b200_delta_chunk_workspace(const GdnB200DeltaArgs *args);
+ * args->workspace for these sizes. */
+size_t gdn_b200_delta_chunk_workspace(uint32_t tokens, uint32_t sequences, uint32_t v_heads);
 /* 0, or -1 if a wait inside gdn_b200_delta_chunk ran out (2 s) on `device`
  * since the last call of this function: the states of that call are then NaN.
  * Waits for the device; for a server's health checks and for tests. */
