@@ -174,7 +174,7 @@ EXPORTS = [
     ("gdn_b200_delta_step", ctypes.c_int, [ctypes.c_char_p]),
     ("gdn_b200_delta_chunk", ctypes.c_int, [ctypes.c_char_p]),
     ("gdn_b200_delta_chunk_workspace", ctypes.c_size_t, [ctypes.c_uint32, ctypes.c_uint32, ctypes.c_uint32]),
-    ("gdn_b200_delta_chunk_status", ctypes.c_int, [ctypes.c_int]),
+    ("gdn_b200_delta_status", ctypes.c_int, [ctypes.c_int]),
     ("gdn_b200_constrain_logits", ctypes.c_int, [ctypes.c_char_p]),
 ]
 

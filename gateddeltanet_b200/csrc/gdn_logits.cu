@@ -13,9 +13,14 @@
  * slices of one cluster's CTAs. Each CTA reads the row's history and keeps
  * what falls into its slice in a shared-memory table, one word per token:
  *   bits 0-19 n | bits 20-30 first bias entry + 1 | bit 31 in the prompt
- * (integer atomics: the order does not show), then passes over its logits
- * with 16-byte loads; nearly all words are 0 and cost one compare. The picks
- * of the slices meet in CTA 0 through distributed shared memory.
+ * (integer atomics: the order does not show), and one bit per token that says
+ * whether the word is set. Tokens without one (nearly all) only meet the mask:
+ * a dense pass copies them 16 bytes at a time and keeps the largest. The few
+ * others are then recomputed from the history and bias lists themselves: who
+ * takes a token's word out of the table (an exchange with 0) does the token,
+ * so that all lanes of a warp have one to do, where a test in the dense pass
+ * left a warp waiting for one lane at nearly every vector. The picks of the
+ * slices meet in CTA 0 through distributed shared memory.
  */
 #include "gdn_ops.h"
 
@@ -30,7 +35,8 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int kLogitsThreads = 512;
-constexpr int kUnroll = 2;      /* 16-byte vectors of a thread in flight */
+constexpr int kUnroll = 4;      /* 16-byte vectors of a thread in flight */
+constexpr int kHistoryUnroll = 4;
 constexpr int kMaxCluster = 8;  /* portable cluster size */
 constexpr uint32_t kCountMask = (1u << 20) - 1, kPromptBit = 1u << 31;
 constexpr uint32_t kFlagWords = (kMaxBiases + 32) / 32;
@@ -44,16 +50,47 @@ __device__ __forceinline__ unsigned long long pick_key(float x, uint32_t v) {
 }
 constexpr uint32_t kKeyNegInf = 0x007FFFFFu; /* value half of the key of -inf */
 
+/* 16 bytes of logits. only(allow): the values whose bit is set, -inf for the others. */
 template <typename T>
-struct Vec {
-    static constexpr int kN = 16 / sizeof(T);
+struct Vec;
+template <>
+struct Vec<float> {
+    static constexpr int kN = 4;
+    static __device__ __forceinline__ float value(const uint4 &w, int j) {
+        return __uint_as_float(j == 0 ? w.x : j == 1 ? w.y : j == 2 ? w.z : w.w);
+    }
+    static __device__ __forceinline__ uint4 only(const uint4 &w, uint32_t allow) {
+        return make_uint4((allow & 1u) ? w.x : 0xFF800000u, (allow & 2u) ? w.y : 0xFF800000u,
+                          (allow & 4u) ? w.z : 0xFF800000u, (allow & 8u) ? w.w : 0xFF800000u);
+    }
+    /* largest value, NaN passed over (-inf if there is nothing else) */
+    static __device__ __forceinline__ float largest(const uint4 &w) {
+        const float lo = __int_as_float(0xff800000);
+        return fmaxf(fmaxf(fmaxf(__uint_as_float(w.x), lo), __uint_as_float(w.y)),
+                     fmaxf(fmaxf(__uint_as_float(w.z), lo), __uint_as_float(w.w)));
+    }
 };
-template <typename T>
-__device__ __forceinline__ float get(const uint4 &w, int j) {
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-    if (sizeof(T) == 4) return __uint_as_float(u[j]);
-    return __uint_as_float((j & 1) ? (u[j >> 1] & 0xFFFF0000u) : (u[j >> 1] << 16));
-}
+template <>
+struct Vec<__nv_bfloat16> {
+    static constexpr int kN = 8;
+    static __device__ __forceinline__ float value(const uint4 &w, int j) {
+        const uint32_t u = j < 2 ? w.x : j < 4 ? w.y : j < 6 ? w.z : w.w;
+        return __uint_as_float((j & 1) ? (u & 0xFFFF0000u) : (u << 16));
+    }
+    static __device__ __forceinline__ uint32_t pair(uint32_t w, uint32_t allow) {
+        const uint32_t m = ((allow & 1u) | ((allow & 2u) << 15)) * 0xFFFFu;
+        return (w & m) | (0xFF80FF80u & ~m);
+    }
+    static __device__ __forceinline__ uint4 only(const uint4 &w, uint32_t allow) {
+        return make_uint4(pair(w.x, allow), pair(w.y, allow >> 2), pair(w.z, allow >> 4), pair(w.w, allow >> 6));
+    }
+    static __device__ __forceinline__ __nv_bfloat162 two(uint32_t w) { return *reinterpret_cast<__nv_bfloat162 *>(&w); }
+    static __device__ __forceinline__ float largest(const uint4 &w) {
+        const __nv_bfloat162 lo = two(0xFF80FF80u);
+        const __nv_bfloat162 m = __hmax2(__hmax2(__hmax2(two(w.x), lo), two(w.y)), __hmax2(__hmax2(two(w.z), lo), two(w.w)));
+        return fmaxf(__low2float(m), __high2float(m));
+    }
+};
 __device__ __forceinline__ float load_one(const float *p) { return *p; }
 __device__ __forceinline__ float load_one(const __nv_bfloat16 *p) { return __bfloat162float(*p); }
 __device__ __forceinline__ float rounded(float x, float) { return x; }
@@ -69,7 +106,8 @@ struct Row {
     uint32_t biases;
 };
 
-__device__ __noinline__ float touched(float x, uint32_t word, const Row &r) {
+/* x with what the table's word says */
+__device__ __forceinline__ float touched(float x, uint32_t word, const Row &r) {
     const uint32_t n = word & kCountMask, entry = (word >> 20) & kMaxBiases;
     if (n != 0 || (word & kPromptBit)) x = x > 0.0f ? __fdiv_rn(x, r.repetition) : __fmul_rn(x, r.repetition);
     if (n != 0) x = __fsub_rn(__fsub_rn(x, __fmul_rn(r.frequency, (float)n)), r.presence);
@@ -87,7 +125,7 @@ __device__ __noinline__ float touched(float x, uint32_t word, const Row &r) {
 template <typename T>
 __global__ void __launch_bounds__(kLogitsThreads) logits_kernel(const __grid_constant__ LogitsParams p) {
     constexpr int N = Vec<T>::kN;
-    extern __shared__ __align__(16) uint32_t table[];
+    extern __shared__ __align__(16) uint32_t table[]; /* words of the slice, then a bit each */
     __shared__ uint32_t multi[kFlagWords];
     __shared__ unsigned long long warp_key[kLogitsThreads / 32], slice_key[kMaxCluster];
     cg::cluster_group cluster = cg::this_cluster();
@@ -105,7 +143,23 @@ __global__ void __launch_bounds__(kLogitsThreads) logits_kernel(const __grid_con
     const int32_t first = (int32_t)(v0 * N) - (int32_t)mis; /* token of table word 0 */
     const int32_t lo = max(first, 0), hi = min((int32_t)V, (int32_t)(v1 * N) - (int32_t)mis);
     const uint32_t *mask = p.mask == nullptr ? nullptr : p.mask + (int64_t)b * p.mask_row;
-    const uint32_t words = p.slice_vecs * N;
+    const uint32_t words = (p.slice_vecs * N + 127) & ~127u;
+    uint32_t *bits = table + words;
+
+    uint4 w[kUnroll];
+    /* the vectors base, base + kLogitsThreads, ... that lie in the row whole */
+    auto whole = [&](uint32_t i) {
+        const int32_t e0 = (int32_t)(i * N) - (int32_t)mis;
+        return i < v1 && e0 >= 0 && e0 + N <= (int32_t)V;
+    };
+    auto load = [&](uint32_t base) {
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+            const uint32_t i = base + u * kLogitsThreads;
+            if (whole(i)) w[u] = __ldcs(reinterpret_cast<const uint4 *>(in + ((int32_t)(i * N) - (int32_t)mis)));
+        }
+    };
+    load(v0 + tid); /* on their way while the table is built */
 
     const bool use_table = p.tokens != nullptr || p.bias_ids != nullptr;
     Row row;
@@ -116,38 +170,44 @@ __global__ void __launch_bounds__(kLogitsThreads) logits_kernel(const __grid_con
     row.bias = p.bias + (int64_t)b * p.bias_row;
     row.multi = multi;
     row.biases = p.bias_ids == nullptr ? 0 : p.biases;
+    const int32_t *ids = p.tokens + (int64_t)b * p.tokens_row;
+    const int32_t len = p.tokens == nullptr ? 0 : p.lens == nullptr ? (int32_t)p.history : min(p.lens[b], (int32_t)p.history);
 
     if (use_table) {
-        for (uint32_t i = tid; i < words / 4; i += kLogitsThreads)
+        for (uint32_t i = tid; i < (words + words / 32) / 4; i += kLogitsThreads)
             reinterpret_cast<uint4 *>(table)[i] = make_uint4(0, 0, 0, 0);
         for (uint32_t i = tid; i < kFlagWords; i += kLogitsThreads) multi[i] = 0;
         __syncthreads();
-        if (p.tokens != nullptr) {
-            const int32_t *ids = p.tokens + (int64_t)b * p.tokens_row;
-            const int32_t len = p.lens == nullptr ? (int32_t)p.history : min(p.lens[b], (int32_t)p.history);
-            const int32_t made = p.prompt_lens == nullptr ? 0 : p.prompt_lens[b];
-            for (int32_t i = (int32_t)tid; i < len; i += kLogitsThreads) {
-                const int32_t id = ids[i];
-                if (id >= lo && id < hi) {
-                    if (i >= made)
-                        atomicAdd(&table[id - first], 1u);
-                    else
-                        atomicOr(&table[id - first], kPromptBit);
-                }
+        const int32_t made = p.prompt_lens == nullptr ? 0 : p.prompt_lens[b];
+        for (int32_t i0 = (int32_t)tid; i0 < len; i0 += kLogitsThreads * kHistoryUnroll) {
+            int32_t id[kHistoryUnroll];
+#pragma unroll
+            for (int u = 0; u < kHistoryUnroll; ++u) {
+                const int32_t i = i0 + u * kLogitsThreads;
+                id[u] = i < len ? ids[i] : -1;
+            }
+#pragma unroll
+            for (int u = 0; u < kHistoryUnroll; ++u) {
+                if (id[u] < lo || id[u] >= hi) continue;
+                const uint32_t at = (uint32_t)(id[u] - first);
+                const uint32_t old = i0 + u * kLogitsThreads >= made ? atomicAdd(&table[at], 1u) : atomicOr(&table[at], kPromptBit);
+                if (old == 0) atomicOr(&bits[at >> 5], 1u << (at & 31));
             }
         }
         /* a biased token's word names its first entry */
         for (uint32_t i = tid; i < row.biases; i += kLogitsThreads) {
             const int32_t id = row.bias_ids[i];
             if (id < lo || id >= hi) continue;
-            uint32_t *w = &table[id - first], old = *w;
+            const uint32_t at = (uint32_t)(id - first);
+            uint32_t old = table[at];
             while (true) {
                 const uint32_t e = (old >> 20) & kMaxBiases;
                 if (e != 0 && e <= i + 1) break;
-                const uint32_t seen = atomicCAS(w, old, (old & ~(kMaxBiases << 20)) | ((i + 1) << 20));
+                const uint32_t seen = atomicCAS(&table[at], old, (old & ~(kMaxBiases << 20)) | ((i + 1) << 20));
                 if (seen == old) break;
                 old = seen;
             }
+            atomicOr(&bits[at >> 5], 1u << (at & 31));
         }
         __syncthreads();
         for (uint32_t i = tid; i < row.biases; i += kLogitsThreads) {
@@ -156,33 +216,32 @@ __global__ void __launch_bounds__(kLogitsThreads) logits_kernel(const __grid_con
             const uint32_t e = (table[id - first] >> 20) & kMaxBiases;
             if (e != i + 1) atomicOr(&multi[(e - 1) >> 5], 1u << ((e - 1) & 31));
         }
-        __syncthreads();
     }
 
+    /* dense pass: the mask, and the largest of the tokens without a word.
+     * Tokens with one keep their value for now. */
     unsigned long long best = 0;
+    float top = __int_as_float(0xff800000);
+    uint32_t top_vec = 0;
+    uint4 top_w = make_uint4(0, 0, 0, 0);
     for (uint32_t base = v0 + tid; base < v1; base += kLogitsThreads * kUnroll) {
-        uint4 w[kUnroll];
-        bool whole[kUnroll];
-#pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-            const uint32_t i = base + u * kLogitsThreads;
-            const int32_t e0 = (int32_t)(i * N) - (int32_t)mis;
-            whole[u] = i < v1 && e0 >= 0 && e0 + N <= (int32_t)V;
-            if (whole[u]) w[u] = __ldcs(reinterpret_cast<const uint4 *>(in + e0));
-        }
+        if (base != v0 + tid) load(base);
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
             const uint32_t i = base + u * kLogitsThreads;
             if (i >= v1) continue;
             const int32_t e0 = (int32_t)(i * N) - (int32_t)mis;
-            if (!whole[u]) {
+            const uint32_t at = (i - v0) * N;
+            const uint32_t own = use_table ? bits[at >> 5] >> (at & 31) : 0u;
+            if (!whole(i)) {
                 /* a row's ragged first or last vector */
                 for (int32_t e = max(e0, 0); e < min(e0 + N, (int32_t)V); ++e) {
                     float x = load_one(in + e);
-                    const uint32_t word = use_table ? table[e - first] : 0u;
-                    if (word != 0) x = touched(x, word, row);
+                    if ((own >> (e - e0)) & 1u) {
+                        store_one(out + e, x);
+                        continue;
+                    }
                     if (mask != nullptr && !((mask[e >> 5] >> (e & 31)) & 1u)) x = __int_as_float(0xff800000);
-                    x = rounded(x, T());
                     store_one(out + e, x);
                     const unsigned long long key = pick_key(x, (uint32_t)e);
                     best = key > best ? key : best;
@@ -191,47 +250,55 @@ __global__ void __launch_bounds__(kLogitsThreads) logits_kernel(const __grid_con
             }
             uint32_t allow = 0xFFFFFFFFu;
             if (mask != nullptr) allow = __funnelshift_r(mask[e0 >> 5], mask[(e0 + N - 1) >> 5], e0 & 31);
-            float x[N];
-#pragma unroll
-            for (int j = 0; j < N; ++j) x[j] = get<T>(w[u], j);
-            if (use_table) {
-                const uint4 *tw = reinterpret_cast<const uint4 *>(table + (e0 - first));
-#pragma unroll
-                for (int j4 = 0; j4 < N / 4; ++j4) {
-                    const uint4 t4 = tw[j4];
-                    if (t4.x | t4.y | t4.z | t4.w) {
-                        if (t4.x) x[4 * j4] = touched(x[4 * j4], t4.x, row);
-                        if (t4.y) x[4 * j4 + 1] = touched(x[4 * j4 + 1], t4.y, row);
-                        if (t4.z) x[4 * j4 + 2] = touched(x[4 * j4 + 2], t4.z, row);
-                        if (t4.w) x[4 * j4 + 3] = touched(x[4 * j4 + 3], t4.w, row);
-                    }
-                }
-            }
-#pragma unroll
-            for (int j = 0; j < N; ++j) {
-                if (!((allow >> j) & 1u)) x[j] = __int_as_float(0xff800000);
-                x[j] = rounded(x[j], T());
-                const unsigned long long key = pick_key(x[j], (uint32_t)(e0 + j));
-                best = key > best ? key : best;
-            }
+            const uint4 o = Vec<T>::only(w[u], allow | own);
             if (wide_out) {
-                uint4 o;
-                if (sizeof(T) == 4) {
-                    o = make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]),
-                                   __float_as_uint(x[3]));
-                } else {
-                    uint32_t h[4];
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        h[j] = (__float_as_uint(x[(2 * j) % N]) >> 16) | (__float_as_uint(x[(2 * j + 1) % N]) & 0xFFFF0000u);
-                    o = make_uint4(h[0], h[1], h[2], h[3]);
-                }
                 __stcs(reinterpret_cast<uint4 *>(out + e0), o);
             } else {
 #pragma unroll
-                for (int j = 0; j < N; ++j) store_one(out + e0 + j, x[j]);
+                for (int j = 0; j < N; ++j) store_one(out + e0 + j, Vec<T>::value(o, j));
+            }
+            const uint4 free = (own & ((1u << N) - 1)) ? Vec<T>::only(w[u], allow & ~own) : o;
+            const float m = Vec<T>::largest(free);
+            if (m > top) {
+                top = m;
+                top_vec = i;
+                top_w = free;
             }
         }
+    }
+    if (top > __int_as_float(0xff800000)) {
+#pragma unroll
+        for (int j = N - 1; j >= 0; --j)
+            if (Vec<T>::value(top_w, j) == top) {
+                const unsigned long long key = pick_key(top, top_vec * N - mis + j);
+                best = key > best ? key : best;
+            }
+    }
+    if (use_table) {
+        __syncthreads();
+        auto recompute = [&](int32_t id) {
+            if (id < lo || id >= hi) return;
+            const uint32_t word = atomicExch(&table[id - first], 0u);
+            if (word == 0) return;
+            /* from out where the dense pass left it: out may be the logits */
+            float x = touched(load_one(out + id), word, row);
+            if (mask != nullptr && !((mask[id >> 5] >> (id & 31)) & 1u)) x = __int_as_float(0xff800000);
+            x = rounded(x, T());
+            store_one(out + id, x);
+            const unsigned long long key = pick_key(x, (uint32_t)id);
+            best = key > best ? key : best;
+        };
+        for (int32_t i0 = (int32_t)tid; i0 < len; i0 += kLogitsThreads * kHistoryUnroll) {
+            int32_t id[kHistoryUnroll];
+#pragma unroll
+            for (int u = 0; u < kHistoryUnroll; ++u) {
+                const int32_t i = i0 + u * kLogitsThreads;
+                id[u] = i < len ? ids[i] : -1;
+            }
+#pragma unroll
+            for (int u = 0; u < kHistoryUnroll; ++u) recompute(id[u]);
+        }
+        for (uint32_t i = tid; i < row.biases; i += kLogitsThreads) recompute(row.bias_ids[i]);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
@@ -264,7 +331,8 @@ cudaError_t launch_logits_t(LogitsParams &p, int sms, cudaStream_t stream) {
     while (C < kMaxCluster && (p.rows * C < 2u * (uint32_t)sms || nvec * N / C > 16384u)) C *= 2;
     p.slice_vecs = (nvec + C - 1) / C;
     const bool use_table = p.tokens != nullptr || p.bias_ids != nullptr;
-    const size_t smem = use_table ? (size_t)p.slice_vecs * N * 4 : 0;
+    const size_t words = (p.slice_vecs * N + 127) & ~127u;
+    const size_t smem = use_table ? (words + words / 32) * 4 : 0;
     cudaError_t e = cudaFuncSetAttribute(logits_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};

@@ -100,8 +100,9 @@ int gdn_b200_delta_step(const GdnB200DeltaArgs *args) {
     const int rc = delta_params("gdn_b200_delta_step", args, p);
     if (rc != 0) return rc > 0 ? 0 : -1;
     DeviceScope scope(args->device);
-    if (!scope.ok) return failf("gdn_b200_delta_step: cannot use device %d", args->device);
-    const cudaError_t e = gdn::ops::launch_delta_step(p, args->dtype == 1, static_cast<cudaStream_t>(args->stream));
+    const int sms = scope.ok ? sm_count(args->device) : 0;
+    if (sms == 0) return failf("gdn_b200_delta_step: cannot use device %d", args->device);
+    const cudaError_t e = gdn::ops::launch_delta_step(p, args->dtype == 1, sms, static_cast<cudaStream_t>(args->stream));
     return e == cudaSuccess ? 0 : failf("gdn_b200_delta_step: launch failed: %s", cudaGetErrorString(e));
 }
 
@@ -109,12 +110,14 @@ size_t gdn_b200_delta_chunk_workspace(uint32_t tokens, uint32_t sequences, uint3
     return gdn::ops::delta_chunk_workspace(tokens, sequences, v_heads);
 }
 
-int gdn_b200_delta_chunk_status(int device) {
+int gdn_b200_delta_status(int device) {
     DeviceScope scope(device);
-    int status = 0;
-    if (!scope.ok || gdn::ops::delta_chunk_status(&status) != cudaSuccess)
-        return failf("gdn_b200_delta_chunk_status: cannot read the status of device %d", device);
-    return status == 0 ? 0 : failf("gdn_b200_delta_chunk: a wait on the device ran out; the call's states are not valid");
+    int step = 0, chunk = 0;
+    if (!scope.ok || gdn::ops::delta_step_status(&step) != cudaSuccess || gdn::ops::delta_chunk_status(&chunk) != cudaSuccess)
+        return failf("gdn_b200_delta_status: cannot read the status of device %d", device);
+    return step == 0 && chunk == 0 ? 0
+                                   : failf("gdn_b200_delta_%s: a wait on the device ran out; the call's states are not valid",
+                                           chunk != 0 ? "chunk" : "step");
 }
 
 int gdn_b200_delta_chunk(const GdnB200DeltaArgs *args) {

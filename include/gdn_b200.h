@@ -329,10 +329,11 @@ int gdn_b200_delta_chunk(const GdnB200DeltaArgs *args);
 /* Bytes of 256-byte aligned device memory that gdn_b200_delta_chunk needs as
  * args->workspace for these sizes. */
 size_t gdn_b200_delta_chunk_workspace(uint32_t tokens, uint32_t sequences, uint32_t v_heads);
-/* 0, or -1 if a wait inside gdn_b200_delta_chunk ran out (2 s) on `device`
- * since the last call of this function: the states of that call are then NaN.
- * Waits for the device; for a server's health checks and for tests. */
-int gdn_b200_delta_chunk_status(int device);
+/* 0, or -1 if a wait inside gdn_b200_delta_step or gdn_b200_delta_chunk ran
+ * out (2 s) on `device` since the last call of this function: the states of
+ * that call are then not valid. Waits for the device; for a server's health
+ * checks and for tests. */
+int gdn_b200_delta_status(int device);
 
 /* Constraints on the logits of `rows` streams, and the greedy pick. With n
  * the times token v stands in the row's history after its prompt:

@@ -295,3 +295,46 @@ def test_refusals(ops):
     wide = torch.empty(4, 2, 67, device="cuda", dtype=torch.bfloat16)[..., 3:]
     with pytest.raises(RuntimeError, match="16-byte"):
         ops.delta_chunk(**{**a, **o, "q": wide})
+
+
+# enough states for the pipeline over row blocks (eight blocks of 32 KB or less for each of 148 SMs)
+MANY = [(150, 8, 8, 64, 64), (60, 2, 10, 128, 128), (20, 8, 8, 256, 256), (19, 4, 8, 256, 256), (67, 1, 6, 256, 96),
+        (301, 2, 4, 64, 96)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("longest", [1, 3, 4, 9])
+@pytest.mark.parametrize("many", MANY, ids=str)
+def test_many_states(ops, many, longest, dtype):
+    n, *shape = many
+    gen = torch.Generator().manual_seed(n + longest)
+    lengths = [1] * n if longest == 1 else torch.randint(0, longest + 1, (n,), generator=gen).tolist()
+    a, o = inputs(lengths, *shape, dtype, seed=n)
+    if longest != 1:
+        o["fresh"] = (torch.rand(n, generator=gen) < 0.3).cuda()
+        a["state"][o["slots"][o["fresh"]].long()] = float("nan")  # not read
+        o["slots"][::9] = -1
+        keep = torch.isin(torch.arange(a["state"].shape[0], device="cuda"), o["slots"])
+        a["state"][~keep] = 0.5
+        clean = dict(a, state=a["state"].nan_to_num(nan=0.0))
+    else:
+        clean = dict(a, state=a["state"].clone())
+    ref_o, ref_s = plain.delta_rule(**clean, **o)
+    out = ops.delta_step(**a, **o)
+    assert plain.rel(out, ref_o) <= OUT_TOL[dtype]
+    assert plain.rel(a["state"], ref_s) <= STATE_TOL
+
+
+def test_many_states_uncovered_tokens(ops):
+    a, o = inputs([2] * 160, 8, 8, 64, 64, torch.bfloat16, seed=21)
+    a.update({n: torch.cat([a[n], a[n][:9]]) for n in ("q", "k", "v", "g", "beta")})
+    ref_o, ref_s = plain.delta_rule(**a, **o)
+    out = torch.full_like(a["v"], float("nan"))
+    ops.delta_step(**a, **o, out=out)
+    assert bool((out[320:] == 0).all()) and plain.rel(out, ref_o) <= OUT_TOL[torch.bfloat16]
+    assert plain.rel(a["state"], ref_s) <= STATE_TOL
+
+
+def test_no_wait_ran_out():
+    import gateddeltanet_b200 as gdn
+    assert gdn.lib().gdn_b200_delta_status(0) == 0, gdn.last_error()
