@@ -10,17 +10,17 @@
  * is one FP32 rounding, so results do not depend on the split.
  *
  * Bound by HBM: every logit is read and written once. A row is cut into the
- * slices of one cluster's CTAs. Each CTA reads the row's history and keeps
- * what falls into its slice in a shared-memory table, one word per token:
- *   bits 0-19 n | bits 20-30 first bias entry + 1 | bit 31 in the prompt
- * (integer atomics: the order does not show), and one bit per token that says
- * whether the word is set. Tokens without one (nearly all) only meet the mask:
- * a dense pass copies them 16 bytes at a time and keeps the largest. The few
- * others are then recomputed from the history and bias lists themselves: who
- * takes a token's word out of the table (an exchange with 0) does the token,
- * so that all lanes of a warp have one to do, where a test in the dense pass
- * left a warp waiting for one lane at nearly every vector. The picks of the
- * slices meet in CTA 0 through distributed shared memory.
+ * slices of one cluster's CTAs. Each CTA reads the row's history and counts
+ * what falls into its slice in shared memory (integer atomics: the order does
+ * not show): n per token, in 16 bits where the history is short enough, and a
+ * bit that history holds the token; another bit says that a bias names it.
+ * Tokens with neither bit, nearly all, only meet the mask: a dense pass copies
+ * them 16 bytes at a time and keeps the largest. The others are then found
+ * from the bits and recomputed, a lane each; as a test in the dense pass they
+ * left whole warps waiting for the lanes that had one. What bounds the kernel
+ * beside HBM are the instructions that a warp spends once (setting up, clearing,
+ * counting, the reductions), so a CTA has few warps with many logits each.
+ * The picks of the slices meet in CTA 0 through distributed shared memory.
  */
 #include "gdn_ops.h"
 
@@ -34,12 +34,10 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kLogitsThreads = 512;
+constexpr uint32_t kThreads = 256;
 constexpr int kUnroll = 4;      /* 16-byte vectors of a thread in flight */
 constexpr int kHistoryUnroll = 4;
 constexpr int kMaxCluster = 8;  /* portable cluster size */
-constexpr uint32_t kCountMask = (1u << 20) - 1, kPromptBit = 1u << 31;
-constexpr uint32_t kFlagWords = (kMaxBiases + 32) / 32;
 
 /* pick key: larger value first, then the lower index; NaN is 0 and so never wins */
 __device__ __forceinline__ unsigned long long pick_key(float x, uint32_t v) {
@@ -98,207 +96,235 @@ __device__ __forceinline__ float rounded(float x, __nv_bfloat16) { return __bflo
 __device__ __forceinline__ void store_one(float *p, float x) { *p = x; }
 __device__ __forceinline__ void store_one(__nv_bfloat16 *p, float x) { *p = __float2bfloat16_rn(x); }
 
-struct Row {
-    float repetition, presence, frequency;
-    const int32_t *bias_ids;
-    const float *bias;
-    const uint32_t *multi; /* bias entries whose token has later entries too */
-    uint32_t biases;
-};
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
-/* x with what the table's word says */
-__device__ __forceinline__ float touched(float x, uint32_t word, const Row &r) {
-    const uint32_t n = word & kCountMask, entry = (word >> 20) & kMaxBiases;
-    if (n != 0 || (word & kPromptBit)) x = x > 0.0f ? __fdiv_rn(x, r.repetition) : __fmul_rn(x, r.repetition);
-    if (n != 0) x = __fsub_rn(__fsub_rn(x, __fmul_rn(r.frequency, (float)n)), r.presence);
-    if (entry != 0) {
-        const uint32_t i = entry - 1;
-        float sum = r.bias[i];
-        if ((r.multi[i >> 5] >> (i & 31)) & 1u)
-            for (uint32_t j = i + 1; j < r.biases; ++j)
-                if (r.bias_ids[j] == r.bias_ids[i]) sum = __fadd_rn(sum, r.bias[j]);
-        x = __fadd_rn(x, sum);
+/* position of the n-th set bit (from 0) of a word that has more than n */
+__device__ __forceinline__ uint32_t nth_bit(uint32_t w, uint32_t n) {
+    uint32_t at = 0;
+#pragma unroll
+    for (uint32_t half = 16; half > 0; half >>= 1) {
+        const uint32_t below = __popc(w & ((1u << half) - 1));
+        if (n >= below) {
+            n -= below;
+            w >>= half;
+            at += half;
+        }
     }
-    return x;
+    return at;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kLogitsThreads) logits_kernel(const __grid_constant__ LogitsParams p) {
+/* W: the type of a token's count. kAligned: every row of logits and of out
+ * starts on a 16-byte boundary. */
+template <typename T, typename W, bool kAligned>
+__global__ void __launch_bounds__(kThreads, 5) logits_kernel(const __grid_constant__ LogitsParams p) {
     constexpr int N = Vec<T>::kN;
-    extern __shared__ __align__(16) uint32_t table[]; /* words of the slice, then a bit each */
-    __shared__ uint32_t multi[kFlagWords];
-    __shared__ unsigned long long warp_key[kLogitsThreads / 32], slice_key[kMaxCluster];
+    constexpr float kNegInf = -__builtin_huge_valf();
+    extern __shared__ __align__(16) uint32_t table[]; /* counts of the slice, two bits each, the slice's biases */
+    __shared__ unsigned long long warp_key[kThreads / 32], slice_key[kMaxCluster];
+    __shared__ uint32_t slice_biases;
     cg::cluster_group cluster = cg::this_cluster();
     const uint32_t C = cluster.num_blocks(), rank = cluster.block_rank(), b = blockIdx.x / C;
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    cluster_arrive(); /* every CTA has begun before one writes to another */
     const T *in = static_cast<const T *>(p.logits) + (int64_t)b * p.logits_row;
     T *out = static_cast<T *>(p.out) + (int64_t)b * p.out_row;
     const uint32_t V = p.vocab;
     /* vectors are cut at 16-byte boundaries of the input row: vector i holds
      * the tokens i N - mis .. i N - mis + N - 1 */
-    const uint32_t mis = (uint32_t)((reinterpret_cast<uintptr_t>(in) / sizeof(T)) % N);
-    const bool wide_out = ((reinterpret_cast<uintptr_t>(in) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0;
+    const uint32_t mis = kAligned ? 0u : (uint32_t)((reinterpret_cast<uintptr_t>(in) / sizeof(T)) % N);
+    const bool wide_out = kAligned || ((reinterpret_cast<uintptr_t>(in) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0;
     const uint32_t nvec = (mis + V + N - 1) / N;
     const uint32_t v0 = min(nvec, rank * p.slice_vecs), v1 = min(nvec, v0 + p.slice_vecs);
-    const int32_t first = (int32_t)(v0 * N) - (int32_t)mis; /* token of table word 0 */
+    const int32_t first = (int32_t)(v0 * N) - (int32_t)mis; /* token of the table's first count */
     const int32_t lo = max(first, 0), hi = min((int32_t)V, (int32_t)(v1 * N) - (int32_t)mis);
     const uint32_t *mask = p.mask == nullptr ? nullptr : p.mask + (int64_t)b * p.mask_row;
-    const uint32_t words = (p.slice_vecs * N + 127) & ~127u;
-    uint32_t *bits = table + words;
+    const uint32_t size = (p.slice_vecs * N + 127) & ~127u; /* tokens of the table */
+    uint32_t *past = table + size * sizeof(W) / 4, *biased = past + size / 32;
 
+    int32_t *slice_id = reinterpret_cast<int32_t *>(biased + size / 32);
+    float *slice_bias = reinterpret_cast<float *>(slice_id + p.biases);
+
+    /* the vectors [va, vb) lie in the row whole */
+    const uint32_t va = max(v0, mis != 0 ? 1u : 0u), vb = min(v1, nvec - ((mis + V) % N != 0 ? 1u : 0u));
+    const uint4 *src = reinterpret_cast<const uint4 *>(in - mis);
     uint4 w[kUnroll];
-    /* the vectors base, base + kLogitsThreads, ... that lie in the row whole */
-    auto whole = [&](uint32_t i) {
-        const int32_t e0 = (int32_t)(i * N) - (int32_t)mis;
-        return i < v1 && e0 >= 0 && e0 + N <= (int32_t)V;
-    };
     auto load = [&](uint32_t base) {
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-            const uint32_t i = base + u * kLogitsThreads;
-            if (whole(i)) w[u] = __ldcs(reinterpret_cast<const uint4 *>(in + ((int32_t)(i * N) - (int32_t)mis)));
-        }
+        for (int u = 0; u < kUnroll; ++u)
+            if (base + u * kThreads < vb) w[u] = __ldcs(src + base + u * kThreads);
     };
-    load(v0 + tid); /* on their way while the table is built */
+    load(va + tid); /* on their way while the table is built */
 
-    const bool use_table = p.tokens != nullptr || p.bias_ids != nullptr;
-    Row row;
-    row.repetition = p.repetition == nullptr ? 1.0f : p.repetition[b];
-    row.presence = p.presence == nullptr ? 0.0f : p.presence[b];
-    row.frequency = p.frequency == nullptr ? 0.0f : p.frequency[b];
-    row.bias_ids = p.bias_ids + (int64_t)b * p.bias_ids_row;
-    row.bias = p.bias + (int64_t)b * p.bias_row;
-    row.multi = multi;
-    row.biases = p.bias_ids == nullptr ? 0 : p.biases;
-    const int32_t *ids = p.tokens + (int64_t)b * p.tokens_row;
+    const uint32_t biases = p.bias_ids == nullptr ? 0 : p.biases;
+    const int32_t *bias_ids = p.bias_ids + (int64_t)b * p.bias_ids_row;
     const int32_t len = p.tokens == nullptr ? 0 : p.lens == nullptr ? (int32_t)p.history : min(p.lens[b], (int32_t)p.history);
-
+    const bool use_table = len > 0 || biases > 0;
     if (use_table) {
-        for (uint32_t i = tid; i < (words + words / 32) / 4; i += kLogitsThreads)
-            reinterpret_cast<uint4 *>(table)[i] = make_uint4(0, 0, 0, 0);
-        for (uint32_t i = tid; i < kFlagWords; i += kLogitsThreads) multi[i] = 0;
-        __syncthreads();
-        const int32_t made = p.prompt_lens == nullptr ? 0 : p.prompt_lens[b];
-        for (int32_t i0 = (int32_t)tid; i0 < len; i0 += kLogitsThreads * kHistoryUnroll) {
-            int32_t id[kHistoryUnroll];
+        const int32_t *ids = p.tokens + (int64_t)b * p.tokens_row;
+        int32_t id[kHistoryUnroll];
+        auto load_ids = [&](int32_t i0) {
 #pragma unroll
             for (int u = 0; u < kHistoryUnroll; ++u) {
-                const int32_t i = i0 + u * kLogitsThreads;
+                const int32_t i = i0 + u * (int32_t)kThreads;
                 id[u] = i < len ? ids[i] : -1;
             }
+        };
+        load_ids((int32_t)tid);
+        int32_t bias_id = warp == 0 && lane < biases ? bias_ids[lane] : -1;
+        const int32_t made = p.prompt_lens == nullptr ? 0 : p.prompt_lens[b];
+        const uint32_t clear = (size * sizeof(W) / 4 + size / 16) / 4;
+        for (uint32_t i = tid; i < clear; i += kThreads) reinterpret_cast<uint4 *>(table)[i] = make_uint4(0, 0, 0, 0);
+        __syncthreads();
+        const uint32_t span = hi > lo ? (uint32_t)(hi - lo) : 0u;
+        for (int32_t i0 = (int32_t)tid; i0 < len; i0 += (int32_t)kThreads * kHistoryUnroll) {
+            if (i0 != (int32_t)tid) load_ids(i0);
 #pragma unroll
             for (int u = 0; u < kHistoryUnroll; ++u) {
-                if (id[u] < lo || id[u] >= hi) continue;
+                if ((uint32_t)(id[u] - lo) >= span) continue;
                 const uint32_t at = (uint32_t)(id[u] - first);
-                const uint32_t old = i0 + u * kLogitsThreads >= made ? atomicAdd(&table[at], 1u) : atomicOr(&table[at], kPromptBit);
-                if (old == 0) atomicOr(&bits[at >> 5], 1u << (at & 31));
+                atomicOr(&past[at >> 5], 1u << (at & 31));
+                if (i0 + u * (int32_t)kThreads >= made) {
+                    if (sizeof(W) == 4)
+                        atomicAdd(&table[at], 1u);
+                    else
+                        atomicAdd(&table[at >> 1], (at & 1) ? 65536u : 1u); /* no count reaches 65536: nothing is carried */
+                }
             }
         }
-        /* a biased token's word names its first entry */
-        for (uint32_t i = tid; i < row.biases; i += kLogitsThreads) {
-            const int32_t id = row.bias_ids[i];
-            if (id < lo || id >= hi) continue;
-            const uint32_t at = (uint32_t)(id - first);
-            uint32_t old = table[at];
-            while (true) {
-                const uint32_t e = (old >> 20) & kMaxBiases;
-                if (e != 0 && e <= i + 1) break;
-                const uint32_t seen = atomicCAS(&table[at], old, (old & ~(kMaxBiases << 20)) | ((i + 1) << 20));
-                if (seen == old) break;
-                old = seen;
+        if (warp == 0) {
+            /* the biases of the slice, in list order */
+            const float *bias = p.bias + (int64_t)b * p.bias_row;
+            uint32_t found = 0;
+            for (uint32_t i0 = 0; i0 < biases; i0 += 32) {
+                if (i0 != 0) bias_id = i0 + lane < biases ? bias_ids[i0 + lane] : -1;
+                const bool here = (uint32_t)(bias_id - lo) < span;
+                const uint32_t who = __ballot_sync(0xffffffffu, here);
+                if (here) {
+                    const uint32_t at = (uint32_t)(bias_id - first), place = found + __popc(who & ((1u << lane) - 1));
+                    atomicOr(&biased[at >> 5], 1u << (at & 31));
+                    slice_id[place] = bias_id;
+                    slice_bias[place] = bias[i0 + lane];
+                }
+                found += __popc(who);
             }
-            atomicOr(&bits[at >> 5], 1u << (at & 31));
+            if (lane == 0) slice_biases = found;
         }
         __syncthreads();
-        for (uint32_t i = tid; i < row.biases; i += kLogitsThreads) {
-            const int32_t id = row.bias_ids[i];
-            if (id < lo || id >= hi) continue;
-            const uint32_t e = (table[id - first] >> 20) & kMaxBiases;
-            if (e != i + 1) atomicOr(&multi[(e - 1) >> 5], 1u << ((e - 1) & 31));
-        }
     }
 
-    /* dense pass: the mask, and the largest of the tokens without a word.
+    /* dense pass: the mask, and the largest of the tokens without a bit.
      * Tokens with one keep their value for now. */
     unsigned long long best = 0;
-    float top = __int_as_float(0xff800000);
+    float top = kNegInf;
     uint32_t top_vec = 0;
-    uint4 top_w = make_uint4(0, 0, 0, 0);
-    for (uint32_t base = v0 + tid; base < v1; base += kLogitsThreads * kUnroll) {
-        if (base != v0 + tid) load(base);
+    const uint8_t *past8 = reinterpret_cast<const uint8_t *>(past), *biased8 = reinterpret_cast<const uint8_t *>(biased);
+    const uint8_t *mask8 = reinterpret_cast<const uint8_t *>(mask);
+    /* N bits of vector i of a row of bits that starts with a vector's first token */
+    auto bits_of = [&](const uint8_t *bits, uint32_t i) {
+        return N == 8 ? (uint32_t)bits[i] : (uint32_t)bits[i >> 1] >> (4 * (i & 1)) & 15u;
+    };
+    auto own_bits = [&](uint32_t i) { return use_table ? bits_of(past8, i - v0) | bits_of(biased8, i - v0) : 0u; };
+    auto edge = [&](uint32_t i) {
+        /* a row's ragged first or last vector */
+        const int32_t e0 = (int32_t)(i * N) - (int32_t)mis;
+        const uint32_t own = own_bits(i);
+        for (int32_t e = max(e0, 0); e < min(e0 + N, (int32_t)V); ++e) {
+            float x = load_one(in + e);
+            const bool keep = (own >> (e - e0)) & 1u;
+            if (!keep && mask != nullptr && !((mask[e >> 5] >> (e & 31)) & 1u)) x = kNegInf;
+            store_one(out + e, x);
+            const unsigned long long key = keep ? 0ull : pick_key(x, (uint32_t)e);
+            best = key > best ? key : best;
+        }
+    };
+    if (tid == 0 && v0 < min(va, v1)) edge(v0);
+    if (tid == 32 && vb < v1 && v1 - 1 >= va) edge(v1 - 1);
+    for (uint32_t base = va + tid; base < vb; base += kThreads * kUnroll) {
+        if (base != va + tid) load(base);
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
-            const uint32_t i = base + u * kLogitsThreads;
-            if (i >= v1) continue;
-            const int32_t e0 = (int32_t)(i * N) - (int32_t)mis;
-            const uint32_t at = (i - v0) * N;
-            const uint32_t own = use_table ? bits[at >> 5] >> (at & 31) : 0u;
-            if (!whole(i)) {
-                /* a row's ragged first or last vector */
-                for (int32_t e = max(e0, 0); e < min(e0 + N, (int32_t)V); ++e) {
-                    float x = load_one(in + e);
-                    if ((own >> (e - e0)) & 1u) {
-                        store_one(out + e, x);
-                        continue;
-                    }
-                    if (mask != nullptr && !((mask[e >> 5] >> (e & 31)) & 1u)) x = __int_as_float(0xff800000);
-                    store_one(out + e, x);
-                    const unsigned long long key = pick_key(x, (uint32_t)e);
-                    best = key > best ? key : best;
-                }
-                continue;
+            const uint32_t i = base + u * kThreads;
+            if (i >= vb) break;
+            const uint32_t own = own_bits(i);
+            uint4 o = w[u];
+            if (mask != nullptr) {
+                const uint32_t e0 = i * N - mis;
+                const uint32_t allow = mis == 0 ? bits_of(mask8, i)
+                                                : __funnelshift_r(mask[e0 >> 5], mask[(e0 + N - 1) >> 5], e0 & 31);
+                o = Vec<T>::only(o, allow | own);
             }
-            uint32_t allow = 0xFFFFFFFFu;
-            if (mask != nullptr) allow = __funnelshift_r(mask[e0 >> 5], mask[(e0 + N - 1) >> 5], e0 & 31);
-            const uint4 o = Vec<T>::only(w[u], allow | own);
             if (wide_out) {
-                __stcs(reinterpret_cast<uint4 *>(out + e0), o);
+                __stcs(reinterpret_cast<uint4 *>(out - mis) + i, o);
             } else {
 #pragma unroll
-                for (int j = 0; j < N; ++j) store_one(out + e0 + j, Vec<T>::value(o, j));
+                for (int j = 0; j < N; ++j) store_one(out - mis + (i * N + j), Vec<T>::value(o, j));
             }
-            const uint4 free = (own & ((1u << N) - 1)) ? Vec<T>::only(w[u], allow & ~own) : o;
-            const float m = Vec<T>::largest(free);
+            if (own) o = Vec<T>::only(o, ~own);
+            const float m = Vec<T>::largest(o);
             if (m > top) {
                 top = m;
                 top_vec = i;
-                top_w = free;
             }
         }
     }
-    if (top > __int_as_float(0xff800000)) {
-#pragma unroll
-        for (int j = N - 1; j >= 0; --j)
-            if (Vec<T>::value(top_w, j) == top) {
-                const unsigned long long key = pick_key(top, top_vec * N - mis + j);
-                best = key > best ? key : best;
-            }
+    if (top > kNegInf) {
+        /* this thread's own vector again: which of its tokens it was */
+        const T *again = out - mis + (size_t)top_vec * N;
+        const uint32_t own = own_bits(top_vec);
+        uint32_t e = 0;
+        while (e + 1 < N && (((own >> e) & 1u) || load_one(again + e) != top)) ++e;
+        const unsigned long long key = pick_key(top, top_vec * N - mis + e);
+        best = key > best ? key : best;
     }
     if (use_table) {
         __syncthreads();
-        auto recompute = [&](int32_t id) {
-            if (id < lo || id >= hi) return;
-            const uint32_t word = atomicExch(&table[id - first], 0u);
-            if (word == 0) return;
-            /* from out where the dense pass left it: out may be the logits */
-            float x = touched(load_one(out + id), word, row);
-            if (mask != nullptr && !((mask[id >> 5] >> (id & 31)) & 1u)) x = __int_as_float(0xff800000);
-            x = rounded(x, T());
-            store_one(out + id, x);
-            const unsigned long long key = pick_key(x, (uint32_t)id);
-            best = key > best ? key : best;
-        };
-        for (int32_t i0 = (int32_t)tid; i0 < len; i0 += kLogitsThreads * kHistoryUnroll) {
-            int32_t id[kHistoryUnroll];
+        const float repetition = p.repetition == nullptr ? 1.0f : p.repetition[b];
+        const float presence = p.presence == nullptr ? 0.0f : p.presence[b];
+        const float frequency = p.frequency == nullptr ? 0.0f : p.frequency[b];
+        /* 32 words of bits at a time: the set ones in order, one for each lane */
+        for (uint32_t w0 = warp * 32; w0 < size / 32; w0 += kThreads) {
+            const uint32_t i = w0 + lane, set = i < size / 32 ? past[i] | biased[i] : 0u;
+            uint32_t upto = __popc(set);
 #pragma unroll
-            for (int u = 0; u < kHistoryUnroll; ++u) {
-                const int32_t i = i0 + u * kLogitsThreads;
-                id[u] = i < len ? ids[i] : -1;
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint32_t below = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= (uint32_t)o) upto += below;
             }
+            const uint32_t total = __shfl_sync(0xffffffffu, upto, 31);
+            for (uint32_t k0 = 0; k0 < total; k0 += 32) {
+                const uint32_t k = k0 + lane;
+                /* the word that the k-th set bit is in: the first whose running count exceeds k */
+                uint32_t src = 0;
 #pragma unroll
-            for (int u = 0; u < kHistoryUnroll; ++u) recompute(id[u]);
+                for (uint32_t half = 16; half > 0; half >>= 1)
+                    if (__shfl_sync(0xffffffffu, upto, src + half - 1) <= k) src += half;
+                src &= 31;
+                const uint32_t word = __shfl_sync(0xffffffffu, set, src), before = __shfl_sync(0xffffffffu, upto, src) - __popc(word);
+                if (k >= total) continue;
+                const uint32_t at = 32 * (w0 + src) + nth_bit(word, k - before);
+                const int32_t id = first + (int32_t)at;
+                const uint32_t n = sizeof(W) == 4 ? table[at] : (table[at >> 1] >> (16 * (at & 1))) & 0xFFFFu;
+                float x = load_one(out + id); /* where the dense pass left it: out may be the logits */
+                if ((past[at >> 5] >> (at & 31)) & 1u) x = x > 0.0f ? __fdiv_rn(x, repetition) : __fmul_rn(x, repetition);
+                if (n != 0) x = __fsub_rn(__fsub_rn(x, __fmul_rn(frequency, (float)n)), presence);
+                if ((biased[at >> 5] >> (at & 31)) & 1u) {
+                    float sum = 0.0f;
+                    bool any = false;
+                    for (uint32_t e = 0; e < slice_biases; ++e)
+                        if (slice_id[e] == id) {
+                            sum = any ? __fadd_rn(sum, slice_bias[e]) : slice_bias[e];
+                            any = true;
+                        }
+                    x = __fadd_rn(x, sum);
+                }
+                if (mask != nullptr && !((mask[id >> 5] >> (id & 31)) & 1u)) x = kNegInf;
+                x = rounded(x, T());
+                store_one(out + id, x);
+                const unsigned long long key = pick_key(x, (uint32_t)id);
+                best = key > best ? key : best;
+            }
         }
-        for (uint32_t i = tid; i < row.biases; i += kLogitsThreads) recompute(row.bias_ids[i]);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
@@ -307,37 +333,39 @@ __global__ void __launch_bounds__(kLogitsThreads) logits_kernel(const __grid_con
     }
     if (lane == 0) warp_key[warp] = best;
     __syncthreads();
-    if (warp == 0) {
-        best = lane < kLogitsThreads / 32 ? warp_key[lane] : 0ull;
+    if (tid == 0) {
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            const unsigned long long other = __shfl_xor_sync(0xffffffffu, best, o);
-            best = other > best ? other : best;
-        }
-        if (lane == 0) cluster.map_shared_rank(slice_key, 0)[rank] = best;
+        for (uint32_t i = 1; i < kThreads / 32; ++i) best = warp_key[i] > best ? warp_key[i] : best;
     }
-    cluster.sync();
-    if (rank == 0 && tid == 0) {
+    cluster_wait();
+    if (tid == 0) cluster.map_shared_rank(slice_key, 0)[rank] = best;
+    cluster_arrive();
+    if (rank != 0) return;
+    cluster_wait();
+    if (tid == 0) {
         for (uint32_t c = 0; c < C; ++c) best = slice_key[c] > best ? slice_key[c] : best;
         p.picks[b] = (uint32_t)(best >> 32) > kKeyNegInf ? (int32_t)(0xFFFFFFFFu - (uint32_t)best) : -1;
     }
 }
 
-template <typename T>
+template <typename T, typename W, bool kAligned>
 cudaError_t launch_logits_t(LogitsParams &p, int sms, cudaStream_t stream) {
     constexpr uint32_t N = Vec<T>::kN;
     const uint32_t nvec = (p.vocab + N - 1) / N + 1; /* a row that starts inside a vector has one more */
+    /* Few rows: eight slices each, for the latency. Many: slices of about
+     * 16384 tokens, whose logits a CTA's threads hold in flight (BF16) while
+     * they count, in a table that lets three CTAs share an SM. */
     uint32_t C = 1;
-    while (C < kMaxCluster && (p.rows * C < 2u * (uint32_t)sms || nvec * N / C > 16384u)) C *= 2;
+    while (C < kMaxCluster && (p.rows * C < 4u * (uint32_t)sms || nvec * N / C > 16384u + N)) C *= 2;
     p.slice_vecs = (nvec + C - 1) / C;
     const bool use_table = p.tokens != nullptr || p.bias_ids != nullptr;
-    const size_t words = (p.slice_vecs * N + 127) & ~127u;
-    const size_t smem = use_table ? (words + words / 32) * 4 : 0;
-    cudaError_t e = cudaFuncSetAttribute(logits_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    const size_t size = (p.slice_vecs * N + 127) & ~(size_t)127;
+    const size_t smem = use_table ? size * sizeof(W) + size / 4 + 8 * (size_t)p.biases : 0;
+    cudaError_t e = cudaFuncSetAttribute(logits_kernel<T, W, kAligned>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(p.rows * C);
-    cfg.blockDim = dim3(kLogitsThreads);
+    cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
@@ -346,13 +374,26 @@ cudaError_t launch_logits_t(LogitsParams &p, int sms, cudaStream_t stream) {
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, logits_kernel<T>, p);
+    return cudaLaunchKernelEx(&cfg, logits_kernel<T, W, kAligned>, p);
 }
 
 }  // namespace
 
 cudaError_t launch_logits(LogitsParams p, bool bf16, int sms, cudaStream_t stream) {
-    return bf16 ? launch_logits_t<__nv_bfloat16>(p, sms, stream) : launch_logits_t<float>(p, sms, stream);
+    const int64_t per = bf16 ? 8 : 4;
+    const bool aligned = ((reinterpret_cast<uintptr_t>(p.logits) | reinterpret_cast<uintptr_t>(p.out)) & 15) == 0 &&
+                         (p.rows == 1 || (p.logits_row % per == 0 && p.out_row % per == 0));
+    auto *launch = launch_logits_t<float, uint16_t, false>;
+    const bool wide = p.history > 65535u;
+    if (bf16)
+        launch = wide ? aligned ? launch_logits_t<__nv_bfloat16, uint32_t, true> : launch_logits_t<__nv_bfloat16, uint32_t, false>
+                 : aligned ? launch_logits_t<__nv_bfloat16, uint16_t, true>
+                           : launch_logits_t<__nv_bfloat16, uint16_t, false>;
+    else
+        launch = wide ? aligned ? launch_logits_t<float, uint32_t, true> : launch_logits_t<float, uint32_t, false>
+                 : aligned ? launch_logits_t<float, uint16_t, true>
+                           : launch_logits_t<float, uint16_t, false>;
+    return launch(p, sms, stream);
 }
 
 }  // namespace ops

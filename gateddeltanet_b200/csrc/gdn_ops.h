@@ -64,8 +64,8 @@ struct LogitsParams {
     uint32_t slice_vecs;  /* 16-byte vectors of a row that one CTA takes */
 };
 
-constexpr uint32_t kMaxHistory = (1u << 20) - 1; /* the table's count field */
-constexpr uint32_t kMaxBiases = 2047;            /* the table's entry field */
+constexpr uint32_t kMaxHistory = (1u << 20) - 1;
+constexpr uint32_t kMaxBiases = 2047;  /* searched once for each biased token */
 constexpr uint32_t kMaxVocab = 1u << 18;
 
 cudaError_t launch_delta_step(const DeltaParams &p, bool bf16, int sms, cudaStream_t stream);
