@@ -2,6 +2,7 @@
 device is touched (no GPU needed), and the plain forms the GPU tests compare
 with agree with a second way of writing the formulas."""
 import ctypes
+import struct
 
 import pytest
 import torch
@@ -10,6 +11,8 @@ import gateddeltanet_b200 as gdn
 import ops_plain as plain
 
 FAKE = 1 << 20  # an aligned address that no check follows
+DELTA = struct.Struct("@13Q13q7I3ifI")   # GdnB200DeltaArgs
+LOGITS = struct.Struct("@13Q6q4I2i")     # GdnB200LogitsArgs
 
 
 @pytest.fixture(scope="module")
@@ -20,13 +23,12 @@ def lib():
 
 
 def delta_args(**change):
-    from gateddeltanet_b200 import ops
     f = dict(q=FAKE, k=FAKE, v=FAKE, g=FAKE, beta=FAKE, state=FAKE, out=FAKE, starts=FAKE, slots=FAKE, fresh=0, workspace=FAKE,
              workspace_bytes=1 << 40, stream=0, q_token=64, q_head=64, k_token=64, k_head=64, v_token=64, v_head=64, g_token=1,
              g_head=1, beta_token=1, beta_head=1, out_token=64, out_head=64, state_slot=4096, sequences=2, tokens=5, heads=1,
              v_heads=1, key_dim=64, value_dim=64, state_slots=2, dtype=1, normalize=0, device=0, scale=1.0, reserved=0)
     assert set(change) <= set(f)
-    return ops._DELTA.pack(*{**f, **change}.values())
+    return DELTA.pack(*{**f, **change}.values())
 
 
 @pytest.mark.parametrize("change,reason", [
@@ -55,12 +57,11 @@ def test_delta_nothing_to_do(lib):
 
 
 def logits_args(**change):
-    from gateddeltanet_b200 import ops
     f = dict(logits=FAKE, out=FAKE, picks=FAKE, tokens=FAKE, lens=FAKE, prompt_lens=FAKE, repetition=FAKE, presence=FAKE,
              frequency=FAKE, bias_ids=FAKE, bias=FAKE, mask=FAKE, stream=0, logits_row=100, out_row=100, tokens_row=5,
              bias_ids_row=2, bias_row=2, mask_row=4, rows=2, vocab=100, history=5, biases=2, dtype=0, device=0)
     assert set(change) <= set(f)
-    return ops._LOGITS.pack(*{**f, **change}.values())
+    return LOGITS.pack(*{**f, **change}.values())
 
 
 @pytest.mark.parametrize("change,reason", [
@@ -105,6 +106,5 @@ def test_plain_constraints_by_hand():
 
 
 def test_argument_layouts():
-    from gateddeltanet_b200 import ops
-    assert ops._DELTA.size == 13 * 8 + 13 * 8 + 12 * 4 and ops._LOGITS.size == 13 * 8 + 6 * 8 + 6 * 4
+    assert DELTA.size == 13 * 8 + 13 * 8 + 12 * 4 and LOGITS.size == 13 * 8 + 6 * 8 + 6 * 4
     assert ctypes.sizeof(ctypes.c_size_t) == 8
