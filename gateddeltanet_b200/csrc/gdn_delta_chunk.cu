@@ -10,7 +10,7 @@
  *   S = e^(G_C) S0 + sum_j e^(G_C - G_j) D_j khat_j^T
  * T and P T do not depend on the state, so a first kernel forms them for all
  * chunks at once; a second one walks each sequence's chunks. The columns of
- * S0^T (value rows) do not mix: a CTA takes kVB of them through the whole
+ * S0^T (value rows) do not mix: a CTA takes VB of them through the whole
  * sequence, with the state in registers.
  *
  * The state has to come out as FP32 arithmetic would give it, from BF16
@@ -19,7 +19,10 @@
  * as BF16 terms that sum to it: three for S0, R and D (24 bits), two for T and
  * P T (16 bits: T's unit diagonal is exact, so what is rounded is its smaller
  * part below, and the outputs are BF16). The terms of an operand are columns
- * of one MMA (N = 3 kVB), whose sums are added when they are read back.
+ * of one MMA (N = 3 VB), whose sums are added when they are read back.
+ *
+ * What bounds the walk is the chain of one chunk: three rounds of MMAs, each
+ * waiting for the epilogue of the one before.
  */
 #include "gdn_ops.h"
 
@@ -31,7 +34,6 @@ namespace ops {
 namespace {
 
 constexpr int kC = 64;      /* tokens of a chunk */
-constexpr int kVB = 16;     /* value rows of a CTA */
 constexpr uint64_t kWaitNs = 2000000000ull;
 
 /* per (chunk, value head): [T; P T] as two BF16 terms in the MMA's layout,
@@ -134,17 +136,36 @@ __device__ __forceinline__ void tc_ld8(uint32_t addr, uint32_t (&r)[8]) {
                  : "r"(addr));
 }
 __device__ __forceinline__ void tc_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-/* the sums of the three terms' columns: eight value rows starting at addr */
+/* pairs of FP32 values */
+__device__ __forceinline__ uint64_t pack2(uint32_t lo, uint32_t hi) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
+    return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, uint32_t &lo, uint32_t &hi) {
+    asm("mov.b64 {%0, %1}, %2;" : "=r"(lo), "=r"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+/* the sums of the three terms' columns (VB apart): eight value rows starting at addr */
+template <int VB>
 __device__ __forceinline__ void tc_sum3(uint32_t addr, float (&x)[8]) {
     uint32_t a[8], b[8], c[8];
     __syncwarp();
     tc_ld8(addr, a);
-    tc_ld8(addr + kVB, b);
-    tc_ld8(addr + 2 * kVB, c);
+    tc_ld8(addr + VB, b);
+    tc_ld8(addr + 2 * VB, c);
     tc_wait();
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-        x[i] = __uint_as_float(a[i]) + (__uint_as_float(b[i]) + __uint_as_float(c[i]));
+    for (int i = 0; i < 8; i += 2) {
+        uint32_t lo, hi;
+        unpack2(add2(pack2(a[i], a[i + 1]), add2(pack2(b[i], b[i + 1]), pack2(c[i], c[i + 1]))), lo, hi);
+        x[i] = __uint_as_float(lo);
+        x[i + 1] = __uint_as_float(hi);
+    }
 }
 
 /* 16-byte piece `piece` of row `row` in the 128-byte swizzle */
@@ -158,35 +179,41 @@ __device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
 /* Eight values as three BF16 terms, eight significant bits each from the top:
  * with the 24 bits of FP32 their sum is the value itself (an infinity or a
  * NaN makes NaN terms, as it would make every sum it enters). Row `row` of an
- * MN-major operand, pieces term * kVB / 8 + half. */
-__device__ __forceinline__ void put_terms(uint8_t *base, uint32_t row, uint32_t half, const float (&x)[8]) {
+ * MN-major operand of `rows` rows: the eight-value pieces term * VB / 8 + sub,
+ * eight of them to a row of 128 bytes, the further ones in a second block. */
+template <int VB>
+__device__ __forceinline__ void put_terms(uint8_t *base, uint32_t rows, uint32_t row, uint32_t sub, const float (&x)[8]) {
     uint32_t r[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) r[i] = __float_as_uint(x[i]);
 #pragma unroll
     for (int term = 0; term < 3; ++term) {
+        const uint32_t piece = term * (VB / 8) + sub;
         uint32_t w[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) w[i] = __byte_perm(r[2 * i], r[2 * i + 1], 0x7632);
-        *reinterpret_cast<uint4 *>(base + piece_at(row, term * (kVB / 8) + half)) = make_uint4(w[0], w[1], w[2], w[3]);
+        *reinterpret_cast<uint4 *>(base + (piece >> 3) * rows * 128 + piece_at(row, piece & 7)) = make_uint4(w[0], w[1], w[2], w[3]);
         if (term < 2) {
+            /* minus the term: its sign bit flipped */
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                r[i] = __float_as_uint(__uint_as_float(r[i]) - __uint_as_float(r[i] & 0xFFFF0000u));
+            for (int i = 0; i < 8; i += 2)
+                unpack2(add2(pack2(r[i], r[i + 1]), pack2((r[i] & 0xFFFF0000u) ^ 0x80000000u, (r[i + 1] & 0xFFFF0000u) ^ 0x80000000u)),
+                        r[i], r[i + 1]);
         }
     }
 }
 
 /* `rows` tokens from t0 on of one head (zeros up to 64) as the rows `first`
- * .. first + 63 of [128 rows][64 columns] blocks in the 128-byte swizzle */
+ * .. first + 63 of blocks of 64 columns (`block` bytes apart) in the 128-byte
+ * swizzle */
 template <int K>
-__device__ __forceinline__ void load_rows(uint32_t tile, uint32_t first, const __nv_bfloat16 *x, int64_t t0, int64_t stride,
+__device__ __forceinline__ void load_rows(uint32_t tile, uint32_t block, uint32_t first, const __nv_bfloat16 *x, int64_t t0, int64_t stride,
                                           uint32_t rows, uint32_t thread, uint32_t threads) {
     constexpr uint32_t kPieces = K / 8;
 #pragma unroll 8
     for (uint32_t i = thread; i < kC * kPieces; i += threads) {
         const uint32_t r = i / kPieces, c = i % kPieces;
-        const uint32_t dst = tile + (c >> 3) * kTermBytes + piece_at(first + r, c & 7);
+        const uint32_t dst = tile + (c >> 3) * block + piece_at(first + r, c & 7);
         const __nv_bfloat16 *src = r < rows ? x + (t0 + r) * stride + c * 8 : x;
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(r < rows ? 16u : 0u)
                      : "memory");
@@ -201,7 +228,34 @@ __device__ __forceinline__ void cp_async_wait_all() {
  * chunk c of sequence n has number starts[n] / 64 + n + c. */
 __host__ __device__ __forceinline__ uint32_t record_of(uint32_t t0, uint32_t n) { return t0 / kC + n; }
 
+/* Programmatic dependent launch: the second kernel may set up while the first
+ * one finishes, and waits for it before it reads anything of its. */
+__device__ __forceinline__ void pdl_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 /* ------------------------------------------------------------ first kernel */
+
+/* order[i]: the i-th longest sequence. The walks start in this order, so that
+ * the last to start are short. The CTAs of the first value head take the
+ * sequences in turn; a place is the number of sequences that come before. */
+__device__ __forceinline__ void place_sequences(const DeltaParams &p, uint32_t *order) {
+    for (uint32_t n = blockIdx.x; n < p.N; n += gridDim.x) {
+        uint32_t a, b, before = 0;
+        sequence_tokens(p, n, a, b);
+        const uint32_t len = b - a;
+        for (uint32_t m = threadIdx.x; m < p.N; m += blockDim.x) {
+            sequence_tokens(p, m, a, b);
+            before += b - a > len || (b - a == len && m < n);
+        }
+        __shared__ uint32_t total;
+        __syncthreads();
+        if (threadIdx.x == 0) total = 0;
+        __syncthreads();
+        if (before) atomicAdd(&total, before);
+        __syncthreads();
+        if (threadIdx.x == 0) order[total] = n;
+    }
+}
 
 constexpr int kPrepThreads = 256;
 constexpr uint32_t kLd = kC + 4; /* row stride of the FP32 matrices, floats */
@@ -248,7 +302,7 @@ __device__ __forceinline__ void put_pair4(uint8_t *rec, uint32_t row, uint32_t c
 }
 
 template <int K>
-__global__ void __launch_bounds__(kPrepThreads) chunk_prep_kernel(const __grid_constant__ DeltaParams p, uint8_t *records) {
+__global__ void __launch_bounds__(kPrepThreads) chunk_prep_kernel(const __grid_constant__ DeltaParams p, uint8_t *records, uint32_t *order) {
     using L = PrepSmem<K>;
     extern __shared__ uint8_t raw[];
     uint8_t *sm = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
@@ -256,6 +310,7 @@ __global__ void __launch_bounds__(kPrepThreads) chunk_prep_kernel(const __grid_c
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t rec = blockIdx.x, h = blockIdx.y, hq = h / (p.HV / p.H);
     __nv_bfloat16 *out = static_cast<__nv_bfloat16 *>(p.out);
+    if (h == 0) place_sequences(p, order);
 
     /* the sequence whose records hold number rec: the last one that starts at or before it */
     uint32_t t0, t1, n;
@@ -293,15 +348,16 @@ __global__ void __launch_bounds__(kPrepThreads) chunk_prep_kernel(const __grid_c
         return;
     }
     sequence_tokens(p, n, t0, t1);
-    t0 += (rec - record_of(t0, n)) * kC;
+    const uint32_t chunk = rec - record_of(t0, n);
+    t0 += chunk * kC;
     if (t0 >= t1) return;
     const uint32_t rows = min((uint32_t)kC, t1 - t0);
     uint8_t *record = records + ((size_t)rec * p.HV + h) * kRecordBytes;
 
     const __nv_bfloat16 *q = static_cast<const __nv_bfloat16 *>(p.q) + (int64_t)hq * p.q_head;
     const __nv_bfloat16 *k = static_cast<const __nv_bfloat16 *>(p.k) + (int64_t)hq * p.k_head;
-    load_rows<K>(base + L::kTile, 0, k, t0, p.k_token, rows, tid, kPrepThreads);
-    load_rows<K>(base + L::kTile, kC, q, t0, p.q_token, rows, tid, kPrepThreads);
+    load_rows<K>(base + L::kTile, kTermBytes, 0, k, t0, p.k_token, rows, tid, kPrepThreads);
+    load_rows<K>(base + L::kTile, kTermBytes, kC, q, t0, p.q_token, rows, tid, kPrepThreads);
 
     float *A = reinterpret_cast<float *>(sm + L::kA), *P = reinterpret_cast<float *>(sm + L::kP);
     float *X = reinterpret_cast<float *>(sm + L::kX), *G = reinterpret_cast<float *>(sm + L::kG);
@@ -355,6 +411,9 @@ __global__ void __launch_bounds__(kPrepThreads) chunk_prep_kernel(const __grid_c
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *slot;
+    /* not before this CTA has its TMEM: a CTA of the second kernel that took
+     * the rest would wait for this one for good */
+    pdl_launch();
     if (warp == 0 && elect_one()) {
         /* [K; Q] K^T */
         const uint32_t at = desc(base + L::kTile, 16);
@@ -465,7 +524,9 @@ __global__ void __launch_bounds__(kPrepThreads) chunk_prep_kernel(const __grid_c
     __syncthreads();
     small_product(A + 32 * kLd, A + 32 * kLd + 32, X, 32, -1.0f, tid, kPrepThreads);
     __syncthreads();
-    /* the record: rows 0..63 T, rows 64..127 P T (both lower triangular) */
+    /* the record: T in the rows of the chunk's k, P T in those of its q (both
+     * lower triangular); the two change places from chunk to chunk */
+    const uint32_t t_row = (chunk & 1) ? kC : 0, p_row = kC - t_row;
     for (uint32_t i = tid; i < kC * (kC / 4); i += kPrepThreads) {
         const uint32_t r = i / (kC / 4), c = (i % (kC / 4)) * 4;
         float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -477,87 +538,85 @@ __global__ void __launch_bounds__(kPrepThreads) chunk_prep_kernel(const __grid_c
             s.z = fmaf(x, y.z, s.z);
             s.w = fmaf(x, y.w, s.w);
         }
-        put_pair4(record, r, c, *reinterpret_cast<const float4 *>(A + r * kLd + c));
-        put_pair4(record, kC + r, c, s);
+        put_pair4(record, t_row + r, c, *reinterpret_cast<const float4 *>(A + r * kLd + c));
+        put_pair4(record, p_row + r, c, s);
     }
 }
 
 /* ----------------------------------------------------------- second kernel */
 
-/* warps 0-7 epilogues, 8 MMAs, 9 records, 10-13 loads of k and q */
-constexpr int kScanThreads = 14 * 32;
-constexpr uint32_t kLoadThreads = 128;
+/* k of two chunks and q of one share blocks of 192 rows: k of even chunks, q,
+ * k of odd chunks. An MMA's 128 rows are then [k; q] for even chunks and [q; k]
+ * for odd ones, and the lanes of an accumulator change their part likewise. */
+constexpr uint32_t kBlockRows = 3 * kC;
+constexpr uint32_t kBlock = kBlockRows * 128; /* bytes of 64 columns */
 
-template <int K>
-struct ScanSmem {
-    static constexpr uint32_t kStage = (K / 64) * kTermBytes;    /* [K; Q] */
+/* Warps: VB / 2 for the epilogues (a TMEM lane and eight value rows each
+ * thread), one for the MMAs, one for the records, four to load k and q. */
+template <int K, int VB>
+struct Scan {
+    static constexpr int kSubs = VB / 8;
+    static constexpr uint32_t kEpiWarps = 4 * kSubs;
+    static constexpr uint32_t kThreads = (kEpiWarps + 6) * 32, kLoadThreads = 128;
+    static constexpr int kMinCtas = K <= 128 && VB == 16 ? 2 : 1;
+    static constexpr int kTiles = K > 128 ? K / 128 : 1;         /* M = 128 tiles of key rows */
+    static constexpr uint32_t kAtoms = 3 * VB > 64 ? 2 : 1;      /* blocks of 64 columns of an operand of 3 VB */
+    /* shared memory */
     static constexpr uint32_t kKQ = 0;
-    static constexpr uint32_t kPair = kKQ + 2 * kStage;          /* [T; P T] */
+    static constexpr uint32_t kPair = kKQ + (K / 64) * kBlock;   /* [T; P T] */
     static constexpr uint32_t kS = kPair + kPairBytes;           /* terms of S0, rows k */
-    static constexpr uint32_t kR = kS + K * 128;                 /* terms of R, rows token */
-    static constexpr uint32_t kD = kR + kC * 128;                /* terms of the scaled D */
-    static constexpr uint32_t kBar = kD + kC * 128;
+    static constexpr uint32_t kR = kS + kAtoms * K * 128;        /* terms of R, rows token */
+    static constexpr uint32_t kD = kR + kAtoms * kC * 128;       /* terms of the scaled D */
+    static constexpr uint32_t kBar = kD + kAtoms * kC * 128;
     static constexpr uint32_t kBytes = kBar + 256 + 1024;
+    /* TMEM columns */
+    static constexpr uint32_t kD1 = 0, kD3 = 4 * VB, kD4 = 8 * VB, kD4Tile = 4 * VB;
+    static constexpr uint32_t kColumns = 16 * VB;                /* a power of two that holds them */
 };
 
-template <int K>
-__global__ void __launch_bounds__(kScanThreads, 1) chunk_scan_kernel(const __grid_constant__ DeltaParams p, const uint8_t *records,
-                                                                     uint32_t out_wide) {
-    using L = ScanSmem<K>;
-    constexpr int kTiles = K > 128 ? K / 128 : 1; /* M = 128 tiles of key rows */
+template <int K, int VB>
+__global__ void __launch_bounds__(Scan<K, VB>::kThreads, Scan<K, VB>::kMinCtas)
+    chunk_scan_kernel(const __grid_constant__ DeltaParams p, const uint8_t *records, const uint32_t *order, uint32_t out_wide) {
+    using L = Scan<K, VB>;
+    constexpr int kTiles = L::kTiles;
+    constexpr uint32_t kMmaWarp = L::kEpiWarps, kRecWarp = kMmaWarp + 1, kLoadWarp = kMmaWarp + 2;
     extern __shared__ uint8_t raw[];
     uint8_t *sm = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
     const uint32_t base = smem_u32(sm);
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const uint32_t vblocks = p.V / kVB;
-    const uint32_t n = blockIdx.x / (p.HV * vblocks), rem = blockIdx.x - n * (p.HV * vblocks);
-    const uint32_t h = rem / vblocks, v0 = (rem - h * vblocks) * kVB, hq = h / (p.HV / p.H);
+    const uint32_t vblocks = p.V / VB;
+    const uint32_t place = blockIdx.x / (p.HV * vblocks), rem = blockIdx.x - place * (p.HV * vblocks);
+    const uint32_t h = rem / vblocks, v0 = (rem - h * vblocks) * VB, hq = h / (p.HV / p.H);
     __nv_bfloat16 *out = static_cast<__nv_bfloat16 *>(p.out) + (int64_t)h * p.out_head + v0;
 
-    uint32_t t0, t1;
-    sequence_tokens(p, n, t0, t1);
-    const int64_t pool = sequence_slot(p, n);
-    const bool fresh = p.fresh != nullptr && p.fresh[n] != 0;
-    if (pool < 0) {
-        for (uint32_t i = tid; i < (t1 - t0) * kVB; i += kScanThreads)
-            out[(int64_t)(t0 + i / kVB) * p.out_token + i % kVB] = __float2bfloat16_rn(0.0f);
-        return;
-    }
-    float *S = p.state + pool * p.state_slot + ((int64_t)h * p.V + v0) * K;
-    if (t0 == t1) {
-        if (fresh)
-            for (uint32_t i = tid; i < kVB * K; i += kScanThreads) S[i] = 0.0f;
-        return;
-    }
-    const uint32_t chunks = (t1 - t0 + kC - 1) / kC, rec0 = record_of(t0, n);
-
     const uint32_t bar = base + L::kBar;
-    const uint32_t full_kq = bar, empty_k = bar + 16, empty_q = bar + 32, full_pair = bar + 48, empty_pair = bar + 56,
-                   s_ready = bar + 64, d1_full = bar + 72, r_ready = bar + 80, d3_full = bar + 88, d_ready = bar + 96,
-                   d4_full = bar + 104, drain = bar + 112;
+    const uint32_t full_kq = bar, empty_k = bar + 16, empty_q = bar + 32, full_pair = bar + 40, empty_pair = bar + 48,
+                   s_ready = bar + 56, d1_full = bar + 72, r_ready = bar + 80, d3_full = bar + 88, d_ready = bar + 96,
+                   d4_full = bar + 104, drain = bar + 120;
     uint32_t *slot = reinterpret_cast<uint32_t *>(sm + L::kBar + 128);
     volatile uint32_t *abort = reinterpret_cast<volatile uint32_t *>(sm + L::kBar + 136);
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
-            mbar_init(full_kq + 8 * i, kLoadThreads / 32);
+            mbar_init(full_kq + 8 * i, L::kLoadThreads / 32);
             mbar_init(empty_k + 8 * i, 1);
-            mbar_init(empty_q + 8 * i, 1);
+            mbar_init(s_ready + 8 * i, L::kEpiWarps);
+            mbar_init(d4_full + 8 * i, 1);
         }
+        mbar_init(empty_q, 1);
         mbar_init(full_pair, 1);
         mbar_init(empty_pair, 1);
-        mbar_init(s_ready, 8);
         mbar_init(d1_full, 1);
-        mbar_init(r_ready, 4);
+        mbar_init(r_ready, L::kEpiWarps / 2);
         mbar_init(d3_full, 1);
-        mbar_init(d_ready, 4);
-        mbar_init(d4_full, 1);
+        mbar_init(d_ready, L::kEpiWarps / 2);
         mbar_init(drain, 1);
         *abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 0) {
         __syncwarp();
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(256u)
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)),
+                     "r"(L::kColumns)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -565,27 +624,47 @@ __global__ void __launch_bounds__(kScanThreads, 1) chunk_scan_kernel(const __gri
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *slot;
-    const uint32_t d1 = tmem, d3 = tmem + 64, d4 = tmem + 128;
+    const uint32_t d1 = tmem + L::kD1, d3 = tmem + L::kD3, d4 = tmem + L::kD4;
 
-    if (warp >= 10) {
-        /* k and q of the chunks, two in flight; a stage's q rows are free once
-         * its first MMAs are done, its k rows after the last ones */
+    pdl_wait();
+    const uint32_t n = __ldcg(order + place);
+    uint32_t t0, t1;
+    sequence_tokens(p, n, t0, t1);
+    const int64_t pool = sequence_slot(p, n);
+    const bool fresh = p.fresh != nullptr && p.fresh[n] != 0;
+    float *S = p.state + (pool < 0 ? 0 : pool * p.state_slot) + ((int64_t)h * p.V + v0) * K;
+    /* no chunks, no waits: only what such a sequence leaves behind */
+    const uint32_t chunks = pool < 0 ? 0 : (t1 - t0 + kC - 1) / kC, rec0 = record_of(t0, n);
+    if (pool < 0) {
+        for (uint64_t i = tid; i < (uint64_t)(t1 - t0) * VB; i += L::kThreads)
+            out[(int64_t)(t0 + i / VB) * p.out_token + i % VB] = __float2bfloat16_rn(0.0f);
+    } else if (chunks == 0 && fresh) {
+        for (uint32_t i = tid; i < VB * K; i += L::kThreads) S[i] = 0.0f;
+    }
+
+    if (chunks == 0) {
+    } else if (warp >= kLoadWarp) {
+        /* q of a chunk once the first MMAs of the chunk before have read
+         * theirs, k two chunks after the same rows' last MMAs */
         const __nv_bfloat16 *q = static_cast<const __nv_bfloat16 *>(p.q) + (int64_t)hq * p.q_head;
         const __nv_bfloat16 *k = static_cast<const __nv_bfloat16 *>(p.k) + (int64_t)hq * p.k_head;
-        const uint32_t th = tid - 10 * 32;
+        const uint32_t th = tid - kLoadWarp * 32;
+        load_rows<K>(base + L::kKQ, kBlock, 0, k, t0, p.k_token, min((uint32_t)kC, t1 - t0), th, L::kLoadThreads);
         for (uint32_t c = 0; c < chunks; ++c) {
-            const uint32_t st = c & 1, tile = base + L::kKQ + st * L::kStage;
-            const uint32_t tc = t0 + c * kC, rows = min((uint32_t)kC, t1 - tc);
-            if (c >= 2 && !wait_bar_warp(empty_q + 8 * st, ((c >> 1) - 1) & 1u, abort)) break;
-            load_rows<K>(tile, kC, q, tc, p.q_token, rows, th, kLoadThreads);
-            if (c >= 2 && !wait_bar_warp(empty_k + 8 * st, ((c >> 1) - 1) & 1u, abort)) break;
-            load_rows<K>(tile, 0, k, tc, p.k_token, rows, th, kLoadThreads);
+            const uint32_t tc = t0 + c * kC;
+            if (c >= 1 && !wait_bar_warp(empty_q, (c - 1) & 1u, abort)) break;
+            load_rows<K>(base + L::kKQ, kBlock, kC, q, tc, p.q_token, min((uint32_t)kC, t1 - tc), th, L::kLoadThreads);
             cp_async_wait_all();
             fence_async();
-            warp_arrive(full_kq + 8 * st);
+            warp_arrive(full_kq + 8 * (c & 1));
+            if (c + 1 < chunks) {
+                const uint32_t st = (c + 1) & 1, tn = tc + kC;
+                if (c >= 1 && !wait_bar_warp(empty_k + 8 * st, ((c - 1) >> 1) & 1u, abort)) break;
+                load_rows<K>(base + L::kKQ, kBlock, st * 2 * kC, k, tn, p.k_token, min((uint32_t)kC, t1 - tn), th, L::kLoadThreads);
+            }
         }
         cp_async_wait_all();
-    } else if (warp == 9) {
+    } else if (warp == kRecWarp) {
         if (lane == 0) {
             uint32_t c = 0;
             for (; c < chunks; ++c) {
@@ -604,25 +683,36 @@ __global__ void __launch_bounds__(kScanThreads, 1) chunk_scan_kernel(const __gri
             while (!mbar_try(full_pair, (c - 1) & 1u) && gtimer() - w0 < kWaitNs) {
             }
         }
-    } else if (warp == 8) {
+    } else if (warp == kMmaWarp) {
         /* the whole warp walks along, so that what the MMAs take stays in
          * uniform registers; one lane issues */
         const uint32_t leader = elect_one();
-        const uint32_t s_desc = desc(base + L::kS, 1024), r_desc = desc(base + L::kR, 1024), x_desc = desc(base + L::kD, 1024),
-                       pair_desc = desc(base + L::kPair, 16);
+        const uint32_t s_desc = desc(base + L::kS, K * 128), r_desc = desc(base + L::kR, kC * 128),
+                       x_desc = desc(base + L::kD, kC * 128), pair_desc = desc(base + L::kPair, 16);
+        constexpr uint32_t kAll = 3 * VB, kTwo = 2 * VB;
         for (uint32_t c = 0; c < chunks; ++c) {
-            const uint32_t st = c & 1, ph = c & 1, tile = base + L::kKQ + st * L::kStage;
-            if (!wait_bar_warp(full_kq + 8 * st, (c >> 1) & 1u, abort) || !wait_bar_warp(s_ready, ph, abort)) break;
-            tc_fence_after();
-            if (leader) {
-                /* [K; Q] S0^T */
-                const uint32_t a = desc(tile, 16);
+            const uint32_t st = c & 1, ph = c & 1;
+            const uint32_t rows = base + L::kKQ + st * kC * 128;      /* [k; q] or [q; k] */
+            const uint32_t k_rows = base + L::kKQ + st * 2 * kC * 128;
+            if (!wait_bar_warp(full_kq + 8 * st, (c >> 1) & 1u, abort)) break;
+            /* [K; Q] S0^T, 128 key rows at a time as the state's terms get ready */
+            bool ok = true;
 #pragma unroll
-                for (int kk = 0; kk < K / 16; ++kk)
-                    mma(d1, a + (((kk / 4) * kTermBytes + (kk % 4) * 32) >> 4), s_desc + ((kk * 2048) >> 4),
-                        instr_desc(128, 3 * kVB, false, true), kk != 0);
+            for (int t = 0; t < kTiles && ok; ++t) {
+                ok = wait_bar_warp(s_ready + 8 * t, ph, abort);
+                tc_fence_after();
+                if (ok && leader) {
+                    const uint32_t a = desc(rows, 16);
+#pragma unroll
+                    for (int kk = t * (K / 16 / kTiles); kk < (t + 1) * (K / 16 / kTiles); ++kk)
+                        mma(d1, a + (((kk / 4) * kBlock + (kk % 4) * 32) >> 4), s_desc + ((kk * 2048) >> 4),
+                            instr_desc(128, kAll, false, true), kk != 0);
+                }
+            }
+            if (!ok) break;
+            if (leader) {
                 commit(d1_full);
-                commit(empty_q + 8 * st);
+                commit(empty_q);
             }
             if (!wait_bar_warp(full_pair, ph, abort) || !wait_bar_warp(r_ready, ph, abort)) break;
             tc_fence_after();
@@ -630,27 +720,27 @@ __global__ void __launch_bounds__(kScanThreads, 1) chunk_scan_kernel(const __gri
                 /* [T; P T] R: the first term with all of R, the second with R's first two */
 #pragma unroll
                 for (int kk = 0; kk < kC / 16; ++kk)
-                    mma(d3, pair_desc + ((kk * 32) >> 4), r_desc + ((kk * 2048) >> 4), instr_desc(128, 3 * kVB, false, true),
-                        kk != 0);
+                    mma(d3, pair_desc + ((kk * 32) >> 4), r_desc + ((kk * 2048) >> 4), instr_desc(128, kAll, false, true), kk != 0);
 #pragma unroll
                 for (int kk = 0; kk < kC / 16; ++kk)
                     mma(d3, pair_desc + ((kTermBytes + kk * 32) >> 4), r_desc + ((kk * 2048) >> 4),
-                        instr_desc(128, 2 * kVB, false, true), true);
+                        instr_desc(128, kTwo, false, true), true);
                 commit(d3_full);
                 commit(empty_pair);
             }
             if (!wait_bar_warp(d_ready, ph, abort)) break;
             tc_fence_after();
             if (leader) {
-                /* K^T D (64 key rows: the upper half of M runs into the q rows and is not read) */
-                const uint32_t a = desc(tile, K >= 128 ? kTermBytes : kTermBytes / 2);
+                /* K^T D (64 key rows: the upper half of M runs into other rows and is not read) */
+                const uint32_t a = desc(k_rows, K >= 128 ? kBlock : kC * 128);
 #pragma unroll
-                for (int t = 0; t < kTiles; ++t)
+                for (int t = 0; t < kTiles; ++t) {
 #pragma unroll
                     for (int kk = 0; kk < kC / 16; ++kk)
-                        mma(d4 + 64 * t, a + ((t * 2 * kTermBytes + kk * 2048) >> 4), x_desc + ((kk * 2048) >> 4),
-                            instr_desc(128, 3 * kVB, true, true), kk != 0);
-                commit(d4_full);
+                        mma(d4 + L::kD4Tile * t, a + ((t * 2 * kBlock + kk * 2048) >> 4), x_desc + ((kk * 2048) >> 4),
+                            instr_desc(128, kAll, true, true), kk != 0);
+                    commit(d4_full + 8 * t);
+                }
                 commit(empty_k + 8 * st);
             }
         }
@@ -662,45 +752,47 @@ __global__ void __launch_bounds__(kScanThreads, 1) chunk_scan_kernel(const __gri
             }
         }
     } else {
-        /* epilogues: thread = TMEM lane (token of [K; Q], or key row) and eight
+        /* epilogues: thread = TMEM lane (token of k or q, or key row) and eight
          * of the value rows */
-        const uint32_t ln = 32 * (warp & 3) + lane, half = warp >> 2;
-        const uint32_t at = ((32 * (warp & 3)) << 16) + 8 * half;
-        const bool is_o = ln >= kC; /* uniform in a warp */
+        const uint32_t ln = 32 * (warp & 3) + lane, sub = warp >> 2;
+        const uint32_t at = ((32 * (warp & 3)) << 16) + 8 * sub;
         const uint32_t i = ln & (kC - 1);
-        const __nv_bfloat16 *v = static_cast<const __nv_bfloat16 *>(p.v) + (int64_t)h * p.v_head + v0 + 8 * half;
+        const __nv_bfloat16 *v = static_cast<const __nv_bfloat16 *>(p.v) + (int64_t)h * p.v_head + v0 + 8 * sub;
         const bool has_s = K >= 128 || ln < (uint32_t)K;
         float s[kTiles][8];
 #pragma unroll
         for (int t = 0; t < kTiles; ++t)
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-                s[t][e] = (has_s && !fresh) ? S[(int64_t)(8 * half + e) * K + 128 * t + ln] : 0.0f;
+                s[t][e] = (has_s && !fresh) ? S[(int64_t)(8 * sub + e) * K + 128 * t + ln] : 0.0f;
         struct {
             float f0, f1, f2, decay;
             uint4 v;
         } next;
+        /* in a chunk, whether this lane is a token of q (uniform in a warp) */
+        auto is_q = [&](uint32_t c) { return (ln >= (uint32_t)kC) != ((c & 1) != 0); };
         auto fetch = [&](uint32_t c) {
             const float *sc = reinterpret_cast<const float *>(records + ((size_t)(rec0 + c) * p.HV + h) * kRecordBytes + kPairBytes);
             const uint32_t t = t0 + c * kC + i;
-            next.decay = sc[kScalDecay * kC];
-            next.f0 = sc[(is_o ? kScalQ : kScalC) * kC + i];
-            next.f1 = sc[kScalBeta * kC + i];
-            next.f2 = sc[kScalEnd * kC + i];
+            const bool q = is_q(c);
+            next.decay = __ldcg(sc + kScalDecay * kC);
+            next.f0 = __ldcg(sc + (q ? kScalQ : kScalC) * kC + i);
+            next.f1 = __ldcg(sc + kScalBeta * kC + i);
+            next.f2 = __ldcg(sc + kScalEnd * kC + i);
             next.v = make_uint4(0, 0, 0, 0);
-            if (!is_o && t < t1) next.v = *reinterpret_cast<const uint4 *>(v + (int64_t)t * p.v_token);
+            if (!q && t < t1) next.v = *reinterpret_cast<const uint4 *>(v + (int64_t)t * p.v_token);
         };
         fetch(0);
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) {
+            if (has_s) put_terms<VB>(sm + L::kS, K, 128 * t + ln, sub, s[t]);
+            fence_async();
+            warp_arrive(s_ready + 8 * t);
+        }
         bool ok = true;
         for (uint32_t c = 0; c < chunks; ++c) {
             const uint32_t ph = c & 1, tc = t0 + c * kC, rows = min((uint32_t)kC, t1 - tc);
-            if (has_s) {
-#pragma unroll
-                for (int t = 0; t < kTiles; ++t) put_terms(sm + L::kS, 128 * t + ln, half, s[t]);
-            }
-            fence_async();
-            tc_fence_before();
-            warp_arrive(s_ready);
+            const bool q = is_q(c);
             /* this chunk's scalars and values were requested a chunk ago; now the next one's */
             const float f0 = next.f0, f1 = next.f1, f2 = next.f2, decay = next.decay;
             const uint4 vw = next.v;
@@ -708,8 +800,8 @@ __global__ void __launch_bounds__(kScanThreads, 1) chunk_scan_kernel(const __gri
             float x[8], o[8];
             if (!(ok = wait_bar_warp(d1_full, ph, abort))) break;
             tc_fence_after();
-            tc_sum3(d1 + at, x);
-            if (is_o) {
+            tc_sum3<VB>(d1 + at, x);
+            if (q) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) o[e] = f0 * x[e];
             } else {
@@ -719,17 +811,17 @@ __global__ void __launch_bounds__(kScanThreads, 1) chunk_scan_kernel(const __gri
                     const float vv = __uint_as_float((e & 1) ? (u[e >> 1] & 0xFFFF0000u) : (u[e >> 1] << 16));
                     x[e] = i < rows ? f1 * fmaf(-f0, x[e], vv) : 0.0f;
                 }
-                put_terms(sm + L::kR, i, half, x);
+                put_terms<VB>(sm + L::kR, kC, i, sub, x);
                 fence_async();
                 tc_fence_before();
                 warp_arrive(r_ready);
             }
             if (!(ok = wait_bar_warp(d3_full, ph, abort))) break;
             tc_fence_after();
-            tc_sum3(d3 + at, x);
-            if (is_o) {
+            tc_sum3<VB>(d3 + at, x);
+            if (q) {
                 if (i < rows) {
-                    __nv_bfloat16 *dst = out + (int64_t)(tc + i) * p.out_token + 8 * half;
+                    __nv_bfloat16 *dst = out + (int64_t)(tc + i) * p.out_token + 8 * sub;
 #pragma unroll
                     for (int e = 0; e < 8; ++e) o[e] += x[e];
                     if (out_wide) {
@@ -743,65 +835,93 @@ __global__ void __launch_bounds__(kScanThreads, 1) chunk_scan_kernel(const __gri
             } else {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) x[e] *= f2;
-                put_terms(sm + L::kD, i, half, x);
+                put_terms<VB>(sm + L::kD, kC, i, sub, x);
                 fence_async();
                 tc_fence_before();
                 warp_arrive(d_ready);
             }
-            if (!(ok = wait_bar_warp(d4_full, ph, abort))) break;
-            tc_fence_after();
 #pragma unroll
             for (int t = 0; t < kTiles; ++t) {
-                tc_sum3(d4 + 64 * t + at, x);
+                if (!(ok = wait_bar_warp(d4_full + 8 * t, ph, abort))) break;
+                tc_fence_after();
+                tc_sum3<VB>(d4 + L::kD4Tile * t + at, x);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) s[t][e] = fmaf(decay, s[t][e], x[e]);
+                if (c + 1 < chunks) {
+                    if (has_s) put_terms<VB>(sm + L::kS, K, 128 * t + ln, sub, s[t]);
+                    fence_async();
+                    tc_fence_before();
+                    warp_arrive(s_ready + 8 * t);
+                }
             }
+            if (!ok) break;
         }
         if (has_s) {
             /* a sequence that was given up leaves no state that could pass for one */
-            const float bad = ok ? 0.0f : __int_as_float(0x7fc00000);
+            const float bad = __int_as_float(0x7fc00000);
 #pragma unroll
             for (int t = 0; t < kTiles; ++t)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) S[(int64_t)(8 * half + e) * K + 128 * t + ln] = ok ? s[t][e] : bad;
+                for (int e = 0; e < 8; ++e) S[(int64_t)(8 * sub + e) * K + 128 * t + ln] = ok ? s[t][e] : bad;
         }
     }
     tc_fence_before();
     __syncthreads();
     if (warp == 0) {
         tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(256u) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(L::kColumns) : "memory");
     }
 }
 
+/* bytes of the order of N sequences, before the records */
+size_t order_bytes(uint32_t sequences) { return ((size_t)sequences * 4 + 255) & ~(size_t)255; }
 uint32_t record_count(uint32_t tokens, uint32_t sequences) { return tokens / kC + sequences + 2; }
 
+template <int K, int VB>
+cudaError_t launch_scan(const DeltaParams &p, const uint8_t *records, const uint32_t *order, cudaStream_t stream) {
+    using L = Scan<K, VB>;
+    cudaError_t e = cudaFuncSetAttribute(chunk_scan_kernel<K, VB>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::kBytes);
+    if (e != cudaSuccess) return e;
+    const uint32_t wide = (reinterpret_cast<uintptr_t>(p.out) & 15) == 0 && p.out_token % 8 == 0 && p.out_head % 8 == 0;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(p.N * p.HV * (p.V / VB));
+    cfg.blockDim = dim3(L::kThreads);
+    cfg.dynamicSmemBytes = L::kBytes;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, chunk_scan_kernel<K, VB>, p, records, order, wide);
+}
+
 template <int K>
-cudaError_t launch_chunk_k(const DeltaParams &p, uint8_t *records, cudaStream_t stream) {
+cudaError_t launch_chunk_k(const DeltaParams &p, uint8_t *workspace, int sms, cudaStream_t stream) {
+    uint32_t *order = reinterpret_cast<uint32_t *>(workspace);
+    uint8_t *records = workspace + order_bytes(p.N);
     cudaError_t e = cudaFuncSetAttribute(chunk_prep_kernel<K>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          (int)PrepSmem<K>::kBytes);
     if (e != cudaSuccess) return e;
-    e = cudaFuncSetAttribute(chunk_scan_kernel<K>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ScanSmem<K>::kBytes);
-    if (e != cudaSuccess) return e;
-    chunk_prep_kernel<K><<<dim3(record_count(p.tokens, p.N), p.HV), kPrepThreads, PrepSmem<K>::kBytes, stream>>>(p, records);
+    chunk_prep_kernel<K><<<dim3(record_count(p.tokens, p.N), p.HV), kPrepThreads, PrepSmem<K>::kBytes, stream>>>(p, records, order);
     if ((e = cudaGetLastError()) != cudaSuccess) return e;
-    const bool wide = (reinterpret_cast<uintptr_t>(p.out) & 15) == 0 && p.out_token % 8 == 0 && p.out_head % 8 == 0;
-    chunk_scan_kernel<K><<<p.N * p.HV * (p.V / kVB), kScanThreads, ScanSmem<K>::kBytes, stream>>>(p, records, wide);
-    return cudaGetLastError();
+    const uint32_t ctas16 = p.N * p.HV * (p.V / 16);
+    if (ctas16 > (uint32_t)sms) return launch_scan<K, 32>(p, records, order, stream);
+    return launch_scan<K, 16>(p, records, order, stream);
 }
 
 }  // namespace
 
 size_t delta_chunk_workspace(uint32_t tokens, uint32_t sequences, uint32_t v_heads) {
-    return (size_t)record_count(tokens, sequences) * v_heads * kRecordBytes;
+    return order_bytes(sequences) + (size_t)record_count(tokens, sequences) * v_heads * kRecordBytes;
 }
 
-cudaError_t launch_delta_chunk(const DeltaParams &p, void *workspace, cudaStream_t stream) {
-    uint8_t *records = static_cast<uint8_t *>(workspace);
+cudaError_t launch_delta_chunk(const DeltaParams &p, void *workspace, int sms, cudaStream_t stream) {
+    uint8_t *w = static_cast<uint8_t *>(workspace);
     switch (p.K) {
-        case 64: return launch_chunk_k<64>(p, records, stream);
-        case 128: return launch_chunk_k<128>(p, records, stream);
-        default: return launch_chunk_k<256>(p, records, stream);
+        case 64: return launch_chunk_k<64>(p, w, sms, stream);
+        case 128: return launch_chunk_k<128>(p, w, sms, stream);
+        default: return launch_chunk_k<256>(p, w, sms, stream);
     }
 }
 

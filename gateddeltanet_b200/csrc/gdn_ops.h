@@ -71,7 +71,7 @@ constexpr uint32_t kMaxVocab = 1u << 18;
 cudaError_t launch_delta_step(const DeltaParams &p, bool bf16, int sms, cudaStream_t stream);
 /* The chunked form (gdn_delta_chunk.cu): BF16, 16-byte aligned rows. */
 size_t delta_chunk_workspace(uint32_t tokens, uint32_t sequences, uint32_t v_heads);
-cudaError_t launch_delta_chunk(const DeltaParams &p, void *workspace, cudaStream_t stream);
+cudaError_t launch_delta_chunk(const DeltaParams &p, void *workspace, int sms, cudaStream_t stream);
 /* *status != 0: a wait of such a kernel on the current device ran out since
  * the last call. They synchronise. */
 cudaError_t delta_step_status(int *status);

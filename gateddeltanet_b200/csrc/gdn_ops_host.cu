@@ -134,8 +134,9 @@ int gdn_b200_delta_chunk(const GdnB200DeltaArgs *args) {
     if (args->workspace == nullptr || !aligned(args->workspace, 256) || args->workspace_bytes < need)
         return failf("gdn_b200_delta_chunk: a workspace of %zu bytes on a 256-byte boundary is needed", need);
     DeviceScope scope(args->device);
-    if (!scope.ok) return failf("gdn_b200_delta_chunk: cannot use device %d", args->device);
-    const cudaError_t e = gdn::ops::launch_delta_chunk(p, args->workspace, static_cast<cudaStream_t>(args->stream));
+    const int sms = scope.ok ? sm_count(args->device) : 0;
+    if (sms == 0) return failf("gdn_b200_delta_chunk: cannot use device %d", args->device);
+    const cudaError_t e = gdn::ops::launch_delta_chunk(p, args->workspace, sms, static_cast<cudaStream_t>(args->stream));
     return e == cudaSuccess ? 0 : failf("gdn_b200_delta_chunk: launch failed: %s", cudaGetErrorString(e));
 }
 
