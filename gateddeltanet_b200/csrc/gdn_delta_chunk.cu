@@ -75,11 +75,18 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
         : "memory");
     return ok != 0;
 }
-/* Bounded wait; false when the CTA gives up (here or elsewhere). */
+/* Bounded wait; false when the CTA gives up (here or elsewhere). The clock and
+ * the other warps' word are looked at now and then: they cost issue slots that
+ * the epilogues need. kPause: nobody waits for this warp to wake at once. */
+template <bool kPause = false>
 __device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, volatile uint32_t *abort) {
     if (mbar_try(bar, parity)) return true;
     const uint64_t t0 = gtimer();
-    while (!mbar_try(bar, parity)) {
+    while (true) {
+        if (kPause) __nanosleep(100);
+#pragma unroll 1
+        for (int i = 0; i < 16; ++i)
+            if (mbar_try(bar, parity)) return true;
         if (*abort) return false;
         if (gtimer() - t0 > kWaitNs) {
             *abort = 1;
@@ -87,11 +94,11 @@ __device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, volatile
             return false;
         }
     }
-    return true;
 }
 /* the same for a whole warp, with one answer */
+template <bool kPause = false>
 __device__ __forceinline__ bool wait_bar_warp(uint32_t bar, uint32_t parity, volatile uint32_t *abort) {
-    return __all_sync(0xffffffffu, wait_bar(bar, parity, abort));
+    return __all_sync(0xffffffffu, wait_bar<kPause>(bar, parity, abort));
 }
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -150,6 +157,23 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+/* x = f s + x */
+__device__ __forceinline__ void decay_add(float f, const float (&s)[8], float (&x)[8]) {
+    const uint64_t ff = pack2(__float_as_uint(f), __float_as_uint(f));
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+        uint32_t lo, hi;
+        unpack2(fma2(ff, pack2(__float_as_uint(s[i]), __float_as_uint(s[i + 1])),
+                     pack2(__float_as_uint(x[i]), __float_as_uint(x[i + 1]))), lo, hi);
+        x[i] = __uint_as_float(lo);
+        x[i + 1] = __uint_as_float(hi);
+    }
+}
 /* the sums of the three terms' columns (VB apart): eight value rows starting at addr */
 template <int VB>
 __device__ __forceinline__ void tc_sum3(uint32_t addr, float (&x)[8]) {
@@ -206,17 +230,27 @@ __device__ __forceinline__ void put_terms(uint8_t *base, uint32_t rows, uint32_t
 /* `rows` tokens from t0 on of one head (zeros up to 64) as the rows `first`
  * .. first + 63 of blocks of 64 columns (`block` bytes apart) in the 128-byte
  * swizzle */
-template <int K>
-__device__ __forceinline__ void load_rows(uint32_t tile, uint32_t block, uint32_t first, const __nv_bfloat16 *x, int64_t t0, int64_t stride,
-                                          uint32_t rows, uint32_t thread, uint32_t threads) {
-    constexpr uint32_t kPieces = K / 8;
-#pragma unroll 8
-    for (uint32_t i = thread; i < kC * kPieces; i += threads) {
-        const uint32_t r = i / kPieces, c = i % kPieces;
-        const uint32_t dst = tile + (c >> 3) * block + piece_at(first + r, c & 7);
-        const __nv_bfloat16 *src = r < rows ? x + (t0 + r) * stride + c * 8 : x;
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(r < rows ? 16u : 0u)
-                     : "memory");
+template <int K, uint32_t kThreads>
+__device__ __forceinline__ void load_rows(uint32_t tile, uint32_t block, uint32_t first, const __nv_bfloat16 *x, int64_t t0,
+                                          int64_t stride, uint32_t rows, uint32_t thread) {
+    /* a thread keeps its piece of a row and goes down in steps of a multiple
+     * of eight rows, so that its place in the swizzle stays the same */
+    constexpr uint32_t kPieces = K / 8, kWide = kPieces < kThreads / 8 ? kPieces : kThreads / 8, kStep = kThreads / kWide;
+    static_assert(kStep % 8 == 0 && kPieces % kWide == 0 && kC % kStep == 0, "loader shape");
+    const uint32_t r0 = thread / kWide;
+#pragma unroll
+    for (uint32_t c0 = 0; c0 < kPieces; c0 += kWide) {
+        const uint32_t c = c0 + thread % kWide;
+        uint32_t dst = tile + (c >> 3) * block + piece_at(first + r0, c & 7);
+        const __nv_bfloat16 *src = x + (t0 + r0) * stride + c * 8;
+#pragma unroll
+        for (uint32_t r = 0; r < kC; r += kStep) {
+            const bool there = r0 + r < rows;
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(there ? src : x), "r"(there ? 16u : 0u)
+                         : "memory");
+            dst += kStep * 128;
+            src += kStep * stride;
+        }
     }
 }
 __device__ __forceinline__ void cp_async_wait_all() {
@@ -260,34 +294,59 @@ __device__ __forceinline__ void place_sequences(const DeltaParams &p, uint32_t *
 constexpr int kPrepThreads = 256;
 constexpr uint32_t kLd = kC + 4; /* row stride of the FP32 matrices, floats */
 
+/* The FP32 matrices take the place of [K; Q] once the MMAs and the norms have
+ * read it, so that three CTAs share an SM. */
 template <int K>
 struct PrepSmem {
     static constexpr uint32_t kTile = 0;                                  /* [K; Q] */
-    static constexpr uint32_t kA = kTile + (K / 64) * kTermBytes;         /* A, then T */
+    static constexpr uint32_t kA = 0;                                     /* A, then T */
     static constexpr uint32_t kP = kA + kC * kLd * 4;
     static constexpr uint32_t kX = kP + kC * kLd * 4;                     /* products of the inversion */
-    static constexpr uint32_t kG = kX + 32 * kLd * 4;                     /* G hi, lo, beta, inverse norms of k, q */
-    static constexpr uint32_t kBar = kG + 5 * kC * 4;
+    static constexpr uint32_t kMat = kX + 32 * kLd * 4;
+    static constexpr uint32_t kG = (K / 64) * kTermBytes > kMat ? (K / 64) * kTermBytes : kMat;
+    static constexpr uint32_t kRows = 7;                                  /* G hi, lo, beta, norms of k, q, two of decays */
+    static constexpr uint32_t kBar = kG + kRows * kC * 4;
     static constexpr uint32_t kBytes = kBar + 32 + 1024;                  /* room to align */
 };
 
-/* out[r][c] (m x m, at out) = sign * a[m x m] b[m x m], all in rows of kLd;
- * the threads of a group of `threads` take one element group each */
+/* out (2 x 4 values at row r, column c) = sign * sum over j in [j0, j1) of
+ * a[r][j] b[j][c], j0 and j1 multiples of 4; rows of kLd */
+__device__ __forceinline__ void product_2x4(const float *a, const float *b, int r, int c, int j0, int j1, float (&s)[2][4]) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[u][e] = 0.0f;
+#pragma unroll 2
+    for (int j = j0; j < j1; j += 4) {
+        const float4 x0 = *reinterpret_cast<const float4 *>(a + r * kLd + j);
+        const float4 x1 = *reinterpret_cast<const float4 *>(a + (r + 1) * kLd + j);
+        const float x[2][4] = {{x0.x, x0.y, x0.z, x0.w}, {x1.x, x1.y, x1.z, x1.w}};
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+            const float4 y = *reinterpret_cast<const float4 *>(b + (j + d) * kLd + c);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                s[u][0] = fmaf(x[u][d], y.x, s[u][0]);
+                s[u][1] = fmaf(x[u][d], y.y, s[u][1]);
+                s[u][2] = fmaf(x[u][d], y.z, s[u][2]);
+                s[u][3] = fmaf(x[u][d], y.w, s[u][3]);
+            }
+        }
+    }
+}
+/* out (m x m) = sign * a b for `threads` threads, where either a (kLeft) or b
+ * is lower triangular */
+template <bool kLeft>
 __device__ __forceinline__ void small_product(float *out, const float *a, const float *b, int m, float sign, int thread,
                                               int threads) {
-    for (int i = thread; i < m * (m / 4); i += threads) {
-        const int r = i / (m / 4), c = (i % (m / 4)) * 4;
-        float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-        for (int j = 0; j < m; ++j) {
-            const float x = a[r * kLd + j];
-            const float4 y = *reinterpret_cast<const float4 *>(b + j * kLd + c);
-            s.x = fmaf(x, y.x, s.x);
-            s.y = fmaf(x, y.y, s.y);
-            s.z = fmaf(x, y.z, s.z);
-            s.w = fmaf(x, y.w, s.w);
-        }
-        *reinterpret_cast<float4 *>(out + r * kLd + c) = make_float4(sign * s.x, sign * s.y, sign * s.z, sign * s.w);
+    for (int i = thread; i < (m / 2) * (m / 4); i += threads) {
+        const int r = (i / (m / 4)) * 2, c = (i % (m / 4)) * 4;
+        float s[2][4];
+        product_2x4(a, b, r, c, kLeft ? 0 : c, kLeft ? (r + 5) & ~3 : m, s);
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+            *reinterpret_cast<float4 *>(out + (r + u) * kLd + c) =
+                make_float4(sign * s[u][0], sign * s[u][1], sign * s[u][2], sign * s[u][3]);
     }
 }
 
@@ -302,7 +361,7 @@ __device__ __forceinline__ void put_pair4(uint8_t *rec, uint32_t row, uint32_t c
 }
 
 template <int K>
-__global__ void __launch_bounds__(kPrepThreads) chunk_prep_kernel(const __grid_constant__ DeltaParams p, uint8_t *records, uint32_t *order) {
+__global__ void __launch_bounds__(kPrepThreads, 3) chunk_prep_kernel(const __grid_constant__ DeltaParams p, uint8_t *records, uint32_t *order) {
     using L = PrepSmem<K>;
     extern __shared__ uint8_t raw[];
     uint8_t *sm = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
@@ -356,12 +415,12 @@ __global__ void __launch_bounds__(kPrepThreads) chunk_prep_kernel(const __grid_c
 
     const __nv_bfloat16 *q = static_cast<const __nv_bfloat16 *>(p.q) + (int64_t)hq * p.q_head;
     const __nv_bfloat16 *k = static_cast<const __nv_bfloat16 *>(p.k) + (int64_t)hq * p.k_head;
-    load_rows<K>(base + L::kTile, kTermBytes, 0, k, t0, p.k_token, rows, tid, kPrepThreads);
-    load_rows<K>(base + L::kTile, kTermBytes, kC, q, t0, p.q_token, rows, tid, kPrepThreads);
+    load_rows<K, kPrepThreads>(base + L::kTile, kTermBytes, 0, k, t0, p.k_token, rows, tid);
+    load_rows<K, kPrepThreads>(base + L::kTile, kTermBytes, kC, q, t0, p.q_token, rows, tid);
 
     float *A = reinterpret_cast<float *>(sm + L::kA), *P = reinterpret_cast<float *>(sm + L::kP);
     float *X = reinterpret_cast<float *>(sm + L::kX), *G = reinterpret_cast<float *>(sm + L::kG);
-    float *Glo = G + kC, *bet = G + 2 * kC, *kin = G + 3 * kC, *qin = G + 4 * kC;
+    float *Glo = G + kC, *bet = G + 2 * kC, *kin = G + 3 * kC, *qin = G + 4 * kC, *dec_i = G + 5 * kC, *dec_j = G + 6 * kC;
     const uint32_t bar = base + L::kBar;
     uint32_t *slot = reinterpret_cast<uint32_t *>(sm + L::kBar + 8);
     volatile uint32_t *abort = reinterpret_cast<volatile uint32_t *>(sm + L::kBar + 16);
@@ -458,30 +517,48 @@ __global__ void __launch_bounds__(kPrepThreads) chunk_prep_kernel(const __grid_c
         sc[kScalQ * kC + tid] = eg * qin[tid];
         sc[kScalEnd * kC + tid] = there ? expf((G[kC - 1] - G[tid]) + (Glo[kC - 1] - Glo[tid])) * kin[tid] : 0.0f;
         if (tid == kC - 1) sc[kScalDecay * kC] = eg;
+        /* the two factors of the decays between the halves of the chunk */
+        if (tid < 32)
+            dec_j[tid] = expf((G[32] - G[tid]) + (Glo[32] - Glo[tid])) * kin[tid];
+        else
+            dec_i[tid] = expf((G[tid] - G[32]) + (Glo[tid] - Glo[32]));
     }
     bool ok = wait_bar_warp(bar, 0, abort);
     tc_fence_after();
+    __syncthreads(); /* the norms are taken, the MMAs done: [K; Q] may go */
     if (ok) {
-        /* lanes 0..63: rows of A; 64..127: rows of P; warps 4..7 take columns 32..63 */
+        /* lanes 0..63: rows of A; 64..127: rows of P; warps 4..7 take columns
+         * 32..63. e^(G_i - G_j) of the lower left quarter is the product of
+         * e^(G_i - G_32) and e^(G_32 - G_j), neither above 1 where nothing
+         * grows; the upper right one is zero. */
         const uint32_t row = 32 * (warp & 3) + lane, i = row & (kC - 1), c0 = (warp >> 2) * 32;
-        const bool is_p = row >= kC;
-        const float gi = G[i], gl = Glo[i], f = is_p ? qin[i] : bet[i] * kin[i];
-        float *dst = (is_p ? P : A) + i * kLd;
+        const bool is_p = row >= kC, low = i >= 32, left = c0 == 0; /* uniform in a warp */
+        const float gi = G[i], gl = Glo[i];
+        float f = is_p ? qin[i] : bet[i] * kin[i];
+        if (low && left) f *= dec_i[i];
+        float *dst = (is_p ? P : A) + i * kLd + c0;
 #pragma unroll
         for (int c = 0; c < 32; c += 8) {
             uint32_t r[8];
-            __syncwarp();
-            tc_ld8(tmem + ((32 * (warp & 3)) << 16) + c0 + c, r);
-            tc_wait();
+            float x[8];
+            if (low || left) {
+                __syncwarp();
+                tc_ld8(tmem + ((32 * (warp & 3)) << 16) + c0 + c, r);
+                tc_wait();
+            }
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 const uint32_t j = c0 + c + e;
-                float x = 0.0f;
-                if (j < i || (is_p && j == i))
-                    x = f * kin[j] * expf((gi - G[j]) + (gl - Glo[j])) * __uint_as_float(r[e]);
-                if (!is_p && j == i) x = 1.0f;
-                dst[j] = x;
+                if (low && left)
+                    x[e] = f * dec_j[j] * __uint_as_float(r[e]);
+                else if (low || left)
+                    x[e] = j < i || (is_p && j == i) ? f * kin[j] * expf((gi - G[j]) + (gl - Glo[j])) * __uint_as_float(r[e])
+                                                      : (j == i ? 1.0f : 0.0f);
+                else
+                    x[e] = 0.0f;
             }
+            *reinterpret_cast<float4 *>(dst + c) = make_float4(x[0], x[1], x[2], x[3]);
+            *reinterpret_cast<float4 *>(dst + c + 4) = make_float4(x[4], x[5], x[6], x[7]);
         }
     }
     tc_fence_before();
@@ -515,31 +592,29 @@ __global__ void __launch_bounds__(kPrepThreads) chunk_prep_kernel(const __grid_c
         /* two blocks of 32: half of the threads each */
         const int b = tid >> 7, th = tid & 127;
         float *D = A + (32 * b) * kLd + 32 * b, *Y = X + (16 * b) * kLd;
-        small_product(Y, D + 16 * kLd, D, 16, 1.0f, th, 128);
+        small_product<false>(Y, D + 16 * kLd, D, 16, 1.0f, th, 128);
         __syncthreads();
-        small_product(D + 16 * kLd, D + 16 * kLd + 16, Y, 16, -1.0f, th, 128);
+        small_product<true>(D + 16 * kLd, D + 16 * kLd + 16, Y, 16, -1.0f, th, 128);
     }
     __syncthreads();
-    small_product(X, A + 32 * kLd, A, 32, 1.0f, tid, kPrepThreads);
+    small_product<false>(X, A + 32 * kLd, A, 32, 1.0f, tid, kPrepThreads);
     __syncthreads();
-    small_product(A + 32 * kLd, A + 32 * kLd + 32, X, 32, -1.0f, tid, kPrepThreads);
+    small_product<true>(A + 32 * kLd, A + 32 * kLd + 32, X, 32, -1.0f, tid, kPrepThreads);
     __syncthreads();
     /* the record: T in the rows of the chunk's k, P T in those of its q (both
      * lower triangular); the two change places from chunk to chunk */
     const uint32_t t_row = (chunk & 1) ? kC : 0, p_row = kC - t_row;
-    for (uint32_t i = tid; i < kC * (kC / 4); i += kPrepThreads) {
-        const uint32_t r = i / (kC / 4), c = (i % (kC / 4)) * 4;
-        float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (uint32_t j = c; j <= r; ++j) {
-            const float x = P[r * kLd + j];
-            const float4 y = *reinterpret_cast<const float4 *>(A + j * kLd + c);
-            s.x = fmaf(x, y.x, s.x);
-            s.y = fmaf(x, y.y, s.y);
-            s.z = fmaf(x, y.z, s.z);
-            s.w = fmaf(x, y.w, s.w);
+    for (uint32_t i = tid; i < (kC / 2) * (kC / 4); i += kPrepThreads) {
+        /* rows that share a warp need sums of about one length: 16 columns of
+         * threads, the rows in pairs downwards */
+        const uint32_t r = (i / (kC / 4)) * 2, c = (i % (kC / 4)) * 4;
+        float s[2][4];
+        product_2x4(P, A, (int)r, (int)c, (int)c, ((int)r + 5) & ~3, s);
+#pragma unroll
+        for (uint32_t u = 0; u < 2; ++u) {
+            put_pair4(record, t_row + r + u, c, *reinterpret_cast<const float4 *>(A + (r + u) * kLd + c));
+            put_pair4(record, p_row + r + u, c, make_float4(s[u][0], s[u][1], s[u][2], s[u][3]));
         }
-        put_pair4(record, t_row + r, c, *reinterpret_cast<const float4 *>(A + r * kLd + c));
-        put_pair4(record, p_row + r, c, s);
     }
 }
 
@@ -649,18 +724,18 @@ __global__ void __launch_bounds__(Scan<K, VB>::kThreads, Scan<K, VB>::kMinCtas)
         const __nv_bfloat16 *q = static_cast<const __nv_bfloat16 *>(p.q) + (int64_t)hq * p.q_head;
         const __nv_bfloat16 *k = static_cast<const __nv_bfloat16 *>(p.k) + (int64_t)hq * p.k_head;
         const uint32_t th = tid - kLoadWarp * 32;
-        load_rows<K>(base + L::kKQ, kBlock, 0, k, t0, p.k_token, min((uint32_t)kC, t1 - t0), th, L::kLoadThreads);
+        load_rows<K, L::kLoadThreads>(base + L::kKQ, kBlock, 0, k, t0, p.k_token, min((uint32_t)kC, t1 - t0), th);
         for (uint32_t c = 0; c < chunks; ++c) {
             const uint32_t tc = t0 + c * kC;
-            if (c >= 1 && !wait_bar_warp(empty_q, (c - 1) & 1u, abort)) break;
-            load_rows<K>(base + L::kKQ, kBlock, kC, q, tc, p.q_token, min((uint32_t)kC, t1 - tc), th, L::kLoadThreads);
+            if (c >= 1 && !wait_bar_warp<true>(empty_q, (c - 1) & 1u, abort)) break;
+            load_rows<K, L::kLoadThreads>(base + L::kKQ, kBlock, kC, q, tc, p.q_token, min((uint32_t)kC, t1 - tc), th);
             cp_async_wait_all();
             fence_async();
             warp_arrive(full_kq + 8 * (c & 1));
             if (c + 1 < chunks) {
                 const uint32_t st = (c + 1) & 1, tn = tc + kC;
-                if (c >= 1 && !wait_bar_warp(empty_k + 8 * st, ((c - 1) >> 1) & 1u, abort)) break;
-                load_rows<K>(base + L::kKQ, kBlock, st * 2 * kC, k, tn, p.k_token, min((uint32_t)kC, t1 - tn), th, L::kLoadThreads);
+                if (c >= 1 && !wait_bar_warp<true>(empty_k + 8 * st, ((c - 1) >> 1) & 1u, abort)) break;
+                load_rows<K, L::kLoadThreads>(base + L::kKQ, kBlock, st * 2 * kC, k, tn, p.k_token, min((uint32_t)kC, t1 - tn), th);
             }
         }
         cp_async_wait_all();
@@ -668,7 +743,7 @@ __global__ void __launch_bounds__(Scan<K, VB>::kThreads, Scan<K, VB>::kMinCtas)
         if (lane == 0) {
             uint32_t c = 0;
             for (; c < chunks; ++c) {
-                if (c >= 1 && !wait_bar(empty_pair, (c - 1) & 1u, abort)) break;
+                if (c >= 1 && !wait_bar<true>(empty_pair, (c - 1) & 1u, abort)) break;
                 const uint8_t *src = records + ((size_t)(rec0 + c) * p.HV + h) * kRecordBytes;
                 asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(full_pair), "r"(kPairBytes)
                              : "memory");
@@ -845,8 +920,9 @@ __global__ void __launch_bounds__(Scan<K, VB>::kThreads, Scan<K, VB>::kMinCtas)
                 if (!(ok = wait_bar_warp(d4_full + 8 * t, ph, abort))) break;
                 tc_fence_after();
                 tc_sum3<VB>(d4 + L::kD4Tile * t + at, x);
+                decay_add(decay, s[t], x);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) s[t][e] = fmaf(decay, s[t][e], x[e]);
+                for (int e = 0; e < 8; ++e) s[t][e] = x[e];
                 if (c + 1 < chunks) {
                     if (has_s) put_terms<VB>(sm + L::kS, K, 128 * t + ln, sub, s[t]);
                     fence_async();
