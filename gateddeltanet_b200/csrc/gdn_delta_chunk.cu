@@ -350,6 +350,18 @@ __device__ __forceinline__ void small_product(float *out, const float *a, const 
     }
 }
 
+__device__ __forceinline__ void load8(const float *p, float (&x)[8]) {
+    const float4 a = *reinterpret_cast<const float4 *>(p), b = *reinterpret_cast<const float4 *>(p + 4);
+    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+}
+__device__ __forceinline__ void store8(float *p, const float (&x)[8]) {
+    *reinterpret_cast<float4 *>(p) = make_float4(x[0], x[1], x[2], x[3]);
+    *reinterpret_cast<float4 *>(p + 4) = make_float4(x[4], x[5], x[6], x[7]);
+}
+/* e^x for a decay: the product with log2 e rounds by 2^-24 |x|, and
+ * |x| e^x stays below 0.37 */
+__device__ __forceinline__ float decay_exp(float x) { return exp2f(x * 1.4426950408889634f); }
+
 /* four values of row `row` as two BF16 terms of the record's [T; P T] */
 __device__ __forceinline__ void put_pair4(uint8_t *rec, uint32_t row, uint32_t col, float4 x) {
     const uint32_t w0 = bf16_pair(x.x, x.y), w1 = bf16_pair(x.z, x.w);
@@ -431,7 +443,7 @@ __global__ void __launch_bounds__(kPrepThreads, 3) chunk_prep_kernel(const __gri
     }
     if (warp == 0) {
         __syncwarp();
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(64u)
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(128u)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -474,39 +486,37 @@ __global__ void __launch_bounds__(kPrepThreads, 3) chunk_prep_kernel(const __gri
      * the rest would wait for this one for good */
     pdl_launch();
     if (warp == 0 && elect_one()) {
-        /* [K; Q] K^T */
+        /* [K; Q] [K; Q]^T: the first 64 columns are wanted, and the diagonal for the norms */
         const uint32_t at = desc(base + L::kTile, 16);
 #pragma unroll
         for (int kk = 0; kk < K / 16; ++kk) {
             const uint32_t off = ((kk / 4) * kTermBytes + (kk % 4) * 32) >> 4;
-            mma(tmem, at + off, at + off, instr_desc(2 * kC, kC, false, false), kk != 0);
+            mma(tmem, at + off, at + off, instr_desc(2 * kC, 2 * kC, false, false), kk != 0);
         }
         commit(bar);
     }
-    /* norms meanwhile: two lanes per row */
-    {
-        const uint32_t r = tid >> 1; /* 0..127: K rows, then Q rows */
+    const bool ok = wait_bar_warp(bar, 0, abort);
+    tc_fence_after();
+    if (warp < 4) {
+        /* warp w: rows and columns 32 w .. 32 w + 31 */
         float ss = 0.0f;
-        for (uint32_t c = tid & 1; c < K / 8; c += 2) {
-            const uint4 w = *reinterpret_cast<const uint4 *>(sm + L::kTile + (c >> 3) * kTermBytes + piece_at(r, c & 7));
-            const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float a = __uint_as_float(u[i] << 16), b = __uint_as_float(u[i] & 0xFFFF0000u);
-                ss = fmaf(a, a, ss);
-                ss = fmaf(b, b, ss);
-            }
+        for (int c = 0; c < 32; c += 8) {
+            uint32_t r[8];
+            __syncwarp();
+            tc_ld8(tmem + ((32 * warp) << 16) + 32 * warp + c, r);
+            tc_wait();
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if ((int)lane == c + e) ss = __uint_as_float(r[e]);
         }
-        ss += __shfl_xor_sync(0xffffffffu, ss, 1);
         const float inv = p.normalize ? 1.0f / sqrtf(ss + 1e-6f) : 1.0f;
-        if ((tid & 1) == 0) {
-            if (r < kC)
-                kin[r] = inv;
-            else
-                qin[r - kC] = inv * p.scale;
-        }
+        if (warp < 2)
+            kin[tid] = inv;
+        else
+            qin[tid - kC] = inv * p.scale;
     }
-    __syncthreads();
+    __syncthreads(); /* [K; Q] has been read: the matrices may take its place */
     /* the record's rows of scalars */
     if (tid < kC) {
         float *sc = reinterpret_cast<float *>(record + kPairBytes);
@@ -523,9 +533,7 @@ __global__ void __launch_bounds__(kPrepThreads, 3) chunk_prep_kernel(const __gri
         else
             dec_i[tid] = expf((G[tid] - G[32]) + (Glo[tid] - Glo[32]));
     }
-    bool ok = wait_bar_warp(bar, 0, abort);
-    tc_fence_after();
-    __syncthreads(); /* the norms are taken, the MMAs done: [K; Q] may go */
+    __syncthreads();
     if (ok) {
         /* lanes 0..63: rows of A; 64..127: rows of P; warps 4..7 take columns
          * 32..63. e^(G_i - G_j) of the lower left quarter is the product of
@@ -537,36 +545,46 @@ __global__ void __launch_bounds__(kPrepThreads, 3) chunk_prep_kernel(const __gri
         float f = is_p ? qin[i] : bet[i] * kin[i];
         if (low && left) f *= dec_i[i];
         float *dst = (is_p ? P : A) + i * kLd + c0;
+        if (low && left) {
 #pragma unroll
-        for (int c = 0; c < 32; c += 8) {
-            uint32_t r[8];
-            float x[8];
-            if (low || left) {
+            for (int c = 0; c < 32; c += 8) {
+                uint32_t r[8];
+                float dj[8], x[8];
+                load8(dec_j + c, dj);
+                __syncwarp();
+                tc_ld8(tmem + ((32 * (warp & 3)) << 16) + c, r);
+                tc_wait();
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = f * dj[e] * __uint_as_float(r[e]);
+                store8(dst + c, x);
+            }
+        } else if (low || left) {
+            const int last = (int)(i - c0) - (is_p ? 0 : 1); /* the last column with a product */
+#pragma unroll
+            for (int c = 0; c < 32; c += 8) {
+                uint32_t r[8];
+                float gj[8], lj[8], kj[8], x[8];
+                load8(G + c0 + c, gj);
+                load8(Glo + c0 + c, lj);
+                load8(kin + c0 + c, kj);
                 __syncwarp();
                 tc_ld8(tmem + ((32 * (warp & 3)) << 16) + c0 + c, r);
                 tc_wait();
-            }
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const uint32_t j = c0 + c + e;
-                if (low && left)
-                    x[e] = f * dec_j[j] * __uint_as_float(r[e]);
-                else if (low || left)
-                    x[e] = j < i || (is_p && j == i) ? f * kin[j] * expf((gi - G[j]) + (gl - Glo[j])) * __uint_as_float(r[e])
-                                                      : (j == i ? 1.0f : 0.0f);
-                else
-                    x[e] = 0.0f;
+                for (int e = 0; e < 8; ++e) {
+                    const float y = f * kj[e] * decay_exp((gi - gj[e]) + (gl - lj[e])) * __uint_as_float(r[e]);
+                    x[e] = c + e <= last ? y : (!is_p && c + e == last + 1 ? 1.0f : 0.0f);
+                }
+                store8(dst + c, x);
             }
-            *reinterpret_cast<float4 *>(dst + c) = make_float4(x[0], x[1], x[2], x[3]);
-            *reinterpret_cast<float4 *>(dst + c + 4) = make_float4(x[4], x[5], x[6], x[7]);
+        } else {
+            const float x[8] = {};
+#pragma unroll
+            for (int c = 0; c < 32; c += 8) store8(dst + c, x);
         }
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 0) {
-        tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(64u) : "memory");
-    }
     /* T = (I + A)^-1 in place: the 16 x 16 diagonal blocks by forward
      * substitution (a lane per column), then twice
      * [[a 0] [c b]]^-1 = [[a^-1 0] [-b^-1 c a^-1, b^-1]] */
@@ -615,6 +633,10 @@ __global__ void __launch_bounds__(kPrepThreads, 3) chunk_prep_kernel(const __gri
             put_pair4(record, t_row + r + u, c, *reinterpret_cast<const float4 *>(A + (r + u) * kLd + c));
             put_pair4(record, p_row + r + u, c, make_float4(s[u][0], s[u][1], s[u][2], s[u][3]));
         }
+    }
+    if (warp == 0) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(128u) : "memory");
     }
 }
 
