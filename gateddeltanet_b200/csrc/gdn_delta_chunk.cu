@@ -37,11 +37,11 @@ constexpr int kC = 64;      /* tokens of a chunk */
 constexpr uint64_t kWaitNs = 2000000000ull;
 
 /* per (chunk, value head): [T; P T] as two BF16 terms in the MMA's layout,
- * then five rows of 64 floats */
+ * then four rows of 64 floats and the chunk's decay */
 constexpr uint32_t kTermBytes = 2 * kC * 128;       /* 128 rows of 64 BF16 */
 constexpr uint32_t kPairBytes = 2 * kTermBytes;
-constexpr uint32_t kScalBytes = 5 * kC * 4;
-constexpr uint32_t kRecordBytes = kPairBytes + kScalBytes;
+constexpr uint32_t kScalBytes = (4 * kC + 4) * 4;
+constexpr uint32_t kRecordBytes = (kPairBytes + kScalBytes + 127) & ~127u;
 enum { kScalC = 0, kScalBeta = 1, kScalQ = 2, kScalEnd = 3, kScalDecay = 4 };
 
 /* set when a wait of a kernel ran out; read and cleared by the host */
@@ -162,17 +162,19 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
     return r;
 }
-/* x = f s + x */
-__device__ __forceinline__ void decay_add(float f, const float (&s)[8], float (&x)[8]) {
-    const uint64_t ff = pack2(__float_as_uint(f), __float_as_uint(f));
+__device__ __forceinline__ uint64_t pack2(float lo, float hi) { return pack2(__float_as_uint(lo), __float_as_uint(hi)); }
+__device__ __forceinline__ void unpack2(uint64_t v, float &lo, float &hi) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+/* y = f x + y and y = x + y */
+__device__ __forceinline__ void scale_add(float f, const float (&x)[8], float (&y)[8]) {
+    const uint64_t ff = pack2(f, f);
 #pragma unroll
-    for (int i = 0; i < 8; i += 2) {
-        uint32_t lo, hi;
-        unpack2(fma2(ff, pack2(__float_as_uint(s[i]), __float_as_uint(s[i + 1])),
-                     pack2(__float_as_uint(x[i]), __float_as_uint(x[i + 1]))), lo, hi);
-        x[i] = __uint_as_float(lo);
-        x[i + 1] = __uint_as_float(hi);
-    }
+    for (int i = 0; i < 8; i += 2) unpack2(fma2(ff, pack2(x[i], x[i + 1]), pack2(y[i], y[i + 1])), y[i], y[i + 1]);
+}
+__device__ __forceinline__ void add_to(const float (&x)[8], float (&y)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) unpack2(add2(pack2(x[i], x[i + 1]), pack2(y[i], y[i + 1])), y[i], y[i + 1]);
 }
 /* the sums of the three terms' columns (VB apart): eight value rows starting at addr */
 template <int VB>
@@ -184,12 +186,8 @@ __device__ __forceinline__ void tc_sum3(uint32_t addr, float (&x)[8]) {
     tc_ld8(addr + 2 * VB, c);
     tc_wait();
 #pragma unroll
-    for (int i = 0; i < 8; i += 2) {
-        uint32_t lo, hi;
-        unpack2(add2(pack2(a[i], a[i + 1]), add2(pack2(b[i], b[i + 1]), pack2(c[i], c[i + 1]))), lo, hi);
-        x[i] = __uint_as_float(lo);
-        x[i + 1] = __uint_as_float(hi);
-    }
+    for (int i = 0; i < 8; i += 2)
+        unpack2(add2(pack2(a[i], a[i + 1]), add2(pack2(b[i], b[i + 1]), pack2(c[i], c[i + 1]))), x[i], x[i + 1]);
 }
 
 /* 16-byte piece `piece` of row `row` in the 128-byte swizzle */
@@ -649,12 +647,15 @@ constexpr uint32_t kBlockRows = 3 * kC;
 constexpr uint32_t kBlock = kBlockRows * 128; /* bytes of 64 columns */
 
 /* Warps: VB / 2 for the epilogues (a TMEM lane and eight value rows each
- * thread), one for the MMAs, one for the records, four to load k and q. */
+ * thread), one for the MMAs, one for the records, two to load k and q. That
+ * makes 20 for 32 value rows, five for each part of the SM, with 96 registers a
+ * thread: at 22 they had 80, spilled the next chunk's values and so waited for
+ * them (7000 cycles a chunk). */
 template <int K, int VB>
 struct Scan {
     static constexpr int kSubs = VB / 8;
     static constexpr uint32_t kEpiWarps = 4 * kSubs;
-    static constexpr uint32_t kThreads = (kEpiWarps + 6) * 32, kLoadThreads = 128;
+    static constexpr uint32_t kThreads = (kEpiWarps + 4) * 32, kLoadThreads = 64;
     static constexpr int kMinCtas = K <= 128 && VB == 16 ? 2 : 1;
     static constexpr int kTiles = K > 128 ? K / 128 : 1;         /* M = 128 tiles of key rows */
     static constexpr uint32_t kAtoms = 3 * VB > 64 ? 2 : 1;      /* blocks of 64 columns of an operand of 3 VB */
@@ -664,8 +665,9 @@ struct Scan {
     static constexpr uint32_t kS = kPair + kPairBytes;           /* terms of S0, rows k */
     static constexpr uint32_t kR = kS + kAtoms * K * 128;        /* terms of R, rows token */
     static constexpr uint32_t kD = kR + kAtoms * kC * 128;       /* terms of the scaled D */
-    static constexpr uint32_t kBar = kD + kAtoms * kC * 128;
-    static constexpr uint32_t kBytes = kBar + 256 + 1024;
+    static constexpr uint32_t kScal = kD + kAtoms * kC * 128;    /* rows of scalars of two chunks */
+    static constexpr uint32_t kBar = kScal + 2 * kScalBytes;
+    static constexpr uint32_t kBytes = kBar + 192; /* the kernel has no other shared memory: its base is aligned */
     /* TMEM columns */
     static constexpr uint32_t kD1 = 0, kD3 = 4 * VB, kD4 = 8 * VB, kD4Tile = 4 * VB;
     static constexpr uint32_t kColumns = 16 * VB;                /* a power of two that holds them */
@@ -677,9 +679,13 @@ __global__ void __launch_bounds__(Scan<K, VB>::kThreads, Scan<K, VB>::kMinCtas)
     using L = Scan<K, VB>;
     constexpr int kTiles = L::kTiles;
     constexpr uint32_t kMmaWarp = L::kEpiWarps, kRecWarp = kMmaWarp + 1, kLoadWarp = kMmaWarp + 2;
-    extern __shared__ uint8_t raw[];
-    uint8_t *sm = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
+    extern __shared__ __align__(1024) uint8_t sm[];
     const uint32_t base = smem_u32(sm);
+    if (base & 1023u) {
+        /* the swizzle would not be where the MMAs look for it */
+        atomicExch(&g_chunk_status, 1);
+        return;
+    }
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t vblocks = p.V / VB;
     const uint32_t place = blockIdx.x / (p.HV * vblocks), rem = blockIdx.x - place * (p.HV * vblocks);
@@ -689,11 +695,12 @@ __global__ void __launch_bounds__(Scan<K, VB>::kThreads, Scan<K, VB>::kMinCtas)
     const uint32_t bar = base + L::kBar;
     const uint32_t full_kq = bar, empty_k = bar + 16, empty_q = bar + 32, full_pair = bar + 40, empty_pair = bar + 48,
                    s_ready = bar + 56, d1_full = bar + 72, r_ready = bar + 80, d3_full = bar + 88, d_ready = bar + 96,
-                   d4_full = bar + 104, drain = bar + 120;
-    uint32_t *slot = reinterpret_cast<uint32_t *>(sm + L::kBar + 128);
-    volatile uint32_t *abort = reinterpret_cast<volatile uint32_t *>(sm + L::kBar + 136);
+                   d4_full = bar + 104, drain = bar + 120, full_scal = bar + 128;
+    uint32_t *slot = reinterpret_cast<uint32_t *>(sm + L::kBar + 144);
+    volatile uint32_t *abort = reinterpret_cast<volatile uint32_t *>(sm + L::kBar + 152);
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
+            mbar_init(full_scal + 8 * i, 1);
             mbar_init(full_kq + 8 * i, L::kLoadThreads / 32);
             mbar_init(empty_k + 8 * i, 1);
             mbar_init(s_ready + 8 * i, L::kEpiWarps);
@@ -763,21 +770,30 @@ __global__ void __launch_bounds__(Scan<K, VB>::kThreads, Scan<K, VB>::kMinCtas)
         cp_async_wait_all();
     } else if (warp == kRecWarp) {
         if (lane == 0) {
+            /* a chunk's scalars may take the place of those of two chunks
+             * before: [T; P T] of the chunk between has been used */
+            auto copy = [&](uint32_t dst, const uint8_t *src, uint32_t bytes, uint32_t full) {
+                asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(full), "r"(bytes) : "memory");
+                asm volatile(
+                    "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+                    "l"(src), "r"(bytes), "r"(full)
+                    : "memory");
+            };
             uint32_t c = 0;
             for (; c < chunks; ++c) {
                 if (c >= 1 && !wait_bar<true>(empty_pair, (c - 1) & 1u, abort)) break;
                 const uint8_t *src = records + ((size_t)(rec0 + c) * p.HV + h) * kRecordBytes;
-                asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(full_pair), "r"(kPairBytes)
-                             : "memory");
-                asm volatile(
-                    "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                        base + L::kPair),
-                    "l"(src), "r"(kPairBytes), "r"(full_pair)
-                    : "memory");
+                if (c == 0) copy(base + L::kScal, src + kPairBytes, kScalBytes, full_scal);
+                copy(base + L::kPair, src, kPairBytes, full_pair);
+                if (c + 1 < chunks)
+                    copy(base + L::kScal + ((c + 1) & 1) * kScalBytes, src + (size_t)p.HV * kRecordBytes + kPairBytes, kScalBytes,
+                         full_scal + 8 * ((c + 1) & 1));
             }
-            /* the last copy lands before the CTA ends (an abort does not stop it) */
+            /* the last copies land before the CTA ends (an abort does not stop them) */
             const uint64_t w0 = gtimer();
-            while (!mbar_try(full_pair, (c - 1) & 1u) && gtimer() - w0 < kWaitNs) {
+            while (!(mbar_try(full_pair, (c - 1) & 1u) &&
+                     mbar_try(full_scal + 8 * (min(c, chunks - 1) & 1), (min(c, chunks - 1) >> 1) & 1u)) &&
+                   gtimer() - w0 < kWaitNs) {
             }
         }
     } else if (warp == kMmaWarp) {
@@ -862,22 +878,14 @@ __global__ void __launch_bounds__(Scan<K, VB>::kThreads, Scan<K, VB>::kMinCtas)
 #pragma unroll
             for (int e = 0; e < 8; ++e)
                 s[t][e] = (has_s && !fresh) ? S[(int64_t)(8 * sub + e) * K + 128 * t + ln] : 0.0f;
-        struct {
-            float f0, f1, f2, decay;
-            uint4 v;
-        } next;
         /* in a chunk, whether this lane is a token of q (uniform in a warp) */
         auto is_q = [&](uint32_t c) { return (ln >= (uint32_t)kC) != ((c & 1) != 0); };
+        /* the lane's value rows of a chunk, requested one chunk ahead */
+        uint4 next = make_uint4(0, 0, 0, 0);
         auto fetch = [&](uint32_t c) {
-            const float *sc = reinterpret_cast<const float *>(records + ((size_t)(rec0 + c) * p.HV + h) * kRecordBytes + kPairBytes);
             const uint32_t t = t0 + c * kC + i;
-            const bool q = is_q(c);
-            next.decay = __ldcg(sc + kScalDecay * kC);
-            next.f0 = __ldcg(sc + (q ? kScalQ : kScalC) * kC + i);
-            next.f1 = __ldcg(sc + kScalBeta * kC + i);
-            next.f2 = __ldcg(sc + kScalEnd * kC + i);
-            next.v = make_uint4(0, 0, 0, 0);
-            if (!q && t < t1) next.v = *reinterpret_cast<const uint4 *>(v + (int64_t)t * p.v_token);
+            next = make_uint4(0, 0, 0, 0);
+            if (!is_q(c) && t < t1) next = *reinterpret_cast<const uint4 *>(v + (int64_t)t * p.v_token);
         };
         fetch(0);
 #pragma unroll
@@ -890,10 +898,25 @@ __global__ void __launch_bounds__(Scan<K, VB>::kThreads, Scan<K, VB>::kMinCtas)
         for (uint32_t c = 0; c < chunks; ++c) {
             const uint32_t ph = c & 1, tc = t0 + c * kC, rows = min((uint32_t)kC, t1 - tc);
             const bool q = is_q(c);
-            /* this chunk's scalars and values were requested a chunk ago; now the next one's */
-            const float f0 = next.f0, f1 = next.f1, f2 = next.f2, decay = next.decay;
-            const uint4 vw = next.v;
+            const float *sc = reinterpret_cast<const float *>(sm + L::kScal + ph * kScalBytes);
+            if (!(ok = wait_bar_warp(full_scal + 8 * ph, (c >> 1) & 1u, abort))) break;
+            const float decay = sc[kScalDecay * kC], f2 = sc[kScalEnd * kC + i];
+            /* what does not need the MMAs' results: beta v, and the decayed state */
+            float bv[8], f0;
+            if (q) {
+                f0 = sc[kScalQ * kC + i];
+            } else {
+                const float beta = sc[kScalBeta * kC + i];
+                const uint32_t u[4] = {next.x, next.y, next.z, next.w};
+                f0 = -beta * sc[kScalC * kC + i];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) bv[e] = beta * __uint_as_float((e & 1) ? (u[e >> 1] & 0xFFFF0000u) : (u[e >> 1] << 16));
+            }
             if (c + 1 < chunks) fetch(c + 1);
+#pragma unroll
+            for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) s[t][e] *= decay;
             float x[8], o[8];
             if (!(ok = wait_bar_warp(d1_full, ph, abort))) break;
             tc_fence_after();
@@ -902,13 +925,9 @@ __global__ void __launch_bounds__(Scan<K, VB>::kThreads, Scan<K, VB>::kMinCtas)
 #pragma unroll
                 for (int e = 0; e < 8; ++e) o[e] = f0 * x[e];
             } else {
-                const uint32_t u[4] = {vw.x, vw.y, vw.z, vw.w};
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float vv = __uint_as_float((e & 1) ? (u[e >> 1] & 0xFFFF0000u) : (u[e >> 1] << 16));
-                    x[e] = i < rows ? f1 * fmaf(-f0, x[e], vv) : 0.0f;
-                }
-                put_terms<VB>(sm + L::kR, kC, i, sub, x);
+                /* rows without a token have zeros for all of it */
+                scale_add(f0, x, bv);
+                put_terms<VB>(sm + L::kR, kC, i, sub, bv);
                 fence_async();
                 tc_fence_before();
                 warp_arrive(r_ready);
@@ -942,9 +961,7 @@ __global__ void __launch_bounds__(Scan<K, VB>::kThreads, Scan<K, VB>::kMinCtas)
                 if (!(ok = wait_bar_warp(d4_full + 8 * t, ph, abort))) break;
                 tc_fence_after();
                 tc_sum3<VB>(d4 + L::kD4Tile * t + at, x);
-                decay_add(decay, s[t], x);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) s[t][e] = x[e];
+                add_to(x, s[t]);
                 if (c + 1 < chunks) {
                     if (has_s) put_terms<VB>(sm + L::kS, K, 128 * t + ln, sub, s[t]);
                     fence_async();
