@@ -149,9 +149,6 @@ __device__ __forceinline__ uint64_t pack2(uint32_t lo, uint32_t hi) {
     asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
     return r;
 }
-__device__ __forceinline__ void unpack2(uint64_t v, uint32_t &lo, uint32_t &hi) {
-    asm("mov.b64 {%0, %1}, %2;" : "=r"(lo), "=r"(hi) : "l"(v));
-}
 __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     uint64_t r;
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
@@ -654,7 +651,7 @@ __global__ void __launch_bounds__(kPrepThreads, 3) chunk_prep_kernel(const __gri
 constexpr uint32_t kBlockRows = 3 * kC;
 constexpr uint32_t kBlock = kBlockRows * 128; /* bytes of 64 columns */
 
-/* Warps: VB / 2 for the epilogues (a TMEM lane and eight value rows each
+/* Warps: up to 16 for the epilogues (a TMEM lane and eight value rows each
  * thread), one for the MMAs, one for the records, two to load k and q. That
  * makes 20 for 32 value rows, five for each part of the SM, with 96 registers a
  * thread: at 22 they had 80, spilled the next chunk's values and so waited for
@@ -662,10 +659,13 @@ constexpr uint32_t kBlock = kBlockRows * 128; /* bytes of 64 columns */
 template <int K, int VB>
 struct Scan {
     static constexpr int kSubs = VB / 8;
-    static constexpr uint32_t kEpiWarps = 4 * kSubs;
+    static constexpr int kTiles = K > 128 ? K / 128 : 1;         /* M = 128 tiles of key rows */
+    /* 16 value rows leave room for warps of their own for each tile of the
+     * state; the tokens are the first group's */
+    static constexpr int kGroups = VB == 16 ? kTiles : 1, kOwn = kTiles / kGroups;
+    static constexpr uint32_t kTokenWarps = 4 * kSubs, kEpiWarps = kTokenWarps * kGroups;
     static constexpr uint32_t kThreads = (kEpiWarps + 4) * 32, kLoadThreads = 64;
     static constexpr int kMinCtas = K <= 128 && VB == 16 ? 2 : 1;
-    static constexpr int kTiles = K > 128 ? K / 128 : 1;         /* M = 128 tiles of key rows */
     static constexpr uint32_t kAtoms = 3 * VB > 64 ? 2 : 1;      /* blocks of 64 columns of an operand of 3 VB */
     /* shared memory */
     static constexpr uint32_t kKQ = 0;
@@ -711,16 +711,16 @@ __global__ void __launch_bounds__(Scan<K, VB>::kThreads, Scan<K, VB>::kMinCtas)
             mbar_init(full_scal + 8 * i, 1);
             mbar_init(full_kq + 8 * i, L::kLoadThreads / 32);
             mbar_init(empty_k + 8 * i, 1);
-            mbar_init(s_ready + 8 * i, L::kEpiWarps);
+            mbar_init(s_ready + 8 * i, L::kTokenWarps);
             mbar_init(d4_full + 8 * i, 1);
         }
         mbar_init(empty_q, 1);
         mbar_init(full_pair, 1);
         mbar_init(empty_pair, 1);
         mbar_init(d1_full, 1);
-        mbar_init(r_ready, L::kEpiWarps / 2);
+        mbar_init(r_ready, L::kTokenWarps / 2);
         mbar_init(d3_full, 1);
-        mbar_init(d_ready, L::kEpiWarps / 2);
+        mbar_init(d_ready, L::kTokenWarps / 2);
         mbar_init(drain, 1);
         *abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -875,17 +875,18 @@ __global__ void __launch_bounds__(Scan<K, VB>::kThreads, Scan<K, VB>::kMinCtas)
     } else {
         /* epilogues: thread = TMEM lane (token of k or q, or key row) and eight
          * of the value rows */
-        const uint32_t ln = 32 * (warp & 3) + lane, sub = warp >> 2;
+        const uint32_t ln = 32 * (warp & 3) + lane, sub = (warp >> 2) % L::kSubs, group = warp / L::kTokenWarps;
         const uint32_t at = ((32 * (warp & 3)) << 16) + 8 * sub;
         const uint32_t i = ln & (kC - 1);
         const __nv_bfloat16 *v = static_cast<const __nv_bfloat16 *>(p.v) + (int64_t)h * p.v_head + v0 + 8 * sub;
         const bool has_s = K >= 128 || ln < (uint32_t)K;
-        float s[kTiles][8];
+        const uint32_t tile0 = group * L::kOwn; /* this warp's tiles of the state */
+        float s[L::kOwn][8];
 #pragma unroll
-        for (int t = 0; t < kTiles; ++t)
+        for (int t = 0; t < L::kOwn; ++t)
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-                s[t][e] = (has_s && !fresh) ? S[(int64_t)(8 * sub + e) * K + 128 * t + ln] : 0.0f;
+                s[t][e] = (has_s && !fresh) ? S[(int64_t)(8 * sub + e) * K + 128 * (tile0 + t) + ln] : 0.0f;
         /* in a chunk, whether this lane is a token of q (uniform in a warp) */
         auto is_q = [&](uint32_t c) { return (ln >= (uint32_t)kC) != ((c & 1) != 0); };
         /* the lane's value rows of a chunk, requested one chunk ahead */
@@ -897,10 +898,10 @@ __global__ void __launch_bounds__(Scan<K, VB>::kThreads, Scan<K, VB>::kMinCtas)
         };
         fetch(0);
 #pragma unroll
-        for (int t = 0; t < kTiles; ++t) {
-            if (has_s) put_terms<VB>(sm + L::kS, K, 128 * t + ln, sub, s[t]);
+        for (int t = 0; t < L::kOwn; ++t) {
+            if (has_s) put_terms<VB>(sm + L::kS, K, 128 * (tile0 + t) + ln, sub, s[t]);
             fence_async();
-            warp_arrive(s_ready + 8 * t);
+            warp_arrive(s_ready + 8 * (tile0 + t));
         }
         bool ok = true;
         for (uint32_t c = 0; c < chunks; ++c) {
@@ -909,72 +910,75 @@ __global__ void __launch_bounds__(Scan<K, VB>::kThreads, Scan<K, VB>::kMinCtas)
             const float *sc = reinterpret_cast<const float *>(sm + L::kScal + ph * kScalBytes);
             if (!(ok = wait_bar_warp(full_scal + 8 * ph, (c >> 1) & 1u, abort))) break;
             const float decay = sc[kScalDecay * kC], f2 = sc[kScalEnd * kC + i];
-            /* what does not need the MMAs' results: beta v, and the decayed state */
-            float bv[8], f0;
-            if (q) {
-                f0 = sc[kScalQ * kC + i];
-            } else {
-                const float beta = sc[kScalBeta * kC + i];
-                const uint32_t u[4] = {next.x, next.y, next.z, next.w};
-                f0 = -beta * sc[kScalC * kC + i];
+            /* the decayed state, and beta v, do not wait for the MMAs */
 #pragma unroll
-                for (int e = 0; e < 8; ++e) bv[e] = beta * __uint_as_float((e & 1) ? (u[e >> 1] & 0xFFFF0000u) : (u[e >> 1] << 16));
-            }
-            if (c + 1 < chunks) fetch(c + 1);
-#pragma unroll
-            for (int t = 0; t < kTiles; ++t)
+            for (int t = 0; t < L::kOwn; ++t)
 #pragma unroll
                 for (int e = 0; e < 8; ++e) s[t][e] *= decay;
-            float x[8], o[8];
-            if (!(ok = wait_bar_warp(d1_full, ph, abort))) break;
-            tc_fence_after();
-            tc_sum3<VB>(d1 + at, x);
-            if (q) {
+            float x[8];
+            if (group == 0) {
+                float bv[8], f0;
+                if (q) {
+                    f0 = sc[kScalQ * kC + i];
+                } else {
+                    const float beta = sc[kScalBeta * kC + i];
+                    const uint32_t u[4] = {next.x, next.y, next.z, next.w};
+                    f0 = -beta * sc[kScalC * kC + i];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) o[e] = f0 * x[e];
-            } else {
-                /* rows without a token have zeros for all of it */
-                scale_add(f0, x, bv);
-                put_terms<VB>(sm + L::kR, kC, i, sub, bv);
-                fence_async();
-                tc_fence_before();
-                warp_arrive(r_ready);
-            }
-            if (!(ok = wait_bar_warp(d3_full, ph, abort))) break;
-            tc_fence_after();
-            tc_sum3<VB>(d3 + at, x);
-            if (q) {
-                if (i < rows) {
-                    __nv_bfloat16 *dst = out + (int64_t)(tc + i) * p.out_token + 8 * sub;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) o[e] += x[e];
-                    if (out_wide) {
-                        *reinterpret_cast<uint4 *>(dst) = make_uint4(bf16_pair(o[0], o[1]), bf16_pair(o[2], o[3]),
-                                                                     bf16_pair(o[4], o[5]), bf16_pair(o[6], o[7]));
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) dst[e] = __float2bfloat16_rn(o[e]);
-                    }
+                    for (int e = 0; e < 8; ++e) bv[e] = beta * __uint_as_float((e & 1) ? (u[e >> 1] & 0xFFFF0000u) : (u[e >> 1] << 16));
                 }
-            } else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] *= f2;
-                put_terms<VB>(sm + L::kD, kC, i, sub, x);
-                fence_async();
-                tc_fence_before();
-                warp_arrive(d_ready);
-            }
-#pragma unroll
-            for (int t = 0; t < kTiles; ++t) {
-                if (!(ok = wait_bar_warp(d4_full + 8 * t, ph, abort))) break;
+                if (c + 1 < chunks) fetch(c + 1);
+                float o[8];
+                if (!(ok = wait_bar_warp(d1_full, ph, abort))) break;
                 tc_fence_after();
-                tc_sum3<VB>(d4 + L::kD4Tile * t + at, x);
-                add_to(x, s[t]);
-                if (c + 1 < chunks) {
-                    if (has_s) put_terms<VB>(sm + L::kS, K, 128 * t + ln, sub, s[t]);
+                tc_sum3<VB>(d1 + at, x);
+                if (q) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) o[e] = f0 * x[e];
+                } else {
+                    /* rows without a token have zeros for all of it */
+                    scale_add(f0, x, bv);
+                    put_terms<VB>(sm + L::kR, kC, i, sub, bv);
                     fence_async();
                     tc_fence_before();
-                    warp_arrive(s_ready + 8 * t);
+                    warp_arrive(r_ready);
+                }
+                if (!(ok = wait_bar_warp(d3_full, ph, abort))) break;
+                tc_fence_after();
+                tc_sum3<VB>(d3 + at, x);
+                if (q) {
+                    if (i < rows) {
+                        __nv_bfloat16 *dst = out + (int64_t)(tc + i) * p.out_token + 8 * sub;
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) o[e] += x[e];
+                        if (out_wide) {
+                            *reinterpret_cast<uint4 *>(dst) = make_uint4(bf16_pair(o[0], o[1]), bf16_pair(o[2], o[3]),
+                                                                         bf16_pair(o[4], o[5]), bf16_pair(o[6], o[7]));
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) dst[e] = __float2bfloat16_rn(o[e]);
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) x[e] *= f2;
+                    put_terms<VB>(sm + L::kD, kC, i, sub, x);
+                    fence_async();
+                    tc_fence_before();
+                    warp_arrive(d_ready);
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < L::kOwn; ++t) {
+                if (!(ok = wait_bar_warp(d4_full + 8 * (tile0 + t), ph, abort))) break;
+                tc_fence_after();
+                tc_sum3<VB>(d4 + L::kD4Tile * (tile0 + t) + at, x);
+                add_to(x, s[t]);
+                if (c + 1 < chunks) {
+                    if (has_s) put_terms<VB>(sm + L::kS, K, 128 * (tile0 + t) + ln, sub, s[t]);
+                    fence_async();
+                    tc_fence_before();
+                    warp_arrive(s_ready + 8 * (tile0 + t));
                 }
             }
             if (!ok) break;
@@ -983,9 +987,9 @@ __global__ void __launch_bounds__(Scan<K, VB>::kThreads, Scan<K, VB>::kMinCtas)
             /* a sequence that was given up leaves no state that could pass for one */
             const float bad = __int_as_float(0x7fc00000);
 #pragma unroll
-            for (int t = 0; t < kTiles; ++t)
+            for (int t = 0; t < L::kOwn; ++t)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) S[(int64_t)(8 * sub + e) * K + 128 * t + ln] = ok ? s[t][e] : bad;
+                for (int e = 0; e < 8; ++e) S[(int64_t)(8 * sub + e) * K + 128 * (tile0 + t) + ln] = ok ? s[t][e] : bad;
         }
     }
     tc_fence_before();
