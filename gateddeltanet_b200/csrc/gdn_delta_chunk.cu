@@ -142,6 +142,11 @@ __device__ __forceinline__ void tc_ld8(uint32_t addr, uint32_t (&r)[8]) {
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
                  : "r"(addr));
 }
+__device__ __forceinline__ void tc_ld32(uint32_t addr, uint32_t (&r)[32]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+                 : "r"(addr));
+}
 __device__ __forceinline__ void tc_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 /* pairs of FP32 values */
 __device__ __forceinline__ uint64_t pack2(uint32_t lo, uint32_t hi) {
@@ -294,63 +299,127 @@ __device__ __forceinline__ void place_sequences(const DeltaParams &p, uint32_t *
     }
 }
 
+/* Two threads per row of [K; Q] form, from the MMA's products, its row of A (k)
+ * or of P (q). T = (I + A)^-1 by blocks,
+ *   [[a 0] [c b]]^-1 = [[a^-1 0] [-b^-1 c a^-1, b^-1]],
+ * the four of 16 on the diagonal by substitution, a warp each and a lane per
+ * row; the products, and P T, with mma.sync of TF32 parts (x = x0 + x1, three
+ * of the four products: 21 bits, of which the record keeps 16). What bounds it
+ * is the chain of these steps, against which three CTAs share an SM. */
 constexpr int kPrepThreads = 256;
-constexpr uint32_t kLd = kC + 4; /* row stride of the FP32 matrices, floats */
+constexpr uint32_t kLdA = kC + 8, kLdP = kC + 4; /* row strides of A, T and X, and of P: fragments without bank conflicts */
 
-/* The FP32 matrices take the place of [K; Q] once the MMAs and the norms have
- * read it, so that three CTAs share an SM. */
+/* The FP32 matrices take the place of [K; Q] once the MMAs have read it. */
 template <int K>
 struct PrepSmem {
     static constexpr uint32_t kTile = 0;                                  /* [K; Q] */
     static constexpr uint32_t kA = 0;                                     /* A, then T */
-    static constexpr uint32_t kP = kA + kC * kLd * 4;
-    static constexpr uint32_t kX = kP + kC * kLd * 4;                     /* products of the inversion */
-    static constexpr uint32_t kMat = kX + 32 * kLd * 4;
+    static constexpr uint32_t kP = kA + kC * kLdA * 4;
+    static constexpr uint32_t kX = kP + kC * kLdP * 4;                    /* c a^-1 */
+    static constexpr uint32_t kMat = kX + 32 * kLdA * 4;
     static constexpr uint32_t kG = (K / 64) * kTermBytes > kMat ? (K / 64) * kTermBytes : kMat;
     static constexpr uint32_t kRows = 7;                                  /* G hi, lo, beta, norms of k, q, two of decays */
     static constexpr uint32_t kBar = kG + kRows * kC * 4;
     static constexpr uint32_t kBytes = kBar + 32 + 1024;                  /* room to align */
 };
 
-/* out (2 x 4 values at row r, column c) = sign * sum over j in [j0, j1) of
- * a[r][j] b[j][c], j0 and j1 multiples of 4; rows of kLd */
-__device__ __forceinline__ void product_2x4(const float *a, const float *b, int r, int c, int j0, int j1, float (&s)[2][4]) {
+/* Row `lane` of the inverse of a 16 x 16 unit lower triangular block, given
+ * its part below the diagonal: x (I + A) = e, from the last column on; each x_j
+ * that is final is taken off the columns before it. */
+__device__ __forceinline__ void invert16(float *A, uint32_t lane) {
+    uint64_t y[8];
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
+    for (int j = 0; j < 8; ++j) y[j] = pack2((uint32_t)(2 * j) == lane ? 1.0f : 0.0f, (uint32_t)(2 * j + 1) == lane ? 1.0f : 0.0f);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[u][e] = 0.0f;
-#pragma unroll 2
-    for (int j = j0; j < j1; j += 4) {
-        const float4 x0 = *reinterpret_cast<const float4 *>(a + r * kLd + j);
-        const float4 x1 = *reinterpret_cast<const float4 *>(a + (r + 1) * kLd + j);
-        const float x[2][4] = {{x0.x, x0.y, x0.z, x0.w}, {x1.x, x1.y, x1.z, x1.w}};
+    for (int j = 15; j >= 1; --j) {
+        float lo, hi;
+        unpack2(y[j / 2], lo, hi);
+        const float x = -((j & 1) ? hi : lo);
+        const uint64_t xx = pack2(x, x);
+        const ulonglong2 *row = reinterpret_cast<const ulonglong2 *>(A + j * kLdA);
 #pragma unroll
-        for (int d = 0; d < 4; ++d) {
-            const float4 y = *reinterpret_cast<const float4 *>(b + (j + d) * kLd + c);
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                s[u][0] = fmaf(x[u][d], y.x, s[u][0]);
-                s[u][1] = fmaf(x[u][d], y.y, s[u][1]);
-                s[u][2] = fmaf(x[u][d], y.z, s[u][2]);
-                s[u][3] = fmaf(x[u][d], y.w, s[u][3]);
+        for (int l = 0; l < j; l += 4) {
+            const ulonglong2 a = row[l / 4];
+            if (l + 1 < j) y[l / 2] = fma2(xx, a.x, y[l / 2]);
+            if (l + 3 < j) y[l / 2 + 1] = fma2(xx, a.y, y[l / 2 + 1]);
+            if ((j & 1) && l + 4 > j) {
+                /* the last column before an odd j: the pair's other half is x_j itself */
+                float alo, ahi, ylo, yhi;
+                unpack2(j - 1 == l ? a.x : a.y, alo, ahi);
+                unpack2(y[j / 2], ylo, yhi);
+                y[j / 2] = pack2(fmaf(x, alo, ylo), yhi);
             }
         }
     }
-}
-/* out (m x m) = sign * a b for `threads` threads, where either a (kLeft) or b
- * is lower triangular */
-template <bool kLeft>
-__device__ __forceinline__ void small_product(float *out, const float *a, const float *b, int m, float sign, int thread,
-                                              int threads) {
-    for (int i = thread; i < (m / 2) * (m / 4); i += threads) {
-        const int r = (i / (m / 4)) * 2, c = (i % (m / 4)) * 4;
-        float s[2][4];
-        product_2x4(a, b, r, c, kLeft ? 0 : c, kLeft ? (r + 5) & ~3 : m, s);
+    __syncwarp();
+    if (lane < 16) {
+        ulonglong2 *out = reinterpret_cast<ulonglong2 *>(A + lane * kLdA);
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
-            *reinterpret_cast<float4 *>(out + (r + u) * kLd + c) =
-                make_float4(sign * s[u][0], sign * s[u][1], sign * s[u][2], sign * s[u][3]);
+        for (int j = 0; j < 8; j += 2) out[j / 2] = make_ulonglong2(y[j], y[j + 1]);
     }
+}
+
+/* Fragments of m16n8k8, g = lane / 4, t = lane % 4, each element in two TF32 parts */
+struct FragA {
+    uint32_t hi[4], lo[4];
+};
+struct FragB {
+    uint32_t hi[2], lo[2];
+};
+__device__ __forceinline__ void tf32_parts(float x, uint32_t &hi, uint32_t &lo) {
+    hi = __float_as_uint(x) & 0xFFFFE000u;
+    lo = __float_as_uint(x - __uint_as_float(hi));
+}
+/* rows r .. r + 15, columns c .. c + 7 of m */
+__device__ __forceinline__ FragA frag_a(const float *m, uint32_t ld, uint32_t r, uint32_t c, uint32_t lane) {
+    FragA f;
+    const float *p = m + (r + (lane >> 2)) * ld + c + (lane & 3);
+    tf32_parts(p[0], f.hi[0], f.lo[0]);
+    tf32_parts(p[8 * ld], f.hi[1], f.lo[1]);
+    tf32_parts(p[4], f.hi[2], f.lo[2]);
+    tf32_parts(p[8 * ld + 4], f.hi[3], f.lo[3]);
+    return f;
+}
+/* rows (k) r .. r + 7, columns (n) c .. c + 7 of m */
+__device__ __forceinline__ FragB frag_b(const float *m, uint32_t ld, uint32_t r, uint32_t c, uint32_t lane) {
+    FragB f;
+    const float *p = m + (r + (lane & 3)) * ld + c + (lane >> 2);
+    tf32_parts(p[0], f.hi[0], f.lo[0]);
+    tf32_parts(p[4 * ld], f.hi[1], f.lo[1]);
+    return f;
+}
+__device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+}
+/* the three products in accumulators of their own, so that they do not wait for one another */
+__device__ __forceinline__ void mma_parts(float (&d)[3][4], const FragA &a, const FragB &b) {
+    mma_tf32(d[0], a.lo, b.hi);
+    mma_tf32(d[1], a.hi, b.lo);
+    mma_tf32(d[2], a.hi, b.hi);
+}
+__device__ __forceinline__ float parts_sum(const float (&d)[3][4], int e) { return d[2][e] + (d[0][e] + d[1][e]); }
+/* rows r .. r + 15, columns c .. c + 7 of out = sign * a b, over kK columns of a;
+ * rows of kLdA */
+template <int kK>
+__device__ __forceinline__ void product_tile(float *out, const float *a, const float *b, float sign, uint32_t r, uint32_t c,
+                                             uint32_t lane) {
+    float d[3][4] = {};
+#pragma unroll
+    for (int k = 0; k < kK; k += 8) mma_parts(d, frag_a(a, kLdA, r, k, lane), frag_b(b, kLdA, k, c, lane));
+    float *p = out + (r + (lane >> 2)) * kLdA + c + 2 * (lane & 3);
+    *reinterpret_cast<float2 *>(p) = make_float2(sign * parts_sum(d, 0), sign * parts_sum(d, 1));
+    *reinterpret_cast<float2 *>(p + 8 * kLdA) = make_float2(sign * parts_sum(d, 2), sign * parts_sum(d, 3));
+}
+/* two neighbouring values of a row of the record as two BF16 terms */
+__device__ __forceinline__ void put_pair2(uint8_t *rec, uint32_t row, uint32_t col, float x, float y) {
+    const uint32_t w = bf16_pair(x, y);
+    const uint32_t u = bf16_pair(x - __uint_as_float(w << 16), y - __uint_as_float(w & 0xFFFF0000u));
+    uint8_t *p = rec + piece_at(row, col >> 3) + (col & 7) * 2;
+    *reinterpret_cast<uint32_t *>(p) = w;
+    *reinterpret_cast<uint32_t *>(p + kTermBytes) = u;
 }
 
 __device__ __forceinline__ void load8(const float *p, float (&x)[8]) {
@@ -363,16 +432,10 @@ __device__ __forceinline__ void store8(float *p, const float (&x)[8]) {
 }
 /* e^x for a decay: the product with log2 e rounds by 2^-24 |x|, and
  * |x| e^x stays below 0.37 */
-__device__ __forceinline__ float decay_exp(float x) { return exp2f(x * 1.4426950408889634f); }
-
-/* four values of row `row` as two BF16 terms of the record's [T; P T] */
-__device__ __forceinline__ void put_pair4(uint8_t *rec, uint32_t row, uint32_t col, float4 x) {
-    const uint32_t w0 = bf16_pair(x.x, x.y), w1 = bf16_pair(x.z, x.w);
-    const uint32_t u0 = bf16_pair(x.x - __uint_as_float(w0 << 16), x.y - __uint_as_float(w0 & 0xFFFF0000u));
-    const uint32_t u1 = bf16_pair(x.z - __uint_as_float(w1 << 16), x.w - __uint_as_float(w1 & 0xFFFF0000u));
-    uint8_t *p = rec + piece_at(row, col >> 3) + (col & 7) * 2;
-    *reinterpret_cast<uint2 *>(p) = make_uint2(w0, w1);
-    *reinterpret_cast<uint2 *>(p + kTermBytes) = make_uint2(u0, u1);
+__device__ __forceinline__ float decay_exp(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x * 1.4426950408889634f));
+    return y;
 }
 
 template <int K>
@@ -498,144 +561,135 @@ __global__ void __launch_bounds__(kPrepThreads, 3) chunk_prep_kernel(const __gri
         }
         commit(bar);
     }
-    const bool ok = wait_bar_warp(bar, 0, abort);
+    wait_bar_warp(bar, 0, abort);
     tc_fence_after();
+    /* rows 32 (warp % 4) .. + 31 of [K; Q], one a lane: token i of k or of q */
+    const uint32_t row = 32 * (warp & 3) + lane, lanes = (32 * (warp & 3)) << 16, i = row & (kC - 1);
+    const bool is_p = row >= (uint32_t)kC, low = i >= 32; /* uniform in a warp */
     if (warp < 4) {
-        /* warp w: rows and columns 32 w .. 32 w + 31 */
+        /* its norm, from the diagonal */
+        uint32_t r[32];
         float ss = 0.0f;
+        __syncwarp();
+        tc_ld32(tmem + lanes + 32 * warp, r);
+        tc_wait();
 #pragma unroll
-        for (int c = 0; c < 32; c += 8) {
-            uint32_t r[8];
-            __syncwarp();
-            tc_ld8(tmem + ((32 * warp) << 16) + 32 * warp + c, r);
-            tc_wait();
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if ((int)lane == c + e) ss = __uint_as_float(r[e]);
-        }
+        for (int e = 0; e < 32; ++e)
+            if ((int)lane == e) ss = __uint_as_float(r[e]);
         const float inv = p.normalize ? 1.0f / sqrtf(ss + 1e-6f) : 1.0f;
-        if (warp < 2)
-            kin[tid] = inv;
+        if (is_p)
+            qin[i] = inv * p.scale;
         else
-            qin[tid - kC] = inv * p.scale;
+            kin[i] = inv;
     }
     __syncthreads(); /* [K; Q] has been read: the matrices may take its place */
     /* the record's rows of scalars */
-    if (tid < kC) {
+    if (warp < 2) {
         float *sc = reinterpret_cast<float *>(record + kPairBytes);
-        const float g1 = G[tid] + Glo[tid], eg = expf(g1);
-        const bool there = tid < rows;
-        sc[kScalC * kC + tid] = there ? eg * kin[tid] : 0.0f;
-        sc[kScalBeta * kC + tid] = bet[tid];
-        sc[kScalQ * kC + tid] = eg * qin[tid];
-        sc[kScalEnd * kC + tid] = there ? expf((G[kC - 1] - G[tid]) + (Glo[kC - 1] - Glo[tid])) * kin[tid] : 0.0f;
-        if (tid == kC - 1) sc[kScalDecay * kC] = eg;
+        const float eg = expf(G[i] + Glo[i]);
+        const bool there = i < rows;
+        sc[kScalC * kC + i] = there ? eg * kin[i] : 0.0f;
+        sc[kScalBeta * kC + i] = bet[i];
+        sc[kScalQ * kC + i] = eg * qin[i];
+        sc[kScalEnd * kC + i] = there ? expf((G[kC - 1] - G[i]) + (Glo[kC - 1] - Glo[i])) * kin[i] : 0.0f;
+        if (i == kC - 1) sc[kScalDecay * kC] = eg;
         /* the two factors of the decays between the halves of the chunk */
-        if (tid < 32)
-            dec_j[tid] = expf((G[32] - G[tid]) + (Glo[32] - Glo[tid])) * kin[tid];
+        if (i < 32)
+            dec_j[i] = expf((G[32] - G[i]) + (Glo[32] - Glo[i])) * kin[i];
         else
-            dec_i[tid] = expf((G[tid] - G[32]) + (Glo[tid] - Glo[32]));
+            dec_i[i] = expf((G[i] - G[32]) + (Glo[i] - Glo[32]));
     }
     __syncthreads();
-    if (ok) {
-        /* lanes 0..63: rows of A; 64..127: rows of P; warps 4..7 take columns
-         * 32..63. e^(G_i - G_j) of the lower left quarter is the product of
-         * e^(G_i - G_32) and e^(G_32 - G_j), neither above 1 where nothing
-         * grows; the upper right one is zero. */
-        const uint32_t row = 32 * (warp & 3) + lane, i = row & (kC - 1), c0 = (warp >> 2) * 32;
-        const bool is_p = row >= kC, low = i >= 32, left = c0 == 0; /* uniform in a warp */
-        const float gi = G[i], gl = Glo[i];
+    /* row i of A or P: warps 0-3 columns 0 .. 31, warps 4-7 the others. e^(G_i -
+     * G_j) of the lower left quarter is the product of e^(G_i - G_32) and
+     * e^(G_32 - G_j), neither above 1 where nothing grows; the upper right one is
+     * zero. */
+    {
+        const bool left = warp < 4;
+        const uint32_t c0 = left ? 0 : 32;
+        float *dst = (is_p ? P + i * kLdP : A + i * kLdA) + c0;
+        uint32_t r[32];
+        if (low || left) {
+            __syncwarp();
+            tc_ld32(tmem + lanes + c0, r);
+            tc_wait();
+        }
         float f = is_p ? qin[i] : bet[i] * kin[i];
-        if (low && left) f *= dec_i[i];
-        float *dst = (is_p ? P : A) + i * kLd + c0;
-        if (low && left) {
+        if (low != left) {
+            /* the quarter with the diagonal */
+            const float gi = G[i], gl = Glo[i];
+            const int last = (int)(i & 31) - (is_p ? 0 : 1); /* the last column with a product */
 #pragma unroll
             for (int c = 0; c < 32; c += 8) {
-                uint32_t r[8];
-                float dj[8], x[8];
-                load8(dec_j + c, dj);
-                __syncwarp();
-                tc_ld8(tmem + ((32 * (warp & 3)) << 16) + c, r);
-                tc_wait();
-#pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] = f * dj[e] * __uint_as_float(r[e]);
-                store8(dst + c, x);
-            }
-        } else if (low || left) {
-            const int last = (int)(i - c0) - (is_p ? 0 : 1); /* the last column with a product */
-#pragma unroll
-            for (int c = 0; c < 32; c += 8) {
-                uint32_t r[8];
                 float gj[8], lj[8], kj[8], x[8];
                 load8(G + c0 + c, gj);
                 load8(Glo + c0 + c, lj);
                 load8(kin + c0 + c, kj);
-                __syncwarp();
-                tc_ld8(tmem + ((32 * (warp & 3)) << 16) + c0 + c, r);
-                tc_wait();
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    const float y = f * kj[e] * decay_exp((gi - gj[e]) + (gl - lj[e])) * __uint_as_float(r[e]);
-                    x[e] = c + e <= last ? y : (!is_p && c + e == last + 1 ? 1.0f : 0.0f);
+                    /* for all columns: taken only where wanted, it cost a branch each (5200 cycles for the 32) */
+                    const float y = f * kj[e] * decay_exp((gi - gj[e]) + (gl - lj[e])) * __uint_as_float(r[c + e]);
+                    x[e] = c + e <= last ? y : 0.0f;
                 }
                 store8(dst + c, x);
             }
         } else {
-            const float x[8] = {};
+            if (low) f *= dec_i[i];
 #pragma unroll
-            for (int c = 0; c < 32; c += 8) store8(dst + c, x);
+            for (int c = 0; c < 32; c += 8) {
+                float dj[8], x[8];
+                load8(dec_j + c, dj);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = low ? f * dj[e] * __uint_as_float(r[c + e]) : 0.0f;
+                store8(dst + c, x);
+            }
         }
     }
     tc_fence_before();
     __syncthreads();
-    /* T = (I + A)^-1 in place: the 16 x 16 diagonal blocks by forward
-     * substitution (a lane per column), then twice
-     * [[a 0] [c b]]^-1 = [[a^-1 0] [-b^-1 c a^-1, b^-1]] */
-    if (warp < 4) {
-        float *D = A + (16 * warp) * kLd + 16 * warp;
-        if (lane < 16) {
-            float x[16];
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                float s = r == (int)lane ? 1.0f : 0.0f;
-#pragma unroll
-                for (int j = 0; j < 16; ++j)
-                    if (j < r) s = fmaf(-D[r * kLd + j], x[j], s);
-                x[r] = s;
-            }
-            __syncwarp(0xffffu);
-#pragma unroll
-            for (int r = 0; r < 16; ++r) D[r * kLd + lane] = x[r];
-        }
-    }
+    constexpr uint32_t kDiag = kLdA + 1;
+    if (warp < 4) invert16(A + 16 * warp * kDiag, lane);
     __syncthreads();
-    {
-        /* two blocks of 32: half of the threads each */
-        const int b = tid >> 7, th = tid & 127;
-        float *D = A + (32 * b) * kLd + 32 * b, *Y = X + (16 * b) * kLd;
-        small_product<false>(Y, D + 16 * kLd, D, 16, 1.0f, th, 128);
-        __syncthreads();
-        small_product<true>(D + 16 * kLd, D + 16 * kLd + 16, Y, 16, -1.0f, th, 128);
-    }
+    /* blocks of 32: warps 0, 1 the first, 2, 3 the second, 8 columns each */
+    float *B = A + 32 * (warp >> 1) * kDiag, *XB = X + 16 * (warp >> 1) * kLdA;
+    if (warp < 4) product_tile<16>(XB, B + 16 * kLdA, B, 1.0f, 0, 8 * (warp & 1), lane);
     __syncthreads();
-    small_product<false>(X, A + 32 * kLd, A, 32, 1.0f, tid, kPrepThreads);
+    if (warp < 4) product_tile<16>(B + 16 * kLdA, B + 16 * kDiag, XB, -1.0f, 0, 8 * (warp & 1), lane);
     __syncthreads();
-    small_product<true>(A + 32 * kLd, A + 32 * kLd + 32, X, 32, -1.0f, tid, kPrepThreads);
+    product_tile<32>(X, A + 32 * kLdA, A, 1.0f, 16 * (warp >> 2), 8 * (warp & 3), lane);
     __syncthreads();
-    /* the record: T in the rows of the chunk's k, P T in those of its q (both
-     * lower triangular); the two change places from chunk to chunk */
+    product_tile<32>(A + 32 * kLdA, A + 32 * kDiag, X, -1.0f, 16 * (warp >> 2), 8 * (warp & 3), lane);
+    __syncthreads();
+    /* the record, in two BF16 terms: T in the rows of the chunk's k, P T in
+     * those of its q (both lower triangular); the two change places from chunk
+     * to chunk */
     const uint32_t t_row = (chunk & 1) ? kC : 0, p_row = kC - t_row;
-    for (uint32_t i = tid; i < (kC / 2) * (kC / 4); i += kPrepThreads) {
-        /* rows that share a warp need sums of about one length: 16 columns of
-         * threads, the rows in pairs downwards */
-        const uint32_t r = (i / (kC / 4)) * 2, c = (i % (kC / 4)) * 4;
-        float s[2][4];
-        product_2x4(P, A, (int)r, (int)c, (int)c, ((int)r + 5) & ~3, s);
+    for (uint32_t x = tid; x < kC * 8; x += kPrepThreads) {
+        const uint32_t r = x >> 3, c = (x & 7) * 8;
+        float v[8];
+        load8(A + r * kLdA + c, v);
+        uint32_t w[4], u[4];
 #pragma unroll
-        for (uint32_t u = 0; u < 2; ++u) {
-            put_pair4(record, t_row + r + u, c, *reinterpret_cast<const float4 *>(A + (r + u) * kLd + c));
-            put_pair4(record, p_row + r + u, c, make_float4(s[u][0], s[u][1], s[u][2], s[u][3]));
+        for (int e = 0; e < 4; ++e) {
+            w[e] = bf16_pair(v[2 * e], v[2 * e + 1]);
+            u[e] = bf16_pair(v[2 * e] - __uint_as_float(w[e] << 16), v[2 * e + 1] - __uint_as_float(w[e] & 0xFFFF0000u));
         }
+        uint8_t *dst = record + piece_at(t_row + r, c >> 3);
+        *reinterpret_cast<uint4 *>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+        *reinterpret_cast<uint4 *>(dst + kTermBytes) = make_uint4(u[0], u[1], u[2], u[3]);
+    }
+    /* P T in tiles of 16 rows (m) and 8 columns (n), each the sum over the
+     * column blocks k = n .. 2 m + 1; a warp's four tiles have 7 to 11 together */
+#pragma unroll
+    for (uint32_t m = 0; m < 4; ++m) {
+        const uint32_t n = m == 2 ? 7 - warp : m == 1 ? warp ^ 4 : warp;
+        float d[3][4] = {};
+#pragma unroll
+        for (uint32_t k = 0; k < 2 * m + 2; ++k)
+            if (k >= n) mma_parts(d, frag_a(P, kLdP, 16 * m, 8 * k, lane), frag_b(A, kLdA, 8 * k, 8 * n, lane));
+        const uint32_t col = 8 * n + 2 * (lane & 3), r = p_row + 16 * m + (lane >> 2);
+        put_pair2(record, r, col, parts_sum(d, 0), parts_sum(d, 1));
+        put_pair2(record, r + 8, col, parts_sum(d, 2), parts_sum(d, 3));
     }
     if (warp == 0) {
         tc_fence_after();
