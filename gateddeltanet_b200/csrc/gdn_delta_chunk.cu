@@ -449,23 +449,34 @@ __global__ void __launch_bounds__(kPrepThreads, 3) chunk_prep_kernel(const __gri
     __nv_bfloat16 *out = static_cast<__nv_bfloat16 *>(p.out);
     if (h == 0) place_sequences(p, order);
 
-    /* the sequence whose records hold number rec: the last one that starts at or before it */
+    /* the sequence whose records hold number rec: the last one whose first
+     * record is at or before it. All threads look at once where that takes
+     * fewer rounds than halving. N: the tokens after the last sequence. */
     uint32_t t0, t1, n;
-    uint32_t lo = 0, hi = p.N; /* N: the tokens after the last sequence */
-    while (lo < hi) {
-        const uint32_t mid = (lo + hi + 1) / 2;
+    auto begins_by = [&](uint32_t m) {
         uint32_t a, b;
-        if (mid == p.N) {
-            sequence_tokens(p, p.N - 1, b, a);
+        if (m < p.N) {
+            sequence_tokens(p, m, a, b);
         } else {
-            sequence_tokens(p, mid, a, b);
+            sequence_tokens(p, p.N - 1, b, a);
         }
-        if (record_of(a, mid) <= rec)
-            lo = mid;
-        else
-            hi = mid - 1;
+        return record_of(a, m) <= rec;
+    };
+    if (p.N <= 8 * kPrepThreads) {
+        n = 0;
+        for (uint32_t m = 1; m <= p.N; m += kPrepThreads)
+            n += (uint32_t)__syncthreads_count(m + tid <= p.N && begins_by(m + tid));
+    } else {
+        uint32_t lo = 0, hi = p.N;
+        while (lo < hi) {
+            const uint32_t mid = (lo + hi + 1) / 2;
+            if (begins_by(mid))
+                lo = mid;
+            else
+                hi = mid - 1;
+        }
+        n = lo;
     }
-    n = lo;
     if (n == 0 && p.starts != nullptr) {
         /* tokens before the first sequence give zeros */
         sequence_tokens(p, 0, t0, t1);

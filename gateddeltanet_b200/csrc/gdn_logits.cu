@@ -27,6 +27,8 @@
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 
+#include <type_traits>
+
 namespace gdn {
 namespace ops {
 
@@ -149,10 +151,25 @@ __global__ void __launch_bounds__(kThreads, 5) logits_kernel(const __grid_consta
     const uint32_t va = max(v0, mis != 0 ? 1u : 0u), vb = min(v1, nvec - ((mis + V) % N != 0 ? 1u : 0u));
     const uint4 *src = reinterpret_cast<const uint4 *>(in - mis);
     uint4 w[kUnroll];
+    uint32_t allow[kUnroll];
+    const uint8_t *mask8 = reinterpret_cast<const uint8_t *>(mask);
+    /* N bits of vector i of a row of bits that starts with a vector's first token */
+    auto bits_of = [](const uint8_t *bits, uint32_t i) {
+        return N == 8 ? (uint32_t)bits[i] : (uint32_t)bits[i >> 1] >> (4 * (i & 1)) & 15u;
+    };
     auto load = [&](uint32_t base) {
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u)
-            if (base + u * kThreads < vb) w[u] = __ldcs(src + base + u * kThreads);
+        for (int u = 0; u < kUnroll; ++u) {
+            const uint32_t i = base + u * kThreads;
+            if (i < vb) {
+                w[u] = __ldcs(src + i);
+                if (mask != nullptr) {
+                    const uint32_t e0 = i * N - mis;
+                    allow[u] = mis == 0 ? bits_of(mask8, i)
+                                        : __funnelshift_r(mask[e0 >> 5], mask[(e0 + N - 1) >> 5], e0 & 31);
+                }
+            }
+        }
     };
     load(va + tid); /* on their way while the table is built */
 
@@ -219,11 +236,6 @@ __global__ void __launch_bounds__(kThreads, 5) logits_kernel(const __grid_consta
     float top = kNegInf;
     uint32_t top_vec = 0;
     const uint8_t *past8 = reinterpret_cast<const uint8_t *>(past), *biased8 = reinterpret_cast<const uint8_t *>(biased);
-    const uint8_t *mask8 = reinterpret_cast<const uint8_t *>(mask);
-    /* N bits of vector i of a row of bits that starts with a vector's first token */
-    auto bits_of = [&](const uint8_t *bits, uint32_t i) {
-        return N == 8 ? (uint32_t)bits[i] : (uint32_t)bits[i >> 1] >> (4 * (i & 1)) & 15u;
-    };
     auto own_bits = [&](uint32_t i) { return use_table ? bits_of(past8, i - v0) | bits_of(biased8, i - v0) : 0u; };
     auto edge = [&](uint32_t i) {
         /* a row's ragged first or last vector */
@@ -240,33 +252,48 @@ __global__ void __launch_bounds__(kThreads, 5) logits_kernel(const __grid_consta
     };
     if (tid == 0 && v0 < min(va, v1)) edge(v0);
     if (tid == 32 && vb < v1 && v1 - 1 >= va) edge(v1 - 1);
-    for (uint32_t base = va + tid; base < vb; base += kThreads * kUnroll) {
-        if (base != va + tid) load(base);
-#pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-            const uint32_t i = base + u * kThreads;
-            if (i >= vb) break;
-            const uint32_t own = own_bits(i);
-            uint4 o = w[u];
-            if (mask != nullptr) {
-                const uint32_t e0 = i * N - mis;
-                const uint32_t allow = mis == 0 ? bits_of(mask8, i)
-                                                : __funnelshift_r(mask[e0 >> 5], mask[(e0 + N - 1) >> 5], e0 & 31);
-                o = Vec<T>::only(o, allow | own);
-            }
+    /* the pass, for rows with and without a table and a mask */
+    auto dense = [&](auto table_on, auto mask_on) {
+        constexpr bool kTable = decltype(table_on)::value, kMask = decltype(mask_on)::value;
+        auto one = [&](uint32_t i, uint4 o, uint32_t may) {
+            const uint32_t own = kTable ? bits_of(past8, i - v0) | bits_of(biased8, i - v0) : 0u;
+            if (kMask) o = Vec<T>::only(o, may | own);
             if (wide_out) {
                 __stcs(reinterpret_cast<uint4 *>(out - mis) + i, o);
             } else {
 #pragma unroll
                 for (int j = 0; j < N; ++j) store_one(out - mis + (i * N + j), Vec<T>::value(o, j));
             }
-            if (own) o = Vec<T>::only(o, ~own);
+            if (kTable && own) o = Vec<T>::only(o, ~own);
             const float m = Vec<T>::largest(o);
             if (m > top) {
                 top = m;
                 top_vec = i;
             }
+        };
+        for (uint32_t base = va + tid; base < vb; base += kThreads * kUnroll) {
+            if (base != va + tid) load(base);
+            if (base + (kUnroll - 1) * kThreads < vb) {
+#pragma unroll
+                for (int u = 0; u < kUnroll; ++u) one(base + u * kThreads, w[u], allow[u]);
+            } else {
+#pragma unroll
+                for (int u = 0; u < kUnroll - 1; ++u)
+                    if (base + u * kThreads < vb) one(base + u * kThreads, w[u], allow[u]);
+            }
         }
+    };
+    using std::bool_constant;
+    if (use_table) {
+        if (mask != nullptr)
+            dense(bool_constant<true>(), bool_constant<true>());
+        else
+            dense(bool_constant<true>(), bool_constant<false>());
+    } else {
+        if (mask != nullptr)
+            dense(bool_constant<false>(), bool_constant<true>());
+        else
+            dense(bool_constant<false>(), bool_constant<false>());
     }
     if (top > kNegInf) {
         /* this thread's own vector again: which of its tokens it was */
