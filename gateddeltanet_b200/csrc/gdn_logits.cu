@@ -12,15 +12,18 @@
  * Bound by HBM: every logit is read and written once. A row is cut into the
  * slices of one cluster's CTAs. Each CTA reads the row's history and counts
  * what falls into its slice in shared memory (integer atomics: the order does
- * not show): n per token, in 16 bits where the history is short enough, and a
- * bit that history holds the token; another bit says that a bias names it.
- * Tokens with neither bit, nearly all, only meet the mask: a dense pass copies
- * them 16 bytes at a time and keeps the largest. The others are then found
- * from the bits and recomputed, a lane each; as a test in the dense pass they
- * left whole warps waiting for the lanes that had one. What bounds the kernel
- * beside HBM are the instructions that a warp spends once (setting up, clearing,
- * counting, the reductions), so a CTA has few warps with many logits each.
- * The picks of the slices meet in CTA 0 through distributed shared memory.
+ * not show): n per token, in 16 bits where the logits have 16 and the history
+ * is short enough, and a bit that history holds the token; another bit says
+ * that a bias names it. The tokens with a bit, a few of a hundred, are found from
+ * the bits and computed a lane each, and their results take the place of their
+ * counts. The other tokens only meet the mask: a dense pass copies 16 bytes at
+ * a time, puts in the results where a bit is set, and keeps the largest. (As
+ * cases of the dense pass the few left whole warps waiting for the lanes that
+ * had one: 135 us for 256 rows of 131072 BF16; computed after it, from what it
+ * had written, they were a second round trip to memory: 71 us.) What bounds
+ * the kernel beside HBM are the instructions that a warp spends once, so a CTA
+ * has few warps with many logits each. The picks of the slices meet in CTA 0
+ * through distributed shared memory.
  */
 #include "gdn_ops.h"
 
@@ -38,7 +41,7 @@ namespace cg = cooperative_groups;
 
 constexpr uint32_t kThreads = 256;
 constexpr int kUnroll = 4;      /* 16-byte vectors of a thread in flight */
-constexpr int kHistoryUnroll = 4;
+constexpr int kHistoryUnroll = 8;
 constexpr int kMaxCluster = 8;  /* portable cluster size */
 
 /* pick key: larger value first, then the lower index; NaN is 0 and so never wins */
@@ -63,6 +66,11 @@ struct Vec<float> {
         return make_uint4((allow & 1u) ? w.x : 0xFF800000u, (allow & 2u) ? w.y : 0xFF800000u,
                           (allow & 4u) ? w.z : 0xFF800000u, (allow & 8u) ? w.w : 0xFF800000u);
     }
+    /* w, with the values of t whose bit is set */
+    static __device__ __forceinline__ uint4 blend(const uint4 &w, const uint4 &t, uint32_t own) {
+        return make_uint4((own & 1u) ? t.x : w.x, (own & 2u) ? t.y : w.y, (own & 4u) ? t.z : w.z, (own & 8u) ? t.w : w.w);
+    }
+    static __device__ __forceinline__ uint32_t bits(float x) { return __float_as_uint(x); }
     /* largest value, NaN passed over (-inf if there is nothing else) */
     static __device__ __forceinline__ float largest(const uint4 &w) {
         const float lo = __int_as_float(0xff800000);
@@ -77,13 +85,20 @@ struct Vec<__nv_bfloat16> {
         const uint32_t u = j < 2 ? w.x : j < 4 ? w.y : j < 6 ? w.z : w.w;
         return __uint_as_float((j & 1) ? (u & 0xFFFF0000u) : (u << 16));
     }
-    static __device__ __forceinline__ uint32_t pair(uint32_t w, uint32_t allow) {
-        const uint32_t m = ((allow & 1u) | ((allow & 2u) << 15)) * 0xFFFFu;
-        return (w & m) | (0xFF80FF80u & ~m);
+    /* of two values those of `yes` whose bit is set, those of `no` for the others */
+    static __device__ __forceinline__ uint32_t pair(uint32_t yes, uint32_t no, uint32_t set) {
+        const uint32_t m = ((set & 1u) | ((set & 2u) << 15)) * 0xFFFFu;
+        return (yes & m) | (no & ~m);
+    }
+    static __device__ __forceinline__ uint4 blend(const uint4 &w, const uint4 &t, uint32_t own) {
+        return make_uint4(pair(t.x, w.x, own), pair(t.y, w.y, own >> 2), pair(t.z, w.z, own >> 4), pair(t.w, w.w, own >> 6));
     }
     static __device__ __forceinline__ uint4 only(const uint4 &w, uint32_t allow) {
-        return make_uint4(pair(w.x, allow), pair(w.y, allow >> 2), pair(w.z, allow >> 4), pair(w.w, allow >> 6));
+        constexpr uint32_t kNone = 0xFF80FF80u;
+        return make_uint4(pair(w.x, kNone, allow), pair(w.y, kNone, allow >> 2), pair(w.z, kNone, allow >> 4),
+                          pair(w.w, kNone, allow >> 6));
     }
+    static __device__ __forceinline__ uint32_t bits(float x) { return __bfloat16_as_ushort(__float2bfloat16_rn(x)); }
     static __device__ __forceinline__ __nv_bfloat162 two(uint32_t w) { return *reinterpret_cast<__nv_bfloat162 *>(&w); }
     static __device__ __forceinline__ float largest(const uint4 &w) {
         const __nv_bfloat162 lo = two(0xFF80FF80u);
@@ -93,8 +108,8 @@ struct Vec<__nv_bfloat16> {
 };
 __device__ __forceinline__ float load_one(const float *p) { return *p; }
 __device__ __forceinline__ float load_one(const __nv_bfloat16 *p) { return __bfloat162float(*p); }
-__device__ __forceinline__ float rounded(float x, float) { return x; }
-__device__ __forceinline__ float rounded(float x, __nv_bfloat16) { return __bfloat162float(__float2bfloat16_rn(x)); }
+__device__ __forceinline__ float from_bits(uint32_t u, float) { return __uint_as_float(u); }
+__device__ __forceinline__ float from_bits(uint32_t u, __nv_bfloat16) { return __uint_as_float(u << 16); }
 __device__ __forceinline__ void store_one(float *p, float x) { *p = x; }
 __device__ __forceinline__ void store_one(__nv_bfloat16 *p, float x) { *p = __float2bfloat16_rn(x); }
 
@@ -116,10 +131,10 @@ __device__ __forceinline__ uint32_t nth_bit(uint32_t w, uint32_t n) {
     return at;
 }
 
-/* W: the type of a token's count. kAligned: every row of logits and of out
+/* W: the type of a token's count, as wide as T or wider. kAligned: every row of logits and of out
  * starts on a 16-byte boundary. */
 template <typename T, typename W, bool kAligned>
-__global__ void __launch_bounds__(kThreads, 5) logits_kernel(const __grid_constant__ LogitsParams p) {
+__global__ void __launch_bounds__(kThreads, 4) logits_kernel(const __grid_constant__ LogitsParams p) {
     constexpr int N = Vec<T>::kN;
     constexpr float kNegInf = -__builtin_huge_valf();
     extern __shared__ __align__(16) uint32_t table[]; /* counts of the slice, two bits each, the slice's biases */
@@ -188,7 +203,19 @@ __global__ void __launch_bounds__(kThreads, 5) logits_kernel(const __grid_consta
             }
         };
         load_ids((int32_t)tid);
-        int32_t bias_id = warp == 0 && lane < biases ? bias_ids[lane] : -1;
+        /* warp 0 takes the biases, 64 at a time */
+        const float *bias = p.bias + (int64_t)b * p.bias_row;
+        int32_t bias_id[2];
+        float bias_value[2];
+        auto load_biases = [&](uint32_t i0) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const uint32_t i = i0 + 32 * u + lane;
+                bias_id[u] = i < biases ? bias_ids[i] : -1;
+                bias_value[u] = i < biases ? bias[i] : 0.0f;
+            }
+        };
+        if (warp == 0) load_biases(0);
         const int32_t made = p.prompt_lens == nullptr ? 0 : p.prompt_lens[b];
         const uint32_t clear = (size * sizeof(W) / 4 + size / 16) / 4;
         for (uint32_t i = tid; i < clear; i += kThreads) reinterpret_cast<uint4 *>(table)[i] = make_uint4(0, 0, 0, 0);
@@ -210,28 +237,76 @@ __global__ void __launch_bounds__(kThreads, 5) logits_kernel(const __grid_consta
             }
         }
         if (warp == 0) {
-            /* the biases of the slice, in list order */
-            const float *bias = p.bias + (int64_t)b * p.bias_row;
+            /* those of the slice, in list order */
             uint32_t found = 0;
-            for (uint32_t i0 = 0; i0 < biases; i0 += 32) {
-                if (i0 != 0) bias_id = i0 + lane < biases ? bias_ids[i0 + lane] : -1;
-                const bool here = (uint32_t)(bias_id - lo) < span;
-                const uint32_t who = __ballot_sync(0xffffffffu, here);
-                if (here) {
-                    const uint32_t at = (uint32_t)(bias_id - first), place = found + __popc(who & ((1u << lane) - 1));
-                    atomicOr(&biased[at >> 5], 1u << (at & 31));
-                    slice_id[place] = bias_id;
-                    slice_bias[place] = bias[i0 + lane];
+            for (uint32_t i0 = 0; i0 < biases; i0 += 64) {
+                if (i0 != 0) load_biases(i0);
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const bool here = (uint32_t)(bias_id[u] - lo) < span;
+                    const uint32_t who = __ballot_sync(0xffffffffu, here);
+                    if (here) {
+                        const uint32_t at = (uint32_t)(bias_id[u] - first), spot = found + __popc(who & ((1u << lane) - 1));
+                        atomicOr(&biased[at >> 5], 1u << (at & 31));
+                        slice_id[spot] = bias_id[u];
+                        slice_bias[spot] = bias_value[u];
+                    }
+                    found += __popc(who);
                 }
-                found += __popc(who);
             }
             if (lane == 0) slice_biases = found;
         }
         __syncthreads();
     }
 
-    /* dense pass: the mask, and the largest of the tokens without a bit.
-     * Tokens with one keep their value for now. */
+    if (use_table) {
+        const float repetition = p.repetition == nullptr ? 1.0f : p.repetition[b];
+        const float presence = p.presence == nullptr ? 0.0f : p.presence[b];
+        const float frequency = p.frequency == nullptr ? 0.0f : p.frequency[b];
+        /* 32 words of bits at a time: the set ones in order, one for each lane */
+        for (uint32_t w0 = warp * 32; w0 < size / 32; w0 += kThreads) {
+            const uint32_t i = w0 + lane, set = i < size / 32 ? past[i] | biased[i] : 0u;
+            uint32_t upto = __popc(set);
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint32_t below = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= (uint32_t)o) upto += below;
+            }
+            const uint32_t total = __shfl_sync(0xffffffffu, upto, 31);
+            for (uint32_t k0 = 0; k0 < total; k0 += 32) {
+                const uint32_t k = k0 + lane;
+                /* the word that the k-th set bit is in: the first whose running count exceeds k */
+                uint32_t src = 0;
+#pragma unroll
+                for (uint32_t half = 16; half > 0; half >>= 1)
+                    if (__shfl_sync(0xffffffffu, upto, src + half - 1) <= k) src += half;
+                src &= 31;
+                const uint32_t word = __shfl_sync(0xffffffffu, set, src), before = __shfl_sync(0xffffffffu, upto, src) - __popc(word);
+                if (k >= total) continue;
+                const uint32_t at = 32 * (w0 + src) + nth_bit(word, k - before);
+                const int32_t id = first + (int32_t)at;
+                const uint32_t n = sizeof(W) == 4 ? table[at] : (table[at >> 1] >> (16 * (at & 1))) & 0xFFFFu;
+                float x = load_one(in + id);
+                if ((past[at >> 5] >> (at & 31)) & 1u) x = x > 0.0f ? __fdiv_rn(x, repetition) : __fmul_rn(x, repetition);
+                if (n != 0) x = __fsub_rn(__fsub_rn(x, __fmul_rn(frequency, (float)n)), presence);
+                if ((biased[at >> 5] >> (at & 31)) & 1u) {
+                    float sum = 0.0f;
+                    bool any = false;
+                    for (uint32_t e = 0; e < slice_biases; ++e)
+                        if (slice_id[e] == id) {
+                            sum = any ? __fadd_rn(sum, slice_bias[e]) : slice_bias[e];
+                            any = true;
+                        }
+                    x = __fadd_rn(x, sum);
+                }
+                if (mask != nullptr && !((mask[id >> 5] >> (id & 31)) & 1u)) x = kNegInf;
+                reinterpret_cast<W *>(table)[at] = (W)Vec<T>::bits(x);
+            }
+        }
+        __syncthreads();
+    }
+
+    /* dense pass: the mask, the results of the tokens with a bit, and the largest */
     unsigned long long best = 0;
     float top = kNegInf;
     uint32_t top_vec = 0;
@@ -243,28 +318,37 @@ __global__ void __launch_bounds__(kThreads, 5) logits_kernel(const __grid_consta
         const uint32_t own = own_bits(i);
         for (int32_t e = max(e0, 0); e < min(e0 + N, (int32_t)V); ++e) {
             float x = load_one(in + e);
-            const bool keep = (own >> (e - e0)) & 1u;
-            if (!keep && mask != nullptr && !((mask[e >> 5] >> (e & 31)) & 1u)) x = kNegInf;
+            if ((own >> (e - e0)) & 1u)
+                x = from_bits(reinterpret_cast<const W *>(table)[e - first], T());
+            else if (mask != nullptr && !((mask[e >> 5] >> (e & 31)) & 1u))
+                x = kNegInf;
             store_one(out + e, x);
-            const unsigned long long key = keep ? 0ull : pick_key(x, (uint32_t)e);
+            const unsigned long long key = pick_key(x, (uint32_t)e);
             best = key > best ? key : best;
         }
     };
     if (tid == 0 && v0 < min(va, v1)) edge(v0);
     if (tid == 32 && vb < v1 && v1 - 1 >= va) edge(v1 - 1);
+    /* the table's words of vector i of the slice, as a vector */
+    auto results = [&](uint32_t i) {
+        const uint4 *t = reinterpret_cast<const uint4 *>(table);
+        if (sizeof(W) == sizeof(T)) return t[i];
+        const uint4 a = t[2 * i], c = t[2 * i + 1];
+        return make_uint4(a.x | (a.y << 16), a.z | (a.w << 16), c.x | (c.y << 16), c.z | (c.w << 16));
+    };
     /* the pass, for rows with and without a table and a mask */
     auto dense = [&](auto table_on, auto mask_on) {
         constexpr bool kTable = decltype(table_on)::value, kMask = decltype(mask_on)::value;
         auto one = [&](uint32_t i, uint4 o, uint32_t may) {
             const uint32_t own = kTable ? bits_of(past8, i - v0) | bits_of(biased8, i - v0) : 0u;
-            if (kMask) o = Vec<T>::only(o, may | own);
+            if (kMask) o = Vec<T>::only(o, may);
+            if (kTable && own) o = Vec<T>::blend(o, results(i - v0), own);
             if (wide_out) {
                 __stcs(reinterpret_cast<uint4 *>(out - mis) + i, o);
             } else {
 #pragma unroll
                 for (int j = 0; j < N; ++j) store_one(out - mis + (i * N + j), Vec<T>::value(o, j));
             }
-            if (kTable && own) o = Vec<T>::only(o, ~own);
             const float m = Vec<T>::largest(o);
             if (m > top) {
                 top = m;
@@ -298,60 +382,10 @@ __global__ void __launch_bounds__(kThreads, 5) logits_kernel(const __grid_consta
     if (top > kNegInf) {
         /* this thread's own vector again: which of its tokens it was */
         const T *again = out - mis + (size_t)top_vec * N;
-        const uint32_t own = own_bits(top_vec);
         uint32_t e = 0;
-        while (e + 1 < N && (((own >> e) & 1u) || load_one(again + e) != top)) ++e;
+        while (e + 1 < N && load_one(again + e) != top) ++e;
         const unsigned long long key = pick_key(top, top_vec * N - mis + e);
         best = key > best ? key : best;
-    }
-    if (use_table) {
-        __syncthreads();
-        const float repetition = p.repetition == nullptr ? 1.0f : p.repetition[b];
-        const float presence = p.presence == nullptr ? 0.0f : p.presence[b];
-        const float frequency = p.frequency == nullptr ? 0.0f : p.frequency[b];
-        /* 32 words of bits at a time: the set ones in order, one for each lane */
-        for (uint32_t w0 = warp * 32; w0 < size / 32; w0 += kThreads) {
-            const uint32_t i = w0 + lane, set = i < size / 32 ? past[i] | biased[i] : 0u;
-            uint32_t upto = __popc(set);
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const uint32_t below = __shfl_up_sync(0xffffffffu, upto, o);
-                if (lane >= (uint32_t)o) upto += below;
-            }
-            const uint32_t total = __shfl_sync(0xffffffffu, upto, 31);
-            for (uint32_t k0 = 0; k0 < total; k0 += 32) {
-                const uint32_t k = k0 + lane;
-                /* the word that the k-th set bit is in: the first whose running count exceeds k */
-                uint32_t src = 0;
-#pragma unroll
-                for (uint32_t half = 16; half > 0; half >>= 1)
-                    if (__shfl_sync(0xffffffffu, upto, src + half - 1) <= k) src += half;
-                src &= 31;
-                const uint32_t word = __shfl_sync(0xffffffffu, set, src), before = __shfl_sync(0xffffffffu, upto, src) - __popc(word);
-                if (k >= total) continue;
-                const uint32_t at = 32 * (w0 + src) + nth_bit(word, k - before);
-                const int32_t id = first + (int32_t)at;
-                const uint32_t n = sizeof(W) == 4 ? table[at] : (table[at >> 1] >> (16 * (at & 1))) & 0xFFFFu;
-                float x = load_one(out + id); /* where the dense pass left it: out may be the logits */
-                if ((past[at >> 5] >> (at & 31)) & 1u) x = x > 0.0f ? __fdiv_rn(x, repetition) : __fmul_rn(x, repetition);
-                if (n != 0) x = __fsub_rn(__fsub_rn(x, __fmul_rn(frequency, (float)n)), presence);
-                if ((biased[at >> 5] >> (at & 31)) & 1u) {
-                    float sum = 0.0f;
-                    bool any = false;
-                    for (uint32_t e = 0; e < slice_biases; ++e)
-                        if (slice_id[e] == id) {
-                            sum = any ? __fadd_rn(sum, slice_bias[e]) : slice_bias[e];
-                            any = true;
-                        }
-                    x = __fadd_rn(x, sum);
-                }
-                if (mask != nullptr && !((mask[id >> 5] >> (id & 31)) & 1u)) x = kNegInf;
-                x = rounded(x, T());
-                store_one(out + id, x);
-                const unsigned long long key = pick_key(x, (uint32_t)id);
-                best = key > best ? key : best;
-            }
-        }
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
@@ -381,7 +415,7 @@ cudaError_t launch_logits_t(LogitsParams &p, int sms, cudaStream_t stream) {
     const uint32_t nvec = (p.vocab + N - 1) / N + 1; /* a row that starts inside a vector has one more */
     /* Few rows: eight slices each, for the latency. Many: slices of about
      * 16384 tokens, whose logits a CTA's threads hold in flight (BF16) while
-     * they count, in a table that lets three CTAs share an SM. */
+     * they count, in a table that lets four CTAs share an SM. */
     uint32_t C = 1;
     while (C < kMaxCluster && (p.rows * C < 4u * (uint32_t)sms || nvec * N / C > 16384u + N)) C *= 2;
     p.slice_vecs = (nvec + C - 1) / C;
@@ -410,16 +444,12 @@ cudaError_t launch_logits(LogitsParams p, bool bf16, int sms, cudaStream_t strea
     const int64_t per = bf16 ? 8 : 4;
     const bool aligned = ((reinterpret_cast<uintptr_t>(p.logits) | reinterpret_cast<uintptr_t>(p.out)) & 15) == 0 &&
                          (p.rows == 1 || (p.logits_row % per == 0 && p.out_row % per == 0));
-    auto *launch = launch_logits_t<float, uint16_t, false>;
-    const bool wide = p.history > 65535u;
+    auto *launch = aligned ? launch_logits_t<float, uint32_t, true> : launch_logits_t<float, uint32_t, false>;
     if (bf16)
-        launch = wide ? aligned ? launch_logits_t<__nv_bfloat16, uint32_t, true> : launch_logits_t<__nv_bfloat16, uint32_t, false>
+        launch = p.history > 65535u
+                     ? aligned ? launch_logits_t<__nv_bfloat16, uint32_t, true> : launch_logits_t<__nv_bfloat16, uint32_t, false>
                  : aligned ? launch_logits_t<__nv_bfloat16, uint16_t, true>
                            : launch_logits_t<__nv_bfloat16, uint16_t, false>;
-    else
-        launch = wide ? aligned ? launch_logits_t<float, uint32_t, true> : launch_logits_t<float, uint32_t, false>
-                 : aligned ? launch_logits_t<float, uint16_t, true>
-                           : launch_logits_t<float, uint16_t, false>;
     return launch(p, sms, stream);
 }
 
