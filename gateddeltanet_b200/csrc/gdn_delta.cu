@@ -183,12 +183,12 @@ __global__ void __launch_bounds__(kStepThreads) delta_step_kernel(const __grid_c
  * Here one CTA per SM walks a contiguous range of row blocks (up to 32 KB of
  * state each) through a ring in shared memory: one thread issues the bulk
  * copies in, eight warps advance a block in place, one thread issues the bulk
- * copy out. Four more warps stage the tokens' vectors ahead. */
+ * copy out. Three more warps stage the tokens' vectors ahead. */
 
-constexpr int kRing = 5;                  /* row blocks in flight */
+constexpr int kRing = 4;                  /* row blocks in flight (256 streams: 3 197, 4 177, 5 189, 6 193 us) */
 constexpr uint32_t kBlockBytes = 32768;
-constexpr int kItems = 4, kItemTokens = 4; /* staged token groups, tokens of one */
-constexpr int kPipeThreads = 13 * 32;     /* 8 warps of rows, the copies, 4 of tokens */
+constexpr int kItems = 3, kItemTokens = 8; /* staged token groups, tokens of one */
+constexpr int kPipeThreads = (9 + kItems) * 32; /* 8 warps of rows, the copies, one for each staged group */
 constexpr uint64_t kWaitNs = 2000000000ull;
 
 /* set when a wait of the pipeline ran out; read and cleared by the host */
@@ -314,6 +314,9 @@ __global__ void __launch_bounds__(kPipeThreads, 1) delta_pipe_kernel(const __gri
                    item_empty = item_full + 8 * kItems;
     BlockMeta *meta = reinterpret_cast<BlockMeta *>(sm + L::kMeta);
     volatile uint32_t *abort = reinterpret_cast<volatile uint32_t *>(sm + L::kBars + 8 * (2 * kRing + 2 * kItems));
+    /* a state is not wanted again before all the others have been */
+    uint64_t policy;
+    asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
     const uint32_t u0 = (uint32_t)(((uint64_t)blockIdx.x * g.units) / gridDim.x);
     const uint32_t u1 = (uint32_t)(((uint64_t)(blockIdx.x + 1) * g.units) / gridDim.x);
     T *out = static_cast<T *>(p.out);
@@ -357,9 +360,9 @@ __global__ void __launch_bounds__(kPipeThreads, 1) delta_pipe_kernel(const __gri
                     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(full + 8 * sl), "r"(bytes)
                                  : "memory");
                     asm volatile(
-                        "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                        "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1], %2, [%3], %4;" ::"r"(
                             base + sl * kBlockBytes),
-                        "l"(S), "r"(bytes), "r"(full + 8 * sl)
+                        "l"(S), "r"(bytes), "r"(full + 8 * sl), "l"(policy)
                         : "memory");
                 } else {
                     mbar_arrive(full + 8 * sl);
@@ -381,7 +384,7 @@ __global__ void __launch_bounds__(kPipeThreads, 1) delta_pipe_kernel(const __gri
         return;
     }
     if (warp > 8) {
-        /* token groups: warp 9 + j takes the groups j, j + 4, ... */
+        /* token groups: warp 9 + j takes the groups j, j + kItems, ... */
         const T *q = static_cast<const T *>(p.q), *k = static_cast<const T *>(p.k), *v = static_cast<const T *>(p.v);
         uint32_t item = 0;
         for (Walk w(p, g, u0); w.u < u1; w.next(p, g, u1)) {
@@ -500,8 +503,8 @@ __global__ void __launch_bounds__(kPipeThreads, 1) delta_pipe_kernel(const __gri
         if (go && tid == 0) {
             if (has_state) {
                 if (groups != 0 && (m.flags & kMetaLast)) mbar_arrive(item_empty + 8 * ((m.item + groups - 1) % kItems));
-                asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(m.state),
-                             "r"(base + sl * kBlockBytes), "r"(g.rows * K * 4)
+                asm volatile("cp.async.bulk.global.shared::cta.bulk_group.L2::cache_hint [%0], [%1], %2, %3;" ::"l"(m.state),
+                             "r"(base + sl * kBlockBytes), "r"(g.rows * K * 4), "l"(policy)
                              : "memory");
             }
             asm volatile("cp.async.bulk.commit_group;" ::: "memory");
@@ -515,21 +518,27 @@ __global__ void __launch_bounds__(kPipeThreads, 1) delta_pipe_kernel(const __gri
 
 template <int K>
 cudaError_t launch_step_k(const DeltaParams &p, bool bf16, int sms, cudaStream_t stream) {
-    /* The pipeline from eight row blocks per SM on, where it has filled; for
-     * long sequences (FP32 prompts) the chain of tokens bounds either kernel
-     * and the one with more CTAs is taken. */
-    Pipe g;
-    g.rows = 32;
-    for (uint32_t r = 64; r <= p.V && r * K * 4 <= kBlockBytes; r += 32)
-        if (p.V % r == 0) g.rows = r;
-    g.blocks = p.V / g.rows;
-    g.units = p.N * p.HV * g.blocks;
-    if (g.units >= 8u * (uint32_t)sms && p.tokens <= 8u * p.N) {
-        auto *kernel = bf16 ? delta_pipe_kernel<K, __nv_bfloat16> : delta_pipe_kernel<K, float>;
-        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PipeSmem<K>::kBytes);
-        if (e != cudaSuccess) return e;
-        kernel<<<sms, kPipeThreads, PipeSmem<K>::kBytes, stream>>>(p, g);
-        return cudaGetLastError();
+    /* The pipeline for one token a sequence (on average at most), from eight
+     * row blocks per SM on, where it has filled: 20 streams of 8 heads of 256 x
+     * 256 17.5 us against 21.2, 256 streams 176 against 268, 256 of 8 heads of
+     * 128 x 128 50 against 60. Not for heads of 64 x 64, a block each (256 of 8
+     * heads 19.6 against 18.5), nor for more tokens: sequences of very
+     * different lengths suit the kernel whose CTAs end on their own (256
+     * streams of 12 heads of 128 x 128 with 0 to 6 tokens 188 against 99). */
+    if constexpr (K >= 128) {
+        Pipe g;
+        g.rows = 32;
+        for (uint32_t r = 64; r <= p.V && r * K * 4 <= kBlockBytes; r += 32)
+            if (p.V % r == 0) g.rows = r;
+        g.blocks = p.V / g.rows;
+        g.units = p.N * p.HV * g.blocks;
+        if (g.units >= 8u * (uint32_t)sms && p.tokens <= p.N) {
+            auto *kernel = bf16 ? delta_pipe_kernel<K, __nv_bfloat16> : delta_pipe_kernel<K, float>;
+            cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PipeSmem<K>::kBytes);
+            if (e != cudaSuccess) return e;
+            kernel<<<sms, kPipeThreads, PipeSmem<K>::kBytes, stream>>>(p, g);
+            return cudaGetLastError();
+        }
     }
     const uint32_t rows = kStepThreads / kLanesPerRow;
     const uint32_t grid = (p.N + (p.starts != nullptr ? 1u : 0u)) * p.HV * (p.V / rows);

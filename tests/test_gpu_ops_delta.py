@@ -325,14 +325,37 @@ def test_many_states(ops, many, longest, dtype):
     assert plain.rel(a["state"], ref_s) <= STATE_TOL
 
 
-def test_many_states_uncovered_tokens(ops):
-    a, o = inputs([2] * 160, 8, 8, 64, 64, torch.bfloat16, seed=21)
-    a.update({n: torch.cat([a[n], a[n][:9]]) for n in ("q", "k", "v", "g", "beta")})
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("many", MANY[1:5], ids=str)
+def test_many_states_few_with_tokens(ops, many, dtype):
+    """No more tokens than sequences, but up to 19 in one: some states untouched, some advanced several times."""
+    n, *shape = many
+    gen = torch.Generator().manual_seed(n)
+    lengths = torch.where(torch.rand(n, generator=gen) < 0.1, 1 + torch.randint(0, 19, (n,), generator=gen), 0)
+    lengths[3] = 8
+    lengths[5] = 9
+    lengths = lengths.tolist()
+    while sum(lengths) > n:
+        lengths[lengths.index(max(lengths))] //= 2
+    a, o = inputs(lengths, *shape, dtype, seed=n)
+    o["fresh"] = (torch.rand(n, generator=gen) < 0.3).cuda()
+    o["slots"][::9] = a["state"].shape[0]
     ref_o, ref_s = plain.delta_rule(**a, **o)
-    out = torch.full_like(a["v"], float("nan"))
-    ops.delta_step(**a, **o, out=out)
-    assert bool((out[320:] == 0).all()) and plain.rel(out, ref_o) <= OUT_TOL[torch.bfloat16]
+    out = ops.delta_step(**a, **o)
+    assert plain.rel(out, ref_o) <= OUT_TOL[dtype]
     assert plain.rel(a["state"], ref_s) <= STATE_TOL
+
+
+def test_many_states_uncovered_tokens(ops):
+    for lengths in ([2] * 160, [1] * 80 + [0] * 80):
+        a, o = inputs(lengths, 8, 8, 128, 128, torch.bfloat16, seed=21)
+        T = sum(lengths)
+        a.update({n: torch.cat([a[n], a[n][:9]]) for n in ("q", "k", "v", "g", "beta")})
+        ref_o, ref_s = plain.delta_rule(**a, **o)
+        out = torch.full_like(a["v"], float("nan"))
+        ops.delta_step(**a, **o, out=out)
+        assert bool((out[T:] == 0).all()) and plain.rel(out, ref_o) <= OUT_TOL[torch.bfloat16]
+        assert plain.rel(a["state"], ref_s) <= STATE_TOL
 
 
 def test_no_wait_ran_out():
