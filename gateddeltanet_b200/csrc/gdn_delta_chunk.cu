@@ -16,10 +16,11 @@
  * The state has to come out as FP32 arithmetic would give it, from BF16
  * tensor cores with FP32 accumulators: k and q enter as they are (exact), their
  * norms and the decays scale rows of results, and each FP32 operand enters
- * as BF16 terms that sum to it: three for S0, R and D (24 bits), two for T and
- * P T (16 bits: T's unit diagonal is exact, so what is rounded is its smaller
- * part below, and the outputs are BF16). The terms of an operand are columns
- * of one MMA (N = 3 VB), whose sums are added when they are read back.
+ * as BF16 terms that sum to it: three for S0, R, D and T (24 bits), two for P T
+ * (16 bits: the outputs are BF16). The terms of an operand are columns of one
+ * MMA (N = 3 VB), whose sums are added when they are read back. (With two terms
+ * for T the states' errors against 64 bits were up to 7e-7 for independent keys
+ * and 5e-6 where all keys of a sequence are alike.)
  *
  * What bounds the walk is the chain of one chunk: three rounds of MMAs, each
  * waiting for the epilogue of the one before.
@@ -36,10 +37,10 @@ namespace {
 constexpr int kC = 64;      /* tokens of a chunk */
 constexpr uint64_t kWaitNs = 2000000000ull;
 
-/* per (chunk, value head): [T; P T] as two BF16 terms in the MMA's layout,
- * then four rows of 64 floats and the chunk's decay */
+/* per (chunk, value head): two BF16 terms of [T; P T] and the third of T in the
+ * MMA's layout, then four rows of 64 floats and the chunk's decay */
 constexpr uint32_t kTermBytes = 2 * kC * 128;       /* 128 rows of 64 BF16 */
-constexpr uint32_t kPairBytes = 2 * kTermBytes;
+constexpr uint32_t kPairBytes = 2 * kTermBytes + kC * 128;
 constexpr uint32_t kScalBytes = (4 * kC + 4) * 4;
 constexpr uint32_t kRecordBytes = (kPairBytes + kScalBytes + 127) & ~127u;
 enum { kScalC = 0, kScalBeta = 1, kScalQ = 2, kScalEnd = 3, kScalDecay = 4 };
@@ -203,10 +204,11 @@ __device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
 /* Eight values as three BF16 terms, eight significant bits each from the top:
  * with the 24 bits of FP32 their sum is the value itself (an infinity or a
  * NaN makes NaN terms, as it would make every sum it enters). Row `row` of an
- * MN-major operand of `rows` rows: the eight-value pieces term * VB / 8 + sub,
- * eight of them to a row of 128 bytes, the further ones in a second block. */
-template <int VB>
-__device__ __forceinline__ void put_terms(uint8_t *base, uint32_t rows, uint32_t row, uint32_t sub, const float (&x)[8]) {
+ * MN-major operand: the eight-value pieces term * VB / 8 + sub, eight of them to
+ * a row of 128 bytes, the further ones from piece kAt on in a second block
+ * (`second` bytes on). */
+template <int VB, uint32_t kAt = 0>
+__device__ __forceinline__ void put_terms(uint8_t *base, uint32_t second, uint32_t row, uint32_t sub, const float (&x)[8]) {
     uint32_t r[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) r[i] = __float_as_uint(x[i]);
@@ -216,7 +218,8 @@ __device__ __forceinline__ void put_terms(uint8_t *base, uint32_t rows, uint32_t
         uint32_t w[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) w[i] = __byte_perm(r[2 * i], r[2 * i + 1], 0x7632);
-        *reinterpret_cast<uint4 *>(base + (piece >> 3) * rows * 128 + piece_at(row, piece & 7)) = make_uint4(w[0], w[1], w[2], w[3]);
+        uint8_t *to = piece < 8 ? base + piece_at(row, piece) : base + second + piece_at(row, (piece & 7) + kAt);
+        *reinterpret_cast<uint4 *>(to) = make_uint4(w[0], w[1], w[2], w[3]);
         if (term < 2) {
             /* minus the term: a mixed FMA takes it from the pair, on the pipe
              * that the packing leaves free (masks and packed subtractions took
@@ -671,23 +674,27 @@ __global__ void __launch_bounds__(kPrepThreads, 3) chunk_prep_kernel(const __gri
     __syncthreads();
     product_tile<32>(A + 32 * kLdA, A + 32 * kDiag, X, -1.0f, 16 * (warp >> 2), 8 * (warp & 3), lane);
     __syncthreads();
-    /* the record, in two BF16 terms: T in the rows of the chunk's k, P T in
-     * those of its q (both lower triangular); the two change places from chunk
-     * to chunk */
+    /* the record: T in the rows of the chunk's k, P T in those of its q (both
+     * lower triangular); the two change places from chunk to chunk. The third
+     * term is T's alone. */
     const uint32_t t_row = (chunk & 1) ? kC : 0, p_row = kC - t_row;
     for (uint32_t x = tid; x < kC * 8; x += kPrepThreads) {
         const uint32_t r = x >> 3, c = (x & 7) * 8;
         float v[8];
         load8(A + r * kLdA + c, v);
-        uint32_t w[4], u[4];
+        uint32_t w[3][4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            w[e] = bf16_pair(v[2 * e], v[2 * e + 1]);
-            u[e] = bf16_pair(v[2 * e] - __uint_as_float(w[e] << 16), v[2 * e + 1] - __uint_as_float(w[e] & 0xFFFF0000u));
-        }
+        for (int term = 0; term < 3; ++term)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                w[term][e] = bf16_pair(v[2 * e], v[2 * e + 1]);
+                v[2 * e] -= __uint_as_float(w[term][e] << 16);
+                v[2 * e + 1] -= __uint_as_float(w[term][e] & 0xFFFF0000u);
+            }
         uint8_t *dst = record + piece_at(t_row + r, c >> 3);
-        *reinterpret_cast<uint4 *>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
-        *reinterpret_cast<uint4 *>(dst + kTermBytes) = make_uint4(u[0], u[1], u[2], u[3]);
+        *reinterpret_cast<uint4 *>(dst) = make_uint4(w[0][0], w[0][1], w[0][2], w[0][3]);
+        *reinterpret_cast<uint4 *>(dst + kTermBytes) = make_uint4(w[1][0], w[1][1], w[1][2], w[1][3]);
+        *reinterpret_cast<uint4 *>(record + 2 * kTermBytes + piece_at(r, c >> 3)) = make_uint4(w[2][0], w[2][1], w[2][2], w[2][3]);
     }
     /* P T in tiles of 16 rows (m) and 8 columns (n), each the sum over the
      * column blocks k = n .. 2 m + 1; a warp's four tiles have 7 to 11 together */
@@ -734,15 +741,18 @@ struct Scan {
     static constexpr uint32_t kAtoms = 3 * VB > 64 ? 2 : 1;      /* blocks of 64 columns of an operand of 3 VB */
     /* shared memory */
     static constexpr uint32_t kKQ = 0;
-    static constexpr uint32_t kPair = kKQ + (K / 64) * kBlock;   /* [T; P T] */
+    static constexpr uint32_t kPair = kKQ + (K / 64) * kBlock;   /* terms of [T; P T], T */
     static constexpr uint32_t kS = kPair + kPairBytes;           /* terms of S0, rows k */
-    static constexpr uint32_t kR = kS + kAtoms * K * 128;        /* terms of R, rows token */
-    static constexpr uint32_t kD = kR + kAtoms * kC * 128;       /* terms of the scaled D */
-    static constexpr uint32_t kScal = kD + kAtoms * kC * 128;    /* rows of scalars of two chunks */
+    /* terms of the scaled D and of R, rows token. The third term of 32 value
+     * rows takes half of a second block: R's first, D's the other half of it. */
+    static constexpr uint32_t kD = kS + kAtoms * K * 128;
+    static constexpr uint32_t kR = kD + kC * 128;
+    static constexpr uint32_t kDNext = kR + kC * 128 - kD;
+    static constexpr uint32_t kScal = kR + kAtoms * kC * 128;    /* rows of scalars of two chunks */
     static constexpr uint32_t kBar = kScal + 2 * kScalBytes;
     static constexpr uint32_t kBytes = kBar + 192; /* the kernel has no other shared memory: its base is aligned */
     /* TMEM columns */
-    static constexpr uint32_t kD1 = 0, kD3 = 4 * VB, kD4 = 8 * VB, kD4Tile = 4 * VB;
+    static constexpr uint32_t kD1 = 0, kD3 = 4 * VB, kD3Third = kD3 + 3 * VB, kD4 = 8 * VB, kD4Tile = 4 * VB;
     static constexpr uint32_t kColumns = 16 * VB;                /* a power of two that holds them */
 };
 
@@ -874,7 +884,8 @@ __global__ void __launch_bounds__(Scan<K, VB>::kThreads, Scan<K, VB>::kMinCtas)
          * uniform registers; one lane issues */
         const uint32_t leader = elect_one();
         const uint32_t s_desc = desc(base + L::kS, K * 128), r_desc = desc(base + L::kR, kC * 128),
-                       x_desc = desc(base + L::kD, kC * 128), pair_desc = desc(base + L::kPair, 16);
+                       x_desc = desc(base + L::kD, L::kDNext + 64), pair_desc = desc(base + L::kPair, 16),
+                       third_desc = desc(base + L::kPair + 2 * kTermBytes, 16);
         constexpr uint32_t kAll = 3 * VB, kTwo = 2 * VB;
         for (uint32_t c = 0; c < chunks; ++c) {
             const uint32_t st = c & 1, ph = c & 1;
@@ -903,7 +914,9 @@ __global__ void __launch_bounds__(Scan<K, VB>::kThreads, Scan<K, VB>::kMinCtas)
             if (!wait_bar_warp(full_pair, ph, abort) || !wait_bar_warp(r_ready, ph, abort)) break;
             tc_fence_after();
             if (leader) {
-                /* [T; P T] R: the first term with all of R, the second with R's first two */
+                /* [T; P T] R: the first term with all of R, the second with R's first
+                 * two, T's third with R's first, in columns of their own: the
+                 * rows of q run into other memory there and are not read */
 #pragma unroll
                 for (int kk = 0; kk < kC / 16; ++kk)
                     mma(d3, pair_desc + ((kk * 32) >> 4), r_desc + ((kk * 2048) >> 4), instr_desc(128, kAll, false, true), kk != 0);
@@ -911,6 +924,10 @@ __global__ void __launch_bounds__(Scan<K, VB>::kThreads, Scan<K, VB>::kMinCtas)
                 for (int kk = 0; kk < kC / 16; ++kk)
                     mma(d3, pair_desc + ((kTermBytes + kk * 32) >> 4), r_desc + ((kk * 2048) >> 4),
                         instr_desc(128, kTwo, false, true), true);
+#pragma unroll
+                for (int kk = 0; kk < kC / 16; ++kk)
+                    mma(tmem + L::kD3Third, third_desc - st * ((kC * 128) >> 4) + ((kk * 32) >> 4), r_desc + ((kk * 2048) >> 4),
+                        instr_desc(128, VB, false, true), kk != 0);
                 commit(d3_full);
                 commit(empty_pair);
             }
@@ -964,7 +981,7 @@ __global__ void __launch_bounds__(Scan<K, VB>::kThreads, Scan<K, VB>::kMinCtas)
         fetch(0);
 #pragma unroll
         for (int t = 0; t < L::kOwn; ++t) {
-            if (has_s) put_terms<VB>(sm + L::kS, K, 128 * (tile0 + t) + ln, sub, s[t]);
+            if (has_s) put_terms<VB>(sm + L::kS, K * 128, 128 * (tile0 + t) + ln, sub, s[t]);
             fence_async();
             warp_arrive(s_ready + 8 * (tile0 + t));
         }
@@ -1003,7 +1020,7 @@ __global__ void __launch_bounds__(Scan<K, VB>::kThreads, Scan<K, VB>::kMinCtas)
                 } else {
                     /* rows without a token have zeros for all of it */
                     scale_add(f0, x, bv);
-                    put_terms<VB>(sm + L::kR, kC, i, sub, bv);
+                    put_terms<VB>(sm + L::kR, kC * 128, i, sub, bv);
                     fence_async();
                     tc_fence_before();
                     warp_arrive(r_ready);
@@ -1025,9 +1042,13 @@ __global__ void __launch_bounds__(Scan<K, VB>::kThreads, Scan<K, VB>::kMinCtas)
                         }
                     }
                 } else {
+                    uint32_t third[8];
+                    __syncwarp();
+                    tc_ld8(tmem + L::kD3Third + at, third);
+                    tc_wait();
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) x[e] *= f2;
-                    put_terms<VB>(sm + L::kD, kC, i, sub, x);
+                    for (int e = 0; e < 8; ++e) x[e] = f2 * (x[e] + __uint_as_float(third[e]));
+                    put_terms<VB, 4>(sm + L::kD, L::kDNext, i, sub, x);
                     fence_async();
                     tc_fence_before();
                     warp_arrive(d_ready);
@@ -1040,7 +1061,7 @@ __global__ void __launch_bounds__(Scan<K, VB>::kThreads, Scan<K, VB>::kMinCtas)
                 tc_sum3<VB>(d4 + L::kD4Tile * (tile0 + t) + at, x);
                 add_to(x, s[t]);
                 if (c + 1 < chunks) {
-                    if (has_s) put_terms<VB>(sm + L::kS, K, 128 * (tile0 + t) + ln, sub, s[t]);
+                    if (has_s) put_terms<VB>(sm + L::kS, K * 128, 128 * (tile0 + t) + ln, sub, s[t]);
                     fence_async();
                     tc_fence_before();
                     warp_arrive(s_ready + 8 * (tile0 + t));

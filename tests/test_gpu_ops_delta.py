@@ -173,6 +173,17 @@ def test_decays(ops, rule, decay):
     compare(getattr(ops, rule), a, o, out_tol(rule, torch.bfloat16))
 
 
+@pytest.mark.parametrize("shape", [(1, 1, 64, 64), (2, 2, 256, 256)], ids=str)
+@pytest.mark.parametrize("alike", [0.3, 0.0])
+def test_chunk_of_like_keys(ops, alike, shape):
+    """All keys of a sequence nearly or fully the same: the chunk's triangular
+    system has a condition number of up to about 64 (its tokens), by which the
+    rounding of an FP32 solution, 2^-24, may grow: 3.8e-6 more than elsewhere."""
+    a, o = inputs([400, 65], *shape, torch.bfloat16, seed=31)
+    a["k"] = (a["k"].float() * alike + 1).bfloat16()
+    compare(ops.delta_chunk, a, o, CHUNK_OUT_TOL, state_tol=STATE_TOL + 64 * 2 ** -24)
+
+
 @pytest.mark.parametrize("rule", ["delta_step", "delta_chunk"])
 def test_zero_keys_and_queries(ops, rule):
     """Rows of zeros (padding) have no norm: they give zeros and only decay the state."""
