@@ -23,7 +23,10 @@
  * and 5e-6 where all keys of a sequence are alike.)
  *
  * What bounds the walk is the chain of one chunk: three rounds of MMAs, each
- * waiting for the epilogue of the one before.
+ * waiting for the epilogue of the one before. Measured with 8 heads of 256 x
+ * 256: 4096 tokens 158 us (2500 token by token), of which the first kernel
+ * takes 24 and a chunk of the second 3900 cycles; 24 prompts of up to 2047
+ * tokens 622 us.
  */
 #include "gdn_ops.h"
 

@@ -65,6 +65,8 @@ int delta_params(const char *who, const GdnB200DeltaArgs *a, gdn::ops::DeltaPara
         return failf("%s: %u value heads do not share %u query/key heads evenly", who, a->v_heads, a->heads);
     if (a->tokens > 0x7fffffffu || a->sequences > 0x3fffffu)
         return failf("%s: %u tokens in %u sequences are too many", who, a->tokens, a->sequences);
+    if (((uint64_t)a->sequences + 1) * a->v_heads * (a->value_dim / 16) > 0x7fffffffu)
+        return failf("%s: %u sequences of %u heads are too many", who, a->sequences, a->v_heads);
     if (a->starts == nullptr && a->tokens != a->sequences)
         return failf("%s: without starts every sequence has one token (%u tokens, %u sequences)", who, a->tokens,
                      a->sequences);

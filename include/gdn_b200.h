@@ -301,7 +301,8 @@ int gdn_b200_test_tile_gemm(uint32_t m, uint32_t k, uint32_t n, const float *w, 
  * pool is one block [v_heads][V][K] on a 16-byte boundary. A sequence
  * whose slot lies outside the pool changes no state and gives zeros, as do
  * tokens that no sequence covers. Entries of starts are clamped to [0, tokens].
- * key_dim is 64, 128 or 256, value_dim a multiple of 32 up to 256. */
+ * key_dim is 64, 128 or 256, value_dim a multiple of 32 up to 256. out must
+ * not overlap the inputs. */
 typedef struct {
     const void *q, *k, *v;
     const float *g, *beta;
@@ -343,7 +344,8 @@ int gdn_b200_delta_status(int device);
  *   mask bit clear:    x = -inf
  * each operation rounded to FP32, the result once to the logits' type. picks
  * gets the lowest index of the row's largest result; NaN is never picked, and
- * -1 says that nothing is above -inf. logits and out (may be logits itself):
+ * -1 says that nothing is above -inf. logits and out (logits itself, or memory
+ * apart from it):
  * [rows][vocab], BF16 (dtype 1) or FP32 (dtype 0). tokens [rows][history]
  * int32 with the first lens[row] in use (NULL: all) of which prompt_lens[row]
  * are the prompt (NULL: none); repetition, presence, frequency FP32 [rows];

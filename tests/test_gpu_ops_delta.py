@@ -260,6 +260,16 @@ def test_state_pool_beyond_32_bit_offsets(ops):
         assert plain.rel(state[at], ref_s) <= STATE_TOL
 
 
+@pytest.mark.parametrize("n", [2047, 2049])
+def test_chunk_of_very_many_sequences(ops, n):
+    """Both ways of finding a record's sequence: by all threads at once, and by halving."""
+    gen = torch.Generator().manual_seed(n)
+    lengths = torch.randint(0, 3, (n,), generator=gen).tolist()
+    lengths[n // 2] = 130
+    a, o = inputs(lengths, 1, 1, 64, 32, torch.bfloat16, seed=n)
+    compare(ops.delta_chunk, a, o, CHUNK_OUT_TOL)
+
+
 def test_chunk_then_steps_is_one_sequence(ops):
     """A prompt through delta_chunk and its next tokens through delta_step."""
     a, o = inputs([140], 2, 2, 256, 256, torch.bfloat16, seed=17)

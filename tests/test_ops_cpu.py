@@ -36,7 +36,8 @@ def delta_args(**change):
     (dict(heads=0), "heads"), (dict(heads=2, v_heads=3), "heads"), (dict(starts=0), "without starts"),
     (dict(sequences=0), "no sequence"), (dict(slots=0, state_slots=1), "slots"), (dict(state=FAKE + 4), "16-byte"),
     (dict(state=0), "state"), (dict(state_slot=4098), "state slots"), (dict(state_slot=64), "state slots"), (dict(q=0), "missing"),
-    (dict(beta=0), "missing"), (dict(tokens=2 ** 32 - 1), "too many")])
+    (dict(beta=0), "missing"), (dict(tokens=2 ** 32 - 1), "too many"),
+    (dict(sequences=2 ** 22), "too many"), (dict(sequences=2 ** 21, v_heads=1024), "too many")])
 @pytest.mark.parametrize("entry", ["gdn_b200_delta_step", "gdn_b200_delta_chunk"])
 def test_delta_refusals(lib, entry, change, reason):
     assert getattr(lib, entry)(delta_args(**change)) == -1
