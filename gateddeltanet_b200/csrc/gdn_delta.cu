@@ -15,8 +15,8 @@
  * token's vectors, so that their norms are formed while it arrives. q, k and
  * the scalars of up to a warp count of tokens are staged in shared memory in
  * FP32; the state stays in registers over all tokens of the sequence. Measured
- * with BF16 heads of 256 x 256: one stream of 8 heads 4.2 us, 16 streams 14.7 us
- * (4.6 TB/s of state); the pipeline below takes over from there: 64 streams 49
+ * with BF16 heads of 256 x 256: one stream of 8 heads 4.2 us, 16 streams 13.2 us
+ * (5.1 TB/s of state); the pipeline below takes over from there: 64 streams 49
  * us (5.5 TB/s), 256 streams 176 us (6.1 TB/s, 0.94 of a copy's).
  */
 #include "gdn_ops.h"
@@ -29,7 +29,9 @@ namespace ops {
 namespace {
 
 constexpr int kLanesPerRow = 8;
-constexpr int kStepThreads = 256;
+/* 16 rows a CTA: five of them share an SM with heads of 256 (64 streams of two
+ * tokens 64 us, with 32 rows 80, with 8 rows 70) */
+constexpr int kStepThreads = 128;
 
 __device__ __forceinline__ float to_float(float x) { return x; }
 __device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
@@ -182,7 +184,7 @@ __global__ void __launch_bounds__(kStepThreads) delta_step_kernel(const __grid_c
 /* ------------------------------------------------- many states: a pipeline
  *
  * With many states the kernel above is held up by its own phases (a CTA loads,
- * computes and stores in turn, and two CTAs fill an SM's registers): 4.0 TB/s
+ * computes and stores in turn, and five CTAs fill an SM's registers): 5.4 TB/s
  * for 256 streams, against 6.1.
  * Here one CTA per SM walks a contiguous range of row blocks (up to 32 KB of
  * state each) through a ring in shared memory: one thread issues the bulk
@@ -192,6 +194,7 @@ __global__ void __launch_bounds__(kStepThreads) delta_step_kernel(const __grid_c
 constexpr int kRing = 4;                  /* row blocks in flight (256 streams: 3 197, 4 177, 5 189, 6 193 us) */
 constexpr uint32_t kBlockBytes = 32768;
 constexpr int kItems = 3, kItemTokens = 8; /* staged token groups, tokens of one */
+constexpr int kRowThreads = 256;
 constexpr int kPipeThreads = (9 + kItems) * 32; /* 8 warps of rows, the copies, one for each staged group */
 constexpr uint64_t kWaitNs = 2000000000ull;
 
@@ -245,7 +248,7 @@ __device__ __forceinline__ bool rows_all(bool v) {
     asm volatile(
         "{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n barrier.red.and.pred q, 1, %2, p;\n selp.u32 %0, 1, 0, q;\n}\n"
         : "=r"(r)
-        : "r"((uint32_t)v), "r"(kStepThreads)
+        : "r"((uint32_t)v), "r"(kRowThreads)
         : "memory");
     return r != 0;
 }
@@ -449,7 +452,7 @@ __global__ void __launch_bounds__(kPipeThreads, 1) delta_pipe_kernel(const __gri
         }
         return;
     }
-    if (p.starts != nullptr && blockIdx.x + 1 == gridDim.x) zero_uncovered<T>(p, tid, kStepThreads);
+    if (p.starts != nullptr && blockIdx.x + 1 == gridDim.x) zero_uncovered<T>(p, tid, kRowThreads);
     /* rows: eight lanes each, 32 rows at a time */
     const uint32_t r8 = tid / kLanesPerRow, l8 = tid & (kLanesPerRow - 1);
     bool go = true;
@@ -463,11 +466,11 @@ __global__ void __launch_bounds__(kPipeThreads, 1) delta_pipe_kernel(const __gri
         float *rows = reinterpret_cast<float *>(sm + sl * kBlockBytes);
         if (ok && !has_state)
             for (uint32_t t = m.t0; t < m.t1; ++t)
-                for (uint32_t r = tid; r < g.rows; r += kStepThreads)
+                for (uint32_t r = tid; r < g.rows; r += kRowThreads)
                     store_out(out + (int64_t)t * p.out_token + (int64_t)m.h * p.out_head + m.row0 + r, 0.0f);
         const uint32_t groups = has_state ? (m.t1 - m.t0 + kItemTokens - 1) / kItemTokens : 0;
         if (has_state && groups == 0)
-            for (uint32_t j = tid; j < g.rows * K / 4; j += kStepThreads)
+            for (uint32_t j = tid; j < g.rows * K / 4; j += kRowThreads)
                 reinterpret_cast<float4 *>(rows)[j] = make_float4(0.f, 0.f, 0.f, 0.f);
         for (uint32_t gi = 0; ok && gi < groups; ++gi) {
             const uint32_t item = m.item + gi, is = item % kItems;
@@ -476,7 +479,7 @@ __global__ void __launch_bounds__(kPipeThreads, 1) delta_pipe_kernel(const __gri
             const uint8_t *it = sm + L::kItemAt + is * L::kItem;
             const uint32_t nt = min((uint32_t)kItemTokens, m.t1 - m.t0 - gi * kItemTokens);
             const bool zero = gi == 0 && (m.flags & kMetaFresh);
-            for (uint32_t r = r8; r < g.rows; r += kStepThreads / kLanesPerRow) {
+            for (uint32_t r = r8; r < g.rows; r += kRowThreads / kLanesPerRow) {
                 float4 *S = reinterpret_cast<float4 *>(rows + r * K) + l8;
                 float4 s[kVec];
 #pragma unroll
@@ -524,8 +527,8 @@ template <int K>
 cudaError_t launch_step_k(const DeltaParams &p, bool bf16, int sms, cudaStream_t stream) {
     /* The pipeline for one token a sequence (on average at most), from eight
      * row blocks per SM on, where it has filled: 20 streams of 8 heads of 256 x
-     * 256 17.5 us against 21.2, 256 streams 176 against 268, 256 of 8 heads of
-     * 128 x 128 50 against 60. Not for heads of 64 x 64, a block each (256 of 8
+     * 256 18.1 us against 18.4, 64 streams 49 against 56, 256 of 8 heads of 128
+     * x 128 50 against 56. Not for heads of 64 x 64, a block each (256 of 8
      * heads 19.6 against 18.5), nor for more tokens: sequences of very
      * different lengths suit the kernel whose CTAs end on their own (256
      * streams of 12 heads of 128 x 128 with 0 to 6 tokens 188 against 99). */
