@@ -15,8 +15,8 @@
  * token's vectors, so that their norms are formed while it arrives. q, k and
  * the scalars of up to a warp count of tokens are staged in shared memory in
  * FP32; the state stays in registers over all tokens of the sequence. Measured
- * with BF16 heads of 256 x 256: one stream of 8 heads 4.2 us, 16 streams 13.2 us
- * (5.1 TB/s of state); the pipeline below takes over from there: 64 streams 49
+ * with BF16 heads of 256 x 256: one stream of 8 heads 3.7 us, 16 streams 13.0 us
+ * (5.2 TB/s of state); the pipeline below takes over from there: 64 streams 49
  * us (5.5 TB/s), 256 streams 176 us (6.1 TB/s, 0.94 of a copy's).
  */
 #include "gdn_ops.h"

@@ -40,7 +40,9 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr uint32_t kThreads = 256;
-constexpr int kUnroll = 4;      /* 16-byte vectors of a thread in flight */
+/* 16-byte vectors of a thread in flight: with four, four CTAs share an SM, with
+ * two, five (256 rows of 131072 BF16 68 and 65 us) */
+constexpr int kUnroll = 2;
 constexpr int kHistoryUnroll = 8;
 constexpr int kMaxCluster = 8;  /* portable cluster size */
 
@@ -134,7 +136,7 @@ __device__ __forceinline__ uint32_t nth_bit(uint32_t w, uint32_t n) {
 /* W: the type of a token's count, as wide as T or wider. kAligned: every row of logits and of out
  * starts on a 16-byte boundary. */
 template <typename T, typename W, bool kAligned>
-__global__ void __launch_bounds__(kThreads, 4) logits_kernel(const __grid_constant__ LogitsParams p) {
+__global__ void __launch_bounds__(kThreads, 5) logits_kernel(const __grid_constant__ LogitsParams p) {
     constexpr int N = Vec<T>::kN;
     constexpr float kNegInf = -__builtin_huge_valf();
     extern __shared__ __align__(16) uint32_t table[]; /* counts of the slice, two bits each, the slice's biases */
@@ -413,7 +415,7 @@ template <typename T, typename W, bool kAligned>
 cudaError_t launch_logits_t(LogitsParams &p, int sms, cudaStream_t stream) {
     constexpr uint32_t N = Vec<T>::kN;
     const uint32_t nvec = (p.vocab + N - 1) / N + 1; /* a row that starts inside a vector has one more */
-    /* Slices: two CTAs for each SM, and a table of at most 32 KB, so that four
+    /* Slices: two CTAs for each SM, and a table of at most 32 KB, so that five
      * fit. 256 rows of 32000: FP32 32 us with four slices, 40 with two; BF16 23 with
      * four, 19 with two. 100 rows FP32: 16.5 with eight, 11.6 with four. */
     uint32_t C = 1;
