@@ -79,16 +79,11 @@ __device__ __forceinline__ float advance(float4 (&s)[kVec], const float4 *q4, co
 template <typename T>
 __device__ __forceinline__ void zero_uncovered(const DeltaParams &p, uint32_t at, uint32_t of) {
     T *out = static_cast<T *>(p.out);
-    uint32_t first, t0, t1, last;
-    sequence_tokens(p, 0, first, t0);
-    sequence_tokens(p, p.N - 1, t1, last);
+    const Covered c = covered_tokens(p);
     const uint32_t width = p.HV * p.V;
-    for (uint32_t t = 0; t < p.tokens; ++t) {
-        if (t == first) t = last;
-        if (t >= p.tokens) break;
+    for (uint32_t t = c.first_outside(); t < p.tokens; t = c.next_outside(t))
         for (uint32_t i = at; i < width; i += of)
             store_out(out + (int64_t)t * p.out_token + (int64_t)(i / p.V) * p.out_head + i % p.V, 0.0f);
-    }
 }
 
 template <int K, typename T>

@@ -31,16 +31,31 @@ struct DeltaParams {
 
 /* Tokens [t0, t1) of sequence n, clamped to the packed tensors so that no
  * content of starts leads out of them. */
-__device__ __forceinline__ void sequence_tokens(const DeltaParams &p, uint32_t n, uint32_t &t0, uint32_t &t1) {
+__host__ __device__ __forceinline__ void sequence_tokens(const DeltaParams &p, uint32_t n, uint32_t &t0, uint32_t &t1) {
     if (p.starts == nullptr) {
         t0 = n;
         t1 = n + 1;
         return;
     }
     const int32_t a = p.starts[n], b = p.starts[n + 1];
-    t0 = a < 0 ? 0u : min((uint32_t)a, p.tokens);
-    t1 = b < 0 ? 0u : min((uint32_t)b, p.tokens);
+    t0 = a < 0 ? 0u : ((uint32_t)a < p.tokens ? (uint32_t)a : p.tokens);
+    t1 = b < 0 ? 0u : ((uint32_t)b < p.tokens ? (uint32_t)b : p.tokens);
     if (t1 < t0) t1 = t0;
+}
+
+/* Tokens [first, end) from the first sequence's begin to the last one's end,
+ * and the walk over the others, which belong to no sequence. Never end < first,
+ * so that the walk moves forward whatever starts holds. */
+struct Covered {
+    uint32_t first, end;
+    __host__ __device__ __forceinline__ uint32_t first_outside() const { return first == 0 ? end : 0; }
+    __host__ __device__ __forceinline__ uint32_t next_outside(uint32_t t) const { return t + 1 == first ? end : t + 1; }
+};
+__host__ __device__ __forceinline__ Covered covered_tokens(const DeltaParams &p) {
+    uint32_t first, t0, t1, last;
+    sequence_tokens(p, 0, first, t0);
+    sequence_tokens(p, p.N - 1, t1, last);
+    return {first, last < first ? first : last};
 }
 
 /* Pool slot of sequence n; negative if it has none (its tokens then give

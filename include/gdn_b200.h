@@ -300,7 +300,9 @@ int gdn_b200_test_tile_gemm(uint32_t m, uint32_t k, uint32_t n, const float *w, 
  * elements; the innermost dimension (K or V) is contiguous, and a slot of the
  * pool is one block [v_heads][V][K] on a 16-byte boundary. A sequence
  * whose slot lies outside the pool changes no state and gives zeros, as do
- * tokens that no sequence covers. Entries of starts are clamped to [0, tokens].
+ * tokens that no sequence covers. Entries of starts are clamped to [0, tokens];
+ * where they decrease the call ends all the same, within its tensors, but with
+ * outputs and states that are not specified.
  * key_dim is 64, 128 or 256, value_dim a multiple of 32 up to 256. out must
  * not overlap the inputs. */
 typedef struct {
