@@ -782,12 +782,13 @@ __global__ void __launch_bounds__(Scan<K, VB>::kThreads, Scan<K, VB>::kMinCtas)
     const uint32_t bar = base + L::kBar;
     const uint32_t full_kq = bar, empty_k = bar + 16, empty_q = bar + 32, full_pair = bar + 40, empty_pair = bar + 48,
                    s_ready = bar + 56, d1_full = bar + 72, r_ready = bar + 80, d3_full = bar + 88, d_ready = bar + 96,
-                   d4_full = bar + 104, drain = bar + 120, full_scal = bar + 128;
+                   d4_full = bar + 104, drain = bar + 120, full_scal = bar + 128, empty_scal = bar + 160;
     uint32_t *slot = reinterpret_cast<uint32_t *>(sm + L::kBar + 144);
     volatile uint32_t *abort = reinterpret_cast<volatile uint32_t *>(sm + L::kBar + 152);
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
             mbar_init(full_scal + 8 * i, 1);
+            mbar_init(empty_scal + 8 * i, L::kEpiWarps);
             mbar_init(full_kq + 8 * i, L::kLoadThreads / 32);
             mbar_init(empty_k + 8 * i, 1);
             mbar_init(s_ready + 8 * i, L::kTokenWarps);
@@ -857,8 +858,10 @@ __global__ void __launch_bounds__(Scan<K, VB>::kThreads, Scan<K, VB>::kMinCtas)
         cp_async_wait_all();
     } else if (warp == kRecWarp) {
         if (lane == 0) {
-            /* a chunk's scalars may take the place of those of two chunks
-             * before: [T; P T] of the chunk between has been used */
+            /* [T; P T] of a chunk once the MMAs have read that of the chunk
+             * before, the next chunk's scalars once every epilogue warp has
+             * read those of two chunks before it: not every one of them waits
+             * for these MMAs. */
             auto copy = [&](uint32_t dst, const uint8_t *src, uint32_t bytes, uint32_t full) {
                 asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(full), "r"(bytes) : "memory");
                 asm volatile(
@@ -866,20 +869,24 @@ __global__ void __launch_bounds__(Scan<K, VB>::kThreads, Scan<K, VB>::kMinCtas)
                     "l"(src), "r"(bytes), "r"(full)
                     : "memory");
             };
-            uint32_t c = 0;
-            for (; c < chunks; ++c) {
-                if (c >= 1 && !wait_bar<true>(empty_pair, (c - 1) & 1u, abort)) break;
-                const uint8_t *src = records + ((size_t)(rec0 + c) * p.HV + h) * kRecordBytes;
-                if (c == 0) copy(base + L::kScal, src + kPairBytes, kScalBytes, full_scal);
+            const uint8_t *src = records + ((size_t)rec0 * p.HV + h) * kRecordBytes;
+            const size_t step = (size_t)p.HV * kRecordBytes;
+            uint32_t pairs = 0, scals = 1; /* copies begun */
+            copy(base + L::kScal, src + kPairBytes, kScalBytes, full_scal);
+            for (; pairs < chunks; src += step) {
+                if (pairs >= 1 && !wait_bar<true>(empty_pair, (pairs - 1) & 1u, abort)) break;
                 copy(base + L::kPair, src, kPairBytes, full_pair);
-                if (c + 1 < chunks)
-                    copy(base + L::kScal + ((c + 1) & 1) * kScalBytes, src + (size_t)p.HV * kRecordBytes + kPairBytes, kScalBytes,
-                         full_scal + 8 * ((c + 1) & 1));
+                if (++pairs == chunks) break;
+                const uint32_t st = scals & 1;
+                if (scals >= 2 && !wait_bar<true>(empty_scal + 8 * st, (scals / 2 - 1) & 1u, abort)) break;
+                copy(base + L::kScal + st * kScalBytes, src + step + kPairBytes, kScalBytes, full_scal + 8 * st);
+                ++scals;
             }
             /* the last copies land before the CTA ends (an abort does not stop them) */
+            auto landed = [&](uint32_t x) { return mbar_try(full_scal + 8 * (x & 1), (x >> 1) & 1u); };
             const uint64_t w0 = gtimer();
-            while (!(mbar_try(full_pair, (c - 1) & 1u) &&
-                     mbar_try(full_scal + 8 * (min(c, chunks - 1) & 1), (min(c, chunks - 1) >> 1) & 1u)) &&
+            while (!((pairs == 0 || mbar_try(full_pair, (pairs - 1) & 1u)) && landed(scals - 1) &&
+                     (scals == 1 || landed(scals - 2))) &&
                    gtimer() - w0 < kWaitNs) {
             }
         }
@@ -1013,6 +1020,7 @@ __global__ void __launch_bounds__(Scan<K, VB>::kThreads, Scan<K, VB>::kMinCtas)
 #pragma unroll
                     for (int e = 0; e < 8; ++e) bv[e] = beta * __uint_as_float((e & 1) ? (u[e >> 1] & 0xFFFF0000u) : (u[e >> 1] << 16));
                 }
+                warp_arrive(empty_scal + 8 * ph);
                 if (c + 1 < chunks) fetch(c + 1);
                 float o[8];
                 if (!(ok = wait_bar_warp(d1_full, ph, abort))) break;
@@ -1057,6 +1065,8 @@ __global__ void __launch_bounds__(Scan<K, VB>::kThreads, Scan<K, VB>::kMinCtas)
                     tc_fence_before();
                     warp_arrive(d_ready);
                 }
+            } else {
+                warp_arrive(empty_scal + 8 * ph);
             }
 #pragma unroll
             for (int t = 0; t < L::kOwn; ++t) {

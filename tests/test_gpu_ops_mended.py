@@ -34,3 +34,25 @@ def test_decreasing_starts_end(ops, rule, starts, pad):
     torch.cuda.synchronize()
     assert bool((wide[:10] == 7).all()) and bool((wide[80:] == 7).all())
     assert bool((state[0] == 7).all()) and bool((state[-1] == 7).all())
+
+
+@pytest.mark.parametrize("shape", [(8, 8, 256, 256), (2, 8, 128, 128), (3, 3, 64, 32)], ids=str)
+def test_chunk_same_bits_beside_other_work(ops, shape):
+    """Warps that come late (the SMs are shared with a product on another stream) still read their own chunk's scalars."""
+    a, o = inputs([1500, 700, 64], *shape, torch.bfloat16, seed=41)
+    start = a.pop("state")
+    first = None
+    side = torch.cuda.Stream()
+    x = torch.randn(2048, 2048, device="cuda", dtype=torch.bfloat16)
+    for _ in range(20):
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            for _ in range(4):
+                y = x @ x
+        state = start.clone()
+        out = ops.delta_chunk(**a, state=state, **o)
+        if first is None:
+            first = (out, state)
+        assert torch.equal(out, first[0]) and torch.equal(state, first[1])
+    torch.cuda.synchronize()
+    assert y.shape == x.shape
