@@ -411,12 +411,22 @@ __global__ void __launch_bounds__(kThreads, 5) logits_kernel(const __grid_consta
     }
 }
 
+/* The largest table: a row of kMaxVocab tokens in kMaxCluster slices. Every
+ * call sets this one limit, so that calls of other threads and calls captured
+ * into a graph before keep theirs. */
+template <typename T, typename W>
+constexpr size_t max_smem() {
+    constexpr size_t N = Vec<T>::kN, vecs = (kMaxVocab + N - 1) / N + 1, size = ((vecs + kMaxCluster - 1) / kMaxCluster * N + 127) & ~(size_t)127;
+    return size * sizeof(W) + size / 4 + 8 * (size_t)kMaxBiases;
+}
+
 template <typename T, typename W, bool kAligned>
 cudaError_t launch_logits_t(LogitsParams &p, int sms, cudaStream_t stream) {
     constexpr uint32_t N = Vec<T>::kN;
     const uint32_t nvec = (p.vocab + N - 1) / N + 1; /* a row that starts inside a vector has one more */
     /* Slices: two CTAs for each SM, and a table of at most 32 KB, so that five
-     * fit. 256 rows of 32000: FP32 32 us with four slices, 40 with two; BF16 23 with
+     * fit, as far as eight slices go (FP32 rows of more than 65536 tokens have
+     * up to 128 KB). 256 rows of 32000: FP32 32 us with four slices, 40 with two; BF16 23 with
      * four, 19 with two. 100 rows FP32: 16.5 with eight, 11.6 with four. */
     uint32_t C = 1;
     while (C < kMaxCluster && (p.rows * C < 2u * (uint32_t)sms || nvec * N / C * sizeof(W) > 32768u + 64)) C *= 2;
@@ -424,7 +434,9 @@ cudaError_t launch_logits_t(LogitsParams &p, int sms, cudaStream_t stream) {
     const bool use_table = p.tokens != nullptr || p.bias_ids != nullptr;
     const size_t size = (p.slice_vecs * N + 127) & ~(size_t)127;
     const size_t smem = use_table ? size * sizeof(W) + size / 4 + 8 * (size_t)p.biases : 0;
-    cudaError_t e = cudaFuncSetAttribute(logits_kernel<T, W, kAligned>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    static_assert(max_smem<T, W>() <= 227 * 1024 - 1024, "the largest table");
+    cudaError_t e = cudaFuncSetAttribute(logits_kernel<T, W, kAligned>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         (int)max_smem<T, W>());
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(p.rows * C);

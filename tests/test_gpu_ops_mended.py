@@ -56,3 +56,36 @@ def test_chunk_same_bits_beside_other_work(ops, shape):
         assert torch.equal(out, first[0]) and torch.equal(state, first[1])
     torch.cuda.synchronize()
     assert y.shape == x.shape
+
+
+def test_threads_with_vocabularies_of_different_sizes(ops):
+    """Calls of several host threads, each on its own stream, with tables of very different sizes."""
+    import threading
+
+    import gateddeltanet_b200 as gdn
+    from test_ops_cpu import logits_args
+    lib = gdn.lib()
+    wrong, keep = [], []
+
+    def work(vocab):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            logits = torch.zeros(1, vocab, device="cuda")
+            tokens = torch.zeros(1, 4, dtype=torch.int32, device="cuda")
+            picks = torch.empty(1, dtype=torch.int32, device="cuda")
+            keep.append((logits, tokens, picks))
+            args = logits_args(logits=logits.data_ptr(), out=logits.data_ptr(), picks=picks.data_ptr(), tokens=tokens.data_ptr(),
+                               lens=0, prompt_lens=0, repetition=0, presence=0, frequency=0, bias_ids=0, bias=0, mask=0,
+                               stream=torch.cuda.current_stream().cuda_stream, logits_row=vocab, out_row=vocab, tokens_row=4,
+                               rows=1, vocab=vocab, history=4, biases=0)
+            for _ in range(4000):
+                if lib.gdn_b200_constrain_logits(args) != 0:
+                    wrong.append((vocab, gdn.last_error()))
+                    return
+    torch.zeros(1, device="cuda")
+    threads = [threading.Thread(target=work, args=(v,)) for v in (200000, 1000, 262144, 50)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not wrong
