@@ -538,17 +538,12 @@ cudaError_t launch_step_k(const DeltaParams &p, bool bf16, int sms, cudaStream_t
             auto *kernel = bf16 ? delta_pipe_kernel<K, __nv_bfloat16> : delta_pipe_kernel<K, float>;
             cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PipeSmem<K>::kBytes);
             if (e != cudaSuccess) return e;
-            kernel<<<sms, kPipeThreads, PipeSmem<K>::kBytes, stream>>>(p, g);
-            return cudaGetLastError();
+            return launch(kernel, dim3(sms), kPipeThreads, PipeSmem<K>::kBytes, stream, p, g);
         }
     }
     const uint32_t rows = kStepThreads / kLanesPerRow;
     const uint32_t grid = (p.N + (p.starts != nullptr ? 1u : 0u)) * p.HV * (p.V / rows);
-    if (bf16)
-        delta_step_kernel<K, __nv_bfloat16><<<grid, kStepThreads, 0, stream>>>(p);
-    else
-        delta_step_kernel<K, float><<<grid, kStepThreads, 0, stream>>>(p);
-    return cudaGetLastError();
+    return launch(bf16 ? delta_step_kernel<K, __nv_bfloat16> : delta_step_kernel<K, float>, dim3(grid), kStepThreads, 0, stream, p);
 }
 
 }  // namespace

@@ -1130,8 +1130,9 @@ cudaError_t launch_chunk_k(const DeltaParams &p, uint8_t *workspace, int sms, cu
     cudaError_t e = cudaFuncSetAttribute(chunk_prep_kernel<K>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          (int)PrepSmem<K>::kBytes);
     if (e != cudaSuccess) return e;
-    chunk_prep_kernel<K><<<dim3(record_count(p.tokens, p.N), p.HV), kPrepThreads, PrepSmem<K>::kBytes, stream>>>(p, records, order);
-    if ((e = cudaGetLastError()) != cudaSuccess) return e;
+    e = launch(chunk_prep_kernel<K>, dim3(record_count(p.tokens, p.N), p.HV), kPrepThreads, PrepSmem<K>::kBytes, stream, p, records,
+               order);
+    if (e != cudaSuccess) return e;
     const uint32_t ctas16 = p.N * p.HV * (p.V / 16);
     if (ctas16 > (uint32_t)sms) return launch_scan<K, 32>(p, records, order, stream);
     return launch_scan<K, 16>(p, records, order, stream);

@@ -83,6 +83,18 @@ constexpr uint32_t kMaxHistory = (1u << 20) - 1;
 constexpr uint32_t kMaxBiases = 2047;  /* searched once for each biased token */
 constexpr uint32_t kMaxVocab = 1u << 18;
 
+/* kernel<<<grid, block, smem, stream>>>(args...) and this launch's own result:
+ * cudaGetLastError would also give that of a call before it. */
+template <typename... Params, typename... Args>
+cudaError_t launch(void (*kernel)(Params...), dim3 grid, uint32_t block, size_t smem, cudaStream_t stream, Args... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(block);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 cudaError_t launch_delta_step(const DeltaParams &p, bool bf16, int sms, cudaStream_t stream);
 /* The chunked form (gdn_delta_chunk.cu): BF16, 16-byte aligned rows. */
 size_t delta_chunk_workspace(uint32_t tokens, uint32_t sequences, uint32_t v_heads);

@@ -4,6 +4,7 @@
 #include "gdn_b200.h"
 #include "gdn_ops.h"
 
+#include <atomic>
 #include <stdarg.h>
 #include <stdio.h>
 
@@ -22,35 +23,50 @@ int failf(const char *fmt, ...) {
     return gdn::host_fail(buf);
 }
 
+/* A CUDA call that failed is reported here and leaves no error behind that a later check would take for its own. */
+int cuda_failf(const char *who, const char *what, cudaError_t e) {
+    cudaGetLastError();
+    return failf("%s: %s: %s", who, what, cudaGetErrorString(e));
+}
+
 bool aligned(const void *p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
 /* The call's device for the thread, and the previous one afterwards. */
 struct DeviceScope {
     int prev = -1;
-    bool ok = false;
+    cudaError_t error;
     explicit DeviceScope(int device) {
-        if (cudaGetDevice(&prev) != cudaSuccess) return;
-        if (prev == device) {
+        error = cudaGetDevice(&prev);
+        if (error != cudaSuccess || prev == device)
             prev = -1;
-            ok = true;
-        } else {
-            ok = cudaSetDevice(device) == cudaSuccess;
-        }
+        else
+            error = cudaSetDevice(device);
     }
     ~DeviceScope() {
         if (prev >= 0) cudaSetDevice(prev);
     }
 };
 
-int sm_count(int device) {
-    static int counts[64]; /* 0: not asked yet; every writer writes the same value */
-    if (device < 0 || device >= 64) return 0;
-    if (counts[device] == 0) {
-        int n = 0;
-        if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) return 0;
-        counts[device] = n;
-    }
-    return counts[device];
+cudaError_t sm_count(int device, int &sms) {
+    static std::atomic<int> counts[64]; /* 0: not asked yet; every writer writes the same value */
+    if (device < 0 || device >= 64) return cudaErrorInvalidDevice;
+    sms = counts[device].load(std::memory_order_relaxed);
+    if (sms != 0) return cudaSuccess;
+    const cudaError_t e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
+    if (e == cudaSuccess) counts[device].store(sms, std::memory_order_relaxed);
+    return e;
+}
+
+/* launch(sms) on `device` */
+template <typename F>
+int on_device(const char *who, int device, F launch) {
+    DeviceScope scope(device);
+    int sms = 0;
+    cudaError_t e = scope.error;
+    if (e == cudaSuccess) e = sm_count(device, sms);
+    if (e != cudaSuccess) return cuda_failf(who, "cannot use the device", e);
+    e = launch(sms);
+    return e == cudaSuccess ? 0 : cuda_failf(who, "launch failed", e);
 }
 
 /* Checks what both forms of the rule ask of their arguments; > 0: nothing to do. */
@@ -101,11 +117,9 @@ int gdn_b200_delta_step(const GdnB200DeltaArgs *args) {
     gdn::ops::DeltaParams p;
     const int rc = delta_params("gdn_b200_delta_step", args, p);
     if (rc != 0) return rc > 0 ? 0 : -1;
-    DeviceScope scope(args->device);
-    const int sms = scope.ok ? sm_count(args->device) : 0;
-    if (sms == 0) return failf("gdn_b200_delta_step: cannot use device %d", args->device);
-    const cudaError_t e = gdn::ops::launch_delta_step(p, args->dtype == 1, sms, static_cast<cudaStream_t>(args->stream));
-    return e == cudaSuccess ? 0 : failf("gdn_b200_delta_step: launch failed: %s", cudaGetErrorString(e));
+    return on_device("gdn_b200_delta_step", args->device, [&](int sms) {
+        return gdn::ops::launch_delta_step(p, args->dtype == 1, sms, static_cast<cudaStream_t>(args->stream));
+    });
 }
 
 size_t gdn_b200_delta_chunk_workspace(uint32_t tokens, uint32_t sequences, uint32_t v_heads) {
@@ -115,8 +129,10 @@ size_t gdn_b200_delta_chunk_workspace(uint32_t tokens, uint32_t sequences, uint3
 int gdn_b200_delta_status(int device) {
     DeviceScope scope(device);
     int step = 0, chunk = 0;
-    if (!scope.ok || gdn::ops::delta_step_status(&step) != cudaSuccess || gdn::ops::delta_chunk_status(&chunk) != cudaSuccess)
-        return failf("gdn_b200_delta_status: cannot read the status of device %d", device);
+    cudaError_t e = scope.error;
+    if (e == cudaSuccess) e = gdn::ops::delta_step_status(&step);
+    if (e == cudaSuccess) e = gdn::ops::delta_chunk_status(&chunk);
+    if (e != cudaSuccess) return cuda_failf("gdn_b200_delta_status", "cannot read the device", e);
     return step == 0 && chunk == 0 ? 0
                                    : failf("gdn_b200_delta_%s: a wait on the device ran out; the call's states are not valid",
                                            chunk != 0 ? "chunk" : "step");
@@ -135,11 +151,9 @@ int gdn_b200_delta_chunk(const GdnB200DeltaArgs *args) {
     const size_t need = gdn::ops::delta_chunk_workspace(args->tokens, args->sequences, args->v_heads);
     if (args->workspace == nullptr || !aligned(args->workspace, 256) || args->workspace_bytes < need)
         return failf("gdn_b200_delta_chunk: a workspace of %zu bytes on a 256-byte boundary is needed", need);
-    DeviceScope scope(args->device);
-    const int sms = scope.ok ? sm_count(args->device) : 0;
-    if (sms == 0) return failf("gdn_b200_delta_chunk: cannot use device %d", args->device);
-    const cudaError_t e = gdn::ops::launch_delta_chunk(p, args->workspace, sms, static_cast<cudaStream_t>(args->stream));
-    return e == cudaSuccess ? 0 : failf("gdn_b200_delta_chunk: launch failed: %s", cudaGetErrorString(e));
+    return on_device("gdn_b200_delta_chunk", args->device, [&](int sms) {
+        return gdn::ops::launch_delta_chunk(p, args->workspace, sms, static_cast<cudaStream_t>(args->stream));
+    });
 }
 
 int gdn_b200_constrain_logits(const GdnB200LogitsArgs *args) {
@@ -163,16 +177,13 @@ int gdn_b200_constrain_logits(const GdnB200LogitsArgs *args) {
     if (!aligned(a.logits, elem) || !aligned(a.out, elem)) return failf("%s: logits or out is misaligned", who);
     if (a.rows > 1 && a.out_row < (int64_t)a.vocab) return failf("%s: rows of out overlap", who);
     if (a.logits_row < 0) return failf("%s: negative row stride", who);
-    DeviceScope scope(a.device);
-    if (!scope.ok) return failf("%s: cannot use device %d", who, a.device);
-    const int sms = sm_count(a.device);
-    if (sms == 0) return failf("%s: device %d does not answer", who, a.device);
     gdn::ops::LogitsParams p{a.logits, a.out, a.picks, a.history ? a.tokens : nullptr, a.lens, a.prompt_lens,
                              a.repetition, a.presence, a.frequency, a.biases ? a.bias_ids : nullptr, a.bias, a.mask,
                              a.logits_row, a.out_row, a.tokens_row, a.bias_ids_row, a.bias_row, a.mask_row,
                              a.rows, a.vocab, a.history, a.biases, 0};
-    const cudaError_t e = gdn::ops::launch_logits(p, a.dtype == 1, sms, static_cast<cudaStream_t>(a.stream));
-    return e == cudaSuccess ? 0 : failf("%s: launch failed: %s", who, cudaGetErrorString(e));
+    return on_device(who, a.device, [&](int sms) {
+        return gdn::ops::launch_logits(p, a.dtype == 1, sms, static_cast<cudaStream_t>(a.stream));
+    });
 }
 
 }  // extern "C"

@@ -89,3 +89,16 @@ def test_threads_with_vocabularies_of_different_sizes(ops):
         t.join()
     torch.cuda.synchronize()
     assert not wrong
+
+
+def test_a_refused_call_leaves_no_error_behind(ops):
+    import gateddeltanet_b200 as gdn
+    a, o = inputs([1] * 40, 8, 8, 256, 256, torch.bfloat16, seed=42)
+    few = {n: (x[:2] if n != "state" else x) for n, x in a.items()}
+    for rule, args in ((ops.delta_step, a), (ops.delta_step, few), (ops.delta_chunk, few)):
+        assert gdn.lib().gdn_b200_delta_status(99) == -1
+        rule(**args, normalize=True)
+        assert gdn.lib().gdn_b200_delta_status(99) == -1
+        torch.zeros(3, device="cuda").add_(1).sum().item()
+    assert gdn.lib().gdn_b200_delta_status(99) == -1
+    ops.constrain_logits(torch.zeros(1, 40, device="cuda"))
