@@ -100,7 +100,7 @@ cudaError_t launch_delta_step(const DeltaParams &p, bool bf16, int sms, cudaStre
 size_t delta_chunk_workspace(uint32_t tokens, uint32_t sequences, uint32_t v_heads);
 cudaError_t launch_delta_chunk(const DeltaParams &p, void *workspace, int sms, cudaStream_t stream);
 /* *status != 0: a wait of such a kernel on the current device ran out since
- * the last call. They synchronise. */
+ * the last call. For kernels that have ended. */
 cudaError_t delta_step_status(int *status);
 cudaError_t delta_chunk_status(int *status);
 cudaError_t launch_logits(LogitsParams p, bool bf16, int sms, cudaStream_t stream);

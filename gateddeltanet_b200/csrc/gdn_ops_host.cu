@@ -130,6 +130,7 @@ int gdn_b200_delta_status(int device) {
     DeviceScope scope(device);
     int step = 0, chunk = 0;
     cudaError_t e = scope.error;
+    if (e == cudaSuccess) e = cudaDeviceSynchronize(); /* the copies below wait for no stream but their own */
     if (e == cudaSuccess) e = gdn::ops::delta_step_status(&step);
     if (e == cudaSuccess) e = gdn::ops::delta_chunk_status(&chunk);
     if (e != cudaSuccess) return cuda_failf("gdn_b200_delta_status", "cannot read the device", e);

@@ -20,9 +20,9 @@ from typing import Optional, Tuple
 
 import torch
 
-from . import HERE, lib
+from . import HERE, last_error, lib
 
-__all__ = ["delta_step", "delta_chunk", "constrain_logits"]
+__all__ = ["delta_step", "delta_chunk", "delta_status", "constrain_logits"]
 
 
 def _load():
@@ -66,6 +66,18 @@ def delta_chunk(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tens
     prompts, 64 tokens at a time on the tensor cores. q, k, v bfloat16 with
     16-byte aligned rows."""
     return _native.delta_chunk(q, k, v, g, beta, state, starts, slots, fresh, scale, normalize, out)
+
+
+def delta_status(device=None) -> None:
+    """gdn_b200_delta_status: waits for the device (None: the current one) and
+    raises RuntimeError if a wait inside delta_step or delta_chunk ran out
+    there since the last call: the states of that call are then not valid."""
+    device = torch.device("cuda" if device is None else device)
+    if device.type != "cuda":
+        raise ValueError(f"delta_status: {device} is not a CUDA device")
+    index = device.index
+    if lib().gdn_b200_delta_status(torch.cuda.current_device() if index is None else index) != 0:
+        raise RuntimeError(last_error())
 
 
 def constrain_logits(logits: torch.Tensor, *, tokens: Optional[torch.Tensor] = None, lens: Optional[torch.Tensor] = None,

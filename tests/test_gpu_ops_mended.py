@@ -102,3 +102,21 @@ def test_a_refused_call_leaves_no_error_behind(ops):
         torch.zeros(3, device="cuda").add_(1).sum().item()
     assert gdn.lib().gdn_b200_delta_status(99) == -1
     ops.constrain_logits(torch.zeros(1, 40, device="cuda"))
+
+
+def test_status_waits_for_every_stream(ops):
+    import gateddeltanet_b200 as gdn
+    x = torch.randn(4096, 4096, device="cuda")
+    torch.cuda.synchronize()
+    side, done = torch.cuda.Stream(), torch.cuda.Event()
+    with torch.cuda.stream(side):
+        for _ in range(60):
+            y = x @ x
+        done.record()
+    assert gdn.lib().gdn_b200_delta_status(0) == 0
+    assert done.query()
+    assert y.shape == x.shape
+    ops.delta_status()
+    ops.delta_status("cuda:0")
+    with pytest.raises(RuntimeError, match="delta_status"):
+        ops.delta_status(99)
