@@ -10,6 +10,7 @@
 #include <ATen/core/Tensor.h>
 #include <ATen/core/grad_mode.h>
 #include <ATen/ops/empty.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -97,9 +98,14 @@ struct Arg {
             reach = d[i].first * d[i].second;
         }
     }
+    /* a gradient or a tangent would end here unseen */
     void no_gradient() const {
-        if (t->requires_grad())
-            throw Refused{PyExc_RuntimeError, std::string(who) + ": no gradient is computed (call it under torch.no_grad())"};
+        if (t == nullptr) return;
+        const bool backward = at::GradMode::is_enabled() && t->requires_grad();
+        const bool forward = c10::AutogradState::get_tls_state().get_fw_grad_mode() && t->_fw_grad(0).defined();
+        if (backward || forward)
+            throw Refused{PyExc_RuntimeError, std::string(who) + ": no gradient is computed for " + what +
+                                                  (backward ? " (call it under torch.no_grad())" : "")};
     }
     template <typename T>
     T *ptr() const {
@@ -143,11 +149,8 @@ PyObject *delta(PyObject *const *args, Py_ssize_t nargs, bool chunk) {
         const Arg q(who, "q", args[0]), k(who, "k", args[1]), v(who, "v", args[2]), g(who, "g", args[3]), beta(who, "beta", args[4]),
             state(who, "state", args[5]), starts(who, "starts", args[6]), slots(who, "slots", args[7]), fresh(who, "fresh", args[8]),
             out(who, "out", args[11]);
-        const bool grad = at::GradMode::is_enabled();
-        for (const Arg *a : {&q, &k, &v, &g, &beta, &state}) {
-            a->present();
-            if (grad) a->no_gradient();
-        }
+        for (const Arg *a : {&q, &k, &v, &g, &beta, &state}) a->present();
+        for (const Arg *a : {&q, &k, &v, &g, &beta, &state, &out}) a->no_gradient();
         q.dims(3);
         v.dims(3);
         state.dims(4);
@@ -268,7 +271,7 @@ PyObject *constrain_logits(PyObject *, PyObject *const *args, Py_ssize_t nargs) 
             frequency(who, "frequency", args[6]), bias_ids(who, "bias_ids", args[7]), bias(who, "bias", args[8]),
             mask(who, "mask", args[9]), out(who, "out", args[10]);
         logits.present();
-        if (at::GradMode::is_enabled()) logits.no_gradient();
+        for (const Arg *a : {&logits, &repetition, &presence, &frequency, &bias, &out}) a->no_gradient();
         logits.dims(2);
         logits.last_contiguous();
         GdnB200LogitsArgs a = {};

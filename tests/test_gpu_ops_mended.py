@@ -120,3 +120,23 @@ def test_status_waits_for_every_stream(ops):
     ops.delta_status("cuda:0")
     with pytest.raises(RuntimeError, match="delta_status"):
         ops.delta_status(99)
+
+
+def test_gradients_are_refused(ops):
+    """Nothing that would lose a gradient is taken: no floating-point input, no output, no tangent."""
+    from torch.autograd import forward_ad
+    from test_gpu_ops_logits import inputs as logits_inputs
+    a = logits_inputs(2, 100, 5, 2, torch.float32)
+    a["out"] = torch.empty_like(a["logits"])
+    d, o = inputs([3, 1], 2, 4, 64, 64, torch.bfloat16)
+    d["out"] = torch.empty_like(d["v"])
+    for call, args, more in ((ops.constrain_logits, a, {}), (ops.delta_step, d, o), (ops.delta_chunk, d, o)):
+        for n, x in args.items():
+            if not x.is_floating_point():
+                continue
+            with pytest.raises(RuntimeError, match="no gradient"):
+                call(**{**args, n: x.clone().requires_grad_()}, **more)
+            with torch.no_grad():
+                call(**{**args, n: x.clone().requires_grad_()}, **more)
+            with forward_ad.dual_level(), pytest.raises(RuntimeError, match="no gradient"):
+                call(**{**args, n: forward_ad.make_dual(x.clone(), torch.ones_like(x))}, **more)
