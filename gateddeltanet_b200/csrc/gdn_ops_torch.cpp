@@ -107,6 +107,11 @@ struct Arg {
             throw Refused{PyExc_RuntimeError, std::string(who) + ": no gradient is computed for " + what +
                                                   (backward ? " (call it under torch.no_grad())" : "")};
     }
+    /* The call wrote it: autograd then notices where it kept the old content.
+     * An inference tensor has no version. */
+    void written() const {
+        if (t != nullptr && !t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+    }
     template <typename T>
     T *ptr() const {
         return t == nullptr ? nullptr : static_cast<T *>(t->data_ptr());
@@ -248,6 +253,8 @@ PyObject *delta(PyObject *const *args, Py_ssize_t nargs, bool chunk) {
         } else {
             called(g_entry.step(&a));
         }
+        state.written();
+        out.written();
         if (out) {
             Py_INCREF(args[11]);
             return args[11];
@@ -347,6 +354,7 @@ PyObject *constrain_logits(PyObject *, PyObject *const *args, Py_ssize_t nargs) 
         a.history = (uint32_t)history, a.biases = (uint32_t)biases;
         a.device = device.index();
         called(g_entry.logits(&a));
+        out.written();
         PyObject *first = out ? Py_NewRef(args[10]) : THPVariable_Wrap(result);
         if (first == nullptr) return nullptr;
         PyObject *second = THPVariable_Wrap(picks);

@@ -140,3 +140,18 @@ def test_gradients_are_refused(ops):
                 call(**{**args, n: x.clone().requires_grad_()}, **more)
             with forward_ad.dual_level(), pytest.raises(RuntimeError, match="no gradient"):
                 call(**{**args, n: forward_ad.make_dual(x.clone(), torch.ones_like(x))}, **more)
+
+
+def test_written_tensors_get_a_new_version(ops):
+    d, o = inputs([3, 1], 2, 4, 64, 64, torch.bfloat16)
+    out, logits = torch.empty_like(d["v"]), torch.zeros(2, 50, device="cuda")
+    for rule in (ops.delta_step, ops.delta_chunk):
+        before = (d["state"]._version, out._version, d["v"]._version)
+        rule(**d, **o, out=out)
+        assert (d["state"]._version, out._version, d["v"]._version) == (before[0] + 1, before[1] + 1, before[2])
+    before = logits._version
+    ops.constrain_logits(logits, out=logits)
+    assert logits._version == before + 1
+    with torch.inference_mode():
+        made = dict(d, state=d["state"] * 1)
+    ops.delta_step(**made, **o)  # tensors without a version
