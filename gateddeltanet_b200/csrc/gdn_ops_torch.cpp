@@ -12,6 +12,7 @@
 #include <ATen/ops/empty.h>
 #include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <algorithm>
@@ -130,17 +131,16 @@ void called(int rc) {
     if (rc != 0) throw Refused{PyExc_RuntimeError, g_entry.last_error()};
 }
 
-/* body() with its refusals and C++ exceptions as Python errors */
+/* body() with its refusals as Python errors, and C++ exceptions as torch's own
+ * (an allocation that fails is a torch.OutOfMemoryError) */
 template <typename F>
 PyObject *guarded(F body) {
     try {
         return body();
     } catch (const Refused &r) {
         PyErr_SetString(r.type, r.what.c_str());
-    } catch (const std::exception &e) {
-        PyErr_SetString(PyExc_RuntimeError, e.what());
     } catch (...) {
-        PyErr_SetString(PyExc_RuntimeError, "unknown error");
+        torch::translate_exception_to_python(std::current_exception());
     }
     return nullptr;
 }

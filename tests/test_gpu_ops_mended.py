@@ -155,3 +155,18 @@ def test_written_tensors_get_a_new_version(ops):
     with torch.inference_mode():
         made = dict(d, state=d["state"] * 1)
     ops.delta_step(**made, **o)  # tensors without a version
+
+
+def test_out_of_memory_is_torchs_own(ops):
+    tokens = 2 ** 30
+    wide = dict(q=torch.zeros(1, 1, 64, device="cuda", dtype=torch.bfloat16), k=torch.zeros(1, 1, 64, device="cuda", dtype=torch.bfloat16),
+                v=torch.zeros(1, 1, 256, device="cuda", dtype=torch.bfloat16), g=torch.zeros(1, 1, device="cuda"),
+                beta=torch.zeros(1, 1, device="cuda"))
+    wide = {n: x.expand(tokens, *x.shape[1:]) for n, x in wide.items()}
+    state = torch.zeros(1, 1, 256, 64, device="cuda")
+    starts = torch.tensor([0, 0], dtype=torch.int32, device="cuda")
+    for rule in (ops.delta_step, ops.delta_chunk):
+        with pytest.raises(torch.OutOfMemoryError):
+            rule(**wide, state=state, starts=starts)
+    with pytest.raises(torch.OutOfMemoryError):
+        ops.constrain_logits(torch.zeros(1, 2 ** 18, device="cuda").expand(2 ** 21, -1))
