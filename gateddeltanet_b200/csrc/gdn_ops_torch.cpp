@@ -119,6 +119,15 @@ struct Arg {
     }
 };
 
+/* Stride of dimension d; of a single entry, whose stride torch leaves to
+ * chance, that of a contiguous tensor. */
+int64_t step(const at::Tensor &t, int64_t d) {
+    if (t.size(d) > 1) return t.stride(d);
+    int64_t n = 1;
+    for (int64_t i = d + 1; i < t.dim(); ++i) n *= t.size(i);
+    return n;
+}
+
 int dtype_code(const Arg &a) {
     switch (a.t->scalar_type()) {
         case at::kFloat: return 0;
@@ -231,13 +240,13 @@ PyObject *delta(PyObject *const *args, Py_ssize_t nargs, bool chunk) {
         a.slots = slots.ptr<const int32_t>();
         a.fresh = fresh.ptr<const uint8_t>();
         a.stream = c10::cuda::getCurrentCUDAStream(device.index()).stream();
-        a.q_token = q.t->stride(0), a.q_head = q.t->stride(1);
-        a.k_token = k.t->stride(0), a.k_head = k.t->stride(1);
-        a.v_token = v.t->stride(0), a.v_head = v.t->stride(1);
-        a.g_token = g.t->stride(0), a.g_head = g.t->stride(1);
-        a.beta_token = beta.t->stride(0), a.beta_head = beta.t->stride(1);
-        a.out_token = result.stride(0), a.out_head = result.stride(1);
-        a.state_slot = ss[0];
+        a.q_token = step(*q.t, 0), a.q_head = step(*q.t, 1);
+        a.k_token = step(*k.t, 0), a.k_head = step(*k.t, 1);
+        a.v_token = step(*v.t, 0), a.v_head = step(*v.t, 1);
+        a.g_token = step(*g.t, 0), a.g_head = step(*g.t, 1);
+        a.beta_token = step(*beta.t, 0), a.beta_head = step(*beta.t, 1);
+        a.out_token = step(result, 0), a.out_head = step(result, 1);
+        a.state_slot = step(*state.t, 0);
         a.sequences = (uint32_t)sequences, a.tokens = (uint32_t)tokens;
         a.heads = (uint32_t)heads, a.v_heads = (uint32_t)v_heads;
         a.key_dim = (uint32_t)key_dim, a.value_dim = (uint32_t)value_dim;

@@ -170,3 +170,16 @@ def test_out_of_memory_is_torchs_own(ops):
             rule(**wide, state=state, starts=starts)
     with pytest.raises(torch.OutOfMemoryError):
         ops.constrain_logits(torch.zeros(1, 2 ** 18, device="cuda").expand(2 ** 21, -1))
+
+
+@pytest.mark.parametrize("rule", ["delta_step", "delta_chunk"])
+def test_strides_of_a_single_entry_do_not_matter(ops, rule):
+    """One token, one head or one slot: where the next one would be is not asked."""
+    for lengths, heads in (([1], 2), ([70], 1)):
+        a, o = inputs(lengths, heads, heads, 64, 32, torch.bfloat16, seed=43)
+        o["slots"] = torch.zeros(1, dtype=torch.int32, device="cuda")
+        for n in ("q", "k", "v", "state"):
+            x = a[n][:1] if n == "state" else a[n]
+            stride = [1003 if size == 1 else step for size, step in zip(x.shape, x.stride())]
+            a[n] = x.contiguous().as_strided(x.shape, stride)
+        compare(getattr(ops, rule), a, o, out_tol(rule, torch.bfloat16))
