@@ -5,7 +5,8 @@
 nvcc compiles the CUDA kernel and the C-ABI host layer into one shared
 library next to this file (gateddeltanet_b200/libgdn_b200.so), linked against
 the static CUDA runtime so it does not depend on torch's copy of libcudart.
-g++ compiles the torch binding of the serving operators (_ops_torch.so).
+g++ compiles the torch binding of the serving operators (_ops_torch.so) where
+torch is installed.
 """
 from __future__ import annotations
 
@@ -44,13 +45,17 @@ def _stale(target: str, sources) -> bool:
 
 
 def build_torch(force: bool = False, verbose: bool = False) -> str:
-    """The torch binding: host code only, against the headers of the installed torch."""
+    """The torch binding: host code only, against the headers of the installed
+    torch. Without a torch there is nothing to bind; the library is whole without it."""
     if not force and not _stale(TORCH_LIB, [TORCH_SOURCE]):
         return TORCH_LIB
     import sysconfig
-
-    import torch
-    from torch.utils import cpp_extension
+    try:
+        import torch
+        from torch.utils import cpp_extension
+    except ImportError as e:
+        print(f"no torch ({e}): the binding of gateddeltanet_b200.ops is not built", file=sys.stderr)
+        return ""
     cuda = os.path.dirname(os.path.dirname(nvcc()))
     libs = cpp_extension.library_paths()
     tmp = TORCH_LIB + ".tmp"
