@@ -63,9 +63,12 @@ def generate(model: Model, prompts: List[List[int]], new: int, masks: Optional[t
              frequency: float = 0.1, presence: float = 0.1, bias: Optional[dict] = None):
     """Greedy continuation of each prompt by `new` tokens under penalties,
     biases {token: value} and masks (int32 [streams, ceil(vocab / 32)], bit set
-    = allowed). Returns (table of all tokens, lengths, states)."""
+    = allowed). A stream whose constraints leave no token ends there. Returns
+    (table of all tokens, lengths, states)."""
     n = len(prompts)
     lengths = [len(p) for p in prompts]
+    if not lengths or min(lengths) == 0:
+        raise ValueError("a prompt of at least one token is needed for each stream")
     device = "cuda"
     table = torch.zeros(n, max(lengths) + new, dtype=torch.int32, device=device)
     for i, p in enumerate(prompts):
@@ -84,14 +87,18 @@ def generate(model: Model, prompts: List[List[int]], new: int, masks: Optional[t
     hidden = model.forward(packed, states, slots, starts=starts, fresh=torch.ones(n, dtype=torch.bool, device=device))
     hidden = hidden[starts[1:].long() - 1]
     rows = torch.arange(n, device=device)
+    going = torch.ones(n, dtype=torch.bool, device=device)
     for step in range(new):
         logits = model.logits(hidden)
         _, picks = ops.constrain_logits(logits, tokens=table, lens=lens, prompt_lens=prompt_lens, mask=masks, out=logits,
                                         **penalties)
+        going &= picks >= 0
+        picks = torch.where(going, picks, 0)
         table[rows, lens.long()] = picks
-        lens += 1
+        lens += going
         if step + 1 < new:
-            hidden = model.forward(picks, states, slots)
+            # slot -1: a stream that has ended stays in the batch, but its states do not change
+            hidden = model.forward(picks, states, torch.where(going, slots, -1))
     return table, lens, [s[slots.long()] for s in states]
 
 
