@@ -741,7 +741,6 @@ struct Scan {
     static constexpr int kGroups = VB == 16 ? kTiles : 1, kOwn = kTiles / kGroups;
     static constexpr uint32_t kTokenWarps = 4 * kSubs, kEpiWarps = kTokenWarps * kGroups;
     static constexpr uint32_t kThreads = (kEpiWarps + 4) * 32, kLoadThreads = 64;
-    static constexpr int kMinCtas = K <= 128 && VB == 16 ? 2 : 1;
     static constexpr uint32_t kAtoms = 3 * VB > 64 ? 2 : 1;      /* blocks of 64 columns of an operand of 3 VB */
     /* shared memory */
     static constexpr uint32_t kKQ = 0;
@@ -761,7 +760,7 @@ struct Scan {
 };
 
 template <int K, int VB>
-__global__ void __launch_bounds__(Scan<K, VB>::kThreads, Scan<K, VB>::kMinCtas)
+__global__ void __launch_bounds__(Scan<K, VB>::kThreads, 1)
     chunk_scan_kernel(const __grid_constant__ DeltaParams p, const uint8_t *records, const uint32_t *order, uint32_t out_wide) {
     using L = Scan<K, VB>;
     constexpr int kTiles = L::kTiles;
