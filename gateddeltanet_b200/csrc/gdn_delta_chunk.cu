@@ -22,6 +22,13 @@
  * for T the states' errors against 64 bits were up to 7e-7 for independent keys
  * and 5e-6 where all keys of a sequence are alike.)
  *
+ * A token whose k, v, g or beta is not finite makes NaN of its own output and
+ * of all that follow, as the rule does, but must not reach the tokens before it
+ * through the zeros of T and P T above their diagonals (0 NaN). So its row of R
+ * enters the MMA as zeros (and its row of A as the identity's); its row of D
+ * is then set to NaN, with which the state follows, and so are the outputs of
+ * the chunk from it on.
+ *
  * What bounds the walk is the chain of one chunk: three rounds of MMAs, each
  * waiting for the epilogue of the one before. Measured with 8 heads of 256 x
  * 256: 4096 tokens 158 us (2500 token by token), of which the first kernel
@@ -181,6 +188,15 @@ __device__ __forceinline__ void scale_add(float f, const float (&x)[8], float (&
 __device__ __forceinline__ void add_to(const float (&x)[8], float (&y)[8]) {
 #pragma unroll
     for (int i = 0; i < 8; i += 2) unpack2(add2(pack2(x[i], x[i + 1]), pack2(y[i], y[i + 1])), y[i], y[i + 1]);
+}
+/* by a product with zeros, in three steps of packed operations */
+__device__ __forceinline__ bool all_finite(const float (&x)[8]) {
+    const uint64_t none = pack2(0.0f, 0.0f);
+    const uint64_t a = fma2(pack2(x[0], x[1]), none, fma2(pack2(x[2], x[3]), none, none));
+    const uint64_t b = fma2(pack2(x[4], x[5]), none, fma2(pack2(x[6], x[7]), none, none));
+    float lo, hi;
+    unpack2(add2(a, b), lo, hi);
+    return lo + hi == 0.0f;
 }
 /* the sums of the three terms' columns (VB apart): eight value rows starting at addr */
 template <int VB>
@@ -516,6 +532,7 @@ __global__ void __launch_bounds__(kPrepThreads, 3) chunk_prep_kernel(const __gri
 
     float *A = reinterpret_cast<float *>(sm + L::kA), *P = reinterpret_cast<float *>(sm + L::kP);
     float *X = reinterpret_cast<float *>(sm + L::kX), *G = reinterpret_cast<float *>(sm + L::kG);
+    uint32_t *first_bad = reinterpret_cast<uint32_t *>(sm + L::kBar + 24); /* the first token whose row of A is not finite */
     float *Glo = G + kC, *bet = G + 2 * kC, *kin = G + 3 * kC, *qin = G + 4 * kC, *dec_i = G + 5 * kC, *dec_j = G + 6 * kC;
     const uint32_t bar = base + L::kBar;
     uint32_t *slot = reinterpret_cast<uint32_t *>(sm + L::kBar + 8);
@@ -523,6 +540,7 @@ __global__ void __launch_bounds__(kPrepThreads, 3) chunk_prep_kernel(const __gri
     if (tid == 0) {
         mbar_init(bar, 1);
         *abort = 0;
+        *first_bad = kC;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 0) {
@@ -579,7 +597,7 @@ __global__ void __launch_bounds__(kPrepThreads, 3) chunk_prep_kernel(const __gri
         }
         commit(bar);
     }
-    wait_bar_warp(bar, 0, abort);
+    if (!wait_bar_warp(bar, 0, abort)) *first_bad = 0; /* nothing that could pass for a result */
     tc_fence_after();
     /* rows 32 (warp % 4) .. + 31 of [K; Q], one a lane: token i of k or of q */
     const uint32_t row = 32 * (warp & 3) + lane, lanes = (32 * (warp & 3)) << 16, i = row & (kC - 1);
@@ -632,7 +650,7 @@ __global__ void __launch_bounds__(kPrepThreads, 3) chunk_prep_kernel(const __gri
             tc_ld32(tmem + lanes + c0, r);
             tc_wait();
         }
-        float f = is_p ? qin[i] : bet[i] * kin[i];
+        float f = is_p ? qin[i] : bet[i] * kin[i], zero = 0.0f; /* zero: NaN when one of the row is not finite */
         if (low != left) {
             /* the quarter with the diagonal */
             const float gi = G[i], gl = Glo[i];
@@ -648,6 +666,7 @@ __global__ void __launch_bounds__(kPrepThreads, 3) chunk_prep_kernel(const __gri
                     /* for all columns: taken only where wanted, it cost a branch each (5200 cycles for the 32) */
                     const float y = f * kj[e] * decay_exp((gi - gj[e]) + (gl - lj[e])) * __uint_as_float(r[c + e]);
                     x[e] = c + e <= last ? y : 0.0f;
+                    zero = fmaf(x[e], 0.0f, zero);
                 }
                 store8(dst + c, x);
             }
@@ -658,13 +677,30 @@ __global__ void __launch_bounds__(kPrepThreads, 3) chunk_prep_kernel(const __gri
                 float dj[8], x[8];
                 load8(dec_j + c, dj);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] = low ? f * dj[e] * __uint_as_float(r[c + e]) : 0.0f;
+                for (int e = 0; e < 8; ++e) {
+                    x[e] = low ? f * dj[e] * __uint_as_float(r[c + e]) : 0.0f;
+                    zero = fmaf(x[e], 0.0f, zero);
+                }
                 store8(dst + c, x);
             }
         }
+        if (!is_p && !(zero == 0.0f)) atomicMin(first_bad, i);
     }
     tc_fence_before();
     __syncthreads();
+    const uint32_t bad = *first_bad;
+    if (bad < (uint32_t)kC) {
+        /* rows that the tokens before do not need; the scalars make NaN of them */
+        for (uint32_t x = tid; x < (kC - bad) * kC; x += kPrepThreads) {
+            A[(bad + x / kC) * kLdA + x % kC] = 0.0f;
+            P[(bad + x / kC) * kLdP + x % kC] = 0.0f;
+        }
+        if (warp < 2 && i >= bad) {
+            float *sc = reinterpret_cast<float *>(record + kPairBytes);
+            sc[kScalC * kC + i] = sc[kScalBeta * kC + i] = sc[kScalQ * kC + i] = __int_as_float(0x7fc00000);
+        }
+        __syncthreads();
+    }
     constexpr uint32_t kDiag = kLdA + 1;
     if (warp < 4) invert16(A + 16 * warp * kDiag, lane);
     __syncthreads();
@@ -753,7 +789,8 @@ struct Scan {
     static constexpr uint32_t kDNext = kR + kC * 128 - kD;
     static constexpr uint32_t kScal = kR + kAtoms * kC * 128;    /* rows of scalars of two chunks */
     static constexpr uint32_t kBar = kScal + 2 * kScalBytes;
-    static constexpr uint32_t kBytes = kBar + 192; /* the kernel has no other shared memory: its base is aligned */
+    static constexpr uint32_t kBad = kBar + 192;                 /* of each value row: the first token that is not finite */
+    static constexpr uint32_t kBytes = kBad + VB * 4; /* the kernel has no other shared memory: its base is aligned */
     /* TMEM columns */
     static constexpr uint32_t kD1 = 0, kD3 = 4 * VB, kD3Third = kD3 + 3 * VB, kD4 = 8 * VB, kD4Tile = 4 * VB;
     static constexpr uint32_t kColumns = 16 * VB;                /* a power of two that holds them */
@@ -784,7 +821,11 @@ __global__ void __launch_bounds__(Scan<K, VB>::kThreads, 1)
                    d4_full = bar + 104, drain = bar + 120, full_scal = bar + 128, empty_scal = bar + 160;
     uint32_t *slot = reinterpret_cast<uint32_t *>(sm + L::kBar + 144);
     volatile uint32_t *abort = reinterpret_cast<volatile uint32_t *>(sm + L::kBar + 152);
+    volatile uint32_t *any_bad = reinterpret_cast<volatile uint32_t *>(sm + L::kBar + 176);
+    uint32_t *first_bad = reinterpret_cast<uint32_t *>(sm + L::kBad);
+    if (tid < (uint32_t)VB) first_bad[tid] = 0xffffffffu;
     if (tid == 0) {
+        *any_bad = 0;
         for (int i = 0; i < 2; ++i) {
             mbar_init(full_scal + 8 * i, 1);
             mbar_init(empty_scal + 8 * i, L::kEpiWarps);
@@ -1010,6 +1051,7 @@ __global__ void __launch_bounds__(Scan<K, VB>::kThreads, 1)
             float x[8];
             if (group == 0) {
                 float bv[8], f0;
+                uint32_t poison = 0; /* value rows of this token that are not finite */
                 if (q) {
                     f0 = sc[kScalQ * kC + i];
                 } else {
@@ -1032,6 +1074,17 @@ __global__ void __launch_bounds__(Scan<K, VB>::kThreads, 1)
                     /* rows without a token have zeros for all of it */
                     scale_add(f0, x, bv);
                     put_terms<VB>(sm + L::kR, kC * 128, i, sub, bv);
+                    if (!all_finite(bv)) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            if (!(bv[e] * 0.0f == 0.0f)) {
+                                bv[e] = 0.0f;
+                                poison |= 1u << e;
+                                atomicMin(first_bad + 8 * sub + e, c * kC + i);
+                            }
+                        *any_bad = 1;
+                        put_terms<VB>(sm + L::kR, kC * 128, i, sub, bv);
+                    }
                     fence_async();
                     tc_fence_before();
                     warp_arrive(r_ready);
@@ -1044,6 +1097,11 @@ __global__ void __launch_bounds__(Scan<K, VB>::kThreads, 1)
                         __nv_bfloat16 *dst = out + (int64_t)(tc + i) * p.out_token + 8 * sub;
 #pragma unroll
                         for (int e = 0; e < 8; ++e) o[e] += x[e];
+                        if (*any_bad) {
+#pragma unroll
+                            for (int e = 0; e < 8; ++e)
+                                if (c * kC + i >= first_bad[8 * sub + e]) o[e] = __int_as_float(0x7fc00000);
+                        }
                         if (out_wide) {
                             *reinterpret_cast<uint4 *>(dst) = make_uint4(bf16_pair(o[0], o[1]), bf16_pair(o[2], o[3]),
                                                                          bf16_pair(o[4], o[5]), bf16_pair(o[6], o[7]));
@@ -1059,6 +1117,11 @@ __global__ void __launch_bounds__(Scan<K, VB>::kThreads, 1)
                     tc_wait();
 #pragma unroll
                     for (int e = 0; e < 8; ++e) x[e] = f2 * (x[e] + __uint_as_float(third[e]));
+                    if (poison) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            if ((poison >> e) & 1u) x[e] = __int_as_float(0x7fc00000);
+                    }
                     put_terms<VB, 4>(sm + L::kD, L::kDNext, i, sub, x);
                     fence_async();
                     tc_fence_before();

@@ -327,7 +327,8 @@ typedef struct {
  * (any number is right; its time grows with the longest sequence). Reads and
  * writes each state once. The workspace is not used. */
 int gdn_b200_delta_step(const GdnB200DeltaArgs *args);
-/* Prompts: any lengths, BF16 only. 16-byte aligned q, k and v rows. */
+/* Prompts: any lengths, BF16 only. 16-byte aligned q, k and v rows. What is
+ * not finite spreads as in gdn_b200_delta_step, but infinities come out as NaN. */
 int gdn_b200_delta_chunk(const GdnB200DeltaArgs *args);
 /* Bytes of 256-byte aligned device memory that gdn_b200_delta_chunk needs as
  * args->workspace for these sizes. */

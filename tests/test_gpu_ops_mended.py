@@ -183,3 +183,28 @@ def test_strides_of_a_single_entry_do_not_matter(ops, rule):
             stride = [1003 if size == 1 else step for size, step in zip(x.shape, x.stride())]
             a[n] = x.contiguous().as_strided(x.shape, stride)
         compare(getattr(ops, rule), a, o, out_tol(rule, torch.bfloat16))
+
+
+@pytest.mark.parametrize("rule", ["delta_step", "delta_chunk"])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")], ids=str)
+@pytest.mark.parametrize("what", ["q", "k", "v", "g", "beta", "state"])
+@pytest.mark.parametrize("shape", [(2, 4, 64, 64), (2, 2, 256, 256), (5, 5, 256, 256), (8, 8, 128, 128)], ids=str)
+def test_no_value_spreads_backwards(ops, rule, what, bad, shape):
+    """A NaN or an infinity of one token reaches neither the tokens before it nor, where it is a value's, other value rows."""
+    if what == "g" and bad < 0:
+        bad = float("nan")  # log 0 is a decay like others
+    lengths = [150, 97]
+    for at in (0, 37, 64, 101, 148):
+        a, o = inputs(lengths, *shape, torch.bfloat16, seed=44, normalize=at % 2 == 0)
+        if what == "state":
+            a["state"][int(o["slots"][0]), 1, 7, 5] = bad
+        else:
+            a[what][(at, 1, 7) if a[what].dim() == 3 else (at, 1)] = bad
+        ref_o, ref_s = plain.delta_rule(**a, **o)
+        out = getattr(ops, rule)(**a, **o).cpu().double()
+        state = a["state"].cpu().double()
+        assert torch.equal(out.isfinite(), ref_o.isfinite()) and torch.equal(state.isfinite(), ref_s.isfinite())
+        fine = ref_o.isfinite()
+        assert plain.rel(out[fine], ref_o[fine]) <= out_tol(rule, torch.bfloat16)
+        fine = ref_s.isfinite()
+        assert plain.rel(state[fine], ref_s[fine]) <= STATE_TOL
