@@ -16,11 +16,12 @@
  * The state has to come out as FP32 arithmetic would give it, from BF16
  * tensor cores with FP32 accumulators: k and q enter as they are (exact), their
  * norms and the decays scale rows of results, and each FP32 operand enters
- * as BF16 terms that sum to it: three for S0, R, D and T (24 bits), two for P T
- * (16 bits: the outputs are BF16). The terms of an operand are columns of one
- * MMA (N = 3 VB), whose sums are added when they are read back. (With two terms
- * for T the states' errors against 64 bits were up to 7e-7 for independent keys
- * and 5e-6 where all keys of a sequence are alike.)
+ * as three BF16 terms that sum to it (24 bits): S0, R, D, T and P T. The terms
+ * of an operand are columns of one MMA (N = 3 VB), whose sums are added when they
+ * are read back. (With two terms for T the states' errors against 64 bits were
+ * up to 7e-7 for independent keys and 5e-6 where all keys of a sequence are
+ * alike; with two for P T the outputs were 2.4e-6 off before their rounding to
+ * BF16, which then went the other way for one in a thousand.)
  *
  * A token whose k, v, g or beta is not finite makes NaN of its own output and
  * of all that follow, as the rule does, but must not reach the tokens before it
@@ -47,10 +48,10 @@ namespace {
 constexpr int kC = 64;      /* tokens of a chunk */
 constexpr uint64_t kWaitNs = 2000000000ull;
 
-/* per (chunk, value head): two BF16 terms of [T; P T] and the third of T in the
- * MMA's layout, then four rows of 64 floats and the chunk's decay */
+/* per (chunk, value head): three BF16 terms of [T; P T] in the MMA's layout,
+ * then four rows of 64 floats and the chunk's decay */
 constexpr uint32_t kTermBytes = 2 * kC * 128;       /* 128 rows of 64 BF16 */
-constexpr uint32_t kPairBytes = 2 * kTermBytes + kC * 128;
+constexpr uint32_t kPairBytes = 3 * kTermBytes;
 constexpr uint32_t kScalBytes = (4 * kC + 4) * 4;
 constexpr uint32_t kRecordBytes = (kPairBytes + kScalBytes + 127) & ~127u;
 enum { kScalC = 0, kScalBeta = 1, kScalQ = 2, kScalEnd = 3, kScalDecay = 4 };
@@ -436,13 +437,16 @@ __device__ __forceinline__ void product_tile(float *out, const float *a, const f
     *reinterpret_cast<float2 *>(p) = make_float2(sign * parts_sum(d, 0), sign * parts_sum(d, 1));
     *reinterpret_cast<float2 *>(p + 8 * kLdA) = make_float2(sign * parts_sum(d, 2), sign * parts_sum(d, 3));
 }
-/* two neighbouring values of a row of the record as two BF16 terms */
-__device__ __forceinline__ void put_pair2(uint8_t *rec, uint32_t row, uint32_t col, float x, float y) {
-    const uint32_t w = bf16_pair(x, y);
-    const uint32_t u = bf16_pair(x - __uint_as_float(w << 16), y - __uint_as_float(w & 0xFFFF0000u));
+/* two neighbouring values of a row of the record as three BF16 terms */
+__device__ __forceinline__ void put_pair3(uint8_t *rec, uint32_t row, uint32_t col, float x, float y) {
     uint8_t *p = rec + piece_at(row, col >> 3) + (col & 7) * 2;
-    *reinterpret_cast<uint32_t *>(p) = w;
-    *reinterpret_cast<uint32_t *>(p + kTermBytes) = u;
+#pragma unroll
+    for (int term = 0; term < 3; ++term) {
+        const uint32_t w = bf16_pair(x, y);
+        *reinterpret_cast<uint32_t *>(p + term * kTermBytes) = w;
+        x -= __uint_as_float(w << 16);
+        y -= __uint_as_float(w & 0xFFFF0000u);
+    }
 }
 
 __device__ __forceinline__ void load8(const float *p, float (&x)[8]) {
@@ -715,8 +719,7 @@ __global__ void __launch_bounds__(kPrepThreads, 3) chunk_prep_kernel(const __gri
     product_tile<32>(A + 32 * kLdA, A + 32 * kDiag, X, -1.0f, 16 * (warp >> 2), 8 * (warp & 3), lane);
     __syncthreads();
     /* the record: T in the rows of the chunk's k, P T in those of its q (both
-     * lower triangular); the two change places from chunk to chunk. The third
-     * term is T's alone. */
+     * lower triangular); the two change places from chunk to chunk */
     const uint32_t t_row = (chunk & 1) ? kC : 0, p_row = kC - t_row;
     for (uint32_t x = tid; x < kC * 8; x += kPrepThreads) {
         const uint32_t r = x >> 3, c = (x & 7) * 8;
@@ -732,9 +735,9 @@ __global__ void __launch_bounds__(kPrepThreads, 3) chunk_prep_kernel(const __gri
                 v[2 * e + 1] -= __uint_as_float(w[term][e] & 0xFFFF0000u);
             }
         uint8_t *dst = record + piece_at(t_row + r, c >> 3);
-        *reinterpret_cast<uint4 *>(dst) = make_uint4(w[0][0], w[0][1], w[0][2], w[0][3]);
-        *reinterpret_cast<uint4 *>(dst + kTermBytes) = make_uint4(w[1][0], w[1][1], w[1][2], w[1][3]);
-        *reinterpret_cast<uint4 *>(record + 2 * kTermBytes + piece_at(r, c >> 3)) = make_uint4(w[2][0], w[2][1], w[2][2], w[2][3]);
+#pragma unroll
+        for (int term = 0; term < 3; ++term)
+            *reinterpret_cast<uint4 *>(dst + term * kTermBytes) = make_uint4(w[term][0], w[term][1], w[term][2], w[term][3]);
     }
     /* P T in tiles of 16 rows (m) and 8 columns (n), each the sum over the
      * column blocks k = n .. 2 m + 1; a warp's four tiles have 7 to 11 together */
@@ -746,8 +749,8 @@ __global__ void __launch_bounds__(kPrepThreads, 3) chunk_prep_kernel(const __gri
         for (uint32_t k = 0; k < 2 * m + 2; ++k)
             if (k >= n) mma_parts(d, frag_a(P, kLdP, 16 * m, 8 * k, lane), frag_b(A, kLdA, 8 * k, 8 * n, lane));
         const uint32_t col = 8 * n + 2 * (lane & 3), r = p_row + 16 * m + (lane >> 2);
-        put_pair2(record, r, col, parts_sum(d, 0), parts_sum(d, 1));
-        put_pair2(record, r + 8, col, parts_sum(d, 2), parts_sum(d, 3));
+        put_pair3(record, r, col, parts_sum(d, 0), parts_sum(d, 1));
+        put_pair3(record, r + 8, col, parts_sum(d, 2), parts_sum(d, 3));
     }
     if (warp == 0) {
         tc_fence_after();
@@ -778,10 +781,16 @@ struct Scan {
     static constexpr uint32_t kTokenWarps = 4 * kSubs, kEpiWarps = kTokenWarps * kGroups;
     static constexpr uint32_t kThreads = (kEpiWarps + 4) * 32, kLoadThreads = 64;
     static constexpr uint32_t kAtoms = 3 * VB > 64 ? 2 : 1;      /* blocks of 64 columns of an operand of 3 VB */
+    /* With 32 value rows and keys of 256 the third term of P T has no place of
+     * its own: it lies in the half of S0's second block that the third term of
+     * S0 leaves free (pieces 4 to 7 of a row: its columns 0 .. 31 in the rows 0
+     * .. 63, the others in the next 64 rows). */
+    static constexpr bool kSplit = K == 256 && VB == 32;
     /* shared memory */
     static constexpr uint32_t kKQ = 0;
-    static constexpr uint32_t kPair = kKQ + (K / 64) * kBlock;   /* terms of [T; P T], T */
-    static constexpr uint32_t kS = kPair + kPairBytes;           /* terms of S0, rows k */
+    static constexpr uint32_t kPair = kKQ + (K / 64) * kBlock;   /* terms of [T; P T] */
+    static constexpr uint32_t kS = kPair + (kSplit ? 2 * kTermBytes + kC * 128 : kPairBytes); /* terms of S0, rows k */
+    static constexpr uint32_t kThirdP = kS + K * 128 + 64;       /* where kSplit */
     /* terms of the scaled D and of R, rows token. The third term of 32 value
      * rows takes half of a second block: R's first, D's the other half of it. */
     static constexpr uint32_t kD = kS + kAtoms * K * 128;
@@ -789,10 +798,11 @@ struct Scan {
     static constexpr uint32_t kDNext = kR + kC * 128 - kD;
     static constexpr uint32_t kScal = kR + kAtoms * kC * 128;    /* rows of scalars of two chunks */
     static constexpr uint32_t kBar = kScal + 2 * kScalBytes;
-    static constexpr uint32_t kBad = kBar + 192;                 /* of each value row: the first token that is not finite */
+    static constexpr uint32_t kBad = kBar + 200;                 /* of each value row: the first token that is not finite */
     static constexpr uint32_t kBytes = kBad + VB * 4; /* the kernel has no other shared memory: its base is aligned */
     /* TMEM columns */
     static constexpr uint32_t kD1 = 0, kD3 = 4 * VB, kD3Third = kD3 + 3 * VB, kD4 = 8 * VB, kD4Tile = 4 * VB;
+    static constexpr uint32_t kOThird = kSplit ? 3 * VB : kD3Third; /* the third term's product for the outputs */
     static constexpr uint32_t kColumns = 16 * VB;                /* a power of two that holds them */
 };
 
@@ -818,7 +828,7 @@ __global__ void __launch_bounds__(Scan<K, VB>::kThreads, 1)
     const uint32_t bar = base + L::kBar;
     const uint32_t full_kq = bar, empty_k = bar + 16, empty_q = bar + 32, full_pair = bar + 40, empty_pair = bar + 48,
                    s_ready = bar + 56, d1_full = bar + 72, r_ready = bar + 80, d3_full = bar + 88, d_ready = bar + 96,
-                   d4_full = bar + 104, drain = bar + 120, full_scal = bar + 128, empty_scal = bar + 160;
+                   d4_full = bar + 104, drain = bar + 120, full_scal = bar + 128, empty_scal = bar + 160, o_full = L::kSplit ? bar + 184 : d_ready, full_third = bar + 192;
     uint32_t *slot = reinterpret_cast<uint32_t *>(sm + L::kBar + 144);
     volatile uint32_t *abort = reinterpret_cast<volatile uint32_t *>(sm + L::kBar + 152);
     volatile uint32_t *any_bad = reinterpret_cast<volatile uint32_t *>(sm + L::kBar + 176);
@@ -842,6 +852,10 @@ __global__ void __launch_bounds__(Scan<K, VB>::kThreads, 1)
         mbar_init(d3_full, 1);
         mbar_init(d_ready, L::kTokenWarps / 2);
         mbar_init(drain, 1);
+        if (L::kSplit) {
+            mbar_init(o_full, 1);
+            mbar_init(full_third, 1);
+        }
         *abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -897,38 +911,72 @@ __global__ void __launch_bounds__(Scan<K, VB>::kThreads, 1)
         }
         cp_async_wait_all();
     } else if (warp == kRecWarp) {
-        if (lane == 0) {
-            /* [T; P T] of a chunk once the MMAs have read that of the chunk
-             * before, the next chunk's scalars once every epilogue warp has
-             * read those of two chunks before it: not every one of them waits
-             * for these MMAs. */
-            auto copy = [&](uint32_t dst, const uint8_t *src, uint32_t bytes, uint32_t full) {
-                asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(full), "r"(bytes) : "memory");
-                asm volatile(
-                    "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
-                    "l"(src), "r"(bytes), "r"(full)
-                    : "memory");
-            };
-            const uint8_t *src = records + ((size_t)rec0 * p.HV + h) * kRecordBytes;
-            const size_t step = (size_t)p.HV * kRecordBytes;
-            uint32_t pairs = 0, scals = 1; /* copies begun */
-            copy(base + L::kScal, src + kPairBytes, kScalBytes, full_scal);
-            for (; pairs < chunks; src += step) {
-                if (pairs >= 1 && !wait_bar<true>(empty_pair, (pairs - 1) & 1u, abort)) break;
-                copy(base + L::kPair, src, kPairBytes, full_pair);
-                if (++pairs == chunks) break;
-                const uint32_t st = scals & 1;
-                if (scals >= 2 && !wait_bar<true>(empty_scal + 8 * st, (scals / 2 - 1) & 1u, abort)) break;
-                copy(base + L::kScal + st * kScalBytes, src + step + kPairBytes, kScalBytes, full_scal + 8 * st);
-                ++scals;
+        /* [T; P T] of a chunk once the MMAs have read that of the chunk
+         * before, the next chunk's scalars once every epilogue warp has
+         * read those of two chunks before it: not every one of them waits
+         * for these MMAs. */
+        auto expect = [&](uint32_t bytes, uint32_t full) {
+            asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(full), "r"(bytes) : "memory");
+        };
+        auto copy = [&](uint32_t dst, const uint8_t *src, uint32_t bytes, uint32_t full) {
+            asm volatile(
+                "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+                "l"(src), "r"(bytes), "r"(full)
+                : "memory");
+        };
+        auto copy_scalars = [&](const uint8_t *src, uint32_t st) {
+            if (lane != 0) return;
+            expect(kScalBytes, full_scal + 8 * st);
+            copy(base + L::kScal + st * kScalBytes, src + kPairBytes, kScalBytes, full_scal + 8 * st);
+        };
+        auto copy_pair = [&](const uint8_t *src, uint32_t chunk) {
+            if (lane != 0) return;
+            constexpr uint32_t kThird = L::kSplit ? kC * 128 : 0;
+            expect(L::kS - L::kPair, full_pair);
+            copy(base + L::kPair, src, L::kSplit ? 2 * kTermBytes : kPairBytes, full_pair);
+            if (L::kSplit)
+                copy(base + L::kPair + 2 * kTermBytes, src + 2 * kTermBytes + (chunk & 1) * kThird, kThird, full_pair);
+        };
+        /* the third term of P T, in the rows of the chunk's q, once the MMAs
+         * have read that of the chunk before. Its pieces keep their places in the
+         * swizzle; those of the columns 0 .. 31 go to the other half of the row. */
+        auto copy_third = [&](const uint8_t *src, uint32_t chunk) {
+            if (chunk >= 1 && !wait_bar_warp<true>(o_full, (chunk - 1) & 1u, abort)) return false;
+            src += 2 * kTermBytes + (1 - (chunk & 1)) * kC * 128;
+            const uint32_t dst = base + L::kThirdP - 64;
+#pragma unroll 4
+            for (uint32_t x = lane; x < kC * 8; x += 32) {
+                const uint32_t r = x >> 3, at = x & 7, right = (at ^ r) & 4; /* where the piece lies; whether of columns 32 .. 63 */
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                                 dst + ((right ? kC : 0) + r) * 128 + ((right ? at : at ^ 4) << 4)),
+                             "l"(src + x * 16)
+                             : "memory");
             }
-            /* the last copies land before the CTA ends (an abort does not stop them) */
-            auto landed = [&](uint32_t x) { return mbar_try(full_scal + 8 * (x & 1), (x >> 1) & 1u); };
-            const uint64_t w0 = gtimer();
-            while (!((pairs == 0 || mbar_try(full_pair, (pairs - 1) & 1u)) && landed(scals - 1) &&
-                     (scals == 1 || landed(scals - 2))) &&
-                   gtimer() - w0 < kWaitNs) {
-            }
+            cp_async_wait_all();
+            fence_async();
+            warp_arrive(full_third);
+            return true;
+        };
+        const uint8_t *src = records + ((size_t)rec0 * p.HV + h) * kRecordBytes;
+        const size_t step = (size_t)p.HV * kRecordBytes;
+        uint32_t pairs = 0, scals = 1; /* copies begun */
+        copy_scalars(src, 0);
+        for (; pairs < chunks; src += step) {
+            if (pairs >= 1 && !wait_bar_warp<true>(empty_pair, (pairs - 1) & 1u, abort)) break;
+            copy_pair(src, pairs++);
+            if (L::kSplit && !copy_third(src, pairs - 1)) break;
+            if (pairs == chunks) break;
+            const uint32_t st = scals & 1;
+            if (scals >= 2 && !wait_bar_warp<true>(empty_scal + 8 * st, (scals / 2 - 1) & 1u, abort)) break;
+            copy_scalars(src + step, st);
+            ++scals;
+        }
+        /* the last copies land before the CTA ends (an abort does not stop them) */
+        auto landed = [&](uint32_t x) { return mbar_try(full_scal + 8 * (x & 1), (x >> 1) & 1u); };
+        const uint64_t w0 = gtimer();
+        while (!((pairs == 0 || mbar_try(full_pair, (pairs - 1) & 1u)) && landed(scals - 1) &&
+                 (scals == 1 || landed(scals - 2))) &&
+               gtimer() - w0 < kWaitNs) {
         }
     } else if (warp == kMmaWarp) {
         /* the whole warp walks along, so that what the MMAs take stays in
@@ -936,7 +984,7 @@ __global__ void __launch_bounds__(Scan<K, VB>::kThreads, 1)
         const uint32_t leader = elect_one();
         const uint32_t s_desc = desc(base + L::kS, K * 128), r_desc = desc(base + L::kR, kC * 128),
                        x_desc = desc(base + L::kD, L::kDNext + 64), pair_desc = desc(base + L::kPair, 16),
-                       third_desc = desc(base + L::kPair + 2 * kTermBytes, 16);
+                       third_desc = desc(base + L::kPair + 2 * kTermBytes, 16), third_p_desc = desc(base + L::kThirdP, 16);
         constexpr uint32_t kAll = 3 * VB, kTwo = 2 * VB;
         for (uint32_t c = 0; c < chunks; ++c) {
             const uint32_t st = c & 1, ph = c & 1;
@@ -966,8 +1014,10 @@ __global__ void __launch_bounds__(Scan<K, VB>::kThreads, 1)
             tc_fence_after();
             if (leader) {
                 /* [T; P T] R: the first term with all of R, the second with R's first
-                 * two, T's third with R's first, in columns of their own: the
-                 * rows of q run into other memory there and are not read */
+                 * two, the third with R's first, in columns of their own. Where
+                 * kSplit, T's third alone: the rows of q run into other memory and
+                 * are not read, nor are those of k with P T's third, which nobody
+                 * but the outputs waits for. */
 #pragma unroll
                 for (int kk = 0; kk < kC / 16; ++kk)
                     mma(d3, pair_desc + ((kk * 32) >> 4), r_desc + ((kk * 2048) >> 4), instr_desc(128, kAll, false, true), kk != 0);
@@ -977,10 +1027,22 @@ __global__ void __launch_bounds__(Scan<K, VB>::kThreads, 1)
                         instr_desc(128, kTwo, false, true), true);
 #pragma unroll
                 for (int kk = 0; kk < kC / 16; ++kk)
-                    mma(tmem + L::kD3Third, third_desc - st * ((kC * 128) >> 4) + ((kk * 32) >> 4), r_desc + ((kk * 2048) >> 4),
-                        instr_desc(128, VB, false, true), kk != 0);
+                    mma(tmem + L::kD3Third, third_desc - (L::kSplit ? st * ((kC * 128) >> 4) : 0) + ((kk * 32) >> 4),
+                        r_desc + ((kk * 2048) >> 4), instr_desc(128, VB, false, true), kk != 0);
                 commit(d3_full);
                 commit(empty_pair);
+            }
+            if (L::kSplit) {
+                if (!wait_bar_warp(full_third, ph, abort)) break;
+                tc_fence_after();
+                if (leader) {
+#pragma unroll
+                    for (int kk = 0; kk < kC / 16; ++kk)
+                        mma(tmem + L::kOThird,
+                            third_p_desc + (((kk >> 1) * kC * 128 + (kk & 1) * 32) >> 4) - (1 - st) * ((kC * 128) >> 4),
+                            r_desc + ((kk * 2048) >> 4), instr_desc(128, VB, false, true), kk != 0);
+                    commit(o_full);
+                }
             }
             if (!wait_bar_warp(d_ready, ph, abort)) break;
             tc_fence_after();
@@ -1089,14 +1151,20 @@ __global__ void __launch_bounds__(Scan<K, VB>::kThreads, 1)
                     tc_fence_before();
                     warp_arrive(r_ready);
                 }
-                if (!(ok = wait_bar_warp(d3_full, ph, abort))) break;
+                /* the outputs' rows let those of D go first, which the state waits
+                 * for (4096 tokens 168.7 us, both at once 170.4) */
+                if (!(ok = wait_bar_warp(q ? o_full : d3_full, ph, abort))) break;
                 tc_fence_after();
                 tc_sum3<VB>(d3 + at, x);
+                uint32_t third[8];
+                __syncwarp();
+                tc_ld8(tmem + (q ? L::kOThird : L::kD3Third) + at, third);
+                tc_wait();
                 if (q) {
                     if (i < rows) {
                         __nv_bfloat16 *dst = out + (int64_t)(tc + i) * p.out_token + 8 * sub;
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) o[e] += x[e];
+                        for (int e = 0; e < 8; ++e) o[e] += x[e] + __uint_as_float(third[e]);
                         if (*any_bad) {
 #pragma unroll
                             for (int e = 0; e < 8; ++e)
@@ -1111,10 +1179,6 @@ __global__ void __launch_bounds__(Scan<K, VB>::kThreads, 1)
                         }
                     }
                 } else {
-                    uint32_t third[8];
-                    __syncwarp();
-                    tc_ld8(tmem + L::kD3Third + at, third);
-                    tc_wait();
 #pragma unroll
                     for (int e = 0; e < 8; ++e) x[e] = f2 * (x[e] + __uint_as_float(third[e]));
                     if (poison) {

@@ -208,3 +208,26 @@ def test_no_value_spreads_backwards(ops, rule, what, bad, shape):
         assert plain.rel(out[fine], ref_o[fine]) <= out_tol(rule, torch.bfloat16)
         fine = ref_s.isfinite()
         assert plain.rel(state[fine], ref_s[fine]) <= STATE_TOL
+
+
+@pytest.mark.parametrize("shape", [(2, 2, 64, 64), (2, 2, 128, 128), (6, 6, 128, 128), (1, 1, 256, 256), (6, 6, 256, 256)], ids=str)
+@pytest.mark.parametrize("length", [64, 700])
+def test_chunk_outputs_are_fp32_before_their_rounding(ops, length, shape):
+    """The output's rounding to BF16 hides an error e before it except where it
+    falls the other way: for a value with spacing u between its neighbours that
+    happens with probability |e| / u and then costs u. With u <= 2^-7 |o| the
+    squares sum to sum |e| u <= 2^-7 ||e|| ||o||: sqrt(2^-7 E) off the rounded
+    exact output for a relative error E. FP32 sums of 256 + 64 products have E =
+    sqrt(320) 2^-24 / sqrt(3) (a rounding is spread evenly over its interval),
+    so 7.0e-5. The count of these outputs varies: a tenth of it, where there
+    are 100; n outputs have about n E 2^7."""
+    E = 320 ** 0.5 * 2 ** -24 / 3 ** 0.5
+    n = max(1, 2000 // length)
+    a, o = inputs([length] * n, *shape, torch.bfloat16, seed=45)
+    a["k"] = (a["k"].float() * 0.5 + 1).bfloat16()  # keys somewhat alike and large beta: outputs that the chunk's tokens make
+    a["beta"] = 0.5 + 0.5 * a["beta"]
+    o["fresh"] = torch.ones(n, dtype=torch.bool, device="cuda")
+    ref_o, _ = plain.delta_rule(**a, **o)
+    out = ops.delta_chunk(**a, **o)
+    flips = ref_o.numel() * E * 2 ** 7
+    assert plain.rel(out, ref_o.bfloat16().double()) <= (2 ** -7 * E) ** 0.5 * (1 + 2 * flips ** -0.5)
