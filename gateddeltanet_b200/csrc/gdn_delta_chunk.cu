@@ -326,8 +326,9 @@ __device__ __forceinline__ void place_sequences(const DeltaParams &p, uint32_t *
  * or of P (q). T = (I + A)^-1 by blocks,
  *   [[a 0] [c b]]^-1 = [[a^-1 0] [-b^-1 c a^-1, b^-1]],
  * the four of 16 on the diagonal by substitution, a warp each and a lane per
- * row; the products, and P T, with mma.sync of TF32 parts (x = x0 + x1, three
- * of the four products: 21 bits of each). What bounds it is the chain of these
+ * row; the products, and P T, with mma.sync of TF32 parts (x = x0 + x1 + x2, six
+ * of the nine products: 24 bits of each; with x0 + x1 and three products, 21
+ * bits, the states of like keys were 1.4e-6 off). What bounds it is the chain of these
  * steps, 17000 cycles, against which three CTAs share an SM: 24 us for 64
  * chunks of 8 heads of 256. */
 constexpr int kPrepThreads = 256;
@@ -383,33 +384,39 @@ __device__ __forceinline__ void invert16(float *A, uint32_t lane) {
     }
 }
 
-/* Fragments of m16n8k8, g = lane / 4, t = lane % 4, each element in two TF32 parts */
+/* Fragments of m16n8k8, g = lane / 4, t = lane % 4, each element in three TF32
+ * parts, 11 significant bits each from the top: all 24 of FP32 */
+constexpr int kParts = 3;
 struct FragA {
-    uint32_t hi[4], lo[4];
+    uint32_t v[kParts][4];
 };
 struct FragB {
-    uint32_t hi[2], lo[2];
+    uint32_t v[kParts][2];
 };
-__device__ __forceinline__ void tf32_parts(float x, uint32_t &hi, uint32_t &lo) {
-    hi = __float_as_uint(x) & 0xFFFFE000u;
-    lo = __float_as_uint(x - __uint_as_float(hi));
+template <int N>
+__device__ __forceinline__ void tf32_parts(float x, uint32_t (&v)[kParts][N], int i) {
+#pragma unroll
+    for (int part = 0; part < kParts; ++part) {
+        v[part][i] = __float_as_uint(x) & 0xFFFFE000u;
+        x -= __uint_as_float(v[part][i]);
+    }
 }
 /* rows r .. r + 15, columns c .. c + 7 of m */
 __device__ __forceinline__ FragA frag_a(const float *m, uint32_t ld, uint32_t r, uint32_t c, uint32_t lane) {
     FragA f;
     const float *p = m + (r + (lane >> 2)) * ld + c + (lane & 3);
-    tf32_parts(p[0], f.hi[0], f.lo[0]);
-    tf32_parts(p[8 * ld], f.hi[1], f.lo[1]);
-    tf32_parts(p[4], f.hi[2], f.lo[2]);
-    tf32_parts(p[8 * ld + 4], f.hi[3], f.lo[3]);
+    tf32_parts(p[0], f.v, 0);
+    tf32_parts(p[8 * ld], f.v, 1);
+    tf32_parts(p[4], f.v, 2);
+    tf32_parts(p[8 * ld + 4], f.v, 3);
     return f;
 }
 /* rows (k) r .. r + 7, columns (n) c .. c + 7 of m */
 __device__ __forceinline__ FragB frag_b(const float *m, uint32_t ld, uint32_t r, uint32_t c, uint32_t lane) {
     FragB f;
     const float *p = m + (r + (lane & 3)) * ld + c + (lane >> 2);
-    tf32_parts(p[0], f.hi[0], f.lo[0]);
-    tf32_parts(p[4 * ld], f.hi[1], f.lo[1]);
+    tf32_parts(p[0], f.v, 0);
+    tf32_parts(p[4 * ld], f.v, 1);
     return f;
 }
 __device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
@@ -418,11 +425,15 @@ __device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], 
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
 }
-/* the three products in accumulators of their own, so that they do not wait for one another */
+/* The products of at least 2^-22 of the first, by size in three accumulators:
+ * they do not wait for one another, and small sums are not lost in large ones. */
 __device__ __forceinline__ void mma_parts(float (&d)[3][4], const FragA &a, const FragB &b) {
-    mma_tf32(d[0], a.lo, b.hi);
-    mma_tf32(d[1], a.hi, b.lo);
-    mma_tf32(d[2], a.hi, b.hi);
+    mma_tf32(d[0], a.v[2], b.v[0]);
+    mma_tf32(d[1], a.v[1], b.v[0]);
+    mma_tf32(d[2], a.v[0], b.v[0]);
+    mma_tf32(d[0], a.v[0], b.v[2]);
+    mma_tf32(d[1], a.v[0], b.v[1]);
+    mma_tf32(d[0], a.v[1], b.v[1]);
 }
 __device__ __forceinline__ float parts_sum(const float (&d)[3][4], int e) { return d[2][e] + (d[0][e] + d[1][e]); }
 /* rows r .. r + 15, columns c .. c + 7 of out = sign * a b, over kK columns of a;

@@ -296,7 +296,8 @@ int gdn_b200_test_tile_gemm(uint32_t m, uint32_t k, uint32_t n, const float *w, 
  *   S = e^g S;  d = beta (v - S k);  S = S + d k^T;  o = scale S q
  * with q and k first divided by sqrt(sum x^2 + 1e-6) if normalize != 0.
  * q, k, v and out are BF16 (dtype 1) or FP32 (dtype 0); g (the log decay),
- * beta and the pool are FP32; all arithmetic is FP32 or closer. Strides count
+ * beta and the pool are FP32; all arithmetic is FP32 or closer (exponentials to
+ * 2^-22). Strides count
  * elements; the innermost dimension (K or V) is contiguous, and a slot of the
  * pool is one block [v_heads][V][K] on a 16-byte boundary. A sequence
  * whose slot lies outside the pool changes no state and gives zeros, as do

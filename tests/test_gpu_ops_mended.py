@@ -231,3 +231,18 @@ def test_chunk_outputs_are_fp32_before_their_rounding(ops, length, shape):
     out = ops.delta_chunk(**a, **o)
     flips = ref_o.numel() * E * 2 ** 7
     assert plain.rel(out, ref_o.bfloat16().double()) <= (2 ** -7 * E) ** 0.5 * (1 + 2 * flips ** -0.5)
+
+
+@pytest.mark.parametrize("shape", [(1, 1, 64, 64), (2, 2, 128, 128), (2, 2, 256, 256)], ids=str)
+@pytest.mark.parametrize("alike", [0.3, 0.1, 0.0])
+@pytest.mark.parametrize("weakest", [0.5, 0.95])
+def test_chunk_of_like_keys_with_large_beta(ops, alike, weakest, shape):
+    """Keys nearly or fully the same and beta near 1: (I + A)^-1 has entries
+    of at most 1 that fall off by 1 - beta from one token to the next, so that
+    no rounding grows: the states are FP32 sums as elsewhere, sqrt(320) 2^-24 /
+    sqrt(3) (a rounding is spread evenly over its interval), for the products
+    of the state and again for those of the inverse."""
+    a, o = inputs([700, 65], *shape, torch.bfloat16, seed=46)
+    a["k"] = (a["k"].float() * alike + 1).bfloat16()
+    a["beta"] = weakest + (1 - weakest) * torch.rand_like(a["beta"])
+    compare(ops.delta_chunk, a, o, out_tol("delta_chunk", torch.bfloat16), state_tol=(320 * 2 / 3) ** 0.5 * 2 ** -24)
