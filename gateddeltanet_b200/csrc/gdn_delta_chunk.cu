@@ -302,8 +302,16 @@ __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;"
 
 /* order[i]: the i-th longest sequence. The walks start in this order, so that
  * the last to start are short. The CTAs of the first value head take the
- * sequences in turn; a place is the number of sequences that come before. */
+ * sequences in turn; a place is the number of sequences that come before. Each
+ * looks at all of them: very many stay in their own order, whose walks are dealt
+ * out over many rounds anyway (300000 single tokens of one small head: 460 ms in
+ * order of length, 16 in their own). */
+constexpr uint32_t kMaxOrdered = 4096;
 __device__ __forceinline__ void place_sequences(const DeltaParams &p, uint32_t *order) {
+    if (p.N > kMaxOrdered) {
+        for (uint32_t n = blockIdx.x * blockDim.x + threadIdx.x; n < p.N; n += gridDim.x * blockDim.x) order[n] = n;
+        return;
+    }
     for (uint32_t n = blockIdx.x; n < p.N; n += gridDim.x) {
         uint32_t a, b, before = 0;
         sequence_tokens(p, n, a, b);

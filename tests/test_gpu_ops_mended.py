@@ -246,3 +246,31 @@ def test_chunk_of_like_keys_with_large_beta(ops, alike, weakest, shape):
     a["k"] = (a["k"].float() * alike + 1).bfloat16()
     a["beta"] = weakest + (1 - weakest) * torch.rand_like(a["beta"])
     compare(ops.delta_chunk, a, o, out_tol("delta_chunk", torch.bfloat16), state_tol=(320 * 2 / 3) ** 0.5 * 2 ** -24)
+
+
+@pytest.mark.parametrize("n", [4096, 4097, 9000])
+def test_chunk_of_more_sequences_than_are_ordered(ops, n):
+    gen = torch.Generator().manual_seed(n)
+    lengths = torch.randint(0, 3, (n,), generator=gen).tolist()
+    lengths[n // 2], lengths[-1] = 130, 70
+    a, o = inputs(lengths, 1, 1, 64, 32, torch.bfloat16, seed=n)
+    compare(ops.delta_chunk, a, o, out_tol("delta_chunk", torch.bfloat16))
+
+
+def test_chunk_time_grows_with_the_sequences_not_their_square(ops):
+    def ms(n):
+        one = lambda width: torch.zeros(n, 1, width, device="cuda", dtype=torch.bfloat16)  # noqa: E731
+        gates = torch.zeros(n, 1, device="cuda")
+        state = torch.zeros(n, 1, 32, 64, device="cuda")
+        starts = torch.arange(n + 1, dtype=torch.int32, device="cuda")
+        begin, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        times = []
+        for _ in range(4):
+            q, k, v = one(64), one(64), one(32)
+            begin.record()
+            ops.delta_chunk(q, k, v, gates, gates, state, starts=starts)
+            end.record()
+            torch.cuda.synchronize()
+            times.append(begin.elapsed_time(end))
+        return min(times)
+    assert ms(100000) <= 10 * ms(20000)  # five times the work; by squares 25 times
