@@ -332,7 +332,10 @@ int gdn_b200_delta_step(const GdnB200DeltaArgs *args);
  * not finite spreads as in gdn_b200_delta_step, but infinities come out as NaN. */
 int gdn_b200_delta_chunk(const GdnB200DeltaArgs *args);
 /* Bytes of 256-byte aligned device memory that gdn_b200_delta_chunk needs as
- * args->workspace for these sizes. */
+ * args->workspace for these sizes: 49.1 KB for each value head and 64 tokens, and
+ * for each value head and sequence (786 bytes a token and value head for long
+ * prompts; a call of few tokens a sequence is better made of gdn_b200_delta_step,
+ * which needs none). */
 size_t gdn_b200_delta_chunk_workspace(uint32_t tokens, uint32_t sequences, uint32_t v_heads);
 /* 0, or -1 if a wait inside gdn_b200_delta_step or gdn_b200_delta_chunk ran
  * out (2 s) on `device` since the last call of this function: the states of

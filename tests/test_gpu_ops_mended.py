@@ -274,3 +274,47 @@ def test_chunk_time_grows_with_the_sequences_not_their_square(ops):
             times.append(begin.elapsed_time(end))
         return min(times)
     assert ms(100000) <= 10 * ms(20000)  # five times the work; by squares 25 times
+
+
+@pytest.mark.parametrize("shape", [(4, 8, 128, 128), (9, 9, 128, 64), (3, 6, 128, 96)], ids=str)
+def test_chunk_many_heads_of_128(ops, shape):
+    """More CTAs than SMs: 32 value rows each."""
+    a, o = inputs([129, 0, 64, 1, 40, 200, 63], *shape, torch.bfloat16, seed=47)
+    o["fresh"] = torch.tensor([True, True, False, False, True, False, False], device="cuda")
+    compare(ops.delta_chunk, a, o, out_tol("delta_chunk", torch.bfloat16))
+
+
+@pytest.mark.parametrize("history", [65535, 65536])
+@pytest.mark.parametrize("shift", [0, 1, 4])
+def test_long_history_of_bfloat16(ops, history, shift):
+    """Counts on both sides of 16 bits, in neighbouring tokens, in rows of any alignment."""
+    tokens = torch.full((2, history), 11, dtype=torch.int32, device="cuda")
+    tokens[0, :7] = 12
+    tokens[1] = 10
+    tokens[1, 5:8] = 700
+    wide = torch.ones(2, 1003 + 8, device="cuda", dtype=torch.bfloat16)
+    logits = wide[:, shift:shift + 1003]
+    each = lambda x: torch.full((2,), x, device="cuda")  # noqa: E731
+    args = dict(tokens=tokens, frequency=each(1.0), repetition=each(2.0), presence=each(0.25),
+                prompt_lens=torch.tensor([3, 0], dtype=torch.int32, device="cuda"))
+    out, picks = ops.constrain_logits(logits, **args)
+    ref = plain.constrain(logits, **args)
+    assert torch.equal(out.cpu(), ref.bfloat16()) and picks.tolist() == [0, 0]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("many", [(60, 2, 10, 128, 128), (20, 8, 8, 256, 256), (67, 1, 6, 256, 96), (301, 2, 4, 128, 96)], ids=str)
+def test_pipeline_of_sequences_with_and_without_tokens(ops, many, dtype):
+    """No more tokens than sequences and eight row blocks for each SM: delta_step's pipeline, with groups of up to
+    eight tokens, longer sequences, fresh ones and slots outside the pool, at its blocks' edges."""
+    n, *shape = many
+    gen = torch.Generator().manual_seed(n + 1)
+    lengths = torch.zeros(n, dtype=torch.int64)
+    for at, length in ((1, 1), (2, 7), (n // 3, 8), (n // 2, 1), (n - 2, 3)):
+        lengths[at] = length
+    lengths[n - 1] = n - int(lengths.sum())  # the last sequence has the rest, more than a group
+    a, o = inputs(lengths.tolist(), *shape, dtype, seed=n)
+    o["fresh"] = (torch.rand(n, generator=gen) < 0.4).cuda()
+    o["fresh"][2], o["fresh"][n - 1] = True, False
+    o["slots"][n // 3] = -1
+    compare(ops.delta_step, a, o, out_tol("delta_step", dtype))
