@@ -176,6 +176,7 @@ EXPORTS = [
     ("gdn_b200_delta_chunk_workspace", ctypes.c_size_t, [ctypes.c_uint32, ctypes.c_uint32, ctypes.c_uint32]),
     ("gdn_b200_delta_status", ctypes.c_int, [ctypes.c_int]),
     ("gdn_b200_constrain_logits", ctypes.c_int, [ctypes.c_char_p]),
+    ("gdn_b200_test_drop_copy", ctypes.c_int, [ctypes.c_uint32]),
 ]
 
 GDN_B200_TP_TOKEN_BYTES = 128

@@ -361,11 +361,12 @@ __global__ void __launch_bounds__(kPipeThreads, 1) delta_pipe_kernel(const __gri
                 if (w.slot >= 0 && !w.fresh) {
                     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(full + 8 * sl), "r"(bytes)
                                  : "memory");
-                    asm volatile(
-                        "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1], %2, [%3], %4;" ::"r"(
-                            base + sl * kBlockBytes),
-                        "l"(S), "r"(bytes), "r"(full + 8 * sl), "l"(policy)
-                        : "memory");
+                    if (w.u + 1 != p.drop)
+                        asm volatile(
+                            "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1], %2, [%3], %4;" ::"r"(
+                                base + sl * kBlockBytes),
+                            "l"(S), "r"(bytes), "r"(full + 8 * sl), "l"(policy)
+                            : "memory");
                 } else {
                     mbar_arrive(full + 8 * sl);
                 }
@@ -516,6 +517,15 @@ __global__ void __launch_bounds__(kPipeThreads, 1) delta_pipe_kernel(const __gri
         }
     }
     if (tid == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    if (!rows_all(*abort == 0)) {
+        /* given up: none of this CTA's states is left that could pass for one */
+        const float bad = __int_as_float(0x7fc00000);
+        for (Walk w(p, g, u0); w.u < u1; w.next(p, g, u1)) {
+            if (w.idle() || w.slot < 0) continue;
+            float4 *S = reinterpret_cast<float4 *>(p.state + w.slot * p.state_slot + ((int64_t)w.h * p.V + w.blk * g.rows) * K);
+            for (uint32_t j = tid; j < g.rows * K / 4; j += kRowThreads) S[j] = make_float4(bad, bad, bad, bad);
+        }
+    }
 }
 
 template <int K>

@@ -952,6 +952,7 @@ __global__ void __launch_bounds__(Scan<K, VB>::kThreads, 1)
             if (lane != 0) return;
             constexpr uint32_t kThird = L::kSplit ? kC * 128 : 0;
             expect(L::kS - L::kPair, full_pair);
+            if (blockIdx.x + 1 == p.drop) return;
             copy(base + L::kPair, src, L::kSplit ? 2 * kTermBytes : kPairBytes, full_pair);
             if (L::kSplit)
                 copy(base + L::kPair + 2 * kTermBytes, src + 2 * kTermBytes + (chunk & 1) * kThird, kThird, full_pair);

@@ -27,6 +27,7 @@ struct DeltaParams {
     uint32_t N, tokens, H, HV, K, V, state_slots;
     int normalize;
     float scale;
+    uint32_t drop; /* for tests, 0: none. 1 + the row block (pipeline) or CTA (chunks) whose copy is not made */
 };
 
 /* Tokens [t0, t1) of sequence n, clamped to the packed tensors so that no

@@ -69,6 +69,8 @@ int on_device(const char *who, int device, F launch) {
     return e == cudaSuccess ? 0 : cuda_failf(who, "launch failed", e);
 }
 
+std::atomic<uint32_t> g_drop{0}; /* gdn_b200_test_drop_copy */
+
 /* Checks what both forms of the rule ask of their arguments; > 0: nothing to do. */
 int delta_params(const char *who, const GdnB200DeltaArgs *a, gdn::ops::DeltaParams &p) {
     if (a == nullptr) return failf("%s: no arguments", who);
@@ -105,7 +107,7 @@ int delta_params(const char *who, const GdnB200DeltaArgs *a, gdn::ops::DeltaPara
                               a->q_token, a->q_head, a->k_token, a->k_head, a->v_token, a->v_head,
                               a->g_token, a->g_head, a->beta_token, a->beta_head, a->out_token, a->out_head,
                               a->state_slot, a->sequences, a->tokens, a->heads, a->v_heads, a->key_dim,
-                              a->value_dim, a->state_slots, a->normalize != 0, a->scale};
+                              a->value_dim, a->state_slots, a->normalize != 0, a->scale, g_drop.exchange(0)};
     return 0;
 }
 
@@ -137,6 +139,11 @@ int gdn_b200_delta_status(int device) {
     return step == 0 && chunk == 0 ? 0
                                    : failf("gdn_b200_delta_%s: a wait on the device ran out; the call's states are not valid",
                                            chunk != 0 ? "chunk" : "step");
+}
+
+int gdn_b200_test_drop_copy(uint32_t index) {
+    g_drop = index + 1;
+    return 0;
 }
 
 int gdn_b200_delta_chunk(const GdnB200DeltaArgs *args) {

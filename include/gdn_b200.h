@@ -343,6 +343,11 @@ size_t gdn_b200_delta_chunk_workspace(uint32_t tokens, uint32_t sequences, uint3
  * checks and for tests. */
 int gdn_b200_delta_status(int device);
 
+/* Test hook: in the next gdn_b200_delta_step or gdn_b200_delta_chunk of the
+ * process the copy of one row block (if that call streams blocks through shared
+ * memory) or of one CTA's first chunk is not made, so that a wait runs out. */
+int gdn_b200_test_drop_copy(uint32_t index);
+
 /* Constraints on the logits of `rows` streams, and the greedy pick. With n
  * the times token v stands in the row's history after its prompt:
  *   in the history:    x = x > 0 ? x / repetition : x * repetition

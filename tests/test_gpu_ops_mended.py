@@ -318,3 +318,30 @@ def test_pipeline_of_sequences_with_and_without_tokens(ops, many, dtype):
     o["fresh"][2], o["fresh"][n - 1] = True, False
     o["slots"][n // 3] = -1
     compare(ops.delta_step, a, o, out_tol("delta_step", dtype))
+
+
+@pytest.mark.parametrize("rule,lengths,shape", [("delta_step", [1] * 40, (8, 8, 256, 256)), ("delta_chunk", [200, 70, 129], (2, 2, 256, 256)),
+                                                ("delta_chunk", [200, 70, 129], (8, 8, 256, 256)),
+                                                ("delta_chunk", [200, 70, 129], (2, 2, 64, 64))], ids=str)
+def test_a_wait_that_runs_out_leaves_no_state_to_pass_for_one(ops, rule, lengths, shape):
+    """A copy that is not made: the CTA that waits for it gives up after its limit, its states are NaN, the others right,
+    the status says so once, and the next call is as if nothing had been."""
+    import gateddeltanet_b200 as gdn
+    ops.delta_status()
+    a, o = inputs(lengths, *shape, torch.bfloat16, seed=49)
+    start = a["state"].clone()
+    ref_o, ref_s = plain.delta_rule(**a, **o)
+    assert gdn.lib().gdn_b200_test_drop_copy(3) == 0
+    getattr(ops, rule)(**a, **o)
+    with pytest.raises(RuntimeError, match="ran out"):
+        ops.delta_status()
+    ops.delta_status()
+    state, slots = a["state"].cpu().double(), o["slots"].cpu().long()
+    bad = state.isnan()
+    rows = bad.any(-1)
+    assert torch.equal(rows, bad.all(-1)) and 0 < int(rows.sum()) < int(rows[slots].numel())
+    assert not bool(rows[[i for i in range(rows.shape[0]) if i not in slots.tolist()]].any())
+    assert plain.rel(state[~bad], ref_s[~bad]) <= STATE_TOL
+    assert bool(rows[slots[0], 0].any())
+    a["state"] = start
+    compare(getattr(ops, rule), a, o, out_tol(rule, torch.bfloat16))
