@@ -31,6 +31,17 @@ int cuda_failf(const char *who, const char *what, cudaError_t e) {
 
 bool aligned(const void *p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
+/* Whether two tables of `rows` rows of `width` bytes share memory, other than
+ * row by row in the same place. Strides are not negative. */
+bool partly_shared(const void *x, int64_t x_row, const void *y, int64_t y_row, int64_t rows, int64_t width) {
+    const int64_t d = (int64_t)(reinterpret_cast<uintptr_t>(y) - reinterpret_cast<uintptr_t>(x));
+    if (rows == 1) x_row = y_row = width;
+    if (d >= (rows - 1) * x_row + width || -d >= (rows - 1) * y_row + width) return false;
+    if (x_row != y_row || x_row < width) return true;
+    const int64_t shift = (d % x_row + x_row) % x_row; /* of y's rows against x's */
+    return d != 0 && (shift < width || shift + width > x_row);
+}
+
 /* The call's device for the thread, and the previous one afterwards. */
 struct DeviceScope {
     int prev = -1;
@@ -185,6 +196,8 @@ int gdn_b200_constrain_logits(const GdnB200LogitsArgs *args) {
     if (!aligned(a.logits, elem) || !aligned(a.out, elem)) return failf("%s: logits or out is misaligned", who);
     if (a.rows > 1 && a.out_row < (int64_t)a.vocab) return failf("%s: rows of out overlap", who);
     if (a.logits_row < 0) return failf("%s: negative row stride", who);
+    if (partly_shared(a.logits, a.logits_row * (int64_t)elem, a.out, a.out_row * (int64_t)elem, a.rows, a.vocab * (int64_t)elem))
+        return failf("%s: out overlaps logits without being logits", who);
     gdn::ops::LogitsParams p{a.logits, a.out, a.picks, a.history ? a.tokens : nullptr, a.lens, a.prompt_lens,
                              a.repetition, a.presence, a.frequency, a.biases ? a.bias_ids : nullptr, a.bias, a.mask,
                              a.logits_row, a.out_row, a.tokens_row, a.bias_ids_row, a.bias_row, a.mask_row,

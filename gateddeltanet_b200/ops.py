@@ -54,7 +54,8 @@ def delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tenso
     sequences' bounds (None: one token each); slots int32 [sequences]: their
     distinct states (None: in order); fresh bool [sequences]: start from zero.
     scale defaults to key_dim ** -0.5; normalize divides q and k by their L2
-    norms. Returns the outputs [tokens, v_heads, value_dim]."""
+    norms. Returns the outputs [tokens, v_heads, value_dim] (`out` if given, in
+    memory apart from the inputs)."""
     return _native.delta_step(q, k, v, g, beta, state, starts, slots, fresh, scale, normalize, out)
 
 
@@ -93,5 +94,6 @@ def constrain_logits(logits: torch.Tensor, *, tokens: Optional[torch.Tensor] = N
     frequency float32 [rows]; bias_ids int32 and bias float32 [rows, entries]
     (id -1: not used); mask int32 [rows, ceil(vocab / 32)], bit v % 32 of word
     v // 32 set where token v is allowed. Returns (out, picks int32 [rows]);
-    out may be the logits themselves, and a pick is -1 where nothing is left."""
+    out may be the logits themselves or memory apart from them, and a pick is -1
+    where nothing is left."""
     return _native.constrain_logits(logits, tokens, lens, prompt_lens, repetition, presence, frequency, bias_ids, bias, mask, out)
