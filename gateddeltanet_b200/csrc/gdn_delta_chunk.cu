@@ -32,9 +32,9 @@
  *
  * What bounds the walk is the chain of one chunk: three rounds of MMAs, each
  * waiting for the epilogue of the one before. Measured with 8 heads of 256 x
- * 256: 4096 tokens 158 us (2500 token by token), of which the first kernel
- * takes 24 and a chunk of the second 3900 cycles; 24 prompts of up to 2047
- * tokens 622 us.
+ * 256: 4096 tokens 171 us (2500 token by token), of which the first kernel
+ * takes 27 and a chunk of the second 4100 cycles; 24 prompts of up to 2047
+ * tokens 626 us.
  */
 #include "gdn_ops.h"
 
@@ -336,9 +336,9 @@ __device__ __forceinline__ void place_sequences(const DeltaParams &p, uint32_t *
  * the four of 16 on the diagonal by substitution, a warp each and a lane per
  * row; the products, and P T, with mma.sync of TF32 parts (x = x0 + x1 + x2, six
  * of the nine products: 24 bits of each; with x0 + x1 and three products, 21
- * bits, the states of like keys were 1.4e-6 off). What bounds it is the chain of these
- * steps, 17000 cycles, against which three CTAs share an SM: 24 us for 64
- * chunks of 8 heads of 256. */
+ * bits, the states of like keys were 1.4e-6 off). What bounds it is the chain
+ * of these steps, 15000 cycles alone and 22000 where three CTAs share an SM to
+ * fill its gaps: 27 us for 64 chunks of 8 heads of 256. */
 constexpr int kPrepThreads = 256;
 constexpr uint32_t kLdA = kC + 8, kLdP = kC + 4; /* row strides of A, T and X, and of P: fragments without bank conflicts */
 

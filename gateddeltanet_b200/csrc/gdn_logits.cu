@@ -41,7 +41,8 @@ namespace cg = cooperative_groups;
 
 constexpr uint32_t kThreads = 256;
 /* 16-byte vectors of a thread in flight: with four, four CTAs share an SM, with
- * two, five (256 rows of 131072 BF16 68 and 65 us) */
+ * two, five (256 rows of 131072 BF16 68 and 65 us, although 48 registers a thread
+ * make it spill: 8 bytes in the aligned BF16 form, up to 28 in the others) */
 constexpr int kUnroll = 2;
 constexpr int kHistoryUnroll = 8;
 constexpr int kMaxCluster = 8;  /* portable cluster size */
