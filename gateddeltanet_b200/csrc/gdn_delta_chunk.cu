@@ -190,7 +190,7 @@ __device__ __forceinline__ void add_to(const float (&x)[8], float (&y)[8]) {
 #pragma unroll
     for (int i = 0; i < 8; i += 2) unpack2(add2(pack2(x[i], x[i + 1]), pack2(y[i], y[i + 1])), y[i], y[i + 1]);
 }
-/* by a product with zeros, in three steps of packed operations */
+/* whether all are finite: by a product with zeros, in three steps of packed operations */
 __device__ __forceinline__ bool all_finite(const float (&x)[8]) {
     const uint64_t none = pack2(0.0f, 0.0f);
     const uint64_t a = fma2(pack2(x[0], x[1]), none, fma2(pack2(x[2], x[3]), none, none));
@@ -847,7 +847,8 @@ __global__ void __launch_bounds__(Scan<K, VB>::kThreads, 1)
     const uint32_t bar = base + L::kBar;
     const uint32_t full_kq = bar, empty_k = bar + 16, empty_q = bar + 32, full_pair = bar + 40, empty_pair = bar + 48,
                    s_ready = bar + 56, d1_full = bar + 72, r_ready = bar + 80, d3_full = bar + 88, d_ready = bar + 96,
-                   d4_full = bar + 104, drain = bar + 120, full_scal = bar + 128, empty_scal = bar + 160, o_full = L::kSplit ? bar + 184 : d_ready, full_third = bar + 192;
+                   d4_full = bar + 104, drain = bar + 120, full_scal = bar + 128, empty_scal = bar + 160,
+                   o_full = L::kSplit ? bar + 184 : d_ready, full_third = bar + 192;
     uint32_t *slot = reinterpret_cast<uint32_t *>(sm + L::kBar + 144);
     volatile uint32_t *abort = reinterpret_cast<volatile uint32_t *>(sm + L::kBar + 152);
     volatile uint32_t *any_bad = reinterpret_cast<volatile uint32_t *>(sm + L::kBar + 176);
