@@ -170,12 +170,16 @@ EXPORTS = [
      [ctypes.POINTER(GDNRunState), ctypes.POINTER(ctypes.c_float), ctypes.c_size_t, ctypes.POINTER(ctypes.c_float),
       ctypes.c_size_t, ctypes.POINTER(ctypes.c_int32), ctypes.POINTER(ctypes.c_int32),
       ctypes.POINTER(ctypes.c_int32)]),
-    # GdnB200DeltaArgs / GdnB200LogitsArgs as packed bytes (ops.py)
+    # the serving operators' argument structs as packed bytes (ops.py)
     ("gdn_b200_delta_step", ctypes.c_int, [ctypes.c_char_p]),
     ("gdn_b200_delta_chunk", ctypes.c_int, [ctypes.c_char_p]),
     ("gdn_b200_delta_chunk_workspace", ctypes.c_size_t, [ctypes.c_uint32, ctypes.c_uint32, ctypes.c_uint32]),
     ("gdn_b200_delta_status", ctypes.c_int, [ctypes.c_int]),
     ("gdn_b200_constrain_logits", ctypes.c_int, [ctypes.c_char_p]),
+    ("gdn_b200_rms_norm", ctypes.c_int, [ctypes.c_char_p]),
+    ("gdn_b200_linear", ctypes.c_int, [ctypes.c_char_p]),
+    ("gdn_b200_linear_status", ctypes.c_int, [ctypes.c_int]),
+    ("gdn_b200_short_conv", ctypes.c_int, [ctypes.c_char_p]),
     ("gdn_b200_test_drop_copy", ctypes.c_int, [ctypes.c_uint32]),
 ]
 

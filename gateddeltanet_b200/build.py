@@ -21,8 +21,8 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libgdn_b200.so")
 SOURCES = ["gdn_decode.cu", "gdn_recurrence.cu", "gdn_batch.cu", "gdn_score.cu", "gdn_host.cu", "gdn_batch_host.cu",
            "gdn_abi_host.cpp", "gdn_delta.cu", "gdn_delta_chunk.cu",
-           "gdn_logits.cu", "gdn_ops_host.cu"]
-HEADERS = ["gdn_engine.h", "gdn_batch.h", "gdn_synth.h", "gdn_math.h", "gdn_ops.h", "exports.map"]
+           "gdn_logits.cu", "gdn_norm.cu", "gdn_conv.cu", "gdn_linear.cu", "gdn_linear_few.cu", "gdn_ops_host.cu"]
+HEADERS = ["gdn_engine.h", "gdn_batch.h", "gdn_synth.h", "gdn_math.h", "gdn_ops.h", "gdn_values.h", "gdn_linear.h", "exports.map"]
 TORCH_LIB = os.path.join(HERE, "_ops_torch.so")  # the Python binding of the serving operators (ops.py)
 TORCH_SOURCE = "gdn_ops_torch.cpp"
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]

@@ -1,0 +1,187 @@
+/* gdn_linear_few.cu -- y = act(sx sw x W^T + bias) + residual for up to 16
+ * tokens (gdn_linear.cu takes more).
+ *
+ * Bound by reading W once. A warp multiplies 16 rows of W with 8 (or 16)
+ * tokens by m16n8k16 MMAs whose operands come straight from memory: in a
+ * fragment, lane (g, t) = (lane / 4, lane % 4) holds values of row g of W and of token
+ * g at four places of k. Which k stand there is free as long as both operands
+ * agree, so each lane loads 16 bytes, neighbours in k, of rows g and g + 8 and
+ * of token g, and feeds them to two MMAs (8-bit values, exact in FP16, to
+ * four). Nothing passes through shared memory but the sums: the warps of a CTA
+ * share its rows and divide k between them, and their partial sums are added in
+ * the order of the warps.
+ */
+#include "gdn_linear.h"
+
+namespace gdn {
+namespace ops {
+
+namespace {
+
+constexpr uint32_t kMaxWarps = 16;
+constexpr int kAhead = 4; /* steps of k whose loads are in flight */
+
+__device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+/* two values of 8 bits as two of 16 */
+__device__ __forceinline__ uint32_t widen(uint32_t two) {
+    uint32_t r;
+    asm("{\n .reg .b16 h;\n cvt.u16.u32 h, %1;\n cvt.rn.f16x2.e4m3x2 %0, h;\n}\n" : "=r"(r) : "r"(two));
+    return r;
+}
+
+/* 16 bytes of row g, of row g + 8 and of a token: their products */
+template <bool kFp8, int kGroups>
+__device__ __forceinline__ void products(float (&d)[kGroups][4], const uint4 &lo, const uint4 &hi, const uint4 (&b)[kGroups]) {
+    const uint32_t l[4] = {lo.x, lo.y, lo.z, lo.w}, h[4] = {hi.x, hi.y, hi.z, hi.w};
+    if constexpr (kFp8) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t a0 = widen(l[i] & 0xFFFFu), a1 = widen(h[i] & 0xFFFFu), a2 = widen(l[i] >> 16), a3 = widen(h[i] >> 16);
+#pragma unroll
+            for (int n = 0; n < kGroups; ++n) {
+                const uint32_t w = i == 0 ? b[n].x : i == 1 ? b[n].y : i == 2 ? b[n].z : b[n].w;
+                mma_f16(d[n], a0, a1, a2, a3, widen(w & 0xFFFFu), widen(w >> 16));
+            }
+        }
+    } else {
+#pragma unroll
+        for (int n = 0; n < kGroups; ++n) {
+            mma_bf16(d[n], l[0], h[0], l[1], h[1], b[n].x, b[n].y);
+            mma_bf16(d[n], l[2], h[2], l[3], h[3], b[n].z, b[n].w);
+        }
+    }
+}
+
+/* 16 bytes at byte k of a row of `size` bytes: zeros past its end. The rows
+ * themselves are whole 16-byte pieces apart, so the last piece is read whole
+ * where it is not the row's own end that cuts it. */
+template <bool kFp8>
+__device__ __forceinline__ uint4 piece(const uint8_t *row, uint32_t k, uint32_t size, bool have) {
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (!have || k >= size) return v;
+    if (k + 16 <= size) return __ldcs(reinterpret_cast<const uint4 *>(row + k));
+    uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < 16; i += kFp8 ? 1 : 2)
+        if (k + i < size) {
+            const uint32_t e = kFp8 ? (uint32_t)row[k + i] : (uint32_t)*reinterpret_cast<const unsigned short *>(row + k + i);
+            w[i / 4] |= e << (8 * (i % 4));
+        }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+/* kGroups: tokens / 8. kPairs (swiglu): a CTA takes 16 rows of either half of W. */
+template <bool kFp8, int kGroups, bool kPairs>
+__global__ void __launch_bounds__(kMaxWarps * 32) linear_few_kernel(const __grid_constant__ LinearParams p) {
+    constexpr int kHalves = kPairs ? 2 : 1;
+    constexpr uint32_t kSums = kHalves * kGroups * 128; /* of a warp */
+    extern __shared__ float sums[];
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, warps = blockDim.x >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const uint32_t n0 = blockIdx.x * 16, size = p.inputs * (kFp8 ? 1 : 2);
+    const uint32_t elem = kFp8 ? 1 : 2;
+    const uint8_t *w[kHalves][2];
+    bool have_w[2], have_x[kGroups];
+    const uint8_t *x[kGroups];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+        have_w[r] = n0 + g + 8 * r < p.outputs;
+#pragma unroll
+        for (int h = 0; h < kHalves; ++h)
+            w[h][r] = static_cast<const uint8_t *>(p.weight) + (int64_t)(have_w[r] ? h * p.outputs + n0 + g + 8 * r : 0) * p.weight_row * elem;
+    }
+#pragma unroll
+    for (int n = 0; n < kGroups; ++n) {
+        have_x[n] = g + 8 * n < p.tokens;
+        x[n] = static_cast<const uint8_t *>(p.x) + (int64_t)(have_x[n] ? g + 8 * n : 0) * p.x_row * elem;
+    }
+    float d[kHalves][kGroups][4];
+#pragma unroll
+    for (int h = 0; h < kHalves; ++h)
+#pragma unroll
+        for (int n = 0; n < kGroups; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) d[h][n][i] = 0.0f;
+
+    /* steps of 64 bytes of k, kAhead neighbours at a time to a warp */
+    const uint32_t stride = warps * kAhead * 64;
+    for (uint32_t k0 = warp * kAhead * 64; k0 < size; k0 += stride) {
+        uint4 a[kAhead][kHalves][2], b[kAhead][kGroups];
+#pragma unroll
+        for (int s = 0; s < kAhead; ++s) {
+            const uint32_t k = k0 + s * 64 + t * 16;
+#pragma unroll
+            for (int h = 0; h < kHalves; ++h)
+#pragma unroll
+                for (int r = 0; r < 2; ++r) a[s][h][r] = piece<kFp8>(w[h][r], k, size, have_w[r]);
+#pragma unroll
+            for (int n = 0; n < kGroups; ++n) b[s][n] = piece<kFp8>(x[n], k, size, have_x[n]);
+        }
+#pragma unroll
+        for (int s = 0; s < kAhead; ++s)
+#pragma unroll
+            for (int h = 0; h < kHalves; ++h) products<kFp8, kGroups>(d[h], a[s][h][0], a[s][h][1], b[s]);
+    }
+    /* the warps' sums: [warp][half][token][16 rows] */
+#pragma unroll
+    for (int h = 0; h < kHalves; ++h)
+#pragma unroll
+        for (int n = 0; n < kGroups; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                sums[warp * kSums + (h * kGroups * 8 + n * 8 + t * 2 + (i & 1)) * 16 + g + 8 * (i >> 1)] = d[h][n][i];
+    __syncthreads();
+    for (uint32_t i = tid; i < kGroups * 128; i += blockDim.x) {
+        const uint32_t token = i / 16, n = n0 + i % 16;
+        if (token >= p.tokens || n >= p.outputs) continue;
+        float v[2] = {0.0f, 0.0f};
+        for (uint32_t q = 0; q < warps; ++q)
+#pragma unroll
+            for (int h = 0; h < kHalves; ++h) v[h] += sums[q * kSums + h * kGroups * 128 + i];
+#pragma unroll
+        for (int h = 0; h < kHalves; ++h) {
+            const uint32_t row = h * p.outputs + n;
+            if (kFp8) v[h] *= p.x_scales[token] * p.weight_scales[row];
+            if (p.bias != nullptr) v[h] += load1(p.bias, row, p.bias_type);
+        }
+        float y = activate(p.activation, v[0], v[1]);
+        if (p.residual != nullptr) y += load1(p.residual, token * p.residual_row + n, p.residual_type);
+        store1(p.out, token * p.out_row + n, p.out_type, y);
+    }
+}
+
+template <bool kFp8, int kGroups, bool kPairs>
+cudaError_t launch_few_t(const LinearParams &p, int sms, cudaStream_t stream) {
+    const uint32_t ctas = (p.outputs + 15) / 16;
+    /* warps enough for about 16 an SM, as far as k goes round */
+    uint32_t warps = 4;
+    const uint32_t steps = (p.inputs * (kFp8 ? 1 : 2) + kAhead * 64 - 1) / (kAhead * 64);
+    while (warps < kMaxWarps && ctas * warps < 16u * (uint32_t)sms && warps < steps) warps *= 2;
+    const size_t smem = (size_t)warps * (kPairs ? 2 : 1) * kGroups * 128 * sizeof(float);
+    return launch(linear_few_kernel<kFp8, kGroups, kPairs>, dim3(ctas), warps * 32, smem, stream, p);
+}
+
+template <bool kFp8>
+cudaError_t launch_few_x(const LinearParams &p, int sms, cudaStream_t stream) {
+    const bool two = p.tokens > 8;
+    if (p.activation == kSwiglu)
+        return two ? launch_few_t<kFp8, 2, true>(p, sms, stream) : launch_few_t<kFp8, 1, true>(p, sms, stream);
+    return two ? launch_few_t<kFp8, 2, false>(p, sms, stream) : launch_few_t<kFp8, 1, false>(p, sms, stream);
+}
+
+}  // namespace
+
+cudaError_t launch_linear_few(const LinearParams &p, int sms, cudaStream_t stream) {
+    return p.type == kE4M3 ? launch_few_x<true>(p, sms, stream) : launch_few_x<false>(p, sms, stream);
+}
+
+}  // namespace ops
+}  // namespace gdn

@@ -1,8 +1,9 @@
 /* Internal interface between the C entries of the serving operators
  * (gdn_ops_host.cu) and their kernels: the gated delta rule over pooled
- * states (gdn_delta.cu) and the constraints on logits (gdn_logits.cu). Device
- * pointers throughout; strides count elements. Not installed; callers use
- * include/gdn_b200.h. */
+ * states (gdn_delta.cu, gdn_delta_chunk.cu), the constraints on logits
+ * (gdn_logits.cu), norms (gdn_norm.cu), the short convolution (gdn_conv.cu) and
+ * projections (gdn_linear.cu, gdn_linear_few.cu). Device pointers throughout;
+ * strides count elements. Not installed; callers use include/gdn_b200.h. */
 #ifndef GDN_OPS_H
 #define GDN_OPS_H
 
@@ -84,6 +85,58 @@ constexpr uint32_t kMaxHistory = (1u << 20) - 1;
 constexpr uint32_t kMaxBiases = 2047;  /* searched once for each biased token */
 constexpr uint32_t kMaxVocab = 1u << 18;
 
+/* Codes of element types, as in include/gdn_b200.h. */
+enum Type : int { kF32 = 0, kBF16 = 1, kE4M3 = 2 };
+
+/* Rows of heads x dim; what is absent is null. */
+struct NormParams {
+    const void *x, *gate, *weight;
+    void *residual, *out;
+    float *scales;
+    int64_t x_token, x_head, gate_token, gate_head, residual_token, residual_head, out_token, out_head;
+    uint32_t tokens, heads, dim;
+    int type, weight_type, residual_type, out_type;
+    float eps;
+};
+constexpr uint32_t kMaxNormThreads = 1024;
+/* Threads of a row of dim values, `each` to a thread: a power of two up to 32, or a multiple of 32. */
+inline uint32_t norm_group(uint32_t dim, uint32_t each) {
+    const uint32_t need = dim / each + (dim % each != 0);
+    if (need > 32) return (need + 31) / 32 * 32;
+    uint32_t group = 1;
+    while (group < need) group *= 2;
+    return group;
+}
+/* Threads that have to be in one CTA: a row's, or those of all heads of a token with one scale. */
+inline uint64_t norm_threads(const NormParams &p, uint32_t each) {
+    return (uint64_t)norm_group(p.dim, each) * (p.out_type == 2 ? p.heads : 1);
+}
+
+/* Packed tokens of N sequences, as in DeltaParams. */
+struct ConvParams {
+    const void *x, *weight, *bias;
+    void *tails, *out;
+    const int32_t *starts, *slots;
+    const uint8_t *fresh;
+    int64_t x_token, out_token, tails_slot, tails_row;
+    uint32_t N, tokens, channels, width, tail_slots;
+    int type, weight_type, tail_type, silu;
+};
+
+enum Activation : int { kNoActivation = 0, kSilu = 1, kGelu = 2, kSwiglu = 3 };
+
+/* y = act(sx sw x W^T + bias) + residual; W has 2 x outputs rows for kSwiglu. */
+struct LinearParams {
+    const void *x, *weight, *bias, *residual;
+    const float *x_scales, *weight_scales;
+    void *out;
+    int64_t x_row, weight_row, residual_row, out_row;
+    uint32_t tokens, inputs, outputs;
+    int type, bias_type, residual_type, out_type, activation;
+    uint32_t drop; /* for tests, 0: none. 1 + the k-block whose copy the first CTA does not make */
+};
+constexpr uint32_t kFewTokens = 16; /* up to here gdn_linear_few.cu, above gdn_linear.cu */
+
 /* kernel<<<grid, block, smem, stream>>>(args...) and this launch's own result:
  * cudaGetLastError would also give that of a call before it. */
 template <typename... Params, typename... Args>
@@ -105,6 +158,11 @@ cudaError_t launch_delta_chunk(const DeltaParams &p, void *workspace, int sms, c
 cudaError_t delta_step_status(int *status);
 cudaError_t delta_chunk_status(int *status);
 cudaError_t launch_logits(LogitsParams p, bool bf16, int sms, cudaStream_t stream);
+cudaError_t launch_norm(const NormParams &p, int sms, cudaStream_t stream);
+cudaError_t launch_conv(const ConvParams &p, int sms, cudaStream_t stream);
+cudaError_t launch_linear(const LinearParams &p, int sms, cudaStream_t stream);
+cudaError_t launch_linear_few(const LinearParams &p, int sms, cudaStream_t stream);
+cudaError_t linear_status(int *status);
 
 }  // namespace ops
 }  // namespace gdn

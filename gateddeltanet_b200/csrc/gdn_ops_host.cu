@@ -5,6 +5,7 @@
 #include "gdn_ops.h"
 
 #include <atomic>
+#include <initializer_list>
 #include <stdarg.h>
 #include <stdio.h>
 
@@ -122,6 +123,33 @@ int delta_params(const char *who, const GdnB200DeltaArgs *a, gdn::ops::DeltaPara
     return 0;
 }
 
+bool float_type(int t) { return t == 0 || t == 1; }
+int64_t size_of(int type) { return type == 0 ? 4 : type == 1 ? 2 : 1; }
+
+/* The memory of a tensor [tokens][heads][dim], by token: from `at` on, `width`
+ * bytes (with the gaps between its heads) every `row` bytes. */
+struct Extent {
+    const void *at;
+    int64_t row, width, rows;
+    Extent(const void *p, int64_t token, int64_t head, uint32_t tokens, uint32_t heads, uint32_t dim, int64_t size)
+        : at(p), row(token * size), width((((int64_t)heads - 1) * head + dim) * size), rows(tokens) {
+        if (rows > 1 && row < width) { /* heads further apart than tokens: taken as one block */
+            width += (rows - 1) * row;
+            rows = 1;
+        }
+    }
+    bool same(const Extent &e) const { return at == e.at && (rows == 1 || row == e.row) && width == e.width && rows == e.rows; }
+    bool meets(const Extent &e) const {
+        if (at == nullptr || e.at == nullptr || width <= 0 || e.width <= 0) return false;
+        if (width == e.width && rows == e.rows) return same(e) || partly_shared(at, row, e.at, e.row, rows, width);
+        const int64_t d = (int64_t)(reinterpret_cast<uintptr_t>(e.at) - reinterpret_cast<uintptr_t>(at));
+        if (d >= (rows - 1) * row + width || -d >= (e.rows - 1) * e.row + e.width) return false;
+        if (rows != e.rows || rows == 1 || row != e.row || row < width || row < e.width) return true;
+        const int64_t shift = (d % row + row) % row; /* of e's rows against these */
+        return shift < width || shift + e.width > row;
+    }
+};
+
 }  // namespace
 
 extern "C" {
@@ -205,6 +233,136 @@ int gdn_b200_constrain_logits(const GdnB200LogitsArgs *args) {
     return on_device(who, a.device, [&](int sms) {
         return gdn::ops::launch_logits(p, a.dtype == 1, sms, static_cast<cudaStream_t>(a.stream));
     });
+}
+
+int gdn_b200_rms_norm(const GdnB200NormArgs *args) {
+    const char *who = "gdn_b200_rms_norm";
+    if (args == nullptr) return failf("%s: no arguments", who);
+    const GdnB200NormArgs &a = *args;
+    if (!float_type(a.dtype)) return failf("%s: dtype %d is neither FP32 (0) nor BF16 (1)", who, a.dtype);
+    if (a.weight != nullptr && !float_type(a.weight_dtype)) return failf("%s: weight_dtype %d is neither FP32 (0) nor BF16 (1)", who, a.weight_dtype);
+    if (a.residual != nullptr && !float_type(a.residual_dtype))
+        return failf("%s: residual_dtype %d is neither FP32 (0) nor BF16 (1)", who, a.residual_dtype);
+    if (!float_type(a.out_dtype) && a.out_dtype != 2) return failf("%s: out_dtype %d is not FP32 (0), BF16 (1) or E4M3 (2)", who, a.out_dtype);
+    if (a.tokens == 0 || a.heads == 0) return 0;
+    if (a.dim == 0) return failf("%s: rows of no values", who);
+    if ((uint64_t)a.tokens * a.heads > 0x7fffffffu) return failf("%s: %u tokens of %u heads are too many", who, a.tokens, a.heads);
+    if (!(a.eps >= 0.0f)) return failf("%s: eps is negative or not a number", who);
+    if (a.x == nullptr || a.out == nullptr) return failf("%s: x or out is missing", who);
+    if (a.out_dtype == 2 && a.scales == nullptr) return failf("%s: scales is missing", who);
+    for (int64_t stride : {a.x_token, a.x_head, a.gate_token, a.gate_head, a.residual_token, a.residual_head, a.out_token, a.out_head})
+        if (stride < 0) return failf("%s: negative stride", who);
+    const int64_t size = size_of(a.dtype), out_size = size_of(a.out_dtype), res_size = size_of(a.residual_dtype);
+    if (!aligned(a.x, size) || !aligned(a.gate, size) || !aligned(a.out, out_size) || (a.residual != nullptr && !aligned(a.residual, res_size)) ||
+        (a.weight != nullptr && !aligned(a.weight, size_of(a.weight_dtype))) || (a.out_dtype == 2 && !aligned(a.scales, 4)))
+        return failf("%s: a tensor is misaligned for its type", who);
+    gdn::ops::NormParams p{a.x, a.gate, a.weight, a.residual, a.out, a.scales, a.x_token, a.x_head, a.gate_token, a.gate_head,
+                           a.residual_token, a.residual_head, a.out_token, a.out_head, a.tokens, a.heads, a.dim,
+                           a.dtype, a.weight_dtype, a.residual_dtype, a.out_dtype, a.eps};
+    if (gdn::ops::norm_threads(p, 16) > gdn::ops::kMaxNormThreads)
+        return failf("%s: rows of %u x %u values are more than one CTA holds", who, a.heads, a.dim);
+    const Extent x(a.x, a.x_token, a.x_head, a.tokens, a.heads, a.dim, size), out(a.out, a.out_token, a.out_head, a.tokens, a.heads, a.dim, out_size),
+        gate(a.gate, a.gate_token, a.gate_head, a.tokens, a.heads, a.dim, size),
+        residual(a.residual, a.residual_token, a.residual_head, a.tokens, a.heads, a.dim, res_size),
+        weight(a.weight, 0, 0, 1, 1, a.dim, size_of(a.weight_dtype)), scales(a.out_dtype == 2 ? a.scales : nullptr, 0, 0, 1, 1, a.tokens, 4);
+    const bool in_place = a.x == a.out && a.dtype == a.out_dtype && (a.tokens == 1 || a.x_token == a.out_token) &&
+                          (a.heads == 1 || a.x_head == a.out_head);
+    if (out.meets(gate) || out.meets(residual) || out.meets(weight) || (!in_place && out.meets(x)))
+        return failf("%s: out overlaps another tensor", who);
+    if (residual.meets(x) || residual.meets(gate) || residual.meets(weight)) return failf("%s: the residual overlaps another tensor", who);
+    for (const Extent *e : {&x, &out, &gate, &residual, &weight})
+        if (scales.meets(*e)) return failf("%s: scales overlaps another tensor", who);
+    return on_device(who, a.device, [&](int sms) { return gdn::ops::launch_norm(p, sms, static_cast<cudaStream_t>(a.stream)); });
+}
+
+int gdn_b200_linear(const GdnB200LinearArgs *args) {
+    const char *who = "gdn_b200_linear";
+    if (args == nullptr) return failf("%s: no arguments", who);
+    const GdnB200LinearArgs &a = *args;
+    if (a.dtype != 1 && a.dtype != 2) return failf("%s: dtype %d is neither BF16 (1) nor E4M3 (2)", who, a.dtype);
+    if (a.bias != nullptr && !float_type(a.bias_dtype)) return failf("%s: bias_dtype %d is neither FP32 (0) nor BF16 (1)", who, a.bias_dtype);
+    if (a.residual != nullptr && !float_type(a.residual_dtype))
+        return failf("%s: residual_dtype %d is neither FP32 (0) nor BF16 (1)", who, a.residual_dtype);
+    if (!float_type(a.out_dtype)) return failf("%s: out_dtype %d is neither FP32 (0) nor BF16 (1)", who, a.out_dtype);
+    if (a.activation < 0 || a.activation > 3) return failf("%s: activation %d is not 0 to 3", who, a.activation);
+    if (a.tokens == 0 || a.outputs == 0) return 0;
+    if (a.inputs == 0) return failf("%s: no inputs", who);
+    if (a.tokens > 1u << 24 || a.outputs > 1u << 24 || a.inputs > 1u << 24 || (uint64_t)a.tokens * a.outputs > 1ull << 38)
+        return failf("%s: %u x %u x %u is too large", who, a.tokens, a.outputs, a.inputs);
+    if (a.x == nullptr || a.weight == nullptr || a.out == nullptr) return failf("%s: x, weight or out is missing", who);
+    if (a.dtype == 2 && (a.x_scales == nullptr || a.weight_scales == nullptr)) return failf("%s: 8-bit operands need scales", who);
+    const int64_t size = size_of(a.dtype), out_size = size_of(a.out_dtype), res_size = size_of(a.residual_dtype);
+    const uint32_t rows = a.activation == 3 ? 2 * a.outputs : a.outputs;
+    if (!aligned(a.x, 16) || !aligned(a.weight, 16) || (a.tokens > 1 && a.x_row * size % 16 != 0) || (rows > 1 && a.weight_row * size % 16 != 0))
+        return failf("%s: rows of x and weight must start on 16-byte boundaries", who);
+    if ((a.tokens > 1 && a.x_row < (int64_t)a.inputs) || (rows > 1 && a.weight_row < (int64_t)a.inputs)) return failf("%s: rows of x or weight overlap", who);
+    if (a.tokens > 1 && a.out_row < (int64_t)a.outputs) return failf("%s: rows of out overlap", who);
+    if (a.residual != nullptr && a.tokens > 1 && a.residual_row < 0) return failf("%s: negative stride", who);
+    if (a.x_row > 1ll << 36 || a.weight_row > 1ll << 36) return failf("%s: rows of x or weight are too far apart", who);
+    if (!aligned(a.out, out_size) || (a.residual != nullptr && !aligned(a.residual, res_size)) || (a.bias != nullptr && !aligned(a.bias, size_of(a.bias_dtype))))
+        return failf("%s: a tensor is misaligned for its type", who);
+    const Extent out(a.out, a.out_row, 0, a.tokens, 1, a.outputs, out_size), x(a.x, a.x_row, 0, a.tokens, 1, a.inputs, size),
+        weight(a.weight, a.weight_row, 0, rows, 1, a.inputs, size), residual(a.residual, a.residual_row, 0, a.tokens, 1, a.outputs, res_size),
+        bias(a.bias, 0, 0, 1, 1, rows, size_of(a.bias_dtype)), x_scales(a.dtype == 2 ? a.x_scales : nullptr, 0, 0, 1, 1, a.tokens, 4),
+        weight_scales(a.dtype == 2 ? a.weight_scales : nullptr, 0, 0, 1, 1, rows, 4);
+    const bool in_place = a.residual == a.out && a.residual_dtype == a.out_dtype && (a.tokens == 1 || a.residual_row == a.out_row);
+    if (out.meets(x) || out.meets(weight) || out.meets(bias) || out.meets(x_scales) || out.meets(weight_scales) || (!in_place && out.meets(residual)))
+        return failf("%s: out overlaps an input", who);
+    const gdn::ops::LinearParams p{a.x, a.weight, a.bias, a.residual, a.x_scales, a.weight_scales, a.out, a.x_row, a.weight_row,
+                                   a.residual_row, a.out_row, a.tokens, a.inputs, a.outputs, a.dtype, a.bias_dtype,
+                                   a.residual_dtype, a.out_dtype, a.activation, g_drop.exchange(0)};
+    return on_device(who, a.device, [&](int sms) {
+        auto *launch = a.tokens <= gdn::ops::kFewTokens ? gdn::ops::launch_linear_few : gdn::ops::launch_linear;
+        return launch(p, sms, static_cast<cudaStream_t>(a.stream));
+    });
+}
+
+int gdn_b200_linear_status(int device) {
+    DeviceScope scope(device);
+    int status = 0;
+    cudaError_t e = scope.error;
+    if (e == cudaSuccess) e = cudaDeviceSynchronize(); /* the copy below waits for no stream but its own */
+    if (e == cudaSuccess) e = gdn::ops::linear_status(&status);
+    if (e != cudaSuccess) return cuda_failf("gdn_b200_linear_status", "cannot read the device", e);
+    return status == 0 ? 0 : failf("gdn_b200_linear: a wait on the device ran out; the call's outputs are not valid");
+}
+
+int gdn_b200_short_conv(const GdnB200ConvArgs *args) {
+    const char *who = "gdn_b200_short_conv";
+    if (args == nullptr) return failf("%s: no arguments", who);
+    const GdnB200ConvArgs &a = *args;
+    if (!float_type(a.dtype)) return failf("%s: dtype %d is neither FP32 (0) nor BF16 (1)", who, a.dtype);
+    if (!float_type(a.weight_dtype)) return failf("%s: weight_dtype %d is neither FP32 (0) nor BF16 (1)", who, a.weight_dtype);
+    if (a.tail_dtype != 0 && a.tail_dtype != a.dtype) return failf("%s: tail_dtype %d is neither FP32 (0) nor that of x", who, a.tail_dtype);
+    if (a.activation != 0 && a.activation != 1) return failf("%s: activation %d is not 0 or 1", who, a.activation);
+    if (a.width < 2 || a.width > 4) return failf("%s: width %u is not 2, 3 or 4", who, a.width);
+    if (a.tokens > 0x3fffffffu || a.sequences > 0x3fffffu) return failf("%s: %u tokens in %u sequences are too many", who, a.tokens, a.sequences);
+    if (a.channels > 1u << 22) return failf("%s: %u channels are too many", who, a.channels);
+    if (a.starts == nullptr && a.tokens != a.sequences)
+        return failf("%s: without starts every sequence has one token (%u tokens, %u sequences)", who, a.tokens, a.sequences);
+    if (a.sequences == 0 && a.tokens != 0) return failf("%s: %u tokens but no sequence", who, a.tokens);
+    if (a.sequences == 0 || a.channels == 0) return 0;
+    if (a.slots == nullptr && a.tail_slots < a.sequences) return failf("%s: %u slots for %u sequences", who, a.tail_slots, a.sequences);
+    if (a.weight == nullptr || (a.tails == nullptr && a.tail_slots != 0)) return failf("%s: weight or tails is missing", who);
+    if (a.tokens != 0 && (a.x == nullptr || a.out == nullptr)) return failf("%s: x or out is missing", who);
+    if (a.x_token < 0) return failf("%s: negative stride", who);
+    if (a.tokens > 1 && a.out_token < (int64_t)a.channels) return failf("%s: rows of out overlap", who);
+    if ((a.width > 2 && a.tails_row < (int64_t)a.channels) ||
+        (a.tail_slots > 1 && a.tails_slot < (a.width > 2 ? ((int64_t)a.width - 2) * a.tails_row : 0) + (int64_t)a.channels))
+        return failf("%s: rows or slots of tails overlap", who);
+    const int64_t size = size_of(a.dtype), tail_size = size_of(a.tail_dtype), weight_size = size_of(a.weight_dtype);
+    if (!aligned(a.x, size) || !aligned(a.out, size) || !aligned(a.tails, tail_size) || !aligned(a.weight, weight_size) || !aligned(a.bias, weight_size))
+        return failf("%s: a tensor is misaligned for its type", who);
+    const Extent x(a.x, a.x_token, 0, a.tokens, 1, a.channels, size), out(a.out, a.out_token, 0, a.tokens, 1, a.channels, size),
+        tails(a.tails, a.tails_slot, a.tails_row, a.tail_slots, a.width - 1, a.channels, tail_size),
+        weight(a.weight, 0, 0, 1, 1, a.channels * a.width, weight_size), bias(a.bias, 0, 0, 1, 1, a.channels, weight_size);
+    if (a.tokens != 0 && (out.meets(x) || out.meets(weight) || out.meets(bias))) return failf("%s: out overlaps an input", who);
+    if (a.tail_slots != 0 && (tails.meets(weight) || tails.meets(bias) || (a.tokens != 0 && (tails.meets(x) || tails.meets(out)))))
+        return failf("%s: tails overlaps another tensor", who);
+    const gdn::ops::ConvParams p{a.x, a.weight, a.bias, a.tails, a.out, a.starts, a.slots, a.fresh, a.x_token, a.out_token, a.tails_slot,
+                                 a.tails_row, a.sequences, a.tokens, a.channels, a.width, a.tail_slots, a.dtype, a.weight_dtype,
+                                 a.tail_dtype, a.activation};
+    return on_device(who, a.device, [&](int sms) { return gdn::ops::launch_conv(p, sms, static_cast<cudaStream_t>(a.stream)); });
 }
 
 }  // extern "C"

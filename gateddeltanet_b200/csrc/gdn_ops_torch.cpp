@@ -12,6 +12,7 @@
 #include <ATen/ops/empty.h>
 #include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -32,6 +33,9 @@ struct Entries {
     int (*chunk)(const GdnB200DeltaArgs *);
     size_t (*chunk_workspace)(uint32_t, uint32_t, uint32_t);
     int (*logits)(const GdnB200LogitsArgs *);
+    int (*norm)(const GdnB200NormArgs *);
+    int (*linear)(const GdnB200LinearArgs *);
+    int (*conv)(const GdnB200ConvArgs *);
     const char *(*last_error)(void);
 } g_entry;
 
@@ -378,15 +382,316 @@ PyObject *constrain_logits(PyObject *, PyObject *const *args, Py_ssize_t nargs) 
     });
 }
 
-/* bind(step, chunk, chunk_workspace, logits, last_error): addresses of the C entries */
+/* the code of a result's type: that of `out`, else `dtype`'s, else `standard` */
+int result_type(const char *who, PyObject *dtype, const Arg &out, at::ScalarType standard, bool eight_bits, at::ScalarType &type) {
+    type = out ? out.t->scalar_type() : standard;
+    if (dtype != Py_None) {
+        if (!THPDtype_Check(dtype)) refuse("%s: dtype is not a torch.dtype", who);
+        type = reinterpret_cast<THPDtype *>(dtype)->scalar_type;
+        if (out) out.type(type);
+    }
+    switch (type) {
+        case at::kFloat: return 0;
+        case at::kBFloat16: return 1;
+        case at::kFloat8_e4m3fn:
+            if (eight_bits) return 2;
+            [[fallthrough]];
+        default: refuse("%s: results of type %s are not computed", who, c10::toString(type));
+    }
+}
+
+/* (x, weight, residual, gate, eps, dtype, out, scales) -> out, or (out, scales) in 8 bits */
+PyObject *rms_norm(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+    return guarded([&]() -> PyObject * {
+        const char *who = "rms_norm";
+        if (nargs != 8) refuse("%s: 8 arguments expected", who);
+        if (g_entry.norm == nullptr) throw Refused{PyExc_RuntimeError, "the library is not bound"};
+        const Arg x(who, "x", args[0]), weight(who, "weight", args[1]), residual(who, "residual", args[2]), gate(who, "gate", args[3]),
+            out(who, "out", args[6]), scales(who, "scales", args[7]);
+        x.present();
+        for (const Arg *a : {&x, &weight, &residual, &gate, &out, &scales}) a->no_gradient();
+        const int64_t n = x.t->dim();
+        if (n != 2) x.dims(3);
+        GdnB200NormArgs a = {};
+        a.dtype = dtype_code(x);
+        const c10::Device device = x.t->device();
+        x.on(device);
+        x.last_contiguous();
+        const int64_t tokens = x.t->size(0), heads = n == 3 ? x.t->size(1) : 1, dim = x.t->size(n - 1);
+        for (int64_t v : {tokens, heads, dim})
+            if (v > 0x7fffffff) refuse("%s: a size of %lld is too large", who, (long long)v);
+        if (weight) {
+            a.weight_dtype = dtype_code(weight);
+            weight.shape({dim});
+            weight.on(device);
+            weight.last_contiguous();
+        }
+        if (residual) {
+            a.residual_dtype = dtype_code(residual);
+            residual.shape(x.t->sizes());
+            residual.on(device);
+            residual.last_contiguous();
+            residual.disjoint();
+        }
+        if (gate) {
+            gate.type(x.t->scalar_type());
+            gate.shape(x.t->sizes());
+            gate.on(device);
+            gate.last_contiguous();
+        }
+        const double eps = PyFloat_AsDouble(args[4]);
+        if (PyErr_Occurred()) return nullptr;
+        at::ScalarType type;
+        a.out_dtype = result_type(who, args[5], out, x.t->scalar_type(), true, type);
+        at::Tensor result, factors;
+        if (out) {
+            out.shape(x.t->sizes());
+            out.on(device);
+            out.last_contiguous();
+            if (args[6] != args[0]) out.disjoint();
+            result = *out.t;
+        } else {
+            result = at::empty(x.t->sizes(), x.t->options().dtype(type).requires_grad(false));
+        }
+        if (a.out_dtype == 2) {
+            if (scales) {
+                scales.type(at::kFloat);
+                scales.shape({tokens});
+                scales.on(device);
+                scales.last_contiguous();
+                factors = *scales.t;
+            } else {
+                factors = at::empty({tokens}, x.t->options().dtype(at::kFloat).requires_grad(false));
+            }
+            a.scales = static_cast<float *>(factors.data_ptr());
+        } else if (scales) {
+            refuse("%s: scales are those of 8-bit results", who);
+        }
+        auto head = [&](const at::Tensor &t) { return n == 3 ? step(t, 1) : dim; };
+        a.x = x.ptr<const void>();
+        a.gate = gate.ptr<const void>();
+        a.weight = weight.ptr<const void>();
+        a.residual = residual.ptr<void>();
+        a.out = result.data_ptr();
+        a.stream = c10::cuda::getCurrentCUDAStream(device.index()).stream();
+        a.x_token = step(*x.t, 0), a.x_head = head(*x.t);
+        if (gate) a.gate_token = step(*gate.t, 0), a.gate_head = head(*gate.t);
+        if (residual) a.residual_token = step(*residual.t, 0), a.residual_head = head(*residual.t);
+        a.out_token = step(result, 0), a.out_head = head(result);
+        a.tokens = (uint32_t)tokens, a.heads = (uint32_t)heads, a.dim = (uint32_t)dim;
+        a.device = device.index();
+        a.eps = (float)eps;
+        called(g_entry.norm(&a));
+        residual.written();
+        out.written();
+        scales.written();
+        PyObject *first = out ? Py_NewRef(args[6]) : THPVariable_Wrap(result);
+        if (a.out_dtype != 2 || first == nullptr) return first;
+        PyObject *second = scales ? Py_NewRef(args[7]) : THPVariable_Wrap(factors);
+        PyObject *both = second == nullptr ? nullptr : PyTuple_Pack(2, first, second);
+        Py_DECREF(first);
+        Py_XDECREF(second);
+        return both;
+    });
+}
+
+/* the number of an activation's name in `names` (None: 0) */
+int activation_code(const char *who, PyObject *o, std::initializer_list<const char *> names) {
+    if (o == Py_None) return 0;
+    const char *name = PyUnicode_Check(o) ? PyUnicode_AsUTF8(o) : nullptr;
+    int code = 0;
+    std::string all;
+    for (const char *n : names) {
+        ++code;
+        if (name != nullptr && std::string(n) == name) return code;
+        all += std::string(all.empty() ? "" : ", ") + n;
+    }
+    PyErr_Clear();
+    refuse("%s: activation is neither None nor one of %s", who, all.c_str());
+}
+
+/* (x, weight, bias, activation, residual, x_scales, weight_scales, dtype, out) -> out */
+PyObject *linear(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+    return guarded([&]() -> PyObject * {
+        const char *who = "linear";
+        if (nargs != 9) refuse("%s: 9 arguments expected", who);
+        if (g_entry.linear == nullptr) throw Refused{PyExc_RuntimeError, "the library is not bound"};
+        const Arg x(who, "x", args[0]), weight(who, "weight", args[1]), bias(who, "bias", args[2]), residual(who, "residual", args[4]),
+            x_scales(who, "x_scales", args[5]), weight_scales(who, "weight_scales", args[6]), out(who, "out", args[8]);
+        x.present();
+        weight.present();
+        for (const Arg *a : {&x, &weight, &bias, &residual, &x_scales, &weight_scales, &out}) a->no_gradient();
+        GdnB200LinearArgs a = {};
+        a.activation = activation_code(who, args[3], {"silu", "gelu", "swiglu"});
+        x.dims(2);
+        weight.dims(2);
+        const bool eight = x.t->scalar_type() == at::kFloat8_e4m3fn;
+        if (!eight && x.t->scalar_type() != at::kBFloat16)
+            refuse("%s: x has type %s, neither bfloat16 nor float8_e4m3fn", who, c10::toString(x.t->scalar_type()));
+        a.dtype = eight ? 2 : 1;
+        const c10::Device device = x.t->device();
+        const int64_t tokens = x.t->size(0), inputs = x.t->size(1), rows = weight.t->size(0);
+        for (int64_t v : {tokens, inputs, rows})
+            if (v > 0x7fffffff) refuse("%s: a size of %lld is too large", who, (long long)v);
+        if (a.activation == 3 && rows % 2 != 0) refuse("%s: swiglu takes the two halves of weight, which has %lld rows", who, (long long)rows);
+        const int64_t outputs = a.activation == 3 ? rows / 2 : rows;
+        weight.type(x.t->scalar_type());
+        weight.shape({rows, inputs});
+        for (const Arg *t : {&x, &weight}) {
+            t->on(device);
+            t->last_contiguous();
+        }
+        auto vector = [&](const Arg &t, int64_t size) {
+            t.shape({size});
+            t.on(device);
+            t.last_contiguous();
+        };
+        if ((bool)x_scales != eight || (bool)weight_scales != eight)
+            refuse(eight ? "%s: 8-bit x and weight need x_scales and weight_scales" : "%s: x_scales and weight_scales are those of 8-bit operands", who);
+        if (eight) {
+            x_scales.type(at::kFloat);
+            weight_scales.type(at::kFloat);
+            vector(x_scales, tokens);
+            vector(weight_scales, rows);
+        }
+        if (bias) {
+            a.bias_dtype = dtype_code(bias);
+            vector(bias, rows);
+        }
+        if (residual) {
+            a.residual_dtype = dtype_code(residual);
+            residual.shape({tokens, outputs});
+            residual.on(device);
+            residual.last_contiguous();
+        }
+        at::ScalarType type;
+        a.out_dtype = result_type(who, args[7], out, at::kBFloat16, false, type);
+        at::Tensor result;
+        if (out) {
+            out.shape({tokens, outputs});
+            out.on(device);
+            out.last_contiguous();
+            out.disjoint();
+            result = *out.t;
+        } else {
+            result = at::empty({tokens, outputs}, x.t->options().dtype(type).requires_grad(false));
+        }
+        a.x = x.ptr<const void>();
+        a.weight = weight.ptr<const void>();
+        a.bias = bias.ptr<const void>();
+        a.residual = residual.ptr<const void>();
+        a.x_scales = x_scales.ptr<const float>();
+        a.weight_scales = weight_scales.ptr<const float>();
+        a.out = result.data_ptr();
+        a.stream = c10::cuda::getCurrentCUDAStream(device.index()).stream();
+        a.x_row = step(*x.t, 0), a.weight_row = step(*weight.t, 0), a.out_row = step(result, 0);
+        if (residual) a.residual_row = step(*residual.t, 0);
+        a.tokens = (uint32_t)tokens, a.inputs = (uint32_t)inputs, a.outputs = (uint32_t)outputs;
+        a.device = device.index();
+        called(g_entry.linear(&a));
+        out.written();
+        return out ? Py_NewRef(args[8]) : THPVariable_Wrap(result);
+    });
+}
+
+/* (x, weight, tails, bias, activation, starts, slots, fresh, out) -> out */
+PyObject *short_conv(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+    return guarded([&]() -> PyObject * {
+        const char *who = "short_conv";
+        if (nargs != 9) refuse("%s: 9 arguments expected", who);
+        if (g_entry.conv == nullptr) throw Refused{PyExc_RuntimeError, "the library is not bound"};
+        const Arg x(who, "x", args[0]), weight(who, "weight", args[1]), tails(who, "tails", args[2]), bias(who, "bias", args[3]),
+            starts(who, "starts", args[5]), slots(who, "slots", args[6]), fresh(who, "fresh", args[7]), out(who, "out", args[8]);
+        for (const Arg *a : {&x, &weight, &tails}) a->present();
+        for (const Arg *a : {&x, &weight, &tails, &bias, &out}) a->no_gradient();
+        GdnB200ConvArgs a = {};
+        a.activation = activation_code(who, args[4], {"silu"});
+        x.dims(2);
+        weight.dims(2);
+        tails.dims(3);
+        a.dtype = dtype_code(x);
+        a.weight_dtype = dtype_code(weight);
+        a.tail_dtype = dtype_code(tails);
+        const c10::Device device = x.t->device();
+        const int64_t tokens = x.t->size(0), channels = x.t->size(1), width = weight.t->size(1), n_slots = tails.t->size(0);
+        weight.shape({channels, width});
+        tails.shape({n_slots, width - 1, channels});
+        if (!weight.t->is_contiguous()) refuse("%s: weight is not contiguous", who);
+        for (const Arg *t : {&x, &tails}) t->last_contiguous();
+        for (const Arg *t : {&x, &weight, &tails}) t->on(device);
+        if (bias) {
+            bias.type(weight.t->scalar_type());
+            bias.shape({channels});
+            bias.on(device);
+            bias.last_contiguous();
+        }
+        int64_t sequences = tokens;
+        if (starts) {
+            starts.type(at::kInt);
+            starts.dims(1);
+            starts.on(device);
+            starts.last_contiguous();
+            sequences = starts.t->size(0) - 1;
+            if (sequences < 0) refuse("%s: starts has shape [0], expected [sequences + 1]", who);
+        }
+        if (slots) {
+            slots.type(at::kInt);
+            slots.shape({sequences});
+            slots.on(device);
+            slots.last_contiguous();
+        }
+        if (fresh) {
+            if (fresh.t->scalar_type() != at::kByte) fresh.type(at::kBool);
+            fresh.shape({sequences});
+            fresh.on(device);
+            fresh.last_contiguous();
+        }
+        for (int64_t v : {tokens, sequences, channels, width, n_slots})
+            if (v > 0x7fffffff) refuse("%s: a size of %lld is too large", who, (long long)v);
+        at::Tensor result;
+        if (out) {
+            out.type(x.t->scalar_type());
+            out.shape(x.t->sizes());
+            out.on(device);
+            out.last_contiguous();
+            out.disjoint();
+            result = *out.t;
+        } else {
+            result = at::empty({tokens, channels}, x.t->options().requires_grad(false));
+        }
+        a.x = x.ptr<const void>();
+        a.weight = weight.ptr<const void>();
+        a.bias = bias.ptr<const void>();
+        a.tails = tails.ptr<void>();
+        a.out = result.data_ptr();
+        a.starts = starts.ptr<const int32_t>();
+        a.slots = slots.ptr<const int32_t>();
+        a.fresh = fresh.ptr<const uint8_t>();
+        a.stream = c10::cuda::getCurrentCUDAStream(device.index()).stream();
+        a.x_token = step(*x.t, 0), a.out_token = step(result, 0);
+        a.tails_slot = step(*tails.t, 0), a.tails_row = step(*tails.t, 1);
+        a.sequences = (uint32_t)sequences, a.tokens = (uint32_t)tokens, a.channels = (uint32_t)channels;
+        a.width = (uint32_t)width, a.tail_slots = (uint32_t)n_slots;
+        a.device = device.index();
+        called(g_entry.conv(&a));
+        tails.written();
+        out.written();
+        return out ? Py_NewRef(args[8]) : THPVariable_Wrap(result);
+    });
+}
+
+/* bind(step, chunk, chunk_workspace, logits, norm, linear, conv, last_error): addresses of the C entries */
 PyObject *bind(PyObject *, PyObject *args) {
-    unsigned long long p[5];
-    if (!PyArg_ParseTuple(args, "KKKKK", p, p + 1, p + 2, p + 3, p + 4)) return nullptr;
+    unsigned long long p[8];
+    if (!PyArg_ParseTuple(args, "KKKKKKKK", p, p + 1, p + 2, p + 3, p + 4, p + 5, p + 6, p + 7)) return nullptr;
     g_entry.step = reinterpret_cast<decltype(g_entry.step)>(p[0]);
     g_entry.chunk = reinterpret_cast<decltype(g_entry.chunk)>(p[1]);
     g_entry.chunk_workspace = reinterpret_cast<decltype(g_entry.chunk_workspace)>(p[2]);
     g_entry.logits = reinterpret_cast<decltype(g_entry.logits)>(p[3]);
-    g_entry.last_error = reinterpret_cast<decltype(g_entry.last_error)>(p[4]);
+    g_entry.norm = reinterpret_cast<decltype(g_entry.norm)>(p[4]);
+    g_entry.linear = reinterpret_cast<decltype(g_entry.linear)>(p[5]);
+    g_entry.conv = reinterpret_cast<decltype(g_entry.conv)>(p[6]);
+    g_entry.last_error = reinterpret_cast<decltype(g_entry.last_error)>(p[7]);
     Py_RETURN_NONE;
 }
 
@@ -395,6 +700,9 @@ PyMethodDef g_methods[] = {
     {"delta_step", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(delta_step)), METH_FASTCALL, nullptr},
     {"delta_chunk", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(delta_chunk)), METH_FASTCALL, nullptr},
     {"constrain_logits", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(constrain_logits)), METH_FASTCALL, nullptr},
+    {"rms_norm", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(rms_norm)), METH_FASTCALL, nullptr},
+    {"linear", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(linear)), METH_FASTCALL, nullptr},
+    {"short_conv", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(short_conv)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_ops_torch", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 

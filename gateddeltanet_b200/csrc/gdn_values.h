@@ -1,0 +1,83 @@
+/* Values of the serving operators' tensors: eight neighbours at a time through
+ * 16-byte accesses, or one by one, as FP32. Loads go past L1 (what another
+ * kernel wrote is in L2). */
+#ifndef GDN_VALUES_H
+#define GDN_VALUES_H
+
+#include <cuda_bf16.h>
+#include <cuda_fp8.h>
+#include <stdint.h>
+
+#include "gdn_ops.h"
+
+namespace gdn {
+namespace ops {
+
+__device__ __forceinline__ float low_bf16(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float high_bf16(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+__device__ __forceinline__ void load8(const float *p, float (&v)[8]) {
+    const float4 a = __ldcg(reinterpret_cast<const float4 *>(p)), b = __ldcg(reinterpret_cast<const float4 *>(p) + 1);
+    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+}
+__device__ __forceinline__ void unpack8(const uint4 &w, float (&v)[8]) {
+    v[0] = low_bf16(w.x), v[1] = high_bf16(w.x), v[2] = low_bf16(w.y), v[3] = high_bf16(w.y);
+    v[4] = low_bf16(w.z), v[5] = high_bf16(w.z), v[6] = low_bf16(w.w), v[7] = high_bf16(w.w);
+}
+__device__ __forceinline__ void load8(const __nv_bfloat16 *p, float (&v)[8]) {
+    unpack8(__ldcg(reinterpret_cast<const uint4 *>(p)), v);
+}
+__device__ __forceinline__ float load1(const float *p) { return __ldcg(p); }
+__device__ __forceinline__ float load1(const __nv_bfloat16 *p) {
+    return __uint_as_float((uint32_t)__ldcg(reinterpret_cast<const unsigned short *>(p)) << 16);
+}
+__device__ __forceinline__ void store8(float *p, const float (&v)[8]) {
+    reinterpret_cast<float4 *>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+    reinterpret_cast<float4 *>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+}
+__device__ __forceinline__ uint4 pack8(const float (&v)[8]) {
+    return make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+}
+__device__ __forceinline__ void store8(__nv_bfloat16 *p, const float (&v)[8]) { *reinterpret_cast<uint4 *>(p) = pack8(v); }
+__device__ __forceinline__ void store1(float *p, float x) { *p = x; }
+__device__ __forceinline__ void store1(__nv_bfloat16 *p, float x) { *p = __float2bfloat16_rn(x); }
+
+/* the same of a tensor whose type is known at run time: element i */
+__device__ __forceinline__ void load8(const void *p, int64_t i, int type, float (&v)[8]) {
+    if (type == kBF16)
+        load8(static_cast<const __nv_bfloat16 *>(p) + i, v);
+    else
+        load8(static_cast<const float *>(p) + i, v);
+}
+__device__ __forceinline__ float load1(const void *p, int64_t i, int type) {
+    return type == kBF16 ? load1(static_cast<const __nv_bfloat16 *>(p) + i) : load1(static_cast<const float *>(p) + i);
+}
+__device__ __forceinline__ void store8(void *p, int64_t i, int type, const float (&v)[8]) {
+    if (type == kBF16)
+        store8(static_cast<__nv_bfloat16 *>(p) + i, v);
+    else
+        store8(static_cast<float *>(p) + i, v);
+}
+__device__ __forceinline__ void store1(void *p, int64_t i, int type, float x) {
+    if (type == kBF16)
+        store1(static_cast<__nv_bfloat16 *>(p) + i, x);
+    else
+        store1(static_cast<float *>(p) + i, x);
+}
+
+/* x sigmoid(x) as x / (1 + e^-x): the division's and the exponential's errors
+ * together stay under 2^-21 (FP32 outputs keep 21 bits or more; others are
+ * rounded to fewer). e^-x is infinite for x < -88.7, where the result is -0. */
+__device__ __forceinline__ float silu(float x) { return __fdividef(x, 1.0f + __expf(-x)); }
+
+__host__ inline bool on16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+}  // namespace ops
+}  // namespace gdn
+
+#endif

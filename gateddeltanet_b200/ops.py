@@ -1,6 +1,7 @@
 """Serving operators on torch CUDA tensors: the gated delta rule over pooled
-states (delta_step for new tokens, delta_chunk for prompts) and the
-constraints on logits with the greedy pick (constrain_logits).
+states (delta_step for new tokens, delta_chunk for prompts), what a layer has
+around it (rms_norm, linear, short_conv) and the constraints on logits with the
+greedy pick (constrain_logits).
 
 A thin layer over the C entries of the same names in include/gdn_b200.h,
 which say what each operator computes; csrc/gdn_ops_torch.cpp checks the
@@ -16,13 +17,13 @@ from __future__ import annotations
 import ctypes
 import importlib.util
 import os
-from typing import Optional, Tuple
+from typing import Optional, Tuple, Union
 
 import torch
 
 from . import HERE, last_error, lib
 
-__all__ = ["delta_step", "delta_chunk", "delta_status", "constrain_logits"]
+__all__ = ["delta_step", "delta_chunk", "delta_status", "constrain_logits", "rms_norm", "linear", "linear_status", "short_conv"]
 
 
 def _load():
@@ -35,7 +36,7 @@ def _load():
     L = lib()
     module.bind(*(ctypes.cast(getattr(L, name), ctypes.c_void_p).value for name in (
         "gdn_b200_delta_step", "gdn_b200_delta_chunk", "gdn_b200_delta_chunk_workspace", "gdn_b200_constrain_logits",
-        "gdn_b200_last_error")))
+        "gdn_b200_rms_norm", "gdn_b200_linear", "gdn_b200_short_conv", "gdn_b200_last_error")))
     return module
 
 
@@ -73,11 +74,15 @@ def delta_status(device=None) -> None:
     """gdn_b200_delta_status: waits for the device (None: the current one) and
     raises RuntimeError if a wait inside delta_step or delta_chunk ran out
     there since the last call: the states of that call are then not valid."""
+    _status("delta_status", lib().gdn_b200_delta_status, device)
+
+
+def _status(who, entry, device):
     device = torch.device("cuda" if device is None else device)
     if device.type != "cuda":
-        raise ValueError(f"delta_status: {device} is not a CUDA device")
+        raise ValueError(f"{who}: {device} is not a CUDA device")
     index = device.index
-    if lib().gdn_b200_delta_status(torch.cuda.current_device() if index is None else index) != 0:
+    if entry(torch.cuda.current_device() if index is None else index) != 0:
         raise RuntimeError(last_error())
 
 
@@ -97,3 +102,52 @@ def constrain_logits(logits: torch.Tensor, *, tokens: Optional[torch.Tensor] = N
     out may be the logits themselves or memory apart from them, and a pick is -1
     where nothing is left."""
     return _native.constrain_logits(logits, tokens, lens, prompt_lens, repetition, presence, frequency, bias_ids, bias, mask, out)
+
+
+def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, *, residual: Optional[torch.Tensor] = None,
+             gate: Optional[torch.Tensor] = None, eps: float = 1e-6, dtype: Optional[torch.dtype] = None,
+             out: Optional[torch.Tensor] = None,
+             scales: Optional[torch.Tensor] = None) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
+    """gdn_b200_rms_norm: root-mean-square norm of x [tokens, dim] or [tokens,
+    heads, dim] (float32 or bfloat16) over dim, times weight [dim]. residual (of
+    x's shape, float32 or bfloat16): x is added to it in place, and the sum is
+    what is normed. gate (x's shape and type): the result is multiplied by
+    silu(gate). dtype (x's by default): float32, bfloat16, or float8_e4m3fn,
+    which returns (out, scales float32 [tokens]) with out * scales the result, a
+    scale for all heads of a token. out may be x itself or memory apart from the
+    others; `out` and `scales` are returned if given."""
+    return _native.rms_norm(x, weight, residual, gate, eps, dtype, out, scales)
+
+
+def linear(x: torch.Tensor, weight: torch.Tensor, *, bias: Optional[torch.Tensor] = None, activation: Optional[str] = None,
+           residual: Optional[torch.Tensor] = None, x_scales: Optional[torch.Tensor] = None,
+           weight_scales: Optional[torch.Tensor] = None, dtype: Optional[torch.dtype] = None,
+           out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """gdn_b200_linear: activation(x @ weight.T + bias) + residual, rounded once.
+    x [tokens, inputs] and weight [outputs, inputs] bfloat16, or float8_e4m3fn
+    with x_scales [tokens] and weight_scales [outputs] float32 that their rows are
+    multiplied by; rows on 16-byte boundaries. activation: None, "silu", "gelu" or
+    "swiglu", where weight (and bias and weight_scales) has 2 x outputs rows and
+    silu of the first half's values is multiplied by the second half's. bias and residual
+    [tokens, outputs] float32 or bfloat16. dtype: bfloat16 (the default) or float32.
+    out may be the residual itself or memory apart from the inputs."""
+    return _native.linear(x, weight, bias, activation, residual, x_scales, weight_scales, dtype, out)
+
+
+def linear_status(device=None) -> None:
+    """gdn_b200_linear_status: waits for the device (None: the current one) and
+    raises RuntimeError if a wait inside linear ran out there since the last
+    call: outputs of that call are then NaN."""
+    _status("linear_status", lib().gdn_b200_linear_status, device)
+
+
+def short_conv(x: torch.Tensor, weight: torch.Tensor, tails: torch.Tensor, *, bias: Optional[torch.Tensor] = None,
+               activation: Optional[str] = "silu", starts: Optional[torch.Tensor] = None, slots: Optional[torch.Tensor] = None,
+               fresh: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """gdn_b200_short_conv: causal convolution of each channel of x [tokens,
+    channels] (float32 or bfloat16) with weight [channels, width] (width 2 to 4,
+    its last column meets the token itself), then bias [channels] and silu
+    (activation None: without it). tails [slots, width - 1, channels] (float32 or
+    x's type) holds the inputs before each sequence, the oldest first, and gets
+    its last ones. starts, slots and fresh as for delta_step."""
+    return _native.short_conv(x, weight, tails, bias, activation, starts, slots, fresh, out)

@@ -343,9 +343,10 @@ size_t gdn_b200_delta_chunk_workspace(uint32_t tokens, uint32_t sequences, uint3
  * checks and for tests. */
 int gdn_b200_delta_status(int device);
 
-/* Test hook: in the next gdn_b200_delta_step or gdn_b200_delta_chunk of the
- * process the copy of one row block (if that call streams blocks through shared
- * memory) or of one CTA's first chunk is not made, so that a wait runs out. */
+/* Test hook: in the next gdn_b200_delta_step, gdn_b200_delta_chunk or gdn_b200_linear
+ * of the process the copy of one row block (if that call streams blocks through shared
+ * memory), of one CTA's first chunk or of x's block `index` of the first CTA's (if
+ * that call has more than 16 tokens) is not made, so that a wait runs out. */
 int gdn_b200_test_drop_copy(uint32_t index);
 
 /* Constraints on the logits of `rows` streams, and the greedy pick. With n
@@ -381,6 +382,93 @@ typedef struct {
     int32_t dtype, device;
 } GdnB200LogitsArgs;
 int gdn_b200_constrain_logits(const GdnB200LogitsArgs *args);
+
+/* Root-mean-square norm of rows [heads][dim] of `tokens` tokens, with the
+ * additions around it:
+ *   h = residual + x            (if residual; written back, rounded to its type)
+ *   y = h / sqrt(mean(h^2) + eps) * weight * (gate / (1 + e^-gate))
+ *   out = y, rounded once, or, in 8 bits, e4m3(y / scales[token]) with
+ *   scales[token] = max(max |y| / 448, 2^-126) over the token's heads
+ * The mean over dim is that of the unrounded h. Types: FP32 (0) or BF16 (1); x and
+ * gate have `dtype`, weight [dim] (contiguous) weight_dtype, the residual
+ * residual_dtype; out_dtype may also be E4M3 (2), with scales FP32 [tokens].
+ * weight, gate and residual may be NULL. All arithmetic is FP32 (results to
+ * 2^-20): squares overflow from 1.8e19 on, and a row with such a value or one that
+ * is not finite has no useful output (in 8 bits: NaN, scale too); other tokens are
+ * not touched by it. Strides count elements, dim is contiguous; any alignment,
+ * rows on 16-byte boundaries with dim a multiple of 8 are faster. out may be x
+ * itself (same type and strides) or memory apart from the other tensors. A token's
+ * values have to fit one CTA's registers: dim <= 16384, and in 8 bits
+ * heads x dim <= 16384 with dim rounded up to 16 times a power of two (up to 512)
+ * or to a multiple of 512. */
+typedef struct {
+    const void *x, *gate, *weight;
+    void *residual, *out;
+    float *scales;
+    void *stream; /* cudaStream_t */
+    int64_t x_token, x_head, gate_token, gate_head, residual_token, residual_head, out_token, out_head;
+    uint32_t tokens, heads, dim;
+    int32_t dtype, weight_dtype, residual_dtype, out_dtype, device;
+    float eps;
+    uint32_t reserved; /* 0 */
+} GdnB200NormArgs;
+int gdn_b200_rms_norm(const GdnB200NormArgs *args);
+
+/* Projection: out = act(s x W^T + bias) + residual, rounded once, with x
+ * [tokens][inputs] and W [rows][inputs] both BF16 (dtype 1, s = 1) or both E4M3
+ * (dtype 2, s = x_scales[token] weight_scales[row], FP32). activation 0: none,
+ * 1: v / (1 + e^-v), 2: gelu (v times the normal distribution function), 3: swiglu,
+ * where W has 2 x outputs rows (bias as many values) and out is silu of the first
+ * half's value times the second half's. rows = outputs for the others. bias
+ * [rows] (contiguous) and residual [tokens][outputs] may be NULL; bias, residual
+ * and out are FP32 (0) or BF16 (1), each its own. Sums are FP32 on the tensor
+ * cores; what is not finite spreads to its token's outputs (from x) or to its
+ * row's (from W) only. Strides count elements; rows of x and W are contiguous and start on
+ * 16-byte boundaries; inputs may be any number. out may be the residual itself
+ * (same type and stride) or memory apart from the inputs. */
+typedef struct {
+    const void *x, *weight, *bias, *residual;
+    const float *x_scales, *weight_scales;
+    void *out;
+    void *stream; /* cudaStream_t */
+    int64_t x_row, weight_row, residual_row, out_row;
+    uint32_t tokens, inputs, outputs;
+    int32_t dtype, bias_dtype, residual_dtype, out_dtype, activation, device;
+    uint32_t reserved; /* 0 */
+} GdnB200LinearArgs;
+int gdn_b200_linear(const GdnB200LinearArgs *args);
+/* 0, or -1 if a wait inside gdn_b200_linear ran out (2 s) on `device` since the
+ * last call of this function: outputs of that call are then NaN. Waits for the
+ * device. */
+int gdn_b200_linear_status(int device);
+
+/* Short causal convolution of each channel over packed sequences, with their last
+ * inputs in a pool:
+ *   out[t][c] = act(bias[c] + sum_j weight[c][j] x[t - (width - 1) + j][c])
+ * sequences, starts, slots and fresh as for the gated delta rule. What lies before
+ * a sequence's first token are the width - 1 rows (the oldest first) of its slot in
+ * tails [slots][width - 1][channels], zeros if it is fresh; they are replaced by
+ * the sequence's last width - 1 inputs (also those of before, where it is shorter).
+ * activation 0: none, 1: v / (1 + e^-v). x and out are FP32 (dtype 0) or BF16 (1),
+ * weight [channels][width] (contiguous) and bias [channels] (may be NULL) of
+ * weight_dtype, tails FP32 or x's type. Arithmetic is FP32. width is 2, 3 or 4. A
+ * sequence whose slot lies outside the pool changes nothing and gives zeros, as do
+ * tokens that no sequence covers. Entries of starts are clamped to [0, tokens];
+ * where they decrease the call ends all the same, within its tensors, but with
+ * outputs and tails that are not specified. Strides count elements, channels are
+ * contiguous; any alignment, rows on 16-byte boundaries with channels a
+ * multiple of 8 are faster. out must not overlap the inputs. */
+typedef struct {
+    const void *x, *weight, *bias;
+    void *tails, *out;
+    const int32_t *starts, *slots;
+    const uint8_t *fresh;
+    void *stream; /* cudaStream_t */
+    int64_t x_token, out_token, tails_slot, tails_row;
+    uint32_t sequences, tokens, channels, width, tail_slots;
+    int32_t dtype, weight_dtype, tail_dtype, activation, device;
+} GdnB200ConvArgs;
+int gdn_b200_short_conv(const GdnB200ConvArgs *args);
 
 #ifdef __cplusplus
 }
