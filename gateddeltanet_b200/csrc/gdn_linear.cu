@@ -6,13 +6,18 @@
  * loads 128 tokens and half of the rows of W, which is what lets L2 keep up with
  * the tensor cores. BF16 operands go to kind::f16 and 8-bit ones to
  * kind::f8f6f4; both come as blocks of 128 bytes of k in the 128-byte swizzle,
- * so that the two differ in the instruction alone. Sums are FP32 in TMEM. For
- * swiglu a tile holds the same outputs of both halves of W side by side.
+ * so that the two differ in the instruction alone. For swiglu a tile holds the
+ * same outputs of both halves of W side by side.
+ *
+ * The tensor cores cut the sums in TMEM to FP32 after each step of k, always
+ * towards zero: over 352 steps (5632 inputs of BF16) results were 4.4e-6 off in the
+ * 2-norm, where FP32 arithmetic is 5e-7. So TMEM takes 32 steps at a time, and the
+ * warps that empty it add these sums in registers, with rounding to nearest.
  *
  * A CTA has one warp that starts the TMA copies into a ring of stages, one
- * that starts the MMAs, and eight that take finished sums from TMEM to memory
- * (scales, bias, activation, residual) while the next tile's MMAs run: there
- * are two accumulators. CTAs walk over the tiles, tokens first.
+ * that starts the MMAs, and eight that add up the sums and take them to memory
+ * (scales, bias, activation, residual) while the next MMAs run: there are two
+ * accumulators. CTAs walk over the tiles, tokens first.
  *
  * Where there are too few tiles for all SMs, the CTAs of a cluster divide k:
  * each one's sums go to its shared memory, and each adds up, in the order of
@@ -34,21 +39,26 @@ namespace {
 
 constexpr uint64_t kWaitNs = 2000000000ull;
 constexpr uint32_t kEpilogueWarps = 8;
-constexpr uint32_t kLinearThreads = (kEpilogueWarps + 2) * 32;
-constexpr uint32_t kBlock = 128;                  /* bytes of k in a stage */
+constexpr uint32_t kLinearThreads = (kEpilogueWarps + 4) * 32; /* three warpgroups: the last has two warps of use */
+/* Registers a thread: 384 threads are launched with 168 (64512 in all); the warps with
+ * the sums then take 216 and the others 64 (63488). With 168 the sums spilled. */
+constexpr int kEpilogueRegs = 216, kOtherRegs = 64;
+constexpr uint32_t kBlock = 128;                  /* bytes of k in a row of a copy */
 constexpr uint32_t kRowsA = 128;                  /* tokens of a CTA */
 constexpr uint32_t kBytesA = kRowsA * kBlock;
 constexpr uint32_t kMaxStages = 8;
 constexpr uint32_t kMaxN = 256;
+constexpr uint32_t kChunk = 8;                    /* blocks of k that TMEM adds up */
 
 /* set when a wait of a kernel ran out; read and cleared by the host */
 __device__ int g_linear_status;
 
 /* a launch's tiles */
 struct LinearShape {
-    uint32_t n;        /* columns of a tile (rows of W): a multiple of 16, of 32 with two CTAs or for swiglu */
+    uint32_t n;        /* columns of a tile (rows of W): a multiple of 16, of 32 for swiglu or with two CTAs */
     uint32_t outs;     /* outputs of a tile: n, or n / 2 for swiglu */
     uint32_t split;    /* CTAs that divide k (one CTA to a tile), or 1 */
+    uint32_t sub;      /* 128-byte blocks of k in a stage: 1 or 2 */
     uint32_t stages;
     uint32_t rows_a;   /* rows of a copy of x: 128, or fewer where there are fewer tokens */
     uint32_t tiles_m, tiles_n, blocks; /* blocks: of k */
@@ -58,8 +68,9 @@ struct LinearShape {
 struct SharedTail {
     uint64_t full[kMaxStages], empty[kMaxStages], sums_full[2], sums_empty[2], drain;
     uint32_t tmem, abort, failed;
-    float scale[2][kMaxN], bias[2][kMaxN]; /* of an accumulator's columns */
+    alignas(16) float scale[2][kMaxN], bias[2][kMaxN]; /* of a tile's columns */
 };
+constexpr uint32_t kTurnBytes = 32 * 64; /* of a warp: 32 tokens of 16 FP32 */
 
 __device__ __forceinline__ uint32_t smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ uint64_t gtimer() {
@@ -80,7 +91,7 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
 __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
     uint32_t ok;
     asm volatile(
-        "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n selp.u32 %0, 1, 0, p;\n}\n"
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n selp.u32 %0, 1, 0, p;\n}\n"
         : "=r"(ok)
         : "r"(bar), "r"(parity), "r"(20000u)
         : "memory");
@@ -102,6 +113,12 @@ __device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, volatile
         }
     }
 }
+/* one lane of a converged warp */
+__device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(r));
+    return r != 0;
+}
 __device__ __forceinline__ uint32_t cluster_rank() {
     uint32_t r;
     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
@@ -121,6 +138,28 @@ __device__ __forceinline__ float4 load_cluster4(uint32_t addr) {
     asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
     return v;
 }
+__device__ __forceinline__ float4 load_shared4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint4 load_shared_u4(uint32_t addr) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ void store_shared4(uint32_t addr, const uint4 &v) {
+    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+/* a lane's row of 16 FP32 to its warp's buffer, for all lanes */
+__device__ __forceinline__ void turn_rows(uint32_t to, uint32_t x, const float (&v)[16]) {
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        store_shared4(to + ((i * 16) ^ x), make_uint4(__float_as_uint(v[4 * i]), __float_as_uint(v[4 * i + 1]), __float_as_uint(v[4 * i + 2]),
+                                                      __float_as_uint(v[4 * i + 3])));
+    __syncwarp();
+}
 __device__ __forceinline__ uint32_t load_cluster(uint32_t addr) {
     uint32_t v;
     asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
@@ -132,11 +171,9 @@ __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::
 
 /* K-major operand in the 128-byte swizzle: start >> 4 (bits 0-13), leading
  * offset (16-29, not used), 1 KB from eight rows to the next (32-45), version 1
- * (46-47), layout 2 (61-63). */
-__device__ __forceinline__ uint64_t smem_desc(uint32_t addr) {
-    return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) |
-           ((uint64_t)2 << 61);
-}
+ * (46-47), layout 2 (61-63). The high word is the same for all. */
+constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t smem_desc(uint32_t addr) { return (addr >> 4) | (1u << 16); }
 /* D FP32 (bits 4-5 = 1); A and B (7-9, 10-12): BF16 is 1 of kind::f16, E4M3 0 of kind::f8f6f4; N >> 3 at 17, M >> 4 at 24 */
 template <bool kFp8>
 __device__ __forceinline__ uint32_t instr_desc(uint32_t m, uint32_t n) {
@@ -144,11 +181,11 @@ __device__ __forceinline__ uint32_t instr_desc(uint32_t m, uint32_t n) {
 }
 
 template <int kCtas, bool kFp8>
-__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
-#define GDN_MMA(GROUP, KIND)                                                                                      \
-    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::" GROUP ".kind::" KIND        \
-                 " [%0], %1, %2, %3, p;\n}\n" ::"r"(d),                                                            \
-                 "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)                                             \
+__device__ __forceinline__ void mma(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool accumulate) {
+#define GDN_MMA(GROUP, KIND)                                                                                              \
+    asm volatile("{\n .reg .pred p;\n .reg .b64 da, db;\n setp.ne.b32 p, %4, 0;\n mov.b64 da, {%1, %5};\n mov.b64 db, {%2, %5};\n" \
+                 " tcgen05.mma.cta_group::" GROUP ".kind::" KIND " [%0], da, db, %3, p;\n}\n" ::"r"(d),                     \
+                 "r"(a), "r"(b), "r"(idesc), "r"((uint32_t)accumulate), "r"(kDescHigh)                                     \
                  : "memory")
     if constexpr (kCtas == 1 && !kFp8) GDN_MMA("1", "f16");
     if constexpr (kCtas == 1 && kFp8) GDN_MMA("1", "f8f6f4");
@@ -193,68 +230,107 @@ __device__ __forceinline__ void tc_ld16(uint32_t addr, float (&v)[16]) {
 __device__ __forceinline__ void tc_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void epilogue_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kEpilogueWarps * 32) : "memory"); }
 
-/* Columns c .. c + 15 of the tile (of its outputs) of one token to memory: v the sums, up
- * those of the second half for swiglu. `scale` and `bias` are those of the tile's
- * columns, with the second half's at g.outs. */
-struct Row {
-    uint32_t token, n; /* n: the output of column c */
-    float scale;
-};
-__device__ __forceinline__ void finish16(const LinearParams &p, const Row &r, float (&v)[16], float (&up)[16], const float *scale,
-                                         const float *bias, uint32_t outs, bool wide_out, bool wide_res) {
-    const bool pairs = p.activation == kSwiglu;
-    if (p.type == kE4M3) {
+/* kN sums of one token to values: v the sums, up those of the second half of W for swiglu.
+ * `scale` and `bias` are those of the tile's columns from v's first on, with the second half's
+ * `outs` further. */
+template <int kN>
+__device__ __forceinline__ void load_columns(const float *from, float (&v)[kN]) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            v[i] *= r.scale * scale[i];
-            if (pairs) up[i] *= r.scale * scale[outs + i];
+    for (int i = 0; i < kN; i += 4) {
+        const float4 e = *reinterpret_cast<const float4 *>(from + i);
+        v[i] = e.x, v[i + 1] = e.y, v[i + 2] = e.z, v[i + 3] = e.w;
+    }
+}
+template <bool kFp8, bool pairs, int kN>
+__device__ __forceinline__ void finish(const LinearParams &p, float row_scale, float (&v)[kN], float (&up)[kN], const float *scale,
+                                       const float *bias, uint32_t outs) {
+    if (kFp8) {
+        float f[kN];
+        load_columns(scale, f);
+#pragma unroll
+        for (int i = 0; i < kN; ++i) v[i] *= row_scale * f[i];
+        if (pairs) {
+            load_columns(scale + outs, f);
+#pragma unroll
+            for (int i = 0; i < kN; ++i) up[i] *= row_scale * f[i];
         }
     }
     if (p.bias != nullptr) {
+        float f[kN];
+        load_columns(bias, f);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            v[i] += bias[i];
-            if (pairs) up[i] += bias[outs + i];
+        for (int i = 0; i < kN; ++i) v[i] += f[i];
+        if (pairs) {
+            load_columns(bias + outs, f);
+#pragma unroll
+            for (int i = 0; i < kN; ++i) up[i] += f[i];
         }
     }
-    if (p.activation != kNoActivation) {
+    if (pairs) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = activate(p.activation, v[i], up[i]);
+        for (int i = 0; i < kN; ++i) v[i] = silu(v[i]) * up[i];
+    } else if (p.activation == kSilu) {
+#pragma unroll
+        for (int i = 0; i < kN; ++i) v[i] = silu(v[i]);
+    } else if (p.activation == kGelu) {
+#pragma unroll
+        for (int i = 0; i < kN; ++i) v[i] = gelu(v[i]);
     }
-    const bool whole = r.n + 16 <= p.outputs;
+}
+/* Rows of out and of the residual in pieces of four values: whether these are aligned. */
+struct Wide {
+    bool out, residual;
+    __device__ __forceinline__ explicit Wide(const LinearParams &p) {
+        const uintptr_t o = p.out_type == kBF16 ? 2 : 4, r = p.residual_type == kBF16 ? 2 : 4;
+        out = ((reinterpret_cast<uintptr_t>(p.out) | (uintptr_t)p.out_row * o) & (4 * o - 1)) == 0;
+        residual = ((reinterpret_cast<uintptr_t>(p.residual) | (uintptr_t)p.residual_row * r) & (4 * r - 1)) == 0;
+    }
+};
+__device__ __forceinline__ float4 load4(const void *p, int64_t i, int type) {
+    if (type == kF32) return __ldcg(reinterpret_cast<const float4 *>(static_cast<const float *>(p) + i));
+    const uint2 w = __ldcg(reinterpret_cast<const uint2 *>(static_cast<const __nv_bfloat16 *>(p) + i));
+    return make_float4(low_bf16(w.x), high_bf16(w.x), low_bf16(w.y), high_bf16(w.y));
+}
+/* Outputs n .. n + 3 of a token: the residual, the rounding and the store. */
+__device__ __forceinline__ void store4(const LinearParams &p, const Wide &wide, uint32_t token, uint32_t n, float4 v) {
+    if (token >= p.tokens || n >= p.outputs) return;
+    const bool whole = n + 4 <= p.outputs;
     if (p.residual != nullptr) {
-        const int64_t at = r.token * p.residual_row + r.n;
-        if (whole && wide_res) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                float e[8];
-                load8(p.residual, at + 8 * h, p.residual_type, e);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[8 * h + i] += e[i];
-            }
+        const int64_t at = token * p.residual_row + n;
+        if (whole && wide.residual) {
+            const float4 e = load4(p.residual, at, p.residual_type);
+            v.x += e.x, v.y += e.y, v.z += e.z, v.w += e.w;
         } else {
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-                if (r.n + i < p.outputs) v[i] += load1(p.residual, at + i, p.residual_type);
+            v.x += load1(p.residual, at, p.residual_type);
+            if (n + 1 < p.outputs) v.y += load1(p.residual, at + 1, p.residual_type);
+            if (n + 2 < p.outputs) v.z += load1(p.residual, at + 2, p.residual_type);
+            if (n + 3 < p.outputs) v.w += load1(p.residual, at + 3, p.residual_type);
         }
     }
-    const int64_t at = r.token * p.out_row + r.n;
-    if (whole && wide_out) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            float e[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) e[i] = v[8 * h + i];
-            store8(p.out, at + 8 * h, p.out_type, e);
-        }
+    const int64_t at = token * p.out_row + n;
+    if (whole && wide.out) {
+        if (p.out_type == kF32)
+            *reinterpret_cast<float4 *>(static_cast<float *>(p.out) + at) = v;
+        else
+            *reinterpret_cast<uint2 *>(static_cast<__nv_bfloat16 *>(p.out) + at) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
     } else {
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-            if (r.n + i < p.outputs) store1(p.out, at + i, p.out_type, v[i]);
+        store1(p.out, at, p.out_type, v.x);
+        if (n + 1 < p.outputs) store1(p.out, at + 1, p.out_type, v.y);
+        if (n + 2 < p.outputs) store1(p.out, at + 2, p.out_type, v.z);
+        if (n + 3 < p.outputs) store1(p.out, at + 3, p.out_type, v.w);
     }
 }
 
-template <int kCtas, bool kFp8>
+/* 32 tokens from row0 on by 16 outputs from n on, some of them past the ends or not aligned: from
+ * a warp's buffer. Its lane has four rows' pieces, 512 bytes apart. */
+__device__ __noinline__ void store_edge(const LinearParams &p, uint32_t row0, uint32_t n, uint32_t turn_in) {
+    const Wide wide(p);
+    const uint32_t lane = threadIdx.x & 31;
+#pragma unroll 1
+    for (int i = 0; i < 4; ++i) store4(p, wide, row0 + i * 8 + (lane >> 2), n + (lane & 3) * 4, load_shared4(turn_in + i * 512));
+}
+
+template <int kCtas, bool kFp8, bool pairs>
 __global__ void __launch_bounds__(kLinearThreads, 1)
     linear_kernel(const __grid_constant__ LinearParams p, const __grid_constant__ CUtensorMap map_x,
                   const __grid_constant__ CUtensorMap map_w, const LinearShape g) {
@@ -262,32 +338,36 @@ __global__ void __launch_bounds__(kLinearThreads, 1)
     constexpr uint32_t kElem = kFp8 ? 1 : 2;
     const uint32_t start = (smem_u32(raw) + 1023u) & ~1023u;
     uint8_t *base = raw + (start - smem_u32(raw));
-    const uint32_t bytes_b = g.n / kCtas * kBlock, stage = kBytesA + bytes_b;
-    SharedTail *s = reinterpret_cast<SharedTail *>(base + g.stages * stage);
+    const uint32_t bytes_b = g.n / kCtas * kBlock, block = kBytesA + bytes_b, stage = g.sub * block;
+    uint8_t *turn_buffers = base + g.stages * stage;
+    SharedTail *s = reinterpret_cast<SharedTail *>(turn_buffers + kEpilogueWarps * kTurnBytes);
     volatile uint32_t *abort = &s->abort;
     const uint32_t full = smem_u32(s->full), empty = smem_u32(s->empty), sums_full = smem_u32(s->sums_full),
                    sums_empty = smem_u32(s->sums_empty), drain = smem_u32(&s->drain);
-    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    /* taken from one lane, so that the compiler sees that all lanes of a warp go the same way */
+    const uint32_t tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     const uint32_t rank = kCtas == 1 && g.split == 1 ? 0 : cluster_rank(), pair = kCtas == 2 ? rank : 0;
     const uint32_t group = kCtas * g.split, worker = blockIdx.x / group, workers = gridDim.x / group;
     const uint32_t tiles = g.tiles_m * g.tiles_n;
     const uint32_t b0 = kCtas == 1 ? (uint32_t)((uint64_t)g.blocks * rank / g.split) : 0;
     const uint32_t b1 = kCtas == 1 ? (uint32_t)((uint64_t)g.blocks * (rank + 1) / g.split) : g.blocks;
-    const bool pairs = p.activation == kSwiglu;
 
-    if (tid == 0) {
-        for (uint32_t i = 0; i < g.stages; ++i) {
-            mbar_init(full + 8 * i, 1);
-            mbar_init(empty + 8 * i, 1);
+    if (warp == kEpilogueWarps) {
+        if (lane == 0) {
+            for (uint32_t i = 0; i < g.stages; ++i) {
+                mbar_init(full + 8 * i, 1);
+                mbar_init(empty + 8 * i, 1);
+            }
+            for (uint32_t i = 0; i < 2; ++i) {
+                mbar_init(sums_full + 8 * i, 1);
+                mbar_init(sums_empty + 8 * i, kCtas * kEpilogueWarps);
+            }
+            mbar_init(drain, 1);
+            s->abort = 0;
+            s->failed = 0;
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         }
-        for (uint32_t i = 0; i < 2; ++i) {
-            mbar_init(sums_full + 8 * i, 1);
-            mbar_init(sums_empty + 8 * i, kCtas * kEpilogueWarps);
-        }
-        mbar_init(drain, 1);
-        s->abort = 0;
-        s->failed = 0;
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        __syncwarp();
     }
     if (warp == 0) {
         if constexpr (kCtas == 1) {
@@ -299,181 +379,295 @@ __global__ void __launch_bounds__(kLinearThreads, 1)
         }
     }
     tc_fence_before();
-    __syncthreads();
-    if (kCtas == 2) cluster_sync(); /* the other CTA's barriers are ready */
+    if (kCtas == 2) {
+        __syncthreads();
+        cluster_sync(); /* the other CTA's barriers are ready */
+    } else if (warp == kEpilogueWarps) {
+        /* the copies need the barriers, which this warp has made, and not TMEM */
+        asm volatile("bar.arrive 2, %0;" ::"n"(kLinearThreads) : "memory");
+    } else {
+        asm volatile("bar.sync 2, %0;" ::"n"(kLinearThreads) : "memory");
+    }
     tc_fence_after();
-    const uint32_t tmem = s->tmem, second = g.columns / 2; /* columns from one accumulator to the other */
+    const uint32_t second = g.columns / 2; /* columns from one accumulator to the other */
 
-    if (warp == kEpilogueWarps) {
-        if (lane == 0) {
+    if (warp >= kEpilogueWarps) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+        /* Whole warps walk and wait, and one lane of them acts: the instructions of the tensor cores take
+         * uniform registers. Slots and phases are counted, not divided for: with the loops of a single
+         * lane that divided, a stage took 1000 cycles whatever its size. */
+        if (warp == kEpilogueWarps) {
             const uint32_t bar0 = kCtas == 2 ? map_rank(full, 0) : full; /* the pair's MMAs wait at the first CTA's */
             const uint32_t bytes = kCtas * (g.rows_a * kBlock + bytes_b);
-            uint32_t it = 0;
+            const uint32_t dropped = blockIdx.x == 0 ? p.drop : 0;
+            uint32_t slot = 0, phase = 1, it = 0, made = 0; /* phase: of the slot's last use, whose end is waited for */
             bool ok = true;
             for (uint32_t tile = worker; ok && tile < tiles; tile += workers) {
                 const uint32_t m0 = (tile % g.tiles_m * kCtas + pair) * kRowsA, n0 = tile / g.tiles_m * g.outs;
-                for (uint32_t b = b0; b < b1; ++b, ++it) {
-                    const uint32_t slot = it % g.stages;
-                    if (it >= g.stages && !wait_bar(empty + 8 * slot, (it / g.stages - 1) & 1u, abort)) {
-                        ok = false;
-                        break;
+                const uint32_t n1 = pairs ? p.outputs + n0 : n0 + g.n / 2;
+                for (uint32_t b = b0; b < b1; b += g.sub, ++it) {
+                    /* a new barrier's wait for the phase before its first returns at once */
+                    ok = __all_sync(0xffffffffu, wait_bar(empty + 8 * slot, phase, abort));
+                    if (!ok) break;
+                    const uint32_t here = min(g.sub, b1 - b), bar = bar0 + 8 * slot;
+                    if (elect_one()) {
+                        if (pair == 0) mbar_expect_tx(full + 8 * slot, here * bytes);
+                        for (uint32_t i = 0; i < here; ++i) {
+                            const uint32_t to = start + slot * stage + i * block, k = (b + i) * (kBlock / kElem);
+                            if (dropped != made + i + 1) copy_box<kCtas>(to, &map_x, k, m0, bar);
+                            if (kCtas == 2) {
+                                copy_box<kCtas>(to + kBytesA, &map_w, k, pair == 0 ? n0 : n1, bar);
+                            } else {
+                                copy_box<kCtas>(to + kBytesA, &map_w, k, n0, bar);
+                                if (pairs) copy_box<kCtas>(to + kBytesA + bytes_b / 2, &map_w, k, n1, bar);
+                            }
+                        }
                     }
-                    if (pair == 0) mbar_expect_tx(full + 8 * slot, bytes);
-                    const uint32_t to = start + slot * stage, bar = bar0 + 8 * slot, k = b * (kBlock / kElem);
-                    if (p.drop != 1 + it || blockIdx.x != 0) copy_box<kCtas>(to, &map_x, k, m0, bar);
-                    if (kCtas == 1) {
-                        copy_box<kCtas>(to + kBytesA, &map_w, k, n0, bar);
-                        copy_box<kCtas>(to + kBytesA + bytes_b / 2, &map_w, k, pairs ? p.outputs + n0 : n0 + g.n / 2, bar);
-                    } else {
-                        copy_box<kCtas>(to + kBytesA, &map_w, k, pair == 0 ? n0 : pairs ? p.outputs + n0 : n0 + g.n / 2, bar);
-                    }
+                    __syncwarp();
+                    made += here;
+                    if (++slot == g.stages) slot = 0, phase ^= 1;
                 }
             }
             /* copies already started land before the CTA exits (giving up does not stop them) */
-            if (pair == 0)
+            if (pair == 0 && lane == 0)
                 for (uint32_t j = it > g.stages ? it - g.stages : 0; j < it; ++j) {
                     const uint64_t w0 = gtimer();
                     while (!mbar_try(full + 8 * (j % g.stages), (j / g.stages) & 1u) && gtimer() - w0 < kWaitNs) {
                     }
                 }
         }
-        __syncwarp();
-    } else if (warp == kEpilogueWarps + 1) {
-        if (lane == 0 && pair == 0) {
-            const uint32_t idesc = instr_desc<kFp8>(kCtas * kRowsA, g.n);
-            uint32_t it = 0, seq = 0;
+        if (warp == kEpilogueWarps + 1 && pair == 0) {
+            const uint32_t idesc = instr_desc<kFp8>(kCtas * kRowsA, g.n), tmem = s->tmem;
+            uint32_t slot = 0, phase = 0, acc = 0, acc_phase = 1;
             bool ok = true;
-            for (uint32_t tile = worker; ok && tile < tiles; tile += workers, ++seq) {
-                const uint32_t acc = seq & 1u;
-                if (seq >= 2 && !wait_bar(sums_empty + 8 * acc, ((seq >> 1) - 1) & 1u, abort)) break;
-                tc_fence_after();
-                const uint32_t d = tmem + acc * second;
-                for (uint32_t b = b0; b < b1; ++b, ++it) {
-                    const uint32_t slot = it % g.stages;
-                    if (!wait_bar(full + 8 * slot, (it / g.stages) & 1u, abort)) {
-                        ok = false;
-                        break;
-                    }
+            for (uint32_t tile = worker; ok && tile < tiles; tile += workers) {
+                for (uint32_t c0 = b0; ok && c0 < b1; c0 += kChunk) {
+                    const uint32_t c1 = min(c0 + kChunk, b1), d = tmem + acc * second;
+                    ok = __all_sync(0xffffffffu, wait_bar(sums_empty + 8 * acc, acc_phase, abort));
+                    if (!ok) break;
                     tc_fence_after();
-                    const uint32_t a = start + slot * stage;
+                    for (uint32_t b = c0; b < c1; b += g.sub) {
+                        ok = __all_sync(0xffffffffu, wait_bar(full + 8 * slot, phase, abort));
+                        if (!ok) break;
+                        tc_fence_after();
+                        if (elect_one()) {
+                            const uint32_t a = smem_desc(start + slot * stage), w = smem_desc(start + slot * stage + kBytesA);
 #pragma unroll
-                    for (uint32_t k = 0; k < kBlock / 32; ++k)
-                        mma<kCtas, kFp8>(d, smem_desc(a + k * 32), smem_desc(a + kBytesA + k * 32), idesc, b != b0 || k != 0);
-                    commit<kCtas>(empty + 8 * slot);
+                            for (uint32_t k = 0; k < kBlock / 32; ++k) mma<kCtas, kFp8>(d, a + 2 * k, w + 2 * k, idesc, b != c0 || k != 0);
+                            if (g.sub == 2 && b + 1 < c1) {
+#pragma unroll
+                                for (uint32_t k = 0; k < kBlock / 32; ++k)
+                                    mma<kCtas, kFp8>(d, a + (block >> 4) + 2 * k, w + (block >> 4) + 2 * k, idesc, true);
+                            }
+                            commit<kCtas>(empty + 8 * slot);
+                            if (b + g.sub >= c1) commit<kCtas>(sums_full + 8 * acc);
+                        }
+                        __syncwarp();
+                        if (++slot == g.stages) slot = 0, phase ^= 1;
+                    }
+                    acc_phase ^= acc;
+                    acc ^= 1;
                 }
-                if (ok) commit<kCtas>(sums_full + 8 * acc);
             }
             /* every MMA has ended, and its arrivals are here, before TMEM and this memory are given back */
-            commit<kCtas>(drain);
+            if (elect_one()) commit<kCtas>(drain);
+            __syncwarp();
         }
-        if (lane == 0) {
+        if (warp == kEpilogueWarps + 1 && lane == 0) {
             const uint64_t w0 = gtimer();
             while (!mbar_try(drain, 0) && gtimer() - w0 < 2 * kWaitNs) {
             }
         }
         __syncwarp();
+        if (kCtas == 1 && g.split > 1) cluster_sync(); /* with the sums */
     } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kEpilogueRegs));
         const uint32_t quarter = warp & 3, half = warp >> 2; /* TMEM lanes, and every other 16 columns */
-        const int64_t out_size = p.out_type == kBF16 ? 2 : 4, res_size = p.residual_type == kBF16 ? 2 : 4;
-        const bool wide_out = ((reinterpret_cast<uintptr_t>(p.out) | (uintptr_t)(p.out_row * out_size)) & 15) == 0;
-        const bool wide_res = ((reinterpret_cast<uintptr_t>(p.residual) | (uintptr_t)(p.residual_row * res_size)) & 15) == 0;
-        uint32_t seq = 0;
+        const uint32_t tmem = s->tmem;
+        const Wide wide(p);
+        const bool has_res = p.residual != nullptr, f32_out = p.out_type == kF32;
+        const bool aligned = wide.out && (!has_res || wide.residual);
+        /* 16-byte piece q of row r of a warp's buffer at r * 64 + (q ^ (r / 2 % 4)) * 16 */
+        const uint32_t turn_base = smem_u32(turn_buffers) + warp * kTurnBytes;
+        const uint32_t turn_out = turn_base + lane * 64, turn_out_x = (lane >> 1 & 3) * 16;
+        const uint32_t turn_in = turn_base + (lane >> 2) * 64 + (((lane & 3) ^ (lane >> 3 & 3)) * 16);
+        uint32_t seq = 0, turn = 0;
         bool ok = true;
-        for (uint32_t tile = worker; tile < tiles; tile += workers, ++seq) {
-            const uint32_t acc = seq & 1u;
+        for (uint32_t tile = worker; tile < tiles; tile += workers, ++turn) {
             const uint32_t n0 = tile / g.tiles_m * g.outs;
-            Row r;
-            r.token = (tile % g.tiles_m * kCtas + pair) * kRowsA + quarter * 32 + lane;
-            r.scale = kFp8 && r.token < p.tokens ? __ldcg(p.x_scales + r.token) : 0.0f;
+            const uint32_t row0 = (tile % g.tiles_m * kCtas + pair) * kRowsA + quarter * 32, token = row0 + lane;
+            const float row_scale = kFp8 && token < p.tokens ? __ldcg(p.x_scales + token) : 0.0f;
+            float *scale = s->scale[turn & 1], *bias = s->bias[turn & 1];
             if (kFp8 || p.bias != nullptr) {
-                /* the accumulator's columns were last read two tiles ago, behind a barrier of the tile between */
+                /* these were last read two tiles ago, behind a barrier of the tile between */
                 for (uint32_t c = tid; c < g.n; c += kEpilogueWarps * 32) {
                     const uint32_t n = c < g.outs ? n0 + c : n0 + c - g.outs;
                     const uint32_t row = c < g.outs ? n : p.outputs + n;
                     const bool have = n < p.outputs;
-                    s->scale[acc][c] = kFp8 && have ? __ldcg(p.weight_scales + row) : 0.0f;
-                    s->bias[acc][c] = p.bias != nullptr && have ? load1(p.bias, row, p.bias_type) : 0.0f;
+                    scale[c] = kFp8 && have ? __ldcg(p.weight_scales + row) : 0.0f;
+                    bias[c] = p.bias != nullptr && have ? load1(p.bias, row, p.bias_type) : 0.0f;
                 }
                 epilogue_sync();
             }
-            ok = ok && wait_bar(sums_full + 8 * acc, (seq >> 1) & 1u, abort);
-            ok = __all_sync(0xffffffffu, ok);
-            tc_fence_after();
-            const uint32_t from = tmem + acc * second + ((quarter * 32) << 16);
-            const float nan = __int_as_float(0x7fc00000);
-            if (kCtas == 1 && g.split > 1) {
-                /* the sums as [4 columns][token] in the stages, whose copies and MMAs have ended */
-                if (!ok) s->failed = 1;
-                for (uint32_t c = half * 16; ok && c < g.n; c += 32) {
-                    float v[16];
-                    tc_ld16(from + c, v);
-                    tc_wait();
+            /* This thread's sums: 16 columns a set. The tile's outputs are units of 16, in turn the first and the
+             * second half's of the warps; for swiglu the sets 2 j and 2 j + 1 are one unit of either half of W. */
+            constexpr int kSets = kMaxN / 32;
+            float sum[kSets][16];
+            auto unit = [&](int set) { return (uint32_t)(pairs ? set / 2 : set) * 2 + half; };
+            auto have = [&](int set) { return unit(set) * 16 < g.outs; };
+            auto column = [&](int set) { return unit(set) * 16 + (pairs && (set & 1) ? g.outs : 0); };
+            for (uint32_t b = b0; b < b1; b += kChunk, ++seq) {
+                const uint32_t acc = seq & 1u;
+                ok = ok && wait_bar(sums_full + 8 * acc, (seq >> 1) & 1u, abort);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t from = tmem + acc * second + ((quarter * 32) << 16);
+                if (b == b0) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        *reinterpret_cast<float4 *>(base + ((c / 4 + i) * kRowsA + quarter * 32 + lane) * 16) =
-                            make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+                    for (int set = 0; set < kSets; ++set)
+                        if (have(set)) tc_ld16(from + column(set), sum[set]);
+                    tc_wait();
+                } else {
+#pragma unroll
+                    for (int set = 0; set < kSets; set += 2) {
+                        if (!have(set)) break;
+                        float v[2][16];
+                        tc_ld16(from + column(set), v[0]);
+                        if (have(set + 1)) tc_ld16(from + column(set + 1), v[1]);
+                        tc_wait();
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) sum[set][i] += v[0][i], sum[set + 1][i] += v[1][i];
+                    }
                 }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster(kCtas == 2 ? map_rank(sums_empty + 8 * acc, 0) : sums_empty + 8 * acc);
+            }
+            if (!ok) {
+#pragma unroll
+                for (int set = 0; set < kSets; ++set)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) sum[set][i] = __int_as_float(0x7fc00000);
+            }
+            if (kCtas == 1 && g.split > 1) {
+                /* to the stages, whose copies and MMAs have ended: piece q of a token at q ^ (token % 8) */
+                if (!ok) s->failed = 1;
+#pragma unroll
+                for (int set = 0; set < kSets; ++set)
+                    if (ok && have(set)) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            *reinterpret_cast<float4 *>(base + (quarter * 32 + lane) * g.n * 4 + (((column(set) / 4 + i) ^ (lane & 7)) * 16)) =
+                                make_float4(sum[set][4 * i], sum[set][4 * i + 1], sum[set][4 * i + 2], sum[set][4 * i + 3]);
+                    }
                 break; /* one tile; the rest below, with the cluster */
             }
-            for (uint32_t c = half * 16; c < g.outs; c += 32) {
-                float v[16], up[16];
-                __syncwarp();
-                if (ok) {
-                    tc_ld16(from + c, v);
-                    if (pairs) tc_ld16(from + g.outs + c, up);
-                    tc_wait();
-                }
-                if (!ok) {
+            /* A row of 16 values a lane is turned so that four lanes have one: whole sectors of memory are read and
+             * written. One lane's pieces are eight rows apart. */
+            const bool inside = aligned && row0 + 32 <= p.tokens;
+            const int64_t out_at = (row0 + (lane >> 2)) * p.out_row + n0, res_at = (row0 + (lane >> 2)) * p.residual_row + n0 + (lane & 3) * 4;
+            constexpr int kStep = pairs ? 2 : 1;
+            if (!has_res && !f32_out && inside) {
+                /* BF16: two units to a turn, four pieces of eight values a row */
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) v[i] = up[i] = nan;
-                }
-                r.n = n0 + c;
-                if (r.token < p.tokens && r.n < p.outputs)
-                    finish16(p, r, v, up, s->scale[acc] + c, s->bias[acc] + c, g.outs, wide_out, wide_res);
-            }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(kCtas == 2 ? map_rank(sums_empty + 8 * acc, 0) : sums_empty + 8 * acc);
-        }
-        __syncwarp();
-    }
-    if (kCtas == 1 && g.split > 1) {
-        cluster_sync();
-        if (warp < kEpilogueWarps && worker < tiles) {
-            const int64_t out_size = p.out_type == kBF16 ? 2 : 4, res_size = p.residual_type == kBF16 ? 2 : 4;
-            const bool wide_out = ((reinterpret_cast<uintptr_t>(p.out) | (uintptr_t)(p.out_row * out_size)) & 15) == 0;
-            const bool wide_res = ((reinterpret_cast<uintptr_t>(p.residual) | (uintptr_t)(p.residual_row * res_size)) & 15) == 0;
-            uint32_t bad = 0;
-            for (uint32_t q = 0; q < g.split; ++q) bad |= load_cluster(map_rank(smem_u32(&s->failed), q));
-            const uint32_t n0 = worker / g.tiles_m * g.outs, m = warp % 4 * 32 + lane;
-            Row r;
-            r.token = worker % g.tiles_m * kRowsA + m;
-            r.scale = kFp8 && r.token < p.tokens ? __ldcg(p.x_scales + r.token) : 0.0f;
-            /* 16 columns at a time, the cluster's CTAs and the two halves of a CTA's warps in turn */
-            for (uint32_t c = (rank * 2 + warp / 4) * 16; c < g.outs; c += g.split * 32) {
-                float v[16], up[16];
-#pragma unroll
-                for (int i = 0; i < 16; ++i) v[i] = up[i] = 0.0f;
-                if (r.token < p.tokens)
-                    for (uint32_t q = 0; q < g.split; ++q) {
-                        const uint32_t from = map_rank(start, q);
+                for (int set = 0; set < kSets; set += 2 * kStep) {
+                    if (!have(set)) break;
+                    const uint32_t c = unit(set) * 16, c2 = c + 32; /* of the second unit */
+                    const bool second_one = c2 < g.outs;
+                    finish<kFp8, pairs>(p, row_scale, sum[set], sum[set + (pairs ? 1 : 0)], scale + c, bias + c, g.outs);
+                    if (second_one)
+                        finish<kFp8, pairs>(p, row_scale, sum[set + kStep], sum[set + kStep + (pairs ? 1 : 0)], scale + c2, bias + c2, g.outs);
+                    if (n0 + (second_one ? c2 : c) + 16 <= p.outputs) {
+                        __syncwarp();
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            const float4 e = load_cluster4(from + ((c / 4 + i) * kRowsA + m) * 16);
-                            v[4 * i] += e.x, v[4 * i + 1] += e.y, v[4 * i + 2] += e.z, v[4 * i + 3] += e.w;
-                            if (pairs) {
-                                const float4 u = load_cluster4(from + (((g.outs + c) / 4 + i) * kRowsA + m) * 16);
-                                up[4 * i] += u.x, up[4 * i + 1] += u.y, up[4 * i + 2] += u.z, up[4 * i + 3] += u.w;
-                            }
+                            float(&v)[16] = sum[set + (i >> 1) * kStep];
+                            const int o = (i & 1) * 8;
+                            store_shared4(turn_out + ((i * 16) ^ turn_out_x),
+                                          make_uint4(pack_bf16(v[o], v[o + 1]), pack_bf16(v[o + 2], v[o + 3]), pack_bf16(v[o + 4], v[o + 5]),
+                                                     pack_bf16(v[o + 6], v[o + 7])));
                         }
-                    }
-                if (bad) {
+                        __syncwarp();
+                        __nv_bfloat16 *to = static_cast<__nv_bfloat16 *>(p.out) + out_at + ((lane & 2) ? c2 : c) + (lane & 1) * 8;
+                        if (second_one || (lane & 2) == 0) {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) v[i] = up[i] = __int_as_float(0x7fc00000);
+                            for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4 *>(to + i * 8 * p.out_row) = load_shared_u4(turn_in + i * 512);
+                        }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 2; ++e)
+                            if (e == 0 || second_one) {
+                                turn_rows(turn_out, turn_out_x, sum[set + e * kStep]);
+                                store_edge(p, row0, n0 + (e ? c2 : c), turn_in);
+                            }
+                    }
                 }
-                r.n = n0 + c;
-                if (r.token < p.tokens && r.n < p.outputs)
-                    finish16(p, r, v, up, s->scale[0] + c, s->bias[0] + c, g.outs, wide_out, wide_res);
+            } else {
+#pragma unroll
+                for (int set = 0; set < kSets; set += kStep) {
+                    const uint32_t c = unit(set) * 16;
+                    if (!have(set) || n0 + c >= p.outputs) break;
+                    const bool whole = inside && n0 + c + 16 <= p.outputs;
+                    float4 e[4];
+                    if (whole && has_res) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) e[i] = load4(p.residual, res_at + c + i * 8 * p.residual_row, p.residual_type);
+                    }
+                    finish<kFp8, pairs>(p, row_scale, sum[set], sum[set + (pairs ? 1 : 0)], scale + c, bias + c, g.outs);
+                    turn_rows(turn_out, turn_out_x, sum[set]);
+                    if (!whole) {
+                        store_edge(p, row0, n0 + c, turn_in);
+                        continue;
+                    }
+                    const int64_t to = out_at + c + (lane & 3) * 4;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        float4 v = load_shared4(turn_in + i * 512);
+                        if (has_res) v.x += e[i].x, v.y += e[i].y, v.z += e[i].z, v.w += e[i].w;
+                        if (f32_out)
+                            *reinterpret_cast<float4 *>(static_cast<float *>(p.out) + to + i * 8 * p.out_row) = v;
+                        else
+                            *reinterpret_cast<uint2 *>(static_cast<__nv_bfloat16 *>(p.out) + to + i * 8 * p.out_row) =
+                                make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
+                    }
+                }
+            }
+        }
+        __syncwarp();
+        if (kCtas == 1 && g.split > 1) {
+            cluster_sync();
+            if (worker < tiles) {
+                uint32_t bad = 0, from[8];
+#pragma unroll
+                for (uint32_t q = 0; q < 8; ++q) {
+                    from[q] = map_rank(start, min(q, g.split - 1));
+                    bad |= load_cluster(map_rank(smem_u32(&s->failed), min(q, g.split - 1)));
+                }
+                const uint32_t n0 = worker / g.tiles_m * g.outs, m0 = worker % g.tiles_m * kRowsA, pieces = g.outs / 4;
+                const uint32_t items = min(kRowsA, p.tokens - m0) * pieces;
+                /* four outputs of a token at a time, in turn over the cluster's threads: all parts' loads go out together */
+                for (uint32_t i = rank * kEpilogueWarps * 32 + tid; i < items; i += g.split * kEpilogueWarps * 32) {
+                    const uint32_t m = i / pieces, q4 = i % pieces;
+                    const uint32_t at = m * g.n * 4 + ((q4 ^ (m & 7)) * 16), at_up = m * g.n * 4 + (((q4 + pieces) ^ (m & 7)) * 16);
+                    float4 e[8], f[8];
+#pragma unroll
+                    for (uint32_t q = 0; q < 8; ++q)
+                        if (q < g.split) {
+                            e[q] = load_cluster4(from[q] + at);
+                            if (pairs) f[q] = load_cluster4(from[q] + at_up);
+                        }
+                    float v[4] = {0.0f, 0.0f, 0.0f, 0.0f}, up[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (uint32_t q = 0; q < 8; ++q)
+                        if (q < g.split) {
+                            v[0] += e[q].x, v[1] += e[q].y, v[2] += e[q].z, v[3] += e[q].w;
+                            if (pairs) up[0] += f[q].x, up[1] += f[q].y, up[2] += f[q].z, up[3] += f[q].w;
+                        }
+                    if (bad) v[0] = v[1] = v[2] = v[3] = __int_as_float(0x7fc00000);
+                    finish<kFp8, pairs>(p, kFp8 ? __ldcg(p.x_scales + m0 + m) : 0.0f, v, up, s->scale[0] + q4 * 4, s->bias[0] + q4 * 4, g.outs);
+                    store4(p, wide, m0 + m, n0 + q4 * 4, make_float4(v[0], v[1], v[2], v[3]));
+                }
             }
         }
     }
@@ -481,6 +675,7 @@ __global__ void __launch_bounds__(kLinearThreads, 1)
     __syncthreads();
     if (kCtas == 2 || g.split > 1) cluster_sync(); /* nobody reads this CTA's memory any more */
     if (warp == 0) {
+        const uint32_t tmem = s->tmem;
         if constexpr (kCtas == 1)
             asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(g.columns) : "memory");
         else
@@ -523,14 +718,17 @@ cudaError_t encode(CUtensorMap &map, const LinearParams &p, const void *at, int6
 
 constexpr size_t kSmemLimit = 232448; /* 227 KB a CTA */
 
+constexpr uint32_t kSmemRest = 1024 + kEpilogueWarps * kTurnBytes + sizeof(SharedTail);
+
 /* What is left to a launch once n, split and the number of CTAs to a tile are chosen. */
-LinearShape shape_of(const LinearParams &p, uint32_t ctas, uint32_t n, uint32_t split) {
+LinearShape shape_of(const LinearParams &p, uint32_t ctas, uint32_t n, uint32_t split, uint32_t sub) {
     LinearShape g;
     g.n = n;
     g.outs = p.activation == kSwiglu ? n / 2 : n;
     g.split = split;
-    const uint32_t stage = kBytesA + n / ctas * kBlock;
-    const uint32_t room = (uint32_t)(kSmemLimit - 1024 - sizeof(SharedTail)) / stage;
+    g.sub = sub;
+    const uint32_t stage = sub * (kBytesA + n / ctas * kBlock);
+    const uint32_t room = (uint32_t)(kSmemLimit - kSmemRest) / stage;
     g.stages = room < kMaxStages ? room : kMaxStages;
     g.rows_a = ctas == 2 || p.tokens >= kRowsA ? kRowsA : (p.tokens + 7) / 8 * 8;
     g.tiles_m = (p.tokens + ctas * kRowsA - 1) / (ctas * kRowsA);
@@ -541,14 +739,14 @@ LinearShape shape_of(const LinearParams &p, uint32_t ctas, uint32_t n, uint32_t 
     return g;
 }
 
-template <int kCtas, bool kFp8>
+template <int kCtas, bool kFp8, bool pairs>
 cudaError_t launch_shape(const LinearParams &p, const LinearShape &g, int sms, cudaStream_t stream) {
     CUtensorMap map_x, map_w;
     cudaError_t e = encode(map_x, p, p.x, p.x_row, p.tokens, g.rows_a);
-    if (e == cudaSuccess) e = encode(map_w, p, p.weight, p.weight_row, (uint64_t)p.outputs * (p.activation == kSwiglu ? 2 : 1), g.n / 2);
+    if (e == cudaSuccess) e = encode(map_w, p, p.weight, p.weight_row, (uint64_t)p.outputs * (pairs ? 2 : 1), kCtas == 2 || pairs ? g.n / 2 : g.n);
     if (e != cudaSuccess) return e;
-    const size_t smem = 1024 + (size_t)g.stages * (kBytesA + g.n / kCtas * kBlock) + sizeof(SharedTail);
-    e = cudaFuncSetAttribute(linear_kernel<kCtas, kFp8>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemLimit);
+    const size_t smem = kSmemRest + (size_t)g.stages * g.sub * (kBytesA + g.n / kCtas * kBlock);
+    e = cudaFuncSetAttribute(linear_kernel<kCtas, kFp8, pairs>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemLimit);
     if (e != cudaSuccess) return e;
     const uint32_t tiles = g.tiles_m * g.tiles_n, group = kCtas * g.split;
     uint32_t workers = (uint32_t)sms / group;
@@ -564,16 +762,22 @@ cudaError_t launch_shape(const LinearParams &p, const LinearShape &g, int sms, c
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = group > 1 ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, linear_kernel<kCtas, kFp8>, p, map_x, map_w, g);
+    return cudaLaunchKernelEx(&cfg, linear_kernel<kCtas, kFp8, pairs>, p, map_x, map_w, g);
 }
 
 }  // namespace
 
-cudaError_t launch_linear_as(const LinearParams &p, uint32_t ctas, uint32_t n, uint32_t split, int sms, cudaStream_t stream) {
-    const LinearShape g = shape_of(p, ctas, n, split);
-    if (p.type == kE4M3)
-        return ctas == 2 ? launch_shape<2, true>(p, g, sms, stream) : launch_shape<1, true>(p, g, sms, stream);
-    return ctas == 2 ? launch_shape<2, false>(p, g, sms, stream) : launch_shape<1, false>(p, g, sms, stream);
+cudaError_t launch_linear_as(const LinearParams &p, uint32_t ctas, uint32_t n, uint32_t split, uint32_t sub, int sms, cudaStream_t stream) {
+    const LinearShape g = shape_of(p, ctas, n, split, sub);
+    const bool fp8 = p.type == kE4M3;
+    if (p.activation == kSwiglu) {
+        auto *launch = ctas == 2 ? fp8 ? launch_shape<2, true, true> : launch_shape<2, false, true>
+                                 : fp8 ? launch_shape<1, true, true> : launch_shape<1, false, true>;
+        return launch(p, g, sms, stream);
+    }
+    auto *launch = ctas == 2 ? fp8 ? launch_shape<2, true, false> : launch_shape<2, false, false>
+                             : fp8 ? launch_shape<1, true, false> : launch_shape<1, false, false>;
+    return launch(p, g, sms, stream);
 }
 
 cudaError_t launch_linear(const LinearParams &p, int sms, cudaStream_t stream) {
@@ -581,9 +785,9 @@ cudaError_t launch_linear(const LinearParams &p, int sms, cudaStream_t stream) {
     const uint32_t rows = p.outputs * (p.activation == kSwiglu ? 2 : 1);
     uint32_t n = 256, split = 1;
     const uint32_t tiles_m = (p.tokens + kRowsA - 1) / kRowsA;
-    while (n > 32 && (uint64_t)tiles_m * ((rows + n - 1) / n) < (uint64_t)sms) n /= 2;
+    while (n > 64 && (uint64_t)tiles_m * ((rows + n - 1) / n) < (uint64_t)sms) n /= 2;
     while (n <= 128 && split < 8 && 2 * (uint64_t)tiles_m * ((rows + n - 1) / n) * split <= (uint64_t)sms && split * 2 * 4 <= blocks) split *= 2;
-    return launch_linear_as(p, p.tokens > 512 && n == 256 ? 2 : 1, n, split, sms, stream);
+    return launch_linear_as(p, p.tokens > 512 && n == 256 ? 2 : 1, n, split, n <= 128 ? 2 : 1, sms, stream);
 }
 
 cudaError_t linear_status(int *status) {

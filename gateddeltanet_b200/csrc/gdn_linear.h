@@ -8,11 +8,13 @@
 namespace gdn {
 namespace ops {
 
-/* v; `up` is the second half's value for kSwiglu. gelu: x times the normal distribution's function at x. */
+/* x times the normal distribution's function at x */
+__device__ __forceinline__ float gelu(float v) { return 0.5f * v * (1.0f + erff(v * 0.70710678f)); }
+/* v; `up` is the second half's value for kSwiglu */
 __device__ __forceinline__ float activate(int activation, float v, float up) {
     switch (activation) {
         case kSilu: return silu(v);
-        case kGelu: return 0.5f * v * (1.0f + erff(v * 0.70710678f));
+        case kGelu: return gelu(v);
         case kSwiglu: return silu(v) * up;
         default: return v;
     }
