@@ -11,7 +11,7 @@
  *
  * The tensor cores cut the sums in TMEM to FP32 after each step of k, always
  * towards zero: over 352 steps (5632 inputs of BF16) results were 4.4e-6 off in the
- * 2-norm, where FP32 arithmetic is 5e-7. So TMEM takes 32 steps at a time, and the
+ * 2-norm, where FP32 arithmetic is 5e-7. So TMEM takes a part of k at a time, and the
  * warps that empty it add these sums in registers, with rounding to nearest.
  *
  * A CTA has one warp that starts the TMA copies into a ring of stages, one
@@ -48,7 +48,10 @@ constexpr uint32_t kRowsA = 128;                  /* tokens of a CTA */
 constexpr uint32_t kBytesA = kRowsA * kBlock;
 constexpr uint32_t kMaxStages = 8;
 constexpr uint32_t kMaxN = 256;
-constexpr uint32_t kChunk = 8;                    /* blocks of k that TMEM adds up */
+/* Blocks of k that TMEM adds up before the sums go on in registers. FP32 outputs: 12 (48 steps; off by up to
+ * 6.8e-7 in the 2-norm for 2048 inputs, where 8 give 4.7e-7 and cost 2 to 15 % more time, 16 give 1.0e-6).
+ * BF16 outputs, which are rounded to 1.7e-3: 32. Even, for stages of two blocks. */
+constexpr uint32_t kChunkF32 = 12, kChunkBF16 = 32;
 
 /* set when a wait of a kernel ran out; read and cleared by the host */
 __device__ int g_linear_status;
@@ -58,6 +61,7 @@ struct LinearShape {
     uint32_t n;        /* columns of a tile (rows of W): a multiple of 16, of 32 for swiglu or with two CTAs */
     uint32_t outs;     /* outputs of a tile: n, or n / 2 for swiglu */
     uint32_t split;    /* CTAs that divide k (one CTA to a tile), or 1 */
+    uint32_t chunk;    /* blocks of k added up in TMEM */
     uint32_t sub;      /* 128-byte blocks of k in a stage: 1 or 2 */
     uint32_t stages;
     uint32_t rows_a;   /* rows of a copy of x: 128, or fewer where there are fewer tokens */
@@ -141,6 +145,11 @@ __device__ __forceinline__ float4 load_cluster4(uint32_t addr) {
 __device__ __forceinline__ float4 load_shared4(uint32_t addr) {
     float4 v;
     asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ float load_shared(uint32_t addr) {
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
     return v;
 }
 __device__ __forceinline__ uint4 load_shared_u4(uint32_t addr) {
@@ -321,13 +330,19 @@ __device__ __forceinline__ void store4(const LinearParams &p, const Wide &wide, 
     }
 }
 
-/* 32 tokens from row0 on by 16 outputs from n on, some of them past the ends or not aligned: from
- * a warp's buffer. Its lane has four rows' pieces, 512 bytes apart. */
-__device__ __noinline__ void store_edge(const LinearParams &p, uint32_t row0, uint32_t n, uint32_t turn_in) {
-    const Wide wide(p);
-    const uint32_t lane = threadIdx.x & 31;
-#pragma unroll 1
-    for (int i = 0; i < 4; ++i) store4(p, wide, row0 + i * 8 + (lane >> 2), n + (lane & 3) * 4, load_shared4(turn_in + i * 512));
+/* 32 tokens from row0 on by 16 outputs from n on, some of them past the ends or not aligned, from
+ * a warp's buffer: two tokens at a time, a value a lane. */
+__device__ __noinline__ void store_edge(const LinearParams &p, uint32_t row0, uint32_t n, uint32_t buffer) {
+    const uint32_t lane = threadIdx.x & 31, c = lane & 15;
+    if (n + c >= p.outputs) return;
+#pragma unroll 4
+    for (uint32_t r = lane >> 4; r < 32; r += 2) {
+        const uint32_t token = row0 + r;
+        if (token >= p.tokens) break;
+        float v = load_shared(buffer + r * 64 + (((c >> 2) ^ (r >> 1 & 3)) << 4) + (c & 3) * 4);
+        if (p.residual != nullptr) v += load1(p.residual, token * p.residual_row + n + c, p.residual_type);
+        store1(p.out, token * p.out_row + n + c, p.out_type, v);
+    }
 }
 
 template <int kCtas, bool kFp8, bool pairs>
@@ -441,8 +456,8 @@ __global__ void __launch_bounds__(kLinearThreads, 1)
             uint32_t slot = 0, phase = 0, acc = 0, acc_phase = 1;
             bool ok = true;
             for (uint32_t tile = worker; ok && tile < tiles; tile += workers) {
-                for (uint32_t c0 = b0; ok && c0 < b1; c0 += kChunk) {
-                    const uint32_t c1 = min(c0 + kChunk, b1), d = tmem + acc * second;
+                for (uint32_t c0 = b0; ok && c0 < b1; c0 += g.chunk) {
+                    const uint32_t c1 = min(c0 + g.chunk, b1), d = tmem + acc * second;
                     ok = __all_sync(0xffffffffu, wait_bar(sums_empty + 8 * acc, acc_phase, abort));
                     if (!ok) break;
                     tc_fence_after();
@@ -497,6 +512,15 @@ __global__ void __launch_bounds__(kLinearThreads, 1)
             const uint32_t n0 = tile / g.tiles_m * g.outs;
             const uint32_t row0 = (tile % g.tiles_m * kCtas + pair) * kRowsA + quarter * 32, token = row0 + lane;
             const float row_scale = kFp8 && token < p.tokens ? __ldcg(p.x_scales + token) : 0.0f;
+            const bool inside = aligned && row0 + 32 <= p.tokens;
+            const int64_t out_at = (row0 + (lane >> 2)) * p.out_row + n0, res_at = (row0 + (lane >> 2)) * p.residual_row + n0 + (lane & 3) * 4;
+            if (has_res && token < p.tokens) {
+                /* this row's part of the residual on its way to L2, in pieces of 128 bytes, while the MMAs run */
+                const int64_t size = p.residual_type == kF32 ? 4 : 2;
+                const char *row = static_cast<const char *>(p.residual) + (token * p.residual_row + n0) * size;
+                const uint32_t bytes = (uint32_t)size * min(g.outs, p.outputs - n0);
+                for (uint32_t i = half * 128; i < bytes; i += 256) asm volatile("prefetch.global.L2 [%0];" ::"l"(row + i));
+            }
             float *scale = s->scale[turn & 1], *bias = s->bias[turn & 1];
             if (kFp8 || p.bias != nullptr) {
                 /* these were last read two tiles ago, behind a barrier of the tile between */
@@ -516,7 +540,7 @@ __global__ void __launch_bounds__(kLinearThreads, 1)
             auto unit = [&](int set) { return (uint32_t)(pairs ? set / 2 : set) * 2 + half; };
             auto have = [&](int set) { return unit(set) * 16 < g.outs; };
             auto column = [&](int set) { return unit(set) * 16 + (pairs && (set & 1) ? g.outs : 0); };
-            for (uint32_t b = b0; b < b1; b += kChunk, ++seq) {
+            for (uint32_t b = b0; b < b1; b += g.chunk, ++seq) {
                 const uint32_t acc = seq & 1u;
                 ok = ok && wait_bar(sums_full + 8 * acc, (seq >> 1) & 1u, abort);
                 ok = __all_sync(0xffffffffu, ok);
@@ -565,8 +589,6 @@ __global__ void __launch_bounds__(kLinearThreads, 1)
             }
             /* A row of 16 values a lane is turned so that four lanes have one: whole sectors of memory are read and
              * written. One lane's pieces are eight rows apart. */
-            const bool inside = aligned && row0 + 32 <= p.tokens;
-            const int64_t out_at = (row0 + (lane >> 2)) * p.out_row + n0, res_at = (row0 + (lane >> 2)) * p.residual_row + n0 + (lane & 3) * 4;
             constexpr int kStep = pairs ? 2 : 1;
             if (!has_res && !f32_out && inside) {
                 /* BF16: two units to a turn, four pieces of eight values a row */
@@ -599,32 +621,38 @@ __global__ void __launch_bounds__(kLinearThreads, 1)
                         for (int e = 0; e < 2; ++e)
                             if (e == 0 || second_one) {
                                 turn_rows(turn_out, turn_out_x, sum[set + e * kStep]);
-                                store_edge(p, row0, n0 + (e ? c2 : c), turn_in);
+                                store_edge(p, row0, n0 + (e ? c2 : c), turn_base);
                             }
                     }
                 }
             } else {
+                float4 e[4]; /* the residual of the next set */
+                auto load_residual = [&](int set) {
+                    const uint32_t c = unit(set) * 16;
+                    if (has_res && inside && c < g.outs && n0 + c + 16 <= p.outputs) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) e[i] = load4(p.residual, res_at + c + i * 8 * p.residual_row, p.residual_type);
+                    }
+                };
+                load_residual(0);
 #pragma unroll
                 for (int set = 0; set < kSets; set += kStep) {
                     const uint32_t c = unit(set) * 16;
                     if (!have(set) || n0 + c >= p.outputs) break;
                     const bool whole = inside && n0 + c + 16 <= p.outputs;
-                    float4 e[4];
-                    if (whole && has_res) {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) e[i] = load4(p.residual, res_at + c + i * 8 * p.residual_row, p.residual_type);
-                    }
+                    const float4 here[4] = {e[0], e[1], e[2], e[3]};
+                    if (set + kStep < kSets) load_residual(set + kStep);
                     finish<kFp8, pairs>(p, row_scale, sum[set], sum[set + (pairs ? 1 : 0)], scale + c, bias + c, g.outs);
                     turn_rows(turn_out, turn_out_x, sum[set]);
                     if (!whole) {
-                        store_edge(p, row0, n0 + c, turn_in);
+                        store_edge(p, row0, n0 + c, turn_base);
                         continue;
                     }
                     const int64_t to = out_at + c + (lane & 3) * 4;
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         float4 v = load_shared4(turn_in + i * 512);
-                        if (has_res) v.x += e[i].x, v.y += e[i].y, v.z += e[i].z, v.w += e[i].w;
+                        if (has_res) v.x += here[i].x, v.y += here[i].y, v.z += here[i].z, v.w += here[i].w;
                         if (f32_out)
                             *reinterpret_cast<float4 *>(static_cast<float *>(p.out) + to + i * 8 * p.out_row) = v;
                         else
@@ -727,6 +755,7 @@ LinearShape shape_of(const LinearParams &p, uint32_t ctas, uint32_t n, uint32_t 
     g.outs = p.activation == kSwiglu ? n / 2 : n;
     g.split = split;
     g.sub = sub;
+    g.chunk = p.out_type == kF32 ? kChunkF32 : kChunkBF16;
     const uint32_t stage = sub * (kBytesA + n / ctas * kBlock);
     const uint32_t room = (uint32_t)(kSmemLimit - kSmemRest) / stage;
     g.stages = room < kMaxStages ? room : kMaxStages;
@@ -780,14 +809,32 @@ cudaError_t launch_linear_as(const LinearParams &p, uint32_t ctas, uint32_t n, u
     return launch(p, g, sms, stream);
 }
 
+/* The tiles of a call are those for which this estimate is least. What it knows, in us on 148 SMs: a block of k takes
+ * 0.0018 n + 0.034 in one CTA (0.3 at least: the MMA reads 128 tokens whatever n is, and a wait is not hidden) and
+ * 0.0013 n + 0.067 in two; a launch 5.0 or 5.7 and 0.008 n for the last tile's way to memory; a further tile of a CTA
+ * 0.5; a cluster that divides k 0.6 + 0.5 a CTA. Of clusters of four and eight not as many as there are SMs for run at
+ * once (13 of eight did, 16 did not). Against sweeps of 110 calls (17 to 4096 tokens, 2048 and 5632 inputs, 2048 to
+ * 32000 outputs, both types) its choices were 1.7 % slower than the best tiles in the mean; 256 columns always,
+ * or 128 split as far as possible, were up to twice as slow at either end. */
 cudaError_t launch_linear(const LinearParams &p, int sms, cudaStream_t stream) {
-    const uint64_t blocks = ((uint64_t)p.inputs * (p.type == kE4M3 ? 1 : 2) + kBlock - 1) / kBlock;
-    const uint32_t rows = p.outputs * (p.activation == kSwiglu ? 2 : 1);
-    uint32_t n = 256, split = 1;
-    const uint32_t tiles_m = (p.tokens + kRowsA - 1) / kRowsA;
-    while (n > 64 && (uint64_t)tiles_m * ((rows + n - 1) / n) < (uint64_t)sms) n /= 2;
-    while (n <= 128 && split < 8 && 2 * (uint64_t)tiles_m * ((rows + n - 1) / n) * split <= (uint64_t)sms && split * 2 * 4 <= blocks) split *= 2;
-    return launch_linear_as(p, p.tokens > 512 && n == 256 ? 2 : 1, n, split, n <= 128 ? 2 : 1, sms, stream);
+    const uint32_t blocks = (uint32_t)(((uint64_t)p.inputs * (p.type == kE4M3 ? 1 : 2) + kBlock - 1) / kBlock);
+    float least = 3.4e38f;
+    uint32_t ctas = 1, n = 256, split = 1;
+    for (uint32_t c = 1; c <= (p.tokens > kRowsA ? 2u : 1u); ++c)
+        for (uint32_t width = 32; width <= kMaxN; width += 32) {
+            const uint32_t outs = p.activation == kSwiglu ? width / 2 : width;
+            const uint64_t tiles = (uint64_t)((p.tokens + c * kRowsA - 1) / (c * kRowsA)) * ((p.outputs + outs - 1) / outs);
+            const float block = c == 2 ? 0.0013f * width + 0.067f : 0.0018f * width + 0.034f > 0.3f ? 0.0018f * width + 0.034f : 0.3f;
+            for (uint32_t s = 1; s <= (c == 1 ? 8u : 1u); s *= 2) {
+                const uint64_t most = (uint64_t)sms * (s < 4 ? 8 : s == 4 ? 7 : 6) / 8;
+                if (s > 1 && (tiles * s > most || blocks / s < 4)) break;
+                const uint64_t waves = (tiles * c * s + sms - 1) / sms;
+                const float t = (float)waves * ((float)((blocks + s - 1) / s) * block + 0.5f) + 0.008f * width + (c == 2 ? 5.7f : 5.0f) +
+                                (s > 1 ? 0.6f + 0.5f * s : 0.0f);
+                if (t < least) least = t, ctas = c, n = width, split = s;
+            }
+        }
+    return launch_linear_as(p, ctas, n, split, n <= 128 ? 2 : 1, sms, stream);
 }
 
 cudaError_t linear_status(int *status) {
