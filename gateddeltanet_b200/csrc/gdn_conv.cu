@@ -45,48 +45,102 @@ __device__ uint32_t begun(const ConvParams &p, uint32_t t) {
     return lo;
 }
 
-/* T: type of x and y. kWide: eight channels a thread. */
+/* What the lanes of a thread do with its channels: C neighbours (16 bytes) or one. */
+template <typename T, bool kWide>
+struct Lane {
+    static constexpr int C = kWide ? 16 / sizeof(T) : 1;
+    static __device__ __forceinline__ void unpack(const uint4 &w, float (&v)[C]) {
+        if constexpr (C == 8)
+            unpack8(w, v);
+        else if constexpr (C == 4)
+            v[0] = __uint_as_float(w.x), v[1] = __uint_as_float(w.y), v[2] = __uint_as_float(w.z), v[3] = __uint_as_float(w.w);
+        else
+            v[0] = __uint_as_float(w.x);
+    }
+    /* as it is in memory (one channel: as FP32) */
+    static __device__ __forceinline__ uint4 fetch(const T *p) {
+        if constexpr (kWide)
+            return __ldcg(reinterpret_cast<const uint4 *>(p));
+        else
+            return make_uint4(__float_as_uint(load1(p)), 0, 0, 0);
+    }
+    static __device__ __forceinline__ void put(T *p, const float (&v)[C]) {
+        if constexpr (C == 8)
+            *reinterpret_cast<uint4 *>(p) = pack8(v);
+        else if constexpr (C == 4)
+            *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]);
+        else
+            store1(p, v[0]);
+    }
+    static __device__ __forceinline__ void get_tail(const ConvParams &p, int64_t at, float (&v)[C]) {
+        if constexpr (C == 8) {
+            load8(p.tails, at, p.tail_type, v);
+        } else if constexpr (C == 4) { /* x is FP32, and so are the tails */
+            unpack(__ldcg(reinterpret_cast<const uint4 *>(static_cast<const float *>(p.tails) + at)), v);
+        } else {
+            v[0] = load1(p.tails, at, p.tail_type);
+        }
+    }
+    static __device__ __forceinline__ void put_tail(const ConvParams &p, int64_t at, const float (&v)[C]) {
+        if constexpr (C == 8)
+            store8(p.tails, at, p.tail_type, v);
+        else if constexpr (C == 4)
+            *reinterpret_cast<float4 *>(static_cast<float *>(p.tails) + at) = make_float4(v[0], v[1], v[2], v[3]);
+        else
+            store1(p.tails, at, p.tail_type, v[0]);
+    }
+};
+
+/* A channel's weights in shared memory: four floats, the last one meets the token itself (a
+ * shorter width has zeros in front, which nobody reads). Rows of kThreads + 1, so that
+ * threads that fill neighbouring channels use different banks. */
+template <int C, uint32_t kLanes>
+struct Weights {
+    float4 w[C][kLanes + 1];
+    template <int W>
+    __device__ __forceinline__ void fill(const ConvParams &p, uint32_t first) {
+        for (uint32_t i = threadIdx.x; i < kLanes * C; i += blockDim.x) {
+            const uint32_t c = first + i;
+            float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (c < p.channels) {
+                if (W == 4 && p.weight_type == kF32 && on16(p.weight)) {
+                    const float4 e = *reinterpret_cast<const float4 *>(static_cast<const float *>(p.weight) + (size_t)c * 4);
+                    v[0] = e.x, v[1] = e.y, v[2] = e.z, v[3] = e.w;
+                } else {
+#pragma unroll
+                    for (int j = 0; j < W; ++j) v[4 - W + j] = load1(p.weight, (int64_t)c * W + j, p.weight_type);
+                }
+            }
+            w[i % C][i / C] = make_float4(v[0], v[1], v[2], v[3]);
+        }
+    }
+};
+
+/* bias + sum of weights times the window's values (oldest first) and the token's own, in this order */
+template <int W>
+__device__ __forceinline__ float tap(const float4 &w, float bias, const float (&v)[W]) {
+    float s = bias;
+    if constexpr (W > 3) s = fmaf(w.x, v[W - 4], s);
+    if constexpr (W > 2) s = fmaf(w.y, v[W - 3], s);
+    s = fmaf(w.z, v[W - 2], s);
+    return fmaf(w.w, v[W - 1], s);
+}
+
+/* T: type of x and y. kWide: 16 bytes of channels a thread. */
 template <typename T, bool kWide, int W>
 __global__ void __launch_bounds__(kThreads) conv_kernel(const __grid_constant__ ConvParams p, const uint32_t tile) {
-    constexpr int C = kWide ? 8 : 1;
-    const uint32_t c0 = (blockIdx.y * kThreads + threadIdx.x) * C;
+    using L = Lane<T, kWide>;
+    constexpr int C = L::C;
+    __shared__ Weights<C, kThreads> weights;
+    const uint32_t tid = threadIdx.x, c0 = (blockIdx.y * kThreads + tid) * C;
     const bool live = c0 < p.channels;
     const T *x = static_cast<const T *>(p.x) + c0;
     T *y = static_cast<T *>(p.out) + c0;
-    auto load = [&](const T *from, float (&v)[C]) {
-        if constexpr (kWide)
-            load8(from, v);
-        else
-            v[0] = load1(from);
-    };
-    auto load_tail = [&](int64_t at, float (&v)[C]) {
-        if constexpr (kWide)
-            load8(p.tails, at, p.tail_type, v);
-        else
-            v[0] = load1(p.tails, at, p.tail_type);
-    };
-    auto store = [&](uint32_t t, const float (&v)[C]) {
-        if constexpr (kWide)
-            store8(y + t * p.out_token, v);
-        else
-            store1(y + t * p.out_token, v[0]);
-    };
-    auto store_tail = [&](int64_t at, const float (&v)[C]) {
-        if constexpr (kWide)
-            store8(p.tails, at, p.tail_type, v);
-        else
-            store1(p.tails, at, p.tail_type, v[0]);
-    };
-
-    float w[W][C], bias[C];
-    if (live) {
+    weights.template fill<W>(p, blockIdx.y * kThreads * C);
+    float bias[C];
 #pragma unroll
-        for (int c = 0; c < C; ++c) {
-            bias[c] = p.bias != nullptr ? load1(p.bias, c0 + c, p.weight_type) : 0.0f;
-#pragma unroll
-            for (int j = 0; j < W; ++j) w[j][c] = load1(p.weight, (int64_t)(c0 + c) * W + j, p.weight_type);
-        }
-    }
+    for (int c = 0; c < C; ++c) bias[c] = live && p.bias != nullptr ? load1(p.bias, c0 + c, p.weight_type) : 0.0f;
+    __syncthreads();
     const uint32_t t0 = blockIdx.x * tile, t1 = min(t0 + tile, p.tokens);
     uint32_t n = t0 < t1 ? begun(p, t0) : 0; /* the sequence of token t0 is n - 1, if it has one */
     uint32_t t = t0;
@@ -105,7 +159,7 @@ __global__ void __launch_bounds__(kThreads) conv_kernel(const __grid_constant__ 
         if (slot < 0 || slot >= (int64_t)p.tail_slots) {
             /* tokens of no sequence, or of one without a slot */
             if (live)
-                for (; t < stop; ++t) store(t, zero);
+                for (; t < stop; ++t) L::put(y + t * p.out_token, zero);
             t = stop;
             ++n;
             continue;
@@ -117,69 +171,98 @@ __global__ void __launch_bounds__(kThreads) conv_kernel(const __grid_constant__ 
         } else {
             stop = min(end, max(t1, begin + (W - 1)));
         }
-        const bool fresh = p.fresh != nullptr && p.fresh[n - 1] != 0;
         if (live) {
-            /* window: inputs t - (W - 1) .. t - 1 */
-            float win[W][C];
-            const int64_t rows = slot * p.tails_slot + c0;
             if (t == begin) {
-                float old[W][C];
-#pragma unroll
-                for (int j = 0; j < W - 1; ++j) {
-#pragma unroll
-                    for (int c = 0; c < C; ++c) old[j][c] = 0.0f;
-                    if (!fresh) load_tail(rows + j * p.tails_row, old[j]);
-#pragma unroll
-                    for (int c = 0; c < C; ++c) win[j][c] = old[j][c];
-                }
-                const uint32_t len = end - begin;
-#pragma unroll
-                for (int j = 0; j < W - 1; ++j) {
-                    float v[C];
-                    if (len + j >= W - 1) {
-                        load(x + (begin + len + j - (W - 1)) * p.x_token, v);
-                    } else {
-#pragma unroll
-                        for (int c = 0; c < C; ++c) v[c] = 0.0f;
-#pragma unroll
-                        for (int i = 0; i < W - 1; ++i)
-                            if ((uint32_t)i == len + j) {
-#pragma unroll
-                                for (int c = 0; c < C; ++c) v[c] = old[i][c];
-                            }
-                    }
-                    store_tail(rows + j * p.tails_row, v);
-                }
-            } else {
+                /* the tokens that meet the slot's rows, one by one */
+                const bool fresh = p.fresh != nullptr && p.fresh[n - 1] != 0;
+                const int64_t rows = slot * p.tails_slot + c0;
+                const uint32_t few = min((uint32_t)(W - 1), end - begin);
+                float win[W - 1][C];
 #pragma unroll
                 for (int j = 0; j < W - 1; ++j) {
 #pragma unroll
                     for (int c = 0; c < C; ++c) win[j][c] = 0.0f;
-                    if (t < stop) load(x + (int64_t)(t - (W - 1) + j) * p.x_token, win[j]);
+                    if (!fresh) L::get_tail(p, rows + j * p.tails_row, win[j]);
                 }
+                for (uint32_t i = 0; i < few; ++i) {
+                    float in[C], out[C];
+                    L::unpack(L::fetch(x + (int64_t)(t + i) * p.x_token), in);
+#pragma unroll
+                    for (int c = 0; c < C; ++c) {
+                        float v[W];
+#pragma unroll
+                        for (int j = 0; j < W - 1; ++j) v[j] = win[j][c];
+                        v[W - 1] = in[c];
+                        const float s = tap<W>(weights.w[c][tid], bias[c], v);
+                        out[c] = p.silu ? silu(s) : s;
+#pragma unroll
+                        for (int j = 0; j < W - 1; ++j) win[j][c] = v[j + 1];
+                    }
+                    L::put(y + (int64_t)(t + i) * p.out_token, out);
+                }
+                /* the window is now the slot's new content, unless there are more tokens */
+                const bool more = end - begin > W - 1;
+#pragma unroll
+                for (int j = 0; j < W - 1; ++j) {
+                    if (more) L::unpack(L::fetch(x + (int64_t)(end - (W - 1) + j) * p.x_token), win[j]);
+                    L::put_tail(p, rows + j * p.tails_row, win[j]);
+                }
+                t += few;
+            }
+            /* the others, kAhead at a time, whose W - 1 inputs before them are in x */
+            uint4 in[W - 1 + kAhead], next[kAhead];
+            if (t < stop) {
+#pragma unroll
+                for (int j = 0; j < W - 1; ++j) in[j] = L::fetch(x + (int64_t)(t - (W - 1) + j) * p.x_token);
+#pragma unroll
+                for (int a = 0; a < kAhead; ++a) next[a] = L::fetch(x + (int64_t)min(t + a, stop - 1) * p.x_token);
             }
             for (; t < stop; t += kAhead) {
-                float in[kAhead][C];
 #pragma unroll
-                for (int a = 0; a < kAhead; ++a)
-                    if (t + a < stop) load(x + (int64_t)(t + a) * p.x_token, in[a]);
+                for (int a = 0; a < kAhead; ++a) in[W - 1 + a] = next[a];
+                if (t + kAhead < stop) {
+#pragma unroll
+                    for (int a = 0; a < kAhead; ++a) next[a] = L::fetch(x + (int64_t)min(t + kAhead + a, stop - 1) * p.x_token);
+                }
+                /* two channels (one) at a time: a word of each input, a word of each output */
+                uint32_t result[kAhead][4];
+                constexpr int kWords = kWide ? 4 : 1, kPer = C / kWords;
+#pragma unroll
+                for (int q = 0; q < kWords; ++q) {
+                    float out[kAhead][2];
+#pragma unroll
+                    for (int e = 0; e < kPer; ++e) {
+                        const int c = q * kPer + e;
+                        const float4 w = weights.w[c][tid];
+                        float v[W - 1 + kAhead];
+#pragma unroll
+                        for (int j = 0; j < W - 1 + kAhead; ++j) {
+                            const uint32_t word = q == 0 ? in[j].x : q == 1 ? in[j].y : q == 2 ? in[j].z : in[j].w;
+                            v[j] = kPer == 1 ? __uint_as_float(word) : e == 0 ? low_bf16(word) : high_bf16(word);
+                        }
+#pragma unroll
+                        for (int a = 0; a < kAhead; ++a) {
+                            float u[W];
+#pragma unroll
+                            for (int j = 0; j < W; ++j) u[j] = v[a + j];
+                            const float s = tap<W>(w, bias[c], u);
+                            out[a][e] = p.silu ? silu(s) : s;
+                        }
+                    }
+#pragma unroll
+                    for (int a = 0; a < kAhead; ++a) result[a][q] = kPer == 2 ? pack_bf16(out[a][0], out[a][1]) : __float_as_uint(out[a][0]);
+                }
 #pragma unroll
                 for (int a = 0; a < kAhead; ++a)
                     if (t + a < stop) {
-                        float out[C];
-#pragma unroll
-                        for (int c = 0; c < C; ++c) {
-                            float s = bias[c];
-#pragma unroll
-                            for (int j = 0; j < W - 1; ++j) s = fmaf(w[j][c], win[j][c], s);
-                            s = fmaf(w[W - 1][c], in[a][c], s);
-#pragma unroll
-                            for (int j = 0; j < W - 2; ++j) win[j][c] = win[j + 1][c];
-                            win[W - 2][c] = in[a][c];
-                            out[c] = p.silu ? silu(s) : s;
-                        }
-                        store(t + a, out);
+                        T *to = y + (int64_t)(t + a) * p.out_token;
+                        if constexpr (kWide)
+                            *reinterpret_cast<uint4 *>(to) = make_uint4(result[a][0], result[a][1], result[a][2], result[a][3]);
+                        else
+                            store1(to, __uint_as_float(result[a][0]));
                     }
+#pragma unroll
+                for (int j = 0; j < W - 1; ++j) in[j] = in[kAhead + j];
             }
         }
         t = stop;
@@ -191,15 +274,65 @@ __global__ void __launch_bounds__(kThreads) conv_kernel(const __grid_constant__ 
             if (p.fresh[i] != 0 && bound_of(p, i + 1) <= bound_of(p, i)) {
                 const int64_t slot = p.slots == nullptr ? (int64_t)i : (int64_t)p.slots[i];
                 if (live && slot >= 0 && slot < (int64_t)p.tail_slots)
-                    for (int j = 0; j < W - 1; ++j) store_tail(slot * p.tails_slot + j * p.tails_row + c0, zero);
+                    for (int j = 0; j < W - 1; ++j) L::put_tail(p, slot * p.tails_slot + j * p.tails_row + c0, zero);
             }
+}
+
+/* One token of every sequence (starts null): a warp a token, so that the slots' rows, which are most of
+ * what moves, are all under way at once. */
+template <typename T, bool kWide, int W>
+__global__ void __launch_bounds__(kThreads) conv_step_kernel(const __grid_constant__ ConvParams p) {
+    using L = Lane<T, kWide>;
+    constexpr int C = L::C;
+    __shared__ Weights<C, 32> weights;
+    const uint32_t lane = threadIdx.x & 31, t = blockIdx.x * (kThreads / 32) + threadIdx.x / 32, c0 = (blockIdx.y * 32 + lane) * C;
+    const bool live = c0 < p.channels && t < p.tokens;
+    int64_t slot = -1;
+    bool fresh = false;
+    if (t < p.tokens) {
+        slot = p.slots == nullptr ? (int64_t)t : (int64_t)p.slots[t];
+        fresh = p.fresh != nullptr && p.fresh[t] != 0;
+    }
+    const bool known = slot >= 0 && slot < (int64_t)p.tail_slots;
+    const int64_t rows = slot * p.tails_slot + c0;
+    float win[W][C], out[C], bias[C];
+    if (live) L::unpack(L::fetch(static_cast<const T *>(p.x) + t * p.x_token + c0), win[W - 1]);
+#pragma unroll
+    for (int j = 0; j < W - 1; ++j) {
+#pragma unroll
+        for (int c = 0; c < C; ++c) win[j][c] = 0.0f;
+        if (live && known && !fresh) L::get_tail(p, rows + j * p.tails_row, win[j]);
+    }
+    weights.template fill<W>(p, blockIdx.y * 32 * C);
+#pragma unroll
+    for (int c = 0; c < C; ++c) bias[c] = live && p.bias != nullptr ? load1(p.bias, c0 + c, p.weight_type) : 0.0f;
+    __syncthreads();
+    if (!live) return;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        float v[W];
+#pragma unroll
+        for (int j = 0; j < W; ++j) v[j] = win[j][c];
+        const float s = tap<W>(weights.w[c][lane], bias[c], v);
+        out[c] = !known ? 0.0f : p.silu ? silu(s) : s;
+    }
+    L::put(static_cast<T *>(p.out) + t * p.out_token + c0, out);
+    if (known) {
+#pragma unroll
+        for (int j = 0; j < W - 1; ++j) L::put_tail(p, rows + j * p.tails_row, win[j + 1]);
+    }
 }
 
 template <typename T, bool kWide, int W>
 cudaError_t launch_conv_t(const ConvParams &p, int sms, cudaStream_t stream) {
-    const uint32_t columns = (p.channels + kThreads * (kWide ? 8 : 1) - 1) / (kThreads * (kWide ? 8 : 1));
+    constexpr uint32_t C = Lane<T, kWide>::C;
+    if (p.starts == nullptr) {
+        const uint32_t columns = (p.channels + 32 * C - 1) / (32 * C);
+        return launch(conv_step_kernel<T, kWide, W>, dim3((p.tokens + kThreads / 32 - 1) / (kThreads / 32), columns), kThreads, 0, stream, p);
+    }
+    const uint32_t columns = (p.channels + kThreads * C - 1) / (kThreads * C);
     /* long tiles read fewer rows twice, short ones make more CTAs */
-    uint32_t tile = 32;
+    uint32_t tile = 64;
     while (tile > 1 && (uint64_t)((p.tokens + tile - 1) / tile) * columns < 8u * (uint32_t)sms) tile /= 2;
     const uint32_t tiles = p.tokens == 0 ? 1 : (p.tokens + tile - 1) / tile;
     return launch(conv_kernel<T, kWide, W>, dim3(tiles, columns), kThreads, 0, stream, p, tile);
@@ -217,7 +350,7 @@ cudaError_t launch_conv_w(const ConvParams &p, int sms, cudaStream_t stream) {
 template <typename T>
 cudaError_t launch_conv_x(const ConvParams &p, int sms, cudaStream_t stream) {
     const int64_t x_size = sizeof(T), tail_size = p.tail_type == kBF16 ? 2 : 4;
-    const bool wide = p.channels % 8 == 0 && on16(p.x) && on16(p.out) && on16(p.tails) &&
+    const bool wide = p.channels % (16 / x_size) == 0 && on16(p.x) && on16(p.out) && on16(p.tails) &&
                       (p.tokens <= 1 || (p.x_token * x_size % 16 == 0 && p.out_token * x_size % 16 == 0)) &&
                       (p.tail_slots <= 1 || p.tails_slot * tail_size % 16 == 0) && (p.width <= 2 || p.tails_row * tail_size % 16 == 0);
     return wide ? launch_conv_w<T, true>(p, sms, stream) : launch_conv_w<T, false>(p, sms, stream);

@@ -50,141 +50,197 @@ __device__ __forceinline__ float meet(float v, uint32_t group, bool all, float *
     return v;
 }
 
-/* T: type of x and gate. kWide: eight neighbours to a vector, all rows on
- * 16-byte boundaries; else values `group` apart. kN: eights of values a thread. */
-template <typename T, bool kWide, int kN>
-__global__ void __launch_bounds__(kMaxNormThreads) norm_kernel(const __grid_constant__ NormParams p, const NormShape g) {
-    __shared__ float partial[2][kMaxNormThreads / 32];
-    const uint32_t tid = threadIdx.x, r = tid / g.group, t = tid % g.group;
-    const uint64_t row = (uint64_t)blockIdx.x * g.rows + r;
-    const uint32_t token = (uint32_t)(row / p.heads), head = (uint32_t)(row % p.heads);
-    const bool live = r < g.rows && row < (uint64_t)p.tokens * p.heads;
-    const uint32_t D = live ? p.dim : 0;
-    const T *x = static_cast<const T *>(p.x) + token * p.x_token + head * p.x_head;
-    const T *gate = static_cast<const T *>(p.gate) + token * p.gate_token + head * p.gate_head;
-    const int64_t res = token * p.residual_token + head * p.residual_head;
-    auto at = [&](int i, int j) { return kWide ? ((uint32_t)i * g.group + t) * 8 + j : ((uint32_t)(i * 8 + j)) * g.group + t; };
-
-    float h[kN][8], z[kN][8];
+/* Eight values of a row as they are in memory (kWide: neighbours, in one or two 16-byte vectors; else values
+ * `step` apart): fetched ahead, and FP32 when they are used. */
+template <typename T, bool kWide>
+struct Eight;
+template <>
+struct Eight<__nv_bfloat16, true> {
+    uint4 w;
+    __device__ __forceinline__ void fetch(const __nv_bfloat16 *p, uint32_t, uint32_t) { w = __ldcg(reinterpret_cast<const uint4 *>(p)); }
+    __device__ __forceinline__ void get(float (&v)[8]) const { unpack8(w, v); }
+};
+template <>
+struct Eight<float, true> {
+    float4 a, b;
+    __device__ __forceinline__ void fetch(const float *p, uint32_t, uint32_t) {
+        a = __ldcg(reinterpret_cast<const float4 *>(p));
+        b = __ldcg(reinterpret_cast<const float4 *>(p) + 1);
+    }
+    __device__ __forceinline__ void get(float (&v)[8]) const {
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    }
+};
+template <typename T>
+struct Eight<T, false> {
+    float x[8];
+    __device__ __forceinline__ void fetch(const T *p, uint32_t step, uint32_t left) {
 #pragma unroll
-    for (int i = 0; i < kN; ++i) {
-        if (kWide) {
+        for (int j = 0; j < 8; ++j) x[j] = (uint32_t)j * step < left ? load1(p + j * step) : 0.0f;
+    }
+    __device__ __forceinline__ void get(float (&v)[8]) const {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = x[j];
+    }
+};
+
+constexpr uint32_t kSmall = 256;
+
+/* T: type of x and gate; R: of the residual. kWide: eight neighbours to a vector, all rows on 16-byte
+ * boundaries; else values `group` apart. kN: eights of values a thread. kAhead: CTAs of up to kSmall
+ * threads, which have the registers to fetch the next row's values while one's meet. */
+template <typename T, typename R, bool kWide, int kN, bool kAhead>
+__global__ void __launch_bounds__(kAhead ? kSmall : kMaxNormThreads, kAhead ? 3 : 1) norm_kernel(const __grid_constant__ NormParams p, const NormShape g) {
+    __shared__ float partial[2][kMaxNormThreads / 32];
+    const uint32_t tid = threadIdx.x, r = tid / g.group, t = tid % g.group, rows = p.tokens * p.heads;
+    const uint32_t step = kWide ? 1 : g.group; /* from one of a thread's eight values to the next */
+    auto at = [&](int i) { return kWide ? (i * g.group + t) * 8 : i * 8 * g.group + t; };
+    auto left = [&](int i) { return p.dim > at(i) ? p.dim - at(i) : 0u; };
+
+    float w[kN][8];
+    if (p.weight != nullptr) {
+#pragma unroll
+        for (int i = 0; i < kN; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) w[i][j] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kN; ++i) {
+            if (kWide) {
+                if (left(i)) load8(p.weight, at(i), p.weight_type, w[i]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (j * step < left(i)) w[i][j] = load1(p.weight, at(i) + j * step, p.weight_type);
+            }
+        }
+    }
+    Eight<T, kWide> x[kN], z[kN];
+    Eight<R, kWide> e[kN];
+    auto fetch = [&](uint32_t row) {
+        if (r >= g.rows || row >= rows) return;
+        const uint32_t token = row / p.heads, head = row - token * p.heads;
+        const T *from = static_cast<const T *>(p.x) + token * p.x_token + head * p.x_head;
+        const T *gate = static_cast<const T *>(p.gate) + token * p.gate_token + head * p.gate_head;
+        const R *res = static_cast<const R *>(p.residual) + token * p.residual_token + head * p.residual_head;
+#pragma unroll
+        for (int i = 0; i < kN; ++i)
+            if (left(i)) x[i].fetch(from + at(i), step, left(i));
+        if (p.residual != nullptr) {
+#pragma unroll
+            for (int i = 0; i < kN; ++i)
+                if (left(i)) e[i].fetch(res + at(i), step, left(i));
+        }
+        if (p.gate != nullptr) {
+#pragma unroll
+            for (int i = 0; i < kN; ++i)
+                if (left(i)) z[i].fetch(gate + at(i), step, left(i));
+        }
+    };
+    uint32_t row = blockIdx.x * g.rows + r;
+    if (kAhead) fetch(row);
+    for (uint32_t first = blockIdx.x * g.rows; first < rows; first += gridDim.x * g.rows, row += gridDim.x * g.rows) {
+        if (!kAhead) fetch(row);
+        const bool live = r < g.rows && row < rows;
+        const uint32_t token = row / p.heads, head = row - token * p.heads;
+        float h[kN][8], gate[kN][8];
+#pragma unroll
+        for (int i = 0; i < kN; ++i) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) h[i][j] = 0.0f;
-            if (at(i, 0) < D) load8(x + at(i, 0), h[i]);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) h[i][j] = at(i, j) < D ? load1(x + at(i, j)) : 0.0f;
+            if (live && left(i)) x[i].get(h[i]);
         }
-    }
-    if (p.gate != nullptr) {
+        if (p.gate != nullptr) {
 #pragma unroll
-        for (int i = 0; i < kN; ++i) {
-            if (kWide) {
-                if (at(i, 0) < D) load8(gate + at(i, 0), z[i]);
-            } else {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) z[i][j] = at(i, j) < D ? load1(gate + at(i, j)) : 0.0f;
-            }
+            for (int i = 0; i < kN; ++i) z[i].get(gate[i]);
         }
-    }
-    if (p.residual != nullptr) {
+        if (p.residual != nullptr && live) {
+            R *res = static_cast<R *>(p.residual) + token * p.residual_token + head * p.residual_head;
 #pragma unroll
-        for (int i = 0; i < kN; ++i) {
-            if (kWide) {
-                if (at(i, 0) < D) {
+            for (int i = 0; i < kN; ++i)
+                if (left(i)) {
                     float v[8];
-                    load8(p.residual, res + at(i, 0), p.residual_type, v);
+                    e[i].get(v);
 #pragma unroll
                     for (int j = 0; j < 8; ++j) h[i][j] += v[j];
-                    store8(p.residual, res + at(i, 0), p.residual_type, h[i]);
-                }
-            } else {
+                    if (kWide) {
+                        store8(res + at(i), h[i]);
+                    } else {
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (at(i, j) < D) {
-                        h[i][j] += load1(p.residual, res + at(i, j), p.residual_type);
-                        store1(p.residual, res + at(i, j), p.residual_type, h[i][j]);
+                        for (int j = 0; j < 8; ++j)
+                            if (j * step < left(i)) store1(res + at(i) + j * step, h[i][j]);
                     }
-            }
+                }
         }
-    }
-    float sum = 0.0f;
+        if (kAhead) fetch(row + gridDim.x * g.rows);
+        float sum = 0.0f;
 #pragma unroll
-    for (int i = 0; i < kN; ++i)
+        for (int i = 0; i < kN; ++i)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) sum = fmaf(h[i][j], h[i][j], sum);
-    sum = meet<false>(sum, g.group, false, partial[0]);
-    const float f = rsqrtf(sum / (float)p.dim + p.eps);
+            for (int j = 0; j < 8; ++j) sum = fmaf(h[i][j], h[i][j], sum);
+        sum = meet<false>(sum, g.group, false, partial[0]);
+        const float f = rsqrtf(sum / (float)p.dim + p.eps);
 
-    float top = 0.0f;
+        float top = 0.0f;
 #pragma unroll
-    for (int i = 0; i < kN; ++i) {
-        float w[8];
-        if (p.weight != nullptr) {
-            if (kWide) {
-                if (at(i, 0) < D) load8(p.weight, at(i, 0), p.weight_type, w);
-            } else {
+        for (int i = 0; i < kN; ++i)
 #pragma unroll
-                for (int j = 0; j < 8; ++j) w[j] = at(i, j) < D ? load1(p.weight, at(i, j), p.weight_type) : 0.0f;
+            for (int j = 0; j < 8; ++j) {
+                float y = h[i][j] * f;
+                if (p.weight != nullptr) y *= w[i][j];
+                if (p.gate != nullptr) y *= silu(gate[i][j]);
+                h[i][j] = y;
+                if (live && (uint32_t)j * step < left(i)) top = larger(top, fabsf(y));
             }
-        }
+        const int64_t out = token * p.out_token + head * p.out_head;
+        if (p.out_type == kE4M3) {
+            top = meet<true>(top, g.group, g.token != 0, partial[1]);
+            float scale = top / 448.0f;
+            if (scale < 0x1p-126f) scale = 0x1p-126f; /* not for a NaN */
+            const float inv = 1.0f / scale;
+            if (live && t == 0 && head == 0) p.scales[token] = scale;
+            uint8_t *o = static_cast<uint8_t *>(p.out) + out;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            float y = h[i][j] * f;
-            if (p.weight != nullptr) y *= w[j];
-            if (p.gate != nullptr) y *= silu(z[i][j]);
-            h[i][j] = y;
-            if (at(i, kWide ? 0 : j) < D) top = larger(top, fabsf(y));
-        }
-    }
-    const int64_t out = token * p.out_token + head * p.out_head;
-    if (p.out_type == kE4M3) {
-        top = meet<true>(top, g.group, g.token != 0, partial[1]);
-        float scale = top / 448.0f;
-        if (scale < 0x1p-126f) scale = 0x1p-126f; /* not for a NaN */
-        const float inv = 1.0f / scale;
-        if (live && t == 0 && head == 0) p.scales[token] = scale;
-        uint8_t *o = static_cast<uint8_t *>(p.out) + out;
-#pragma unroll
-        for (int i = 0; i < kN; ++i) {
-            if (kWide) {
-                if (at(i, 0) < D) {
-                    uint32_t w[4];
+            for (int i = 0; i < kN; ++i) {
+                if (!live || !left(i)) continue;
+                if (kWide) {
+                    uint32_t b[4];
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
-                        w[j] = __nv_cvt_float2_to_fp8x2(make_float2(h[i][2 * j] * inv, h[i][2 * j + 1] * inv), __NV_SATFINITE, __NV_E4M3);
-                    *reinterpret_cast<uint2 *>(o + at(i, 0)) = make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
+                        b[j] = __nv_cvt_float2_to_fp8x2(make_float2(h[i][2 * j] * inv, h[i][2 * j + 1] * inv), __NV_SATFINITE, __NV_E4M3);
+                    *reinterpret_cast<uint2 *>(o + at(i)) = make_uint2(b[0] | (b[1] << 16), b[2] | (b[3] << 16));
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        if (j * step < left(i)) o[at(i) + j * step] = __nv_cvt_float_to_fp8(h[i][j] * inv, __NV_SATFINITE, __NV_E4M3);
                 }
-            } else {
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (at(i, j) < D) o[at(i, j)] = __nv_cvt_float_to_fp8(h[i][j] * inv, __NV_SATFINITE, __NV_E4M3);
             }
-        }
-        return;
-    }
-#pragma unroll
-    for (int i = 0; i < kN; ++i) {
-        if (kWide) {
-            if (at(i, 0) < D) store8(p.out, out + at(i, 0), p.out_type, h[i]);
         } else {
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (at(i, j) < D) store1(p.out, out + at(i, j), p.out_type, h[i][j]);
+            for (int i = 0; i < kN; ++i) {
+                if (!live || !left(i)) continue;
+                if (kWide) {
+                    store8(p.out, out + at(i), p.out_type, h[i]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        if (j * step < left(i)) store1(p.out, out + at(i) + j * step, p.out_type, h[i][j]);
+                }
+            }
         }
+        if (g.group > 32 || g.token) __syncthreads(); /* `partial` is free again */
     }
 }
 
-template <typename T, bool kWide, int kN>
-cudaError_t launch_norm_t(const NormParams &p, cudaStream_t stream) {
+template <typename T, typename R, bool kWide, int kN, bool kAhead>
+cudaError_t launch_norm_t(const NormParams &p, int sms, cudaStream_t stream) {
     NormShape g;
     g.group = norm_group(p.dim, 8 * kN);
     g.token = p.out_type == kE4M3 && p.heads > 1;
     g.rows = g.token ? p.heads : g.group >= 128 ? 1 : 128 / g.group;
     const uint32_t block = (g.group * g.rows + 31) / 32 * 32;
-    const uint64_t rows = (uint64_t)p.tokens * p.heads, grid = (rows + g.rows - 1) / g.rows;
-    return launch(norm_kernel<T, kWide, kN>, dim3((uint32_t)grid), block, 0, stream, p, g);
+    /* as many CTAs as run at once, each with rows in turn */
+    const uint32_t all = (p.tokens * p.heads + g.rows - 1) / g.rows, most = (uint32_t)sms * ((kAhead ? 3 * kSmall : kMaxNormThreads) / block);
+    return launch(norm_kernel<T, R, kWide, kN, kAhead>, dim3(all < most ? all : most), block, 0, stream, p, g);
 }
 
 /* rows of an operand that all start on a 16-byte boundary (8 bytes of 8-bit values) */
@@ -196,23 +252,28 @@ bool wide_rows(const void *p, int64_t token, int64_t head, const NormParams &n, 
 }
 
 template <typename T>
-cudaError_t launch_norm_x(const NormParams &p, cudaStream_t stream) {
+cudaError_t launch_norm_x(const NormParams &p, int sms, cudaStream_t stream) {
     auto size = [](int type) { return type == kF32 ? 4 : type == kBF16 ? 2 : 1; };
     const bool wide = p.dim % 8 == 0 && wide_rows(p.x, p.x_token, p.x_head, p, sizeof(T)) &&
                       wide_rows(p.gate, p.gate_token, p.gate_head, p, sizeof(T)) &&
                       wide_rows(p.residual, p.residual_token, p.residual_head, p, size(p.residual_type)) &&
                       wide_rows(p.out, p.out_token, p.out_head, p, size(p.out_type)) && on16(p.weight);
     /* eight values a thread, or sixteen where a CTA would have too few threads */
-    const bool two = norm_threads(p, 8) > kMaxNormThreads;
-    auto *launch = wide ? two ? launch_norm_t<T, true, 2> : launch_norm_t<T, true, 1>
-                        : two ? launch_norm_t<T, false, 2> : launch_norm_t<T, false, 1>;
-    return launch(p, stream);
+    const uint64_t threads = norm_threads(p, 8);
+    auto pick = [&](auto r) {
+        using R = decltype(r);
+        if (threads <= kSmall) return wide ? launch_norm_t<T, R, true, 1, true> : launch_norm_t<T, R, false, 1, true>;
+        if (threads <= kMaxNormThreads) return wide ? launch_norm_t<T, R, true, 1, false> : launch_norm_t<T, R, false, 1, false>;
+        return wide ? launch_norm_t<T, R, true, 2, false> : launch_norm_t<T, R, false, 2, false>;
+    };
+    auto *launch = p.residual != nullptr && p.residual_type == kBF16 ? pick(__nv_bfloat16()) : pick(float());
+    return launch(p, sms, stream);
 }
 
 }  // namespace
 
-cudaError_t launch_norm(const NormParams &p, int, cudaStream_t stream) {
-    return p.type == kBF16 ? launch_norm_x<__nv_bfloat16>(p, stream) : launch_norm_x<float>(p, stream);
+cudaError_t launch_norm(const NormParams &p, int sms, cudaStream_t stream) {
+    return p.type == kBF16 ? launch_norm_x<__nv_bfloat16>(p, sms, stream) : launch_norm_x<float>(p, sms, stream);
 }
 
 }  // namespace ops

@@ -75,7 +75,7 @@ __device__ __forceinline__ void store1(void *p, int64_t i, int type, float x) {
  * rounded to fewer). e^-x is infinite for x < -88.7, where the result is -0. */
 __device__ __forceinline__ float silu(float x) { return __fdividef(x, 1.0f + __expf(-x)); }
 
-__host__ inline bool on16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+__host__ __device__ inline bool on16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 }  // namespace ops
 }  // namespace gdn
