@@ -18,6 +18,8 @@ namespace ops {
 
 namespace {
 
+constexpr uint32_t kSmall = 256; /* threads of the CTAs that fetch ahead */
+
 struct NormShape {
     uint32_t group; /* threads of a row: a power of two up to 32, or a multiple of 32 */
     uint32_t rows;  /* rows of a CTA */
@@ -35,17 +37,29 @@ __device__ __forceinline__ float join(float a, float b) {
 }
 /* Over the `group` threads of this thread's row: every one of them gets it.
  * `all` (part of a CTA's threads may have no row): over the whole CTA. */
-template <bool kMax>
+template <bool kMax, bool kFewWarps>
 __device__ __forceinline__ float meet(float v, uint32_t group, bool all, float *partial) {
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const uint32_t width = all || group > 32 ? 32 : group;
-    for (uint32_t o = width / 2; o > 0; o >>= 1) v = join<kMax>(v, __shfl_xor_sync(0xffffffffu, v, o));
-    if (width == 32 && (all || group > 32)) {
+    if (group >= 32 || all) {
+#pragma unroll
+        for (uint32_t o = 16; o > 0; o >>= 1) v = join<kMax>(v, __shfl_xor_sync(0xffffffffu, v, o));
+    } else {
+        for (uint32_t o = group / 2; o > 0; o >>= 1) v = join<kMax>(v, __shfl_xor_sync(0xffffffffu, v, o));
+    }
+    if (all || group > 32) {
         if (lane == 0) partial[warp] = v;
         __syncthreads();
         const uint32_t first = all ? 0 : tid / group * (group / 32), n = all ? blockDim.x / 32 : group / 32;
-        v = lane < n ? partial[first + lane] : 0.0f;
-        for (uint32_t o = 16; o > 0; o >>= 1) v = join<kMax>(v, __shfl_xor_sync(0xffffffffu, v, o));
+        if (kFewWarps) {
+            v = partial[first];
+#pragma unroll
+            for (uint32_t i = 1; i < kSmall / 32; ++i)
+                if (i < n) v = join<kMax>(v, partial[first + i]);
+        } else {
+            v = lane < n ? partial[first + lane] : 0.0f;
+#pragma unroll
+            for (uint32_t o = 16; o > 0; o >>= 1) v = join<kMax>(v, __shfl_xor_sync(0xffffffffu, v, o));
+        }
     }
     return v;
 }
@@ -84,8 +98,6 @@ struct Eight<T, false> {
     }
 };
 
-constexpr uint32_t kSmall = 256;
-
 /* T: type of x and gate; R: of the residual. kWide: eight neighbours to a vector, all rows on 16-byte
  * boundaries; else values `group` apart. kN: eights of values a thread. kAhead: CTAs of up to kSmall
  * threads, which have the registers to fetch the next row's values while one's meet. */
@@ -116,32 +128,35 @@ __global__ void __launch_bounds__(kAhead ? kSmall : kMaxNormThreads, kAhead ? 3 
     }
     Eight<T, kWide> x[kN], z[kN];
     Eight<R, kWide> e[kN];
-    auto fetch = [&](uint32_t row) {
+    const float per_dim = 1.0f / (float)p.dim;
+    /* this thread's row, and the step to its next one */
+    uint32_t row = blockIdx.x * g.rows + r, token = row / p.heads, head = row - token * p.heads;
+    const uint32_t row_step = gridDim.x * g.rows, token_step = row_step / p.heads, head_step = row_step - token_step * p.heads;
+    auto fetch = [&]() {
         if (r >= g.rows || row >= rows) return;
-        const uint32_t token = row / p.heads, head = row - token * p.heads;
         const T *from = static_cast<const T *>(p.x) + token * p.x_token + head * p.x_head;
-        const T *gate = static_cast<const T *>(p.gate) + token * p.gate_token + head * p.gate_head;
-        const R *res = static_cast<const R *>(p.residual) + token * p.residual_token + head * p.residual_head;
 #pragma unroll
         for (int i = 0; i < kN; ++i)
             if (left(i)) x[i].fetch(from + at(i), step, left(i));
         if (p.residual != nullptr) {
+            const R *res = static_cast<const R *>(p.residual) + token * p.residual_token + head * p.residual_head;
 #pragma unroll
             for (int i = 0; i < kN; ++i)
                 if (left(i)) e[i].fetch(res + at(i), step, left(i));
         }
         if (p.gate != nullptr) {
+            const T *gate = static_cast<const T *>(p.gate) + token * p.gate_token + head * p.gate_head;
 #pragma unroll
             for (int i = 0; i < kN; ++i)
                 if (left(i)) z[i].fetch(gate + at(i), step, left(i));
         }
     };
-    uint32_t row = blockIdx.x * g.rows + r;
-    if (kAhead) fetch(row);
-    for (uint32_t first = blockIdx.x * g.rows; first < rows; first += gridDim.x * g.rows, row += gridDim.x * g.rows) {
-        if (!kAhead) fetch(row);
-        const bool live = r < g.rows && row < rows;
-        const uint32_t token = row / p.heads, head = row - token * p.heads;
+    if (kAhead) fetch();
+    for (uint32_t first = blockIdx.x * g.rows; first < rows; first += row_step) {
+        if (!kAhead) fetch();
+        const bool live = r < g.rows && row < rows, first_head = head == 0;
+        const uint32_t this_token = token;
+        const int64_t out = token * p.out_token + head * p.out_head;
         float h[kN][8], gate[kN][8];
 #pragma unroll
         for (int i = 0; i < kN; ++i) {
@@ -171,33 +186,44 @@ __global__ void __launch_bounds__(kAhead ? kSmall : kMaxNormThreads, kAhead ? 3 
                     }
                 }
         }
-        if (kAhead) fetch(row + gridDim.x * g.rows);
+        row += row_step, token += token_step, head += head_step;
+        if (head >= p.heads) head -= p.heads, ++token;
+        if (kAhead) fetch();
         float sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < kN; ++i)
 #pragma unroll
             for (int j = 0; j < 8; ++j) sum = fmaf(h[i][j], h[i][j], sum);
-        sum = meet<false>(sum, g.group, false, partial[0]);
-        const float f = rsqrtf(sum / (float)p.dim + p.eps);
-
-        float top = 0.0f;
+        sum = meet<false, kAhead>(sum, g.group, false, partial[0]);
+        const float f = rsqrtf(fmaf(sum, per_dim, p.eps));
 #pragma unroll
         for (int i = 0; i < kN; ++i)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                float y = h[i][j] * f;
-                if (p.weight != nullptr) y *= w[i][j];
-                if (p.gate != nullptr) y *= silu(gate[i][j]);
-                h[i][j] = y;
-                if (live && (uint32_t)j * step < left(i)) top = larger(top, fabsf(y));
-            }
-        const int64_t out = token * p.out_token + head * p.out_head;
+            for (int j = 0; j < 8; ++j) h[i][j] *= f;
+        if (p.weight != nullptr) {
+#pragma unroll
+            for (int i = 0; i < kN; ++i)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) h[i][j] *= w[i][j];
+        }
+        if (p.gate != nullptr) {
+#pragma unroll
+            for (int i = 0; i < kN; ++i)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) h[i][j] *= silu(gate[i][j]);
+        }
         if (p.out_type == kE4M3) {
-            top = meet<true>(top, g.group, g.token != 0, partial[1]);
+            float top = 0.0f;
+#pragma unroll
+            for (int i = 0; i < kN; ++i)
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (live && (uint32_t)j * step < left(i)) top = larger(top, fabsf(h[i][j]));
+            top = meet<true, kAhead>(top, g.group, g.token != 0, partial[1]);
             float scale = top / 448.0f;
             if (scale < 0x1p-126f) scale = 0x1p-126f; /* not for a NaN */
             const float inv = 1.0f / scale;
-            if (live && t == 0 && head == 0) p.scales[token] = scale;
+            if (live && t == 0 && first_head) p.scales[this_token] = scale;
             uint8_t *o = static_cast<uint8_t *>(p.out) + out;
 #pragma unroll
             for (int i = 0; i < kN; ++i) {
