@@ -101,8 +101,9 @@ struct Eight<T, false> {
 /* T: type of x and gate; R: of the residual. kWide: eight neighbours to a vector, all rows on 16-byte
  * boundaries; else values `group` apart. kN: eights of values a thread. kAhead: CTAs of up to kSmall
  * threads, which have the registers to fetch the next row's values while one's meet. */
+constexpr int ctas_of(int n) { return n == 1 ? 3 : n == 2 ? 2 : 1; } /* that fit an SM with their registers */
 template <typename T, typename R, bool kWide, int kN, bool kAhead>
-__global__ void __launch_bounds__(kAhead ? kSmall : kMaxNormThreads, kAhead ? 3 : 1) norm_kernel(const __grid_constant__ NormParams p, const NormShape g) {
+__global__ void __launch_bounds__(kAhead ? kSmall : kMaxNormThreads, kAhead ? ctas_of(kN) : 1) norm_kernel(const __grid_constant__ NormParams p, const NormShape g) {
     __shared__ float partial[2][kMaxNormThreads / 32];
     const uint32_t tid = threadIdx.x, r = tid / g.group, t = tid % g.group, rows = p.tokens * p.heads;
     const uint32_t step = kWide ? 1 : g.group; /* from one of a thread's eight values to the next */
@@ -265,7 +266,7 @@ cudaError_t launch_norm_t(const NormParams &p, int sms, cudaStream_t stream) {
     g.rows = g.token ? p.heads : g.group >= 128 ? 1 : 128 / g.group;
     const uint32_t block = (g.group * g.rows + 31) / 32 * 32;
     /* as many CTAs as run at once, each with rows in turn */
-    const uint32_t all = (p.tokens * p.heads + g.rows - 1) / g.rows, most = (uint32_t)sms * ((kAhead ? 3 * kSmall : kMaxNormThreads) / block);
+    const uint32_t all = (p.tokens * p.heads + g.rows - 1) / g.rows, most = (uint32_t)sms * ((kAhead ? ctas_of(kN) * kSmall : kMaxNormThreads) / block);
     return launch(norm_kernel<T, R, kWide, kN, kAhead>, dim3(all < most ? all : most), block, 0, stream, p, g);
 }
 
@@ -285,11 +286,12 @@ cudaError_t launch_norm_x(const NormParams &p, int sms, cudaStream_t stream) {
                       wide_rows(p.residual, p.residual_token, p.residual_head, p, size(p.residual_type)) &&
                       wide_rows(p.out, p.out_token, p.out_head, p, size(p.out_type)) && on16(p.weight);
     /* eight values a thread, or sixteen where a CTA would have too few threads */
-    const uint64_t threads = norm_threads(p, 8);
     auto pick = [&](auto r) {
         using R = decltype(r);
-        if (threads <= kSmall) return wide ? launch_norm_t<T, R, true, 1, true> : launch_norm_t<T, R, false, 1, true>;
-        if (threads <= kMaxNormThreads) return wide ? launch_norm_t<T, R, true, 1, false> : launch_norm_t<T, R, false, 1, false>;
+        if (wide && norm_threads(p, 16) <= kSmall) return launch_norm_t<T, R, true, 2, true>;
+        if (wide && norm_threads(p, 32) <= kSmall) return launch_norm_t<T, R, true, 4, true>;
+        if (!wide && norm_threads(p, 8) <= kSmall) return launch_norm_t<T, R, false, 1, true>;
+        if (norm_threads(p, 8) <= kMaxNormThreads) return wide ? launch_norm_t<T, R, true, 1, false> : launch_norm_t<T, R, false, 1, false>;
         return wide ? launch_norm_t<T, R, true, 2, false> : launch_norm_t<T, R, false, 2, false>;
     };
     auto *launch = p.residual != nullptr && p.residual_type == kBF16 ? pick(__nv_bfloat16()) : pick(float());
