@@ -91,16 +91,59 @@ struct Lane {
     }
 };
 
-/* A channel's weights in shared memory: four floats, the last one meets the token itself (a
- * shorter width has zeros in front, which nobody reads). Rows of kThreads + 1, so that
- * threads that fill neighbouring channels use different banks. */
+/* Two FP32 values as one operand: their products and sums are rounded as by themselves. */
+__device__ __forceinline__ uint64_t pair_of(float lo, float hi) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ void split(uint64_t v, float &lo, float &hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+/* silu of both, as silu() */
+__device__ __forceinline__ uint64_t silu2(uint64_t x) {
+    float a, b;
+    split(mul2(x, pair_of(-1.44269504f, -1.44269504f)), a, b);
+    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(a));
+    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(b));
+    split(add2(pair_of(a, b), pair_of(1.0f, 1.0f)), a, b);
+    asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(a));
+    asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(b));
+    return mul2(x, pair_of(a, b));
+}
+
+/* The weights of a CTA's channels in shared memory, by pairs of channels: four taps each, the last one
+ * meets the token itself (a shorter width has zeros in front, which nobody reads). One more row than
+ * threads, so that threads that fill neighbouring channels use different banks. */
 template <int C, uint32_t kLanes>
 struct Weights {
-    float4 w[C][kLanes + 1];
+    float4 pairs[(C + 1) / 2][2][kLanes + 1]; /* taps 0 and 1 of both channels, taps 2 and 3 */
+    __device__ __forceinline__ uint64_t tap(int pair, int j, uint32_t lane) const {
+        const float4 e = pairs[pair][j >> 1][lane];
+        return j & 1 ? pair_of(e.z, e.w) : pair_of(e.x, e.y);
+    }
+    /* the four of channel c */
+    __device__ __forceinline__ float4 of(int c, uint32_t lane) const {
+        const float4 a = pairs[c / 2][0][lane], b = pairs[c / 2][1][lane];
+        return c & 1 ? make_float4(a.y, a.w, b.y, b.w) : make_float4(a.x, a.z, b.x, b.z);
+    }
     template <int W>
     __device__ __forceinline__ void fill(const ConvParams &p, uint32_t first) {
         for (uint32_t i = threadIdx.x; i < kLanes * C; i += blockDim.x) {
-            const uint32_t c = first + i;
+            const uint32_t c = first + i, of = i % C;
             float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
             if (c < p.channels) {
                 if (W == 4 && p.weight_type == kF32 && on16(p.weight)) {
@@ -111,7 +154,8 @@ struct Weights {
                     for (int j = 0; j < W; ++j) v[4 - W + j] = load1(p.weight, (int64_t)c * W + j, p.weight_type);
                 }
             }
-            w[i % C][i / C] = make_float4(v[0], v[1], v[2], v[3]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) reinterpret_cast<float *>(&pairs[of / 2][j >> 1][i / C])[(j & 1) * 2 + (of & 1)] = v[j];
         }
     }
 };
@@ -193,7 +237,7 @@ __global__ void __launch_bounds__(kThreads) conv_kernel(const __grid_constant__ 
 #pragma unroll
                         for (int j = 0; j < W - 1; ++j) v[j] = win[j][c];
                         v[W - 1] = in[c];
-                        const float s = tap<W>(weights.w[c][tid], bias[c], v);
+                        const float s = tap<W>(weights.of(c, tid), bias[c], v);
                         out[c] = p.silu ? silu(s) : s;
 #pragma unroll
                         for (int j = 0; j < W - 1; ++j) win[j][c] = v[j + 1];
@@ -224,33 +268,44 @@ __global__ void __launch_bounds__(kThreads) conv_kernel(const __grid_constant__ 
 #pragma unroll
                     for (int a = 0; a < kAhead; ++a) next[a] = L::fetch(x + (int64_t)min(t + kAhead + a, stop - 1) * p.x_token);
                 }
-                /* two channels (one) at a time: a word of each input, a word of each output */
                 uint32_t result[kAhead][4];
-                constexpr int kWords = kWide ? 4 : 1, kPer = C / kWords;
+                auto word = [](const uint4 &v, int q) { return q == 0 ? v.x : q == 1 ? v.y : q == 2 ? v.z : v.w; };
+                if constexpr (kWide) {
+                    /* two channels at a time: a word of 16-bit inputs, two of 32 bits */
 #pragma unroll
-                for (int q = 0; q < kWords; ++q) {
-                    float out[kAhead][2];
+                    for (int q = 0; q < C / 2; ++q) {
+                        uint64_t v[W - 1 + kAhead], w[W];
 #pragma unroll
-                    for (int e = 0; e < kPer; ++e) {
-                        const int c = q * kPer + e;
-                        const float4 w = weights.w[c][tid];
-                        float v[W - 1 + kAhead];
+                        for (int j = 0; j < W; ++j) w[j] = weights.tap(q, 4 - W + j, tid);
 #pragma unroll
-                        for (int j = 0; j < W - 1 + kAhead; ++j) {
-                            const uint32_t word = q == 0 ? in[j].x : q == 1 ? in[j].y : q == 2 ? in[j].z : in[j].w;
-                            v[j] = kPer == 1 ? __uint_as_float(word) : e == 0 ? low_bf16(word) : high_bf16(word);
-                        }
+                        for (int j = 0; j < W - 1 + kAhead; ++j)
+                            v[j] = C == 8 ? pair_of(low_bf16(word(in[j], q)), high_bf16(word(in[j], q)))
+                                          : pair_of(__uint_as_float(word(in[j], 2 * q)), __uint_as_float(word(in[j], 2 * q + 1)));
+                        const uint64_t b = pair_of(bias[2 * q], bias[2 * q + 1]);
 #pragma unroll
                         for (int a = 0; a < kAhead; ++a) {
-                            float u[W];
+                            uint64_t o = b;
 #pragma unroll
-                            for (int j = 0; j < W; ++j) u[j] = v[a + j];
-                            const float s = tap<W>(w, bias[c], u);
-                            out[a][e] = p.silu ? silu(s) : s;
+                            for (int j = 0; j < W; ++j) o = fma2(w[j], v[a + j], o);
+                            if (p.silu) o = silu2(o);
+                            float lo, hi;
+                            split(o, lo, hi);
+                            if (C == 8)
+                                result[a][q] = pack_bf16(lo, hi);
+                            else
+                                result[a][2 * q] = __float_as_uint(lo), result[a][2 * q + 1] = __float_as_uint(hi);
                         }
                     }
+                } else {
+                    const float4 w = weights.of(0, tid);
 #pragma unroll
-                    for (int a = 0; a < kAhead; ++a) result[a][q] = kPer == 2 ? pack_bf16(out[a][0], out[a][1]) : __float_as_uint(out[a][0]);
+                    for (int a = 0; a < kAhead; ++a) {
+                        float u[W];
+#pragma unroll
+                        for (int j = 0; j < W; ++j) u[j] = __uint_as_float(in[a + j].x);
+                        const float o = tap<W>(w, bias[0], u);
+                        result[a][0] = __float_as_uint(p.silu ? silu(o) : o);
+                    }
                 }
 #pragma unroll
                 for (int a = 0; a < kAhead; ++a)
@@ -313,7 +368,7 @@ __global__ void __launch_bounds__(kThreads) conv_step_kernel(const __grid_consta
         float v[W];
 #pragma unroll
         for (int j = 0; j < W; ++j) v[j] = win[j][c];
-        const float s = tap<W>(weights.w[c][lane], bias[c], v);
+        const float s = tap<W>(weights.of(c, lane), bias[c], v);
         out[c] = !known ? 0.0f : p.silu ? silu(s) : s;
     }
     L::put(static_cast<T *>(p.out) + t * p.out_token + c0, out);
