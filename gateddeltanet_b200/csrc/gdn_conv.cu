@@ -21,7 +21,9 @@ namespace ops {
 namespace {
 
 constexpr uint32_t kThreads = 128;
-constexpr int kAhead = 4; /* tokens whose loads are in flight */
+/* Tokens computed together, while the loads of as many more are in flight: with two 64 registers and eight CTAs an SM,
+ * with four 90 and five. 24 ragged prompts of BF16 117 us with two, 122 with four; 4 x 1000 tokens of FP32 48.8 and 43.4. */
+__host__ __device__ constexpr int ahead_of(int channels) { return channels == 8 ? 2 : 4; }
 
 __device__ __forceinline__ uint32_t bound_of(const ConvParams &p, uint32_t n) {
     if (p.starts == nullptr) return n;
@@ -142,20 +144,30 @@ struct Weights {
     }
     template <int W>
     __device__ __forceinline__ void fill(const ConvParams &p, uint32_t first) {
-        for (uint32_t i = threadIdx.x; i < kLanes * C; i += blockDim.x) {
-            const uint32_t c = first + i, of = i % C;
-            float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            if (c < p.channels) {
-                if (W == 4 && p.weight_type == kF32 && on16(p.weight)) {
-                    const float4 e = *reinterpret_cast<const float4 *>(static_cast<const float *>(p.weight) + (size_t)c * 4);
-                    v[0] = e.x, v[1] = e.y, v[2] = e.z, v[3] = e.w;
-                } else {
+        constexpr int kEach = (kLanes * C + kThreads - 1) / kThreads;
+        const bool whole = W == 4 && p.weight_type == kF32 && on16(p.weight);
+        float v[kEach][4];
 #pragma unroll
-                    for (int j = 0; j < W; ++j) v[4 - W + j] = load1(p.weight, (int64_t)c * W + j, p.weight_type);
-                }
+        for (int k = 0; k < kEach; ++k) {
+            const uint32_t i = k * kThreads + threadIdx.x, c = first + i;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[k][j] = 0.0f;
+            if (i >= kLanes * C || c >= p.channels) continue;
+            if (whole) {
+                const float4 e = *reinterpret_cast<const float4 *>(static_cast<const float *>(p.weight) + (size_t)c * 4);
+                v[k][0] = e.x, v[k][1] = e.y, v[k][2] = e.z, v[k][3] = e.w;
+            } else {
+#pragma unroll
+                for (int j = 0; j < W; ++j) v[k][4 - W + j] = load1(p.weight, (int64_t)c * W + j, p.weight_type);
             }
+        }
 #pragma unroll
-            for (int j = 0; j < 4; ++j) reinterpret_cast<float *>(&pairs[of / 2][j >> 1][i / C])[(j & 1) * 2 + (of & 1)] = v[j];
+        for (int k = 0; k < kEach; ++k) {
+            const uint32_t i = k * kThreads + threadIdx.x, of = i % C;
+            if (i < kLanes * C) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) reinterpret_cast<float *>(&pairs[of / 2][j >> 1][i / C])[(j & 1) * 2 + (of & 1)] = v[k][j];
+            }
         }
     }
 };
@@ -172,9 +184,9 @@ __device__ __forceinline__ float tap(const float4 &w, float bias, const float (&
 
 /* T: type of x and y. kWide: 16 bytes of channels a thread. */
 template <typename T, bool kWide, int W>
-__global__ void __launch_bounds__(kThreads) conv_kernel(const __grid_constant__ ConvParams p, const uint32_t tile) {
+__global__ void __launch_bounds__(kThreads, Lane<T, kWide>::C == 8 ? 8 : 1) conv_kernel(const __grid_constant__ ConvParams p, const uint32_t tile) {
     using L = Lane<T, kWide>;
-    constexpr int C = L::C;
+    constexpr int C = L::C, kAhead = ahead_of(C);
     __shared__ Weights<C, kThreads> weights;
     const uint32_t tid = threadIdx.x, c0 = (blockIdx.y * kThreads + tid) * C;
     const bool live = c0 < p.channels;
@@ -388,7 +400,7 @@ cudaError_t launch_conv_t(const ConvParams &p, int sms, cudaStream_t stream) {
     const uint32_t columns = (p.channels + kThreads * C - 1) / (kThreads * C);
     /* long tiles read fewer rows twice, short ones make more CTAs */
     uint32_t tile = 64;
-    while (tile > 1 && (uint64_t)((p.tokens + tile - 1) / tile) * columns < 8u * (uint32_t)sms) tile /= 2;
+    while (tile > 1 && (uint64_t)((p.tokens + tile - 1) / tile) * columns < 4u * (uint32_t)sms) tile /= 2;
     const uint32_t tiles = p.tokens == 0 ? 1 : (p.tokens + tile - 1) / tile;
     return launch(conv_kernel<T, kWide, W>, dim3(tiles, columns), kThreads, 0, stream, p, tile);
 }
