@@ -27,7 +27,7 @@ __host__ __device__ constexpr int ahead_of(int channels) { return channels == 8 
 
 __device__ __forceinline__ uint32_t bound_of(const ConvParams &p, uint32_t n) {
     if (p.starts == nullptr) return n;
-    const int32_t s = p.starts[n];
+    const int32_t s = __ldcg(p.starts + n);
     return s < 0 ? 0u : ((uint32_t)s < p.tokens ? (uint32_t)s : p.tokens);
 }
 
@@ -154,7 +154,7 @@ struct Weights {
             for (int j = 0; j < 4; ++j) v[k][j] = 0.0f;
             if (i >= kLanes * C || c >= p.channels) continue;
             if (whole) {
-                const float4 e = *reinterpret_cast<const float4 *>(static_cast<const float *>(p.weight) + (size_t)c * 4);
+                const float4 e = __ldcg(reinterpret_cast<const float4 *>(static_cast<const float *>(p.weight) + (size_t)c * 4));
                 v[k][0] = e.x, v[k][1] = e.y, v[k][2] = e.z, v[k][3] = e.w;
             } else {
 #pragma unroll
@@ -192,6 +192,8 @@ __global__ void __launch_bounds__(kThreads, Lane<T, kWide>::C == 8 ? 8 : 1) conv
     const bool live = c0 < p.channels;
     const T *x = static_cast<const T *>(p.x) + c0;
     T *y = static_cast<T *>(p.out) + c0;
+    wait_for_previous();
+    let_next_start();
     weights.template fill<W>(p, blockIdx.y * kThreads * C);
     float bias[C];
 #pragma unroll
@@ -211,7 +213,7 @@ __global__ void __launch_bounds__(kThreads, Lane<T, kWide>::C == 8 ? 8 : 1) conv
             continue;
         }
         uint32_t stop = min(end, t1);
-        const int64_t slot = n == 0 || n > p.N ? -1 : p.slots == nullptr ? (int64_t)(n - 1) : (int64_t)p.slots[n - 1];
+        const int64_t slot = n == 0 || n > p.N ? -1 : p.slots == nullptr ? (int64_t)(n - 1) : (int64_t)__ldcg(p.slots + n - 1);
         if (slot < 0 || slot >= (int64_t)p.tail_slots) {
             /* tokens of no sequence, or of one without a slot */
             if (live)
@@ -230,7 +232,7 @@ __global__ void __launch_bounds__(kThreads, Lane<T, kWide>::C == 8 ? 8 : 1) conv
         if (live) {
             if (t == begin) {
                 /* the tokens that meet the slot's rows, one by one */
-                const bool fresh = p.fresh != nullptr && p.fresh[n - 1] != 0;
+                const bool fresh = p.fresh != nullptr && __ldcg(p.fresh + n - 1) != 0;
                 const int64_t rows = slot * p.tails_slot + c0;
                 const uint32_t few = min((uint32_t)(W - 1), end - begin);
                 float win[W - 1][C];
@@ -338,8 +340,8 @@ __global__ void __launch_bounds__(kThreads, Lane<T, kWide>::C == 8 ? 8 : 1) conv
     /* fresh sequences without tokens: nobody else touches their slots */
     if (p.starts != nullptr && p.fresh != nullptr)
         for (uint32_t i = blockIdx.x; i < p.N; i += gridDim.x)
-            if (p.fresh[i] != 0 && bound_of(p, i + 1) <= bound_of(p, i)) {
-                const int64_t slot = p.slots == nullptr ? (int64_t)i : (int64_t)p.slots[i];
+            if (__ldcg(p.fresh + i) != 0 && bound_of(p, i + 1) <= bound_of(p, i)) {
+                const int64_t slot = p.slots == nullptr ? (int64_t)i : (int64_t)__ldcg(p.slots + i);
                 if (live && slot >= 0 && slot < (int64_t)p.tail_slots)
                     for (int j = 0; j < W - 1; ++j) L::put_tail(p, slot * p.tails_slot + j * p.tails_row + c0, zero);
             }
@@ -354,11 +356,13 @@ __global__ void __launch_bounds__(kThreads) conv_step_kernel(const __grid_consta
     __shared__ Weights<C, 32> weights;
     const uint32_t lane = threadIdx.x & 31, t = blockIdx.x * (kThreads / 32) + threadIdx.x / 32, c0 = (blockIdx.y * 32 + lane) * C;
     const bool live = c0 < p.channels && t < p.tokens;
+    wait_for_previous();
+    let_next_start();
     int64_t slot = -1;
     bool fresh = false;
     if (t < p.tokens) {
-        slot = p.slots == nullptr ? (int64_t)t : (int64_t)p.slots[t];
-        fresh = p.fresh != nullptr && p.fresh[t] != 0;
+        slot = p.slots == nullptr ? (int64_t)t : (int64_t)__ldcg(p.slots + t);
+        fresh = p.fresh != nullptr && __ldcg(p.fresh + t) != 0;
     }
     const bool known = slot >= 0 && slot < (int64_t)p.tail_slots;
     const int64_t rows = slot * p.tails_slot + c0;
@@ -395,14 +399,14 @@ cudaError_t launch_conv_t(const ConvParams &p, int sms, cudaStream_t stream) {
     constexpr uint32_t C = Lane<T, kWide>::C;
     if (p.starts == nullptr) {
         const uint32_t columns = (p.channels + 32 * C - 1) / (32 * C);
-        return launch(conv_step_kernel<T, kWide, W>, dim3((p.tokens + kThreads / 32 - 1) / (kThreads / 32), columns), kThreads, 0, stream, p);
+        return launch_overlapped(conv_step_kernel<T, kWide, W>, dim3((p.tokens + kThreads / 32 - 1) / (kThreads / 32), columns), kThreads, 0, stream, p);
     }
     const uint32_t columns = (p.channels + kThreads * C - 1) / (kThreads * C);
     /* long tiles read fewer rows twice, short ones make more CTAs */
     uint32_t tile = 64;
     while (tile > 1 && (uint64_t)((p.tokens + tile - 1) / tile) * columns < 4u * (uint32_t)sms) tile /= 2;
     const uint32_t tiles = p.tokens == 0 ? 1 : (p.tokens + tile - 1) / tile;
-    return launch(conv_kernel<T, kWide, W>, dim3(tiles, columns), kThreads, 0, stream, p, tile);
+    return launch_overlapped(conv_kernel<T, kWide, W>, dim3(tiles, columns), kThreads, 0, stream, p, tile);
 }
 
 template <typename T, bool kWide>

@@ -404,6 +404,8 @@ __global__ void __launch_bounds__(kLinearThreads, 1)
         asm volatile("bar.sync 2, %0;" ::"n"(kLinearThreads) : "memory");
     }
     tc_fence_after();
+    wait_for_previous();
+    let_next_start();
     const uint32_t second = g.columns / 2; /* columns from one accumulator to the other */
 
     if (warp >= kEpilogueWarps) {
@@ -785,12 +787,14 @@ cudaError_t launch_shape(const LinearParams &p, const LinearShape &g, int sms, c
     cfg.blockDim = dim3(kLinearThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = group;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization; /* as launch_overlapped */
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = group;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = group > 1 ? 1 : 0;
+    cfg.numAttrs = group > 1 ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, linear_kernel<kCtas, kFp8, pairs>, p, map_x, map_w, g);
 }
 

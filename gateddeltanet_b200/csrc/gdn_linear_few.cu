@@ -19,7 +19,6 @@ namespace ops {
 namespace {
 
 constexpr uint32_t kMaxWarps = 16;
-constexpr int kAhead = 4; /* steps of k whose loads are in flight */
 
 __device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -61,48 +60,51 @@ __device__ __forceinline__ void products(float (&d)[kGroups][4], const uint4 &lo
     }
 }
 
-/* 16 bytes at byte k of a row of `size` bytes: zeros past its end. The rows
- * themselves are whole 16-byte pieces apart, so the last piece is read whole
- * where it is not the row's own end that cuts it. */
+/* weights: read once */
+__device__ __forceinline__ uint4 load16(const uint8_t *p) {
+    uint4 v;
+    asm volatile("ld.global.cs.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+/* 16 bytes at byte k of a row of `size` bytes, zeros past its end */
 template <bool kFp8>
-__device__ __forceinline__ uint4 piece(const uint8_t *row, uint32_t k, uint32_t size, bool have) {
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (!have || k >= size) return v;
-    if (k + 16 <= size) return __ldcs(reinterpret_cast<const uint4 *>(row + k));
+__device__ __forceinline__ uint4 piece(const uint8_t *row, uint32_t k, uint32_t size) {
+    if (k >= size) return make_uint4(0, 0, 0, 0);
+    if (k + 16 <= size) return __ldcg(reinterpret_cast<const uint4 *>(row + k));
     uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
     for (int i = 0; i < 16; i += kFp8 ? 1 : 2)
         if (k + i < size) {
-            const uint32_t e = kFp8 ? (uint32_t)row[k + i] : (uint32_t)*reinterpret_cast<const unsigned short *>(row + k + i);
+            const uint32_t e = kFp8 ? (uint32_t)__ldcg(row + k + i) : (uint32_t)__ldcg(reinterpret_cast<const unsigned short *>(row + k + i));
             w[i / 4] |= e << (8 * (i % 4));
         }
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+/* Steps of k (64 bytes of a row) at a time, while the next ones' loads are in flight: what 128 registers hold. */
+__host__ __device__ constexpr int ahead_of(int products) { return products == 1 ? 4 : 2; }
+
 /* kGroups: tokens / 8. kPairs (swiglu): a CTA takes 16 rows of either half of W. */
 template <bool kFp8, int kGroups, bool kPairs>
 __global__ void __launch_bounds__(kMaxWarps * 32) linear_few_kernel(const __grid_constant__ LinearParams p) {
     constexpr int kHalves = kPairs ? 2 : 1;
+    constexpr int kAhead = ahead_of(kGroups * kHalves);
     constexpr uint32_t kSums = kHalves * kGroups * 128; /* of a warp */
     extern __shared__ float sums[];
     const uint32_t tid = threadIdx.x, warp = tid >> 5, warps = blockDim.x >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const uint32_t n0 = blockIdx.x * 16, size = p.inputs * (kFp8 ? 1 : 2);
     const uint32_t elem = kFp8 ? 1 : 2;
-    const uint8_t *w[kHalves][2];
-    bool have_w[2], have_x[kGroups];
-    const uint8_t *x[kGroups];
+    wait_for_previous();
+    let_next_start();
+    /* rows past the ends are read as the last one: their sums go nowhere */
+    const uint8_t *w[kHalves][2], *x[kGroups];
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-        have_w[r] = n0 + g + 8 * r < p.outputs;
+    for (int r = 0; r < 2; ++r)
 #pragma unroll
         for (int h = 0; h < kHalves; ++h)
-            w[h][r] = static_cast<const uint8_t *>(p.weight) + (int64_t)(have_w[r] ? h * p.outputs + n0 + g + 8 * r : 0) * p.weight_row * elem;
-    }
+            w[h][r] = static_cast<const uint8_t *>(p.weight) + (h * p.outputs + min(n0 + g + 8 * r, p.outputs - 1)) * p.weight_row * elem + t * 16;
 #pragma unroll
-    for (int n = 0; n < kGroups; ++n) {
-        have_x[n] = g + 8 * n < p.tokens;
-        x[n] = static_cast<const uint8_t *>(p.x) + (int64_t)(have_x[n] ? g + 8 * n : 0) * p.x_row * elem;
-    }
+    for (int n = 0; n < kGroups; ++n) x[n] = static_cast<const uint8_t *>(p.x) + min(g + 8 * n, p.tokens - 1) * p.x_row * elem + t * 16;
     float d[kHalves][kGroups][4];
 #pragma unroll
     for (int h = 0; h < kHalves; ++h)
@@ -111,24 +113,48 @@ __global__ void __launch_bounds__(kMaxWarps * 32) linear_few_kernel(const __grid
 #pragma unroll
             for (int i = 0; i < 4; ++i) d[h][n][i] = 0.0f;
 
-    /* steps of 64 bytes of k, kAhead neighbours at a time to a warp */
-    const uint32_t stride = warps * kAhead * 64;
-    for (uint32_t k0 = warp * kAhead * 64; k0 < size; k0 += stride) {
+    struct Loads {
         uint4 a[kAhead][kHalves][2], b[kAhead][kGroups];
+    };
+    auto load = [&](Loads &l, uint32_t k0) {
 #pragma unroll
         for (int s = 0; s < kAhead; ++s) {
-            const uint32_t k = k0 + s * 64 + t * 16;
 #pragma unroll
             for (int h = 0; h < kHalves; ++h)
 #pragma unroll
-                for (int r = 0; r < 2; ++r) a[s][h][r] = piece<kFp8>(w[h][r], k, size, have_w[r]);
+                for (int r = 0; r < 2; ++r) l.a[s][h][r] = load16(w[h][r] + k0 + s * 64);
 #pragma unroll
-            for (int n = 0; n < kGroups; ++n) b[s][n] = piece<kFp8>(x[n], k, size, have_x[n]);
+            for (int n = 0; n < kGroups; ++n) l.b[s][n] = __ldcg(reinterpret_cast<const uint4 *>(x[n] + k0 + s * 64));
         }
+    };
+    auto multiply = [&](const Loads &l) {
 #pragma unroll
         for (int s = 0; s < kAhead; ++s)
 #pragma unroll
-            for (int h = 0; h < kHalves; ++h) products<kFp8, kGroups>(d[h], a[s][h][0], a[s][h][1], b[s]);
+            for (int h = 0; h < kHalves; ++h) products<kFp8, kGroups>(d[h], l.a[s][h][0], l.a[s][h][1], l.b[s]);
+    };
+    /* the whole steps, in turn over the warps, each time with the next one's loads under way */
+    const uint32_t whole = size / (kAhead * 64) * (kAhead * 64), stride = warps * kAhead * 64;
+    uint32_t k0 = warp * kAhead * 64;
+    Loads one, two;
+    if (k0 < whole) load(one, k0);
+    while (k0 < whole) {
+        if (k0 + stride < whole) load(two, k0 + stride);
+        multiply(one);
+        k0 += stride;
+        if (k0 >= whole) break;
+        if (k0 + stride < whole) load(one, k0 + stride);
+        multiply(two);
+        k0 += stride;
+    }
+    /* the rest of a row */
+    for (uint32_t k = whole + warp * 64; k < size; k += warps * 64) {
+        uint4 b[kGroups];
+#pragma unroll
+        for (int n = 0; n < kGroups; ++n) b[n] = piece<kFp8>(x[n] - t * 16, k + t * 16, size);
+#pragma unroll
+        for (int h = 0; h < kHalves; ++h)
+            products<kFp8, kGroups>(d[h], piece<kFp8>(w[h][0] - t * 16, k + t * 16, size), piece<kFp8>(w[h][1] - t * 16, k + t * 16, size), b);
     }
     /* the warps' sums: [warp][half][token][16 rows] */
 #pragma unroll
@@ -149,7 +175,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32) linear_few_kernel(const __grid
 #pragma unroll
         for (int h = 0; h < kHalves; ++h) {
             const uint32_t row = h * p.outputs + n;
-            if (kFp8) v[h] *= p.x_scales[token] * p.weight_scales[row];
+            if (kFp8) v[h] *= __ldcg(p.x_scales + token) * __ldcg(p.weight_scales + row);
             if (p.bias != nullptr) v[h] += load1(p.bias, row, p.bias_type);
         }
         float y = activate(p.activation, v[0], v[1]);
@@ -161,12 +187,13 @@ __global__ void __launch_bounds__(kMaxWarps * 32) linear_few_kernel(const __grid
 template <bool kFp8, int kGroups, bool kPairs>
 cudaError_t launch_few_t(const LinearParams &p, int sms, cudaStream_t stream) {
     const uint32_t ctas = (p.outputs + 15) / 16;
-    /* warps enough for about 16 an SM, as far as k goes round */
-    uint32_t warps = 4;
+    constexpr int kAhead = ahead_of(kGroups * (kPairs ? 2 : 1));
+    /* as many warps as let all CTAs run at once (about 20 an SM), as far as k goes round */
     const uint32_t steps = (p.inputs * (kFp8 ? 1 : 2) + kAhead * 64 - 1) / (kAhead * 64);
-    while (warps < kMaxWarps && ctas * warps < 16u * (uint32_t)sms && warps < steps) warps *= 2;
+    uint32_t warps = ctas <= (uint32_t)sms ? kMaxWarps : ctas <= 2u * (uint32_t)sms ? 8 : 4;
+    while (warps > 1 && warps > steps) warps /= 2;
     const size_t smem = (size_t)warps * (kPairs ? 2 : 1) * kGroups * 128 * sizeof(float);
-    return launch(linear_few_kernel<kFp8, kGroups, kPairs>, dim3(ctas), warps * 32, smem, stream, p);
+    return launch_overlapped(linear_few_kernel<kFp8, kGroups, kPairs>, dim3(ctas), warps * 32, smem, stream, p);
 }
 
 template <bool kFp8>

@@ -110,6 +110,8 @@ __global__ void __launch_bounds__(kAhead ? kSmall : kMaxNormThreads, kAhead ? ct
     auto at = [&](int i) { return kWide ? (i * g.group + t) * 8 : i * 8 * g.group + t; };
     auto left = [&](int i) { return p.dim > at(i) ? p.dim - at(i) : 0u; };
 
+    wait_for_previous();
+    let_next_start();
     float w[kN][8];
     if (p.weight != nullptr) {
 #pragma unroll
@@ -267,7 +269,7 @@ cudaError_t launch_norm_t(const NormParams &p, int sms, cudaStream_t stream) {
     const uint32_t block = (g.group * g.rows + 31) / 32 * 32;
     /* as many CTAs as run at once, each with rows in turn */
     const uint32_t all = (p.tokens * p.heads + g.rows - 1) / g.rows, most = (uint32_t)sms * ((kAhead ? ctas_of(kN) * kSmall : kMaxNormThreads) / block);
-    return launch(norm_kernel<T, R, kWide, kN, kAhead>, dim3(all < most ? all : most), block, 0, stream, p, g);
+    return launch_overlapped(norm_kernel<T, R, kWide, kN, kAhead>, dim3(all < most ? all : most), block, 0, stream, p, g);
 }
 
 /* rows of an operand that all start on a 16-byte boundary (8 bytes of 8-bit values) */

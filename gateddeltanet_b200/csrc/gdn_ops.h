@@ -149,6 +149,23 @@ cudaError_t launch(void (*kernel)(Params...), dim3 grid, uint32_t block, size_t 
     return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
+/* the same for a kernel that begins with wait_for_previous(), so that its launch and set-up overlap the
+ * end of the kernel before it */
+template <typename... Params, typename... Args>
+cudaError_t launch_overlapped(void (*kernel)(Params...), dim3 grid, uint32_t block, size_t smem, cudaStream_t stream, Args... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(block);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 cudaError_t launch_delta_step(const DeltaParams &p, bool bf16, int sms, cudaStream_t stream);
 /* The chunked form (gdn_delta_chunk.cu): BF16, 16-byte aligned rows. */
 size_t delta_chunk_workspace(uint32_t tokens, uint32_t sequences, uint32_t v_heads);

@@ -70,6 +70,13 @@ __device__ __forceinline__ void store1(void *p, int64_t i, int type, float x) {
         store1(static_cast<float *>(p) + i, x);
 }
 
+/* The start of a kernel launched with launch_overlapped: it may run before the kernel before it on the
+ * stream has ended. wait_for_previous: until it has, and what it wrote is in L2 (every thread that touches
+ * global memory calls it first, and reads what other kernels write past L1, which may hold lines from
+ * before). let_next_start: the next kernel's CTAs may come as soon as there is room for them. */
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 /* x sigmoid(x) as x / (1 + e^-x) with the approximate instructions for 2^x and 1 / x: together under
  * (4 + |x| / 4) 2^-22 of the result (their own errors, and that of -x log2 e, which counts by
  * |x| sigmoid(-x) < 0.28), where results keep 20 bits at least. For x < -87 (results under 1e-36) -0. */
