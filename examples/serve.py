@@ -1,18 +1,22 @@
 """A small server on the serving operators (gateddeltanet_b200/ops.py).
 
-Gated-delta-rule layers with random weights: the prompts of a ragged batch go
-through delta_chunk, every new token through delta_step on the same pooled
-states, and the logits of each step through constrain_logits, which also picks
-the next token. Token table, states and logits stay on the device.
+Gated-delta-rule layers with random weights, each made of the operators: norm,
+projection, short convolution, delta rule, gated norm and projection onto the
+residual, norm, gate and up projection, projection onto the residual. The
+prompts of a ragged batch go through delta_chunk, every new token through
+delta_step on the same pooled states and last inputs, and the logits of each
+step through constrain_logits, which also picks the next token. Token table,
+states and logits stay on the device. With 8-bit weights the norms give 8-bit
+activations with a scale for each token.
 
-    python examples/serve.py [--streams 8] [--layers 4] [--new 64]
+    python examples/serve.py [--streams 8] [--layers 4] [--new 64] [--eight-bits]
 """
 from __future__ import annotations
 
 import argparse
 import os
 import sys
-from typing import List, Optional
+from typing import List, Optional, Tuple
 
 import torch
 import torch.nn.functional as F
@@ -21,41 +25,74 @@ sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 from gateddeltanet_b200 import ops  # noqa: E402
 
 
-class Model:
-    """Embedding, `layers` gated-delta-rule mixers, tied LM head."""
+E4M3 = torch.float8_e4m3fn
 
-    def __init__(self, vocab: int = 32000, hidden: int = 2048, layers: int = 4, heads: int = 8, head_dim: int = 256, seed: int = 1):
+
+class Model:
+    """Embedding, `layers` gated-delta-rule layers with their MLPs, tied LM head."""
+
+    def __init__(self, vocab: int = 32000, hidden: int = 2048, layers: int = 4, heads: int = 8, head_dim: int = 256, seed: int = 1,
+                 intermediate: Optional[int] = None, eight_bits: bool = False):
         gen = torch.Generator("cuda").manual_seed(seed)
 
         def weight(*shape):
             return (torch.randn(shape, generator=gen, device="cuda") * shape[-1] ** -0.5).bfloat16()
 
-        self.vocab, self.heads, self.head_dim = vocab, heads, head_dim
-        width = heads * head_dim
-        self.embedding = weight(vocab, hidden)
-        self.layers = [dict(qkvg=weight(4 * width, hidden), ab=weight(2 * heads, hidden), o=weight(hidden, width),
-                            a_log=torch.rand(heads, generator=gen, device="cuda") * 2) for _ in range(layers)]
+        def projection(rows, columns):
+            """Arguments of ops.linear: a weight, in 8 bits with the scales of its rows."""
+            w = weight(rows, columns)
+            if not eight_bits:
+                return dict(weight=w)
+            scales = w.float().abs().amax(1) / 448
+            return dict(weight=(w.float() / scales[:, None]).to(E4M3), weight_scales=scales)
 
-    def states(self, slots: int) -> List[torch.Tensor]:
-        """A pool of states for each layer."""
-        return [torch.zeros(slots, self.heads, self.head_dim, self.head_dim, device="cuda") for _ in self.layers]
+        self.vocab, self.heads, self.head_dim, self.eight_bits = vocab, heads, head_dim, eight_bits
+        width = heads * head_dim
+        inner = intermediate or hidden * 11 // 64 * 16  # 5632 of 2048
+        ones = lambda n: torch.ones(n, device="cuda")  # noqa: E731
+        self.embedding = weight(vocab, hidden)
+        self.layers = [dict(
+            attn_norm=ones(hidden), o_norm=ones(head_dim), mlp_norm=ones(hidden),
+            # q, k, v, gate and the two gates' rows; whole 16-byte rows of the result
+            qkvgab=projection(-(-(4 * width + 2 * heads) // 8) * 8, hidden),
+            conv=(torch.rand(3 * width, 4, generator=gen, device="cuda") - 0.5), o=projection(hidden, width),
+            gate_up=projection(2 * inner, hidden), down=dict(weight=weight(hidden, inner)),
+            a_log=torch.rand(heads, generator=gen, device="cuda") * 2) for _ in range(layers)]
+        self.norm = ones(hidden)
+
+    def states(self, slots: int) -> List[Tuple[torch.Tensor, torch.Tensor]]:
+        """For each layer a pool of states and one of the convolution's last inputs."""
+        return [(torch.zeros(slots, self.heads, self.head_dim, self.head_dim, device="cuda"),
+                 torch.zeros(slots, 3, 3 * self.heads * self.head_dim, device="cuda")) for _ in self.layers]
+
+    def normed(self, x: torch.Tensor, weight: torch.Tensor, gate: Optional[torch.Tensor] = None) -> dict:
+        """Arguments of ops.linear: the norm of x, in 8 bits for 8-bit weights."""
+        if not self.eight_bits:
+            return dict(x=ops.rms_norm(x, weight, gate=gate, dtype=torch.bfloat16).flatten(1))
+        y, scales = ops.rms_norm(x, weight, gate=gate, dtype=E4M3)
+        return dict(x=y.flatten(1), x_scales=scales)
 
     def forward(self, tokens: torch.Tensor, states, slots, starts: Optional[torch.Tensor] = None,
                 fresh: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Hidden vectors of packed tokens: prompts (starts given) or one new token of each stream."""
-        x = self.embedding[tokens.long()]
+        residual = self.embedding[tokens.long()].float()
         rule = ops.delta_step if starts is None else ops.delta_chunk
-        for layer, state in zip(self.layers, states):
-            h = F.rms_norm(x, x.shape[-1:])
-            q, k, v, gate = (h @ layer["qkvg"].T).unflatten(1, (4, self.heads, self.head_dim)).unbind(1)
-            a, b = (h @ layer["ab"].T).float().chunk(2, dim=1)
-            o = rule(q, k, v, -layer["a_log"].exp() * F.softplus(a - 4), torch.sigmoid(b), state, starts=starts, slots=slots,
-                     fresh=fresh, normalize=True)
-            x = x + (F.rms_norm(o, o.shape[-1:]) * F.silu(gate)).flatten(1) @ layer["o"].T
-        return F.rms_norm(x, x.shape[-1:])
+        width = self.heads * self.head_dim
+        sequences = dict(starts=starts, slots=slots, fresh=fresh)
+        for layer, (state, tails) in zip(self.layers, states):
+            qkvgab = ops.linear(**self.normed(residual, layer["attn_norm"]), **layer["qkvgab"])
+            qkv = ops.short_conv(qkvgab[:, :3 * width], layer["conv"], tails, **sequences)
+            q, k, v = qkv.unflatten(1, (3, self.heads, self.head_dim)).unbind(1)
+            gate = qkvgab[:, 3 * width:4 * width].unflatten(1, (self.heads, self.head_dim))
+            a, b = qkvgab[:, 4 * width:4 * width + 2 * self.heads].float().chunk(2, dim=1)
+            o = rule(q, k, v, -layer["a_log"].exp() * F.softplus(a - 4), torch.sigmoid(b), state, normalize=True, **sequences)
+            ops.linear(**self.normed(o, layer["o_norm"], gate), **layer["o"], residual=residual, out=residual)
+            inner = ops.linear(**self.normed(residual, layer["mlp_norm"]), **layer["gate_up"], activation="swiglu")
+            ops.linear(inner, **layer["down"], residual=residual, out=residual)
+        return ops.rms_norm(residual, self.norm, dtype=torch.bfloat16)
 
     def logits(self, hidden: torch.Tensor) -> torch.Tensor:
-        return hidden @ self.embedding.T
+        return ops.linear(hidden, self.embedding, dtype=torch.float32)
 
 
 @torch.no_grad()
@@ -99,7 +136,7 @@ def generate(model: Model, prompts: List[List[int]], new: int, masks: Optional[t
         if step + 1 < new:
             # slot -1: a stream that has ended stays in the batch, but its states do not change
             hidden = model.forward(picks, states, torch.where(going, slots, -1))
-    return table, lens, [s[slots.long()] for s in states]
+    return table, lens, [state[slots.long()] for state, _ in states]
 
 
 def main() -> None:
@@ -107,8 +144,9 @@ def main() -> None:
     ap.add_argument("--streams", type=int, default=8)
     ap.add_argument("--layers", type=int, default=4)
     ap.add_argument("--new", type=int, default=64)
+    ap.add_argument("--eight-bits", action="store_true")
     args = ap.parse_args()
-    model = Model(layers=args.layers)
+    model = Model(layers=args.layers, eight_bits=args.eight_bits)
     gen = torch.Generator().manual_seed(2)
     prompts = [torch.randint(0, model.vocab, (int(torch.randint(1, 500, (1,), generator=gen)),), generator=gen).tolist()
                for _ in range(args.streams)]
