@@ -337,7 +337,7 @@ int gdn_b200_short_conv(const GdnB200ConvArgs *args) {
     if (a.activation != 0 && a.activation != 1) return failf("%s: activation %d is not 0 or 1", who, a.activation);
     if (a.width < 2 || a.width > 4) return failf("%s: width %u is not 2, 3 or 4", who, a.width);
     if (a.tokens > 0x3fffffffu || a.sequences > 0x3fffffu) return failf("%s: %u tokens in %u sequences are too many", who, a.tokens, a.sequences);
-    if (a.channels > 1u << 22) return failf("%s: %u channels are too many", who, a.channels);
+    if (a.channels > 1u << 20) return failf("%s: %u channels are too many", who, a.channels);
     if (a.starts == nullptr && a.tokens != a.sequences)
         return failf("%s: without starts every sequence has one token (%u tokens, %u sequences)", who, a.tokens, a.sequences);
     if (a.sequences == 0 && a.tokens != 0) return failf("%s: %u tokens but no sequence", who, a.tokens);
