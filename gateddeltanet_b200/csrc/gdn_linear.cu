@@ -286,12 +286,13 @@ __device__ __forceinline__ void finish(const LinearParams &p, float row_scale, f
         for (int i = 0; i < kN; ++i) v[i] = gelu(v[i]);
     }
 }
-/* Rows of out and of the residual in pieces of four values: whether these are aligned. */
+/* Rows of out and of the residual in pieces of four values: whether these are aligned; and out's in pieces of 16 bytes. */
 struct Wide {
-    bool out, residual;
+    bool out, residual, out16;
     __device__ __forceinline__ explicit Wide(const LinearParams &p) {
         const uintptr_t o = p.out_type == kBF16 ? 2 : 4, r = p.residual_type == kBF16 ? 2 : 4;
         out = ((reinterpret_cast<uintptr_t>(p.out) | (uintptr_t)p.out_row * o) & (4 * o - 1)) == 0;
+        out16 = ((reinterpret_cast<uintptr_t>(p.out) | (uintptr_t)p.out_row * o) & 15) == 0;
         residual = ((reinterpret_cast<uintptr_t>(p.residual) | (uintptr_t)p.residual_row * r) & (4 * r - 1)) == 0;
     }
 };
@@ -592,7 +593,7 @@ __global__ void __launch_bounds__(kLinearThreads, 1)
             /* A row of 16 values a lane is turned so that four lanes have one: whole sectors of memory are read and
              * written. One lane's pieces are eight rows apart. */
             constexpr int kStep = pairs ? 2 : 1;
-            if (!has_res && !f32_out && inside) {
+            if (!has_res && !f32_out && inside && wide.out16) {
                 /* BF16: two units to a turn, four pieces of eight values a row */
 #pragma unroll
                 for (int set = 0; set < kSets; set += 2 * kStep) {

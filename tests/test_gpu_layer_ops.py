@@ -215,6 +215,22 @@ def test_linear_what_is_not_finite_stays_in_its_row(ops, tokens, eight):
     assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("outputs", [100, 132, 260, 98, 97, 104])
+@pytest.mark.parametrize("shift", [0, 1, 2, 4])
+@pytest.mark.parametrize("tokens", [7, 64, 300])
+def test_linear_rows_of_results_at_any_alignment(ops, outputs, shift, tokens):
+    """Rows that are multiples of 2, 4, 8 and 16 bytes apart and start there."""
+    a = operands(tokens, 128, outputs, False)
+    for dtype in (BF16, F32):
+        for residual in (None, BF16, F32):
+            flat = torch.full((tokens * outputs + shift + 8,), 7.0, device="cuda", dtype=dtype)
+            out = flat[shift:shift + tokens * outputs].view(tokens, outputs)
+            r = None if residual is None else rand(tokens * outputs + shift, seed=6, dtype=residual)[shift:].view(tokens, outputs)
+            want, off = plain.linear(**a, residual=r)
+            plain.check(ops.linear(**a, residual=r, out=out), want, off)
+            assert bool((flat[:shift] == 7).all()) and bool((flat[shift + tokens * outputs:] == 7).all())
+
+
 def test_linear_the_same_bits_each_time(ops):
     for tokens, outputs in ((1, 2048), (64, 2048), (130, 5632), (2000, 2048)):
         a = operands(tokens, 2048, outputs, False)
