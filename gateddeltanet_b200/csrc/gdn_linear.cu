@@ -333,17 +333,39 @@ __device__ __forceinline__ void store4(const LinearParams &p, const Wide &wide, 
 
 /* 32 tokens from row0 on by 16 outputs from n on, some of them past the ends or not aligned, from
  * a warp's buffer: two tokens at a time, a value a lane. */
-__device__ __noinline__ void store_edge(const LinearParams &p, uint32_t row0, uint32_t n, uint32_t buffer) {
-    const uint32_t lane = threadIdx.x & 31, c = lane & 15;
+template <typename T>
+__device__ __forceinline__ void store_values(const LinearParams &p, uint32_t row0, uint32_t n, uint32_t buffer) {
+    const uint32_t lane = threadIdx.x & 31, c = lane & 15, high = lane >> 4;
     if (n + c >= p.outputs) return;
-#pragma unroll 4
-    for (uint32_t r = lane >> 4; r < 32; r += 2) {
-        const uint32_t token = row0 + r;
-        if (token >= p.tokens) break;
-        float v = load_shared(buffer + r * 64 + (((c >> 2) ^ (r >> 1 & 3)) << 4) + (c & 3) * 4);
-        if (p.residual != nullptr) v += load1(p.residual, token * p.residual_row + n + c, p.residual_type);
-        store1(p.out, token * p.out_row + n + c, p.out_type, v);
+    const uint32_t from = buffer + high * 64 + (c & 3) * 4;
+    auto value = [&](uint32_t i) { return load_shared(from + i * 128 + (((c >> 2) ^ (i & 3)) << 4)); }; /* of row 2 i + high */
+    T *to = static_cast<T *>(p.out) + (row0 + high) * p.out_row + n + c;
+    const int64_t res = (row0 + high) * p.residual_row + n + c;
+    if (row0 + 32 <= p.tokens) {
+#pragma unroll
+        for (uint32_t half = 0; half < 16; half += 8) {
+            float e[8];
+#pragma unroll
+            for (uint32_t i = 0; i < 8; ++i) e[i] = p.residual != nullptr ? load1(p.residual, res + (int64_t)(half + i) * 2 * p.residual_row, p.residual_type) : 0.0f;
+#pragma unroll
+            for (uint32_t i = 0; i < 8; ++i) {
+                const float v = value(half + i);
+                store1(to + (int64_t)(half + i) * 2 * p.out_row, p.residual != nullptr ? v + e[i] : v);
+            }
+        }
+        return;
     }
+    for (uint32_t i = 0; i < 16 && row0 + 2 * i + high < p.tokens; ++i) {
+        float v = value(i);
+        if (p.residual != nullptr) v += load1(p.residual, res + (int64_t)i * 2 * p.residual_row, p.residual_type);
+        store1(to + (int64_t)i * 2 * p.out_row, v);
+    }
+}
+__device__ __noinline__ void store_edge(const LinearParams &p, uint32_t row0, uint32_t n, uint32_t buffer) {
+    if (p.out_type == kBF16)
+        store_values<__nv_bfloat16>(p, row0, n, buffer);
+    else
+        store_values<float>(p, row0, n, buffer);
 }
 
 template <int kCtas, bool kFp8, bool pairs>

@@ -290,6 +290,7 @@ cudaError_t launch_norm_x(const NormParams &p, int sms, cudaStream_t stream) {
     /* eight values a thread, or sixteen where a CTA would have too few threads */
     auto pick = [&](auto r) {
         using R = decltype(r);
+        if (wide && sizeof(T) == 4 && norm_threads(p, 8) <= kSmall) return launch_norm_t<T, R, true, 1, true>;
         if (wide && norm_threads(p, 16) <= kSmall) return launch_norm_t<T, R, true, 2, true>;
         if (wide && norm_threads(p, 32) <= kSmall) return launch_norm_t<T, R, true, 4, true>;
         if (!wide && norm_threads(p, 8) <= kSmall) return launch_norm_t<T, R, false, 1, true>;
