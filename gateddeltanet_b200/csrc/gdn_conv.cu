@@ -27,7 +27,7 @@ __host__ __device__ constexpr int ahead_of(int channels) { return channels == 8 
 
 __device__ __forceinline__ uint32_t bound_of(const ConvParams &p, uint32_t n) {
     if (p.starts == nullptr) return n;
-    const int32_t s = __ldcg(p.starts + n);
+    const int32_t s = p.starts[n];
     return s < 0 ? 0u : ((uint32_t)s < p.tokens ? (uint32_t)s : p.tokens);
 }
 
@@ -47,49 +47,54 @@ __device__ uint32_t begun(const ConvParams &p, uint32_t t) {
     return lo;
 }
 
-/* What the lanes of a thread do with its channels: C neighbours (16 bytes) or one. */
+/* A thread's channels: C neighbours (16 bytes), or, where rows are not on 16-byte boundaries, two that are `gap`
+ * apart (0: the second is past the end, and follows the first one's values without being stored). */
 template <typename T, bool kWide>
 struct Lane {
-    static constexpr int C = kWide ? 16 / sizeof(T) : 1;
+    static constexpr int C = kWide ? 16 / sizeof(T) : 2;
+    uint32_t gap;
     static __device__ __forceinline__ void unpack(const uint4 &w, float (&v)[C]) {
         if constexpr (C == 8)
             unpack8(w, v);
         else if constexpr (C == 4)
             v[0] = __uint_as_float(w.x), v[1] = __uint_as_float(w.y), v[2] = __uint_as_float(w.z), v[3] = __uint_as_float(w.w);
         else
-            v[0] = __uint_as_float(w.x);
+            v[0] = __uint_as_float(w.x), v[1] = __uint_as_float(w.y);
     }
-    /* as it is in memory (one channel: as FP32) */
-    static __device__ __forceinline__ uint4 fetch(const T *p) {
+    /* as it is in memory (two channels apart: as FP32) */
+    __device__ __forceinline__ uint4 fetch(const T *p) const {
         if constexpr (kWide)
             return __ldcg(reinterpret_cast<const uint4 *>(p));
         else
-            return make_uint4(__float_as_uint(load1(p)), 0, 0, 0);
+            return make_uint4(__float_as_uint(load1(p)), __float_as_uint(load1(p + gap)), 0, 0);
     }
-    static __device__ __forceinline__ void put(T *p, const float (&v)[C]) {
-        if constexpr (C == 8)
-            *reinterpret_cast<uint4 *>(p) = pack8(v);
-        else if constexpr (C == 4)
-            *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]);
-        else
-            store1(p, v[0]);
-    }
-    static __device__ __forceinline__ void get_tail(const ConvParams &p, int64_t at, float (&v)[C]) {
+    __device__ __forceinline__ void put(T *p, const float (&v)[C]) const {
         if constexpr (C == 8) {
-            load8(p.tails, at, p.tail_type, v);
-        } else if constexpr (C == 4) { /* x is FP32, and so are the tails */
-            unpack(__ldcg(reinterpret_cast<const uint4 *>(static_cast<const float *>(p.tails) + at)), v);
+            *reinterpret_cast<uint4 *>(p) = pack8(v);
+        } else if constexpr (C == 4) {
+            *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]);
         } else {
-            v[0] = load1(p.tails, at, p.tail_type);
+            store1(p, v[0]);
+            if (gap) store1(p + gap, v[1]);
         }
     }
-    static __device__ __forceinline__ void put_tail(const ConvParams &p, int64_t at, const float (&v)[C]) {
+    __device__ __forceinline__ void get_tail(const ConvParams &p, int64_t at, float (&v)[C]) const {
         if constexpr (C == 8)
-            store8(p.tails, at, p.tail_type, v);
-        else if constexpr (C == 4)
-            *reinterpret_cast<float4 *>(static_cast<float *>(p.tails) + at) = make_float4(v[0], v[1], v[2], v[3]);
+            load8(p.tails, at, p.tail_type, v);
+        else if constexpr (C == 4) /* x is FP32, and so are the tails */
+            unpack(__ldcg(reinterpret_cast<const uint4 *>(static_cast<const float *>(p.tails) + at)), v);
         else
+            v[0] = load1(p.tails, at, p.tail_type), v[1] = load1(p.tails, at + gap, p.tail_type);
+    }
+    __device__ __forceinline__ void put_tail(const ConvParams &p, int64_t at, const float (&v)[C]) const {
+        if constexpr (C == 8) {
+            store8(p.tails, at, p.tail_type, v);
+        } else if constexpr (C == 4) {
+            *reinterpret_cast<float4 *>(static_cast<float *>(p.tails) + at) = make_float4(v[0], v[1], v[2], v[3]);
+        } else {
             store1(p.tails, at, p.tail_type, v[0]);
+            if (gap) store1(p.tails, at + gap, p.tail_type, v[1]);
+        }
     }
 };
 
@@ -130,7 +135,7 @@ __device__ __forceinline__ uint64_t silu2(uint64_t x) {
 /* The weights of a CTA's channels in shared memory, by pairs of channels: four taps each, the last one
  * meets the token itself (a shorter width has zeros in front, which nobody reads). One more row than
  * threads, so that threads that fill neighbouring channels use different banks. */
-template <int C, uint32_t kLanes>
+template <int C, uint32_t kLanes, bool kWide>
 struct Weights {
     float4 pairs[(C + 1) / 2][2][kLanes + 1]; /* taps 0 and 1 of both channels, taps 2 and 3 */
     __device__ __forceinline__ uint64_t tap(int pair, int j, uint32_t lane) const {
@@ -154,7 +159,7 @@ struct Weights {
             for (int j = 0; j < 4; ++j) v[k][j] = 0.0f;
             if (i >= kLanes * C || c >= p.channels) continue;
             if (whole) {
-                const float4 e = __ldcg(reinterpret_cast<const float4 *>(static_cast<const float *>(p.weight) + (size_t)c * 4));
+                const float4 e = *reinterpret_cast<const float4 *>(static_cast<const float *>(p.weight) + (size_t)c * 4);
                 v[k][0] = e.x, v[k][1] = e.y, v[k][2] = e.z, v[k][3] = e.w;
             } else {
 #pragma unroll
@@ -163,10 +168,10 @@ struct Weights {
         }
 #pragma unroll
         for (int k = 0; k < kEach; ++k) {
-            const uint32_t i = k * kThreads + threadIdx.x, of = i % C;
+            const uint32_t i = k * kThreads + threadIdx.x, of = kWide ? i % C : i / kLanes, lane = kWide ? i / C : i % kLanes;
             if (i < kLanes * C) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) reinterpret_cast<float *>(&pairs[of / 2][j >> 1][i / C])[(j & 1) * 2 + (of & 1)] = v[k][j];
+                for (int j = 0; j < 4; ++j) reinterpret_cast<float *>(&pairs[of / 2][j >> 1][lane])[(j & 1) * 2 + (of & 1)] = v[k][j];
             }
         }
     }
@@ -187,17 +192,17 @@ template <typename T, bool kWide, int W>
 __global__ void __launch_bounds__(kThreads, Lane<T, kWide>::C == 8 ? 8 : 1) conv_kernel(const __grid_constant__ ConvParams p, const uint32_t tile) {
     using L = Lane<T, kWide>;
     constexpr int C = L::C, kAhead = ahead_of(C);
-    __shared__ Weights<C, kThreads> weights;
-    const uint32_t tid = threadIdx.x, c0 = (blockIdx.y * kThreads + tid) * C;
+    __shared__ Weights<C, kThreads, kWide> weights;
+    const uint32_t tid = threadIdx.x, c0 = kWide ? (blockIdx.y * kThreads + tid) * C : blockIdx.y * kThreads * C + tid;
     const bool live = c0 < p.channels;
+    const L at{c0 + kThreads < p.channels ? kThreads : 0};
     const T *x = static_cast<const T *>(p.x) + c0;
     T *y = static_cast<T *>(p.out) + c0;
     wait_for_previous();
-    let_next_start();
     weights.template fill<W>(p, blockIdx.y * kThreads * C);
     float bias[C];
 #pragma unroll
-    for (int c = 0; c < C; ++c) bias[c] = live && p.bias != nullptr ? load1(p.bias, c0 + c, p.weight_type) : 0.0f;
+    for (int c = 0; c < C; ++c) bias[c] = live && p.bias != nullptr ? load1(p.bias, c0 + (kWide ? c : c * at.gap), p.weight_type) : 0.0f;
     __syncthreads();
     const uint32_t t0 = blockIdx.x * tile, t1 = min(t0 + tile, p.tokens);
     uint32_t n = t0 < t1 ? begun(p, t0) : 0; /* the sequence of token t0 is n - 1, if it has one */
@@ -213,11 +218,11 @@ __global__ void __launch_bounds__(kThreads, Lane<T, kWide>::C == 8 ? 8 : 1) conv
             continue;
         }
         uint32_t stop = min(end, t1);
-        const int64_t slot = n == 0 || n > p.N ? -1 : p.slots == nullptr ? (int64_t)(n - 1) : (int64_t)__ldcg(p.slots + n - 1);
+        const int64_t slot = n == 0 || n > p.N ? -1 : p.slots == nullptr ? (int64_t)(n - 1) : (int64_t)p.slots[n - 1];
         if (slot < 0 || slot >= (int64_t)p.tail_slots) {
             /* tokens of no sequence, or of one without a slot */
             if (live)
-                for (; t < stop; ++t) L::put(y + t * p.out_token, zero);
+                for (; t < stop; ++t) at.put(y + t * p.out_token, zero);
             t = stop;
             ++n;
             continue;
@@ -232,7 +237,7 @@ __global__ void __launch_bounds__(kThreads, Lane<T, kWide>::C == 8 ? 8 : 1) conv
         if (live) {
             if (t == begin) {
                 /* the tokens that meet the slot's rows, one by one */
-                const bool fresh = p.fresh != nullptr && __ldcg(p.fresh + n - 1) != 0;
+                const bool fresh = p.fresh != nullptr && p.fresh[n - 1] != 0;
                 const int64_t rows = slot * p.tails_slot + c0;
                 const uint32_t few = min((uint32_t)(W - 1), end - begin);
                 float win[W - 1][C];
@@ -240,11 +245,11 @@ __global__ void __launch_bounds__(kThreads, Lane<T, kWide>::C == 8 ? 8 : 1) conv
                 for (int j = 0; j < W - 1; ++j) {
 #pragma unroll
                     for (int c = 0; c < C; ++c) win[j][c] = 0.0f;
-                    if (!fresh) L::get_tail(p, rows + j * p.tails_row, win[j]);
+                    if (!fresh) at.get_tail(p, rows + j * p.tails_row, win[j]);
                 }
                 for (uint32_t i = 0; i < few; ++i) {
                     float in[C], out[C];
-                    L::unpack(L::fetch(x + (int64_t)(t + i) * p.x_token), in);
+                    L::unpack(at.fetch(x + (int64_t)(t + i) * p.x_token), in);
 #pragma unroll
                     for (int c = 0; c < C; ++c) {
                         float v[W];
@@ -256,14 +261,14 @@ __global__ void __launch_bounds__(kThreads, Lane<T, kWide>::C == 8 ? 8 : 1) conv
 #pragma unroll
                         for (int j = 0; j < W - 1; ++j) win[j][c] = v[j + 1];
                     }
-                    L::put(y + (int64_t)(t + i) * p.out_token, out);
+                    at.put(y + (int64_t)(t + i) * p.out_token, out);
                 }
                 /* the window is now the slot's new content, unless there are more tokens */
                 const bool more = end - begin > W - 1;
 #pragma unroll
                 for (int j = 0; j < W - 1; ++j) {
-                    if (more) L::unpack(L::fetch(x + (int64_t)(end - (W - 1) + j) * p.x_token), win[j]);
-                    L::put_tail(p, rows + j * p.tails_row, win[j]);
+                    if (more) L::unpack(at.fetch(x + (int64_t)(end - (W - 1) + j) * p.x_token), win[j]);
+                    at.put_tail(p, rows + j * p.tails_row, win[j]);
                 }
                 t += few;
             }
@@ -271,54 +276,42 @@ __global__ void __launch_bounds__(kThreads, Lane<T, kWide>::C == 8 ? 8 : 1) conv
             uint4 in[W - 1 + kAhead], next[kAhead];
             if (t < stop) {
 #pragma unroll
-                for (int j = 0; j < W - 1; ++j) in[j] = L::fetch(x + (int64_t)(t - (W - 1) + j) * p.x_token);
+                for (int j = 0; j < W - 1; ++j) in[j] = at.fetch(x + (int64_t)(t - (W - 1) + j) * p.x_token);
 #pragma unroll
-                for (int a = 0; a < kAhead; ++a) next[a] = L::fetch(x + (int64_t)min(t + a, stop - 1) * p.x_token);
+                for (int a = 0; a < kAhead; ++a) next[a] = at.fetch(x + (int64_t)min(t + a, stop - 1) * p.x_token);
             }
             for (; t < stop; t += kAhead) {
 #pragma unroll
                 for (int a = 0; a < kAhead; ++a) in[W - 1 + a] = next[a];
                 if (t + kAhead < stop) {
 #pragma unroll
-                    for (int a = 0; a < kAhead; ++a) next[a] = L::fetch(x + (int64_t)min(t + kAhead + a, stop - 1) * p.x_token);
+                    for (int a = 0; a < kAhead; ++a) next[a] = at.fetch(x + (int64_t)min(t + kAhead + a, stop - 1) * p.x_token);
                 }
                 uint32_t result[kAhead][4];
                 auto word = [](const uint4 &v, int q) { return q == 0 ? v.x : q == 1 ? v.y : q == 2 ? v.z : v.w; };
-                if constexpr (kWide) {
-                    /* two channels at a time: a word of 16-bit inputs, two of 32 bits */
+                /* two channels at a time: a word of 16-bit inputs, two of 32 bits */
 #pragma unroll
-                    for (int q = 0; q < C / 2; ++q) {
-                        uint64_t v[W - 1 + kAhead], w[W];
+                for (int q = 0; q < C / 2; ++q) {
+                    uint64_t v[W - 1 + kAhead], w[W];
 #pragma unroll
-                        for (int j = 0; j < W; ++j) w[j] = weights.tap(q, 4 - W + j, tid);
+                    for (int j = 0; j < W; ++j) w[j] = weights.tap(q, 4 - W + j, tid);
 #pragma unroll
-                        for (int j = 0; j < W - 1 + kAhead; ++j)
-                            v[j] = C == 8 ? pair_of(low_bf16(word(in[j], q)), high_bf16(word(in[j], q)))
-                                          : pair_of(__uint_as_float(word(in[j], 2 * q)), __uint_as_float(word(in[j], 2 * q + 1)));
-                        const uint64_t b = pair_of(bias[2 * q], bias[2 * q + 1]);
-#pragma unroll
-                        for (int a = 0; a < kAhead; ++a) {
-                            uint64_t o = b;
-#pragma unroll
-                            for (int j = 0; j < W; ++j) o = fma2(w[j], v[a + j], o);
-                            if (p.silu) o = silu2(o);
-                            float lo, hi;
-                            split(o, lo, hi);
-                            if (C == 8)
-                                result[a][q] = pack_bf16(lo, hi);
-                            else
-                                result[a][2 * q] = __float_as_uint(lo), result[a][2 * q + 1] = __float_as_uint(hi);
-                        }
-                    }
-                } else {
-                    const float4 w = weights.of(0, tid);
+                    for (int j = 0; j < W - 1 + kAhead; ++j)
+                        v[j] = C == 8 ? pair_of(low_bf16(word(in[j], q)), high_bf16(word(in[j], q)))
+                                      : pair_of(__uint_as_float(word(in[j], 2 * q)), __uint_as_float(word(in[j], 2 * q + 1)));
+                    const uint64_t b = pair_of(bias[2 * q], bias[2 * q + 1]);
 #pragma unroll
                     for (int a = 0; a < kAhead; ++a) {
-                        float u[W];
+                        uint64_t o = b;
 #pragma unroll
-                        for (int j = 0; j < W; ++j) u[j] = __uint_as_float(in[a + j].x);
-                        const float o = tap<W>(w, bias[0], u);
-                        result[a][0] = __float_as_uint(p.silu ? silu(o) : o);
+                        for (int j = 0; j < W; ++j) o = fma2(w[j], v[a + j], o);
+                        if (p.silu) o = silu2(o);
+                        float lo, hi;
+                        split(o, lo, hi);
+                        if (C == 8)
+                            result[a][q] = pack_bf16(lo, hi);
+                        else
+                            result[a][2 * q] = __float_as_uint(lo), result[a][2 * q + 1] = __float_as_uint(hi);
                     }
                 }
 #pragma unroll
@@ -328,7 +321,7 @@ __global__ void __launch_bounds__(kThreads, Lane<T, kWide>::C == 8 ? 8 : 1) conv
                         if constexpr (kWide)
                             *reinterpret_cast<uint4 *>(to) = make_uint4(result[a][0], result[a][1], result[a][2], result[a][3]);
                         else
-                            store1(to, __uint_as_float(result[a][0]));
+                            at.put(to, {__uint_as_float(result[a][0]), __uint_as_float(result[a][1])});
                     }
 #pragma unroll
                 for (int j = 0; j < W - 1; ++j) in[j] = in[kAhead + j];
@@ -340,10 +333,10 @@ __global__ void __launch_bounds__(kThreads, Lane<T, kWide>::C == 8 ? 8 : 1) conv
     /* fresh sequences without tokens: nobody else touches their slots */
     if (p.starts != nullptr && p.fresh != nullptr)
         for (uint32_t i = blockIdx.x; i < p.N; i += gridDim.x)
-            if (__ldcg(p.fresh + i) != 0 && bound_of(p, i + 1) <= bound_of(p, i)) {
-                const int64_t slot = p.slots == nullptr ? (int64_t)i : (int64_t)__ldcg(p.slots + i);
+            if (p.fresh[i] != 0 && bound_of(p, i + 1) <= bound_of(p, i)) {
+                const int64_t slot = p.slots == nullptr ? (int64_t)i : (int64_t)p.slots[i];
                 if (live && slot >= 0 && slot < (int64_t)p.tail_slots)
-                    for (int j = 0; j < W - 1; ++j) L::put_tail(p, slot * p.tails_slot + j * p.tails_row + c0, zero);
+                    for (int j = 0; j < W - 1; ++j) at.put_tail(p, slot * p.tails_slot + j * p.tails_row + c0, zero);
             }
 }
 
@@ -353,30 +346,32 @@ template <typename T, bool kWide, int W>
 __global__ void __launch_bounds__(kThreads) conv_step_kernel(const __grid_constant__ ConvParams p) {
     using L = Lane<T, kWide>;
     constexpr int C = L::C;
-    __shared__ Weights<C, 32> weights;
-    const uint32_t lane = threadIdx.x & 31, t = blockIdx.x * (kThreads / 32) + threadIdx.x / 32, c0 = (blockIdx.y * 32 + lane) * C;
+    __shared__ Weights<C, 32, kWide> weights;
+    const uint32_t lane = threadIdx.x & 31, t = blockIdx.x * (kThreads / 32) + threadIdx.x / 32;
+    const uint32_t c0 = kWide ? (blockIdx.y * 32 + lane) * C : blockIdx.y * 32 * C + lane;
     const bool live = c0 < p.channels && t < p.tokens;
+    const L at{c0 + 32 < p.channels ? 32u : 0u};
     wait_for_previous();
     let_next_start();
     int64_t slot = -1;
     bool fresh = false;
     if (t < p.tokens) {
-        slot = p.slots == nullptr ? (int64_t)t : (int64_t)__ldcg(p.slots + t);
-        fresh = p.fresh != nullptr && __ldcg(p.fresh + t) != 0;
+        slot = p.slots == nullptr ? (int64_t)t : (int64_t)p.slots[t];
+        fresh = p.fresh != nullptr && p.fresh[t] != 0;
     }
     const bool known = slot >= 0 && slot < (int64_t)p.tail_slots;
     const int64_t rows = slot * p.tails_slot + c0;
     float win[W][C], out[C], bias[C];
-    if (live) L::unpack(L::fetch(static_cast<const T *>(p.x) + t * p.x_token + c0), win[W - 1]);
+    if (live) L::unpack(at.fetch(static_cast<const T *>(p.x) + t * p.x_token + c0), win[W - 1]);
 #pragma unroll
     for (int j = 0; j < W - 1; ++j) {
 #pragma unroll
         for (int c = 0; c < C; ++c) win[j][c] = 0.0f;
-        if (live && known && !fresh) L::get_tail(p, rows + j * p.tails_row, win[j]);
+        if (live && known && !fresh) at.get_tail(p, rows + j * p.tails_row, win[j]);
     }
     weights.template fill<W>(p, blockIdx.y * 32 * C);
 #pragma unroll
-    for (int c = 0; c < C; ++c) bias[c] = live && p.bias != nullptr ? load1(p.bias, c0 + c, p.weight_type) : 0.0f;
+    for (int c = 0; c < C; ++c) bias[c] = live && p.bias != nullptr ? load1(p.bias, c0 + (kWide ? c : c * at.gap), p.weight_type) : 0.0f;
     __syncthreads();
     if (!live) return;
 #pragma unroll
@@ -387,10 +382,10 @@ __global__ void __launch_bounds__(kThreads) conv_step_kernel(const __grid_consta
         const float s = tap<W>(weights.of(c, lane), bias[c], v);
         out[c] = !known ? 0.0f : p.silu ? silu(s) : s;
     }
-    L::put(static_cast<T *>(p.out) + t * p.out_token + c0, out);
+    at.put(static_cast<T *>(p.out) + t * p.out_token + c0, out);
     if (known) {
 #pragma unroll
-        for (int j = 0; j < W - 1; ++j) L::put_tail(p, rows + j * p.tails_row, win[j + 1]);
+        for (int j = 0; j < W - 1; ++j) at.put_tail(p, rows + j * p.tails_row, win[j + 1]);
     }
 }
 
