@@ -565,6 +565,7 @@ __global__ void __launch_bounds__(kLinearThreads, 1)
             auto unit = [&](int set) { return (uint32_t)(pairs ? set / 2 : set) * 2 + half; };
             auto have = [&](int set) { return unit(set) * 16 < g.outs; };
             auto column = [&](int set) { return unit(set) * 16 + (pairs && (set & 1) ? g.outs : 0); };
+            const bool rows = row0 < p.tokens; /* this warp has any */
             for (uint32_t b = b0; b < b1; b += g.chunk, ++seq) {
                 const uint32_t acc = seq & 1u;
                 ok = ok && wait_bar(sums_full + 8 * acc, (seq >> 1) & 1u, abort);
@@ -572,7 +573,8 @@ __global__ void __launch_bounds__(kLinearThreads, 1)
                 if (!ok) break;
                 tc_fence_after();
                 const uint32_t from = tmem + acc * second + ((quarter * 32) << 16);
-                if (b == b0) {
+                if (!rows) {
+                } else if (b == b0) {
 #pragma unroll
                     for (int set = 0; set < kSets; ++set)
                         if (have(set)) tc_ld16(from + column(set), sum[set]);
@@ -604,7 +606,7 @@ __global__ void __launch_bounds__(kLinearThreads, 1)
                 if (!ok) s->failed = 1;
 #pragma unroll
                 for (int set = 0; set < kSets; ++set)
-                    if (ok && have(set)) {
+                    if (ok && rows && have(set)) {
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
                             *reinterpret_cast<float4 *>(base + (quarter * 32 + lane) * g.n * 4 + (((column(set) / 4 + i) ^ (lane & 7)) * 16)) =
@@ -615,7 +617,8 @@ __global__ void __launch_bounds__(kLinearThreads, 1)
             /* A row of 16 values a lane is turned so that four lanes have one: whole sectors of memory are read and
              * written. One lane's pieces are eight rows apart. */
             constexpr int kStep = pairs ? 2 : 1;
-            if (!has_res && !f32_out && inside && wide.out16) {
+            if (!rows) {
+            } else if (!has_res && !f32_out && inside && wide.out16) {
                 /* BF16: two units to a turn, four pieces of eight values a row */
 #pragma unroll
                 for (int set = 0; set < kSets; set += 2 * kStep) {
