@@ -213,8 +213,8 @@ __global__ void __launch_bounds__(kThreads, Lane<T, kWide>::C == 8 ? 8 : 1) conv
 
     while (t < t1) {
         const uint32_t end = n <= p.N ? bound_of(p, n) : p.tokens; /* the first token of the next sequence */
-        if (end <= t && n <= p.N) { /* a sequence without tokens, or starts that decrease */
-            ++n;
+        if (end <= t && n <= p.N) { /* a sequence without tokens, of which there may be many, or starts that decrease */
+            n = max(n + 1, begun(p, t));
             continue;
         }
         uint32_t stop = min(end, t1);

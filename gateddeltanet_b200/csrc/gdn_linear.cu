@@ -43,6 +43,7 @@ constexpr uint32_t kLinearThreads = (kEpilogueWarps + 4) * 32; /* three warpgrou
 /* Registers a thread: 384 threads are launched with 168 (64512 in all); the warps with
  * the sums then take 216 and the others 64 (63488). With 168 the sums spilled. */
 constexpr int kEpilogueRegs = 216, kOtherRegs = 64;
+constexpr uint32_t kSplitRegs = kEpilogueWarps * 32 * kEpilogueRegs + 4 * 32 * kOtherRegs; /* at most those of the launch, or the split waits for good */
 constexpr uint32_t kBlock = 128;                  /* bytes of k in a row of a copy */
 constexpr uint32_t kRowsA = 128;                  /* tokens of a CTA */
 constexpr uint32_t kBytesA = kRowsA * kBlock;
@@ -805,6 +806,12 @@ cudaError_t launch_shape(const LinearParams &p, const LinearShape &g, int sms, c
     const size_t smem = kSmemRest + (size_t)g.stages * g.sub * (kBytesA + g.n / kCtas * kBlock);
     e = cudaFuncSetAttribute(linear_kernel<kCtas, kFp8, pairs>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemLimit);
     if (e != cudaSuccess) return e;
+    static const cudaError_t registers = [] {
+        cudaFuncAttributes attr;
+        const cudaError_t error = cudaFuncGetAttributes(&attr, linear_kernel<kCtas, kFp8, pairs>);
+        return error != cudaSuccess ? error : (uint32_t)attr.numRegs * kLinearThreads < kSplitRegs ? cudaErrorInvalidKernelImage : cudaSuccess;
+    }();
+    if (registers != cudaSuccess) return registers;
     const uint32_t tiles = g.tiles_m * g.tiles_n, group = kCtas * g.split;
     uint32_t workers = (uint32_t)sms / group;
     if (g.split > 1 || workers > tiles) workers = tiles;

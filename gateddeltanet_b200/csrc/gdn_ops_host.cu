@@ -81,6 +81,19 @@ int on_device(const char *who, int device, F launch) {
     return e == cudaSuccess ? 0 : cuda_failf(who, "launch failed", e);
 }
 
+/* Whether rows [tokens][heads] of dim values share memory (strides not negative). */
+bool rows_overlap(int64_t token, int64_t head, uint32_t tokens, uint32_t heads, uint32_t dim) {
+    int64_t inner = head, outer = token;
+    uint32_t n_inner = heads, n_outer = tokens;
+    if (heads == 1 || (tokens > 1 && token < head)) inner = token, outer = head, n_inner = tokens, n_outer = heads;
+    int64_t reach = dim;
+    if (n_inner > 1) {
+        if (inner < reach) return true;
+        reach += (n_inner - 1) * inner;
+    }
+    return n_outer > 1 && outer < reach;
+}
+
 std::atomic<uint32_t> g_drop{0}; /* gdn_b200_test_drop_copy */
 
 /* Checks what both forms of the rule ask of their arguments; > 0: nothing to do. */
@@ -267,6 +280,9 @@ int gdn_b200_rms_norm(const GdnB200NormArgs *args) {
         weight(a.weight, 0, 0, 1, 1, a.dim, size_of(a.weight_dtype)), scales(a.out_dtype == 2 ? a.scales : nullptr, 0, 0, 1, 1, a.tokens, 4);
     const bool in_place = a.x == a.out && a.dtype == a.out_dtype && (a.tokens == 1 || a.x_token == a.out_token) &&
                           (a.heads == 1 || a.x_head == a.out_head);
+    if (rows_overlap(a.out_token, a.out_head, a.tokens, a.heads, a.dim)) return failf("%s: rows of out overlap", who);
+    if (a.residual != nullptr && rows_overlap(a.residual_token, a.residual_head, a.tokens, a.heads, a.dim))
+        return failf("%s: rows of the residual overlap", who);
     if (out.meets(gate) || out.meets(residual) || out.meets(weight) || (!in_place && out.meets(x)))
         return failf("%s: out overlaps another tensor", who);
     if (residual.meets(x) || residual.meets(gate) || residual.meets(weight)) return failf("%s: the residual overlaps another tensor", who);

@@ -274,6 +274,21 @@ def test_conv(ops, starts, width, channels, x_type, tail_type):
     assert torch.equal(tails.cpu().double(), after)
 
 
+def test_conv_many_sequences_without_tokens(ops):
+    """Between two tokens, before and after them, with a slot for some."""
+    lengths = [0] * 3000 + [2] + [0] * 5000 + [1, 0, 0, 70] + [0] * 40000
+    starts = torch.tensor([0] + lengths).cumsum(0).int()
+    slots = torch.full((len(lengths),), -1).int()
+    used = [i for i, n in enumerate(lengths) if n] + [0, 4000, 47000]
+    slots[used] = torch.arange(len(used)).int()
+    fresh = torch.zeros(len(lengths), dtype=torch.bool)
+    fresh[4000] = True
+    x, weight, tails = rand(73, 64, dtype=BF16), rand(64, 4, seed=2), rand(len(used), 3, 64, seed=3)
+    want, after, off = plain.conv(x, weight, tails, starts=starts, slots=slots, fresh=fresh)
+    plain.check(ops.short_conv(x, weight, tails, starts=starts.cuda(), slots=slots.cuda(), fresh=fresh.cuda()), want, off)
+    assert torch.equal(tails.cpu().double(), after)
+
+
 @pytest.mark.parametrize("extra", [8, 3])
 @pytest.mark.parametrize("starts", [None, [0, 20, 21, 50]], ids=str)
 def test_conv_strides(ops, extra, starts):

@@ -51,7 +51,9 @@ def conv_args(**change):
     (dict(heads=1, dim=16385), "more than one CTA"), (dict(out_dtype=2, scales=FAR, heads=257, dim=64), "more than one CTA"),
     (dict(out=FAKE + 2), "out overlaps"), (dict(out=FAKE, out_dtype=0), "out overlaps"), (dict(gate=FAKE + (1 << 26)), "out overlaps"),
     (dict(residual=FAKE, residual_dtype=1), "residual overlaps"), (dict(residual=FAR, gate=FAR), "residual overlaps"),
-    (dict(out_dtype=2, scales=FAKE), "scales overlaps"), (dict(out=FAKE, out_token=512), "out overlaps")])
+    (dict(out_dtype=2, scales=FAKE), "scales overlaps"), (dict(out=FAKE, out_token=512), "out overlaps"),
+    (dict(out=FAKE, x_token=0, out_token=0), "rows of out"), (dict(out_head=63), "rows of out"), (dict(out_token=255), "rows of out"),
+    (dict(out_token=64, out_head=319), "rows of out"), (dict(residual=FAR + (1 << 26), residual_head=0), "rows of the residual")])
 def test_norm_refusals(lib, change, reason):  # noqa: F811
     assert lib.gdn_b200_rms_norm(norm_args(**change)) == -1
     assert reason in gdn.last_error()
@@ -60,7 +62,7 @@ def test_norm_refusals(lib, change, reason):  # noqa: F811
 @pytest.mark.parametrize("change", [
     dict(), dict(out=FAKE), dict(weight=0), dict(residual=FAR + (1 << 26)), dict(gate=FAKE), dict(out_dtype=2, scales=FAR + 4096),
     dict(heads=1, dim=16384, x_token=16384, out_token=16384), dict(x=FAKE + 2), dict(tokens=1, heads=1, x_token=0, out_token=0),
-    dict(x_token=512, gate=FAKE + 512, gate_token=512, out=FAKE, out_token=512)], ids=str)
+    dict(out_token=64, out_head=320), dict(x_token=0), dict(x_token=512, gate=FAKE + 512, gate_token=512, out=FAKE, out_token=512)], ids=str)
 def test_norm_is_taken(lib, change):  # noqa: F811
     assert lib.gdn_b200_rms_norm(norm_args(**change)) == -1
     assert "device" in gdn.last_error()  # refused for the device alone
