@@ -31,6 +31,7 @@
 #include <cuda.h>
 
 #include <atomic>
+#include <type_traits>
 
 namespace gdn {
 namespace ops {
@@ -287,89 +288,54 @@ __device__ __forceinline__ void finish(const LinearParams &p, float row_scale, f
         for (int i = 0; i < kN; ++i) v[i] = gelu(v[i]);
     }
 }
-/* Rows of out and of the residual in pieces of four values: whether these are aligned; and out's in pieces of 16 bytes. */
-struct Wide {
-    bool out, residual, out16;
-    __device__ __forceinline__ explicit Wide(const LinearParams &p) {
-        const uintptr_t o = p.out_type == kBF16 ? 2 : 4, r = p.residual_type == kBF16 ? 2 : 4;
-        out = ((reinterpret_cast<uintptr_t>(p.out) | (uintptr_t)p.out_row * o) & (4 * o - 1)) == 0;
-        out16 = ((reinterpret_cast<uintptr_t>(p.out) | (uintptr_t)p.out_row * o) & 15) == 0;
-        residual = ((reinterpret_cast<uintptr_t>(p.residual) | (uintptr_t)p.residual_row * r) & (4 * r - 1)) == 0;
-    }
-};
 __device__ __forceinline__ float4 load4(const void *p, int64_t i, int type) {
     if (type == kF32) return __ldcg(reinterpret_cast<const float4 *>(static_cast<const float *>(p) + i));
     const uint2 w = __ldcg(reinterpret_cast<const uint2 *>(static_cast<const __nv_bfloat16 *>(p) + i));
     return make_float4(low_bf16(w.x), high_bf16(w.x), low_bf16(w.y), high_bf16(w.y));
 }
-/* Outputs n .. n + 3 of a token: the residual, the rounding and the store. */
-__device__ __forceinline__ void store4(const LinearParams &p, const Wide &wide, uint32_t token, uint32_t n, float4 v) {
-    if (token >= p.tokens || n >= p.outputs) return;
-    const bool whole = n + 4 <= p.outputs;
-    if (p.residual != nullptr) {
-        const int64_t at = token * p.residual_row + n;
-        if (whole && wide.residual) {
-            const float4 e = load4(p.residual, at, p.residual_type);
-            v.x += e.x, v.y += e.y, v.z += e.z, v.w += e.w;
-        } else {
-            v.x += load1(p.residual, at, p.residual_type);
-            if (n + 1 < p.outputs) v.y += load1(p.residual, at + 1, p.residual_type);
-            if (n + 2 < p.outputs) v.z += load1(p.residual, at + 2, p.residual_type);
-            if (n + 3 < p.outputs) v.w += load1(p.residual, at + 3, p.residual_type);
-        }
-    }
-    const int64_t at = token * p.out_row + n;
-    if (whole && wide.out) {
-        if (p.out_type == kF32)
-            *reinterpret_cast<float4 *>(static_cast<float *>(p.out) + at) = v;
-        else
-            *reinterpret_cast<uint2 *>(static_cast<__nv_bfloat16 *>(p.out) + at) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
-    } else {
-        store1(p.out, at, p.out_type, v.x);
-        if (n + 1 < p.outputs) store1(p.out, at + 1, p.out_type, v.y);
-        if (n + 2 < p.outputs) store1(p.out, at + 2, p.out_type, v.z);
-        if (n + 3 < p.outputs) store1(p.out, at + 3, p.out_type, v.w);
-    }
+__device__ __forceinline__ void put4(void *p, int64_t i, int type, const float4 &v) {
+    if (type == kF32)
+        *reinterpret_cast<float4 *>(static_cast<float *>(p) + i) = v;
+    else
+        *reinterpret_cast<uint2 *>(static_cast<__nv_bfloat16 *>(p) + i) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
 }
-
-/* 32 tokens from row0 on by 16 outputs from n on, some of them past the ends or not aligned, from
- * a warp's buffer: two tokens at a time, a value a lane. */
-template <typename T>
-__device__ __forceinline__ void store_values(const LinearParams &p, uint32_t row0, uint32_t n, uint32_t buffer) {
-    const uint32_t lane = threadIdx.x & 31, c = lane & 15, high = lane >> 4;
-    if (n + c >= p.outputs) return;
-    const uint32_t from = buffer + high * 64 + (c & 3) * 4;
-    auto value = [&](uint32_t i) { return load_shared(from + i * 128 + (((c >> 2) ^ (i & 3)) << 4)); }; /* of row 2 i + high */
-    T *to = static_cast<T *>(p.out) + (row0 + high) * p.out_row + n + c;
-    const int64_t res = (row0 + high) * p.residual_row + n + c;
-    if (row0 + 32 <= p.tokens) {
-#pragma unroll
-        for (uint32_t half = 0; half < 16; half += 8) {
-            float e[8];
-#pragma unroll
-            for (uint32_t i = 0; i < 8; ++i) e[i] = p.residual != nullptr ? load1(p.residual, res + (int64_t)(half + i) * 2 * p.residual_row, p.residual_type) : 0.0f;
-#pragma unroll
-            for (uint32_t i = 0; i < 8; ++i) {
-                const float v = value(half + i);
-                store1(to + (int64_t)(half + i) * 2 * p.out_row, p.residual != nullptr ? v + e[i] : v);
-            }
+/* Outputs n .. n + 3 of a token: the residual, the rounding and the store. kWide: whole and aligned, or past the end. */
+template <bool kWide>
+__device__ __forceinline__ void store4(const LinearParams &p, uint32_t token, uint32_t n, float4 v) {
+    if (token >= p.tokens || n >= p.outputs) return;
+    const int64_t to = token * p.out_row + n, from = token * p.residual_row + n;
+    if (kWide) {
+        if (p.residual != nullptr) {
+            const float4 e = load4(p.residual, from, p.residual_type);
+            v.x += e.x, v.y += e.y, v.z += e.z, v.w += e.w;
         }
+        put4(p.out, to, p.out_type, v);
         return;
     }
-    for (uint32_t i = 0; i < 16 && row0 + 2 * i + high < p.tokens; ++i) {
-        float v = value(i);
-        if (p.residual != nullptr) v += load1(p.residual, res + (int64_t)i * 2 * p.residual_row, p.residual_type);
-        store1(to + (int64_t)i * 2 * p.out_row, v);
-    }
-}
-__device__ __noinline__ void store_edge(const LinearParams &p, uint32_t row0, uint32_t n, uint32_t buffer) {
-    if (p.out_type == kBF16)
-        store_values<__nv_bfloat16>(p, row0, n, buffer);
-    else
-        store_values<float>(p, row0, n, buffer);
+    const float value[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (n + i < p.outputs)
+            store1(p.out, to + i, p.out_type, p.residual != nullptr ? value[i] + load1(p.residual, from + i, p.residual_type) : value[i]);
 }
 
-template <int kCtas, bool kFp8, bool pairs>
+/* 16 values of a lane of a block of 32 tokens by 16 outputs: those of output lane % 16 of every other token from lane / 16
+ * on. `at`: the first one's place; `row`: from a token to the next; `left`: tokens from the first one on. */
+template <typename T>
+__device__ __forceinline__ void load_column(const T *at, int64_t row, uint32_t left, float (&v)[16]) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i, at += 2 * row) v[i] = 2u * i < left ? load1(at) : 0.0f;
+}
+template <typename T>
+__device__ __forceinline__ void store_column(T *at, int64_t row, uint32_t left, const float (&v)[16]) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i, at += 2 * row)
+        if (2u * i < left) store1(at, v[i]);
+}
+
+/* kWide: rows of out and of the residual are whole pieces of four values that are aligned. The others are compiled by
+ * themselves: together they spilled 2.9 KB a thread. */
+template <int kCtas, bool kFp8, bool pairs, bool kWide>
 __global__ void __launch_bounds__(kLinearThreads, 1)
     linear_kernel(const __grid_constant__ LinearParams p, const __grid_constant__ CUtensorMap map_x,
                   const __grid_constant__ CUtensorMap map_w, const LinearShape g) {
@@ -525,9 +491,8 @@ __global__ void __launch_bounds__(kLinearThreads, 1)
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kEpilogueRegs));
         const uint32_t quarter = warp & 3, half = warp >> 2; /* TMEM lanes, and every other 16 columns */
         const uint32_t tmem = s->tmem;
-        const Wide wide(p);
         const bool has_res = p.residual != nullptr, f32_out = p.out_type == kF32;
-        const bool aligned = wide.out && (!has_res || wide.residual);
+        const bool out16 = ((reinterpret_cast<uintptr_t>(p.out) | (uintptr_t)p.out_row * 2 | (uintptr_t)p.outputs * 2) & 15) == 0; /* BF16 */
         /* 16-byte piece q of row r of a warp's buffer at r * 64 + (q ^ (r / 2 % 4)) * 16 */
         const uint32_t turn_base = smem_u32(turn_buffers) + warp * kTurnBytes;
         const uint32_t turn_out = turn_base + lane * 64, turn_out_x = (lane >> 1 & 3) * 16;
@@ -538,7 +503,6 @@ __global__ void __launch_bounds__(kLinearThreads, 1)
             const uint32_t n0 = tile / g.tiles_m * g.outs;
             const uint32_t row0 = (tile % g.tiles_m * kCtas + pair) * kRowsA + quarter * 32, token = row0 + lane;
             const float row_scale = kFp8 && token < p.tokens ? __ldcg(p.x_scales + token) : 0.0f;
-            const bool inside = aligned && row0 + 32 <= p.tokens;
             const int64_t out_at = (row0 + (lane >> 2)) * p.out_row + n0, res_at = (row0 + (lane >> 2)) * p.residual_row + n0 + (lane & 3) * 4;
             if (has_res && token < p.tokens) {
                 /* this row's part of the residual on its way to L2, in pieces of 128 bytes, while the MMAs run */
@@ -619,8 +583,9 @@ __global__ void __launch_bounds__(kLinearThreads, 1)
              * written. One lane's pieces are eight rows apart. */
             constexpr int kStep = pairs ? 2 : 1;
             if (!rows) {
-            } else if (!has_res && !f32_out && inside && wide.out16) {
+            } else if (kWide && !has_res && !f32_out && out16) {
                 /* BF16: two units to a turn, four pieces of eight values a row */
+                const uint32_t left = row0 + (lane >> 2) < p.tokens ? p.tokens - row0 - (lane >> 2) : 0;
 #pragma unroll
                 for (int set = 0; set < kSets; set += 2 * kStep) {
                     if (!have(set)) break;
@@ -629,38 +594,33 @@ __global__ void __launch_bounds__(kLinearThreads, 1)
                     finish<kFp8, pairs>(p, row_scale, sum[set], sum[set + (pairs ? 1 : 0)], scale + c, bias + c, g.outs);
                     if (second_one)
                         finish<kFp8, pairs>(p, row_scale, sum[set + kStep], sum[set + kStep + (pairs ? 1 : 0)], scale + c2, bias + c2, g.outs);
-                    if (n0 + (second_one ? c2 : c) + 16 <= p.outputs) {
-                        __syncwarp();
+                    __syncwarp();
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            float(&v)[16] = sum[set + (i >> 1) * kStep];
-                            const int o = (i & 1) * 8;
-                            store_shared4(turn_out + ((i * 16) ^ turn_out_x),
-                                          make_uint4(pack_bf16(v[o], v[o + 1]), pack_bf16(v[o + 2], v[o + 3]), pack_bf16(v[o + 4], v[o + 5]),
-                                                     pack_bf16(v[o + 6], v[o + 7])));
-                        }
-                        __syncwarp();
-                        __nv_bfloat16 *to = static_cast<__nv_bfloat16 *>(p.out) + out_at + ((lane & 2) ? c2 : c) + (lane & 1) * 8;
-                        if (second_one || (lane & 2) == 0) {
+                    for (int i = 0; i < 4; ++i) {
+                        float(&v)[16] = sum[set + (i >> 1) * kStep];
+                        const int o = (i & 1) * 8;
+                        store_shared4(turn_out + ((i * 16) ^ turn_out_x),
+                                      make_uint4(pack_bf16(v[o], v[o + 1]), pack_bf16(v[o + 2], v[o + 3]), pack_bf16(v[o + 4], v[o + 5]),
+                                                 pack_bf16(v[o + 6], v[o + 7])));
+                    }
+                    __syncwarp();
+                    const uint32_t n = ((lane & 2) ? c2 : c) + (lane & 1) * 8;
+                    __nv_bfloat16 *to = static_cast<__nv_bfloat16 *>(p.out) + out_at + n;
+                    if (n < g.outs && n0 + n < p.outputs) {
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4 *>(to + i * 8 * p.out_row) = load_shared_u4(turn_in + i * 512);
-                        }
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 2; ++e)
-                            if (e == 0 || second_one) {
-                                turn_rows(turn_out, turn_out_x, sum[set + e * kStep]);
-                                store_edge(p, row0, n0 + (e ? c2 : c), turn_base);
-                            }
+                        for (int i = 0; i < 4; ++i)
+                            if (8u * i < left) *reinterpret_cast<uint4 *>(to + i * 8 * p.out_row) = load_shared_u4(turn_in + i * 512);
                     }
                 }
-            } else {
+            } else if (kWide) {
+                const uint32_t left = row0 + (lane >> 2) < p.tokens ? p.tokens - row0 - (lane >> 2) : 0, mine = (lane & 3) * 4;
                 float4 e[4]; /* the residual of the next set */
                 auto load_residual = [&](int set) {
                     const uint32_t c = unit(set) * 16;
-                    if (has_res && inside && c < g.outs && n0 + c + 16 <= p.outputs) {
+                    if (has_res && have(set) && n0 + c + mine < p.outputs) {
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) e[i] = load4(p.residual, res_at + c + i * 8 * p.residual_row, p.residual_type);
+                        for (int i = 0; i < 4; ++i)
+                            if (8u * i < left) e[i] = load4(p.residual, res_at + c + i * 8 * p.residual_row, p.residual_type);
                     }
                 };
                 load_residual(0);
@@ -668,25 +628,52 @@ __global__ void __launch_bounds__(kLinearThreads, 1)
                 for (int set = 0; set < kSets; set += kStep) {
                     const uint32_t c = unit(set) * 16;
                     if (!have(set) || n0 + c >= p.outputs) break;
-                    const bool whole = inside && n0 + c + 16 <= p.outputs;
                     const float4 here[4] = {e[0], e[1], e[2], e[3]};
                     if (set + kStep < kSets) load_residual(set + kStep);
                     finish<kFp8, pairs>(p, row_scale, sum[set], sum[set + (pairs ? 1 : 0)], scale + c, bias + c, g.outs);
                     turn_rows(turn_out, turn_out_x, sum[set]);
-                    if (!whole) {
-                        store_edge(p, row0, n0 + c, turn_base);
-                        continue;
-                    }
-                    const int64_t to = out_at + c + (lane & 3) * 4;
+                    const int64_t to = out_at + c + mine;
+                    if (n0 + c + mine < p.outputs) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        float4 v = load_shared4(turn_in + i * 512);
-                        if (has_res) v.x += here[i].x, v.y += here[i].y, v.z += here[i].z, v.w += here[i].w;
+                        for (int i = 0; i < 4; ++i) {
+                            float4 v = load_shared4(turn_in + i * 512);
+                            if (has_res) v.x += here[i].x, v.y += here[i].y, v.z += here[i].z, v.w += here[i].w;
+                            if (8u * i < left) put4(p.out, to + i * 8 * p.out_row, p.out_type, v);
+                        }
+                    }
+                }
+            } else {
+                /* value by value: a column of every other token a lane */
+                const uint32_t column16 = lane & 15, high = lane >> 4, left = row0 + high < p.tokens ? p.tokens - row0 - high : 0;
+                const int64_t column_out = (row0 + high) * p.out_row + n0 + column16, column_res = (row0 + high) * p.residual_row + n0 + column16;
+                float e[16];
+                auto load_residual = [&](int set) {
+                    const uint32_t c = unit(set) * 16;
+                    if (!has_res || !have(set) || n0 + c + column16 >= p.outputs) return;
+                    if (p.residual_type == kF32)
+                        load_column(static_cast<const float *>(p.residual) + column_res + c, p.residual_row, left, e);
+                    else
+                        load_column(static_cast<const __nv_bfloat16 *>(p.residual) + column_res + c, p.residual_row, left, e);
+                };
+                load_residual(0);
+#pragma unroll
+                for (int set = 0; set < kSets; set += kStep) {
+                    const uint32_t c = unit(set) * 16;
+                    if (!have(set) || n0 + c >= p.outputs) break;
+                    float v[16];
+                    finish<kFp8, pairs>(p, row_scale, sum[set], sum[set + (pairs ? 1 : 0)], scale + c, bias + c, g.outs);
+                    turn_rows(turn_out, turn_out_x, sum[set]);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        v[i] = load_shared(turn_base + (2 * i + high) * 64 + (((column16 >> 2) ^ (i & 3)) << 4) + (column16 & 3) * 4);
+                        if (has_res) v[i] += e[i];
+                    }
+                    if (set + kStep < kSets) load_residual(set + kStep); /* the next one's, while this one is stored */
+                    if (n0 + c + column16 < p.outputs) {
                         if (f32_out)
-                            *reinterpret_cast<float4 *>(static_cast<float *>(p.out) + to + i * 8 * p.out_row) = v;
+                            store_column(static_cast<float *>(p.out) + column_out + c, p.out_row, left, v);
                         else
-                            *reinterpret_cast<uint2 *>(static_cast<__nv_bfloat16 *>(p.out) + to + i * 8 * p.out_row) =
-                                make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
+                            store_column(static_cast<__nv_bfloat16 *>(p.out) + column_out + c, p.out_row, left, v);
                     }
                 }
             }
@@ -723,7 +710,7 @@ __global__ void __launch_bounds__(kLinearThreads, 1)
                         }
                     if (bad) v[0] = v[1] = v[2] = v[3] = __int_as_float(0x7fc00000);
                     finish<kFp8, pairs>(p, kFp8 ? __ldcg(p.x_scales + m0 + m) : 0.0f, v, up, s->scale[0] + q4 * 4, s->bias[0] + q4 * 4, g.outs);
-                    store4(p, wide, m0 + m, n0 + q4 * 4, make_float4(v[0], v[1], v[2], v[3]));
+                    store4<kWide>(p, m0 + m, n0 + q4 * 4, make_float4(v[0], v[1], v[2], v[3]));
                 }
             }
         }
@@ -797,18 +784,18 @@ LinearShape shape_of(const LinearParams &p, uint32_t ctas, uint32_t n, uint32_t 
     return g;
 }
 
-template <int kCtas, bool kFp8, bool pairs>
+template <int kCtas, bool kFp8, bool pairs, bool kWide>
 cudaError_t launch_shape(const LinearParams &p, const LinearShape &g, int sms, cudaStream_t stream) {
     CUtensorMap map_x, map_w;
     cudaError_t e = encode(map_x, p, p.x, p.x_row, p.tokens, g.rows_a);
     if (e == cudaSuccess) e = encode(map_w, p, p.weight, p.weight_row, (uint64_t)p.outputs * (pairs ? 2 : 1), kCtas == 2 || pairs ? g.n / 2 : g.n);
     if (e != cudaSuccess) return e;
     const size_t smem = kSmemRest + (size_t)g.stages * g.sub * (kBytesA + g.n / kCtas * kBlock);
-    e = cudaFuncSetAttribute(linear_kernel<kCtas, kFp8, pairs>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemLimit);
+    e = cudaFuncSetAttribute(linear_kernel<kCtas, kFp8, pairs, kWide>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemLimit);
     if (e != cudaSuccess) return e;
     static const cudaError_t registers = [] {
         cudaFuncAttributes attr;
-        const cudaError_t error = cudaFuncGetAttributes(&attr, linear_kernel<kCtas, kFp8, pairs>);
+        const cudaError_t error = cudaFuncGetAttributes(&attr, linear_kernel<kCtas, kFp8, pairs, kWide>);
         return error != cudaSuccess ? error : (uint32_t)attr.numRegs * kLinearThreads < kSplitRegs ? cudaErrorInvalidKernelImage : cudaSuccess;
     }();
     if (registers != cudaSuccess) return registers;
@@ -828,21 +815,27 @@ cudaError_t launch_shape(const LinearParams &p, const LinearShape &g, int sms, c
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = group > 1 ? 2 : 1;
-    return cudaLaunchKernelEx(&cfg, linear_kernel<kCtas, kFp8, pairs>, p, map_x, map_w, g);
+    return cudaLaunchKernelEx(&cfg, linear_kernel<kCtas, kFp8, pairs, kWide>, p, map_x, map_w, g);
 }
 
 }  // namespace
 
 cudaError_t launch_linear_as(const LinearParams &p, uint32_t ctas, uint32_t n, uint32_t split, uint32_t sub, int sms, cudaStream_t stream) {
     const LinearShape g = shape_of(p, ctas, n, split, sub);
-    const bool fp8 = p.type == kE4M3;
-    if (p.activation == kSwiglu) {
-        auto *launch = ctas == 2 ? fp8 ? launch_shape<2, true, true> : launch_shape<2, false, true>
-                                 : fp8 ? launch_shape<1, true, true> : launch_shape<1, false, true>;
-        return launch(p, g, sms, stream);
-    }
-    auto *launch = ctas == 2 ? fp8 ? launch_shape<2, true, false> : launch_shape<2, false, false>
-                             : fp8 ? launch_shape<1, true, false> : launch_shape<1, false, false>;
+    auto pick = [&](auto pairs, auto wide) {
+        constexpr bool kPairs = decltype(pairs)::value, kWide = decltype(wide)::value;
+        if (p.type == kE4M3) return ctas == 2 ? launch_shape<2, true, kPairs, kWide> : launch_shape<1, true, kPairs, kWide>;
+        return ctas == 2 ? launch_shape<2, false, kPairs, kWide> : launch_shape<1, false, kPairs, kWide>;
+    };
+    using std::bool_constant;
+    auto aligned = [&](const void *at, int64_t row, int type) {
+        const uintptr_t size = type == kF32 ? 4 : 2;
+        return ((reinterpret_cast<uintptr_t>(at) | (p.tokens == 1 ? 0 : (uintptr_t)row * size)) & (4 * size - 1)) == 0;
+    };
+    const bool wide = p.outputs % 4 == 0 && aligned(p.out, p.out_row, p.out_type) &&
+                      (p.residual == nullptr || aligned(p.residual, p.residual_row, p.residual_type));
+    auto *launch = p.activation == kSwiglu ? wide ? pick(bool_constant<true>(), bool_constant<true>()) : pick(bool_constant<true>(), bool_constant<false>())
+                                           : wide ? pick(bool_constant<false>(), bool_constant<true>()) : pick(bool_constant<false>(), bool_constant<false>());
     return launch(p, g, sms, stream);
 }
 
