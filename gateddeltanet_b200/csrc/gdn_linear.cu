@@ -293,6 +293,11 @@ __device__ __forceinline__ float4 load4(const void *p, int64_t i, int type) {
     const uint2 w = __ldcg(reinterpret_cast<const uint2 *>(static_cast<const __nv_bfloat16 *>(p) + i));
     return make_float4(low_bf16(w.x), high_bf16(w.x), low_bf16(w.y), high_bf16(w.y));
 }
+/* four values as they are in memory */
+__device__ __forceinline__ float4 value4(const uint4 &w, int type) {
+    if (type == kF32) return make_float4(__uint_as_float(w.x), __uint_as_float(w.y), __uint_as_float(w.z), __uint_as_float(w.w));
+    return make_float4(low_bf16(w.x), high_bf16(w.x), low_bf16(w.y), high_bf16(w.y));
+}
 __device__ __forceinline__ void put4(void *p, int64_t i, int type, const float4 &v) {
     if (type == kF32)
         *reinterpret_cast<float4 *>(static_cast<float *>(p) + i) = v;
@@ -322,24 +327,44 @@ __device__ __forceinline__ void store4(const LinearParams &p, uint32_t token, ui
 /* 16 values of a lane of a block of 32 tokens by 16 outputs: those of output lane % 16 of every other token from lane / 16
  * on. `at`: the first one's place; `row`: from a token to the next; `left`: tokens from the first one on. */
 template <typename T>
-__device__ __forceinline__ void load_column(const T *at, int64_t row, uint32_t left, float (&v)[16]) {
+__device__ __forceinline__ void load_column(const T *at, int64_t row, uint32_t left, bool all, uint32_t (&v)[16]) {
+    auto one = [](const T *from) {
+        if constexpr (sizeof(T) == 4)
+            return __ldcg(reinterpret_cast<const uint32_t *>(from));
+        else
+            return (uint32_t)__ldcg(reinterpret_cast<const unsigned short *>(from));
+    };
+    if (all) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i, at += 2 * row) v[i] = 2u * i < left ? load1(at) : 0.0f;
+        for (int i = 0; i < 16; ++i, at += 2 * row) v[i] = one(at);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i, at += 2 * row) v[i] = 2u * i < left ? one(at) : 0u;
+    }
 }
 template <typename T>
-__device__ __forceinline__ void store_column(T *at, int64_t row, uint32_t left, const float (&v)[16]) {
+__device__ __forceinline__ void store_column(T *at, int64_t row, uint32_t left, bool all, const float (&v)[16]) {
+    if (all) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i, at += 2 * row)
-        if (2u * i < left) store1(at, v[i]);
+        for (int i = 0; i < 16; ++i, at += 2 * row) store1(at, v[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i, at += 2 * row)
+            if (2u * i < left) store1(at, v[i]);
+    }
 }
 
-/* kWide: rows of out and of the residual are whole pieces of four values that are aligned. The others are compiled by
- * themselves: together they spilled 2.9 KB a thread. */
-template <int kCtas, bool kFp8, bool pairs, bool kWide>
+/* How a block of results goes to memory: in pieces of four values, where rows of out and of the residual are whole
+ * aligned ones, or value by value, without a residual and with one. Compiled apart: together they spilled 2.9 KB a
+ * thread. */
+enum Way { kPieces = 0, kValues = 1, kValuesAdded = 2 };
+
+template <int kCtas, bool kFp8, bool pairs, int kWay>
 __global__ void __launch_bounds__(kLinearThreads, 1)
     linear_kernel(const __grid_constant__ LinearParams p, const __grid_constant__ CUtensorMap map_x,
                   const __grid_constant__ CUtensorMap map_w, const LinearShape g) {
     extern __shared__ uint8_t raw[];
+    constexpr bool kWide = kWay == kPieces;
     constexpr uint32_t kElem = kFp8 ? 1 : 2;
     const uint32_t start = (smem_u32(raw) + 1023u) & ~1023u;
     uint8_t *base = raw + (start - smem_u32(raw));
@@ -491,7 +516,7 @@ __global__ void __launch_bounds__(kLinearThreads, 1)
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kEpilogueRegs));
         const uint32_t quarter = warp & 3, half = warp >> 2; /* TMEM lanes, and every other 16 columns */
         const uint32_t tmem = s->tmem;
-        const bool has_res = p.residual != nullptr, f32_out = p.out_type == kF32;
+        const bool has_res = kWide ? p.residual != nullptr : kWay == kValuesAdded, f32_out = p.out_type == kF32;
         const bool out16 = ((reinterpret_cast<uintptr_t>(p.out) | (uintptr_t)p.out_row * 2 | (uintptr_t)p.outputs * 2) & 15) == 0; /* BF16 */
         /* 16-byte piece q of row r of a warp's buffer at r * 64 + (q ^ (r / 2 % 4)) * 16 */
         const uint32_t turn_base = smem_u32(turn_buffers) + warp * kTurnBytes;
@@ -503,7 +528,6 @@ __global__ void __launch_bounds__(kLinearThreads, 1)
             const uint32_t n0 = tile / g.tiles_m * g.outs;
             const uint32_t row0 = (tile % g.tiles_m * kCtas + pair) * kRowsA + quarter * 32, token = row0 + lane;
             const float row_scale = kFp8 && token < p.tokens ? __ldcg(p.x_scales + token) : 0.0f;
-            const int64_t out_at = (row0 + (lane >> 2)) * p.out_row + n0, res_at = (row0 + (lane >> 2)) * p.residual_row + n0 + (lane & 3) * 4;
             if (has_res && token < p.tokens) {
                 /* this row's part of the residual on its way to L2, in pieces of 128 bytes, while the MMAs run */
                 const int64_t size = p.residual_type == kF32 ? 4 : 2;
@@ -531,8 +555,52 @@ __global__ void __launch_bounds__(kLinearThreads, 1)
             auto have = [&](int set) { return unit(set) * 16 < g.outs; };
             auto column = [&](int set) { return unit(set) * 16 + (pairs && (set & 1) ? g.outs : 0); };
             const bool rows = row0 < p.tokens; /* this warp has any */
+            /* The residual of the sets, two ahead of the one that is finished, the first two from before the last sums
+             * are there: pieces of four values of eight tokens apart, or (not kWide) a column of every other token. */
+            constexpr int kStep = pairs ? 2 : 1;
+            const uint32_t piece = (lane & 3) * 4, column16 = lane & 15, high = kWide ? lane >> 2 : lane >> 4;
+            const uint32_t left = row0 + high < p.tokens ? p.tokens - row0 - high : 0; /* tokens from this lane's first one on */
+            const int64_t out_at = (row0 + high) * p.out_row + n0 + (kWide ? 0 : column16);
+            const int64_t res_at = (row0 + high) * p.residual_row + n0 + (kWide ? piece : column16);
+            const bool all = row0 + 32 <= p.tokens;
+            uint4 e[kWide ? 2 : 1][4];
+            uint32_t f[kWay == kValuesAdded ? 2 : 1][16];
+            auto load_residual = [&](int set) {
+                const int to = set / kStep & 1;
+                const uint32_t c = unit(set) * 16;
+                if (!has_res || set >= kSets || !have(set)) return;
+                if constexpr (kWide) {
+                    /* past the ends, where nothing is stored, the last token's and the tile's first outputs: the loads are not
+                     * branched around, so that nothing waits for one of them */
+                    const uint32_t n = n0 + c + piece < p.outputs ? n0 + c + piece : n0;
+                    int64_t at[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) at[i] = min(row0 + high + 8 * i, p.tokens - 1) * p.residual_row + n;
+                    if (p.residual_type == kF32) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) e[to][i] = __ldcg(reinterpret_cast<const uint4 *>(static_cast<const float *>(p.residual) + at[i]));
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const uint2 w = __ldcg(reinterpret_cast<const uint2 *>(static_cast<const __nv_bfloat16 *>(p.residual) + at[i]));
+                            e[to][i].x = w.x, e[to][i].y = w.y;
+                        }
+                    }
+                } else if constexpr (kWay == kValuesAdded) {
+                    if (n0 + c + column16 < p.outputs) {
+                        if (p.residual_type == kF32)
+                            load_column(static_cast<const float *>(p.residual) + res_at + c, p.residual_row, left, all, f[to]);
+                        else
+                            load_column(static_cast<const __nv_bfloat16 *>(p.residual) + res_at + c, p.residual_row, left, all, f[to]);
+                    }
+                }
+            };
             for (uint32_t b = b0; b < b1; b += g.chunk, ++seq) {
                 const uint32_t acc = seq & 1u;
+                if (b + g.chunk >= b1 && !(kCtas == 1 && g.split > 1)) {
+                    load_residual(0);
+                    load_residual(kStep);
+                }
                 ok = ok && wait_bar(sums_full + 8 * acc, (seq >> 1) & 1u, abort);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
@@ -581,11 +649,9 @@ __global__ void __launch_bounds__(kLinearThreads, 1)
             }
             /* A row of 16 values a lane is turned so that four lanes have one: whole sectors of memory are read and
              * written. One lane's pieces are eight rows apart. */
-            constexpr int kStep = pairs ? 2 : 1;
             if (!rows) {
             } else if (kWide && !has_res && !f32_out && out16) {
                 /* BF16: two units to a turn, four pieces of eight values a row */
-                const uint32_t left = row0 + (lane >> 2) < p.tokens ? p.tokens - row0 - (lane >> 2) : 0;
 #pragma unroll
                 for (int set = 0; set < kSets; set += 2 * kStep) {
                     if (!have(set)) break;
@@ -613,49 +679,36 @@ __global__ void __launch_bounds__(kLinearThreads, 1)
                     }
                 }
             } else if (kWide) {
-                const uint32_t left = row0 + (lane >> 2) < p.tokens ? p.tokens - row0 - (lane >> 2) : 0, mine = (lane & 3) * 4;
-                float4 e[4]; /* the residual of the next set */
-                auto load_residual = [&](int set) {
-                    const uint32_t c = unit(set) * 16;
-                    if (has_res && have(set) && n0 + c + mine < p.outputs) {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            if (8u * i < left) e[i] = load4(p.residual, res_at + c + i * 8 * p.residual_row, p.residual_type);
-                    }
-                };
-                load_residual(0);
 #pragma unroll
                 for (int set = 0; set < kSets; set += kStep) {
                     const uint32_t c = unit(set) * 16;
                     if (!have(set) || n0 + c >= p.outputs) break;
-                    const float4 here[4] = {e[0], e[1], e[2], e[3]};
-                    if (set + kStep < kSets) load_residual(set + kStep);
                     finish<kFp8, pairs>(p, row_scale, sum[set], sum[set + (pairs ? 1 : 0)], scale + c, bias + c, g.outs);
                     turn_rows(turn_out, turn_out_x, sum[set]);
-                    const int64_t to = out_at + c + mine;
-                    if (n0 + c + mine < p.outputs) {
+                    float4 v[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) v[i] = load_shared4(turn_in + i * 512);
+                    if (has_res) {
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            float4 v = load_shared4(turn_in + i * 512);
-                            if (has_res) v.x += here[i].x, v.y += here[i].y, v.z += here[i].z, v.w += here[i].w;
-                            if (8u * i < left) put4(p.out, to + i * 8 * p.out_row, p.out_type, v);
+                            const float4 r = value4(e[set / kStep & 1][i], p.residual_type);
+                            v[i].x += r.x, v[i].y += r.y, v[i].z += r.z, v[i].w += r.w;
                         }
                     }
+                    const bool have_piece = n0 + c + piece < p.outputs;
+                    const int64_t to = out_at + c + piece;
+                    if (f32_out) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (have_piece && 8u * i < left) put4(p.out, to + i * 8 * p.out_row, kF32, v[i]);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (have_piece && 8u * i < left) put4(p.out, to + i * 8 * p.out_row, kBF16, v[i]);
+                    }
+                    load_residual(set + 2 * kStep);
                 }
             } else {
-                /* value by value: a column of every other token a lane */
-                const uint32_t column16 = lane & 15, high = lane >> 4, left = row0 + high < p.tokens ? p.tokens - row0 - high : 0;
-                const int64_t column_out = (row0 + high) * p.out_row + n0 + column16, column_res = (row0 + high) * p.residual_row + n0 + column16;
-                float e[16];
-                auto load_residual = [&](int set) {
-                    const uint32_t c = unit(set) * 16;
-                    if (!has_res || !have(set) || n0 + c + column16 >= p.outputs) return;
-                    if (p.residual_type == kF32)
-                        load_column(static_cast<const float *>(p.residual) + column_res + c, p.residual_row, left, e);
-                    else
-                        load_column(static_cast<const __nv_bfloat16 *>(p.residual) + column_res + c, p.residual_row, left, e);
-                };
-                load_residual(0);
 #pragma unroll
                 for (int set = 0; set < kSets; set += kStep) {
                     const uint32_t c = unit(set) * 16;
@@ -666,15 +719,16 @@ __global__ void __launch_bounds__(kLinearThreads, 1)
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
                         v[i] = load_shared(turn_base + (2 * i + high) * 64 + (((column16 >> 2) ^ (i & 3)) << 4) + (column16 & 3) * 4);
-                        if (has_res) v[i] += e[i];
+                        if constexpr (kWay == kValuesAdded)
+                            v[i] += __uint_as_float(p.residual_type == kF32 ? f[set / kStep & 1][i] : f[set / kStep & 1][i] << 16);
                     }
-                    if (set + kStep < kSets) load_residual(set + kStep); /* the next one's, while this one is stored */
                     if (n0 + c + column16 < p.outputs) {
                         if (f32_out)
-                            store_column(static_cast<float *>(p.out) + column_out + c, p.out_row, left, v);
+                            store_column(static_cast<float *>(p.out) + out_at + c, p.out_row, left, all, v);
                         else
-                            store_column(static_cast<__nv_bfloat16 *>(p.out) + column_out + c, p.out_row, left, v);
+                            store_column(static_cast<__nv_bfloat16 *>(p.out) + out_at + c, p.out_row, left, all, v);
                     }
+                    load_residual(set + 2 * kStep);
                 }
             }
         }
@@ -784,18 +838,18 @@ LinearShape shape_of(const LinearParams &p, uint32_t ctas, uint32_t n, uint32_t 
     return g;
 }
 
-template <int kCtas, bool kFp8, bool pairs, bool kWide>
+template <int kCtas, bool kFp8, bool pairs, int kWay>
 cudaError_t launch_shape(const LinearParams &p, const LinearShape &g, int sms, cudaStream_t stream) {
     CUtensorMap map_x, map_w;
     cudaError_t e = encode(map_x, p, p.x, p.x_row, p.tokens, g.rows_a);
     if (e == cudaSuccess) e = encode(map_w, p, p.weight, p.weight_row, (uint64_t)p.outputs * (pairs ? 2 : 1), kCtas == 2 || pairs ? g.n / 2 : g.n);
     if (e != cudaSuccess) return e;
     const size_t smem = kSmemRest + (size_t)g.stages * g.sub * (kBytesA + g.n / kCtas * kBlock);
-    e = cudaFuncSetAttribute(linear_kernel<kCtas, kFp8, pairs, kWide>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemLimit);
+    e = cudaFuncSetAttribute(linear_kernel<kCtas, kFp8, pairs, kWay>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemLimit);
     if (e != cudaSuccess) return e;
     static const cudaError_t registers = [] {
         cudaFuncAttributes attr;
-        const cudaError_t error = cudaFuncGetAttributes(&attr, linear_kernel<kCtas, kFp8, pairs, kWide>);
+        const cudaError_t error = cudaFuncGetAttributes(&attr, linear_kernel<kCtas, kFp8, pairs, kWay>);
         return error != cudaSuccess ? error : (uint32_t)attr.numRegs * kLinearThreads < kSplitRegs ? cudaErrorInvalidKernelImage : cudaSuccess;
     }();
     if (registers != cudaSuccess) return registers;
@@ -815,27 +869,30 @@ cudaError_t launch_shape(const LinearParams &p, const LinearShape &g, int sms, c
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = group > 1 ? 2 : 1;
-    return cudaLaunchKernelEx(&cfg, linear_kernel<kCtas, kFp8, pairs, kWide>, p, map_x, map_w, g);
+    return cudaLaunchKernelEx(&cfg, linear_kernel<kCtas, kFp8, pairs, kWay>, p, map_x, map_w, g);
 }
 
 }  // namespace
 
 cudaError_t launch_linear_as(const LinearParams &p, uint32_t ctas, uint32_t n, uint32_t split, uint32_t sub, int sms, cudaStream_t stream) {
     const LinearShape g = shape_of(p, ctas, n, split, sub);
-    auto pick = [&](auto pairs, auto wide) {
-        constexpr bool kPairs = decltype(pairs)::value, kWide = decltype(wide)::value;
-        if (p.type == kE4M3) return ctas == 2 ? launch_shape<2, true, kPairs, kWide> : launch_shape<1, true, kPairs, kWide>;
-        return ctas == 2 ? launch_shape<2, false, kPairs, kWide> : launch_shape<1, false, kPairs, kWide>;
+    auto pick = [&](auto pairs, auto way) {
+        constexpr bool kPairs = decltype(pairs)::value;
+        constexpr int kWay = decltype(way)::value;
+        if (p.type == kE4M3) return ctas == 2 ? launch_shape<2, true, kPairs, kWay> : launch_shape<1, true, kPairs, kWay>;
+        return ctas == 2 ? launch_shape<2, false, kPairs, kWay> : launch_shape<1, false, kPairs, kWay>;
     };
-    using std::bool_constant;
+    auto pick_way = [&](auto pairs, bool wide) {
+        if (wide) return pick(pairs, std::integral_constant<int, kPieces>());
+        return p.residual == nullptr ? pick(pairs, std::integral_constant<int, kValues>()) : pick(pairs, std::integral_constant<int, kValuesAdded>());
+    };
     auto aligned = [&](const void *at, int64_t row, int type) {
         const uintptr_t size = type == kF32 ? 4 : 2;
         return ((reinterpret_cast<uintptr_t>(at) | (p.tokens == 1 ? 0 : (uintptr_t)row * size)) & (4 * size - 1)) == 0;
     };
     const bool wide = p.outputs % 4 == 0 && aligned(p.out, p.out_row, p.out_type) &&
                       (p.residual == nullptr || aligned(p.residual, p.residual_row, p.residual_type));
-    auto *launch = p.activation == kSwiglu ? wide ? pick(bool_constant<true>(), bool_constant<true>()) : pick(bool_constant<true>(), bool_constant<false>())
-                                           : wide ? pick(bool_constant<false>(), bool_constant<true>()) : pick(bool_constant<false>(), bool_constant<false>());
+    auto *launch = p.activation == kSwiglu ? pick_way(std::true_type(), wide) : pick_way(std::false_type(), wide);
     return launch(p, g, sms, stream);
 }
 
