@@ -6,10 +6,20 @@
  * The mean is that of the unrounded sums h, in FP32.
  *
  * Bound by HBM: each value is read and written once. A row is held in
- * registers by a group of threads, eight values (or sixteen) each, from the
- * loads to the stores; the sum of squares, and the largest value of a token
- * for its scale, are met through shuffles and shared memory in a fixed order.
+ * registers by a group of threads, sixteen values each, from the loads to the
+ * stores; the sum of squares, and the largest value of a token for its scale,
+ * are met through shuffles and shared memory in a fixed order. What would cost
+ * most is the wait for a row's loads and its two meetings, so each CTA takes
+ * rows in turn and the loads of the next one are on their way meanwhile: one
+ * row to a CTA without that took 41.6 us where this took 16.4, a ring of rows in
+ * shared memory 28.7 where this took 22.5.
+ *
+ * Measured: 4096 x 2048 BF16 with an FP32 residual, to 8 bits, 17.8 us (5.2
+ * TB/s), with a BF16 residual, to BF16, 14.4 us (4.7 TB/s), 4096 x 8 gated heads
+ * of 256 14.4 us (3.5 TB/s), one row of 2048 2.1 us, which is the launch.
  */
+#include <type_traits>
+
 #include "gdn_ops.h"
 #include "gdn_values.h"
 
@@ -64,29 +74,17 @@ __device__ __forceinline__ float meet(float v, uint32_t group, bool all, float *
     return v;
 }
 
-/* Eight values of a row as they are in memory (kWide: neighbours, in one or two 16-byte vectors; else values
- * `step` apart): fetched ahead, and FP32 when they are used. */
-template <typename T, bool kWide>
-struct Eight;
-template <>
-struct Eight<__nv_bfloat16, true> {
-    uint4 w;
-    __device__ __forceinline__ void fetch(const __nv_bfloat16 *p, uint32_t, uint32_t) { w = __ldcg(reinterpret_cast<const uint4 *>(p)); }
-    __device__ __forceinline__ void get(float (&v)[8]) const { unpack8(w, v); }
-};
-template <>
-struct Eight<float, true> {
-    float4 a, b;
-    __device__ __forceinline__ void fetch(const float *p, uint32_t, uint32_t) {
-        a = __ldcg(reinterpret_cast<const float4 *>(p));
-        b = __ldcg(reinterpret_cast<const float4 *>(p) + 1);
-    }
-    __device__ __forceinline__ void get(float (&v)[8]) const {
-        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-    }
-};
-template <typename T>
-struct Eight<T, false> {
+/* How a thread's eight values lie in a row, `step` values between its pieces:
+ *   kEights  neighbours, on 16-byte boundaries (of 8 bits on 8 bytes)
+ *   kQuads   two pieces of four, where a row's length or boundaries allow no more
+ *   kSingles one by one, for rows off the boundaries of these pieces
+ * 4096 rows of 2044 BF16 values and residuals take 15.7 us in pieces of four, 31.0 one by one; of 2048 values with an
+ * FP32 residual, to 8 bits, 17.8 by eights, 19.1 by fours. */
+enum Layout { kEights, kQuads, kSingles };
+
+/* Eight values as they are in memory: fetched ahead, and FP32 when they are used. */
+template <typename T, Layout kLayout>
+struct Eight {
     float x[8];
     __device__ __forceinline__ void fetch(const T *p, uint32_t step, uint32_t left) {
 #pragma unroll
@@ -97,18 +95,69 @@ struct Eight<T, false> {
         for (int j = 0; j < 8; ++j) v[j] = x[j];
     }
 };
+template <>
+struct Eight<__nv_bfloat16, kEights> {
+    uint4 w;
+    __device__ __forceinline__ void fetch(const __nv_bfloat16 *p, uint32_t, uint32_t) { w = __ldcg(reinterpret_cast<const uint4 *>(p)); }
+    __device__ __forceinline__ void get(float (&v)[8]) const { unpack8(w, v); }
+};
+template <>
+struct Eight<float, kEights> {
+    float4 a, b;
+    __device__ __forceinline__ void fetch(const float *p, uint32_t, uint32_t) {
+        a = __ldcg(reinterpret_cast<const float4 *>(p));
+        b = __ldcg(reinterpret_cast<const float4 *>(p) + 1);
+    }
+    __device__ __forceinline__ void get(float (&v)[8]) const {
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    }
+};
+template <>
+struct Eight<__nv_bfloat16, kQuads> {
+    uint2 a, b;
+    __device__ __forceinline__ void fetch(const __nv_bfloat16 *p, uint32_t step, uint32_t left) {
+        a = __ldcg(reinterpret_cast<const uint2 *>(p));
+        b = step < left ? __ldcg(reinterpret_cast<const uint2 *>(p + step)) : make_uint2(0, 0);
+    }
+    __device__ __forceinline__ void get(float (&v)[8]) const { unpack8(make_uint4(a.x, a.y, b.x, b.y), v); }
+};
+template <>
+struct Eight<float, kQuads> {
+    float4 a, b;
+    __device__ __forceinline__ void fetch(const float *p, uint32_t step, uint32_t left) {
+        a = __ldcg(reinterpret_cast<const float4 *>(p));
+        b = step < left ? __ldcg(reinterpret_cast<const float4 *>(p + step)) : make_float4(0, 0, 0, 0);
+    }
+    __device__ __forceinline__ void get(float (&v)[8]) const {
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    }
+};
+template <Layout kLayout, typename T>
+__device__ __forceinline__ void store_eight(T *p, uint32_t step, uint32_t left, const float (&v)[8]) {
+    if constexpr (kLayout == kEights) {
+        store8(p, v);
+    } else if constexpr (kLayout == kQuads) {
+        store4(p, v[0], v[1], v[2], v[3]);
+        if (step < left) store4(p + step, v[4], v[5], v[6], v[7]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (j * step < left) store1(p + j * step, v[j]);
+    }
+}
 
-/* T: type of x and gate; R: of the residual. kWide: eight neighbours to a vector, all rows on 16-byte
- * boundaries; else values `group` apart. kN: eights of values a thread. kAhead: CTAs of up to kSmall
+/* T: type of x and gate; R: of the residual. kN: eights of values a thread. kAhead: CTAs of up to kSmall
  * threads, which have the registers to fetch the next row's values while one's meet. */
 constexpr int ctas_of(int n) { return n == 1 ? 3 : n == 2 ? 2 : 1; } /* that fit an SM with their registers */
-template <typename T, typename R, bool kWide, int kN, bool kAhead>
+template <typename T, typename R, Layout kLayout, int kN, bool kAhead>
 __global__ void __launch_bounds__(kAhead ? kSmall : kMaxNormThreads, kAhead ? ctas_of(kN) : 1) norm_kernel(const __grid_constant__ NormParams p, const NormShape g) {
     __shared__ float partial[2][kMaxNormThreads / 32];
     const uint32_t tid = threadIdx.x, r = tid / g.group, t = tid % g.group, rows = p.tokens * p.heads;
-    const uint32_t step = kWide ? 1 : g.group; /* from one of a thread's eight values to the next */
-    auto at = [&](int i) { return kWide ? (i * g.group + t) * 8 : i * 8 * g.group + t; };
+    const uint32_t step = kLayout == kEights ? 8 : kLayout == kQuads ? 4 * g.group : g.group;
+    auto at = [&](int i) { return kLayout == kEights ? (i * g.group + t) * 8 : i * 8 * g.group + (kLayout == kQuads ? 4 * t : t); };
     auto left = [&](int i) { return p.dim > at(i) ? p.dim - at(i) : 0u; };
+    /* where the j-th of eight is from the first */
+    auto apart = [&](int j) { return kLayout == kEights ? (uint32_t)j : kLayout == kQuads ? j / 4 * step + j % 4 : j * step; };
 
     wait_for_previous();
     let_next_start();
@@ -120,8 +169,14 @@ __global__ void __launch_bounds__(kAhead ? kSmall : kMaxNormThreads, kAhead ? ct
             for (int j = 0; j < 8; ++j) w[i][j] = 0.0f;
 #pragma unroll
         for (int i = 0; i < kN; ++i) {
-            if (kWide) {
+            if (kLayout == kEights) {
                 if (left(i)) load8(p.weight, at(i), p.weight_type, w[i]);
+            } else if (kLayout == kQuads && p.weight_type == kF32) {
+                Eight<float, kQuads> v;
+                if (left(i)) v.fetch(static_cast<const float *>(p.weight) + at(i), step, left(i)), v.get(w[i]);
+            } else if (kLayout == kQuads) {
+                Eight<__nv_bfloat16, kQuads> v;
+                if (left(i)) v.fetch(static_cast<const __nv_bfloat16 *>(p.weight) + at(i), step, left(i)), v.get(w[i]);
             } else {
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
@@ -129,8 +184,8 @@ __global__ void __launch_bounds__(kAhead ? kSmall : kMaxNormThreads, kAhead ? ct
             }
         }
     }
-    Eight<T, kWide> x[kN], z[kN];
-    Eight<R, kWide> e[kN];
+    Eight<T, kLayout> x[kN], z[kN];
+    Eight<R, kLayout> e[kN];
     const float per_dim = 1.0f / (float)p.dim;
     /* this thread's row, and the step to its next one */
     uint32_t row = blockIdx.x * g.rows + r, token = row / p.heads, head = row - token * p.heads;
@@ -180,13 +235,7 @@ __global__ void __launch_bounds__(kAhead ? kSmall : kMaxNormThreads, kAhead ? ct
                     e[i].get(v);
 #pragma unroll
                     for (int j = 0; j < 8; ++j) h[i][j] += v[j];
-                    if (kWide) {
-                        store8(res + at(i), h[i]);
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 8; ++j)
-                            if (j * step < left(i)) store1(res + at(i) + j * step, h[i][j]);
-                    }
+                    store_eight<kLayout>(res + at(i), step, left(i), h[i]);
                 }
         }
         row += row_step, token += token_step, head += head_step;
@@ -221,7 +270,7 @@ __global__ void __launch_bounds__(kAhead ? kSmall : kMaxNormThreads, kAhead ? ct
             for (int i = 0; i < kN; ++i)
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
-                    if (live && (uint32_t)j * step < left(i)) top = larger(top, fabsf(h[i][j]));
+                    if (live && apart(j) < left(i)) top = larger(top, fabsf(h[i][j]));
             top = meet<true, kAhead>(top, g.group, g.token != 0, partial[1]);
             float scale = top / 448.0f;
             if (scale < 0x1p-126f) scale = 0x1p-126f; /* not for a NaN */
@@ -231,36 +280,41 @@ __global__ void __launch_bounds__(kAhead ? kSmall : kMaxNormThreads, kAhead ? ct
 #pragma unroll
             for (int i = 0; i < kN; ++i) {
                 if (!live || !left(i)) continue;
-                if (kWide) {
+                if constexpr (kLayout == kSingles) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        if (j * step < left(i)) o[at(i) + j * step] = __nv_cvt_float_to_fp8(h[i][j] * inv, __NV_SATFINITE, __NV_E4M3);
+                } else {
                     uint32_t b[4];
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
                         b[j] = __nv_cvt_float2_to_fp8x2(make_float2(h[i][2 * j] * inv, h[i][2 * j + 1] * inv), __NV_SATFINITE, __NV_E4M3);
-                    *reinterpret_cast<uint2 *>(o + at(i)) = make_uint2(b[0] | (b[1] << 16), b[2] | (b[3] << 16));
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        if (j * step < left(i)) o[at(i) + j * step] = __nv_cvt_float_to_fp8(h[i][j] * inv, __NV_SATFINITE, __NV_E4M3);
+                    const uint2 v = make_uint2(b[0] | (b[1] << 16), b[2] | (b[3] << 16));
+                    if constexpr (kLayout == kEights) {
+                        *reinterpret_cast<uint2 *>(o + at(i)) = v;
+                    } else {
+                        *reinterpret_cast<uint32_t *>(o + at(i)) = v.x;
+                        if (step < left(i)) *reinterpret_cast<uint32_t *>(o + at(i) + step) = v.y;
+                    }
                 }
             }
         } else {
 #pragma unroll
             for (int i = 0; i < kN; ++i) {
                 if (!live || !left(i)) continue;
-                if (kWide) {
+                if constexpr (kLayout == kEights)
                     store8(p.out, out + at(i), p.out_type, h[i]);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        if (j * step < left(i)) store1(p.out, out + at(i) + j * step, p.out_type, h[i][j]);
-                }
+                else if (p.out_type == kBF16)
+                    store_eight<kLayout>(static_cast<__nv_bfloat16 *>(p.out) + out + at(i), step, left(i), h[i]);
+                else
+                    store_eight<kLayout>(static_cast<float *>(p.out) + out + at(i), step, left(i), h[i]);
             }
         }
         if (g.group > 32 || g.token) __syncthreads(); /* `partial` is free again */
     }
 }
 
-template <typename T, typename R, bool kWide, int kN, bool kAhead>
+template <typename T, typename R, Layout kLayout, int kN, bool kAhead>
 cudaError_t launch_norm_t(const NormParams &p, int sms, cudaStream_t stream) {
     NormShape g;
     g.group = norm_group(p.dim, 8 * kN);
@@ -269,35 +323,48 @@ cudaError_t launch_norm_t(const NormParams &p, int sms, cudaStream_t stream) {
     const uint32_t block = (g.group * g.rows + 31) / 32 * 32;
     /* as many CTAs as run at once, each with rows in turn */
     const uint32_t all = (p.tokens * p.heads + g.rows - 1) / g.rows, most = (uint32_t)sms * ((kAhead ? ctas_of(kN) * kSmall : kMaxNormThreads) / block);
-    return launch_overlapped(norm_kernel<T, R, kWide, kN, kAhead>, dim3(all < most ? all : most), block, 0, stream, p, g);
+    return launch_overlapped(norm_kernel<T, R, kLayout, kN, kAhead>, dim3(all < most ? all : most), block, 0, stream, p, g);
 }
 
-/* rows of an operand that all start on a 16-byte boundary (8 bytes of 8-bit values) */
-bool wide_rows(const void *p, int64_t token, int64_t head, const NormParams &n, int64_t size) {
-    if (p == nullptr) return true;
-    const int64_t step = 8 * size < 16 ? 8 : 16;
-    return reinterpret_cast<uintptr_t>(p) % step == 0 && (n.tokens == 1 || token * size % step == 0) &&
-           (n.heads == 1 || head * size % step == 0);
+/* rows of an operand that all start on a boundary of `values` of its values, of 16 bytes at most */
+bool rows_on(uint32_t values, const void *p, int64_t token, int64_t head, const NormParams &n, int type) {
+    const int64_t size = type == kF32 ? 4 : type == kBF16 ? 2 : 1, step = size * values < 16 ? size * values : 16;
+    return p == nullptr || (reinterpret_cast<uintptr_t>(p) % step == 0 && (n.tokens == 1 || token * size % step == 0) &&
+                            (n.heads == 1 || head * size % step == 0));
 }
 
 template <typename T>
 cudaError_t launch_norm_x(const NormParams &p, int sms, cudaStream_t stream) {
-    auto size = [](int type) { return type == kF32 ? 4 : type == kBF16 ? 2 : 1; };
-    const bool wide = p.dim % 8 == 0 && wide_rows(p.x, p.x_token, p.x_head, p, sizeof(T)) &&
-                      wide_rows(p.gate, p.gate_token, p.gate_head, p, sizeof(T)) &&
-                      wide_rows(p.residual, p.residual_token, p.residual_head, p, size(p.residual_type)) &&
-                      wide_rows(p.out, p.out_token, p.out_head, p, size(p.out_type)) && on16(p.weight);
-    /* eight values a thread, or sixteen where a CTA would have too few threads */
+    auto all_on = [&](uint32_t values) {
+        return p.dim % values == 0 && rows_on(values, p.x, p.x_token, p.x_head, p, p.type) &&
+               rows_on(values, p.gate, p.gate_token, p.gate_head, p, p.type) &&
+               rows_on(values, p.residual, p.residual_token, p.residual_head, p, p.residual_type) &&
+               rows_on(values, p.out, p.out_token, p.out_head, p, p.out_type);
+    };
+    const bool weight_on16 = on16(p.weight);
+    const int layout = all_on(8) && weight_on16 ? kEights : all_on(4) && weight_on16 ? kQuads : kSingles;
+    /* Sixteen values a thread, or thirty-two of long rows: 4096 rows of 2048 FP32 values to BF16 take 11.6 us so and
+     * 12.7 with eight, with an FP32 residual 21.0 and 20.7. One by one eight, for want of registers. Rows too long for
+     * 256 threads are not fetched ahead. */
+    auto pick_as = [&](auto r, auto as) {
+        using R = decltype(r);
+        constexpr Layout kL = decltype(as)::value;
+        if constexpr (kL != kSingles) {
+            if (norm_threads(p, 16) <= kSmall) return launch_norm_t<T, R, kL, 2, true>;
+            if (norm_threads(p, 32) <= kSmall) return launch_norm_t<T, R, kL, 4, true>;
+        } else if (norm_threads(p, 8) <= kSmall) {
+            return launch_norm_t<T, R, kL, 1, true>;
+        }
+        return norm_threads(p, 8) <= kMaxNormThreads ? launch_norm_t<T, R, kL, 1, false> : launch_norm_t<T, R, kL, 2, false>;
+    };
     auto pick = [&](auto r) {
         using R = decltype(r);
-        if (wide && sizeof(T) == 4 && norm_threads(p, 8) <= kSmall) return launch_norm_t<T, R, true, 1, true>;
-        if (wide && norm_threads(p, 16) <= kSmall) return launch_norm_t<T, R, true, 2, true>;
-        if (wide && norm_threads(p, 32) <= kSmall) return launch_norm_t<T, R, true, 4, true>;
-        if (!wide && norm_threads(p, 8) <= kSmall) return launch_norm_t<T, R, false, 1, true>;
-        if (norm_threads(p, 8) <= kMaxNormThreads) return wide ? launch_norm_t<T, R, true, 1, false> : launch_norm_t<T, R, false, 1, false>;
-        return wide ? launch_norm_t<T, R, true, 2, false> : launch_norm_t<T, R, false, 2, false>;
+        return layout == kEights  ? pick_as(r, std::integral_constant<Layout, kEights>())
+               : layout == kQuads ? pick_as(r, std::integral_constant<Layout, kQuads>())
+                                  : pick_as(r, std::integral_constant<Layout, kSingles>());
     };
-    auto *launch = p.residual != nullptr && p.residual_type == kBF16 ? pick(__nv_bfloat16()) : pick(float());
+    /* without a residual its type is x's */
+    auto *launch = (p.residual != nullptr ? p.residual_type : p.type) == kBF16 ? pick(__nv_bfloat16()) : pick(float());
     return launch(p, sms, stream);
 }
 
@@ -309,3 +376,4 @@ cudaError_t launch_norm(const NormParams &p, int sms, cudaStream_t stream) {
 
 }  // namespace ops
 }  // namespace gdn
+

@@ -97,6 +97,29 @@ def test_norm_strides(ops, extra, out_type):
         plain.check(out, want, off, "out")
 
 
+@pytest.mark.parametrize("dim", [4, 12, 2044, 4100, 8188, 8204, 16380])
+@pytest.mark.parametrize("x_type,res_type,out_type", [(BF16, BF16, BF16), (BF16, F32, E4M3), (F32, BF16, F32), (BF16, None, F32)], ids=str)
+@pytest.mark.parametrize("shift", [0, 4, 2])
+def test_norm_rows_of_fours(ops, dim, x_type, res_type, out_type, shift):
+    """Lengths that are multiples of four alone, on 8-byte boundaries of BF16 rows and off them."""
+    x = rand(5 * dim + shift, seed=2, dtype=x_type)[shift:].view(5, dim)
+    weight = rand(dim, seed=3, dtype=BF16)
+    residual = None if res_type is None else rand(5, dim + 4, seed=4, dtype=res_type)[:, :dim]
+    kept = None if res_type is None else residual._base[:, dim:].clone()
+    far = torch.full((5, dim + 4), 7.0, device="cuda").to(out_type)
+    want, h = plain.norm(x, weight, residual)
+    got = ops.rms_norm(x, weight, residual=residual, dtype=out_type, out=far[:, :dim])
+    off = plain.norm_error(None) * want.abs()
+    if residual is not None:
+        plain.check(residual, h, plain.U * h.abs(), "residual")
+        assert torch.equal(residual._base[:, dim:], kept)
+    assert bool((far[:, dim:].float() == 7).all())
+    if out_type == E4M3:
+        check_eight(got, want, off)
+    else:
+        plain.check(got, want, off, "out")
+
+
 def test_norm_heads_before_tokens(ops):
     x = rand(4, 6, 128, dtype=BF16).transpose(0, 1)
     want, _ = plain.norm(x)
