@@ -897,12 +897,12 @@ cudaError_t launch_linear_as(const LinearParams &p, uint32_t ctas, uint32_t n, u
 }
 
 /* The tiles of a call are those for which this estimate is least. What it knows, in us on 148 SMs: a block of k takes
- * 0.0018 n + 0.034 in one CTA (0.3 at least: the MMA reads 128 tokens whatever n is, and a wait is not hidden) and
- * 0.0013 n + 0.067 in two; a launch 5.0 or 5.7 and 0.008 n for the last tile's way to memory; a further tile of a CTA
- * 0.5; a cluster that divides k 0.6 + 0.5 a CTA. Of clusters of four and eight not as many as there are SMs for run at
- * once (13 of eight did, 16 did not). Against sweeps of 110 calls (17 to 4096 tokens, 2048 and 5632 inputs, 2048 to
- * 32000 outputs, both types) its choices were 1.7 % slower than the best tiles in the mean; 256 columns always,
- * or 128 split as far as possible, were up to twice as slow at either end. */
+ * 0.0014 n + 0.07 in one CTA and 0.00125 n + 0.04 in two, of which each computes half the columns of both; a launch
+ * 4.5 or 5.4; each tile of a CTA 1.5; a cluster that divides k 0.7 + 0.2 a CTA. Of clusters of four and eight not as
+ * many as there are SMs for run at once (13 of eight did, 16 did not). Against sweeps of all tiles of 196 calls (17 to
+ * 4096 tokens, 128 to 5632 inputs, 501 to 32000 outputs, both types, all activations) its choices were 0.8 % slower
+ * than the best tiles in the mean; 256 columns always, or 128 split as far as possible, were up to twice as slow at
+ * either end. */
 cudaError_t launch_linear(const LinearParams &p, int sms, cudaStream_t stream) {
     const uint32_t blocks = (uint32_t)(((uint64_t)p.inputs * (p.type == kE4M3 ? 1 : 2) + kBlock - 1) / kBlock);
     float least = 3.4e38f;
@@ -911,13 +911,13 @@ cudaError_t launch_linear(const LinearParams &p, int sms, cudaStream_t stream) {
         for (uint32_t width = 32; width <= kMaxN; width += 32) {
             const uint32_t outs = p.activation == kSwiglu ? width / 2 : width;
             const uint64_t tiles = (uint64_t)((p.tokens + c * kRowsA - 1) / (c * kRowsA)) * ((p.outputs + outs - 1) / outs);
-            const float block = c == 2 ? 0.0013f * width + 0.067f : 0.0018f * width + 0.034f > 0.3f ? 0.0018f * width + 0.034f : 0.3f;
+            const float block = c == 2 ? 0.00125f * width + 0.04f : 0.0014f * width + 0.07f;
             for (uint32_t s = 1; s <= (c == 1 ? 8u : 1u); s *= 2) {
                 const uint64_t most = (uint64_t)sms * (s < 4 ? 8 : s == 4 ? 7 : 6) / 8;
                 if (s > 1 && (tiles * s > most || blocks / s < 4)) break;
                 const uint64_t waves = (tiles * c * s + sms - 1) / sms;
-                const float t = (float)waves * ((float)((blocks + s - 1) / s) * block + 0.5f) + 0.008f * width + (c == 2 ? 5.7f : 5.0f) +
-                                (s > 1 ? 0.6f + 0.5f * s : 0.0f);
+                const float t = (float)waves * ((float)((blocks + s - 1) / s) * block + 1.5f) + 0.001f * width + (c == 2 ? 5.4f : 4.5f) +
+                                (s > 1 ? 0.7f + 0.2f * s : 0.0f);
                 if (t < least) least = t, ctas = c, n = width, split = s;
             }
         }
