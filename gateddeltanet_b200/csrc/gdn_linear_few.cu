@@ -10,6 +10,11 @@
  * four). Nothing passes through shared memory but the sums: the warps of a CTA
  * share its rows and divide k between them, and their partial sums are added in
  * the order of the warps.
+ *
+ * Measured: one token of 2048 inputs by 8208 outputs of BF16 7.1 us (4.7 TB/s),
+ * by 32000 19.9 us (6.6 TB/s, the rate of a copy), of 8 bits 6.3 and 14.9 us;
+ * what small calls take above the bytes is the launch and one wait for memory,
+ * about 2.5 us. 16 tokens read as much of x as of W: 11.4 and 28.6 us.
  */
 #include "gdn_linear.h"
 
@@ -94,8 +99,6 @@ __global__ void __launch_bounds__(kMaxWarps * 32) linear_few_kernel(const __grid
     const uint32_t tid = threadIdx.x, warp = tid >> 5, warps = blockDim.x >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const uint32_t n0 = blockIdx.x * 16, size = p.inputs * (kFp8 ? 1 : 2);
     const uint32_t elem = kFp8 ? 1 : 2;
-    wait_for_previous();
-    let_next_start();
     /* rows past the ends are read as the last one: their sums go nowhere */
     const uint8_t *w[kHalves][2], *x[kGroups];
 #pragma unroll
@@ -113,6 +116,21 @@ __global__ void __launch_bounds__(kMaxWarps * 32) linear_few_kernel(const __grid
 #pragma unroll
             for (int i = 0; i < 4; ++i) d[h][n][i] = 0.0f;
 
+    const uint32_t whole = size / (kAhead * 64) * (kAhead * 64), stride = warps * kAhead * 64;
+    uint32_t k0 = warp * kAhead * 64;
+    /* Before the kernel before this one has ended, the first rows of W are on their way to L2 (which the loads below
+     * read: they see what that kernel wrote). One row of 2048 by 8208 of BF16 7.1 us instead of 8.1, by 2048 3.1 instead
+     * of 3.5; all of a warp's rows 7.9. 8-bit rows without pairs do not gain (by 32000 15.4 us instead of 14.9). */
+    if ((!kFp8 || kPairs) && k0 < whole) {
+#pragma unroll
+        for (int s = 0; s < kAhead; ++s)
+#pragma unroll
+            for (int h = 0; h < kHalves; ++h)
+#pragma unroll
+                for (int r = 0; r < 2; ++r) asm volatile("prefetch.global.L2 [%0];" ::"l"(w[h][r] + k0 + s * 64));
+    }
+    wait_for_previous();
+    let_next_start();
     struct Loads {
         uint4 a[kAhead][kHalves][2], b[kAhead][kGroups];
     };
@@ -134,8 +152,6 @@ __global__ void __launch_bounds__(kMaxWarps * 32) linear_few_kernel(const __grid
             for (int h = 0; h < kHalves; ++h) products<kFp8, kGroups>(d[h], l.a[s][h][0], l.a[s][h][1], l.b[s]);
     };
     /* the whole steps, in turn over the warps, each time with the next one's loads under way */
-    const uint32_t whole = size / (kAhead * 64) * (kAhead * 64), stride = warps * kAhead * 64;
-    uint32_t k0 = warp * kAhead * 64;
     Loads one, two;
     if (k0 < whole) load(one, k0);
     while (k0 < whole) {
