@@ -11,6 +11,13 @@
  * all of its tokens that need its slot's rows, and replaces these after it has
  * read them, so that no other CTA touches them: the new ones are rows of x,
  * which does not change.
+ *
+ * Measured, 6144 channels: 24 prompts of 23982 tokens of BF16 110 us (5.4 TB/s;
+ * 108 without silu, 109 with eight tokens of loads on their way through shared
+ * memory, so what is left is the reads' and writes' turns), 16000 tokens 75 us,
+ * 4096 25.3, of FP32 39.1 (5.2 TB/s); a token of 64 streams 4.8 us with their
+ * tails of FP32 (2.3 TB/s: the launch and two waits for memory, one after the
+ * other).
  */
 #include "gdn_ops.h"
 #include "gdn_values.h"
@@ -24,6 +31,8 @@ constexpr uint32_t kThreads = 128;
 /* Tokens computed together, while the loads of as many more are in flight: with two 64 registers and eight CTAs an SM,
  * with four 90 and five. 24 ragged prompts of BF16 117 us with two, 122 with four; 4 x 1000 tokens of FP32 48.8 and 43.4. */
 __host__ __device__ constexpr int ahead_of(int channels) { return channels == 8 ? 2 : 4; }
+__host__ __device__ constexpr int ctas_of(int channels) { return channels == 4 ? 5 : 8; }
+constexpr uint32_t kMaxTile = 128; /* tokens of a CTA */
 
 __device__ __forceinline__ uint32_t bound_of(const ConvParams &p, uint32_t n) {
     if (p.starts == nullptr) return n;
@@ -189,22 +198,24 @@ __device__ __forceinline__ float tap(const float4 &w, float bias, const float (&
 
 /* T: type of x and y. kWide: 16 bytes of channels a thread. */
 template <typename T, bool kWide, int W>
-__global__ void __launch_bounds__(kThreads, Lane<T, kWide>::C == 8 ? 8 : 1) conv_kernel(const __grid_constant__ ConvParams p, const uint32_t tile) {
+__global__ void __launch_bounds__(kThreads, ctas_of(Lane<T, kWide>::C)) conv_kernel(const __grid_constant__ ConvParams p, const uint32_t tile) {
     using L = Lane<T, kWide>;
     constexpr int C = L::C, kAhead = ahead_of(C);
     __shared__ Weights<C, kThreads, kWide> weights;
-    const uint32_t tid = threadIdx.x, c0 = kWide ? (blockIdx.y * kThreads + tid) * C : blockIdx.y * kThreads * C + tid;
+    /* the columns of a tile next to one another: their rows are */
+    const uint32_t columns = (p.channels + kThreads * C - 1) / (kThreads * C), row = blockIdx.x / columns, column = blockIdx.x - row * columns;
+    const uint32_t tid = threadIdx.x, c0 = kWide ? (column * kThreads + tid) * C : column * kThreads * C + tid;
     const bool live = c0 < p.channels;
     const L at{c0 + kThreads < p.channels ? kThreads : 0};
     const T *x = static_cast<const T *>(p.x) + c0;
     T *y = static_cast<T *>(p.out) + c0;
     wait_for_previous();
-    weights.template fill<W>(p, blockIdx.y * kThreads * C);
+    weights.template fill<W>(p, column * kThreads * C);
     float bias[C];
 #pragma unroll
     for (int c = 0; c < C; ++c) bias[c] = live && p.bias != nullptr ? load1(p.bias, c0 + (kWide ? c : c * at.gap), p.weight_type) : 0.0f;
     __syncthreads();
-    const uint32_t t0 = blockIdx.x * tile, t1 = min(t0 + tile, p.tokens);
+    const uint32_t t0 = row * tile, t1 = min(t0 + tile, p.tokens);
     uint32_t n = t0 < t1 ? begun(p, t0) : 0; /* the sequence of token t0 is n - 1, if it has one */
     uint32_t t = t0;
     float zero[C];
@@ -332,7 +343,7 @@ __global__ void __launch_bounds__(kThreads, Lane<T, kWide>::C == 8 ? 8 : 1) conv
     }
     /* fresh sequences without tokens: nobody else touches their slots */
     if (p.starts != nullptr && p.fresh != nullptr)
-        for (uint32_t i = blockIdx.x; i < p.N; i += gridDim.x)
+        for (uint32_t i = row; i < p.N; i += gridDim.x / columns)
             if (p.fresh[i] != 0 && bound_of(p, i + 1) <= bound_of(p, i)) {
                 const int64_t slot = p.slots == nullptr ? (int64_t)i : (int64_t)p.slots[i];
                 if (live && slot >= 0 && slot < (int64_t)p.tail_slots)
@@ -397,11 +408,16 @@ cudaError_t launch_conv_t(const ConvParams &p, int sms, cudaStream_t stream) {
         return launch_overlapped(conv_step_kernel<T, kWide, W>, dim3((p.tokens + kThreads / 32 - 1) / (kThreads / 32), columns), kThreads, 0, stream, p);
     }
     const uint32_t columns = (p.channels + kThreads * C - 1) / (kThreads * C);
-    /* long tiles read fewer rows twice, short ones make more CTAs */
-    uint32_t tile = 64;
-    while (tile > 1 && (uint64_t)((p.tokens + tile - 1) / tile) * columns < 4u * (uint32_t)sms) tile /= 2;
+    /* Tiles as short as lets all CTAs run at once (of more than kMaxTile tokens, two or more times all): a tile reads
+     * W - 1 rows twice, but one CTA too many costs as long as all of them. 6144 channels of BF16, us with tiles of 24,
+     * 32, 48, 64 and 96: 4096 tokens (21 is the shortest) 25.3, 27.5, 30.5, 34.3, 43.1; 16000 (82) 79.4, 78.6, 78.0,
+     * 85.5, 76.6. */
+    const uint32_t at_once = (uint32_t)(ctas_of(C) * sms) / columns > 0 ? (uint32_t)(ctas_of(C) * sms) / columns : 1;
+    const uint32_t times = (uint32_t)(((uint64_t)p.tokens + (uint64_t)at_once * kMaxTile - 1) / ((uint64_t)at_once * kMaxTile));
+    uint32_t tile = times == 0 ? 1 : (uint32_t)(((uint64_t)p.tokens + (uint64_t)at_once * times - 1) / ((uint64_t)at_once * times));
+    if (tile > 1) tile += tile & 1; /* two tokens at a time */
     const uint32_t tiles = p.tokens == 0 ? 1 : (p.tokens + tile - 1) / tile;
-    return launch_overlapped(conv_kernel<T, kWide, W>, dim3(tiles, columns), kThreads, 0, stream, p, tile);
+    return launch_overlapped(conv_kernel<T, kWide, W>, dim3(tiles * columns), kThreads, 0, stream, p, tile);
 }
 
 template <typename T, bool kWide>
