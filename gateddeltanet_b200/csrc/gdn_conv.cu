@@ -417,6 +417,7 @@ cudaError_t launch_conv_t(const ConvParams &p, int sms, cudaStream_t stream) {
     uint32_t tile = times == 0 ? 1 : (uint32_t)(((uint64_t)p.tokens + (uint64_t)at_once * times - 1) / ((uint64_t)at_once * times));
     if (tile > 1) tile += tile & 1; /* two tokens at a time */
     const uint32_t tiles = p.tokens == 0 ? 1 : (p.tokens + tile - 1) / tile;
+    if ((uint64_t)tiles * columns > 0x7fffffffu) return cudaErrorInvalidConfiguration;
     return launch_overlapped(conv_kernel<T, kWide, W>, dim3(tiles * columns), kThreads, 0, stream, p, tile);
 }
 

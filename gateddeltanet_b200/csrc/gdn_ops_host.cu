@@ -257,8 +257,8 @@ int gdn_b200_rms_norm(const GdnB200NormArgs *args) {
     if (a.residual != nullptr && !float_type(a.residual_dtype))
         return failf("%s: residual_dtype %d is neither FP32 (0) nor BF16 (1)", who, a.residual_dtype);
     if (!float_type(a.out_dtype) && a.out_dtype != 2) return failf("%s: out_dtype %d is not FP32 (0), BF16 (1) or E4M3 (2)", who, a.out_dtype);
-    if (a.tokens == 0 || a.heads == 0) return 0;
-    if (a.dim == 0) return failf("%s: rows of no values", who);
+    if (a.tokens == 0 || (a.heads == 0 && a.out_dtype != 2)) return 0;
+    if (a.dim == 0 || a.heads == 0) return failf("%s: rows of no values", who); /* without heads a token's scale says nothing */
     if ((uint64_t)a.tokens * a.heads > 0x7fffffffu) return failf("%s: %u tokens of %u heads are too many", who, a.tokens, a.heads);
     if (!(a.eps >= 0.0f)) return failf("%s: eps is negative or not a number", who);
     if (a.x == nullptr || a.out == nullptr) return failf("%s: x or out is missing", who);
@@ -315,7 +315,8 @@ int gdn_b200_linear(const GdnB200LinearArgs *args) {
     if (a.tokens > 1 && a.out_row < (int64_t)a.outputs) return failf("%s: rows of out overlap", who);
     if (a.residual != nullptr && a.tokens > 1 && a.residual_row < 0) return failf("%s: negative stride", who);
     if (a.x_row > 1ll << 36 || a.weight_row > 1ll << 36) return failf("%s: rows of x or weight are too far apart", who);
-    if (!aligned(a.out, out_size) || (a.residual != nullptr && !aligned(a.residual, res_size)) || (a.bias != nullptr && !aligned(a.bias, size_of(a.bias_dtype))))
+    if (!aligned(a.out, out_size) || (a.residual != nullptr && !aligned(a.residual, res_size)) || (a.bias != nullptr && !aligned(a.bias, size_of(a.bias_dtype))) ||
+        (a.dtype == 2 && (!aligned(a.x_scales, 4) || !aligned(a.weight_scales, 4))))
         return failf("%s: a tensor is misaligned for its type", who);
     const Extent out(a.out, a.out_row, 0, a.tokens, 1, a.outputs, out_size), x(a.x, a.x_row, 0, a.tokens, 1, a.inputs, size),
         weight(a.weight, a.weight_row, 0, rows, 1, a.inputs, size), residual(a.residual, a.residual_row, 0, a.tokens, 1, a.outputs, res_size),
@@ -367,7 +368,8 @@ int gdn_b200_short_conv(const GdnB200ConvArgs *args) {
         (a.tail_slots > 1 && a.tails_slot < (a.width > 2 ? ((int64_t)a.width - 2) * a.tails_row : 0) + (int64_t)a.channels))
         return failf("%s: rows or slots of tails overlap", who);
     const int64_t size = size_of(a.dtype), tail_size = size_of(a.tail_dtype), weight_size = size_of(a.weight_dtype);
-    if (!aligned(a.x, size) || !aligned(a.out, size) || !aligned(a.tails, tail_size) || !aligned(a.weight, weight_size) || !aligned(a.bias, weight_size))
+    if (!aligned(a.x, size) || !aligned(a.out, size) || !aligned(a.tails, tail_size) || !aligned(a.weight, weight_size) || !aligned(a.bias, weight_size) ||
+        !aligned(a.starts, 4) || !aligned(a.slots, 4))
         return failf("%s: a tensor is misaligned for its type", who);
     const Extent x(a.x, a.x_token, 0, a.tokens, 1, a.channels, size), out(a.out, a.out_token, 0, a.tokens, 1, a.channels, size),
         tails(a.tails, a.tails_slot, a.tails_row, a.tail_slots, a.width - 1, a.channels, tail_size),

@@ -175,3 +175,18 @@ def test_plain_forms_by_torch():
     y, after, _ = plain.conv(x, w, tails, activation=None, starts=torch.tensor([0, 7]), slots=torch.tensor([1]))
     line = torch.cat([tails[1], x]).T[None]
     assert torch.allclose(y, F.conv1d(line, w[:, None], groups=6)[0].T) and torch.equal(after[1], x[-3:]) and torch.equal(after[0], tails[0])
+
+
+@pytest.mark.parametrize("entry,args,reason", [
+    ("gdn_b200_linear", lambda: linear_args(dtype=2, x_scales=FAKE + 2, weight_scales=FAR), "misaligned"),
+    ("gdn_b200_linear", lambda: linear_args(dtype=2, x_scales=FAKE, weight_scales=FAR + 1), "misaligned"),
+    ("gdn_b200_short_conv", lambda: conv_args(starts=FAKE + 2), "misaligned"),
+    ("gdn_b200_short_conv", lambda: conv_args(slots=FAKE + 1), "misaligned"),
+    ("gdn_b200_rms_norm", lambda: norm_args(heads=0, out_dtype=2, scales=FAR), "no values")])
+def test_vectors_off_their_boundaries_and_scales_of_nothing(lib, entry, args, reason):  # noqa: F811
+    assert getattr(lib, entry)(args()) == -1
+    assert reason in gdn.last_error()
+
+
+def test_norm_of_no_heads(lib):  # noqa: F811
+    assert lib.gdn_b200_rms_norm(norm_args(heads=0)) == 0
