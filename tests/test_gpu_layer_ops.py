@@ -328,6 +328,25 @@ def test_conv_strides(ops, extra, starts):
     assert torch.equal(tails.cpu().double(), after) and around(pool, tails) and around(big, out)
 
 
+@pytest.mark.parametrize("channels,starts,x_type", [(8, [0, 150001, 150003, 330001], BF16), (4, [0, 100, 101, 100001], F32),
+                                                    (1001, [0, 20011, 20012, 40000], BF16), (6144, [0, 3000, 4096], BF16)], ids=str)
+def test_conv_long_sequences(ops, channels, starts, x_type):
+    """Tiles of every length the choice has, and more of them than run at once; sequence by sequence in 64 bits."""
+    T, N = starts[-1], len(starts) - 1
+    x, w = rand(T, channels, dtype=x_type), rand(channels, 4, seed=2)
+    tails, b = rand(N, 3, channels, seed=3), rand(channels, seed=4)
+    old = tails.double()
+    y = ops.short_conv(x, w, tails, bias=b, starts=torch.tensor(starts, dtype=torch.int32, device="cuda"))
+    for n in range(N):
+        line = torch.cat([old[n], x[starts[n]:starts[n + 1]].double()])
+        taps = [line[j:len(line) - 3 + j] * w[:, j].double() for j in range(4)]
+        s, size = sum(taps) + b.double(), sum(t.abs() for t in taps) + b.double().abs()
+        want = plain.silu(s)
+        off = 1.1 * 5 * plain.U * size + 24 * plain.U * want.abs()  # as in plain.conv
+        plain.check(y[starts[n]:starts[n + 1]], want.cpu(), off.cpu(), f"sequence {n}")
+        assert torch.equal(tails[n].double(), line[len(line) - 3:])
+
+
 def test_conv_by_pieces(ops):
     """A prompt in pieces, then token by token, as in one call: the same bits."""
     x, weight = rand(300, 512, dtype=BF16), rand(512, 4, seed=2)
