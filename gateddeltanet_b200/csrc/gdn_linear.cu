@@ -60,10 +60,12 @@ constexpr uint32_t kRowsA = 128;                  /* tokens of a CTA */
 constexpr uint32_t kBytesA = kRowsA * kBlock;
 constexpr uint32_t kMaxStages = 8;
 constexpr uint32_t kMaxN = 256;
-/* Blocks of k that TMEM adds up before the sums go on in registers. FP32 outputs: 12 (48 steps; off by up to
- * 6.8e-7 in the 2-norm for 2048 inputs, where 8 give 4.7e-7 and cost 2 to 15 % more time, 16 give 1.0e-6).
- * BF16 outputs, which are rounded to 1.7e-3: 32. Even, for stages of two blocks. */
-constexpr uint32_t kChunkF32 = 12, kChunkBF16 = 32;
+/* Blocks of k that TMEM adds up before the sums go on in registers. FP32 outputs of BF16: 12 (48 steps; off by up to
+ * 7.3e-7 in the 2-norm, 8.6e-7 after silu, where 8 give 4.8e-7 and cost 2 to 15 % more time, 16 1.0e-6); of swiglu,
+ * whose two sums are off the same way, 6 (7.0e-7, where 12 give 1.5e-6 and 8 9.5e-7; 10 to 20 % more time for 4096 tokens,
+ * none for 300). BF16 outputs, which are rounded to 1.7e-3, and 8-bit operands, whose products are short (3.0e-7 after 32
+ * blocks of 2048 and 5632 inputs): 32. Even, for stages of two blocks. */
+constexpr uint32_t kChunkF32 = 12, kChunkPairs = 6, kChunkShort = 32;
 
 /* set when a wait of a kernel ran out; read and cleared by the host */
 __device__ int g_linear_status;
@@ -870,7 +872,7 @@ LinearShape shape_of(const LinearParams &p, uint32_t ctas, uint32_t n, uint32_t 
     g.outs = p.activation == kSwiglu ? n / 2 : n;
     g.split = split;
     g.sub = sub;
-    g.chunk = p.out_type == kF32 ? kChunkF32 : kChunkBF16;
+    g.chunk = p.out_type == kBF16 || p.type == kE4M3 ? kChunkShort : p.activation == kSwiglu ? kChunkPairs : kChunkF32;
     const uint32_t stage = sub * (kBytesA + n / ctas * kBlock);
     const uint32_t room = (uint32_t)(kSmemLimit - kSmemRest) / stage;
     g.stages = room < kMaxStages ? room : kMaxStages;

@@ -1,5 +1,5 @@
 /* gdn_linear_few.cu -- y = act(sx sw x W^T + bias) + residual for up to 16
- * tokens (gdn_linear.cu takes more).
+ * tokens (gdn_linear.cu takes more, and 9 and more with many weights).
  *
  * Bound by reading W once. A warp multiplies 16 rows of W with 8 (or 16)
  * tokens by m16n8k16 MMAs whose operands come straight from memory: in a
@@ -14,7 +14,7 @@
  * Measured: one token of 2048 inputs by 8208 outputs of BF16 7.1 us (4.7 TB/s),
  * by 32000 19.9 us (6.6 TB/s, the rate of a copy), of 8 bits 6.3 and 14.9 us;
  * what small calls take above the bytes is the launch and one wait for memory,
- * about 2.5 us. 16 tokens read as much of x as of W: 11.4 and 28.6 us.
+ * about 2.5 us. 16 tokens read as much of x as of W: 12.1 and 29.4 us.
  */
 #include "gdn_linear.h"
 
@@ -145,11 +145,21 @@ __global__ void __launch_bounds__(kMaxWarps * 32) linear_few_kernel(const __grid
             for (int n = 0; n < kGroups; ++n) l.b[s][n] = __ldcg(reinterpret_cast<const uint4 *>(x[n] + k0 + s * 64));
         }
     };
+    /* The tensor cores cut their sums towards zero: the ones of a set are added to the others with rounding to nearest. In
+     * one sum of 1408 inputs a warp, results of 5632 inputs were 1.4e-6 off in the 2-norm, 2.9e-6 of swiglu; so 1.4e-7
+     * and 2.0e-7, at no cost but for 16 tokens of swiglu (2048 by 2 x 5632 15.2 us instead of 14.4, for want of registers). */
     auto multiply = [&](const Loads &l) {
+        float part[kHalves][kGroups][4] = {};
 #pragma unroll
         for (int s = 0; s < kAhead; ++s)
 #pragma unroll
-            for (int h = 0; h < kHalves; ++h) products<kFp8, kGroups>(d[h], l.a[s][h][0], l.a[s][h][1], l.b[s]);
+            for (int h = 0; h < kHalves; ++h) products<kFp8, kGroups>(part[h], l.a[s][h][0], l.a[s][h][1], l.b[s]);
+#pragma unroll
+        for (int h = 0; h < kHalves; ++h)
+#pragma unroll
+            for (int n = 0; n < kGroups; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) d[h][n][i] += part[h][n][i];
     };
     /* the whole steps, in turn over the warps, each time with the next one's loads under way */
     Loads one, two;
@@ -221,6 +231,14 @@ cudaError_t launch_few_x(const LinearParams &p, int sms, cudaStream_t stream) {
 }
 
 }  // namespace
+
+/* More than eight tokens double what this kernel reads of x, and it slows down where there are many weights; the other's
+ * tiles take 5 us at least. 16 tokens of 2048 by 2048 4.2 us here and 7.3 there, of 5632 by 2048 7.4 and 10.3 (8 bits 5.9 and
+ * 8.1), of 2048 by 8208 12.1 and 10.8 (8 bits 8.9 and 7.7), by 2 x 5632 15.2 and 13.0 (11.8 and 9.0), by 32000 29.4 and 27.7
+ * (20.1 and 18.2); 8 tokens by 32000 23.0. */
+bool takes_few(const LinearParams &p) {
+    return p.tokens <= 8 || (p.tokens <= kFewTokens && (uint64_t)p.inputs * p.outputs * (p.activation == kSwiglu ? 2 : 1) <= 14000000u);
+}
 
 cudaError_t launch_linear_few(const LinearParams &p, int sms, cudaStream_t stream) {
     return p.type == kE4M3 ? launch_few_x<true>(p, sms, stream) : launch_few_x<false>(p, sms, stream);

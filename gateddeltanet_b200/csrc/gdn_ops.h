@@ -135,7 +135,7 @@ struct LinearParams {
     int type, bias_type, residual_type, out_type, activation;
     uint32_t drop; /* for tests, 0: none. 1 + the k-block whose copy the first CTA does not make */
 };
-constexpr uint32_t kFewTokens = 16; /* up to here gdn_linear_few.cu, above gdn_linear.cu */
+constexpr uint32_t kFewTokens = 16; /* that gdn_linear_few.cu can take */
 
 /* kernel<<<grid, block, smem, stream>>>(args...) and this launch's own result:
  * cudaGetLastError would also give that of a call before it. */
@@ -178,6 +178,7 @@ cudaError_t launch_logits(LogitsParams p, bool bf16, int sms, cudaStream_t strea
 cudaError_t launch_norm(const NormParams &p, int sms, cudaStream_t stream);
 cudaError_t launch_conv(const ConvParams &p, int sms, cudaStream_t stream);
 cudaError_t launch_linear(const LinearParams &p, int sms, cudaStream_t stream);
+bool takes_few(const LinearParams &p); /* whether launch_linear_few is the faster one */
 cudaError_t launch_linear_few(const LinearParams &p, int sms, cudaStream_t stream);
 cudaError_t linear_status(int *status);
 

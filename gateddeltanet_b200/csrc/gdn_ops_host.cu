@@ -329,7 +329,7 @@ int gdn_b200_linear(const GdnB200LinearArgs *args) {
                                    a.residual_row, a.out_row, a.tokens, a.inputs, a.outputs, a.dtype, a.bias_dtype,
                                    a.residual_dtype, a.out_dtype, a.activation, g_drop.exchange(0)};
     return on_device(who, a.device, [&](int sms) {
-        auto *launch = a.tokens <= gdn::ops::kFewTokens ? gdn::ops::launch_linear_few : gdn::ops::launch_linear;
+        auto *launch = gdn::ops::takes_few(p) ? gdn::ops::launch_linear_few : gdn::ops::launch_linear;
         return launch(p, sms, static_cast<cudaStream_t>(a.stream));
     });
 }

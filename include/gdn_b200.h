@@ -346,7 +346,7 @@ int gdn_b200_delta_status(int device);
 /* Test hook: in the next gdn_b200_delta_step, gdn_b200_delta_chunk or gdn_b200_linear
  * of the process the copy of one row block (if that call streams blocks through shared
  * memory), of one CTA's first chunk or of x's block `index` of the first CTA's (if
- * that call has more than 16 tokens) is not made, so that a wait runs out. */
+ * that call has more than 16 tokens, or 9 and very many weights) is not made, so that a wait runs out. */
 int gdn_b200_test_drop_copy(uint32_t index);
 
 /* Constraints on the logits of `rows` streams, and the greedy pick. With n
@@ -422,7 +422,8 @@ int gdn_b200_rms_norm(const GdnB200NormArgs *args);
  * half's value times the second half's. rows = outputs for the others. bias
  * [rows] (contiguous) and residual [tokens][outputs] may be NULL; bias, residual
  * and out are FP32 (0) or BF16 (1), each its own. Sums are FP32 on the tensor
- * cores; what is not finite spreads to its token's outputs (from x) or to its
+ * cores, in parts so short that FP32 results keep 20 bits (2-norm, independent
+ * operands); what is not finite spreads to its token's outputs (from x) or to its
  * row's (from W) only. Strides count elements; rows of x and W are contiguous and start on
  * 16-byte boundaries; inputs may be any number. out may be the residual itself
  * (same type and stride) or memory apart from the inputs. */

@@ -193,6 +193,41 @@ def test_linear(ops, tokens, eight, inputs, outputs, activation, extras):
         plain.check(got, want, off, str(dtype))
 
 
+@pytest.mark.parametrize("tokens", [8, 9, 13, 16, 17])
+@pytest.mark.parametrize("eight", [False, True], ids=["bf16", "fp8"])
+@pytest.mark.parametrize("inputs,outputs,activation", [(2048, 8208, None), (2000, 3700, "swiglu"), (5632, 2486, "gelu"), (5632, 2485, None)])
+def test_linear_few_tokens_and_many_weights(ops, tokens, eight, inputs, outputs, activation):
+    """Around the number of weights and of tokens where the other kernel takes over."""
+    rows = outputs * (2 if activation == "swiglu" else 1)
+    x, w = rand(tokens, inputs), rand(rows, inputs, seed=2) * inputs ** -0.5
+    s = {}
+    if eight:
+        (x, s["x_scales"]), (w, s["weight_scales"]) = eight_bits(x), eight_bits(w)
+    else:
+        x, w = x.to(BF16), w.to(BF16)
+    residual = rand(tokens, outputs, seed=3)
+    want, off = plain.linear(x, w, activation=activation, residual=residual, **s)
+    plain.check(ops.linear(x, w, activation=activation, residual=residual, dtype=F32, **s), want, off)
+
+
+@pytest.mark.parametrize("tokens", [3, 16, 40, 300])
+@pytest.mark.parametrize("eight", [False, True], ids=["bf16", "fp8"])
+@pytest.mark.parametrize("activation", [None, "silu", "gelu", "swiglu"])
+@pytest.mark.parametrize("inputs", [768, 5632])
+def test_linear_keeps_twenty_bits(ops, tokens, eight, activation, inputs):
+    """FP32 results to 2^-20 in the 2-norm: sums that the tensor cores cut are kept short. Sums of 64 bits of what they see."""
+    rows = 1000 * (2 if activation == "swiglu" else 1)
+    x, w = rand(tokens, inputs), rand(rows, inputs, seed=2) * inputs ** -0.5
+    s = {}
+    if eight:
+        (x, s["x_scales"]), (w, s["weight_scales"]) = eight_bits(x), eight_bits(w)
+    else:
+        x, w = x.to(BF16), w.to(BF16)
+    want, _ = plain.linear(x, w, activation=activation, **s)
+    got = ops.linear(x, w, activation=activation, dtype=F32, **s).cpu().double()
+    assert float((got - want).norm() / want.norm()) <= 2.0 ** -20
+
+
 @pytest.mark.parametrize("tokens", [3, 40, 300])
 @pytest.mark.parametrize("eight", [False, True], ids=["bf16", "fp8"])
 @pytest.mark.parametrize("inputs", [1, 5, 63, 65, 130, 1001])
