@@ -26,15 +26,15 @@
  * Every wait is bounded (2 s). A CTA whose wait ran out writes NaN to its
  * outputs and sets g_linear_status.
  *
- * Measured. 4096 tokens of 2048 by 2 x 5632 of 8 bits with swiglu 67.5 us (2.8
- * PFLOP/s), of 5632 by 2048 of BF16 67.7 us (1.4 PFLOP/s), with an FP32 residual
- * and FP32 outputs 82: bound by the tensor cores (66 to 78 % of cycles) and, of
- * runs of a second, by the power limit (82 to 98 us at 1.46 GHz); 128 tiles of
+ * Measured. 4096 tokens of 2048 by 2 x 5632 of 8 bits with swiglu 65 us (2.9
+ * PFLOP/s), of 5632 by 2048 of BF16 68 us (1.4 PFLOP/s), with an FP32 residual
+ * and FP32 outputs 78: bound by the tensor cores (66 to 78 % of cycles) and, of
+ * runs of a second, by the power limit (79 to 92 us at 1.46 GHz); 128 tiles of
  * 256 by 256 for 74 pairs of CTAs leave 14 % of them idle. 64 tokens by 32000 of
- * BF16 29 us (4.7 TB/s), by 2 x 5632 with swiglu 14.1 us (3.3 TB/s): bound by
- * reading W, after which the last sums' way takes 4.5 us: through TMEM and the
- * cluster 3, the end of all CTAs 1. It begins 2.4 us after the kernel before has
- * ended, when the first blocks come.
+ * BF16 25 us (5.2 TB/s), FP32 out 28, by 2 x 5632 with swiglu 13.4 us (3.4 TB/s):
+ * bound by reading W, after which the last sums' way takes about 4 us: through
+ * TMEM and the cluster, to memory, and the end of all CTAs. It begins 2.4 us after
+ * the kernel before has ended, when the first blocks come.
  */
 #include "gdn_linear.h"
 
@@ -61,10 +61,10 @@ constexpr uint32_t kBytesA = kRowsA * kBlock;
 constexpr uint32_t kMaxStages = 8;
 constexpr uint32_t kMaxN = 256;
 /* Blocks of k that TMEM adds up before the sums go on in registers. FP32 outputs of BF16: 12 (48 steps; off by up to
- * 7.3e-7 in the 2-norm, 8.6e-7 after silu, where 8 give 4.8e-7 and cost 2 to 15 % more time, 16 1.0e-6); of swiglu,
- * whose two sums are off the same way, 6 (7.0e-7, where 12 give 1.5e-6 and 8 9.5e-7; 10 to 20 % more time for 4096 tokens,
- * none for 300). BF16 outputs, which are rounded to 1.7e-3, and 8-bit operands, whose products are short (3.0e-7 after 32
- * blocks of 2048 and 5632 inputs): 32. Even, for stages of two blocks. */
+ * 7.3e-7 in the 2-norm, 8.6e-7 after silu, where 8 give 4.8e-7 and cost 4 to 7 % of 4096 tokens' time, 16 1.0e-6); of
+ * swiglu, whose two sums are off the same way, 6 (7.0e-7, where 12 give 1.5e-6; up to 4 % more time). BF16 outputs, which
+ * are rounded to 1.7e-3, and 8-bit operands, whose products are short (3.0e-7 after 32 blocks of 2048 and 5632 inputs): 32.
+ * Even, for stages of two blocks. */
 constexpr uint32_t kChunkF32 = 12, kChunkPairs = 6, kChunkShort = 32;
 
 /* set when a wait of a kernel ran out; read and cleared by the host */
@@ -925,6 +925,16 @@ cudaError_t launch_shape(const LinearParams &p, const LinearShape &g, int sms, c
     return cudaLaunchKernelEx(&cfg, linear_kernel<kCtas, kFp8, pairs, kWay>, p, map_x, map_w, g);
 }
 
+/* whether all results, and their residuals, are pieces of four values on their boundaries */
+bool whole_pieces(const LinearParams &p) {
+    auto aligned = [&](const void *at, int64_t row, int type) {
+        const uintptr_t size = type == kF32 ? 4 : 2;
+        return ((reinterpret_cast<uintptr_t>(at) | (p.tokens == 1 ? 0 : (uintptr_t)row * size)) & (4 * size - 1)) == 0;
+    };
+    return p.outputs % 4 == 0 && aligned(p.out, p.out_row, p.out_type) &&
+           (p.residual == nullptr || aligned(p.residual, p.residual_row, p.residual_type));
+}
+
 }  // namespace
 
 cudaError_t launch_linear_as(const LinearParams &p, uint32_t ctas, uint32_t n, uint32_t split, uint32_t sub, int sms, cudaStream_t stream) {
@@ -939,38 +949,34 @@ cudaError_t launch_linear_as(const LinearParams &p, uint32_t ctas, uint32_t n, u
         if (wide) return pick(pairs, std::integral_constant<int, kPieces>());
         return p.residual == nullptr ? pick(pairs, std::integral_constant<int, kValues>()) : pick(pairs, std::integral_constant<int, kValuesAdded>());
     };
-    auto aligned = [&](const void *at, int64_t row, int type) {
-        const uintptr_t size = type == kF32 ? 4 : 2;
-        return ((reinterpret_cast<uintptr_t>(at) | (p.tokens == 1 ? 0 : (uintptr_t)row * size)) & (4 * size - 1)) == 0;
-    };
-    const bool wide = p.outputs % 4 == 0 && aligned(p.out, p.out_row, p.out_type) &&
-                      (p.residual == nullptr || aligned(p.residual, p.residual_row, p.residual_type));
+    const bool wide = whole_pieces(p);
     auto *launch = p.activation == kSwiglu ? pick_way(std::true_type(), wide) : pick_way(std::false_type(), wide);
     return launch(p, g, sms, stream);
 }
 
 /* The tiles of a call are those for which this estimate is least. What it knows, in us on 148 SMs: a block of k takes
- * 0.0014 n + 0.07 in one CTA and 0.00125 n + 0.04 in two, of which each computes half the columns of both; a launch
- * 4.5 or 5.4; each tile of a CTA 1.5; a cluster that divides k 0.7 + 0.2 a CTA. Of clusters of four and eight not as
- * many as there are SMs for run at once (13 of eight did, 16 did not). Against sweeps of all tiles of 196 calls (17 to
- * 4096 tokens, 128 to 5632 inputs, 501 to 32000 outputs, both types, all activations) its choices were 0.8 % slower
- * than the best tiles in the mean; 256 columns always, or 128 split as far as possible, were up to twice as slow at
- * either end. */
+ * 0.00144 n + 0.05 in one CTA and 0.00128 n + 0.024 in two, of which each computes half the columns of both; a launch
+ * 4.5 or 5.2; each tile of a CTA 1.0; the last tile's results, where they go value by value, 0.01 n; a cluster that
+ * divides k 0.9 + 0.04 a CTA. Of clusters of four and eight not as many as there are SMs for run at once (13 of eight
+ * did, 16 did not). Against sweeps of all tiles of 196 calls (17 to 4096 tokens, 128 to 5632 inputs, 501 to 32000
+ * outputs, both types, all activations) its choices were 1.1 % slower than the best tiles in the mean; 256 columns
+ * always, or 128 split as far as possible, were up to twice as slow at either end. */
 cudaError_t launch_linear(const LinearParams &p, int sms, cudaStream_t stream) {
     const uint32_t blocks = (uint32_t)(((uint64_t)p.inputs * (p.type == kE4M3 ? 1 : 2) + kBlock - 1) / kBlock);
     float least = 3.4e38f;
     uint32_t ctas = 1, n = 256, split = 1;
+    const bool whole = whole_pieces(p);
     for (uint32_t c = 1; c <= (p.tokens > kRowsA ? 2u : 1u); ++c)
         for (uint32_t width = 32; width <= kMaxN; width += 32) {
             const uint32_t outs = p.activation == kSwiglu ? width / 2 : width;
             const uint64_t tiles = (uint64_t)((p.tokens + c * kRowsA - 1) / (c * kRowsA)) * ((p.outputs + outs - 1) / outs);
-            const float block = c == 2 ? 0.00125f * width + 0.04f : 0.0014f * width + 0.07f;
+            const float block = c == 2 ? 0.00128f * width + 0.024f : 0.00144f * width + 0.053f;
             for (uint32_t s = 1; s <= (c == 1 ? 8u : 1u); s *= 2) {
                 const uint64_t most = (uint64_t)sms * (s < 4 ? 8 : s == 4 ? 7 : 6) / 8;
                 if (s > 1 && (tiles * s > most || blocks / s < 4)) break;
                 const uint64_t waves = (tiles * c * s + sms - 1) / sms;
-                const float t = (float)waves * ((float)((blocks + s - 1) / s) * block + 1.5f) + 0.001f * width + (c == 2 ? 5.4f : 4.5f) +
-                                (s > 1 ? 0.7f + 0.2f * s : 0.0f);
+                const float t = (float)waves * ((float)((blocks + s - 1) / s) * block + 1.0f) + (c == 2 ? 5.2f : 4.5f) +
+                                (whole ? 0.0f : 0.01f * width) + (s > 1 ? 0.9f + 0.04f * s : 0.0f);
                 if (t < least) least = t, ctas = c, n = width, split = s;
             }
         }
