@@ -380,7 +380,7 @@ __device__ __forceinline__ void store_column(T *at, int64_t row, uint32_t left, 
 
 /* The outputs of a tile from the sums of the kSplit CTAs of its cluster, in the order of their ranks: four of a token at
  * a time, in turn over the cluster's threads. The loads of several fours go out together, those of the residual too: 300
- * tokens of 5632 by 2048 with a residual took 19.8 us with one four at a time and take 18.2. */
+ * tokens of 5632 by 2048 with a residual took 19.8 us with one four at a time and 18.2 so. */
 template <bool kFp8, bool pairs, bool kWide, int kSplit>
 __device__ __forceinline__ void join_parts(const LinearParams &p, const LinearShape &g, const SharedTail &s, uint32_t start, uint32_t rank,
                                            uint32_t worker, uint32_t tid) {

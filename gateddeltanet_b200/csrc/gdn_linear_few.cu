@@ -233,9 +233,9 @@ cudaError_t launch_few_x(const LinearParams &p, int sms, cudaStream_t stream) {
 }  // namespace
 
 /* More than eight tokens double what this kernel reads of x, and it slows down where there are many weights; the other's
- * tiles take 5 us at least. 16 tokens of 2048 by 2048 4.2 us here and 7.3 there, of 5632 by 2048 7.4 and 10.3 (8 bits 5.9 and
- * 8.1), of 2048 by 8208 12.1 and 10.8 (8 bits 8.9 and 7.7), by 2 x 5632 15.2 and 13.0 (11.8 and 9.0), by 32000 29.4 and 27.7
- * (20.1 and 18.2); 8 tokens by 32000 23.0. */
+ * tiles take 5 us at least. 16 tokens of 2048 by 2048 4.2 us here and 6.7 there, of 5632 by 2048 7.4 and 9.6 (8 bits 5.9 and
+ * 7.5), of 2048 by 8208 12.1 and 10.1 (8 bits 8.9 and 7.1), by 2 x 5632 15.2 and 12.9 (11.8 and 8.7), by 32000 29.4 and 26.8
+ * (20.1 and 17.8); 8 tokens by 32000 23.0. */
 bool takes_few(const LinearParams &p) {
     return p.tokens <= 8 || (p.tokens <= kFewTokens && (uint64_t)p.inputs * p.outputs * (p.activation == kSwiglu ? 2 : 1) <= 14000000u);
 }
