@@ -228,29 +228,25 @@ __global__ void __launch_bounds__(kThreads, ctas_of(Lane<T, kWide>::C)) conv_ker
             n = max(n + 1, begun(p, t));
             continue;
         }
-        uint32_t stop = min(end, t1);
         const int64_t slot = n == 0 || n > p.N ? -1 : p.slots == nullptr ? (int64_t)(n - 1) : (int64_t)p.slots[n - 1];
         if (slot < 0 || slot >= (int64_t)p.tail_slots) {
             /* tokens of no sequence, or of one without a slot */
+            const uint32_t stop = min(end, t1);
             if (live)
                 for (; t < stop; ++t) at.put(y + t * p.out_token, zero);
             t = stop;
             ++n;
             continue;
         }
-        const uint32_t begin = min(bound_of(p, n - 1), t);
-        if (begin < t0) {
-            t = max(t, min(end, begin + (W - 1))); /* the tokens before belong to an earlier tile */
-            stop = max(stop, t);
-        } else {
-            stop = min(end, max(t1, begin + (W - 1)));
-        }
+        const ConvPart part = conv_part(bound_of(p, n - 1), end, t, t0, t1, W - 1);
+        const uint32_t stop = part.stop;
+        t = part.t;
         if (live) {
-            if (t == begin) {
+            if (part.begins) {
                 /* the tokens that meet the slot's rows, one by one */
                 const bool fresh = p.fresh != nullptr && p.fresh[n - 1] != 0;
                 const int64_t rows = slot * p.tails_slot + c0;
-                const uint32_t few = min((uint32_t)(W - 1), end - begin);
+                const uint32_t few = min((uint32_t)(W - 1), end - t);
                 float win[W - 1][C];
 #pragma unroll
                 for (int j = 0; j < W - 1; ++j) {
@@ -275,10 +271,10 @@ __global__ void __launch_bounds__(kThreads, ctas_of(Lane<T, kWide>::C)) conv_ker
                     at.put(y + (int64_t)(t + i) * p.out_token, out);
                 }
                 /* the window is now the slot's new content, unless there are more tokens */
-                const bool more = end - begin > W - 1;
+                const bool more = end - t > W - 1;
 #pragma unroll
                 for (int j = 0; j < W - 1; ++j) {
-                    if (more) L::unpack(at.fetch(x + (int64_t)(end - (W - 1) + j) * p.x_token), win[j]);
+                    if (more) L::unpack(at.fetch(x + ((int64_t)end - (W - 1) + j) * p.x_token), win[j]);
                     at.put_tail(p, rows + j * p.tails_row, win[j]);
                 }
                 t += few;
@@ -287,7 +283,7 @@ __global__ void __launch_bounds__(kThreads, ctas_of(Lane<T, kWide>::C)) conv_ker
             uint4 in[W - 1 + kAhead], next[kAhead];
             if (t < stop) {
 #pragma unroll
-                for (int j = 0; j < W - 1; ++j) in[j] = at.fetch(x + (int64_t)(t - (W - 1) + j) * p.x_token);
+                for (int j = 0; j < W - 1; ++j) in[j] = at.fetch(x + ((int64_t)t - (W - 1) + j) * p.x_token);
 #pragma unroll
                 for (int a = 0; a < kAhead; ++a) next[a] = at.fetch(x + (int64_t)min(t + a, stop - 1) * p.x_token);
             }

@@ -123,6 +123,25 @@ struct ConvParams {
     int type, weight_type, tail_type, silu;
 };
 
+/* What the walk over a tile [t0, t1), come to token t in it, does with the sequence that has the entries `bound` and
+ * `end` of starts (end > t, both clamped): its tokens [t, stop) here, none if they are equal. The tile in which a sequence
+ * begins takes its first `back` tokens (which meet the slot's rows) also where they lie behind the tile's end, and the tiles
+ * after it leave them out. Where starts do not decrease a bound in the tile is t itself; where they do, it may be before
+ * or behind t, and the sequence is taken to begin at t. So t of a sequence that does not begin here is never below
+ * `back`: the rows before it that its first outputs read are in the tensor whatever starts holds. */
+struct ConvPart {
+    uint32_t t, stop;
+    bool begins;
+};
+__host__ __device__ __forceinline__ ConvPart conv_part(uint32_t bound, uint32_t end, uint32_t t, uint32_t t0, uint32_t t1, uint32_t back) {
+    if (bound >= t0) {
+        const uint32_t least = t1 > t + back ? t1 : t + back;
+        return {t, end < least ? end : least, true};
+    }
+    const uint32_t first = bound + back < end ? bound + back : end, from = t > first ? t : first, stop = end < t1 ? end : t1;
+    return {from, stop > from ? stop : from, false};
+}
+
 enum Activation : int { kNoActivation = 0, kSilu = 1, kGelu = 2, kSwiglu = 3 };
 
 /* y = act(sx sw x W^T + bias) + residual; W has 2 x outputs rows for kSwiglu. */
