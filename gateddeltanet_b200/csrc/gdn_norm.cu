@@ -247,7 +247,8 @@ __global__ void __launch_bounds__(kAhead ? kSmall : kMaxNormThreads, kAhead ? ct
 #pragma unroll
             for (int j = 0; j < 8; ++j) sum = fmaf(h[i][j], h[i][j], sum);
         sum = meet<false, kAhead>(sum, g.group, false, partial[0]);
-        const float f = rsqrtf(fmaf(sum, per_dim, p.eps));
+        /* squares that overflowed: NaN, where rsqrtf of infinity would make a row of zeros */
+        const float f = sum <= 3.40282347e38f ? rsqrtf(fmaf(sum, per_dim, p.eps)) : __int_as_float(0x7fc00000);
 #pragma unroll
         for (int i = 0; i < kN; ++i)
 #pragma unroll

@@ -393,9 +393,10 @@ int gdn_b200_constrain_logits(const GdnB200LogitsArgs *args);
  * gate have `dtype`, weight [dim] (contiguous) weight_dtype, the residual
  * residual_dtype; out_dtype may also be E4M3 (2), with scales FP32 [tokens].
  * weight, gate and residual may be NULL. All arithmetic is FP32 (results to
- * 2^-20): squares overflow from 1.8e19 on, and a row with such a value or one that
- * is not finite has no useful output (in 8 bits: NaN, scale too); other tokens are
- * not touched by it. Strides count elements, dim is contiguous; any alignment,
+ * 2^-20). A row with a value that is not finite, or whose sum of squares is over
+ * FP32's range (one value of 1.9e19 is enough), is NaN throughout; in 8 bits its token
+ * is, with its scale. Other rows are not touched by it. Squares under 1.5e-45 are lost, which
+ * only an eps of 0 or about as small lets one see. Strides count elements, dim is contiguous; any alignment,
  * rows on 16-byte boundaries with dim a multiple of 8 are faster. out may be x
  * itself (same type and strides) or memory apart from the other tensors. A token's
  * values have to fit one CTA's registers: dim <= 16384, and in 8 bits
