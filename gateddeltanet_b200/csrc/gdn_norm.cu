@@ -247,8 +247,10 @@ __global__ void __launch_bounds__(kAhead ? kSmall : kMaxNormThreads, kAhead ? ct
 #pragma unroll
             for (int j = 0; j < 8; ++j) sum = fmaf(h[i][j], h[i][j], sum);
         sum = meet<false, kAhead>(sum, g.group, false, partial[0]);
-        /* squares that overflowed: NaN, where rsqrtf of infinity would make a row of zeros */
-        const float f = sum <= 3.40282347e38f ? rsqrtf(fmaf(sum, per_dim, p.eps)) : __int_as_float(0x7fc00000);
+        /* 1 / sqrt: the instruction's value r after a step of Newton's method, r + r (1 - v r^2) / 2, so that it is off
+         * by its rounding. Where squares have overflowed the step makes NaN of r = 0, which would be a row of zeros. */
+        const float v = fmaf(sum, per_dim, p.eps), root = rsqrtf(v);
+        const float f = fmaf(0.5f * root, fmaf(-v * root, root, 1.0f), root);
 #pragma unroll
         for (int i = 0; i < kN; ++i)
 #pragma unroll

@@ -67,3 +67,12 @@ def test_norm_of_heads_whose_squares_overflow(ops):
     assert bool(y[1, 2].all()) and int(y.sum()) == 64
     y, scales = ops.rms_norm(x, dtype=E4M3)
     assert scales.isnan().tolist() == [False, True, False] and bool(y.float()[1].isnan().all())
+
+
+def test_norm_by_a_root_off_by_its_rounding(ops):
+    """Of 1 + eps, exact in FP32, with all that follows exact: the product in Newton's step is off by U, which counts half, and
+    the sum after it by U; errors of the instruction's own value come in squared."""
+    one, eps = torch.ones(1, 1, device="cuda"), torch.arange(1, 2 ** 20, 2 ** 10 - 3).double() / 2 ** 20 * 3
+    got = torch.cat([ops.rms_norm(one, eps=e) for e in eps.tolist()])[:, 0].cpu().double()
+    want = (1 + eps) ** -0.5
+    assert float(((got - want).abs() / want).max()) <= 1.51 * plain.U
