@@ -387,8 +387,9 @@ int gdn_b200_constrain_logits(const GdnB200LogitsArgs *args);
  * additions around it:
  *   h = residual + x            (if residual; written back, rounded to its type)
  *   y = h / sqrt(mean(h^2) + eps) * weight * (gate / (1 + e^-gate))
- *   out = y, rounded once, or, in 8 bits, e4m3(y / scales[token]) with
- *   scales[token] = max(max |y| / 448, 2^-126) over the token's heads
+ *   out = y, rounded once, or, in 8 bits, e4m3(y (1 / scales[token])) with
+ *   scales[token] = max(max |y| / 448, 2^-126) over the token's heads; the
+ *   reciprocal and the product are rounded to FP32 before the one rounding to E4M3
  * The mean over dim is that of the unrounded h. Types: FP32 (0) or BF16 (1); x and
  * gate have `dtype`, weight [dim] (contiguous) weight_dtype, the residual
  * residual_dtype; out_dtype may also be E4M3 (2), with scales FP32 [tokens].
