@@ -129,16 +129,30 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
-/* silu of both, as silu() */
+/* silu of both, with the same bits as silu_of() */
+template <typename T>
 __device__ __forceinline__ uint64_t silu2(uint64_t x) {
+    uint64_t near = x;
     float a, b;
-    split(mul2(x, pair_of(-1.44269504f, -1.44269504f)), a, b);
+    if constexpr (sizeof(T) == 4) {
+        split(x, a, b);
+        near = pair_of(fminf(fmaxf(a, -88.0f), 88.0f), fminf(fmaxf(b, -88.0f), 88.0f));
+    }
+    const uint64_t t = mul2(near, pair_of(-1.44269504f, -1.44269504f));
+    split(t, a, b);
     asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(a));
     asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(b));
-    split(add2(pair_of(a, b), pair_of(1.0f, 1.0f)), a, b);
+    uint64_t e = pair_of(a, b);
+    if constexpr (sizeof(T) == 4) e = fma2(e, fma2(t, pair_of(-0.693147181f, -0.693147181f), mul2(near, pair_of(-1.0f, -1.0f))), e);
+    split(add2(e, pair_of(1.0f, 1.0f)), a, b);
     asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(a));
     asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(b));
     return mul2(x, pair_of(a, b));
+}
+/* for results of type T */
+template <typename T>
+__device__ __forceinline__ float silu_of(float x) {
+    return sizeof(T) == 4 ? silu(x) : silu_short(x);
 }
 
 /* The weights of a CTA's channels in shared memory, by pairs of channels: four taps each, the last one
@@ -264,7 +278,7 @@ __global__ void __launch_bounds__(kThreads, ctas_of(Lane<T, kWide>::C)) conv_ker
                         for (int j = 0; j < W - 1; ++j) v[j] = win[j][c];
                         v[W - 1] = in[c];
                         const float s = tap<W>(weights.of(c, tid), bias[c], v);
-                        out[c] = p.silu ? silu(s) : s;
+                        out[c] = p.silu ? silu_of<T>(s) : s;
 #pragma unroll
                         for (int j = 0; j < W - 1; ++j) win[j][c] = v[j + 1];
                     }
@@ -312,7 +326,7 @@ __global__ void __launch_bounds__(kThreads, ctas_of(Lane<T, kWide>::C)) conv_ker
                         uint64_t o = b;
 #pragma unroll
                         for (int j = 0; j < W; ++j) o = fma2(w[j], v[a + j], o);
-                        if (p.silu) o = silu2(o);
+                        if (p.silu) o = silu2<T>(o);
                         float lo, hi;
                         split(o, lo, hi);
                         if (C == 8)
@@ -387,7 +401,7 @@ __global__ void __launch_bounds__(kThreads) conv_step_kernel(const __grid_consta
 #pragma unroll
         for (int j = 0; j < W; ++j) v[j] = win[j][c];
         const float s = tap<W>(weights.of(c, lane), bias[c], v);
-        out[c] = !known ? 0.0f : p.silu ? silu(s) : s;
+        out[c] = !known ? 0.0f : p.silu ? silu_of<T>(s) : s;
     }
     at.put(static_cast<T *>(p.out) + t * p.out_token + c0, out);
     if (known) {

@@ -291,12 +291,18 @@ __device__ __forceinline__ void finish(const LinearParams &p, float row_scale, f
             for (int i = 0; i < kN; ++i) up[i] += f[i];
         }
     }
-    if (pairs) {
+    if (pairs || p.activation == kSilu) {
+        if (p.out_type == kF32) {
 #pragma unroll
-        for (int i = 0; i < kN; ++i) v[i] = silu(v[i]) * up[i];
-    } else if (p.activation == kSilu) {
+            for (int i = 0; i < kN; ++i) v[i] = silu(v[i]);
+        } else {
 #pragma unroll
-        for (int i = 0; i < kN; ++i) v[i] = silu(v[i]);
+            for (int i = 0; i < kN; ++i) v[i] = silu_short(v[i]);
+        }
+        if (pairs) {
+#pragma unroll
+            for (int i = 0; i < kN; ++i) v[i] *= up[i];
+        }
     } else if (p.activation == kGelu) {
 #pragma unroll
         for (int i = 0; i < kN; ++i) v[i] = gelu(v[i]);

@@ -261,11 +261,16 @@ __global__ void __launch_bounds__(kAhead ? kSmall : kMaxNormThreads, kAhead ? ct
 #pragma unroll
                 for (int j = 0; j < 8; ++j) h[i][j] *= w[i][j];
         }
-        if (p.gate != nullptr) {
+        if (p.gate != nullptr && p.out_type == kF32) {
 #pragma unroll
             for (int i = 0; i < kN; ++i)
 #pragma unroll
                 for (int j = 0; j < 8; ++j) h[i][j] *= silu(gate[i][j]);
+        } else if (p.gate != nullptr) {
+#pragma unroll
+            for (int i = 0; i < kN; ++i)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) h[i][j] *= silu_short(gate[i][j]);
         }
         if (p.out_type == kE4M3) {
             float top = 0.0f;

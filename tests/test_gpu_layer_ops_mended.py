@@ -76,3 +76,64 @@ def test_norm_by_a_root_off_by_its_rounding(ops):
     got = torch.cat([ops.rms_norm(one, eps=e) for e in eps.tolist()])[:, 0].cpu().double()
     want = (1 + eps) ** -0.5
     assert float(((got - want).abs() / want).max()) <= 1.51 * plain.U
+
+
+SILU_RANGES = [(-87, -40), (-40, -15), (-15, -6), (-6, -3), (-3, 0), (0, 3), (3, 40)]
+
+
+def silu_is(x, got):
+    """FP32 results: 2^t by ex2.approx 4 U, its correction 2 U, the sum and the product U each, 1 / x by rcp.approx 2 U less what
+    the sum's own slope takes from the errors of 2^t, in all 9 U at most; and ln 2, rounded to 2.8e-9, counts by |x|."""
+    x = x.cpu().double()
+    want = plain.silu(x)
+    off = (got.cpu().double() - want).abs()
+    assert bool((off <= (9 + x.abs() / 20) * plain.U * want.abs()).all())
+
+
+@pytest.mark.parametrize("low,high", SILU_RANGES)
+def test_silu_of_far_values(ops, low, high):
+    """To the last bits at both ends, in every operator that has it."""
+    x = (torch.rand(1 << 12, 64, generator=torch.Generator().manual_seed(3)) * (high - low) + low).cuda()
+    itself = torch.tensor([[0.0, 1.0]], device="cuda").repeat(64, 1)
+    silu_is(x, ops.short_conv(x, itself, torch.zeros(len(x), 1, 64, device="cuda")))
+    silu_is(x, ops.short_conv(x, itself, torch.zeros(1, 1, 64, device="cuda"), starts=torch.tensor([0, len(x)], dtype=torch.int32, device="cuda")))
+    short = x.to(BF16)
+    diagonal = torch.eye(64, device="cuda", dtype=BF16)
+    for tokens in (5, 4000):  # either kernel: sums with one term
+        silu_is(short[:tokens], ops.linear(short[:tokens], diagonal, activation="silu", dtype=F32))
+        twice = torch.cat([diagonal, torch.zeros_like(diagonal)])
+        silu_is(short[:tokens], ops.linear(short[:tokens], twice, bias=torch.cat([torch.zeros(64), torch.ones(64)]).cuda(), activation="swiglu", dtype=F32))
+    ones = torch.ones_like(x)
+    assert bool((ops.rms_norm(ones, eps=0.0) == 1).all())
+    silu_is(x, ops.rms_norm(ones, gate=x, eps=0.0))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=str)
+def test_silu_past_its_range(ops, dtype):
+    """Where e^-x is no FP32 number any more: the value itself above, nothing below, and what is not finite as the formula has it."""
+    x = torch.tensor([87.5, 88, 89, 128, 1e4, 1e30, 2.3e38, 3e38, float("inf"), -87.5, -88, -89, -104, -128, -1e4, -1e30, -2.3e38, -3e38,
+                      float("-inf"), float("nan"), 0.0, -0.0]).to(dtype).cuda()[None].repeat(8, 1).contiguous()
+    n = x.shape[1]
+    itself, index = torch.tensor([[0.0, 1.0]], device="cuda").repeat(n, 1), torch.tensor([0, 8], dtype=torch.int32, device="cuda")
+    rows = [ops.short_conv(x, itself, torch.zeros(8, 1, n, device="cuda")), ops.short_conv(x, itself, torch.zeros(1, 1, n, device="cuda"), starts=index),
+            ops.rms_norm(torch.ones_like(x), gate=x, eps=0.0)]
+    zero, bias = torch.zeros(20, 64, device="cuda", dtype=BF16), x[0].contiguous()
+    for tokens in (3, 20):
+        rows.append(ops.linear(zero[:tokens], torch.zeros(n, 64, device="cuda", dtype=BF16), bias=bias, activation="silu", dtype=dtype))
+    # in a sequence the infinity of the token before meets the weight 0, which is NaN
+    assert bool(rows[1][1:, 8].isnan().all())
+    rows[1][1:, 8] = float("inf")
+    for y in rows:
+        for row in y:
+            assert torch.equal(row[:9], x[0, :9])
+            assert bool((row[9:18].abs() <= 1e-35).all()) and bool(row[18:20].isnan().all()) and bool((row[20:] == 0).all())
+
+
+def test_silu_of_16_bits(ops):
+    """Half a step of BF16 and what comes before it; one token at a time gives the bits of many."""
+    x = ((torch.rand(1 << 12, 64, generator=torch.Generator().manual_seed(3)) - 0.7) * 120).cuda().to(BF16)
+    itself = torch.tensor([[0.0, 1.0]], device="cuda").repeat(64, 1)
+    got = ops.short_conv(x, itself, torch.zeros(1, 1, 64, device="cuda"), starts=torch.tensor([0, len(x)], dtype=torch.int32, device="cuda"))
+    want = plain.silu(x.cpu().double())
+    assert bool(((got.cpu().double() - want).abs() <= (2.0 ** -8 + 2.0 ** -17) * want.abs()).all())
+    assert torch.equal(ops.short_conv(x, itself, torch.zeros(len(x), 1, 64, device="cuda")), got)
