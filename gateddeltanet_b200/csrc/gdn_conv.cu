@@ -107,49 +107,7 @@ struct Lane {
     }
 };
 
-/* Two FP32 values as one operand: their products and sums are rounded as by themselves. */
-__device__ __forceinline__ uint64_t pair_of(float lo, float hi) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-    return r;
-}
-__device__ __forceinline__ void split(uint64_t v, float &lo, float &hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-/* silu of both, with the same bits as silu_of() */
-template <typename T>
-__device__ __forceinline__ uint64_t silu2(uint64_t x) {
-    uint64_t near = x;
-    float a, b;
-    if constexpr (sizeof(T) == 4) {
-        split(x, a, b);
-        near = pair_of(fminf(fmaxf(a, -88.0f), 88.0f), fminf(fmaxf(b, -88.0f), 88.0f));
-    }
-    const uint64_t t = mul2(near, pair_of(-1.44269504f, -1.44269504f));
-    split(t, a, b);
-    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(a));
-    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(b));
-    uint64_t e = pair_of(a, b);
-    if constexpr (sizeof(T) == 4) e = fma2(e, fma2(t, pair_of(-0.693147181f, -0.693147181f), mul2(near, pair_of(-1.0f, -1.0f))), e);
-    split(add2(e, pair_of(1.0f, 1.0f)), a, b);
-    asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(a));
-    asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(b));
-    return mul2(x, pair_of(a, b));
-}
-/* for results of type T */
+/* for results of type T, with the same bits as silu2 */
 template <typename T>
 __device__ __forceinline__ float silu_of(float x) {
     return sizeof(T) == 4 ? silu(x) : silu_short(x);
@@ -326,7 +284,7 @@ __global__ void __launch_bounds__(kThreads, ctas_of(Lane<T, kWide>::C)) conv_ker
                         uint64_t o = b;
 #pragma unroll
                         for (int j = 0; j < W; ++j) o = fma2(w[j], v[a + j], o);
-                        if (p.silu) o = silu2<T>(o);
+                        if (p.silu) o = silu2<sizeof(T) == 4>(o);
                         float lo, hi;
                         split(o, lo, hi);
                         if (C == 8)

@@ -292,20 +292,15 @@ __device__ __forceinline__ void finish(const LinearParams &p, float row_scale, f
         }
     }
     if (pairs || p.activation == kSilu) {
-        if (p.out_type == kF32) {
 #pragma unroll
-            for (int i = 0; i < kN; ++i) v[i] = silu(v[i]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < kN; ++i) v[i] = silu_short(v[i]);
-        }
-        if (pairs) {
-#pragma unroll
-            for (int i = 0; i < kN; ++i) v[i] *= up[i];
-        }
+        for (int i = 0; i < kN; i += 2) split(silu2<true>(pair_of(v[i], v[i + 1])), v[i], v[i + 1]);
     } else if (p.activation == kGelu) {
 #pragma unroll
-        for (int i = 0; i < kN; ++i) v[i] = gelu(v[i]);
+        for (int i = 0; i < kN; i += 2) split(gelu2(pair_of(v[i], v[i + 1])), v[i], v[i + 1]);
+    }
+    if (pairs) {
+#pragma unroll
+        for (int i = 0; i < kN; ++i) v[i] *= up[i];
     }
 }
 __device__ __forceinline__ float4 load4(const void *p, int64_t i, int type) {

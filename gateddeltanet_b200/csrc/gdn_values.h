@@ -104,6 +104,49 @@ __device__ __forceinline__ float silu_short(float x) {
     return x * r;
 }
 
+/* Two FP32 values as one operand: their products and sums are rounded as by themselves. */
+__device__ __forceinline__ uint64_t pair_of(float lo, float hi) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ void split(uint64_t v, float &lo, float &hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+/* silu of both, with the bits of silu() or, if not kLong, of silu_short() */
+template <bool kLong>
+__device__ __forceinline__ uint64_t silu2(uint64_t x) {
+    uint64_t near = x;
+    float a, b;
+    if (kLong) {
+        split(x, a, b);
+        near = pair_of(fminf(fmaxf(a, -88.0f), 88.0f), fminf(fmaxf(b, -88.0f), 88.0f));
+    }
+    const uint64_t t = mul2(near, pair_of(-1.44269504f, -1.44269504f));
+    split(t, a, b);
+    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(a));
+    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(b));
+    uint64_t e = pair_of(a, b);
+    if (kLong) e = fma2(e, fma2(t, pair_of(-0.693147181f, -0.693147181f), mul2(near, pair_of(-1.0f, -1.0f))), e);
+    split(add2(e, pair_of(1.0f, 1.0f)), a, b);
+    asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(a));
+    asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(b));
+    return mul2(x, pair_of(a, b));
+}
+
 __host__ __device__ inline bool on16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 }  // namespace ops

@@ -137,3 +137,32 @@ def test_silu_of_16_bits(ops):
     want = plain.silu(x.cpu().double())
     assert bool(((got.cpu().double() - want).abs() <= (2.0 ** -8 + 2.0 ** -17) * want.abs()).all())
     assert torch.equal(ops.short_conv(x, itself, torch.zeros(len(x), 1, 64, device="cuda")), got)
+
+
+def gelu_is(x, got):
+    """Results of gelu(x), x exact: FP32 (20 + x^2 / 40) U, as gdn_linear.h counts; 16 bits half a step more."""
+    x, dtype = x.cpu().double(), got.dtype
+    want = 0.5 * x * torch.special.erfc(-x * 0.5 ** 0.5)
+    off = (20 + x * x / 40) * plain.U + (plain.half_step(dtype) if dtype != F32 else 0)
+    assert bool(((got.cpu().double() - want).abs() <= off * want.abs()).all())
+
+
+@pytest.mark.parametrize("low,high", [(-13, -8), (-8, -5), (-5, -3), (-3, -1), (-1, 0), (0, 1), (1, 8)])
+@pytest.mark.parametrize("outputs", [512, 511])
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=str)
+def test_gelu_keeps_its_bits_below_zero(ops, low, high, outputs, dtype):
+    """Of biases alone, in each kernel: a few tokens, tiles, two CTAs a tile; results in pieces and value by value."""
+    x = ((torch.rand(outputs, generator=torch.Generator().manual_seed(3))) * (high - low) + low).cuda()
+    weight = torch.zeros(outputs, 64, device="cuda", dtype=BF16)
+    for tokens in (1, 16, 20, 300, 3000):
+        y = ops.linear(torch.zeros(tokens, 64, device="cuda", dtype=BF16), weight, bias=x, activation="gelu", dtype=dtype)
+        gelu_is(x.expand(tokens, -1), y)
+
+
+def test_gelu_past_its_range(ops):
+    x = torch.tensor([13.5, 20, 1e5, 1e30, 3e38, float("inf"), -13.5, -20, -1e5, -1e30, -3e38, float("-inf"), float("nan"), 0.0, -0.0, 1e-40]).cuda()
+    weight = torch.zeros(16, 64, device="cuda", dtype=BF16)
+    for tokens in (3, 40):
+        for row in ops.linear(torch.zeros(tokens, 64, device="cuda", dtype=BF16), weight, bias=x, activation="gelu", dtype=F32):
+            assert torch.equal(row[:6], x[:6]) and bool((row[6:11].abs() <= 1e-35).all())
+            assert bool(row[11:13].isnan().all()) and bool((row[13:15] == 0).all()) and 0 <= float(row[15]) <= 6e-41
