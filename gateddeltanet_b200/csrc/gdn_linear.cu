@@ -60,12 +60,20 @@ constexpr uint32_t kRowsA = 128;                  /* tokens of a CTA */
 constexpr uint32_t kBytesA = kRowsA * kBlock;
 constexpr uint32_t kMaxStages = 8;
 constexpr uint32_t kMaxN = 256;
-/* Blocks of k that TMEM adds up before the sums go on in registers. FP32 outputs of BF16: 12 (48 steps; off by up to
- * 7.3e-7 in the 2-norm, 8.6e-7 after silu, where 8 give 4.8e-7 and cost 4 to 7 % of 4096 tokens' time, 16 1.0e-6); of
- * swiglu, whose two sums are off the same way, 6 (7.0e-7, where 12 give 1.5e-6; up to 4 % more time). BF16 outputs, which
- * are rounded to 1.7e-3, and 8-bit operands, whose products are short (3.0e-7 after 32 blocks of 2048 and 5632 inputs): 32.
- * Even, for stages of two blocks. */
-constexpr uint32_t kChunkF32 = 12, kChunkPairs = 6, kChunkShort = 32;
+/* Blocks of k that TMEM adds up before the sums go on in registers. FP32 results of BF16 are off by 2.3e-7, 3.4e-7, 4.7e-7
+ * and 7.0e-7 in the 2-norm with parts of 4, 6, 8 and 12 blocks, whatever the number of inputs, while FP32 arithmetic loses
+ * more of longer sums (x.float() @ w.float().T 2.5e-7 of 1024 inputs, 3.9e-7 of 2048, 7.5e-7 of 5632): so parts grow with
+ * the sum, and results stay under 2^-21 up to 2560 inputs. 2048 tokens of 1024 by 2048 take the same 12.7 us with 4 as with
+ * 12, 64 of 2048 by 32000 27.3 with 6 and 27.2 with 12, 4096 of 2048 by 2048 39.5 and 36.3, 4096 of 5632 by 2048 91
+ * and 85. The two sums of swiglu are off the same way, towards zero, which adds up: 4.6e-7 with 4 and 6.7e-7 with 6 (FP32
+ * arithmetic 6.0e-7 of 2048 inputs, 1.2e-6 of 5632). BF16 results, which are rounded to 1.7e-3, and 8-bit operands, whose
+ * products are short (3.0e-7 after 32 blocks, where FP32 arithmetic is 1.1e-6 off): 32. Even, for stages of two blocks. */
+uint32_t chunk_of(const LinearParams &p, uint32_t blocks) {
+    if (p.out_type == kBF16 || p.type == kE4M3) return 32;
+    const bool pairs = p.activation == kSwiglu;
+    const uint32_t most = pairs ? 6 : 12, chunk = (blocks / 8 + (pairs ? 0 : 2)) & ~1u;
+    return chunk < 4 ? 4 : chunk < most ? chunk : most;
+}
 
 /* set when a wait of a kernel ran out; read and cleared by the host */
 __device__ int g_linear_status;
@@ -879,7 +887,6 @@ LinearShape shape_of(const LinearParams &p, uint32_t ctas, uint32_t n, uint32_t 
     g.outs = p.activation == kSwiglu ? n / 2 : n;
     g.split = split;
     g.sub = sub;
-    g.chunk = p.out_type == kBF16 || p.type == kE4M3 ? kChunkShort : p.activation == kSwiglu ? kChunkPairs : kChunkF32;
     const uint32_t stage = sub * (kBytesA + n / ctas * kBlock);
     const uint32_t room = (uint32_t)(kSmemLimit - kSmemRest) / stage;
     g.stages = room < kMaxStages ? room : kMaxStages;
@@ -887,6 +894,7 @@ LinearShape shape_of(const LinearParams &p, uint32_t ctas, uint32_t n, uint32_t 
     g.tiles_m = (p.tokens + ctas * kRowsA - 1) / (ctas * kRowsA);
     g.tiles_n = (p.outputs + g.outs - 1) / g.outs;
     g.blocks = (uint32_t)(((uint64_t)p.inputs * (p.type == kE4M3 ? 1 : 2) + kBlock - 1) / kBlock);
+    g.chunk = chunk_of(p, g.blocks);
     g.columns = 32;
     while (g.columns < 2 * n) g.columns *= 2;
     return g;

@@ -424,8 +424,9 @@ int gdn_b200_rms_norm(const GdnB200NormArgs *args);
  * half's value times the second half's. rows = outputs for the others. bias
  * [rows] (contiguous) and residual [tokens][outputs] may be NULL; bias, residual
  * and out are FP32 (0) or BF16 (1), each its own. Sums are FP32 on the tensor
- * cores, in parts so short that FP32 results keep 20 bits (2-norm, independent
- * operands); what is not finite spreads to its token's outputs (from x) or to its
+ * cores, in parts so short that FP32 results are under 2^-21 off up to 2560 inputs
+ * and under 2^-20 beyond (2-norm, independent operands), where gelu and silu keep
+ * single values' relative error too; what is not finite spreads to its token's outputs (from x) or to its
  * row's (from W) only. Strides count elements; rows of x and W are contiguous and start on
  * 16-byte boundaries; inputs may be any number. out may be the residual itself
  * (same type and stride) or memory apart from the inputs. */
