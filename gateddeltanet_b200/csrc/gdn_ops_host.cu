@@ -6,6 +6,7 @@
 
 #include <atomic>
 #include <initializer_list>
+#include <numeric>
 #include <stdarg.h>
 #include <stdio.h>
 
@@ -140,22 +141,37 @@ bool float_type(int t) { return t == 0 || t == 1; }
 int64_t size_of(int type) { return type == 0 ? 4 : type == 1 ? 2 : 1; }
 
 /* The memory of a tensor [tokens][heads][dim], by token: from `at` on, `width`
- * bytes (with the gaps between its heads) every `row` bytes. */
+ * bytes (with the gaps between its heads) every `row` bytes; and by runs of `run`
+ * bytes, whose distances are multiples of `period` (0: there is one run). */
 struct Extent {
     const void *at;
-    int64_t row, width, rows;
+    int64_t row, width, rows, run, period;
     Extent(const void *p, int64_t token, int64_t head, uint32_t tokens, uint32_t heads, uint32_t dim, int64_t size)
-        : at(p), row(token * size), width((((int64_t)heads - 1) * head + dim) * size), rows(tokens) {
+        : at(p), row(token * size), width((((int64_t)heads - 1) * head + dim) * size), rows(tokens), run(dim * size), period(0) {
+        if (heads > 1 && head == (int64_t)dim)
+            run = width; /* heads without gaps */
+        else if (heads > 1)
+            period = head * size;
+        if (tokens > 1) period = std::gcd(period, row);
         if (rows > 1 && row < width) { /* heads further apart than tokens: taken as one block */
             width += (rows - 1) * row;
             rows = 1;
         }
     }
     bool same(const Extent &e) const { return at == e.at && (rows == 1 || row == e.row) && width == e.width && rows == e.rows; }
+    /* Whether the runs of either lie in the gaps of the other: every run of e begins `shift` bytes, and a multiple of the
+     * common period, from one of these. */
+    bool interleaved(const Extent &e, int64_t d) const {
+        const int64_t common = std::gcd(period, e.period);
+        if (common == 0) return false;
+        const int64_t shift = (d % common + common) % common;
+        return shift >= run && shift + e.run <= common;
+    }
     bool meets(const Extent &e) const {
         if (at == nullptr || e.at == nullptr || width <= 0 || e.width <= 0) return false;
-        if (width == e.width && rows == e.rows) return same(e) || partly_shared(at, row, e.at, e.row, rows, width);
         const int64_t d = (int64_t)(reinterpret_cast<uintptr_t>(e.at) - reinterpret_cast<uintptr_t>(at));
+        if (interleaved(e, d)) return false;
+        if (width == e.width && rows == e.rows) return same(e) || partly_shared(at, row, e.at, e.row, rows, width);
         if (d >= (rows - 1) * row + width || -d >= (e.rows - 1) * e.row + e.width) return false;
         if (rows != e.rows || rows == 1 || row != e.row || row < width || row < e.width) return true;
         const int64_t shift = (d % row + row) % row; /* of e's rows against these */

@@ -399,7 +399,9 @@ int gdn_b200_constrain_logits(const GdnB200LogitsArgs *args);
  * is, with its scale. Other rows are not touched by it. Squares under 1.5e-45 are lost, which
  * only an eps of 0 or about as small lets one see. Strides count elements, dim is contiguous; any alignment,
  * rows on 16-byte boundaries with dim a multiple of 8 are faster. out may be x
- * itself (same type and strides) or memory apart from the other tensors. A token's
+ * itself (same type and strides) or memory apart from the other tensors: behind or before
+ * them, or between their rows where all strides have a common divisor into which
+ * a run of dim values of either fits (x, out and gate of the heads of one projection). A token's
  * values have to fit one CTA's registers: dim <= 16384, and in 8 bits
  * heads x dim <= 16384 with dim rounded up to 16 times a power of two (up to 512)
  * or to a multiple of 512. */

@@ -179,3 +179,19 @@ def test_linear_keeps_its_bits(ops, tokens, inputs, activation):
     want, _ = plain.linear(x, w, activation=activation)
     got = ops.linear(x, w, activation=activation, dtype=F32).cpu().double()
     assert float((got - want).norm() / want.norm()) <= (2.0 ** -21 if inputs <= 2560 else 2.0 ** -20)
+
+
+def test_norm_of_heads_side_by_side(ops):
+    """x, gate, out and the residual of each head next to one another: results between the inputs, and in their place."""
+    big = rand(30, 4, 4, 128, dtype=BF16)
+    x, gate, out, residual = big.unbind(2)
+    want, h = plain.norm(x, None, residual, gate)
+    kept = x.clone(), gate.clone()
+    assert ops.rms_norm(x, residual=residual, gate=gate, out=out) is out
+    plain.check(out, want, plain.norm_error(gate) * want.abs(), "out")
+    plain.check(residual, h, plain.U * h.abs(), "residual")
+    assert torch.equal(x, kept[0]) and torch.equal(gate, kept[1])
+    want, _ = plain.norm(x, None, None, gate)
+    ops.rms_norm(x, gate=gate, out=x)
+    plain.check(x, want, plain.norm_error(gate) * want.abs(), "in place")
+    assert torch.equal(gate, kept[1])
