@@ -65,5 +65,5 @@ def test_projections_between_rows(lib):  # noqa: F811
     """The result in the gap between the rows of weight, which are as far apart and more."""
     fit = dict(weight=FAR, weight_row=256, out=FAR + 128, out_row=256, outputs=50)
     assert lib.gdn_b200_linear(linear_args(**fit)) == -1 and "device" in gdn.last_error()
-    assert lib.gdn_b200_linear(linear_args(**fit, out_dtype=0, inputs=63)) == -1 and "overlaps" in gdn.last_error()
+    assert lib.gdn_b200_linear(linear_args(**{**fit, "outputs": 100}, out_dtype=0)) == -1 and "overlaps" in gdn.last_error()
     assert lib.gdn_b200_linear(linear_args(**{**fit, "out": FAR + 126})) == -1 and "overlaps" in gdn.last_error()
