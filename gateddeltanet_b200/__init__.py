@@ -181,6 +181,7 @@ EXPORTS = [
     ("gdn_b200_linear_status", ctypes.c_int, [ctypes.c_int]),
     ("gdn_b200_short_conv", ctypes.c_int, [ctypes.c_char_p]),
     ("gdn_b200_test_drop_copy", ctypes.c_int, [ctypes.c_uint32]),
+    ("gdn_b200_test_linear_tiles", ctypes.c_int, [ctypes.c_uint32, ctypes.c_uint32, ctypes.c_uint32]),
 ]
 
 GDN_B200_TP_TOKEN_BYTES = 128

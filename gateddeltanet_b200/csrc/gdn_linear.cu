@@ -80,7 +80,7 @@ __device__ int g_linear_status;
 
 /* a launch's tiles */
 struct LinearShape {
-    uint32_t n;        /* columns of a tile (rows of W): a multiple of 16, of 32 for swiglu or with two CTAs */
+    uint32_t n;        /* columns of a tile (rows of W): a multiple of 32 */
     uint32_t outs;     /* outputs of a tile: n, or n / 2 for swiglu */
     uint32_t split;    /* CTAs that divide k (one CTA to a tile), or 1 */
     uint32_t chunk;    /* blocks of k added up in TMEM */
@@ -880,6 +880,9 @@ constexpr size_t kSmemLimit = 232448; /* 227 KB a CTA */
 
 constexpr uint32_t kSmemRest = 1024 + kEpilogueWarps * kTurnBytes + sizeof(SharedTail);
 
+/* 128-byte blocks of k */
+uint32_t blocks_of(const LinearParams &p) { return (uint32_t)(((uint64_t)p.inputs * (p.type == kE4M3 ? 1 : 2) + kBlock - 1) / kBlock); }
+
 /* What is left to a launch once n, split and the number of CTAs to a tile are chosen. */
 LinearShape shape_of(const LinearParams &p, uint32_t ctas, uint32_t n, uint32_t split, uint32_t sub) {
     LinearShape g;
@@ -893,7 +896,7 @@ LinearShape shape_of(const LinearParams &p, uint32_t ctas, uint32_t n, uint32_t 
     g.rows_a = ctas == 2 || p.tokens >= kRowsA ? kRowsA : (p.tokens + 7) / 8 * 8;
     g.tiles_m = (p.tokens + ctas * kRowsA - 1) / (ctas * kRowsA);
     g.tiles_n = (p.outputs + g.outs - 1) / g.outs;
-    g.blocks = (uint32_t)(((uint64_t)p.inputs * (p.type == kE4M3 ? 1 : 2) + kBlock - 1) / kBlock);
+    g.blocks = blocks_of(p);
     g.chunk = chunk_of(p, g.blocks);
     g.columns = 32;
     while (g.columns < 2 * n) g.columns *= 2;
@@ -944,9 +947,23 @@ bool whole_pieces(const LinearParams &p) {
            (p.residual == nullptr || aligned(p.residual, p.residual_row, p.residual_type));
 }
 
-}  // namespace
+uint64_t tiles_of(const LinearParams &p, uint32_t ctas, uint32_t n) {
+    const uint32_t outs = p.activation == kSwiglu ? n / 2 : n;
+    return (uint64_t)((p.tokens + ctas * kRowsA - 1) / (ctas * kRowsA)) * ((p.outputs + outs - 1) / outs);
+}
+/* What a call may take: n a multiple of 32, so that the eight pieces of a row of sums that tokens take in turn are the row's own;
+ * two CTAs where there are tokens for both; a divided k of at least four blocks a CTA, with tiles whose clusters run at once
+ * (of clusters of four and eight not as many CTAs as there are SMs: 13 of eight did, 16 did not). */
+bool possible(const LinearParams &p, uint32_t ctas, uint32_t n, uint32_t split, int sms) {
+    if (n == 0 || n > kMaxN || n % 32 != 0 || ctas == 0 || ctas > (p.tokens > kRowsA ? 2u : 1u)) return false;
+    if (split == 1) return true;
+    const uint64_t most = (uint64_t)sms * (split < 4 ? 8 : split == 4 ? 7 : 6) / 8;
+    return ctas == 1 && (split == 2 || split == 4 || split == 8) && tiles_of(p, 1, n) * split <= most && blocks_of(p) / split >= 4;
+}
 
-cudaError_t launch_linear_as(const LinearParams &p, uint32_t ctas, uint32_t n, uint32_t split, uint32_t sub, int sms, cudaStream_t stream) {
+cudaError_t launch_linear_as(const LinearParams &p, uint32_t ctas, uint32_t n, uint32_t split, int sms, cudaStream_t stream) {
+    if (!possible(p, ctas, n, split, sms)) return cudaErrorInvalidValue;
+    const uint32_t sub = n <= 128 ? 2 : 1; /* stages of 36 to 64 KB: three at least */
     const LinearShape g = shape_of(p, ctas, n, split, sub);
     auto pick = [&](auto pairs, auto way) {
         constexpr bool kPairs = decltype(pairs)::value;
@@ -963,33 +980,32 @@ cudaError_t launch_linear_as(const LinearParams &p, uint32_t ctas, uint32_t n, u
     return launch(p, g, sms, stream);
 }
 
+}  // namespace
+
 /* The tiles of a call are those for which this estimate is least. What it knows, in us on 148 SMs: a block of k takes
  * 0.00144 n + 0.05 in one CTA and 0.00128 n + 0.024 in two, of which each computes half the columns of both; a launch
  * 4.5 or 5.2; each tile of a CTA 1.0; the last tile's results, where they go value by value, 0.01 n; a cluster that
- * divides k 0.9 + 0.04 a CTA. Of clusters of four and eight not as many as there are SMs for run at once (13 of eight
- * did, 16 did not). Against sweeps of all tiles of 196 calls (17 to 4096 tokens, 128 to 5632 inputs, 501 to 32000
+ * divides k 0.9 + 0.04 a CTA. Against sweeps of all tiles of 196 calls (17 to 4096 tokens, 128 to 5632 inputs, 501 to 32000
  * outputs, both types, all activations) its choices were 1.1 % slower than the best tiles in the mean; 256 columns
  * always, or 128 split as far as possible, were up to twice as slow at either end. */
 cudaError_t launch_linear(const LinearParams &p, int sms, cudaStream_t stream) {
-    const uint32_t blocks = (uint32_t)(((uint64_t)p.inputs * (p.type == kE4M3 ? 1 : 2) + kBlock - 1) / kBlock);
+    if (p.tiles != 0) return launch_linear_as(p, p.tiles & 15, p.tiles >> 4 & 4095, p.tiles >> 16, sms, stream);
+    const uint32_t blocks = blocks_of(p);
     float least = 3.4e38f;
     uint32_t ctas = 1, n = 256, split = 1;
     const bool whole = whole_pieces(p);
     for (uint32_t c = 1; c <= (p.tokens > kRowsA ? 2u : 1u); ++c)
         for (uint32_t width = 32; width <= kMaxN; width += 32) {
-            const uint32_t outs = p.activation == kSwiglu ? width / 2 : width;
-            const uint64_t tiles = (uint64_t)((p.tokens + c * kRowsA - 1) / (c * kRowsA)) * ((p.outputs + outs - 1) / outs);
+            const uint64_t tiles = tiles_of(p, c, width);
             const float block = c == 2 ? 0.00128f * width + 0.024f : 0.00144f * width + 0.053f;
-            for (uint32_t s = 1; s <= (c == 1 ? 8u : 1u); s *= 2) {
-                const uint64_t most = (uint64_t)sms * (s < 4 ? 8 : s == 4 ? 7 : 6) / 8;
-                if (s > 1 && (tiles * s > most || blocks / s < 4)) break;
+            for (uint32_t s = 1; s <= 8 && possible(p, c, width, s, sms); s *= 2) {
                 const uint64_t waves = (tiles * c * s + sms - 1) / sms;
                 const float t = (float)waves * ((float)((blocks + s - 1) / s) * block + 1.0f) + (c == 2 ? 5.2f : 4.5f) +
                                 (whole ? 0.0f : 0.01f * width) + (s > 1 ? 0.9f + 0.04f * s : 0.0f);
                 if (t < least) least = t, ctas = c, n = width, split = s;
             }
         }
-    return launch_linear_as(p, ctas, n, split, n <= 128 ? 2 : 1, sms, stream);
+    return launch_linear_as(p, ctas, n, split, sms, stream);
 }
 
 cudaError_t linear_status(int *status) {

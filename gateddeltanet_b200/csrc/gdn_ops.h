@@ -153,6 +153,7 @@ struct LinearParams {
     uint32_t tokens, inputs, outputs;
     int type, bias_type, residual_type, out_type, activation;
     uint32_t drop; /* for tests, 0: none. 1 + the k-block whose copy the first CTA does not make */
+    uint32_t tiles; /* for tests, 0: those of the rule. CTAs to a tile, columns << 4 and CTAs that divide k << 16 */
 };
 constexpr uint32_t kFewTokens = 16; /* that gdn_linear_few.cu can take */
 

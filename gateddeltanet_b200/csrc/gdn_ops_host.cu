@@ -95,7 +95,8 @@ bool rows_overlap(int64_t token, int64_t head, uint32_t tokens, uint32_t heads, 
     return n_outer > 1 && outer < reach;
 }
 
-std::atomic<uint32_t> g_drop{0}; /* gdn_b200_test_drop_copy */
+std::atomic<uint32_t> g_drop{0};  /* gdn_b200_test_drop_copy */
+std::atomic<uint32_t> g_tiles{0}; /* gdn_b200_test_linear_tiles */
 
 /* Checks what both forms of the rule ask of their arguments; > 0: nothing to do. */
 int delta_params(const char *who, const GdnB200DeltaArgs *a, gdn::ops::DeltaParams &p) {
@@ -211,6 +212,12 @@ int gdn_b200_delta_status(int device) {
 
 int gdn_b200_test_drop_copy(uint32_t index) {
     g_drop = index + 1;
+    return 0;
+}
+
+int gdn_b200_test_linear_tiles(uint32_t ctas, uint32_t columns, uint32_t split) {
+    if (ctas > 15 || columns > 4095 || split > 65535) return failf("gdn_b200_test_linear_tiles: no such tiles");
+    g_tiles = ctas | columns << 4 | split << 16;
     return 0;
 }
 
@@ -343,9 +350,9 @@ int gdn_b200_linear(const GdnB200LinearArgs *args) {
         return failf("%s: out overlaps an input", who);
     const gdn::ops::LinearParams p{a.x, a.weight, a.bias, a.residual, a.x_scales, a.weight_scales, a.out, a.x_row, a.weight_row,
                                    a.residual_row, a.out_row, a.tokens, a.inputs, a.outputs, a.dtype, a.bias_dtype,
-                                   a.residual_dtype, a.out_dtype, a.activation, g_drop.exchange(0)};
+                                   a.residual_dtype, a.out_dtype, a.activation, g_drop.exchange(0), g_tiles.exchange(0)};
     return on_device(who, a.device, [&](int sms) {
-        auto *launch = gdn::ops::takes_few(p) ? gdn::ops::launch_linear_few : gdn::ops::launch_linear;
+        auto *launch = p.tiles == 0 && gdn::ops::takes_few(p) ? gdn::ops::launch_linear_few : gdn::ops::launch_linear;
         return launch(p, sms, static_cast<cudaStream_t>(a.stream));
     });
 }

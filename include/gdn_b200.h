@@ -348,6 +348,11 @@ int gdn_b200_delta_status(int device);
  * memory), of one CTA's first chunk or of x's block `index` of the first CTA's (if
  * that call has more than 16 tokens, or 9 and very many weights) is not made, so that a wait runs out. */
 int gdn_b200_test_drop_copy(uint32_t index);
+/* Test hook: the next gdn_b200_linear of the process takes tiles of `columns` rows of W (a
+ * multiple of 32 up to 256), by one CTA or two (more than 128 tokens), k divided between `split` of
+ * them (1, or with one CTA 2, 4 or 8), whatever the rule would choose; it is refused
+ * where they are not possible. */
+int gdn_b200_test_linear_tiles(uint32_t ctas, uint32_t columns, uint32_t split);
 
 /* Constraints on the logits of `rows` streams, and the greedy pick. With n
  * the times token v stands in the row's history after its prompt:
