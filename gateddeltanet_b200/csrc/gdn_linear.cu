@@ -54,7 +54,8 @@ constexpr uint32_t kLinearThreads = (kEpilogueWarps + 4) * 32; /* three warpgrou
 /* Registers a thread: 384 threads are launched with 168 (64512 in all); the warps with
  * the sums then take 216 and the others 64 (63488). With 168 the sums spilled. */
 constexpr int kEpilogueRegs = 216, kOtherRegs = 64;
-constexpr uint32_t kSplitRegs = kEpilogueWarps * 32 * kEpilogueRegs + 4 * 32 * kOtherRegs; /* at most those of the launch, or the split waits for good */
+constexpr uint32_t kSplitRegs = kEpilogueWarps * 32 * kEpilogueRegs + 4 * 32 * kOtherRegs;
+static_assert(kSplitRegs <= 168 * kLinearThreads, "more than the launch has: the split would wait for good");
 constexpr uint32_t kBlock = 128;                  /* bytes of k in a row of a copy */
 constexpr uint32_t kRowsA = 128;                  /* tokens of a CTA */
 constexpr uint32_t kBytesA = kRowsA * kBlock;
