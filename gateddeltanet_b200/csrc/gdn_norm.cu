@@ -353,12 +353,16 @@ cudaError_t launch_norm_x(const NormParams &p, int sms, cudaStream_t stream) {
     };
     const bool weight_on16 = on16(p.weight);
     const int layout = all_on(8) && weight_on16 ? kEights : all_on(4) && weight_on16 ? kQuads : kSingles;
-    /* Sixteen values a thread, or thirty-two of long rows: 4096 rows of 2048 FP32 values to BF16 take 11.6 us so and
-     * 12.7 with eight, with an FP32 residual 21.0 and 20.7. One by one eight, for want of registers. Rows too long for
-     * 256 threads are not fetched ahead. */
+    /* Sixteen values a thread, or thirty-two of long rows; eight where x, residual and results are all FP32, the most bytes.
+     * 4096 rows of 2048 with sixteen and with eight: FP32 to BF16 11.0 and 12.0 us, to FP32 13.5 and 14.7, with an FP32
+     * residual to 8 bits 19.6 and 23.5, to BF16 20.0 and 19.8, to FP32 25.9 and 23.4 (8192 of 1024 25.7 and 24.8, 16384 of
+     * 512 28.1 and 26.2; by fours, 2044, 23.0 either way). One by one eight, for want of registers. Rows too long for 256
+     * threads are not fetched ahead. */
     auto pick_as = [&](auto r, auto as) {
         using R = decltype(r);
         constexpr Layout kL = decltype(as)::value;
+        if constexpr (kL == kEights && sizeof(T) == 4 && sizeof(R) == 4)
+            if (p.residual != nullptr && p.out_type == kF32 && norm_threads(p, 8) <= kSmall) return launch_norm_t<T, R, kL, 1, true>;
         if constexpr (kL != kSingles) {
             if (norm_threads(p, 16) <= kSmall) return launch_norm_t<T, R, kL, 2, true>;
             if (norm_threads(p, 32) <= kSmall) return launch_norm_t<T, R, kL, 4, true>;
