@@ -1,6 +1,7 @@
 /* Values of the serving operators' tensors: eight neighbours at a time through
- * 16-byte accesses, or one by one, as FP32. Loads go past L1 (what another
- * kernel wrote is in L2). */
+ * 16-byte accesses, or one by one, as FP32. Loads go past L1, where nothing would be
+ * found: a CTA reads each value once. What its threads share (a convolution's starts, slots and weights) goes
+ * through L1. */
 #ifndef GDN_VALUES_H
 #define GDN_VALUES_H
 
@@ -75,9 +76,9 @@ __device__ __forceinline__ void store1(void *p, int64_t i, int type, float x) {
 }
 
 /* The start of a kernel launched with launch_overlapped: it may run before the kernel before it on the
- * stream has ended. wait_for_previous: until it has, and what it wrote is in L2 (every thread that touches
- * global memory calls it first, and reads what other kernels write past L1, which may hold lines from
- * before). let_next_start: the next kernel's CTAs may come as soon as there is room for them. */
+ * stream has ended. wait_for_previous: until it has, and all that it wrote is visible, to loads of any kind. Every thread
+ * that reads or writes global memory calls it first; before it only prefetches to L2, where that kernel's writes go
+ * too. let_next_start: the next kernel's CTAs may come as soon as there is room for them. */
 __device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 

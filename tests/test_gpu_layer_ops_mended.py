@@ -195,3 +195,38 @@ def test_norm_of_heads_side_by_side(ops):
     ops.rms_norm(x, gate=gate, out=x)
     plain.check(x, want, plain.norm_error(gate) * want.abs(), "in place")
     assert torch.equal(gate, kept[1])
+
+
+def test_what_the_kernel_before_wrote(ops):
+    """Calls whose launches overlap read weights, bounds and slots that were written just before, again and again in the same
+    buffers, by a copy or by an operator: as with a wait after every call."""
+    x, xs = rand(200, 512, dtype=BF16), [rand(n, 512, seed=2, dtype=BF16) for n in (3, 12)]
+    bounds = [torch.tensor(b, dtype=torch.int32, device="cuda") for b in ([0, 50, 200], [0, 0, 10], [3, 150, 170])]
+    places = [torch.tensor(b, dtype=torch.int32, device="cuda") for b in ([0, 1], [2, 0], [1, -1])]
+    taps, flags = [rand(512, 4, seed=3 + i) for i in range(3)], [torch.tensor(b, device="cuda") for b in ([True, False], [False, False], [True, True])]
+    left = rand(1000, 512, seed=9, dtype=BF16) * 0.05
+
+    def chain(wait):
+        starts, slots, fresh, weight, w = (torch.zeros_like(t) for t in (bounds[0], places[0], flags[0], taps[0], left))
+        tails, results = torch.zeros(3, 3, 512, device="cuda"), []
+
+        def after(y=None):
+            if y is not None:
+                results.append(y)
+            if wait:
+                torch.cuda.synchronize()
+        for i in range(30):
+            after(ops.rms_norm(x))
+            for to, by in ((starts, bounds), (slots, places), (fresh, flags), (weight, taps)):
+                to.copy_(by[i % 3])
+                after()
+            after(ops.short_conv(x, weight, tails, starts=starts, slots=slots, fresh=fresh))
+            ops.linear(left, left[i:i + 512], activation="silu" if i % 2 else None, out=w)  # the next products' weight
+            after()
+            for a in xs:
+                after(ops.linear(a, w, dtype=F32))
+            after(ops.linear(x, w))
+        return results + [tails]
+    want = chain(True)
+    for _ in range(3):
+        assert all(torch.equal(a, b) for a, b in zip(chain(False), want))
