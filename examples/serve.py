@@ -28,6 +28,16 @@ from gateddeltanet_b200 import ops  # noqa: E402
 E4M3 = torch.float8_e4m3fn
 
 
+def aligned(n: int, columns: int, dtype: torch.dtype) -> torch.Tensor:
+    """[n, columns] whose rows start on 16-byte boundaries, as ops.linear takes them."""
+    return torch.empty(n, -(-columns // 16) * 16, dtype=dtype, device="cuda")[:, :columns]
+
+
+def room(n: int, columns: int, dtype: torch.dtype) -> Optional[torch.Tensor]:
+    """Such rows for a result that ops.linear reads; None where it has them by itself."""
+    return None if columns % 16 == 0 else aligned(n, columns, dtype)
+
+
 class Model:
     """Embedding, `layers` gated-delta-rule layers with their MLPs, tied LM head."""
 
@@ -36,7 +46,7 @@ class Model:
         gen = torch.Generator("cuda").manual_seed(seed)
 
         def weight(*shape):
-            return (torch.randn(shape, generator=gen, device="cuda") * shape[-1] ** -0.5).bfloat16()
+            return aligned(*shape, torch.bfloat16).copy_(torch.randn(shape, generator=gen, device="cuda") * shape[-1] ** -0.5)
 
         def projection(rows, columns):
             """Arguments of ops.linear: a weight, in 8 bits with the scales of its rows."""
@@ -44,11 +54,11 @@ class Model:
             if not eight_bits:
                 return dict(weight=w)
             scales = w.float().abs().amax(1) / 448
-            return dict(weight=(w.float() / scales[:, None]).to(E4M3), weight_scales=scales)
+            return dict(weight=aligned(*w.shape, E4M3).copy_(w.float() / scales[:, None]), weight_scales=scales)
 
         self.vocab, self.heads, self.head_dim, self.eight_bits = vocab, heads, head_dim, eight_bits
         width = heads * head_dim
-        inner = intermediate or hidden * 11 // 64 * 16  # 5632 of 2048
+        inner = intermediate or max(16, hidden * 11 // 64 * 16)  # 5632 of 2048
         ones = lambda n: torch.ones(n, device="cuda")  # noqa: E731
         self.embedding = weight(vocab, hidden)
         self.layers = [dict(
@@ -67,10 +77,9 @@ class Model:
 
     def normed(self, x: torch.Tensor, weight: torch.Tensor, gate: Optional[torch.Tensor] = None) -> dict:
         """Arguments of ops.linear: the norm of x, in 8 bits for 8-bit weights."""
-        if not self.eight_bits:
-            return dict(x=ops.rms_norm(x, weight, gate=gate, dtype=torch.bfloat16).flatten(1))
-        y, scales = ops.rms_norm(x, weight, gate=gate, dtype=E4M3)
-        return dict(x=y.flatten(1), x_scales=scales)
+        dtype = E4M3 if self.eight_bits else torch.bfloat16
+        y = ops.rms_norm(x, weight, gate=gate, dtype=dtype, out=room(*x.shape[-2:], dtype))
+        return dict(x=y[0].flatten(1), x_scales=y[1]) if self.eight_bits else dict(x=y.flatten(1))
 
     def forward(self, tokens: torch.Tensor, states, slots, starts: Optional[torch.Tensor] = None,
                 fresh: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -87,11 +96,14 @@ class Model:
             a, b = qkvgab[:, 4 * width:4 * width + 2 * self.heads].float().chunk(2, dim=1)
             o = rule(q, k, v, -layer["a_log"].exp() * F.softplus(a - 4), torch.sigmoid(b), state, normalize=True, **sequences)
             ops.linear(**self.normed(o, layer["o_norm"], gate), **layer["o"], residual=residual, out=residual)
-            inner = ops.linear(**self.normed(residual, layer["mlp_norm"]), **layer["gate_up"], activation="swiglu")
+            inner = ops.linear(**self.normed(residual, layer["mlp_norm"]), **layer["gate_up"], activation="swiglu",
+                               out=room(len(residual), layer["down"]["weight"].shape[1], torch.bfloat16))
             ops.linear(inner, **layer["down"], residual=residual, out=residual)
         return ops.rms_norm(residual, self.norm, dtype=torch.bfloat16)
 
     def logits(self, hidden: torch.Tensor) -> torch.Tensor:
+        if hidden.shape[1] % 16:
+            hidden = aligned(*hidden.shape, hidden.dtype).copy_(hidden)
         return ops.linear(hidden, self.embedding, dtype=torch.float32)
 
 

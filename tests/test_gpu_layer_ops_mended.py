@@ -1,4 +1,7 @@
 """Calls of the layer operators that once went wrong."""
+import importlib.util
+import os
+
 import pytest
 import torch
 
@@ -230,3 +233,17 @@ def test_what_the_kernel_before_wrote(ops):
     want = chain(True)
     for _ in range(3):
         assert all(torch.equal(a, b) for a, b in zip(chain(False), want))
+
+
+@pytest.mark.parametrize("eight_bits", [False, True], ids=["bf16", "fp8"])
+@pytest.mark.parametrize("hidden,intermediate", [(100, None), (77, 71), (4, None)])
+def test_server_of_any_width(ops, hidden, intermediate, eight_bits):
+    """Hidden sizes whose rows are no multiples of 16 bytes: as they ran before the layers were made of operators."""
+    spec = importlib.util.spec_from_file_location("serve", os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "serve.py"))
+    serve = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(serve)
+    model = serve.Model(vocab=103, hidden=hidden, layers=2, heads=2, head_dim=64, seed=3, intermediate=intermediate, eight_bits=eight_bits)
+    prompts = [[5], list(range(70)), [1, 2, 3]]
+    table, lens, states = serve.generate(model, prompts, 4)
+    assert lens.tolist() == [5, 74, 7] and all(bool(s.isfinite().all()) for s in states)
+    assert all(table[i, :len(p)].tolist() == p for i, p in enumerate(prompts))
