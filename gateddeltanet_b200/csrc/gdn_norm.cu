@@ -261,12 +261,13 @@ __global__ void __launch_bounds__(kAhead ? kSmall : kMaxNormThreads, kAhead ? ct
 #pragma unroll
                 for (int j = 0; j < 8; ++j) h[i][j] *= w[i][j];
         }
-        if (p.gate != nullptr && p.out_type == kF32) {
+        /* rows that are not fetched ahead spill, and more with two forms: 1024 x 16384 FP32 86 us, 76 with one */
+        if (p.gate != nullptr && (!kAhead || p.out_type == kF32)) {
 #pragma unroll
             for (int i = 0; i < kN; ++i)
 #pragma unroll
                 for (int j = 0; j < 8; ++j) h[i][j] *= silu(gate[i][j]);
-        } else if (p.gate != nullptr) {
+        } else if (kAhead && p.gate != nullptr) {
 #pragma unroll
             for (int i = 0; i < kN; ++i)
 #pragma unroll
