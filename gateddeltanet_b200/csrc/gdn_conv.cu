@@ -4,9 +4,10 @@
  * where what lies before a sequence's first token are the W - 1 rows of its
  * slot (zeros if it is fresh), which then get the sequence's last W - 1 inputs.
  *
- * Bound by HBM: x is read and y written once. A thread takes eight
- * neighbouring channels (or one, where rows are not on 16-byte boundaries)
- * through a tile of tokens, the window and the weights in registers; the loads
+ * Bound by HBM: x is read and y written once. A thread takes 16 bytes of
+ * neighbouring channels (eight of BF16, four of FP32), or, where rows are not on
+ * 16-byte boundaries, two channels as far apart as a CTA has threads, through a
+ * tile of tokens, the window in registers and the weights in shared memory; the loads
  * of the next tokens go out together. The tile in which a sequence begins takes
  * all of its tokens that need its slot's rows, and replaces these after it has
  * read them, so that no other CTA touches them: the new ones are rows of x,
@@ -14,10 +15,11 @@
  *
  * Measured, 6144 channels: 24 prompts of 23982 tokens of BF16 110 us (5.4 TB/s;
  * 108 without silu, 109 with eight tokens of loads on their way through shared
- * memory, so what is left is the reads' and writes' turns), 16000 tokens 75 us,
- * 4096 25.3, of FP32 39.1 (5.2 TB/s); a token of 64 streams 4.8 us with their
- * tails of FP32 (2.3 TB/s: the launch and two waits for memory, one after the
- * other).
+ * memory, so what is left is the reads' and writes' turns), 16000 tokens 74 us,
+ * 4096 24.2 to 25.0 (each CTA waits for its weights, the search of starts and x in turn, for 22 tokens), of FP32 37.5 (5.4 TB/s);
+ * a token of 64 streams 4.5 to 5.2 us with their tails of FP32 (2.3 TB/s: the launch and two
+ * waits for memory, one after the other). Off the boundaries: 4000 tokens of 6145 channels of BF16 34.8 us (2.9
+ * TB/s), of 1001 of FP32 11.3 (2.8).
  */
 #include "gdn_ops.h"
 #include "gdn_values.h"

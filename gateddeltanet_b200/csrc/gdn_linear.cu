@@ -26,12 +26,12 @@
  * Every wait is bounded (2 s). A CTA whose wait ran out writes NaN to its
  * outputs and sets g_linear_status.
  *
- * Measured. 4096 tokens of 2048 by 2 x 5632 of 8 bits with swiglu 65 us (2.9
- * PFLOP/s), of 5632 by 2048 of BF16 68 us (1.4 PFLOP/s), with an FP32 residual
- * and FP32 outputs 78: bound by the tensor cores (66 to 78 % of cycles) and, of
- * runs of a second, by the power limit (79 to 92 us at 1.46 GHz); 128 tiles of
+ * Measured. 4096 tokens of 2048 by 2 x 5632 of 8 bits with swiglu 65 to 75 us (2.5 to 2.9
+ * PFLOP/s), of 5632 by 2048 of BF16 68 to 73 us (1.3 to 1.4 PFLOP/s), with an FP32 residual
+ * and FP32 outputs 78 to 88: bound by the tensor cores (66 to 78 % of cycles) and, of
+ * runs of a second, by the power limit (81, 79 and 95 to 101 us at 1.46 GHz); 128 tiles of
  * 256 by 256 for 74 pairs of CTAs leave 14 % of them idle. 64 tokens by 32000 of
- * BF16 25 us (5.2 TB/s), FP32 out 28, by 2 x 5632 with swiglu 13.4 us (3.4 TB/s):
+ * BF16 25 us (5.2 TB/s), FP32 out 27 to 29, by 2 x 5632 with swiglu 13.6 us (3.5 TB/s):
  * bound by reading W, after which the last sums' way takes about 4 us: through
  * TMEM and the cluster, to memory, and the end of all CTAs. It begins 2.4 us after
  * the kernel before has ended, when the first blocks come.
@@ -986,9 +986,9 @@ cudaError_t launch_linear_as(const LinearParams &p, uint32_t ctas, uint32_t n, u
 /* The tiles of a call are those for which this estimate is least. What it knows, in us on 148 SMs: a block of k takes
  * 0.00144 n + 0.05 in one CTA and 0.00128 n + 0.024 in two, of which each computes half the columns of both; a launch
  * 4.5 or 5.2; each tile of a CTA 1.0; the last tile's results, where they go value by value, 0.01 n; a cluster that
- * divides k 0.9 + 0.04 a CTA. Against sweeps of all tiles of 196 calls (17 to 4096 tokens, 128 to 5632 inputs, 501 to 32000
- * outputs, both types, all activations) its choices were 1.1 % slower than the best tiles in the mean; 256 columns
- * always, or 128 split as far as possible, were up to twice as slow at either end. */
+ * divides k 0.9 + 0.04 a CTA. Against all tiles of 138 calls (17 to 4096 tokens, 128 to 5632 inputs, 501 to 32000
+ * outputs, both types, all activations; gdn_b200_test_linear_tiles) its choices were 1.0 % slower than the best tiles in the mean, 6 %
+ * or more for a tenth of them and 25 % at most; 256 columns undivided are 85 % slower in the mean and up to five times. */
 cudaError_t launch_linear(const LinearParams &p, int sms, cudaStream_t stream) {
     if (p.tiles != 0) return launch_linear_as(p, p.tiles & 15, p.tiles >> 4 & 4095, p.tiles >> 16, sms, stream);
     const uint32_t blocks = blocks_of(p);

@@ -11,10 +11,12 @@
  * share its rows and divide k between them, and their partial sums are added in
  * the order of the warps.
  *
- * Measured: one token of 2048 inputs by 8208 outputs of BF16 7.1 us (4.7 TB/s),
- * by 32000 19.9 us (6.6 TB/s, the rate of a copy), of 8 bits 6.3 and 14.9 us;
+ * Measured: one token of 2048 inputs by 8208 outputs of BF16 6.9 us (4.9 TB/s),
+ * by 32000 19.1 us (6.9 TB/s, the rate of a copy), of 8 bits 6.2 and 14.5 us;
  * what small calls take above the bytes is the launch and one wait for memory,
- * about 2.5 us. 16 tokens read as much of x as of W: 12.1 and 29.4 us.
+ * about 2.5 us, and in 8 bits the conversions to FP16: four of W and two of each eight tokens an MMA. 16 tokens
+ * read as much of x as of W: 12.1 and 29.4 us. With swiglu they spill 88 (BF16) and 120 bytes a thread (2048 by 2 x 2048
+ * 6.2 us).
  */
 #include "gdn_linear.h"
 

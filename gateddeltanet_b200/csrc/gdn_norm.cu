@@ -14,9 +14,11 @@
  * row to a CTA without that took 41.6 us where this took 16.4, a ring of rows in
  * shared memory 28.7 where this took 22.5.
  *
- * Measured: 4096 x 2048 BF16 with an FP32 residual, to 8 bits, 17.8 us (5.2
- * TB/s), with a BF16 residual, to BF16, 14.4 us (4.7 TB/s), 4096 x 8 gated heads
- * of 256 14.4 us (3.5 TB/s), one row of 2048 2.1 us, which is the launch.
+ * Measured: 4096 x 2048 BF16 with an FP32 residual, to 8 bits, 17.0 to 17.9 us (5.2 to 5.4
+ * TB/s), with a BF16 residual, to BF16, 13.5 us (5.0 TB/s), all FP32 23.4 (5.7), 4096 x 8 gated
+ * heads of 256 13.0 to 13.7 us (3.7 TB/s), one row of 2048 1.9 us, which is the launch. Rows of more
+ * than 8192 values have 64 registers a thread, spill 150 to 460 bytes and are not fetched ahead: 1024 x
+ * 16384 BF16 with a residual 35.0 us (3.8 TB/s), FP32 76.5 (3.5), where 4096 x 8192 BF16 take 49.6 (5.4).
  */
 #include <type_traits>
 

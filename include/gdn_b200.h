@@ -435,7 +435,8 @@ int gdn_b200_rms_norm(const GdnB200NormArgs *args);
  * and under 2^-20 beyond (2-norm, independent operands), where gelu and silu keep
  * single values' relative error too; what is not finite spreads to its token's outputs (from x) or to its
  * row's (from W) only. Strides count elements; rows of x and W are contiguous and start on
- * 16-byte boundaries; inputs may be any number. out may be the residual itself
+ * 16-byte boundaries; inputs may be any number from 1 on. Up to 2^24 tokens, inputs
+ * and outputs, and 2^38 results. out may be the residual itself
  * (same type and stride) or memory apart from the inputs. */
 typedef struct {
     const void *x, *weight, *bias, *residual;
@@ -468,7 +469,8 @@ int gdn_b200_linear_status(int device);
  * where they decrease the call ends all the same, within its tensors, but with
  * outputs and tails that are not specified. Strides count elements, channels are
  * contiguous; any alignment, rows on 16-byte boundaries with channels a
- * multiple of 8 are faster. out must not overlap the inputs. */
+ * multiple of 8 are faster. Up to 2^20 channels, 2^30 - 1 tokens and 2^22 - 1 sequences.
+ * out must not overlap the inputs. */
 typedef struct {
     const void *x, *weight, *bias;
     void *tails, *out;
