@@ -5,6 +5,7 @@
 #include "gdn_ops.h"
 
 #include <atomic>
+#include <cmath>
 #include <initializer_list>
 #include <numeric>
 #include <stdarg.h>
@@ -283,7 +284,7 @@ int gdn_b200_rms_norm(const GdnB200NormArgs *args) {
     if (a.tokens == 0 || (a.heads == 0 && a.out_dtype != 2)) return 0;
     if (a.dim == 0 || a.heads == 0) return failf("%s: rows of no values", who); /* without heads a token's scale says nothing */
     if ((uint64_t)a.tokens * a.heads > 0x7fffffffu) return failf("%s: %u tokens of %u heads are too many", who, a.tokens, a.heads);
-    if (!(a.eps >= 0.0f)) return failf("%s: eps is negative or not a number", who);
+    if (!(a.eps >= 0.0f) || std::isinf(a.eps)) return failf("%s: eps is negative or not finite", who);
     if (a.x == nullptr || a.out == nullptr) return failf("%s: x or out is missing", who);
     if (a.out_dtype == 2 && a.scales == nullptr) return failf("%s: scales is missing", who);
     for (int64_t stride : {a.x_token, a.x_head, a.gate_token, a.gate_head, a.residual_token, a.residual_head, a.out_token, a.out_head})
