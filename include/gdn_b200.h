@@ -398,7 +398,7 @@ int gdn_b200_constrain_logits(const GdnB200LogitsArgs *args);
  * The mean over dim is that of the unrounded h. Types: FP32 (0) or BF16 (1); x and
  * gate have `dtype`, weight [dim] (contiguous) weight_dtype, the residual
  * residual_dtype; out_dtype may also be E4M3 (2), with scales FP32 [tokens].
- * weight, gate and residual may be NULL. All arithmetic is FP32 (results to
+ * weight, gate and residual may be NULL; eps is finite and not negative. All arithmetic is FP32 (results to
  * 2^-20). A row with a value that is not finite, or whose sum of squares is over
  * FP32's range (one value of 1.9e19 is enough), is NaN throughout; in 8 bits its token
  * is, with its scale. Other rows are not touched by it. Squares under 1.5e-45 are lost, which

@@ -247,3 +247,32 @@ def test_server_of_any_width(ops, hidden, intermediate, eight_bits):
     table, lens, states = serve.generate(model, prompts, 4)
     assert lens.tolist() == [5, 74, 7] and all(bool(s.isfinite().all()) for s in states)
     assert all(table[i, :len(p)].tolist() == p for i, p in enumerate(prompts))
+
+
+def test_conv_by_pieces_of_fp32(ops):
+    """A prompt at once, in pieces and token by token: the same bits, also where silu is far from 0."""
+    x = (torch.rand(300, 512, generator=torch.Generator().manual_seed(1)) * 120 - 90).cuda()
+    weight = torch.tensor([0.0, 0.3, 0.0, 1.0], device="cuda").repeat(512, 1)
+    index = lambda *s: torch.tensor(s, dtype=torch.int32, device="cuda")  # noqa: E731
+    whole, tails = torch.zeros(1, 3, 512, device="cuda"), torch.zeros(1, 3, 512, device="cuda")
+    want = ops.short_conv(x, weight, whole, starts=index(0, 300))
+    parts, at = [], 0
+    for n in (1, 2, 100, 3, 100):
+        parts.append(ops.short_conv(x[at:at + n], weight, tails, starts=index(0, n)))
+        at += n
+    parts += [ops.short_conv(x[t:t + 1], weight, tails) for t in range(at, 300)]
+    assert torch.equal(torch.cat(parts), want) and torch.equal(tails, whole)
+
+
+@pytest.mark.parametrize("activation", ["silu", "gelu", "swiglu"])
+def test_activations_have_the_same_bits_in_every_kernel(ops, activation):
+    """Of biases alone: a few tokens (one value at a time), tiles and divided sums (pairs of values)."""
+    outputs = 500
+    rows = outputs * (2 if activation == "swiglu" else 1)
+    bias = ((torch.rand(rows, generator=torch.Generator().manual_seed(1)) - 0.6) * 60).cuda()
+    weight = torch.zeros(rows, 2048, device="cuda", dtype=BF16)
+    want = None
+    for tokens in (1, 16, 20, 100, 600):
+        y = ops.linear(torch.zeros(tokens, 2048, device="cuda", dtype=BF16), weight, bias=bias, activation=activation, dtype=F32)
+        want = y[:1] if want is None else want
+        assert torch.equal(y, want.expand(tokens, -1))
